@@ -17,6 +17,7 @@ import os
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(HERE)
@@ -27,8 +28,9 @@ CUDA_HOME = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 NVCC = os.path.join(CUDA_HOME, "bin", "nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
-KERNEL_SOURCES = ["fa_fwd_sm100.cu", "fa_abi.cu"]
-KERNEL_HEADERS = ["sm100_ptx.cuh", "fa_softmax.cuh", "fa_fwd.h", "fa_bwd_sm100.cuh",
+KERNEL_SOURCES = ["fa_fwd_sm100.cu", "fa_abi.cu", "fa_paged_abi.cu", "fa_paged_cache.cu",
+                  "fa_paged_attn.cu"]
+KERNEL_HEADERS = ["fa_host.h", "fa_paged.h", "sm100_ptx.cuh", "fa_softmax.cuh", "fa_fwd.h", "fa_bwd_sm100.cuh",
                   "fa_decode_sm100.cuh", "fa_fwd_tile.cuh", "fa_fwd_pair2.cuh"]
 
 
@@ -66,12 +68,15 @@ def build_lib(force=False, verbose=False):
     deps = srcs + [os.path.join(CSRC, h) for h in KERNEL_HEADERS] + [os.path.join(INC, "fa_b200.h")]
     if not force and not _stale(out, deps):
         return out
-    objs = []
-    for s in srcs:
-        o = os.path.join(LIB, os.path.basename(s) + ".o")
+    objs = [os.path.join(LIB, os.path.basename(s) + ".o") for s in srcs]
+
+    def compile_one(s, o):
         _run([NVCC, "-O3", "-std=c++17", *ARCH, "-lineinfo", "-Xcompiler", "-fPIC",
               "-I", INC, "-I", CSRC, "-c", s, "-o", o], verbose)
-        objs.append(o)
+
+    with ThreadPoolExecutor(max_workers=len(srcs)) as pool:
+        for done in [pool.submit(compile_one, s, o) for s, o in zip(srcs, objs)]:
+            done.result()
     _run([NVCC, "-shared", *ARCH, "-o", out, *objs, "-lcudart"], verbose)
     for o in objs:
         os.remove(o)

@@ -15,6 +15,7 @@
 
 #include "fa_b200.h"
 #include "fa_fwd.h"
+#include "fa_host.h"
 
 namespace {
 
@@ -678,6 +679,13 @@ int launch_ranged(bool packed, const void* Q, const void* K, const void* V, void
 
 }  // namespace
 
+namespace fa {
+
+int host_check_device() { return check_device(); }
+int host_sm_count() { return sm_count(); }
+
+}  // namespace fa
+
 extern "C" {
 
 int fa_fwd(const void* Q, const void* K, const void* V, void* O, float* lse, int B, int Hq,
@@ -992,6 +1000,9 @@ const char* fa_error_string(int code) {
     case FA_ERR_TOO_LARGE: return "problem size exceeds the kernel's index range";
     case FA_ERR_SCRATCH_LIMIT:
       return "batch*heads*seq_len^2 exceeds the 4Mi-float scratch of fa_naive_fwd_noalloc";
+    case FA_ERR_PAGE_SIZE: return "page_size must be a positive multiple of 16";
+    case FA_ERR_GROUP: return "at most 128 query heads per KV head";
+    case FA_ERR_SCALES: return "8-bit caches need k_scale and v_scale, 16-bit caches take none";
     default: break;
   }
   if (code >= FA_ERR_TIMEOUT_BASE) return "device watchdog: an in-kernel wait timed out";

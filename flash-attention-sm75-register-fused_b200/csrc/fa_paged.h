@@ -1,0 +1,73 @@
+// Device-side view of a paged KV cache and of the new tokens of a call, and
+// the launchers of the paged kernels (fa_paged_cache.cu, fa_paged_decode.cu).
+#pragma once
+#include <cuda_runtime.h>
+
+#include "fa_b200.h"
+
+namespace fa {
+
+struct PagedCache {
+  const uint8_t* k;  // pages (element size 2, or 1 in 8-bit caches)
+  const uint8_t* v;
+  float* ks;         // scales of an 8-bit cache
+  float* vs;
+  long long page_stride, head_stride, row_stride;  // bytes
+  long long s_page, s_head, s_row;                 // scale elements
+  const int* table;
+  long long table_stride;
+  int max_pages, num_pages, heads, page_size;
+  int page_shift;    // log2(page_size), or -1 if it is no power of two
+
+  __device__ __forceinline__ int page_of(int pos) const {
+    return page_shift >= 0 ? pos >> page_shift : pos / page_size;
+  }
+  // Page id that holds position pos (>= 0) of sequence b, -1 if none does.
+  __device__ __forceinline__ int lookup(int b, int pos) const {
+    const int i = page_of(pos);
+    if (i >= max_pages) return -1;
+    const int page = __ldg(table + static_cast<long long>(b) * table_stride + i);
+    return static_cast<unsigned>(page) < static_cast<unsigned>(num_pages) ? page : -1;
+  }
+  __device__ __forceinline__ int row_in_page(int pos) const {
+    return page_shift >= 0 ? pos & (page_size - 1) : pos % page_size;
+  }
+};
+
+// New tokens: sequence b owns packed rows [cu[b], cu[b+1]) and ends at
+// position lens[b] of its cache.
+struct PagedRows {
+  const int* cu;
+  const int* lens;
+  int B;
+  int total;  // packed rows
+};
+
+// K/V rows of new tokens (strides in bytes).
+struct PagedSource {
+  const uint8_t* k;
+  const uint8_t* v;
+  long long k_token, k_head, v_token, v_head;
+};
+
+struct PagedAttn {
+  PagedCache c;
+  PagedRows r;
+  const uint8_t* q;           // strides in bytes
+  long long q_token, q_head;
+  void* o;                    // [total, Hq, d]
+  float* lse;                 // [Hq, total] or nullptr
+  int Hq, group;              // group = Hq / heads
+  int max_q, max_k;
+  int causal;                 // FA_CAUSAL_*
+  float scale_log2;           // scale * log2(e)
+};
+
+cudaError_t launch_cache_write(const PagedCache& c, const PagedRows& r, const PagedSource& s,
+                               int head_dim, int cache_dtype, bool bf16, cudaStream_t stream);
+cudaError_t launch_cache_read(const PagedCache& c, const PagedRows& r, void* k, void* v,
+                              int head_dim, int cache_dtype, bool bf16, cudaStream_t stream);
+cudaError_t launch_paged_simple(const PagedAttn& a, int head_dim, int cache_dtype, bool bf16,
+                                cudaStream_t stream);
+
+}  // namespace fa

@@ -6,7 +6,8 @@
 //
 // Additions: native GQA (K/V may have fewer heads than Q), bf16 inputs,
 // flash_attention_forward_lse returning (O, LSE), flash_attention_forward_kvcache
-// (Nq != Nk: decode and chunked prefill), and diagnostics.
+// (Nq != Nk: decode and chunked prefill), the paged KV cache (write, read back,
+// attention), and diagnostics.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -452,6 +453,198 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> flash_attention_backward
   return {dQ, dK, dV};
 }
 
+// ---- paged KV cache
+
+// Stride of a dimension, 0 where it has one entry and the stride is free.
+int64_t stride_of(const torch::Tensor& t, int64_t dim) {
+  return t.size(dim) > 1 ? t.stride(dim) : 0;
+}
+
+// The C description of a paged cache: pages [num_pages, Hkv, page_size, d] of
+// any strides with d contiguous, block_table int32 [B, max_pages], scales fp32
+// [num_pages, Hkv, page_size] for 8-bit pages.  `like` (new tokens or results)
+// fixes the device and, for 16-bit pages, the type.
+fa_paged_cache paged_cache(const torch::Tensor& k, const torch::Tensor& v,
+                           const torch::Tensor& table, const c10::optional<torch::Tensor>& ks,
+                           const c10::optional<torch::Tensor>& vs, const torch::Device& device,
+                           torch::ScalarType dtype) {
+  TORCH_CHECK(k.is_cuda() && k.device() == device && v.device() == device,
+              "k_cache and v_cache must be on the inputs' CUDA device");
+  TORCH_CHECK(k.dim() == 4, "k_cache must be [num_pages, Hkv, page_size, D]");
+  TORCH_CHECK(k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type(),
+              "k_cache and v_cache must share shape and dtype");
+  TORCH_CHECK(k.size(3) == 64 || k.size(3) == 128,
+              "flash_attention_sm75 supports head_dim=64 or 128, got ", k.size(3));
+  fa_paged_cache c{};
+  const auto kind = k.scalar_type();
+  const bool eight = kind == torch::kInt8 || kind == torch::kFloat8_e4m3fn;
+  TORCH_CHECK(eight || kind == dtype, "the pages must be int8, float8_e4m3fn or ", dtype,
+              " like the rows, got ", kind);
+  c.dtype = kind == torch::kInt8            ? FA_DTYPE_INT8
+            : kind == torch::kFloat8_e4m3fn ? FA_DTYPE_E4M3
+            : kind == torch::kBFloat16      ? FA_DTYPE_BF16
+                                            : FA_DTYPE_F16;
+  TORCH_CHECK(k.size(2) > 0 && k.size(2) % 16 == 0, "page_size must be a multiple of 16, got ",
+              k.size(2));
+  TORCH_CHECK(k.stride(3) == 1 && v.stride(3) == 1, "the pages' rows must be contiguous");
+  for (int64_t i = 0; i < 3; ++i) {
+    const int64_t st = stride_of(k, i);
+    TORCH_CHECK(st == stride_of(v, i), "k_cache and v_cache must have the same strides");
+    TORCH_CHECK(st * static_cast<int64_t>(k.element_size()) % 16 == 0,
+                "the pages' strides must be multiples of 16 bytes");
+  }
+  TORCH_CHECK(k.size(0) <= INT32_MAX && k.size(1) <= INT32_MAX && k.size(2) <= INT32_MAX,
+              "size exceeds int32");
+  c.k = k.data_ptr();
+  c.v = v.data_ptr();
+  c.page_stride = stride_of(k, 0);
+  c.head_stride = stride_of(k, 1);
+  c.row_stride = stride_of(k, 2);
+  TORCH_CHECK(eight == (ks.has_value() && vs.has_value()) && eight == (ks.has_value() || vs.has_value()),
+              "8-bit pages need k_scale and v_scale, 16-bit pages take none");
+  if (eight) {
+    for (const auto* t : {&*ks, &*vs}) {
+      TORCH_CHECK(t->device() == device && t->scalar_type() == torch::kFloat32 && t->dim() == 3 &&
+                      t->size(0) == k.size(0) && t->size(1) == k.size(1) && t->size(2) == k.size(2),
+                  "k_scale and v_scale must be fp32 [num_pages, Hkv, page_size] on the pages' device");
+      for (int64_t i = 0; i < 3; ++i)
+        TORCH_CHECK(stride_of(*t, i) == stride_of(*ks, i),
+                    "k_scale and v_scale must have the same strides");
+    }
+    c.k_scale = ks->data_ptr<float>();
+    c.v_scale = vs->data_ptr<float>();
+    c.scale_page_stride = stride_of(*ks, 0);
+    c.scale_head_stride = stride_of(*ks, 1);
+    c.scale_row_stride = stride_of(*ks, 2);
+  }
+  TORCH_CHECK(table.device() == device && table.scalar_type() == torch::kInt32 &&
+                  table.dim() == 2 && (table.size(1) <= 1 || table.stride(1) == 1),
+              "block_table must be int32 [B, max_pages] with contiguous rows on the pages' device");
+  TORCH_CHECK(table.size(0) <= INT32_MAX && table.size(1) <= INT32_MAX, "size exceeds int32");
+  // (an empty table has no data: any valid pointer serves)
+  c.block_table = table.numel() > 0 ? table.data_ptr<int>() : static_cast<const int*>(k.data_ptr());
+  c.table_stride = stride_of(table, 0);
+  c.max_pages = static_cast<int>(table.size(1));
+  c.num_pages = static_cast<int>(k.size(0));
+  c.kv_heads = static_cast<int>(k.size(1));
+  c.page_size = static_cast<int>(k.size(2));
+  c.head_dim = static_cast<int>(k.size(3));
+  return c;
+}
+
+// Number of sequences; checks cu_seqlens [B + 1] and seqlens_k [B] against the table.
+int paged_batch(const torch::Tensor& cu, const torch::Tensor& lens, const torch::Tensor& table,
+                const torch::Device& device) {
+  TORCH_CHECK(cu.device() == device && lens.device() == device,
+              "cu_seqlens and seqlens_k must be on the inputs' device");
+  TORCH_CHECK(cu.scalar_type() == torch::kInt32 && lens.scalar_type() == torch::kInt32 &&
+                  cu.is_contiguous() && lens.is_contiguous() && cu.dim() == 1 && lens.dim() == 1,
+              "cu_seqlens and seqlens_k must be contiguous 1-D int32 tensors");
+  TORCH_CHECK(lens.size(0) == table.size(0) && cu.size(0) == table.size(0) + 1,
+              "block_table [B, max_pages], seqlens_k [B] and cu_seqlens [B + 1] must agree, got B = ",
+              table.size(0), ", ", lens.size(0), ", ", cu.size(0) - 1);
+  return static_cast<int>(table.size(0));
+}
+
+// New rows [total, H, D], f16 / bf16, any token and head strides of 16 bytes.
+void check_new_rows(const torch::Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda(), std::string(name) + " must be a CUDA tensor");
+  TORCH_CHECK(t.scalar_type() == torch::kFloat16 || t.scalar_type() == torch::kBFloat16,
+              std::string(name) + " must be FP16 or BF16");
+  TORCH_CHECK(t.dim() == 3, std::string(name) + " must be [total, H, D]");
+  TORCH_CHECK(t.size(0) <= INT32_MAX && t.size(1) <= INT32_MAX, "size exceeds int32");
+}
+
+// `t` itself if the kernels can read it in place (contiguous rows, token and
+// head strides and base multiples of 16 bytes), else a contiguous copy.
+torch::Tensor readable_rows(const torch::Tensor& t) {
+  if (t.numel() == 0) return t;
+  const bool ok = t.stride(2) == 1 && stride_of(t, 0) % 8 == 0 && stride_of(t, 1) % 8 == 0 &&
+                  reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+void kvcache_write_paged(const torch::Tensor& k_in, const torch::Tensor& v_in,
+                         const torch::Tensor& k_cache, const torch::Tensor& v_cache,
+                         const torch::Tensor& table, const torch::Tensor& cu,
+                         const torch::Tensor& lens, const c10::optional<torch::Tensor>& ks,
+                         const c10::optional<torch::Tensor>& vs) {
+  check_new_rows(k_in, "k");
+  check_new_rows(v_in, "v");
+  TORCH_CHECK(k_in.sizes() == v_in.sizes() && k_in.scalar_type() == v_in.scalar_type() &&
+                  k_in.device() == v_in.device(),
+              "k and v must share shape, dtype and device");
+  const auto c = paged_cache(k_cache, v_cache, table, ks, vs, k_in.device(), k_in.scalar_type());
+  TORCH_CHECK(k_in.size(1) == c.kv_heads && k_in.size(2) == c.head_dim,
+              "k and v must be [total, ", c.kv_heads, ", ", c.head_dim, "] for these pages");
+  const int B = paged_batch(cu, lens, table, k_in.device());
+  if (k_in.numel() == 0) return;
+  const c10::cuda::CUDAGuard guard(k_in.device());
+  const auto k = readable_rows(k_in), v = readable_rows(v_in);
+  const int rc = fa_kvcache_write(
+      &c, k.data_ptr(), v.data_ptr(), stride_of(k, 0), stride_of(k, 1), stride_of(v, 0),
+      stride_of(v, 1), cu.data_ptr<int>(), lens.data_ptr<int>(), B, static_cast<int>(k.size(0)),
+      k.scalar_type() == torch::kBFloat16 ? FA_DTYPE_BF16 : FA_DTYPE_F16, stream_of(k));
+  TORCH_CHECK(rc == FA_OK, "kvcache_write_paged: ", fa_error_string(rc));
+}
+
+std::tuple<torch::Tensor, torch::Tensor> kvcache_read_paged(
+    const torch::Tensor& k_cache, const torch::Tensor& v_cache, const torch::Tensor& table,
+    const torch::Tensor& cu, const torch::Tensor& lens, int64_t total,
+    const c10::optional<torch::Tensor>& ks, const c10::optional<torch::Tensor>& vs, bool bf16) {
+  const auto dtype = bf16 ? torch::kBFloat16 : torch::kFloat16;
+  const auto c = paged_cache(k_cache, v_cache, table, ks, vs, k_cache.device(), dtype);
+  TORCH_CHECK(total >= 0 && total <= INT32_MAX, "total must be a count of rows, got ", total);
+  const int B = paged_batch(cu, lens, table, k_cache.device());
+  const c10::cuda::CUDAGuard guard(k_cache.device());
+  const auto opt = k_cache.options().dtype(dtype);
+  auto k = torch::empty({total, c.kv_heads, c.head_dim}, opt);
+  auto v = torch::empty({total, c.kv_heads, c.head_dim}, opt);
+  if (total == 0) return {k, v};
+  const int rc = fa_kvcache_read(&c, k.data_ptr(), v.data_ptr(), cu.data_ptr<int>(),
+                                 B > 0 ? lens.data_ptr<int>() : nullptr, B,
+                                 static_cast<int>(total), bf16 ? FA_DTYPE_BF16 : FA_DTYPE_F16,
+                                 stream_of(k_cache));
+  TORCH_CHECK(rc == FA_OK, "kvcache_read_paged: ", fa_error_string(rc));
+  return {k, v};
+}
+
+// O [total_q, Hq, d] and, if asked for, LSE fp32 [Hq, total_q].
+std::tuple<torch::Tensor, c10::optional<torch::Tensor>> flash_attention_forward_paged(
+    const torch::Tensor& q_in, const torch::Tensor& k_cache, const torch::Tensor& v_cache,
+    const torch::Tensor& table, const torch::Tensor& cu, const torch::Tensor& lens,
+    int64_t max_seqlen_q, int64_t max_seqlen_k, int64_t causal, float scale, bool want_lse,
+    const c10::optional<torch::Tensor>& ks, const c10::optional<torch::Tensor>& vs) {
+  check_new_rows(q_in, "q");
+  const auto c = paged_cache(k_cache, v_cache, table, ks, vs, q_in.device(), q_in.scalar_type());
+  TORCH_CHECK(q_in.size(2) == c.head_dim, "head_dim mismatch");
+  TORCH_CHECK(c.kv_heads > 0 && q_in.size(1) % c.kv_heads == 0, "GQA: Q heads (", q_in.size(1),
+              ") not divisible by K/V heads (", c.kv_heads, ")");
+  const int B = paged_batch(cu, lens, table, q_in.device());
+  TORCH_CHECK(max_seqlen_q >= 0 && max_seqlen_k >= 0 && max_seqlen_q <= INT32_MAX &&
+                  max_seqlen_k <= INT32_MAX,
+              "max_seqlen_q and max_seqlen_k must be lengths");
+  const c10::cuda::CUDAGuard guard(q_in.device());
+  const auto q = readable_rows(q_in);
+  const int Hq = static_cast<int>(q.size(1)), total = static_cast<int>(q.size(0));
+  auto O = torch::empty(q.sizes(), q.options());
+  c10::optional<torch::Tensor> lse;
+  if (want_lse) lse = torch::empty({Hq, total}, q.options().dtype(torch::kFloat32));
+  if (q.numel() == 0) return {O, lse};
+  const int mq = static_cast<int>(max_seqlen_q), mk = static_cast<int>(max_seqlen_k);
+  const size_t ws_bytes = fa_fwd_paged_workspace_bytes(&c, B, Hq, total, mq, mk);
+  auto ws = torch::empty({static_cast<int64_t>(ws_bytes > 0 ? ws_bytes : 16)},
+                         q.options().dtype(torch::kUInt8));
+  const int rc = fa_fwd_paged(&c, q.data_ptr(), stride_of(q, 0), stride_of(q, 1), O.data_ptr(),
+                              want_lse ? lse->data_ptr<float>() : nullptr, cu.data_ptr<int>(),
+                              B > 0 ? lens.data_ptr<int>() : nullptr, B, Hq, total, mq, mk, scale,
+                              static_cast<int>(causal),
+                              q.scalar_type() == torch::kBFloat16 ? FA_DTYPE_BF16 : FA_DTYPE_F16,
+                              ws.data_ptr(), ws_bytes, stream_of(q));
+  TORCH_CHECK(rc == FA_OK, "flash_attention_forward_paged: ", fa_error_string(rc));
+  return {O, lse};
+}
+
 int device_status(bool reset) { return fa_device_status(reset ? 1 : 0); }
 
 }  // namespace
@@ -478,6 +671,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "(dQ, dK, dV) of flash_attention_forward_padded for square padded batches");
   m.def("flash_attention_backward_varlen", &flash_attention_backward_varlen,
         "(dQ, dK, dV) of flash_attention_forward_varlen for packed self-attention batches");
+  m.def("kvcache_write_paged", &kvcache_write_paged,
+        "Stores K, V rows of new tokens in the pages (quantised for 8-bit pages)");
+  m.def("kvcache_read_paged", &kvcache_read_paged,
+        "(K, V) packed 16-bit rows of the described tokens");
+  m.def("flash_attention_forward_paged", &flash_attention_forward_paged,
+        "(O [total_q, Hq, d], LSE [Hq, total_q] or None) of new tokens over a paged cache");
   m.def("device_status", &device_status, pybind11::arg("reset") = false,
         "Error code recorded by the in-kernel watchdog (0 = none)");
   m.def("set_watchdog_ns", &fa_set_watchdog_ns);

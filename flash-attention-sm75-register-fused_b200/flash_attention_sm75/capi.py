@@ -13,7 +13,29 @@ LIB_PATH = os.path.join(PKG_DIR, "lib", "libfa_b200.so")
 
 c_vp, c_int, c_float, c_bool = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_bool
 
+c_ll = ctypes.c_longlong
+
+
+class PagedCache(ctypes.Structure):
+    """fa_paged_cache of include/fa_b200.h."""
+    _fields_ = [("k", c_vp), ("v", c_vp), ("k_scale", c_vp), ("v_scale", c_vp),
+                ("page_stride", c_ll), ("head_stride", c_ll), ("row_stride", c_ll),
+                ("scale_page_stride", c_ll), ("scale_head_stride", c_ll),
+                ("scale_row_stride", c_ll), ("block_table", c_vp), ("table_stride", c_ll),
+                ("max_pages", c_int), ("num_pages", c_int), ("kv_heads", c_int),
+                ("page_size", c_int), ("head_dim", c_int), ("dtype", c_int)]
+
+
 SIGNATURES = {
+    "fa_kvcache_write": (c_int, [ctypes.POINTER(PagedCache), c_vp, c_vp, c_ll, c_ll, c_ll, c_ll,
+                                 c_vp, c_vp, c_int, c_int, c_int, c_vp]),
+    "fa_kvcache_read": (c_int, [ctypes.POINTER(PagedCache), c_vp, c_vp, c_vp, c_vp, c_int, c_int,
+                                c_int, c_vp]),
+    "fa_fwd_paged": (c_int, [ctypes.POINTER(PagedCache), c_vp, c_ll, c_ll, c_vp, c_vp, c_vp, c_vp,
+                             c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_vp,
+                             ctypes.c_size_t, c_vp]),
+    "fa_fwd_paged_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(PagedCache), c_int, c_int,
+                                                       c_int, c_int, c_int]),
     "fa_fwd": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_int, c_float,
                        c_int, c_int, c_vp]),
     "fa_fwd_kvcache": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_int,
@@ -212,3 +234,59 @@ def fa_bwd_varlen(q, k, v, o, do, lse, cu, max_seqlen, dq, dk, dv, causal=False,
     return lib.fa_bwd_varlen(ptr(q), ptr(k), ptr(v), ptr(o), ptr(do), ptr(lse), ptr(cu), ptr(dq),
                              ptr(dk), ptr(dv), B, Hq, Hkv, T, int(max_seqlen), d, float(scale),
                              int(bool(causal)), dtype, ptr(ws), nbytes, stream_ptr(stream))
+
+
+def paged_cache(k_cache, v_cache, block_table, k_scale=None, v_scale=None):
+    """fa_paged_cache of torch tensors: pages [num_pages, Hkv, page, d] (any
+    strides), block_table int32 [B, max_pages], scales [num_pages, Hkv, page]."""
+    import torch
+    kinds = {torch.float16: 0, torch.bfloat16: 1, torch.int8: 2, torch.float8_e4m3fn: 3}
+    c = PagedCache()
+    c.k, c.v = k_cache.data_ptr(), v_cache.data_ptr()
+    c.page_stride, c.head_stride, c.row_stride = k_cache.stride()[:3]
+    if k_scale is not None:
+        c.k_scale, c.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
+        c.scale_page_stride, c.scale_head_stride, c.scale_row_stride = k_scale.stride()
+    c.block_table, c.table_stride = block_table.data_ptr(), block_table.stride(0)
+    c.max_pages = block_table.size(1)
+    c.num_pages, c.kv_heads, c.page_size, c.head_dim = k_cache.shape
+    c.dtype = kinds[k_cache.dtype]
+    return c
+
+
+def fa_kvcache_write(cache, k, v, cu_seqlens, seqlens_k, stream=None):
+    """Call fa_kvcache_write on torch CUDA tensors (k, v [total, Hkv, d]).  Returns the status."""
+    import torch
+    return load().fa_kvcache_write(ctypes.byref(cache), ptr(k), ptr(v), k.stride(0), k.stride(1),
+                                   v.stride(0), v.stride(1), ptr(cu_seqlens), ptr(seqlens_k),
+                                   seqlens_k.numel(), k.shape[0],
+                                   1 if k.dtype == torch.bfloat16 else 0, stream_ptr(stream))
+
+
+def fa_kvcache_read(cache, k, v, cu_seqlens, seqlens_k, stream=None):
+    """Call fa_kvcache_read into torch CUDA tensors (k, v [total, Hkv, d]).  Returns the status."""
+    import torch
+    return load().fa_kvcache_read(ctypes.byref(cache), ptr(k), ptr(v), ptr(cu_seqlens),
+                                  ptr(seqlens_k), seqlens_k.numel(), k.shape[0],
+                                  1 if k.dtype == torch.bfloat16 else 0, stream_ptr(stream))
+
+
+def fa_fwd_paged(cache, q, o, lse, cu_seqlens_q, seqlens_k, max_seqlen_q, max_seqlen_k,
+                 causal=CAUSAL_NONE, scale=None, stream=None):
+    """Call fa_fwd_paged on torch CUDA tensors (q, o [total_q, Hq, d], lse
+    [Hq, total_q] or None); allocates the workspace.  Returns the status."""
+    import math
+    import torch
+    T, Hq, d = q.shape
+    if scale is None:
+        scale = 1.0 / math.sqrt(d)
+    lib = load()
+    B = seqlens_k.numel()
+    nbytes = lib.fa_fwd_paged_workspace_bytes(ctypes.byref(cache), B, Hq, T, int(max_seqlen_q),
+                                              int(max_seqlen_k))
+    ws = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=q.device)
+    return lib.fa_fwd_paged(ctypes.byref(cache), ptr(q), q.stride(0), q.stride(1), ptr(o), ptr(lse),
+                            ptr(cu_seqlens_q), ptr(seqlens_k), B, Hq, T, int(max_seqlen_q),
+                            int(max_seqlen_k), float(scale), int(causal),
+                            1 if q.dtype == torch.bfloat16 else 0, ptr(ws), nbytes,
+                            stream_ptr(stream))

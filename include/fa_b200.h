@@ -40,10 +40,18 @@ enum {
   FA_ERR_CUDA = 9,                 /* another CUDA runtime call failed */
   FA_ERR_TOO_LARGE = 10,           /* a size overflows the kernel's index types */
   FA_ERR_SCRATCH_LIMIT = 11,       /* fa_naive_fwd_noalloc: problem larger than its static scratch */
+  FA_ERR_PAGE_SIZE = 12,           /* paged cache: page_size not a positive multiple of 16 */
+  FA_ERR_GROUP = 13,               /* paged attention: more than 128 query heads per KV head */
+  FA_ERR_SCALES = 14,              /* 8-bit cache without scales, or a 16-bit cache with them */
   FA_ERR_TIMEOUT_BASE = 100        /* device watchdog: 100 + wait site id */
 };
 
-enum { FA_DTYPE_F16 = 0, FA_DTYPE_BF16 = 1 };
+enum {
+  FA_DTYPE_F16 = 0,
+  FA_DTYPE_BF16 = 1,
+  FA_DTYPE_INT8 = 2, /* paged caches only: value = int8 * scale of its row */
+  FA_DTYPE_E4M3 = 3  /* paged caches only: value = e4m3 * scale of its row */
+};
 
 /* Causal alignment for fa_fwd_kvcache (fa_fwd takes 0/1; for Nq == Nk both
  * alignments are the reference's top-left mask, attention_ref.py:33-40). */
@@ -205,6 +213,108 @@ int fa_bwd_varlen(const void* Q, const void* K, const void* V, const void* O, co
                   const float* lse, const int* cu_seqlens, void* dQ, void* dK, void* dV, int B,
                   int Hq, int Hkv, int total, int max_seqlen, int head_dim, float scale,
                   int causal, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- paged KV cache ----
+ *
+ * A cache of `num_pages` pages of `page_size` tokens.  Element (page, head,
+ * row, c) of K lies at k[page * page_stride + head * head_stride +
+ * row * row_stride + c] (strides in elements; V the same from v), so head-major
+ * pages [num_pages, kv_heads, page_size, d], token-major pages
+ * [num_pages, page_size, kv_heads, d] and slices of a larger array all fit.
+ * Pointers are 16-byte aligned and the strides multiples of 16 bytes.
+ *
+ * Position p of sequence b is row p % page_size of page
+ * block_table[b * table_stride + p / page_size] (int32, on the device).  Table
+ * entries outside [0, num_pages) are skipped by writes and read as rows of
+ * zeros; nothing outside the cache is addressed whatever the tables hold.
+ *
+ * 8-bit caches (dtype FA_DTYPE_INT8 / FA_DTYPE_E4M3) hold one fp32 scale per
+ * token and head for K and for V, at k_scale[page * scale_page_stride +
+ * head * scale_head_stride + row * scale_row_stride]; 16-bit caches have none
+ * (k_scale = v_scale = NULL).
+ *
+ * Every entry point takes the same description of new tokens: sequence b
+ * brings n_b = cu_seqlens[b+1] - cu_seqlens[b] of them (rows cu_seqlens[b] ..
+ * of the packed arrays), the last of which is position seqlens_k[b] - 1, so
+ * token i is position seqlens_k[b] - n_b + i.  cu_seqlens (B + 1 entries, from
+ * 0 up, non-decreasing) and seqlens_k (B entries) are int32 DEVICE arrays; the
+ * kernels clamp what they read to the arrays' bounds.  Positions below 0 or
+ * beyond max_pages * page_size hold nothing.
+ */
+typedef struct fa_paged_cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  long long page_stride, head_stride, row_stride;
+  long long scale_page_stride, scale_head_stride, scale_row_stride;
+  const int* block_table;
+  long long table_stride;
+  int max_pages; /* entries of one table row */
+  int num_pages;
+  int kv_heads;
+  int page_size; /* a multiple of 16 */
+  int head_dim;  /* 64 or 128 */
+  int dtype;     /* FA_DTYPE_* of the pages */
+} fa_paged_cache;
+
+/*
+ * fa_kvcache_write — stores the K and V rows of new tokens in their pages.
+ * K/V: f16 or bf16 (`dtype`), token t's row of head h at t * token_stride +
+ * h * head_stride (elements, multiples of 8; 16-byte aligned).  A 16-bit cache
+ * must have the same dtype (the rows are copied); an 8-bit cache stores
+ *   a = max |x| of the row, scale = a / qmax, q = round(x * (qmax / a))
+ * with qmax = 127 (int8, ties to even) or 448 (e4m3, nearest even); rows with
+ * a < 2^-100 are stored as zeros with scale 0, and a row that holds an
+ * infinity or a NaN reads back as NaN.  Asynchronous on `stream`.  Two tokens
+ * must not have the same place.
+ *
+ * No reference counterpart: the reference has no KV cache (reference
+ * src/flash_attention_sm75/llama_attention_replacement.py:63-65 leaves cached
+ * decode to PyTorch SDPA).
+ */
+int fa_kvcache_write(const fa_paged_cache* cache, const void* K, const void* V,
+                     long long k_token_stride, long long k_head_stride,
+                     long long v_token_stride, long long v_head_stride, const int* cu_seqlens,
+                     const int* seqlens_k, int B, int total, int dtype, void* stream);
+
+/*
+ * fa_kvcache_read — the reverse: K/V rows [total, kv_heads, d] (contiguous,
+ * f16 or bf16; a 16-bit cache's own dtype) of the described tokens, e.g. of
+ * whole prefixes (cu_seqlens = running sums of seqlens_k), in the layout
+ * fa_fwd_varlen takes.  8-bit values are multiplied by their scale in fp32 and
+ * rounded once.  Rows of tokens without a place, and of no sequence, are zero.
+ * Asynchronous on `stream`.
+ */
+int fa_kvcache_read(const fa_paged_cache* cache, void* K, void* V, const int* cu_seqlens,
+                    const int* seqlens_k, int B, int total, int dtype, void* stream);
+
+/*
+ * fa_fwd_paged — attention of new tokens over a paged cache that already holds
+ * their own keys and values: Q row (t, h) at t * q_token_stride +
+ * h * q_head_stride (elements, multiples of 8; 16-byte aligned), O
+ * [total_q, Hq, d] contiguous, LSE (may be NULL) fp32 [Hq, total_q].  Sequence
+ * b's queries see keys j < seqlens_k[b], with `causal` FA_CAUSAL_BOTTOM_RIGHT
+ * those with j <= i + seqlens_k[b] - n_b, with FA_CAUSAL_TOP_LEFT j <= i.  Rows
+ * that see no key, and rows of no sequence, get O = 0, LSE = -inf.  Keys that
+ * no query may see have no effect, whatever their rows of the pages hold.
+ * `dtype` (f16 / bf16) is that of Q and O; a 16-bit cache has the same.
+ * max_seqlen_q / max_seqlen_k bound n_b and seqlens_k (tokens and keys beyond
+ * them are not computed / not seen).  Hq / kv_heads is at most 128.
+ * `workspace` (16-byte aligned) needs fa_fwd_paged_workspace_bytes() bytes.
+ * Asynchronous on `stream`.
+ *
+ * No reference counterpart (reference llama_attention_replacement.py:63-65).
+ */
+int fa_fwd_paged(const fa_paged_cache* cache, const void* Q, long long q_token_stride,
+                 long long q_head_stride, void* O, float* lse, const int* cu_seqlens_q,
+                 const int* seqlens_k, int B, int Hq, int total_q, int max_seqlen_q,
+                 int max_seqlen_k, float scale, int causal, int dtype, void* workspace,
+                 size_t workspace_bytes, void* stream);
+
+/* Workspace bytes of fa_fwd_paged (a function of its sizes alone). */
+size_t fa_fwd_paged_workspace_bytes(const fa_paged_cache* cache, int B, int Hq, int total_q,
+                                    int max_seqlen_q, int max_seqlen_k);
 
 /* ---- reference-compatible launchers (void, fp16, blocking) ----
  * Same signatures and conventions as the reference: errors are printed to
