@@ -67,6 +67,14 @@ cudaError_t launch_cache_write(const PagedCache& c, const PagedRows& r, const Pa
                                int head_dim, int cache_dtype, bool bf16, cudaStream_t stream);
 cudaError_t launch_cache_read(const PagedCache& c, const PagedRows& r, void* k, void* v,
                               int head_dim, int cache_dtype, bool bf16, cudaStream_t stream);
+
+// Decode kernel: sequences with at most max_rows <= paged_decode_rows() query
+// rows (new tokens x group) per KV head, and the rows of sequences without
+// visible keys or of no sequence.  Sequences with more rows are left alone.
+int paged_decode_rows();
+size_t paged_decode_ws_bytes(int max_rows, int head_dim, int sms);
+cudaError_t launch_paged_decode(const PagedAttn& a, int max_rows, int head_dim, int cache_dtype,
+                                bool bf16, int sms, void* workspace, cudaStream_t stream);
 cudaError_t launch_paged_simple(const PagedAttn& a, int head_dim, int cache_dtype, bool bf16,
                                 cudaStream_t stream);
 

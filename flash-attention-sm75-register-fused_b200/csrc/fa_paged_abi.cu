@@ -117,7 +117,12 @@ int fa_kvcache_read(const fa_paged_cache* cache, void* K, void* V, const int* cu
 
 size_t fa_fwd_paged_workspace_bytes(const fa_paged_cache* cache, int B, int Hq, int total_q,
                                     int max_seqlen_q, int max_seqlen_k) {
-  (void)cache; (void)B; (void)Hq; (void)total_q; (void)max_seqlen_q; (void)max_seqlen_k;
+  (void)B; (void)total_q; (void)max_seqlen_k;
+  const int group = cache && cache->kv_heads > 0 ? Hq / cache->kv_heads : 1;
+  const long long rows = static_cast<long long>(max_seqlen_q) * group;
+  if (rows <= fa::paged_decode_rows())
+    return fa::paged_decode_ws_bytes(static_cast<int>(rows), cache ? cache->head_dim : 128,
+                                     fa::host_sm_count());
   return 16;
 }
 
@@ -154,9 +159,14 @@ int fa_fwd_paged(const fa_paged_cache* cache, const void* Q, long long q_token_s
   a.max_k = max_seqlen_k;
   a.causal = causal;
   a.scale_log2 = scale * 1.4426950408889634f;
-  const cudaError_t e = fa::launch_paged_simple(a, cache->head_dim, cache->dtype,
-                                                dtype == FA_DTYPE_BF16,
-                                                static_cast<cudaStream_t>(stream));
+  const long long rows = static_cast<long long>(max_seqlen_q) * a.group;
+  const bool bf16 = dtype == FA_DTYPE_BF16;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const cudaError_t e =
+      rows <= fa::paged_decode_rows() && B > 0 && rows > 0
+          ? fa::launch_paged_decode(a, static_cast<int>(rows), cache->head_dim, cache->dtype, bf16,
+                                    fa::host_sm_count(), workspace, st)
+          : fa::launch_paged_simple(a, cache->head_dim, cache->dtype, bf16, st);
   return e == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
 
