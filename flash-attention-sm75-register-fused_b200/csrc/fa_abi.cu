@@ -683,6 +683,57 @@ namespace fa {
 
 int host_check_device() { return check_device(); }
 int host_sm_count() { return sm_count(); }
+unsigned host_next_epoch() { return g_epoch.fetch_add(1, std::memory_order_relaxed); }
+unsigned long long host_timeout_ns() { return g_timeout_ns.load(std::memory_order_relaxed); }
+
+bool host_tensor_map(CUtensorMap* map, const TiledMap& t) {
+  // a map is a pure function of its description (see g_map_cache)
+  struct Entry {
+    TiledMap key;
+    CUtensorMap map;
+    bool valid;
+  };
+  constexpr int kEntries = 64;
+  static std::mutex mu;
+  static Entry cache[kEntries];
+  auto same = [&t](const TiledMap& o) {
+    if (o.base != t.base || o.bf16 != t.bf16 || o.rank != t.rank) return false;
+    for (int i = 0; i < t.rank; ++i)
+      if (o.dims[i] != t.dims[i] || o.box[i] != t.box[i] || (i > 0 && o.strides[i - 1] != t.strides[i - 1]))
+        return false;
+    return true;
+  };
+  uint64_t h = reinterpret_cast<uintptr_t>(t.base) * 0x9E3779B97F4A7C15ull;
+  for (int i = 0; i < t.rank; ++i) h = (h ^ (t.dims[i] * 31 + t.box[i])) * 0xC2B2AE3D27D4EB4Full;
+  Entry& e = cache[(h >> 32) % kEntries];
+  {
+    std::lock_guard<std::mutex> lock(mu);
+    if (e.valid && same(e.key)) {
+      *map = e.map;
+      return true;
+    }
+  }
+  auto fn = encode_fn();
+  if (fn == nullptr) return false;
+  cuuint64_t dims[4], strides[3];
+  cuuint32_t box[4];
+  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  for (int i = 0; i < t.rank; ++i) {
+    dims[i] = t.dims[i];
+    box[i] = t.box[i];
+    if (i > 0) strides[i - 1] = t.strides[i - 1];
+  }
+  const CUresult r = fn(map, t.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                        static_cast<cuuint32_t>(t.rank), const_cast<void*>(t.base), dims, strides, box,
+                        ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return false;
+  std::lock_guard<std::mutex> lock(mu);
+  e.key = t;
+  e.map = *map;
+  e.valid = true;
+  return true;
+}
 
 }  // namespace fa
 

@@ -1,5 +1,6 @@
 // Host helpers of fa_abi.cu that the paged-cache entry points share.
 #pragma once
+#include <cuda.h>
 
 namespace fa {
 
@@ -7,5 +8,20 @@ namespace fa {
 // current on the calling thread.
 int host_check_device();
 int host_sm_count();
+// Number of the next watched launch (tags device status words) and the
+// watchdog's deadline.
+unsigned host_next_epoch();
+unsigned long long host_timeout_ns();
+
+// Tiled tensor map of a 16-bit tensor with the given dimensions, byte strides
+// (of dimensions 1 ..; multiples of 16) and box, 128-byte swizzle, zero fill.
+// Recent encodings are reused.  False if the encoder refuses it.
+struct TiledMap {
+  const void* base;
+  int bf16, rank;
+  unsigned long long dims[4], strides[3];
+  unsigned box[4];
+};
+bool host_tensor_map(CUtensorMap* map, const TiledMap& t);
 
 }  // namespace fa

@@ -1,7 +1,10 @@
 // Device-side view of a paged KV cache and of the new tokens of a call, and
 // the launchers of the paged kernels (fa_paged_cache.cu, fa_paged_decode.cu).
 #pragma once
+#include <cuda.h>
 #include <cuda_runtime.h>
+
+#include <cstdint>
 
 #include "fa_b200.h"
 
@@ -63,6 +66,22 @@ struct PagedAttn {
   float scale_log2;           // scale * log2(e)
 };
 
+struct alignas(64) ChunkParams {
+  CUtensorMap tm_q;  // (d, Hq, T), box (64, G, tq)
+  CUtensorMap tm_k;  // (d, page rows, heads, pages), box (64, box_rows, 1, 1)
+  CUtensorMap tm_v;
+  PagedAttn a;
+  int tq;            // tokens of a 128-row tile: 128 / group
+  int box_rows;
+  int skip_rows;     // sequences with at most this many rows per KV head are not ours
+  int n_splits;
+  int fill_outside;  // write the rows of no sequence
+  float* ws_o;       // [n_splits][total * Hq][d] fp32, normalised
+  float* ws_lse;     // [n_splits][total * Hq], natural log
+  unsigned epoch;
+  unsigned long long timeout_ns;
+};
+
 cudaError_t launch_cache_write(const PagedCache& c, const PagedRows& r, const PagedSource& s,
                                int head_dim, int cache_dtype, bool bf16, cudaStream_t stream);
 cudaError_t launch_cache_read(const PagedCache& c, const PagedRows& r, void* k, void* v,
@@ -75,7 +94,8 @@ int paged_decode_rows();
 size_t paged_decode_ws_bytes(int max_rows, int head_dim, int sms);
 cudaError_t launch_paged_decode(const PagedAttn& a, int max_rows, int head_dim, int cache_dtype,
                                 bool bf16, int sms, void* workspace, cudaStream_t stream);
-cudaError_t launch_paged_simple(const PagedAttn& a, int head_dim, int cache_dtype, bool bf16,
-                                cudaStream_t stream);
+// Chunk kernel and, for n_splits > 1, the join of its key splits.
+cudaError_t launch_paged_chunk(const ChunkParams& p, int head_dim, int cache_dtype, bool bf16,
+                               int grid, cudaStream_t stream);
 
 }  // namespace fa

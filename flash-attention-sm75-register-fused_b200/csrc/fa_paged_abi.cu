@@ -70,6 +70,106 @@ int check_rows(const int* cu, const int* lens, int B, int total, fa::PagedRows* 
   return FA_OK;
 }
 
+// Which kernels a call runs and how its keys are split.
+//
+// Sequences of at most 16 query rows per KV head go to the decode kernel, the
+// others to the chunk kernel.  The lengths are on the device, so the host goes
+// by bounds: with max_seqlen_q rows of at most 16 every sequence is short; when
+// the packed rows are exactly B full-length sequences every one is long; else
+// both kernels run, each on its own sequences.
+struct PagedPlan {
+  bool decode = false, chunk = false;
+  int decode_rows = 0;  // rows per KV head the decode kernel takes at most
+  int tq = 0;           // chunk kernel: tokens of a query tile
+  int slots = 0;        // ... pairs of tiles there may be
+  int n_splits = 1;
+  size_t ws_decode = 0, ws_o = 0, ws_bytes = 16;
+};
+
+PagedPlan make_paged_plan(int B, int heads, int group, int head_dim, int total, int max_q, int max_k) {
+  PagedPlan k;
+  const int sms = fa::host_sm_count();
+  const long long rows = static_cast<long long>(max_q) * group;
+  const int cap = fa::paged_decode_rows();
+  k.chunk = rows > cap || B == 0 || max_q == 0;
+  k.decode = !k.chunk || (rows > cap && B > 1 && group <= cap &&
+                          total < static_cast<long long>(B) * max_q);
+  k.decode_rows = k.chunk ? (cap / group) * group : static_cast<int>(rows);
+  if (k.decode) k.ws_decode = fa::paged_decode_ws_bytes(k.decode_rows, head_dim, sms);
+  if (k.chunk) {
+    k.tq = 128 / group;
+    const int pair = 2 * k.tq;
+    // sequences of the chunk kernel bring at least this many tokens
+    const int least = k.decode ? k.decode_rows / group + 1 : 1;
+    const long long n_seq = total / least < B ? total / least : B;
+    const long long slots = total / pair + n_seq;
+    k.slots = slots < 1 ? 1 : static_cast<int>(slots);
+    // One CTA per (pair, head, split): the split with the fewest waves x (key
+    // tiles per split + 4 tiles of start-up and join), as for chunked prefill
+    // over a contiguous cache; the number of pairs is estimated from the rows.
+    const long long pairs = B <= 1 ? (total + pair - 1) / pair : total / pair + (n_seq + 1) / 2;
+    const long long items = (pairs < 1 ? 1 : pairs) * heads;
+    const long long n = (static_cast<long long>(max_k) + 127) / 128;
+    long long best = -1;
+    for (long long ns = 1; ns <= 32 && ns <= (n < 1 ? 1 : n); ++ns) {
+      const long long waves = (items * ns + sms - 1) / sms;
+      const long long cost = waves * ((n + ns - 1) / ns + 4) + (ns > 1 ? 2 : 0);
+      if (best < 0 || cost < best) {
+        best = cost;
+        k.n_splits = static_cast<int>(ns);
+      }
+    }
+    if (k.n_splits > 1)
+      k.ws_o = static_cast<size_t>(k.n_splits) * total * heads * group * head_dim * sizeof(float);
+  }
+  const size_t chunk_bytes =
+      k.n_splits > 1 ? k.ws_o + static_cast<size_t>(k.n_splits) * total * heads * group * sizeof(float) : 0;
+  // (the kernels run one after another, so they share the workspace)
+  k.ws_bytes = k.ws_decode > chunk_bytes ? k.ws_decode : chunk_bytes;
+  if (k.ws_bytes < 16) k.ws_bytes = 16;
+  return k;
+}
+
+int gcd_128(int x) {  // of x (a multiple of 16) and 128
+  int g = 16;
+  while (g < 128 && x % (2 * g) == 0) g *= 2;
+  return g;
+}
+
+// Tensor maps of a 16-bit cache and its queries (the stride of a dimension
+// with one entry is free: any valid one serves).
+bool chunk_maps(const PagedPlan& k, const fa_paged_cache& c, const void* q, long long q_token,
+                long long q_head, int Hq, int total, bool bf16, fa::ChunkParams* p) {
+  const unsigned long long row = 2ull * c.head_dim;
+  auto st = [row](long long elems) { return elems > 0 ? 2ull * elems : row; };
+  fa::TiledMap t{};
+  t.bf16 = bf16 ? 1 : 0;
+  t.base = q;
+  t.rank = 3;
+  t.dims[0] = c.head_dim;
+  t.dims[1] = Hq;
+  t.dims[2] = total;
+  t.strides[0] = st(q_head);
+  t.strides[1] = st(q_token);
+  t.box[0] = 64;
+  t.box[1] = Hq / c.kv_heads;
+  t.box[2] = k.tq;
+  if (!fa::host_tensor_map(&p->tm_q, t)) return false;
+  t.rank = 4;
+  t.dims[1] = c.page_size;
+  t.dims[2] = c.kv_heads;
+  t.dims[3] = c.num_pages > 0 ? c.num_pages : 1;
+  t.strides[0] = st(c.row_stride);
+  t.strides[1] = st(c.head_stride);
+  t.strides[2] = st(c.page_stride);
+  t.box[1] = p->box_rows;
+  t.box[2] = t.box[3] = 1;
+  t.base = c.k;
+  if (!fa::host_tensor_map(&p->tm_k, t)) return false;
+  t.base = c.v;
+  return fa::host_tensor_map(&p->tm_v, t);
+}
+
 }  // namespace
 
 extern "C" {
@@ -117,13 +217,12 @@ int fa_kvcache_read(const fa_paged_cache* cache, void* K, void* V, const int* cu
 
 size_t fa_fwd_paged_workspace_bytes(const fa_paged_cache* cache, int B, int Hq, int total_q,
                                     int max_seqlen_q, int max_seqlen_k) {
-  (void)B; (void)total_q; (void)max_seqlen_k;
-  const int group = cache && cache->kv_heads > 0 ? Hq / cache->kv_heads : 1;
-  const long long rows = static_cast<long long>(max_seqlen_q) * group;
-  if (rows <= fa::paged_decode_rows())
-    return fa::paged_decode_ws_bytes(static_cast<int>(rows), cache ? cache->head_dim : 128,
-                                     fa::host_sm_count());
-  return 16;
+  if (!cache || cache->kv_heads <= 0 || Hq <= 0 || total_q <= 0) return 16;
+  const int group = Hq / cache->kv_heads > 0 ? Hq / cache->kv_heads : 1;
+  if (group > 128 || B < 0 || max_seqlen_q < 0 || max_seqlen_k < 0) return 16;  // refused sizes
+  return make_paged_plan(B, cache->kv_heads, group, cache->head_dim, total_q, max_seqlen_q,
+                         max_seqlen_k)
+      .ws_bytes;
 }
 
 int fa_fwd_paged(const fa_paged_cache* cache, const void* Q, long long q_token_stride,
@@ -144,9 +243,14 @@ int fa_fwd_paged(const fa_paged_cache* cache, const void* Q, long long q_token_s
   if (!aligned16(Q) || !aligned16(O) || !aligned16(workspace) ||
       ((q_token_stride | q_head_stride) & 7) || (reinterpret_cast<uintptr_t>(lse) & 3u))
     return FA_ERR_ALIGNMENT;
-  if (workspace_bytes <
-      fa_fwd_paged_workspace_bytes(cache, B, Hq, total_q, max_seqlen_q, max_seqlen_k))
-    return FA_ERR_INVALID_ARG;
+  const int group = Hq / a.c.heads;
+  const PagedPlan k = make_paged_plan(B, a.c.heads, group, cache->head_dim, total_q, max_seqlen_q,
+                                      max_seqlen_k);
+  if (workspace_bytes < k.ws_bytes) return FA_ERR_INVALID_ARG;
+  const long long grid = static_cast<long long>(k.slots) * a.c.heads * k.n_splits;
+  if (grid > 0x7fffffffLL || static_cast<long long>(B) * a.c.heads > 0x7fffffffLL ||
+      static_cast<long long>(total_q) * Hq > (1LL << 33))
+    return FA_ERR_TOO_LARGE;
   if (int rc = fa::host_check_device()) return rc;
   a.q = static_cast<const uint8_t*>(Q);
   a.q_token = 2 * q_token_stride;
@@ -154,20 +258,37 @@ int fa_fwd_paged(const fa_paged_cache* cache, const void* Q, long long q_token_s
   a.o = O;
   a.lse = lse;
   a.Hq = Hq;
-  a.group = Hq / a.c.heads;
+  a.group = group;
   a.max_q = max_seqlen_q;
   a.max_k = max_seqlen_k;
   a.causal = causal;
   a.scale_log2 = scale * 1.4426950408889634f;
-  const long long rows = static_cast<long long>(max_seqlen_q) * a.group;
   const bool bf16 = dtype == FA_DTYPE_BF16;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const cudaError_t e =
-      rows <= fa::paged_decode_rows() && B > 0 && rows > 0
-          ? fa::launch_paged_decode(a, static_cast<int>(rows), cache->head_dim, cache->dtype, bf16,
-                                    fa::host_sm_count(), workspace, st)
-          : fa::launch_paged_simple(a, cache->head_dim, cache->dtype, bf16, st);
-  return e == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
+  if (k.decode &&
+      fa::launch_paged_decode(a, k.decode_rows, cache->head_dim, cache->dtype, bf16,
+                              fa::host_sm_count(), workspace, st) != cudaSuccess)
+    return FA_ERR_LAUNCH;
+  if (k.chunk) {
+    fa::ChunkParams p;
+    p.a = a;
+    p.tq = k.tq;
+    p.box_rows = gcd_128(cache->page_size);
+    p.skip_rows = k.decode ? k.decode_rows : 0;
+    p.n_splits = k.n_splits;
+    p.fill_outside = k.decode ? 0 : 1;
+    p.ws_o = static_cast<float*>(workspace);
+    p.ws_lse = reinterpret_cast<float*>(static_cast<char*>(workspace) + k.ws_o);
+    p.epoch = fa::host_next_epoch();
+    p.timeout_ns = fa::host_timeout_ns();
+    if (!is_8bit(cache->dtype) &&
+        !chunk_maps(k, *cache, Q, q_token_stride, q_head_stride, Hq, total_q, bf16, &p))
+      return FA_ERR_TENSOR_MAP;
+    if (fa::launch_paged_chunk(p, cache->head_dim, cache->dtype, bf16, static_cast<int>(grid), st) !=
+        cudaSuccess)
+      return FA_ERR_LAUNCH;
+  }
+  return FA_OK;
 }
 
 }  // extern "C"

@@ -41,6 +41,7 @@
 #include <cstdint>
 
 #include "fa_paged.h"
+#include "fa_paged_dev.cuh"
 #include "sm100_ptx.cuh"
 
 namespace fa {
@@ -132,55 +133,11 @@ __device__ __forceinline__ uint32_t pack2f(float lo, float hi) {
   }
 }
 
-// Two pairs of 8-bit values of a word as f16 pairs, exactly: bytes (0, 1) and
-// (2, 3), or with kCross bytes (0, 2) and (1, 3).
-// int8: x ^ 0x80 = x + 128 in the low byte of the f16 1024 + (x + 128).
-template <int KV, bool kCross>
-__device__ __forceinline__ void widen(uint32_t w, uint32_t& p0, uint32_t& p1) {
-  if constexpr (KV == FA_DTYPE_INT8) {
-    const uint32_t u = w ^ 0x80808080u;
-    const uint32_t a = __byte_perm(u, 0x64646464u, kCross ? 0x4240 : 0x4140);
-    const uint32_t b = __byte_perm(u, 0x64646464u, kCross ? 0x4341 : 0x4342);
-    const __half2 off = __half2half2(__ushort_as_half(0x6480));  // 1152
-    const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&a), off);
-    const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
-    p0 = *reinterpret_cast<const uint32_t*>(&x);
-    p1 = *reinterpret_cast<const uint32_t*>(&y);
-  } else {
-    const uint32_t u = kCross ? __byte_perm(w, 0u, 0x3120) : w;
-    asm("{\n\t.reg .b16 lo, hi;\n\t"
-        "mov.b32 {lo, hi}, %2;\n\t"
-        "cvt.rn.f16x2.e4m3x2 %0, lo;\n\t"
-        "cvt.rn.f16x2.e4m3x2 %1, hi;\n\t}\n"
-        : "=r"(p0), "=r"(p1)
-        : "r"(u));
-  }
-}
-
-// What a sequence brings to this kernel.
-struct Seq {
-  int c0, nq;    // first packed row; new tokens computed (0: not here)
-  int nk, off;   // visible keys: key j < lim(i) = min(nk, i + off + 1) (causal) or nk
-  int vis;       // keys any of its rows may see
-};
-
-__device__ __forceinline__ int row_limit(const PagedAttn& a, const Seq& s, int i) {
-  return a.causal == FA_CAUSAL_NONE ? s.nk : max(min(s.nk, i + s.off + 1), 0);
-}
-
-// max_rows: query rows per KV head this kernel takes.
-__device__ __forceinline__ Seq load_seq(const PagedAttn& a, int b, int max_rows) {
-  Seq s;
-  const int c0 = min(max(__ldg(a.r.cu + b), 0), a.r.total);
-  const int c1 = min(max(__ldg(a.r.cu + b + 1), c0), a.r.total);
-  const int len = __ldg(a.r.lens + b);
-  const int n = c1 - c0;
-  s.c0 = c0;
-  s.nq = min(n, a.max_q);
-  if (static_cast<long long>(s.nq) * a.group > max_rows) s.nq = 0;
-  s.nk = max(min(min(len, a.max_k), a.c.max_pages * a.c.page_size), 0);
-  s.off = a.causal == FA_CAUSAL_BOTTOM_RIGHT ? s.nk - n : 0;
-  s.vis = s.nq > 0 ? row_limit(a, s, s.nq - 1) : 0;
+// load_seq for this kernel, which takes sequences of at most max_rows query
+// rows per KV head (nq = vis = 0 for the others).
+__device__ __forceinline__ Seq load_short(const PagedAttn& a, int b, int max_rows) {
+  Seq s = load_seq(a, b);
+  if (static_cast<long long>(s.nq) * a.group > max_rows) s.nq = s.vis = 0;
   return s;
 }
 
@@ -191,31 +148,7 @@ struct Spot {
 };
 
 __device__ __forceinline__ int units_of(const PagedAttn& a, int b, int sub, int max_rows) {
-  return (load_seq(a, b, max_rows).vis + sub - 1) / sub;
-}
-
-// Exclusive prefix sum of `sum` over the block's threads; *total its sum.
-// sh: one entry per warp.
-template <int kThreads>
-__device__ __forceinline__ long long block_scan(long long sum, long long* sh, long long* total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long incl = sum;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long up = __shfl_up_sync(0xffffffffu, incl, o);
-    if (lane >= o) incl += up;
-  }
-  if (lane == 31) sh[warp] = incl;
-  __syncthreads();
-  long long base = 0, all = 0;
-#pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) {
-    const long long v = sh[w];
-    if (w < warp) base += v;
-    all += v;
-  }
-  *total = all;
-  return base + incl - sum;
+  return (load_short(a, b, max_rows).vis + sub - 1) / sub;
 }
 
 template <int kThreads>
@@ -309,7 +242,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm)
 
   auto seek = [&](Cursor& c, int b) {  // first unit of the next sequence with keys, from b
     for (; b < a.r.B; ++b) {
-      c.s = load_seq(a, b, p.max_rows);
+      c.s = load_short(a, b, p.max_rows);
       c.n = (c.s.vis + C::kSub - 1) / C::kSub;
       c.b = b;
       if (c.n > 0) break;
@@ -739,7 +672,7 @@ __global__ void __launch_bounds__(kCombineThreads)
           a.lse[static_cast<long long>(i) * a.r.total + t] = -INFINITY;
     }
   }
-  const Seq s = load_seq(a, b, p.max_rows);
+  const Seq s = load_short(a, b, p.max_rows);
   const Spot sp = find_spot<kCombineThreads>(a, sub, p.max_rows, b, sh);
   // the decode kernel's results are complete and visible after this
   ptx::grid_dep_wait();

@@ -87,6 +87,10 @@ def test_workspace_depends_on_sizes_alone():
     for args in ((1, 4, 1, 1, 64), (8, 4, 8, 1, 8192), (3, 4, 700, 512, 4096), (0, 4, 5, 1, 1)):
         n = f(ctypes.byref(_cache()), *args)
         assert 0 < n == f(ctypes.byref(_cache(k=P16 * 2, block_table=P16 * 4)), *args)
+    # sizes that the call itself refuses
+    for args in ((1, 258, 9, 9, 64), (-1, 4, 9, 9, 64), (1, 4, -9, 9, 64), (1, 4, 9, -1, 64)):
+        assert f(ctypes.byref(_cache()), *args) > 0
+    assert f(None, 1, 4, 9, 9, 64) > 0 and f(ctypes.byref(_cache(kv_heads=0)), 1, 4, 9, 9, 64) > 0
 
 
 @pytest.mark.parametrize("mode", [0, 1, 2])
