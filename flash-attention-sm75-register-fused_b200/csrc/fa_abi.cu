@@ -697,7 +697,7 @@ bool host_tensor_map(CUtensorMap* map, const TiledMap& t) {
   static std::mutex mu;
   static Entry cache[kEntries];
   auto same = [&t](const TiledMap& o) {
-    if (o.base != t.base || o.bf16 != t.bf16 || o.rank != t.rank) return false;
+    if (o.base != t.base || o.type != t.type || o.rank != t.rank) return false;
     for (int i = 0; i < t.rank; ++i)
       if (o.dims[i] != t.dims[i] || o.box[i] != t.box[i] || (i > 0 && o.strides[i - 1] != t.strides[i - 1]))
         return false;
@@ -723,9 +723,13 @@ bool host_tensor_map(CUtensorMap* map, const TiledMap& t) {
     box[i] = t.box[i];
     if (i > 0) strides[i - 1] = t.strides[i - 1];
   }
-  const CUresult r = fn(map, t.bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                        static_cast<cuuint32_t>(t.rank), const_cast<void*>(t.base), dims, strides, box,
-                        ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+  const CUtensorMapDataType type = t.type == TiledMap::kBytes  ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                   : t.type == TiledMap::kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                               : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const unsigned inner = t.box[0] * (t.type == TiledMap::kBytes ? 1 : 2);
+  const CUresult r = fn(map, type, static_cast<cuuint32_t>(t.rank), const_cast<void*>(t.base), dims, strides,
+                        box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        inner == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return false;
   std::lock_guard<std::mutex> lock(mu);

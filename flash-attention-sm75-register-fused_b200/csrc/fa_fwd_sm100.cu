@@ -1479,8 +1479,9 @@ cudaError_t read_status(unsigned long long* out, bool reset) {
 
 }  // namespace fa
 
-// Decode, backward and paged chunk kernels (same translation unit: they share
-// the device helpers above).
+// Decode, backward and paged-cache attention kernels (same translation unit:
+// they share the device helpers above).
 #include "fa_decode_sm100.cuh"
 #include "fa_bwd_sm100.cuh"
 #include "fa_paged_chunk.cuh"
+#include "fa_paged_decode.cuh"

@@ -13,12 +13,14 @@ int host_sm_count();
 unsigned host_next_epoch();
 unsigned long long host_timeout_ns();
 
-// Tiled tensor map of a 16-bit tensor with the given dimensions, byte strides
-// (of dimensions 1 ..; multiples of 16) and box, 128-byte swizzle, zero fill.
-// Recent encodings are reused.  False if the encoder refuses it.
+// Tiled tensor map of a tensor with the given dimensions, byte strides (of
+// dimensions 1 ..; multiples of 16) and box, zero fill, swizzled over the box's
+// inner extent (64 or 128 bytes).  Recent encodings are reused.  False if the
+// encoder refuses it.
 struct TiledMap {
+  enum { kF16, kBf16, kBytes };
   const void* base;
-  int bf16, rank;
+  int type, rank;
   unsigned long long dims[4], strides[3];
   unsigned box[4];
 };

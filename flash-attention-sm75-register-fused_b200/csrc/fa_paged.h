@@ -87,13 +87,24 @@ cudaError_t launch_cache_write(const PagedCache& c, const PagedRows& r, const Pa
 cudaError_t launch_cache_read(const PagedCache& c, const PagedRows& r, void* k, void* v,
                               int head_dim, int cache_dtype, bool bf16, cudaStream_t stream);
 
+struct alignas(64) DecodeParams {
+  CUtensorMap tm_k;  // (d, page rows, heads, pages), box (min(row, 128 bytes), 16, 1, 1)
+  CUtensorMap tm_v;
+  PagedAttn a;
+  float* ws;
+  int n_teams;   // teams of the launch, set by launch_paged_decode
+  int max_rows;  // query rows per KV head of the sequences handled
+  unsigned epoch;
+  unsigned long long timeout_ns;
+};
+
 // Decode kernel: sequences with at most max_rows <= paged_decode_rows() query
 // rows (new tokens x group) per KV head, and the rows of sequences without
 // visible keys or of no sequence.  Sequences with more rows are left alone.
 int paged_decode_rows();
 size_t paged_decode_ws_bytes(int max_rows, int head_dim, int sms);
-cudaError_t launch_paged_decode(const PagedAttn& a, int max_rows, int head_dim, int cache_dtype,
-                                bool bf16, int sms, void* workspace, cudaStream_t stream);
+cudaError_t launch_paged_decode(DecodeParams p, int head_dim, int cache_dtype, bool bf16, int sms,
+                                cudaStream_t stream);
 // Chunk kernel and, for n_splits > 1, the join of its key splits.
 cudaError_t launch_paged_chunk(const ChunkParams& p, int head_dim, int cache_dtype, bool bf16,
                                int grid, cudaStream_t stream);

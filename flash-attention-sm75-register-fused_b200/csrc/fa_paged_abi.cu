@@ -72,11 +72,14 @@ int check_rows(const int* cu, const int* lens, int B, int total, fa::PagedRows* 
 
 // Which kernels a call runs and how its keys are split.
 //
-// Sequences of at most 16 query rows per KV head go to the decode kernel, the
-// others to the chunk kernel.  The lengths are on the device, so the host goes
-// by bounds: with max_seqlen_q rows of at most 16 every sequence is short; when
+// Sequences of few query rows per KV head go to the decode kernel, the others
+// to the chunk kernel.  The lengths are on the device, so the host goes by
+// bounds: with max_seqlen_q rows of at most 64 every sequence is short; when
 // the packed rows are exactly B full-length sequences every one is long; else
-// both kernels run, each on its own sequences.
+// both kernels run, the decode kernel on the sequences of at most kMixedRows
+// rows (single tokens mostly: a team of one warp).
+constexpr int kMixedRows = 16;
+
 struct PagedPlan {
   bool decode = false, chunk = false;
   int decode_rows = 0;  // rows per KV head the decode kernel takes at most
@@ -92,9 +95,9 @@ PagedPlan make_paged_plan(int B, int heads, int group, int head_dim, int total, 
   const long long rows = static_cast<long long>(max_q) * group;
   const int cap = fa::paged_decode_rows();
   k.chunk = rows > cap || B == 0 || max_q == 0;
-  k.decode = !k.chunk || (rows > cap && B > 1 && group <= cap &&
+  k.decode = !k.chunk || (rows > cap && B > 1 && group <= kMixedRows &&
                           total < static_cast<long long>(B) * max_q);
-  k.decode_rows = k.chunk ? (cap / group) * group : static_cast<int>(rows);
+  k.decode_rows = k.chunk ? (kMixedRows / group) * group : static_cast<int>(rows);
   if (k.decode) k.ws_decode = fa::paged_decode_ws_bytes(k.decode_rows, head_dim, sms);
   if (k.chunk) {
     k.tq = 128 / group;
@@ -136,14 +139,40 @@ int gcd_128(int x) {  // of x (a multiple of 16) and 128
   return g;
 }
 
-// Tensor maps of a 16-bit cache and its queries (the stride of a dimension
-// with one entry is free: any valid one serves).
-bool chunk_maps(const PagedPlan& k, const fa_paged_cache& c, const void* q, long long q_token,
-                long long q_head, int Hq, int total, bool bf16, fa::ChunkParams* p) {
+// Tensor maps of the pages, for boxes of `rows` rows (and 64 columns, or a
+// whole 8-bit row).  The stride of a dimension with one entry is free: any
+// valid one serves.
+bool page_maps(const fa_paged_cache& c, int rows, CUtensorMap* k, CUtensorMap* v) {
+  const int es = is_8bit(c.dtype) ? 1 : 2;
+  const unsigned long long row = static_cast<unsigned long long>(es) * c.head_dim;
+  auto st = [row, es](long long elems) { return elems > 0 ? static_cast<unsigned long long>(es) * elems : row; };
+  fa::TiledMap t{};
+  t.type = es == 1 ? fa::TiledMap::kBytes : c.dtype == FA_DTYPE_BF16 ? fa::TiledMap::kBf16 : fa::TiledMap::kF16;
+  t.rank = 4;
+  t.dims[0] = c.head_dim;
+  t.dims[1] = c.page_size;
+  t.dims[2] = c.kv_heads;
+  t.dims[3] = c.num_pages > 0 ? c.num_pages : 1;
+  t.strides[0] = st(c.row_stride);
+  t.strides[1] = st(c.head_stride);
+  t.strides[2] = st(c.page_stride);
+  t.box[0] = es == 1 ? c.head_dim : 64;
+  t.box[1] = rows;
+  t.box[2] = t.box[3] = 1;
+  t.base = c.k;
+  if (!fa::host_tensor_map(k, t)) return false;
+  t.base = c.v;
+  return fa::host_tensor_map(v, t);
+}
+
+// Tensor map of the queries: boxes of a query tile, `tq` tokens x the heads of
+// a group.
+bool query_map(const fa_paged_cache& c, int tq, const void* q, long long q_token, long long q_head,
+               int Hq, int total, bool bf16, CUtensorMap* map) {
   const unsigned long long row = 2ull * c.head_dim;
   auto st = [row](long long elems) { return elems > 0 ? 2ull * elems : row; };
   fa::TiledMap t{};
-  t.bf16 = bf16 ? 1 : 0;
+  t.type = bf16 ? fa::TiledMap::kBf16 : fa::TiledMap::kF16;
   t.base = q;
   t.rank = 3;
   t.dims[0] = c.head_dim;
@@ -153,21 +182,8 @@ bool chunk_maps(const PagedPlan& k, const fa_paged_cache& c, const void* q, long
   t.strides[1] = st(q_token);
   t.box[0] = 64;
   t.box[1] = Hq / c.kv_heads;
-  t.box[2] = k.tq;
-  if (!fa::host_tensor_map(&p->tm_q, t)) return false;
-  t.rank = 4;
-  t.dims[1] = c.page_size;
-  t.dims[2] = c.kv_heads;
-  t.dims[3] = c.num_pages > 0 ? c.num_pages : 1;
-  t.strides[0] = st(c.row_stride);
-  t.strides[1] = st(c.head_stride);
-  t.strides[2] = st(c.page_stride);
-  t.box[1] = p->box_rows;
-  t.box[2] = t.box[3] = 1;
-  t.base = c.k;
-  if (!fa::host_tensor_map(&p->tm_k, t)) return false;
-  t.base = c.v;
-  return fa::host_tensor_map(&p->tm_v, t);
+  t.box[2] = tq;
+  return fa::host_tensor_map(map, t);
 }
 
 }  // namespace
@@ -265,10 +281,18 @@ int fa_fwd_paged(const fa_paged_cache* cache, const void* Q, long long q_token_s
   a.scale_log2 = scale * 1.4426950408889634f;
   const bool bf16 = dtype == FA_DTYPE_BF16;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (k.decode &&
-      fa::launch_paged_decode(a, k.decode_rows, cache->head_dim, cache->dtype, bf16,
-                              fa::host_sm_count(), workspace, st) != cudaSuccess)
-    return FA_ERR_LAUNCH;
+  if (k.decode) {
+    fa::DecodeParams p;
+    p.a = a;
+    p.ws = static_cast<float*>(workspace);
+    p.max_rows = k.decode_rows;
+    p.epoch = fa::host_next_epoch();
+    p.timeout_ns = fa::host_timeout_ns();
+    if (!page_maps(*cache, 16, &p.tm_k, &p.tm_v)) return FA_ERR_TENSOR_MAP;
+    if (fa::launch_paged_decode(p, cache->head_dim, cache->dtype, bf16, fa::host_sm_count(), st) !=
+        cudaSuccess)
+      return FA_ERR_LAUNCH;
+  }
   if (k.chunk) {
     fa::ChunkParams p;
     p.a = a;
@@ -282,7 +306,8 @@ int fa_fwd_paged(const fa_paged_cache* cache, const void* Q, long long q_token_s
     p.epoch = fa::host_next_epoch();
     p.timeout_ns = fa::host_timeout_ns();
     if (!is_8bit(cache->dtype) &&
-        !chunk_maps(k, *cache, Q, q_token_stride, q_head_stride, Hq, total_q, bf16, &p))
+        (!page_maps(*cache, p.box_rows, &p.tm_k, &p.tm_v) ||
+         !query_map(*cache, p.tq, Q, q_token_stride, q_head_stride, Hq, total_q, bf16, &p.tm_q)))
       return FA_ERR_TENSOR_MAP;
     if (fa::launch_paged_chunk(p, cache->head_dim, cache->dtype, bf16, static_cast<int>(grid), st) !=
         cudaSuccess)

@@ -108,16 +108,6 @@ __device__ __forceinline__ float exp_tile_scaled(const float (&x)[kBlockN], floa
   return a0 + a1;
 }
 
-// 4-D tiled load (d, page row, head, page).
-__device__ __forceinline__ void tma_load_4d(uint32_t smem_dst, const void* tmap, uint32_t bar, int c0,
-                                            int c1, int c2, int c3, uint64_t policy) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
-      " [%0], [%1, {%3, %4, %5, %6}], [%2], %7;" ::"r"(smem_dst),
-      "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "l"(policy)
-      : "memory");
-}
-
 // The work item of a CTA.
 struct ChunkItem {
   Seq s;
@@ -287,7 +277,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
         __syncwarp();
         const uint32_t dst = sbase + L::kOffKV + slot * L::kTile;
         if (issues)
-          tma_load_4d(dst + dst_off, (i & 1) ? &p.tm_v : &p.tm_k, full, col * 64,
+          ptx::tma_load_4d(dst + dst_off, (i & 1) ? &p.tm_v : &p.tm_k, full, col * 64,
                       a.c.row_in_page(tile * kBlockN + box * p.box_rows), it.h, page, pol_kv);
         if (tail) {
           tail_used = true;

@@ -1,57 +1,56 @@
-// Attention of a few new tokens per sequence over a paged KV cache: at most 16
+// Attention of a few new tokens per sequence over a paged KV cache: at most 64
 // query rows per (sequence, KV head), i.e. new tokens x query heads of a group.
+// Included by fa_fwd_sm100.cu (bounded mbarrier waits, device status word).
 //
 //   s_ij = scale q_i . k_j,   O_i = sum_j softmax(s_i)_j v_j,
 //   LSE_i = log sum_j exp(s_ij)
 //
 // Bound by HBM: every key and value is read once for all rows of its group.
 // The kernel is therefore built around the loads.  A *unit* of work is 8 KB of
-// the cache, the K and V rows of `Sub` consecutive keys of one head (16 keys of
+// the cache, the K and V rows of kSub consecutive keys of one head (16 keys of
 // 16-bit d = 128 pages, 64 of 8-bit d = 64 pages).  All units of the batch, in
-// order of sequence, head and key, are cut into equal runs, one per warp,
-// whatever the sequences' lengths: no warp waits for another until the end of
-// the kernel, and ragged batches stay balanced.  A warp streams its run through
-// a private ring of shared-memory stages filled with 16-byte asynchronous
-// copies (zero-filled past the last visible key, so stale rows of a page never
-// enter the arithmetic), and keeps the online softmax (running maximum m, sum
-// l, O rescaled when m grows) in registers:
+// order of sequence, head and key, are cut into equal runs, one per team of
+// warps (one warp for up to 16 rows), whatever the sequences' lengths: no team
+// waits for another until the end of the kernel, and ragged batches stay
+// balanced.  A team streams its run through a ring of shared-memory stages,
+// filled by TMA boxes of 16 rows (one per lane, each with its own page), and
+// every warp keeps the online softmax of its 8 or 16 rows in registers
+// (running maximum m, sum l, O rescaled when m grows):
 //
 //   S^T = K Q^T     m16n8k16, keys on M, query rows on N: 8 rows cost one
 //                   instruction, not a 16-row tile
 //   P   = exp2(S - m), transposed in registers (movmatrix) into the B operand
 //   O^T += V^T P^T  V read transposed from the same stage
 //
-// The warp's tensor instructions are the small register-operand form: at 8 or
-// 16 rows they need a fifth to two thirds of what HBM delivers, and take
-// operands converted in registers, which 8-bit pages need: int8 and e4m3 both
-// become f16 exactly, K's scale multiplies the score and V's scale the
-// probability.  Because f16 has few exponent bits, V's scales are taken
-// relative to a power of two per warp that follows the largest one seen; bf16
-// queries over 8-bit pages are scaled per row by a power of two likewise.
+// The tensor instructions are the register-operand form: at 8 rows they need a
+// tenth of their rate to keep up with HBM, and they take operands converted in
+// registers, which 8-bit pages need: int8 and e4m3 both become f16 exactly, K's
+// scale multiplies the score and V's scale the probability.  Because f16 has
+// few exponent bits, V's scales are taken relative to a power of two per warp
+// that follows the largest one seen; bf16 queries over 8-bit pages are scaled
+// per row by a power of two likewise.
 //
-// A warp whose run covers a whole (sequence, head) writes O and LSE; otherwise
+// A team whose run covers a whole (sequence, head) writes O and LSE; otherwise
 // its unnormalised O, m and l go to one of its two workspace slots (its run's
-// first part, which continues a head of the warp before, or its last, which
-// the next warp continues) and paged_combine_kernel joins them in order.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_runtime.h>
-
-#include <cmath>
-#include <cstdint>
-
+// first part, which continues a head of the team before, or its last, which
+// the next team continues) and paged_combine_kernel joins them in order.
 #include "fa_paged.h"
 #include "fa_paged_dev.cuh"
-#include "sm100_ptx.cuh"
 
 namespace fa {
 namespace {
+namespace pdec {
 
-constexpr int kWarps = 4;    // per CTA
-constexpr int kStages = 3;   // ring stages of 8 KB per warp
-constexpr int kCtasPerSm = 2;
-constexpr int kRowsMax = 16;
+constexpr int kWarps = 4;  // per CTA
+constexpr int kRowsMax = 64;
 constexpr int kCombineThreads = 256;
+// Score maximum of a row that has seen no key: finite, so that differences of
+// maxima are never NaN, and below any score.
+constexpr float kNoMax = -1e30f;
+
+// NT: 8-row column blocks of a warp.
+__host__ __device__ constexpr int ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
+__host__ __device__ constexpr int stages_per_warp(int nt) { return nt == 1 ? 2 : 3; }
 
 template <int D, int KV>
 struct Cfg {
@@ -59,34 +58,29 @@ struct Cfg {
   static constexpr bool kBf16 = KV == FA_DTYPE_BF16;   // type of the products
   static constexpr int kRowBytes = k8 ? D : 2 * D;     // one K or V row
   static constexpr int kSub = 4096 / kRowBytes;        // keys of a unit
-  static constexpr int kChunks = kRowBytes / 16;       // 16-byte pieces of a row
-  static constexpr int kRowsPerPass = 32 / kChunks;
-  static constexpr int kPasses = kSub / kRowsPerPass;  // 8
-  static constexpr int kMT = kSub / 16;                // 16-key tiles
+  static constexpr int kBoxBytes = kRowBytes < 128 ? kRowBytes : 128;  // inner extent of a box
+  static constexpr int kCols = kRowBytes / kBoxBytes;  // boxes side by side
+  static constexpr int kMT = kSub / 16;                // 16-key groups
+  static constexpr int kBoxes = 2 * kCols * kMT;       // of a unit: (K, V) x columns x groups
   static constexpr int kKS = D / 16;                   // 16-column steps of d
   static constexpr int kScaleBytes = k8 ? kSub * 8 : 0;
-  static constexpr int kStageBytes = 8192 + kScaleBytes;
-  static constexpr int kSmem = kWarps * kStages * kStageBytes;
-  // 16-byte piece c of row r is stored at piece c ^ swz(r): eight rows at one
-  // piece lie in eight different bank groups
-  __device__ static __forceinline__ int swz(int r) {
-    return kChunks >= 8 ? (r & 7) : ((r >> 1) & 3);
+  __host__ __device__ static constexpr int smem(int nt) {
+    return 1024 + kWarps * stages_per_warp(nt) * (8192 + kScaleBytes);
   }
+  // Address of 16-byte piece c of row r of a K or V half stage: boxes of 16
+  // rows in the TMA swizzle (128-byte rows: piece ^ row % 8; 64-byte rows:
+  // piece ^ (row / 2) % 4), so eight rows at one piece hit eight bank groups.
+  __device__ static __forceinline__ uint32_t piece(int r, int c) {
+    if constexpr (kCols == 2) {
+      return (c >> 3) * 2048 + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+    } else if constexpr (kBoxBytes == 128) {
+      return r * 128 + ((c ^ (r & 7)) << 4);
+    } else {
+      return r * 64 + ((c ^ ((r >> 1) & 3)) << 4);
+    }
+  }
+  static_assert(kCols == 1 || kSub == 16, "two columns: one group of rows");
 };
-
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool valid) {
-  const int n = valid ? 16 : 0;
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void cp4(uint32_t dst, const void* src, bool valid) {
-  const int n = valid ? 4 : 0;
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -119,17 +113,6 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
         "{%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  }
-}
-
-template <bool BF16>
-__device__ __forceinline__ uint32_t pack2f(float lo, float hi) {
-  if constexpr (BF16) {
-    __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<uint32_t*>(&v);
-  } else {
-    __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<uint32_t*>(&v);
   }
 }
 
@@ -174,49 +157,57 @@ __host__ __device__ constexpr long long slot_floats(int rows, int d) {
   return static_cast<long long>(rows) * (d + 2);
 }
 
-struct DecodeParams {
-  PagedAttn a;
-  float* ws;
-  int n_warps;   // warps of the launch that take runs
-  int max_rows;  // query rows per KV head handled here (<= 8 * NT)
-};
-
-// Position of a warp in its run: the current unit's sequence, head and key.
+// Position of a team in its run: unit t of n of (sequence b, head h).
 struct Cursor {
   Seq s;
-  int b, h, t, n;  // unit t of n of (b, h)
+  int b, h, t, n;
 };
 
-template <int D, int KV, bool QBF16, int NT>
-__global__ void __launch_bounds__(32 * kWarps, kCtasPerSm)
+template <int D, int KV, bool QBF16, int NT, int TEAM>
+__global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
     paged_decode_kernel(const __grid_constant__ DecodeParams p) {
   using C = Cfg<D, KV>;
+  constexpr int kStages = stages_per_warp(NT) * TEAM;
+  constexpr int kTeams = kWarps / TEAM;
   const PagedAttn& a = p.a;
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ uint8_t smem_raw[];
   __shared__ long long sh_scan[kWarps];
-  __shared__ int sh_b[kWarps];
-  __shared__ long long sh_rel[kWarps];
+  __shared__ int sh_b[kTeams];
+  __shared__ long long sh_rel[kTeams];
+  __shared__ __align__(8) unsigned long long sh_bar[kTeams * kStages];
+  __shared__ int sh_abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, j = lane & 3;
   const int H = a.c.heads;
+  const int team = warp / TEAM, trank = warp % TEAM;
+  const int tid = static_cast<int>(blockIdx.x) * kTeams + team;
+  volatile int* abort_flag = &sh_abort;
   ptx::launch_dependents();
 
-  // ---- the warp's run [u0, u1) and where it starts
-  long long total, per, u0, u1;
-  int b_first = 0;
-  long long rel = 0;
+  // ---- set-up, and the team's run [u0, u1) of the batch's units
+  if (threadIdx.x == 0) {
+    const unsigned long long st = *reinterpret_cast<volatile unsigned long long*>(&g_fa_status);
+    sh_abort = ((st >> 32) == p.epoch && (st & 0xffffffffull) != 0ull) ? 1 : 0;
+    // a stage is full when its boxes have landed (and, 8-bit pages, the 32
+    // lanes' scales)
+    for (int i = 0; i < kTeams * kStages; ++i)
+      ptx::mbar_init(ptx::smem_u32(&sh_bar[i]), C::k8 ? 33u : 1u);
+    ptx::fence_barrier_init();
+  }
+  long long u0, u1, rel;
+  int b_first;
   {
     const int share = (a.r.B + 32 * kWarps - 1) / (32 * kWarps);
     const int s0 = min(static_cast<int>(threadIdx.x) * share, a.r.B), s1 = min(s0 + share, a.r.B);
-    long long sum = 0;
+    long long sum = 0, total;
     for (int b = s0; b < s1; ++b) sum += units_of(a, b, C::kSub, p.max_rows);
     const long long excl = block_scan<32 * kWarps>(sum, sh_scan, &total);
     total *= H;
-    per = (total + p.n_warps - 1) / p.n_warps;
+    const long long per = (total + p.n_teams - 1) / p.n_teams;
     const long long lo = excl * H, hi = (excl + sum) * H;
-    // the thread whose share holds a warp's first unit finds its sequence
-    for (int w = 0; w < kWarps; ++w) {
-      const long long u = per * (static_cast<long long>(blockIdx.x) * kWarps + w);
+    // the thread whose share holds a team's first unit finds its sequence
+    for (int w = 0; w < kTeams; ++w) {
+      const long long u = per * (static_cast<long long>(blockIdx.x) * kTeams + w);
       if (u < total && u >= lo && u < hi) {
         long long x = lo;
         for (int b = s0; b < s1; ++b) {
@@ -231,16 +222,23 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm)
       }
     }
     __syncthreads();
-    const int wid = static_cast<int>(blockIdx.x) * kWarps + warp;
-    u0 = min(per * wid, total);
+    u0 = min(per * tid, total);
     u1 = min(u0 + per, total);
-    if (u0 >= u1) return;
-    b_first = sh_b[warp];
-    rel = sh_rel[warp];
+    if (u0 >= u1 || *abort_flag) return;
+    b_first = sh_b[team];
+    rel = sh_rel[team];
   }
-  const int wid = static_cast<int>(blockIdx.x) * kWarps + warp;
+  const WaitCtl wc{abort_flag, p.timeout_ns, p.epoch};
+  // all warps of the team; a warp that failed makes the team leave together
+  auto team_ok = [&](bool v) -> bool {
+    if constexpr (TEAM == 1) {
+      return __all_sync(0xffffffffu, v);
+    } else {
+      return ptx::bar_and(1 + team, 32 * TEAM, v);
+    }
+  };
 
-  auto seek = [&](Cursor& c, int b) {  // first unit of the next sequence with keys, from b
+  auto seek = [&](Cursor& c, int b) {  // the next sequence with units, from b
     for (; b < a.r.B; ++b) {
       c.s = load_short(a, b, p.max_rows);
       c.n = (c.s.vis + C::kSub - 1) / C::kSub;
@@ -259,100 +257,105 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm)
   seek(cc, b_first);
   cc.h = static_cast<int>(rel / cc.n);
   cc.t = static_cast<int>(rel % cc.n);
-  Cursor ci = cc;  // unit being loaded
+  Cursor ci = cc;  // unit being loaded (the team's first warp)
 
   // ---- loads
-  const uint32_t ring = ptx::smem_u32(smem) + warp * (kStages * C::kStageBytes);
-  const int lrow = lane / C::kChunks, lchunk = lane % C::kChunks;
+  uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                                   ~static_cast<uintptr_t>(1023)) +
+                        team * kStages * 8192;
+  const uint32_t ring = ptx::smem_u32(smem);
+  // scales of all stages behind the data of all teams: per key K's, V's
+  const uint32_t sring = ring + (kWarps * stages_per_warp(NT) - team * kStages) * 8192 +
+                         team * kStages * C::kScaleBytes;
+  const uint32_t bars = ptx::smem_u32(&sh_bar[team * kStages]);
+  const uint64_t policy = ptx::policy_evict_first();  // every key is read once
+  // lane = (group * kCols + column) * 2 + (0: K, 1: V)
+  const int bgrp = lane / (2 * C::kCols), bcol = (lane >> 1) % C::kCols;
+  const bool boxes = lane < C::kBoxes;
+  const uint32_t box_dst = (lane & 1) * 4096 + (C::kCols == 2 ? bcol * 2048 : bgrp * 16 * C::kRowBytes);
+  const void* const box_map = (lane & 1) ? &p.tm_v : &p.tm_k;
   long long iu = u0;  // unit of ci
-  int pages[C::kMT];  // pages of ci's 16-key groups
-  auto load_pages = [&] {
-#pragma unroll
-    for (int m = 0; m < C::kMT; ++m) {
-      const int pos = ci.t * C::kSub + 16 * m;
-      pages[m] = pos < ci.s.vis ? a.c.lookup(ci.b, pos) : -1;
-    }
+  auto page_of_box = [&] {  // -1 (no key any row may see, or no page) reads as zeros
+    const int pos = ci.t * C::kSub + 16 * bgrp;
+    return boxes && pos < ci.s.vis ? a.c.lookup(ci.b, pos) : -1;
   };
-  load_pages();
+  int page = -1;
   int wstage = 0;
   auto issue = [&] {
-    if (iu < u1) {
-      const uint32_t st = ring + wstage * C::kStageBytes;
-      const int key0 = ci.t * C::kSub;
-      const int left = ci.s.vis - key0;  // rows of the unit that exist
-      const long long hoff = ci.h * a.c.head_stride + 16 * lchunk;
-      long long off[C::kMT];
+    if (iu >= u1) return;
+    const uint32_t bar = bars + 8 * wstage;
+    const int key0 = ci.t * C::kSub;
+    if (lane == 0) ptx::mbar_arrive_expect_tx(bar, 8192);
+    __syncwarp();
+    if (boxes)
+      ptx::tma_load_4d(ring + wstage * 8192 + box_dst, box_map, bar, bcol * (C::kBoxBytes / (C::k8 ? 1 : 2)),
+                       a.c.row_in_page(key0 + 16 * bgrp), ci.h, page, policy);
+    if constexpr (C::k8) {
+      const int left = ci.s.vis - key0;
 #pragma unroll
-      for (int m = 0; m < C::kMT; ++m)
-        off[m] = static_cast<long long>(pages[m]) * a.c.page_stride + hoff +
-                 static_cast<long long>(a.c.row_in_page(key0 + 16 * m)) * a.c.row_stride;
-#pragma unroll
-      for (int x = 0; x < C::kPasses; ++x) {
-        const int r = x * C::kRowsPerPass + lrow;  // key of the unit
-        const int m = (x * C::kRowsPerPass) / 16;
-        const bool ok = r < left && pages[m] >= 0;
-        const long long o = ok ? off[m] + static_cast<long long>(r & 15) * a.c.row_stride : 0;
-        const uint32_t d = st + r * C::kRowBytes + ((lchunk ^ C::swz(r)) << 4);
-        cp16(d, a.c.k + o, ok);
-        cp16(d + 4096, a.c.v + o, ok);
+      for (int x = 0; x < C::kSub / 32; ++x) {
+        const int r = x * 32 + lane;
+        const int pg = __shfl_sync(0xffffffffu, page, (r >> 4) * 2);
+        const bool ok = r < left && pg >= 0;
+        const long long o =
+            ok ? static_cast<long long>(pg) * a.c.s_page + ci.h * a.c.s_head +
+                     static_cast<long long>(a.c.row_in_page(key0 + (r & ~15)) + (r & 15)) * a.c.s_row
+               : 0;
+        const uint32_t d = sring + wstage * C::kScaleBytes + 8 * r;
+        ptx::cp_async4(d, a.c.ks + o, ok);
+        ptx::cp_async4(d + 4, a.c.vs + o, ok);
       }
-      if constexpr (C::k8) {
-#pragma unroll
-        for (int x = 0; x < C::kSub / 32; ++x) {
-          const int r = x * 32 + lane;
-          const int page = lane < 16 ? pages[2 * x] : pages[2 * x + 1];
-          const bool ok = r < left && page >= 0;
-          const long long o =
-              ok ? static_cast<long long>(page) * a.c.s_page + ci.h * a.c.s_head +
-                       static_cast<long long>(a.c.row_in_page(key0 + (r & ~15)) + (r & 15)) * a.c.s_row
-                 : 0;
-          cp4(st + 8192 + 8 * r, a.c.ks + o, ok);
-          cp4(st + 8192 + 8 * r + 4, a.c.vs + o, ok);
-        }
-      }
-      if (++wstage == kStages) wstage = 0;
-      if (++iu < u1) {
-        advance(ci);
-        load_pages();
-      }
+      ptx::cp_async_arrive(bar);
     }
-    cp_commit();
+    if (++wstage == kStages) wstage = 0;
+    if (++iu < u1) {
+      advance(ci);
+      page = page_of_box();
+    }
   };
-#pragma unroll
-  for (int x = 0; x < kStages - 1; ++x) issue();
+  if (trank == 0) {
+    page = page_of_box();
+    for (int x = 0; x < kStages - 1; ++x) issue();
+  }
 
   // ---- the segments (sequence, head) of the run
-  constexpr float kGrow = 8.f;        // O and l are rescaled when m grows by more (log2)
-  constexpr float kTinyScale = 7.8886090522101181e-31f;  // 2^-100
+  constexpr float kGrow = 8.f;  // O and l are rescaled when m grows by more (log2)
+  // a negative scale goes into Q's sign; a zero one must not meet a masked -inf
+  const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+  const float scale_abs = fmaxf(fabsf(a.scale_log2), 1e-30f);
   int rstage = 0;
+  uint32_t rphase = 0;
+  bool ok = true;
   long long u = u0;
-  while (u < u1) {
+  while (ok && u < u1) {
     const Seq s = cc.s;
     const int t_begin = cc.t, n_units = cc.n;
     const int t_end = static_cast<int>(min(static_cast<long long>(n_units), t_begin + (u1 - u)));
     const int rows = s.nq * a.group;
-    // Q as the B operand: row 8 nt + g, columns 16 ks + {2j, 2j + 1, 8 + 2j, 9 + 2j}
-    // (8-bit pages: 16 ks + 4j .. 4j + 3, the order their bytes come in)
+    const int row0 = trank * 8 * NT;  // of this warp
+    const bool active = row0 < rows;
+    // Q as the B operand: row row0 + 8 nt + g, columns 16 ks + {2j, 2j + 1,
+    // 8 + 2j, 9 + 2j} (8-bit pages: 16 ks + 4j .. 4j + 3, the order their
+    // bytes come in)
     uint32_t q[NT][C::kKS][2];
-    float colscale[NT][2];
+    float cs[NT][2];  // score scale of this thread's columns
     int lim[NT][2];
-    int min_lim = 0x7fffffff;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int r = nt * 8 + g;
+      const int r = row0 + nt * 8 + g;
       const int tok = r / a.group, hq = cc.h * a.group + r % a.group;
       const uint8_t* src = a.q + static_cast<long long>(s.c0 + tok) * a.q_token + hq * a.q_head;
-      const bool ok = r < rows;
+      const bool have = r < rows;
 #pragma unroll
       for (int k = 0; k < C::kKS; ++k) {
         if constexpr (C::k8) {
           uint2 w = make_uint2(0u, 0u);
-          if (ok) w = __ldg(reinterpret_cast<const uint2*>(src + 32 * k + 8 * j));
+          if (have) w = __ldg(reinterpret_cast<const uint2*>(src + 32 * k + 8 * j));
           q[nt][k][0] = w.x;
           q[nt][k][1] = w.y;
         } else {
-          q[nt][k][0] = ok ? __ldg(reinterpret_cast<const uint32_t*>(src + 32 * k + 4 * j)) : 0u;
-          q[nt][k][1] = ok ? __ldg(reinterpret_cast<const uint32_t*>(src + 32 * k + 16 + 4 * j)) : 0u;
+          q[nt][k][0] = have ? __ldg(reinterpret_cast<const uint32_t*>(src + 32 * k + 4 * j)) : 0u;
+          q[nt][k][1] = have ? __ldg(reinterpret_cast<const uint32_t*>(src + 32 * k + 16 + 4 * j)) : 0u;
         }
       }
       float unit = 1.f;
@@ -377,19 +380,23 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&q[nt][k][i]));
-            q[nt][k][i] = pack2f<false>(f.x * inv, f.y * inv);
+            q[nt][k][i] = pack2<false>(f.x * inv, f.y * inv);
           }
       }
 #pragma unroll
+      for (int k = 0; k < C::kKS; ++k) {
+        q[nt][k][0] ^= flip;
+        q[nt][k][1] ^= flip;
+      }
+#pragma unroll
       for (int c = 0; c < 2; ++c) {
-        colscale[nt][c] = a.scale_log2;
-        if constexpr (C::k8 && QBF16)
-          colscale[nt][c] *= __shfl_sync(0xffffffffu, unit, (2 * j + c) * 4);
-        const int rc = nt * 8 + 2 * j + c;
+        cs[nt][c] = scale_abs;
+        if constexpr (C::k8 && QBF16) cs[nt][c] *= __shfl_sync(0xffffffffu, unit, (2 * j + c) * 4);
+        const int rc = row0 + nt * 8 + 2 * j + c;
         lim[nt][c] = rc < rows ? row_limit(a, s, rc / a.group) : 0;
       }
     }
-    min_lim = row_limit(a, s, 0);
+    const int min_lim = row_limit(a, s, 0);
 
     float o[NT][C::kKS][4];
     float m[NT][2], l[NT][2];
@@ -399,17 +406,41 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm)
       for (int k = 0; k < C::kKS; ++k)
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[nt][k][i] = 0.f;
-      m[nt][0] = m[nt][1] = -INFINITY;
+      m[nt][0] = m[nt][1] = kNoMax;
       l[nt][0] = l[nt][1] = 0.f;
     }
-    float vref = kTinyScale, rv = 1.f / kTinyScale;  // V scales relative to vref
+    // V's scales are relative to 2^lv: p = exp2(s - m - lv) is summed, and
+    // p * vs multiplies V's 8-bit values
+    int lv = C::k8 ? -60 : 0;
 
     for (int t = t_begin; t < t_end; ++t) {
-      cp_wait<kStages - 2>();
-      __syncwarp();
-      issue();
-      const uint32_t st = ring + rstage * C::kStageBytes;
-      if (++rstage == kStages) rstage = 0;
+      ok = bar_wait(bars + 8 * rstage, rphase, wc, 50);
+      // (also: every warp is done with the stage before, which is refilled now)
+      if (!(ok = team_ok(ok))) break;
+      if (trank == 0) issue();
+      const uint32_t st = ring + rstage * 8192;
+      const uint32_t sst = sring + rstage * C::kScaleBytes;
+      uint8_t* const stage = smem + rstage * 8192;
+      if (++rstage == kStages) {
+        rstage = 0;
+        rphase ^= 1u;
+      }
+      const int key0 = t * C::kSub;
+      const int left = s.vis - key0;
+      if (KV != FA_DTYPE_INT8 && left < C::kSub) {
+        // rows of V behind the last visible key are stale and might hold NaN
+        // (those of a group without any visible key are zero already; int8
+        // has no NaN)
+        const int end = min(C::kSub, (left + 15) & ~15);
+        for (int x = left * 32 + static_cast<int>(threadIdx.x % (32 * TEAM)); x < end * 32; x += 32 * TEAM) {
+          const int r = x >> 5, c = x & 31;
+          if (c < C::kRowBytes / 16)
+            *reinterpret_cast<uint4*>(stage + 4096 + C::piece(r, c)) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        ptx::fence_proxy_async_smem();  // before a later copy into this stage
+        if (!(ok = team_ok(true))) break;
+      }
+      if (!active) continue;
       // S^T = K Q^T
       float sc[NT][C::kMT][4];
 #pragma unroll
@@ -420,23 +451,21 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm)
           for (int i = 0; i < 4; ++i) sc[nt][mt][i] = 0.f;
         if constexpr (!C::k8) {
           const int r = mt * 16 + (lane & 15);
-          const uint32_t row = st + r * C::kRowBytes;
 #pragma unroll
           for (int k = 0; k < C::kKS; ++k) {
             uint32_t f[4];
-            ldsm4(row + (((2 * k + (lane >> 4)) ^ C::swz(r)) << 4), f);
+            ldsm4(st + C::piece(r, 2 * k + (lane >> 4)), f);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
               mma16816<C::kBf16>(sc[nt][mt], f[0], f[1], f[2], f[3], q[nt][k][0], q[nt][k][1]);
           }
         } else {
           // two 16-column steps per ldmatrix: keys 0-7 and 8-15 of pieces k, k + 1
-          const int r = mt * 16 + (lane & 7) + ((lane & 8) ? 8 : 0);
-          const uint32_t row = st + r * C::kRowBytes;
+          const int r = mt * 16 + (lane & 15);
 #pragma unroll
           for (int k = 0; k < C::kKS; k += 2) {
             uint32_t f[4];
-            ldsm4(row + (((k + (lane >> 4)) ^ C::swz(r)) << 4), f);
+            ldsm4(st + C::piece(r, k + (lane >> 4)), f);
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
               uint32_t a0, a1, a2, a3;
@@ -449,48 +478,68 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm)
           }
         }
       }
-      // scores in log2 units, masked; do the maxima grow?
+      // scores (without their common factor cs), masked, and their maxima
       float vsc[C::kMT][2];
-      const int key0 = t * C::kSub;
-      const bool masked = key0 + C::kSub > min_lim;
-      bool grow = false, vgrow = false;
+      float vmax = 0.f;
+      if constexpr (C::k8) {
 #pragma unroll
-      for (int mt = 0; mt < C::kMT; ++mt)
+        for (int mt = 0; mt < C::kMT; ++mt)
 #pragma unroll
-        for (int hh = 0; hh < 2; ++hh) {
-          float ks = 1.f;
-          const int r = mt * 16 + g + 8 * hh;
-          if constexpr (C::k8) {
+          for (int hh = 0; hh < 2; ++hh) {
             float2 f;
-            asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(f.x), "=f"(f.y) : "r"(st + 8192 + 8 * r) : "memory");
-            ks = f.x;
+            asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];"
+                         : "=f"(f.x), "=f"(f.y)
+                         : "r"(sst + 8 * (mt * 16 + g + 8 * hh))
+                         : "memory");
             vsc[mt][hh] = f.y;
-            vgrow |= f.y * rv > 64.f;
+            vmax = fmaxf(vmax, f.y);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              sc[nt][mt][2 * hh] *= f.x;
+              sc[nt][mt][2 * hh + 1] *= f.x;
+            }
           }
+      }
+      if (key0 + C::kSub > min_lim) {
+#pragma unroll
+        for (int mt = 0; mt < C::kMT; ++mt)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-              float x = sc[nt][mt][2 * hh + c];
-              if constexpr (C::k8) x *= ks;
-              x *= colscale[nt][c];
-              if (masked && key0 + r >= lim[nt][c]) x = -INFINITY;
-              sc[nt][mt][2 * hh + c] = x;
-              grow |= x > m[nt][c] + kGrow;
-            }
+            for (int i = 0; i < 4; ++i)
+              if (key0 + mt * 16 + g + 8 * (i >> 1) >= lim[nt][i & 1]) sc[nt][mt][i] = -INFINITY;
+      }
+      bool grow = C::k8 && __float_as_int(vmax) >= (lv + 127 + 6) << 23;
+      float top[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float x = fmaxf(sc[nt][0][c], sc[nt][0][2 + c]);
+#pragma unroll
+          for (int mt = 1; mt < C::kMT; ++mt) x = fmaxf(x, fmaxf(sc[nt][mt][c], sc[nt][mt][2 + c]));
+          top[nt][c] = x;
+          grow |= fmaf(x, cs[nt][c], -m[nt][c]) > kGrow;
         }
       if (__any_sync(0xffffffffu, grow)) {
+        float fv = 1.f;
+        if constexpr (C::k8) {
+          // vmax < 2^(lv + 1) now; p * vs stays below 2^8 * 2^6 until lv moves again
+          const int e = (__reduce_max_sync(0xffffffffu, __float_as_int(vmax)) >> 23) - 127;
+          const int nlv = max(lv, min(e, 100));
+          fv = ptx::ex2_approx(static_cast<float>(lv - nlv));
+          lv = nlv;
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float x = m[nt][c];
-#pragma unroll
-            for (int mt = 0; mt < C::kMT; ++mt) x = fmaxf(x, fmaxf(sc[nt][mt][c], sc[nt][mt][2 + c]));
+            float x = top[nt][c];
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
             x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-            const float f = x == -INFINITY ? 1.f : ptx::ex2_approx(m[nt][c] - x);
+            x = fmaxf(m[nt][c], x * cs[nt][c]);
+            const float f = ptx::ex2_approx(m[nt][c] - x) * fv;
             m[nt][c] = x;
             l[nt][c] *= f;
 #pragma unroll
@@ -500,56 +549,34 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm)
             }
           }
       }
-      if constexpr (C::k8) {
-        if (__any_sync(0xffffffffu, vgrow)) {
-          float x = 0.f;
-#pragma unroll
-          for (int mt = 0; mt < C::kMT; ++mt) x = fmaxf(x, fmaxf(vsc[mt][0], vsc[mt][1]));
-#pragma unroll
-          for (int w = 16; w > 0; w >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, w));
-          const float nref = __uint_as_float(__float_as_uint(x) & 0x7f800000u);
-          rv = 1.f / nref;
-          const float f = vref * rv;
-          vref = nref;
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int k = 0; k < C::kKS; ++k)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) o[nt][k][i] *= f;
-        }
-      }
       // P and O^T += V^T P^T
       uint32_t pb[NT][C::kMT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const float n0 = m[nt][0] == -INFINITY ? 0.f : -m[nt][0];
-        const float n1 = m[nt][1] == -INFINITY ? 0.f : -m[nt][1];
+        const float n0 = -(m[nt][0] + static_cast<float>(lv)), n1 = -(m[nt][1] + static_cast<float>(lv));
 #pragma unroll
         for (int mt = 0; mt < C::kMT; ++mt)
 #pragma unroll
           for (int hh = 0; hh < 2; ++hh) {
-            float p0 = ptx::ex2_approx(sc[nt][mt][2 * hh] + n0);
-            float p1 = ptx::ex2_approx(sc[nt][mt][2 * hh + 1] + n1);
+            float p0 = ptx::ex2_approx(fmaf(sc[nt][mt][2 * hh], cs[nt][0], n0));
+            float p1 = ptx::ex2_approx(fmaf(sc[nt][mt][2 * hh + 1], cs[nt][1], n1));
             l[nt][0] += p0;
             l[nt][1] += p1;
             if constexpr (C::k8) {
-              const float f = vsc[mt][hh] * rv;
-              p0 *= f;
-              p1 *= f;
+              p0 *= vsc[mt][hh];
+              p1 *= vsc[mt][hh];
             }
-            pb[nt][mt][hh] = transpose8(pack2f<C::kBf16>(p0, p1));
+            pb[nt][mt][hh] = transpose8(pack2<C::kBf16>(p0, p1));
           }
       }
       if constexpr (!C::k8) {
 #pragma unroll
         for (int mt = 0; mt < C::kMT; ++mt) {
           const int r = mt * 16 + (lane & 7) + ((lane & 16) ? 8 : 0);
-          const uint32_t row = st + 4096 + r * C::kRowBytes;
 #pragma unroll
           for (int k = 0; k < C::kKS; ++k) {
             uint32_t f[4];
-            ldsm4t(row + (((2 * k + ((lane >> 3) & 1)) ^ C::swz(r)) << 4), f);
+            ldsm4t(st + 4096 + C::piece(r, 2 * k + ((lane >> 3) & 1)), f);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
               mma16816<C::kBf16>(o[nt][k], f[0], f[1], f[2], f[3], pb[nt][mt][0], pb[nt][mt][1]);
@@ -561,11 +588,10 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm)
 #pragma unroll
         for (int mt = 0; mt < C::kMT; mt += 2) {
           const int r = mt * 16 + lane;
-          const uint32_t row = st + 4096 + r * C::kRowBytes;
 #pragma unroll
           for (int k = 0; k < C::kKS; ++k) {
             uint32_t f[4];
-            ldsm4t(row + ((k ^ C::swz(r)) << 4), f);
+            ldsm4t(st + 4096 + C::piece(r, k), f);
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
               uint32_t a0, a1, a2, a3;
@@ -579,10 +605,10 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm)
         }
       }
     }
+    if (!ok) break;
 
     // ---- the segment's result
     const bool first = t_begin == 0, last = t_end == n_units;
-    const float ov = C::k8 ? vref : 1.f;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -592,6 +618,7 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm)
         x += __shfl_xor_sync(0xffffffffu, x, 8);
         x += __shfl_xor_sync(0xffffffffu, x, 16);
         l[nt][c] = x;
+        m[nt][c] += static_cast<float>(lv);
       }
     // column of o[..][k][2 hh + c]
     auto col = [&](int k, int hh) { return C::k8 ? 16 * k + 2 * g + hh : 16 * k + g + 8 * hh; };
@@ -599,15 +626,15 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm)
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const int r = nt * 8 + 2 * j + c;
+        const int r = row0 + nt * 8 + 2 * j + c;
         if (r >= rows) continue;
         if (first && last) {
           const int tok = s.c0 + r / a.group, hq = cc.h * a.group + r % a.group;
-          const float inv = l[nt][c] > 0.f ? ov / l[nt][c] : 0.f;
+          const float inv = l[nt][c] == 0.f ? 0.f : 1.f / l[nt][c];
           uint16_t* dst = static_cast<uint16_t*>(a.o) + (static_cast<long long>(tok) * a.Hq + hq) * D;
 #pragma unroll
           for (int k = 0; k < C::kKS; ++k) {
-            const uint32_t w = pack2f<QBF16>(o[nt][k][c] * inv, o[nt][k][2 + c] * inv);
+            const uint32_t w = pack2<QBF16>(o[nt][k][c] * inv, o[nt][k][2 + c] * inv);
             if constexpr (C::k8) {
               *reinterpret_cast<uint32_t*>(dst + col(k, 0)) = w;
             } else {
@@ -617,18 +644,19 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm)
           }
           if (g == 0 && a.lse != nullptr)
             a.lse[static_cast<long long>(hq) * a.r.total + tok] =
-                l[nt][c] > 0.f ? (m[nt][c] + __log2f(l[nt][c])) * 0.69314718055994530942f : -INFINITY;
+                l[nt][c] == 0.f ? -INFINITY : (m[nt][c] + __log2f(l[nt][c])) * 0.69314718055994530942f;
         } else {
-          // slot 0: continues the head of an earlier warp; slot 1: begins one
-          float* slot = p.ws + (2ll * wid + (first ? 1 : 0)) * slot_floats(8 * NT, D);
+          // slot 0: continues the head of an earlier team; slot 1: begins one
+          constexpr int kSlotRows = 8 * NT * TEAM;
+          float* slot = p.ws + (2ll * tid + (first ? 1 : 0)) * slot_floats(kSlotRows, D);
 #pragma unroll
           for (int k = 0; k < C::kKS; ++k) {
-            slot[r * D + col(k, 0)] = o[nt][k][c] * ov;
-            slot[r * D + col(k, 1)] = o[nt][k][2 + c] * ov;
+            slot[r * D + col(k, 0)] = o[nt][k][c];
+            slot[r * D + col(k, 1)] = o[nt][k][2 + c];
           }
           if (g == 0) {
-            slot[8 * NT * D + r] = m[nt][c];
-            slot[8 * NT * D + 8 * NT + r] = l[nt][c];
+            slot[kSlotRows * D + r] = m[nt][c];
+            slot[kSlotRows * D + kSlotRows + r] = l[nt][c];
           }
         }
       }
@@ -639,13 +667,24 @@ __global__ void __launch_bounds__(32 * kWarps, kCtasPerSm)
       advance(cc);
     }
   }
-  cp_wait<0>();
+  // after a failed wait: copies in flight land before the CTA exits
+  if (!ok && trank == 0) {
+    for (int x = 0; x < kStages; ++x) {
+      bar_wait(bars + 8 * rstage, rphase, wc, 51, false);
+      if (++rstage == kStages) {
+        rstage = 0;
+        rphase ^= 1u;
+      }
+      if (rstage == wstage) break;
+    }
+    ptx::cp_async_wait_all();
+  }
 }
 
 // Joins the partial results of (sequence, KV head) blockIdx.x, query row
-// blockIdx.y: with M = max m_s over its slots in order of the warps,
+// blockIdx.y: with M = max m_s over its slots in order of the teams,
 //   O = sum 2^(m_s - M) O_s / sum 2^(m_s - M) l_s.
-// Also writes the rows that no warp of the decode kernel computes: rows of
+// Also writes the rows that no team of the decode kernel computes: rows of
 // sequences without visible keys and packed rows of no sequence.
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kCombineThreads)
@@ -687,22 +726,22 @@ __global__ void __launch_bounds__(kCombineThreads)
     return;
   }
   const long long total = sp.total * a.c.heads;
-  const long long per = (total + p.n_warps - 1) / p.n_warps;
+  const long long per = (total + p.n_teams - 1) / p.n_teams;
   const long long t0 = sp.before * a.c.heads + static_cast<long long>(h) * n;
   const int w0 = static_cast<int>(t0 / per), w1 = static_cast<int>((t0 + n - 1) / per);
-  if (w0 == w1) return;  // one warp had it all
+  if (w0 == w1) return;  // one team had it all
   const long long stride = slot_floats(slot_rows, D);
   auto slot_of = [&](int w) { return p.ws + (2ll * w + (w == w0 ? 1 : 0)) * stride; };
   // each warp joins every 8th slot, the block joins the warps
   constexpr int E = D / 32;
-  float mm = -INFINITY, ll = 0.f, acc[E] = {};
+  float mm = kNoMax, ll = 0.f, acc[E] = {};
   constexpr int kBatch = 4;
   for (int w = w0 + warp; w <= w1; w += kBatch * (kCombineThreads / 32)) {
     float mi[kBatch], li[kBatch], v[kBatch][E];
 #pragma unroll
     for (int x = 0; x < kBatch; ++x) {
       const int ww = w + x * (kCombineThreads / 32);
-      mi[x] = -INFINITY;
+      mi[x] = kNoMax;
       li[x] = 0.f;
 #pragma unroll
       for (int e = 0; e < E; ++e) v[x][e] = 0.f;
@@ -725,9 +764,8 @@ __global__ void __launch_bounds__(kCombineThreads)
     }
 #pragma unroll
     for (int x = 0; x < kBatch; ++x) {
-      if (mi[x] == -INFINITY) continue;
       const float mn = fmaxf(mm, mi[x]);
-      const float f0 = mm == -INFINITY ? 0.f : exp2f(mm - mn), f1 = exp2f(mi[x] - mn);
+      const float f0 = exp2f(mm - mn), f1 = exp2f(mi[x] - mn);
       mm = mn;
       ll = ll * f0 + li[x] * f1;
 #pragma unroll
@@ -742,42 +780,42 @@ __global__ void __launch_bounds__(kCombineThreads)
   for (int e = 0; e < E; ++e) sh_o[warp][lane * E + e] = acc[e];
   __syncthreads();
   if (threadIdx.x < D / 2) {
-    float M = -INFINITY;
+    float M = kNoMax;
 #pragma unroll
     for (int w = 0; w < kCombineThreads / 32; ++w) M = fmaxf(M, sh_m[w]);
     float L = 0.f, x0 = 0.f, x1 = 0.f;
 #pragma unroll
     for (int w = 0; w < kCombineThreads / 32; ++w) {
-      const float f = sh_m[w] == -INFINITY ? 0.f : exp2f(sh_m[w] - M);
+      const float f = exp2f(sh_m[w] - M);
       L += f * sh_l[w];
       x0 += f * sh_o[w][2 * threadIdx.x];
       x1 += f * sh_o[w][2 * threadIdx.x + 1];
     }
-    const float inv = L > 0.f ? 1.f / L : 0.f;
-    reinterpret_cast<uint32_t*>(dst)[threadIdx.x] = pack2f<BF16>(x0 * inv, x1 * inv);
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    reinterpret_cast<uint32_t*>(dst)[threadIdx.x] = pack2<BF16>(x0 * inv, x1 * inv);
     if (threadIdx.x == 0 && a.lse != nullptr)
       a.lse[static_cast<long long>(hq) * a.r.total + tok] =
-          L > 0.f ? (M + log2f(L)) * 0.69314718055994530942f : -INFINITY;
+          L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994530942f;
   }
 }
 
-template <int D, int KV, bool QBF16, int NT>
-cudaError_t launch_kv(const DecodeParams& p, int n_ctas, cudaStream_t stream) {
+template <int D, int KV, bool QBF16, int NT, int TEAM>
+cudaError_t launch_impl(const DecodeParams& p, int n_ctas, cudaStream_t stream) {
   using C = Cfg<D, KV>;
-  auto kern = paged_decode_kernel<D, KV, QBF16, NT>;
+  auto kern = paged_decode_kernel<D, KV, QBF16, NT, TEAM>;
   static int attr_done[64] = {0};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !attr_done[dev]) {
     const cudaError_t e =
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::smem(NT));
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) attr_done[dev] = 1;
   }
-  kern<<<n_ctas, 32 * kWarps, C::kSmem, stream>>>(p);
+  kern<<<n_ctas, 32 * kWarps, C::smem(NT), stream>>>(p);
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  // the combine may start while the last warps finish; it waits for them
+  // the combine may start while the last teams finish; it waits for them
   // before it reads a slot
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(static_cast<unsigned>(p.a.r.B) * p.a.c.heads, p.max_rows);
@@ -788,58 +826,66 @@ cudaError_t launch_kv(const DecodeParams& p, int n_ctas, cudaStream_t stream) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_combine_kernel<D, QBF16>, p, static_cast<int>(C::kSub), 8 * NT);
+  return cudaLaunchKernelEx(&cfg, paged_combine_kernel<D, QBF16>, p, static_cast<int>(C::kSub),
+                            8 * NT * TEAM);
+}
+
+// Rows of a team and how it is made up: one warp for 8 or 16 rows, two or four
+// of 16 rows each for more.
+struct Team {
+  int nt, warps;
+};
+Team team_for(int max_rows) {
+  return max_rows <= 8 ? Team{1, 1} : max_rows <= 16 ? Team{2, 1} : max_rows <= 32 ? Team{2, 2} : Team{2, 4};
 }
 
 template <int D, int KV, bool QBF16>
-cudaError_t launch_nt(const DecodeParams& p, int n_ctas, cudaStream_t s) {
-  return p.max_rows <= 8 ? launch_kv<D, KV, QBF16, 1>(p, n_ctas, s)
-                         : launch_kv<D, KV, QBF16, 2>(p, n_ctas, s);
+cudaError_t launch_rows(const DecodeParams& p, int n_ctas, cudaStream_t s) {
+  if (p.max_rows <= 8) return launch_impl<D, KV, QBF16, 1, 1>(p, n_ctas, s);
+  if (p.max_rows <= 16) return launch_impl<D, KV, QBF16, 2, 1>(p, n_ctas, s);
+  if (p.max_rows <= 32) return launch_impl<D, KV, QBF16, 2, 2>(p, n_ctas, s);
+  return launch_impl<D, KV, QBF16, 2, 4>(p, n_ctas, s);
 }
 
 template <int D>
 cudaError_t launch_d(const DecodeParams& p, int kv, bool bf16, int n_ctas, cudaStream_t s) {
   switch (kv) {
     case FA_DTYPE_INT8:
-      return bf16 ? launch_nt<D, FA_DTYPE_INT8, true>(p, n_ctas, s)
-                  : launch_nt<D, FA_DTYPE_INT8, false>(p, n_ctas, s);
+      return bf16 ? launch_rows<D, FA_DTYPE_INT8, true>(p, n_ctas, s)
+                  : launch_rows<D, FA_DTYPE_INT8, false>(p, n_ctas, s);
     case FA_DTYPE_E4M3:
-      return bf16 ? launch_nt<D, FA_DTYPE_E4M3, true>(p, n_ctas, s)
-                  : launch_nt<D, FA_DTYPE_E4M3, false>(p, n_ctas, s);
-    case FA_DTYPE_BF16: return launch_nt<D, FA_DTYPE_BF16, true>(p, n_ctas, s);
-    default: return launch_nt<D, FA_DTYPE_F16, false>(p, n_ctas, s);
+      return bf16 ? launch_rows<D, FA_DTYPE_E4M3, true>(p, n_ctas, s)
+                  : launch_rows<D, FA_DTYPE_E4M3, false>(p, n_ctas, s);
+    case FA_DTYPE_BF16: return launch_rows<D, FA_DTYPE_BF16, true>(p, n_ctas, s);
+    default: return launch_rows<D, FA_DTYPE_F16, false>(p, n_ctas, s);
   }
 }
 
-int decode_ctas(int sms) { return sms * kCtasPerSm; }
-
+}  // namespace pdec
 }  // namespace
 
-int paged_decode_rows() { return kRowsMax; }
+int paged_decode_rows() { return pdec::kRowsMax; }
 
 size_t paged_decode_ws_bytes(int max_rows, int head_dim, int sms) {
-  const int rows = max_rows <= 8 ? 8 : 16;
-  return static_cast<size_t>(decode_ctas(sms)) * kWarps * 2 *
-         static_cast<size_t>(slot_floats(rows, head_dim)) * sizeof(float);
+  const pdec::Team t = pdec::team_for(max_rows);
+  const size_t teams = static_cast<size_t>(sms) * pdec::ctas_per_sm(t.nt) * (pdec::kWarps / t.warps);
+  return 2 * teams * static_cast<size_t>(pdec::slot_floats(8 * t.nt * t.warps, head_dim)) * sizeof(float);
 }
 
-cudaError_t launch_paged_decode(const PagedAttn& a, int max_rows, int head_dim, int cache_dtype,
-                                bool bf16, int sms, void* workspace, cudaStream_t stream) {
-  DecodeParams p;
-  p.a = a;
-  p.ws = static_cast<float*>(workspace);
-  p.max_rows = max_rows;
-  // no more warps than units there can be
-  const int row_bytes = head_dim * (cache_dtype >= FA_DTYPE_INT8 ? 1 : 2);
-  const int sub = 4096 / row_bytes;
-  const long long units =
-      static_cast<long long>(a.r.B) * a.c.heads * ((static_cast<long long>(a.max_k) + sub - 1) / sub);
-  long long ctas = (units + kWarps - 1) / kWarps;
-  if (ctas > decode_ctas(sms)) ctas = decode_ctas(sms);
-  if (ctas < 1) ctas = 1;
-  p.n_warps = static_cast<int>(ctas) * kWarps;
-  return head_dim == 64 ? launch_d<64>(p, cache_dtype, bf16, static_cast<int>(ctas), stream)
-                        : launch_d<128>(p, cache_dtype, bf16, static_cast<int>(ctas), stream);
+cudaError_t launch_paged_decode(DecodeParams p, int head_dim, int kv, bool bf16, int sms,
+                                cudaStream_t stream) {
+  const pdec::Team t = pdec::team_for(p.max_rows);
+  const int per_cta = pdec::kWarps / t.warps;
+  // no more teams than units there can be
+  const int sub = 4096 / (head_dim * (kv >= FA_DTYPE_INT8 ? 1 : 2));
+  const long long units = static_cast<long long>(p.a.r.B) * p.a.c.heads *
+                          ((static_cast<long long>(p.a.max_k) + sub - 1) / sub);
+  long long ctas = (units + per_cta - 1) / per_cta;
+  const long long most = static_cast<long long>(sms) * pdec::ctas_per_sm(t.nt);
+  ctas = ctas > most ? most : ctas < 1 ? 1 : ctas;
+  p.n_teams = static_cast<int>(ctas) * per_cta;
+  return head_dim == 64 ? pdec::launch_d<64>(p, kv, bf16, static_cast<int>(ctas), stream)
+                        : pdec::launch_d<128>(p, kv, bf16, static_cast<int>(ctas), stream);
 }
 
 }  // namespace fa
