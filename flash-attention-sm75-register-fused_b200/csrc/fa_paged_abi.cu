@@ -36,7 +36,7 @@ int check_cache(const fa_paged_cache* c, int dtype, fa::PagedCache* out) {
       (reinterpret_cast<uintptr_t>(c->k_scale) & 3u) || (reinterpret_cast<uintptr_t>(c->v_scale) & 3u))
     return FA_ERR_ALIGNMENT;
   // positions are int32
-  if (static_cast<long long>(c->max_pages) * c->page_size > (1LL << 30) || c->kv_heads > (1 << 16))
+  if (static_cast<long long>(c->max_pages) * c->page_size > (1LL << 30) || c->kv_heads > (1 << 14))
     return FA_ERR_TOO_LARGE;
   out->k = static_cast<const uint8_t*>(c->k);
   out->v = static_cast<const uint8_t*>(c->v);
@@ -203,7 +203,8 @@ int fa_kvcache_write(const fa_paged_cache* cache, const void* K, const void* V,
   if (!aligned16(K) || !aligned16(V) ||
       ((k_token_stride | k_head_stride | v_token_stride | v_head_stride) & 7))
     return FA_ERR_ALIGNMENT;
-  if (static_cast<long long>(total) * c.heads > (1LL << 34)) return FA_ERR_TOO_LARGE;
+  // (rows are numbered with 32 bits, in tiles of 16 tokens)
+  if ((static_cast<long long>(total) + 15) * 2 * c.heads > 0xffff0000LL) return FA_ERR_TOO_LARGE;
   if (int rc = fa::host_check_device()) return rc;
   const fa::PagedSource s{static_cast<const uint8_t*>(K), static_cast<const uint8_t*>(V),
                           2 * k_token_stride, 2 * k_head_stride, 2 * v_token_stride,
@@ -223,7 +224,8 @@ int fa_kvcache_read(const fa_paged_cache* cache, void* K, void* V, const int* cu
   if (total == 0) return FA_OK;
   if (!K || !V) return FA_ERR_INVALID_ARG;
   if (!aligned16(K) || !aligned16(V)) return FA_ERR_ALIGNMENT;
-  if (static_cast<long long>(total) * c.heads > (1LL << 34)) return FA_ERR_TOO_LARGE;
+  // (rows are numbered with 32 bits, in tiles of 16 tokens)
+  if ((static_cast<long long>(total) + 15) * 2 * c.heads > 0xffff0000LL) return FA_ERR_TOO_LARGE;
   if (int rc = fa::host_check_device()) return rc;
   const cudaError_t e =
       fa::launch_cache_read(c, r, K, V, cache->head_dim, cache->dtype, dtype == FA_DTYPE_BF16,

@@ -8,12 +8,13 @@
 //   read   x = q * scale in fp32, rounded once to f16 / bf16.
 //
 // Both move every byte once and compute little: they are bound by HBM, or by
-// latency for a few tokens.  A row (d values of one token and head) is taken
-// by d / 8 lanes, 16 bytes each on the 16-bit side, so the row's maximum is 3
-// or 4 shuffles and both sides are coalesced.  A CTA takes `U` rows per lane
-// group; their places (sequence, position, page) are found once per token in
-// shared memory, in three dependent loads (cu_seqlens / seqlens, table) that
-// overlap the source rows' own loads when writing.
+// latency for a few tokens.  A row (d values of one token and head) is taken by
+// the lanes that cover it with 16-byte loads, so the row's maximum is 3 or 4
+// shuffles and both sides are coalesced.  Warps work alone: a warp takes U rows
+// per lane group, finds the places of the few tokens they belong to (sequence
+// by a 32-way search and ballots, page by one lookup per token: two dependent
+// loads for up to 32 sequences, which overlap the source rows' own loads when
+// writing) and keeps U independent 16-byte loads per lane in flight.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -22,20 +23,15 @@
 #include <cstdint>
 
 #include "fa_paged.h"
+#include "fa_paged_dev.cuh"
 
 namespace fa {
 namespace {
 
-constexpr int kCacheThreads = 256;
+constexpr int kCacheThreads = 128;
 constexpr float kTinyRow = 7.8886090522101181e-31f;  // 2^-100
 
 enum { kCopy = 0, kInt8 = 1, kE4m3 = 2 };
-
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
 
 template <bool BF16>
 __device__ __forceinline__ float2 unpack2(uint32_t u) {
@@ -43,6 +39,19 @@ __device__ __forceinline__ float2 unpack2(uint32_t u) {
     return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&u));
   } else {
     return __half22float2(*reinterpret_cast<__half2*>(&u));
+  }
+}
+
+// max(|a|, |b|) per half of two pairs; a NaN stays.  `b` is a magnitude already.
+template <bool BF16>
+__device__ __forceinline__ uint32_t absmax2(uint32_t a, uint32_t b) {
+  a &= 0x7fff7fffu;
+  if constexpr (BF16) {
+    const __nv_bfloat162 m = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+  } else {
+    const __half2 m = __hmax2_nan(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
   }
 }
 
@@ -57,125 +66,156 @@ __device__ __forceinline__ uint32_t pack2_rn(float a, float b) {
   }
 }
 
-// Places of the tokens a CTA handles: page (-1: none) and row in the page.
-struct Places {
-  static constexpr int kMax = 2 * kCacheThreads / 8 * 4 / 2 + 2;  // see rows_per_cta
-  int page[kMax];
-  int row[kMax];
+// Place of one token: byte offset of its row (of head 0) in the pages, -1 if
+// it has none, and offset of its scale.
+struct Place {
+  long long row, scale;
 };
+__device__ __forceinline__ long long shfl64(long long x, int src) {
+  const int lo = __shfl_sync(0xffffffffu, static_cast<int>(x), src);
+  const int hi = __shfl_sync(0xffffffffu, static_cast<int>(x >> 32), src);
+  return (static_cast<long long>(hi) << 32) | static_cast<unsigned>(lo);
+}
 
-// Fills pl for packed rows [t0, t0 + n): every thread checks its share of the
-// sequences for tokens of that range, then one thread per token looks up its
-// page.  Ends with a barrier.
-__device__ __forceinline__ void find_places(const PagedCache& c, const PagedRows& r, int t0, int n,
-                                            Places& pl) {
-  for (int i = threadIdx.x; i < n; i += kCacheThreads) pl.page[i] = -1;
-  __syncthreads();
-  for (int b = threadIdx.x; b < r.B; b += kCacheThreads) {
-    const int c0 = max(__ldg(r.cu + b), 0);
-    const int c1 = min(__ldg(r.cu + b + 1), r.total);
-    const int last = __ldg(r.lens + b) - c1;  // position of row t is last + t
-    const int hi = min(c1, t0 + n);
-    for (int t = max(c0, t0); t < hi; ++t) {
-      pl.page[t - t0] = b;
-      pl.row[t - t0] = last + t;
+// Places of packed rows t0 .. t0 + n - 1 (n <= 32): lane i gets that of row
+// t0 + i.  The whole warp calls it.
+__device__ __forceinline__ Place find_places(const PagedCache& c, const PagedRows& r, int t0, int n) {
+  const int lane = threadIdx.x & 31;
+  // a sequence that starts at or before t0, by 32-way steps
+  int b0 = 0;
+  for (int len = r.B; len > 32;) {
+    const int step = (len + 31) / 32;
+    const int probe = b0 + lane * step;
+    const bool le = lane * step < len && __ldg(r.cu + probe) <= t0;
+    const int cnt = __popc(__ballot_sync(0xffffffffu, le));
+    const int skip = max(cnt - 1, 0) * step;
+    b0 += skip;
+    len = min(step, len - skip);
+  }
+  int b = -1, pos = -1;  // of token t0 + lane
+  const int t = t0 + lane;
+  for (; b0 < r.B; b0 += 32) {
+    int c0 = 0x7fffffff, c1 = 0, last = 0;
+    if (b0 + lane < r.B) {
+      c0 = max(__ldg(r.cu + b0 + lane), 0);
+      c1 = min(__ldg(r.cu + b0 + lane + 1), r.total);
+      last = __ldg(r.lens + b0 + lane) - c1;  // position of row t is last + t
     }
+    // the sequences that have some of the rows (one or two, mostly)
+    for (unsigned left = __ballot_sync(0xffffffffu, c0 < t0 + n && c1 > t0 && c0 < c1); left != 0u;
+         left &= left - 1u) {
+      const int src = __ffs(left) - 1;
+      const int s0 = __shfl_sync(0xffffffffu, c0, src), s1 = __shfl_sync(0xffffffffu, c1, src);
+      const int l = __shfl_sync(0xffffffffu, last, src);
+      if (t >= s0 && t < s1 && lane < n) {
+        b = b0 + src;
+        pos = l + t;
+      }
+    }
+    if (__shfl_sync(0xffffffffu, c1, 31) >= t0 + n) break;  // (0 past the last sequence)
   }
-  __syncthreads();
-  for (int i = threadIdx.x; i < n; i += kCacheThreads) {
-    const int b = pl.page[i], pos = pl.row[i];
-    const int page = (b >= 0 && pos >= 0) ? c.lookup(b, pos) : -1;
-    pl.page[i] = page;
-    pl.row[i] = page >= 0 ? c.row_in_page(pos) : 0;
-  }
-  __syncthreads();
+  const int page = b >= 0 && pos >= 0 ? c.lookup(b, pos) : -1;
+  if (page < 0) return {-1, 0};
+  const long long row = c.row_in_page(pos);
+  return {page * c.page_stride + row * c.row_stride, page * c.s_page + row * c.s_row};
 }
 
-template <int D, int U>
-__host__ __device__ constexpr int rows_per_cta() {
-  return kCacheThreads / (D / 8) * U;
-}
-
-// Row number -> token (relative to t0), K or V, head: rows go token by token,
-// the K heads of a token before its V heads.
-struct RowId {
-  int token, kv, head;
+// Rows go token by token, the K heads of a token before its V heads.  A warp's
+// first row has token t0 (and is `skip` rows into it); `magic` = 2^32 / (2
+// heads) rounded up divides the small row numbers within a warp.
+struct RowMap {
+  unsigned n_rows;  // total * 2 * heads
+  unsigned magic;
 };
-__device__ __forceinline__ RowId row_id(long long row, int heads) {
-  const long long t = row / (2 * heads);
-  const int rem = static_cast<int>(row - t * (2 * heads));
-  return {static_cast<int>(t), rem >= heads ? 1 : 0, rem >= heads ? rem - heads : rem};
+struct RowId {
+  int token, kv, head;  // token: relative to t0
+};
+__device__ __forceinline__ RowId row_id(unsigned rel, int heads, unsigned magic) {
+  const int t = static_cast<int>(__umulhi(rel, magic));
+  const int rem = static_cast<int>(rel) - t * 2 * heads;
+  return {t, rem >= heads ? 1 : 0, rem >= heads ? rem - heads : rem};
 }
 
+// A lane holds 8 (copies) or 16 (8-bit) values of a row: those at 8 * part and,
+// for 8-bit pages, at d / 2 + 8 * part, so that every load and store of a lane
+// group is one contiguous run on both sides.
 template <int D, bool BF16, int KIND, int U>
 __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(const PagedCache c,
                                                                    const PagedRows r,
-                                                                   const PagedSource s) {
-  constexpr int L = D / 8;  // lanes per row
-  constexpr int kRows = kCacheThreads / L;
-  __shared__ Places pl;
-  const long long n_rows = static_cast<long long>(r.total) * 2 * c.heads;
-  const long long row0 = static_cast<long long>(blockIdx.x) * (kRows * U);
-  const int part = threadIdx.x % L;
+                                                                   const PagedSource s,
+                                                                   const RowMap map) {
+  constexpr int kPer = KIND == kCopy ? 1 : 2;  // 16-byte loads of a lane
+  constexpr int L = D / (8 * kPer);            // lanes per row
+  constexpr int kRows = 32 / L;
+  const int lane = threadIdx.x & 31, part = lane % L;
+  const unsigned row0 = (blockIdx.x * (kCacheThreads / 32) + (threadIdx.x >> 5)) * (kRows * U);
+  if (row0 >= map.n_rows) return;
+  const unsigned heads2 = 2u * c.heads;
+  const int t0 = static_cast<int>(row0 / heads2);
+  const unsigned skip = row0 - t0 * heads2;
+  const int n_tokens = row_id(skip + min(kRows * U, map.n_rows - row0) - 1u, c.heads, map.magic).token + 1;
   RowId id[U];
-  uint4 x[U];
+  uint4 x[U][kPer];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const long long row = row0 + u * kRows + threadIdx.x / L;
-    id[u].token = -1;
-    x[u] = make_uint4(0u, 0u, 0u, 0u);
-    if (row < n_rows) {
-      id[u] = row_id(row, c.heads);
-      const uint8_t* src =
-          id[u].kv ? s.v + id[u].token * s.v_token + id[u].head * s.v_head
-                   : s.k + id[u].token * s.k_token + id[u].head * s.k_head;
-      x[u] = __ldcs(reinterpret_cast<const uint4*>(src) + part);
+    id[u] = row_id(skip + u * kRows + lane / L, c.heads, map.magic);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) x[u][i] = make_uint4(0u, 0u, 0u, 0u);
+    if (row0 + u * kRows + lane / L < map.n_rows) {
+      const long long t = static_cast<long long>(t0) + id[u].token;
+      const uint8_t* src = id[u].kv ? s.v + t * s.v_token + id[u].head * s.v_head
+                                    : s.k + t * s.k_token + id[u].head * s.k_head;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        x[u][i] = __ldcs(reinterpret_cast<const uint4*>(src) + i * (D / 16) + part);
     }
   }
-  const int t0 = row_id(row0, c.heads).token;
-  const long long last = min(row0 + kRows * U, n_rows) - 1;
-  find_places(c, r, t0, row_id(last, c.heads).token - t0 + 1, pl);
+  const Place pl = find_places(c, r, t0, n_tokens);
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int page = id[u].token >= 0 ? pl.page[id[u].token - t0] : -1;
-    const int prow = id[u].token >= 0 ? pl.row[id[u].token - t0] : 0;
-    uint8_t* dst = const_cast<uint8_t*>(id[u].kv ? c.v : c.k) + page * c.page_stride +
-                   id[u].head * c.head_stride + prow * c.row_stride;
+    const long long found = shfl64(pl.row, id[u].token);
+    const bool ok = found >= 0 && row0 + u * kRows + lane / L < map.n_rows;
+    uint8_t* dst = const_cast<uint8_t*>(id[u].kv ? c.v : c.k) + found + id[u].head * c.head_stride;
     if constexpr (KIND == kCopy) {
-      if (page >= 0) reinterpret_cast<uint4*>(dst)[part] = x[u];
+      if (ok) reinterpret_cast<uint4*>(dst)[part] = x[u][0];
     } else {
-      float2 v[4] = {unpack2<BF16>(x[u].x), unpack2<BF16>(x[u].y), unpack2<BF16>(x[u].z),
-                     unpack2<BF16>(x[u].w)};
-      float a = 0.f;
+      const uint32_t in8[8] = {x[u][0].x, x[u][0].y, x[u][0].z, x[u][0].w,
+                               x[u][1].x, x[u][1].y, x[u][1].z, x[u][1].w};
+      uint32_t m = 0u;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) a = max_nan(a, max_nan(fabsf(v[i].x), fabsf(v[i].y)));
+      for (int i = 0; i < 8; ++i) m = absmax2<BF16>(in8[i], m);
 #pragma unroll
-      for (int o = L / 2; o > 0; o >>= 1) a = max_nan(a, __shfl_xor_sync(0xffffffffu, a, o));
+      for (int o = L / 2; o > 0; o >>= 1) m = absmax2<BF16>(__shfl_xor_sync(0xffffffffu, m, o), m);
+      const float2 m2 = unpack2<BF16>(m);
+      const float a = m2.x != m2.x ? m2.x : (m2.y > m2.x || m2.y != m2.y ? m2.y : m2.x);
       constexpr float kQmax = KIND == kInt8 ? 127.f : 448.f;
       const bool zero = a < kTinyRow;
       const float inv = zero ? 0.f : __fdiv_rn(kQmax, a);
-      const float scale = zero ? 0.f : __fdiv_rn(a, kQmax);
-      uint32_t w[2];
+      uint32_t w[4];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const float y0 = __fmul_rn(v[2 * i].x, inv), y1 = __fmul_rn(v[2 * i].y, inv);
-        const float y2 = __fmul_rn(v[2 * i + 1].x, inv), y3 = __fmul_rn(v[2 * i + 1].y, inv);
+      for (int i = 0; i < 4; ++i) {
+        const float2 y0 = unpack2<BF16>(in8[2 * i]), y1 = unpack2<BF16>(in8[2 * i + 1]);
+        const float f0 = __fmul_rn(y0.x, inv), f1 = __fmul_rn(y0.y, inv);
+        const float f2 = __fmul_rn(y1.x, inv), f3 = __fmul_rn(y1.y, inv);
         if constexpr (KIND == kInt8) {
-          auto q8 = [](float y) {
-            return static_cast<uint32_t>(min(max(__float2int_rn(y), -127), 127)) & 0xffu;
-          };
-          w[i] = q8(y0) | (q8(y1) << 8) | (q8(y2) << 16) | (q8(y3) << 24);
+          // 1.5 * 2^23 + y rounds y to an integer (ties to even) in the low
+          // mantissa bits; |y| <= 127 (1 + 2^-23), so the low byte is the value
+          auto q8 = [](float y) { return __float_as_uint(__fadd_rn(y, 12582912.f)); };
+          w[i] = __byte_perm(__byte_perm(q8(f0), q8(f1), 0x0040), __byte_perm(q8(f2), q8(f3), 0x0040), 0x5410);
         } else {
-          const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y0, y1), __NV_SATFINITE, __NV_E4M3);
-          const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y2, y3), __NV_SATFINITE, __NV_E4M3);
+          const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f0, f1), __NV_SATFINITE, __NV_E4M3);
+          const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(f2, f3), __NV_SATFINITE, __NV_E4M3);
           w[i] = lo | (hi << 16);
         }
       }
-      if (page >= 0) {
+      const long long so = shfl64(pl.scale, id[u].token);
+      if (ok) {
         reinterpret_cast<uint2*>(dst)[part] = make_uint2(w[0], w[1]);
+        reinterpret_cast<uint2*>(dst)[D / 16 + part] = make_uint2(w[2], w[3]);
+        // (an infinite or NaN maximum makes the scale NaN)
         if (part == 0)
-          (id[u].kv ? c.vs : c.ks)[page * c.s_page + id[u].head * c.s_head + prow * c.s_row] =
-              scale;
+          (id[u].kv ? c.vs : c.ks)[so + id[u].head * c.s_head] =
+              zero ? 0.f : __fdiv_rn(a, kQmax) + (a - a);
       }
     }
   }
@@ -185,106 +225,113 @@ template <int D, bool BF16, int KIND, int U>
 __global__ void __launch_bounds__(kCacheThreads) cache_read_kernel(const PagedCache c,
                                                                   const PagedRows r,
                                                                   uint4* __restrict__ k,
-                                                                  uint4* __restrict__ v) {
-  constexpr int L = D / 8;
-  constexpr int kRows = kCacheThreads / L;
-  __shared__ Places pl;
-  const long long n_rows = static_cast<long long>(r.total) * 2 * c.heads;
-  const long long row0 = static_cast<long long>(blockIdx.x) * (kRows * U);
-  const int part = threadIdx.x % L;
-  const int t0 = row_id(row0, c.heads).token;
-  const long long last = min(row0 + kRows * U, n_rows) - 1;
-  find_places(c, r, t0, row_id(last, c.heads).token - t0 + 1, pl);
+                                                                  uint4* __restrict__ v,
+                                                                  const RowMap map) {
+  constexpr int kPer = KIND == kCopy ? 1 : 2;  // 16-byte results of a lane
+  constexpr int L = D / (8 * kPer);            // lanes per row
+  constexpr int kRows = 32 / L;
+  const int lane = threadIdx.x & 31, part = lane % L;
+  const unsigned row0 = (blockIdx.x * (kCacheThreads / 32) + (threadIdx.x >> 5)) * (kRows * U);
+  if (row0 >= map.n_rows) return;
+  const unsigned heads2 = 2u * c.heads;
+  const int t0 = static_cast<int>(row0 / heads2);
+  const unsigned skip = row0 - t0 * heads2;
+  const int n_tokens = row_id(skip + min(kRows * U, map.n_rows - row0) - 1u, c.heads, map.magic).token + 1;
+  const Place pl = find_places(c, r, t0, n_tokens);
+  RowId id[U];
   uint4 x[U];
   float scale[U];
-  RowId id[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const long long row = row0 + u * kRows + threadIdx.x / L;
-    id[u].token = -1;
+    id[u] = row_id(skip + u * kRows + lane / L, c.heads, map.magic);
+    const long long found = shfl64(pl.row, id[u].token);
+    const long long so = KIND != kCopy ? shfl64(pl.scale, id[u].token) : 0;
     x[u] = make_uint4(0u, 0u, 0u, 0u);
     scale[u] = 0.f;
-    if (row < n_rows) {
-      id[u] = row_id(row, c.heads);
-      const int page = pl.page[id[u].token - t0], prow = pl.row[id[u].token - t0];
-      if (page >= 0) {
-        const uint8_t* src = (id[u].kv ? c.v : c.k) + page * c.page_stride +
-                             id[u].head * c.head_stride + prow * c.row_stride;
-        if constexpr (KIND == kCopy) {
-          x[u] = __ldg(reinterpret_cast<const uint4*>(src) + part);
-        } else {
-          const uint2 t = __ldg(reinterpret_cast<const uint2*>(src) + part);
-          x[u].x = t.x;
-          x[u].y = t.y;
-          scale[u] = __ldg((id[u].kv ? c.vs : c.ks) + page * c.s_page + id[u].head * c.s_head +
-                           prow * c.s_row);
-        }
+    if (found >= 0 && row0 + u * kRows + lane / L < map.n_rows) {
+      const uint8_t* src = (id[u].kv ? c.v : c.k) + found + id[u].head * c.head_stride;
+      if constexpr (KIND == kCopy) {
+        x[u] = __ldcs(reinterpret_cast<const uint4*>(src) + part);
+      } else {
+        const uint2 lo = __ldcs(reinterpret_cast<const uint2*>(src) + part);
+        const uint2 hi = __ldcs(reinterpret_cast<const uint2*>(src) + D / 16 + part);
+        x[u] = make_uint4(lo.x, lo.y, hi.x, hi.y);
       }
+      if constexpr (KIND != kCopy) scale[u] = __ldg((id[u].kv ? c.vs : c.ks) + so + id[u].head * c.s_head);
     }
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    if (id[u].token < 0) continue;
-    if constexpr (KIND != kCopy) {
-      uint32_t w[4];
-      const uint32_t in[2] = {x[u].x, x[u].y};
+    if (row0 + u * kRows + lane / L >= map.n_rows) continue;
+    uint4* dst = (id[u].kv ? v : k) +
+                 ((static_cast<long long>(t0) + id[u].token) * c.heads + id[u].head) * (D / 8) + part;
+    if constexpr (KIND == kCopy) {
+      __stcs(dst, x[u]);
+    } else {
+      const uint32_t in[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+      uint32_t w[8];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint32_t two = in[i / 2] >> (16 * (i & 1));
-        float y0, y1;
-        if constexpr (KIND == kInt8) {
-          y0 = static_cast<float>(static_cast<int8_t>(two & 0xffu));
-          y1 = static_cast<float>(static_cast<int8_t>((two >> 8) & 0xffu));
-        } else {
-          const __half2_raw h =
-              __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two & 0xffffu), __NV_E4M3);
-          const float2 f = __half22float2(__half2(h));
-          y0 = f.x;
-          y1 = f.y;
+        uint32_t p[2];  // the values as f16, exactly
+        widen<KIND == kInt8 ? FA_DTYPE_INT8 : FA_DTYPE_E4M3, false>(in[i], p[0], p[1]);
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const float2 f = unpack2<false>(p[y]);
+          w[2 * i + y] = pack2_rn<BF16>(__fmul_rn(f.x, scale[u]), __fmul_rn(f.y, scale[u]));
         }
-        w[i] = pack2_rn<BF16>(__fmul_rn(y0, scale[u]), __fmul_rn(y1, scale[u]));
       }
-      x[u] = make_uint4(w[0], w[1], w[2], w[3]);
+      __stcs(dst, make_uint4(w[0], w[1], w[2], w[3]));
+      __stcs(dst + D / 16, make_uint4(w[4], w[5], w[6], w[7]));
     }
-    uint4* dst = (id[u].kv ? v : k) +
-                 (static_cast<long long>(id[u].token) * c.heads + id[u].head) * (D / 8) + part;
-    __stcs(dst, x[u]);
   }
 }
 
-// U rows per lane group: 4 keep 4 independent loads in flight per thread; few
-// rows spread over more CTAs instead.
-bool few_rows(long long n_rows, int head_dim) {
-  return n_rows <= 2LL * 148 * (kCacheThreads / (head_dim / 8));
+// U rows per lane group, each an independent load per lane: 4 for copies, 2 for
+// 8-bit pages, whose rows take more registers and instructions; few rows spread
+// over more warps instead.  Measured on B200 (GPU time; 128 threads, U = 1 / 2 /
+// 4): 195 MB of f16 rows read back 44 / 36 / 33 us, 217 MB of int8 45 / 39 / 44;
+// 256 threads +2 %, 512 +7-15 %.
+template <int KIND>
+constexpr int kRowsInFlight = KIND == kCopy ? 4 : 2;
+template <int kRowsPerU>
+unsigned blocks_for(unsigned n_rows, int u) {
+  const unsigned per = kCacheThreads / 32 * kRowsPerU * u;
+  return (n_rows + per - 1) / per;
 }
+RowMap row_map(const PagedCache& c, const PagedRows& r) {
+  const unsigned heads2 = 2u * c.heads;
+  return {static_cast<unsigned>(r.total) * heads2,
+          static_cast<unsigned>(((1ull << 32) + heads2 - 1) / heads2)};
+}
+bool few_rows(unsigned n_rows) { return n_rows <= 148u * 64u; }
 
 template <int D, bool BF16, int KIND>
 cudaError_t write_impl(const PagedCache& c, const PagedRows& r, const PagedSource& s,
                        cudaStream_t stream) {
-  const long long n_rows = static_cast<long long>(r.total) * 2 * c.heads;
-  if (few_rows(n_rows, D)) {
-    const unsigned grid = static_cast<unsigned>((n_rows + rows_per_cta<D, 1>() - 1) / rows_per_cta<D, 1>());
-    cache_write_kernel<D, BF16, KIND, 1><<<grid, kCacheThreads, 0, stream>>>(c, r, s);
-  } else {
-    const unsigned grid = static_cast<unsigned>((n_rows + rows_per_cta<D, 4>() - 1) / rows_per_cta<D, 4>());
-    cache_write_kernel<D, BF16, KIND, 4><<<grid, kCacheThreads, 0, stream>>>(c, r, s);
-  }
+  const RowMap m = row_map(c, r);
+  constexpr int kRows = (KIND == kCopy ? 256 : 512) / D;
+  if (few_rows(m.n_rows))
+    cache_write_kernel<D, BF16, KIND, 1>
+        <<<blocks_for<kRows>(m.n_rows, 1), kCacheThreads, 0, stream>>>(c, r, s, m);
+  else
+    cache_write_kernel<D, BF16, KIND, kRowsInFlight<KIND>>
+        <<<blocks_for<kRows>(m.n_rows, kRowsInFlight<KIND>), kCacheThreads, 0, stream>>>(c, r, s, m);
   return cudaGetLastError();
 }
 
 template <int D, bool BF16, int KIND>
 cudaError_t read_impl(const PagedCache& c, const PagedRows& r, void* k, void* v,
                       cudaStream_t stream) {
-  const long long n_rows = static_cast<long long>(r.total) * 2 * c.heads;
+  const RowMap m = row_map(c, r);
+  constexpr int kRows = (KIND == kCopy ? 256 : 512) / D;
   uint4* k4 = static_cast<uint4*>(k);
   uint4* v4 = static_cast<uint4*>(v);
-  if (few_rows(n_rows, D)) {
-    const unsigned grid = static_cast<unsigned>((n_rows + rows_per_cta<D, 1>() - 1) / rows_per_cta<D, 1>());
-    cache_read_kernel<D, BF16, KIND, 1><<<grid, kCacheThreads, 0, stream>>>(c, r, k4, v4);
-  } else {
-    const unsigned grid = static_cast<unsigned>((n_rows + rows_per_cta<D, 4>() - 1) / rows_per_cta<D, 4>());
-    cache_read_kernel<D, BF16, KIND, 4><<<grid, kCacheThreads, 0, stream>>>(c, r, k4, v4);
-  }
+  if (few_rows(m.n_rows))
+    cache_read_kernel<D, BF16, KIND, 1>
+        <<<blocks_for<kRows>(m.n_rows, 1), kCacheThreads, 0, stream>>>(c, r, k4, v4, m);
+  else
+    cache_read_kernel<D, BF16, KIND, kRowsInFlight<KIND>>
+        <<<blocks_for<kRows>(m.n_rows, kRowsInFlight<KIND>), kCacheThreads, 0, stream>>>(c, r, k4, v4, m);
   return cudaGetLastError();
 }
 

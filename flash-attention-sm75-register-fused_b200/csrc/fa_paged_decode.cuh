@@ -124,15 +124,21 @@ __device__ __forceinline__ Seq load_short(const PagedAttn& a, int b, int max_row
   return s;
 }
 
-// Units of one head: in the sequences before b, and in the whole batch (a
+// The runs are cut from positions, not units: a segment (sequence, head) of n
+// units has kSegCost positions before its units' n, for what a team spends on a
+// segment besides its units (queries, results).  Without them the teams that
+// get many short sequences finish last.
+constexpr int kSegCost = 1;
+__device__ __forceinline__ int positions_of(const PagedAttn& a, int b, int sub, int max_rows) {
+  const int n = (load_short(a, b, max_rows).vis + sub - 1) / sub;
+  return n > 0 ? n + kSegCost : 0;
+}
+
+// Positions of one head: in the sequences before b, and in the whole batch (a
 // block-wide pass over the lengths).
 struct Spot {
   long long before, total;
 };
-
-__device__ __forceinline__ int units_of(const PagedAttn& a, int b, int sub, int max_rows) {
-  return (load_short(a, b, max_rows).vis + sub - 1) / sub;
-}
 
 template <int kThreads>
 __device__ Spot find_spot(const PagedAttn& a, int sub, int max_rows, int b, long long* sh) {
@@ -140,11 +146,11 @@ __device__ Spot find_spot(const PagedAttn& a, int sub, int max_rows, int b, long
   const int share = (a.r.B + kThreads - 1) / kThreads;
   const int b0 = min(static_cast<int>(threadIdx.x) * share, a.r.B), b1 = min(b0 + share, a.r.B);
   long long sum = 0;
-  for (int i = b0; i < b1; ++i) sum += units_of(a, i, sub, max_rows);
+  for (int i = b0; i < b1; ++i) sum += positions_of(a, i, sub, max_rows);
   Spot sp;
   long long x = block_scan<kThreads>(sum, sh, &sp.total);
   if (b >= b0 && b < b1) {
-    for (int i = b0; i < b; ++i) x += units_of(a, i, sub, max_rows);
+    for (int i = b0; i < b; ++i) x += positions_of(a, i, sub, max_rows);
     sh[kThreads / 32] = x;
   }
   __syncthreads();
@@ -157,10 +163,11 @@ __host__ __device__ constexpr long long slot_floats(int rows, int d) {
   return static_cast<long long>(rows) * (d + 2);
 }
 
-// Position of a team in its run: unit t of n of (sequence b, head h).
+// Place of a team in its run: unit t of n of (sequence b, head h), position v.
 struct Cursor {
   Seq s;
   int b, h, t, n;
+  long long v;
 };
 
 template <int D, int KV, bool QBF16, int NT, int TEAM>
@@ -184,7 +191,7 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
   volatile int* abort_flag = &sh_abort;
   ptx::launch_dependents();
 
-  // ---- set-up, and the team's run [u0, u1) of the batch's units
+  // ---- set-up, and the team's run [v0, v1) of the batch's positions
   if (threadIdx.x == 0) {
     const unsigned long long st = *reinterpret_cast<volatile unsigned long long*>(&g_fa_status);
     sh_abort = ((st >> 32) == p.epoch && (st & 0xffffffffull) != 0ull) ? 1 : 0;
@@ -194,27 +201,27 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
       ptx::mbar_init(ptx::smem_u32(&sh_bar[i]), C::k8 ? 33u : 1u);
     ptx::fence_barrier_init();
   }
-  long long u0, u1, rel;
+  long long v1, rel;
   int b_first;
   {
     const int share = (a.r.B + 32 * kWarps - 1) / (32 * kWarps);
     const int s0 = min(static_cast<int>(threadIdx.x) * share, a.r.B), s1 = min(s0 + share, a.r.B);
     long long sum = 0, total;
-    for (int b = s0; b < s1; ++b) sum += units_of(a, b, C::kSub, p.max_rows);
+    for (int b = s0; b < s1; ++b) sum += positions_of(a, b, C::kSub, p.max_rows);
     const long long excl = block_scan<32 * kWarps>(sum, sh_scan, &total);
     total *= H;
     const long long per = (total + p.n_teams - 1) / p.n_teams;
     const long long lo = excl * H, hi = (excl + sum) * H;
-    // the thread whose share holds a team's first unit finds its sequence
+    // the thread whose share holds a team's first position finds its sequence
     for (int w = 0; w < kTeams; ++w) {
-      const long long u = per * (static_cast<long long>(blockIdx.x) * kTeams + w);
-      if (u < total && u >= lo && u < hi) {
+      const long long v = per * (static_cast<long long>(blockIdx.x) * kTeams + w);
+      if (v < total && v >= lo && v < hi) {
         long long x = lo;
         for (int b = s0; b < s1; ++b) {
-          const long long nb = static_cast<long long>(units_of(a, b, C::kSub, p.max_rows)) * H;
-          if (u < x + nb) {
+          const long long nb = static_cast<long long>(positions_of(a, b, C::kSub, p.max_rows)) * H;
+          if (v < x + nb) {
             sh_b[w] = b;
-            sh_rel[w] = u - x;
+            sh_rel[w] = v - x;
             break;
           }
           x += nb;
@@ -222,11 +229,12 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
       }
     }
     __syncthreads();
-    u0 = min(per * tid, total);
-    u1 = min(u0 + per, total);
-    if (u0 >= u1 || *abort_flag) return;
+    const long long v0 = min(per * tid, total);
+    v1 = min(v0 + per, total);
+    if (v0 >= v1 || *abort_flag) return;
     b_first = sh_b[team];
     rel = sh_rel[team];
+    v1 -= v0 - rel;  // relative to the first sequence's first position, like rel
   }
   const WaitCtl wc{abort_flag, p.timeout_ns, p.epoch};
   // all warps of the team; a warp that failed makes the team leave together
@@ -246,8 +254,11 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
       if (c.n > 0) break;
     }
   };
-  auto advance = [&](Cursor& c) {  // (not past the run's last unit)
+  auto advance = [&](Cursor& c) {  // to the next unit, if the run has one
+    ++c.v;
     if (++c.t < c.n) return;
+    c.v += kSegCost;
+    if (c.v >= v1) return;
     c.t = 0;
     if (++c.h < H) return;
     c.h = 0;
@@ -255,8 +266,13 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
   };
   Cursor cc;  // unit being computed
   seek(cc, b_first);
-  cc.h = static_cast<int>(rel / cc.n);
-  cc.t = static_cast<int>(rel % cc.n);
+  {
+    const long long seg = cc.n + kSegCost;
+    cc.h = static_cast<int>(rel / seg);
+    cc.t = max(static_cast<int>(rel % seg) - kSegCost, 0);
+    cc.v = cc.h * seg + kSegCost + cc.t;
+    if (cc.v >= v1) return;  // nothing but a segment's set-up
+  }
   Cursor ci = cc;  // unit being loaded (the team's first warp)
 
   // ---- loads
@@ -274,7 +290,6 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
   const bool boxes = lane < C::kBoxes;
   const uint32_t box_dst = (lane & 1) * 4096 + (C::kCols == 2 ? bcol * 2048 : bgrp * 16 * C::kRowBytes);
   const void* const box_map = (lane & 1) ? &p.tm_v : &p.tm_k;
-  long long iu = u0;  // unit of ci
   auto page_of_box = [&] {  // -1 (no key any row may see, or no page) reads as zeros
     const int pos = ci.t * C::kSub + 16 * bgrp;
     return boxes && pos < ci.s.vis ? a.c.lookup(ci.b, pos) : -1;
@@ -282,7 +297,7 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
   int page = -1;
   int wstage = 0;
   auto issue = [&] {
-    if (iu >= u1) return;
+    if (ci.v >= v1) return;
     const uint32_t bar = bars + 8 * wstage;
     const int key0 = ci.t * C::kSub;
     if (lane == 0) ptx::mbar_arrive_expect_tx(bar, 8192);
@@ -308,10 +323,8 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
       ptx::cp_async_arrive(bar);
     }
     if (++wstage == kStages) wstage = 0;
-    if (++iu < u1) {
-      advance(ci);
-      page = page_of_box();
-    }
+    advance(ci);
+    if (ci.v < v1) page = page_of_box();
   };
   if (trank == 0) {
     page = page_of_box();
@@ -326,11 +339,10 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
   int rstage = 0;
   uint32_t rphase = 0;
   bool ok = true;
-  long long u = u0;
-  while (ok && u < u1) {
+  while (ok && cc.v < v1) {
     const Seq s = cc.s;
     const int t_begin = cc.t, n_units = cc.n;
-    const int t_end = static_cast<int>(min(static_cast<long long>(n_units), t_begin + (u1 - u)));
+    const int t_end = static_cast<int>(min(static_cast<long long>(n_units), t_begin + (v1 - cc.v)));
     const int rows = s.nq * a.group;
     const int row0 = trank * 8 * NT;  // of this warp
     const bool active = row0 < rows;
@@ -661,11 +673,9 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
         }
       }
     // ---- next segment
-    u += t_end - t_begin;
-    if (u < u1) {
-      cc.t = t_end - 1;
-      advance(cc);
-    }
+    cc.v += t_end - t_begin - 1;
+    cc.t = t_end - 1;
+    advance(cc);
   }
   // after a failed wait: copies in flight land before the CTA exits
   if (!ok && trank == 0) {
@@ -681,19 +691,41 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
   }
 }
 
-// Joins the partial results of (sequence, KV head) blockIdx.x, query row
-// blockIdx.y: with M = max m_s over its slots in order of the teams,
-//   O = sum 2^(m_s - M) O_s / sum 2^(m_s - M) l_s.
+// Joins the partial results of (sequence, KV head) blockIdx.x, query rows
+// blockIdx.y * kRows ..: with M = max m_s over the segment's slots,
+//   O = sum 2^(m_s - M) O_s / sum 2^(m_s - M) l_s,
+// slots in the order of their teams (so the result does not depend on timing).
+// kRows = 8 (many rows to join, few slots each): one warp per row.  kRows = 1
+// (few rows, many slots), or a segment of more than kManySlots: the block's
+// warps share a row's slots and are joined at the end.
 // Also writes the rows that no team of the decode kernel computes: rows of
 // sequences without visible keys and packed rows of no sequence.
-template <int D, bool BF16>
+constexpr int kManySlots = 32;
+
+template <int D>
+struct Partial {
+  static constexpr int E = D / 32;  // columns of a lane
+  float m = kNoMax, l = 0.f, o[E] = {};
+  __device__ __forceinline__ void add(float mi, float li, const float (&v)[E]) {
+    const float mn = fmaxf(m, mi);
+    const float f0 = exp2f(m - mn), f1 = exp2f(mi - mn);
+    m = mn;
+    l = l * f0 + li * f1;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = o[e] * f0 + v[e] * f1;
+  }
+};
+
+template <int D, bool BF16, int kRows>
 __global__ void __launch_bounds__(kCombineThreads)
     paged_combine_kernel(const __grid_constant__ DecodeParams p, int sub, int slot_rows) {
+  constexpr int kW = kCombineThreads / 32;
+  constexpr int E = D / 32;
   const PagedAttn& a = p.a;
-  __shared__ long long sh[kCombineThreads / 32 + 1];
-  __shared__ float sh_o[kCombineThreads / 32][D];
-  __shared__ float sh_m[kCombineThreads / 32], sh_l[kCombineThreads / 32];
-  const int b = blockIdx.x / a.c.heads, h = blockIdx.x % a.c.heads, row = blockIdx.y;
+  __shared__ long long sh[kW + 1];
+  __shared__ float sh_o[kW][D];
+  __shared__ float sh_m[kW], sh_l[kW];
+  const int b = blockIdx.x / a.c.heads, h = blockIdx.x % a.c.heads;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint16_t* out = static_cast<uint16_t*>(a.o);
   // rows of no sequence: before the first and after the last
@@ -715,87 +747,90 @@ __global__ void __launch_bounds__(kCombineThreads)
   const Spot sp = find_spot<kCombineThreads>(a, sub, p.max_rows, b, sh);
   // the decode kernel's results are complete and visible after this
   ptx::grid_dep_wait();
-  if (row >= s.nq * a.group) return;
-  const int tok = s.c0 + row / a.group, hq = h * a.group + row % a.group;
-  uint16_t* dst = out + (static_cast<long long>(tok) * a.Hq + hq) * D;
+  const int row0 = blockIdx.y * kRows;
+  const int rows = min(s.nq * a.group - row0, kRows);  // of this block
+  if (rows <= 0) return;
   const int n = (s.vis + sub - 1) / sub;
-  if (n == 0) {
-    for (int i = threadIdx.x; i < D / 2; i += kCombineThreads) reinterpret_cast<uint32_t*>(dst)[i] = 0u;
-    if (threadIdx.x == 0 && a.lse != nullptr)
-      a.lse[static_cast<long long>(hq) * a.r.total + tok] = -INFINITY;
-    return;
-  }
   const long long total = sp.total * a.c.heads;
   const long long per = (total + p.n_teams - 1) / p.n_teams;
-  const long long t0 = sp.before * a.c.heads + static_cast<long long>(h) * n;
-  const int w0 = static_cast<int>(t0 / per), w1 = static_cast<int>((t0 + n - 1) / per);
+  const long long t0 = sp.before * a.c.heads + static_cast<long long>(h) * (n + kSegCost) + kSegCost;
+  const int w0 = n > 0 ? static_cast<int>(t0 / per) : 0;
+  const int w1 = n > 0 ? static_cast<int>((t0 + n - 1) / per) : -1;
   if (w0 == w1) return;  // one team had it all
   const long long stride = slot_floats(slot_rows, D);
-  auto slot_of = [&](int w) { return p.ws + (2ll * w + (w == w0 ? 1 : 0)) * stride; };
-  // each warp joins every 8th slot, the block joins the warps
-  constexpr int E = D / 32;
-  float mm = kNoMax, ll = 0.f, acc[E] = {};
-  constexpr int kBatch = 4;
-  for (int w = w0 + warp; w <= w1; w += kBatch * (kCombineThreads / 32)) {
-    float mi[kBatch], li[kBatch], v[kBatch][E];
+  // slots first, first + step, ... of row `row`
+  auto gather = [&](int row, int first, int step) {
+    Partial<D> acc;
+    constexpr int kBatch = 8;
+    for (int w = w0 + first; w <= w1; w += kBatch * step) {
+      float mi[kBatch], li[kBatch], v[kBatch][E];
 #pragma unroll
-    for (int x = 0; x < kBatch; ++x) {
-      const int ww = w + x * (kCombineThreads / 32);
-      mi[x] = kNoMax;
-      li[x] = 0.f;
+      for (int x = 0; x < kBatch; ++x) {
+        const int ww = w + x * step;
+        mi[x] = kNoMax;
+        li[x] = 0.f;
 #pragma unroll
-      for (int e = 0; e < E; ++e) v[x][e] = 0.f;
-      if (ww <= w1) {
-        const float* sl = slot_of(ww);
-        mi[x] = __ldcg(sl + slot_rows * D + row);
-        li[x] = __ldcg(sl + slot_rows * D + slot_rows + row);
-        if constexpr (E == 4) {
-          const float4 f = __ldcg(reinterpret_cast<const float4*>(sl + row * D) + lane);
-          v[x][0] = f.x;
-          v[x][1] = f.y;
-          v[x][2] = f.z;
-          v[x][3] = f.w;
-        } else {
-          const float2 f = __ldcg(reinterpret_cast<const float2*>(sl + row * D) + lane);
-          v[x][0] = f.x;
-          v[x][1] = f.y;
+        for (int e = 0; e < E; ++e) v[x][e] = 0.f;
+        if (ww <= w1) {
+          const float* sl = p.ws + (2ll * ww + (ww == w0 ? 1 : 0)) * stride;
+          mi[x] = __ldcg(sl + slot_rows * D + row);
+          li[x] = __ldcg(sl + slot_rows * D + slot_rows + row);
+          if constexpr (E == 4) {
+            const float4 f = __ldcg(reinterpret_cast<const float4*>(sl + row * D) + lane);
+            v[x][0] = f.x;
+            v[x][1] = f.y;
+            v[x][2] = f.z;
+            v[x][3] = f.w;
+          } else {
+            const float2 f = __ldcg(reinterpret_cast<const float2*>(sl + row * D) + lane);
+            v[x][0] = f.x;
+            v[x][1] = f.y;
+          }
         }
       }
+#pragma unroll
+      for (int x = 0; x < kBatch; ++x)
+        if (w + x * step <= w1) acc.add(mi[x], li[x], v[x]);
     }
+    return acc;
+  };
+  // one warp writes a row
+  auto finish = [&](int row, const Partial<D>& r) {
+    const int tok = s.c0 + row / a.group, hq = h * a.group + row % a.group;
+    const float inv = r.l == 0.f ? 0.f : 1.f / r.l;
+    uint32_t* dst =
+        reinterpret_cast<uint32_t*>(out + (static_cast<long long>(tok) * a.Hq + hq) * D) + lane * (E / 2);
 #pragma unroll
-    for (int x = 0; x < kBatch; ++x) {
-      const float mn = fmaxf(mm, mi[x]);
-      const float f0 = exp2f(mm - mn), f1 = exp2f(mi[x] - mn);
-      mm = mn;
-      ll = ll * f0 + li[x] * f1;
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = acc[e] * f0 + v[x][e] * f1;
-    }
-  }
-  if (lane == 0) {
-    sh_m[warp] = mm;
-    sh_l[warp] = ll;
-  }
-#pragma unroll
-  for (int e = 0; e < E; ++e) sh_o[warp][lane * E + e] = acc[e];
-  __syncthreads();
-  if (threadIdx.x < D / 2) {
-    float M = kNoMax;
-#pragma unroll
-    for (int w = 0; w < kCombineThreads / 32; ++w) M = fmaxf(M, sh_m[w]);
-    float L = 0.f, x0 = 0.f, x1 = 0.f;
-#pragma unroll
-    for (int w = 0; w < kCombineThreads / 32; ++w) {
-      const float f = exp2f(sh_m[w] - M);
-      L += f * sh_l[w];
-      x0 += f * sh_o[w][2 * threadIdx.x];
-      x1 += f * sh_o[w][2 * threadIdx.x + 1];
-    }
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    reinterpret_cast<uint32_t*>(dst)[threadIdx.x] = pack2<BF16>(x0 * inv, x1 * inv);
-    if (threadIdx.x == 0 && a.lse != nullptr)
+    for (int e = 0; e < E; e += 2) dst[e / 2] = pack2<BF16>(r.o[e] * inv, r.o[e + 1] * inv);
+    if (lane == 0 && a.lse != nullptr)
       a.lse[static_cast<long long>(hq) * a.r.total + tok] =
-          L == 0.f ? -INFINITY : (M + log2f(L)) * 0.69314718055994530942f;
+          r.l == 0.f ? -INFINITY : (r.m + log2f(r.l)) * 0.69314718055994530942f;
+  };
+  if (kRows > 1 && w1 - w0 < kManySlots) {
+    for (int r = warp; r < rows; r += kW) finish(row0 + r, gather(row0 + r, 0, 1));
+    return;
+  }
+  for (int r = 0; r < rows; ++r) {
+    const Partial<D> mine = gather(row0 + r, warp, kW);
+    if (lane == 0) {
+      sh_m[warp] = mine.m;
+      sh_l[warp] = mine.l;
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) sh_o[warp][lane * E + e] = mine.o[e];
+    __syncthreads();
+    if (warp == 0) {
+      Partial<D> all;
+#pragma unroll
+      for (int w = 0; w < kW; ++w) {
+        float v[E];
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = sh_o[w][lane * E + e];
+        all.add(sh_m[w], sh_l[w], v);
+      }
+      finish(row0 + r, all);
+    }
+    __syncthreads();
   }
 }
 
@@ -818,7 +853,9 @@ cudaError_t launch_impl(const DecodeParams& p, int n_ctas, cudaStream_t stream) 
   // the combine may start while the last teams finish; it waits for them
   // before it reads a slot
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.a.r.B) * p.a.c.heads, p.max_rows);
+  const unsigned segments = static_cast<unsigned>(p.a.r.B) * p.a.c.heads;
+  const bool many = static_cast<long long>(segments) * p.max_rows > 4 * 148;
+  cfg.gridDim = dim3(segments, many ? (p.max_rows + 7) / 8 : p.max_rows);
   cfg.blockDim = dim3(kCombineThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -826,8 +863,8 @@ cudaError_t launch_impl(const DecodeParams& p, int n_ctas, cudaStream_t stream) 
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_combine_kernel<D, QBF16>, p, static_cast<int>(C::kSub),
-                            8 * NT * TEAM);
+  return cudaLaunchKernelEx(&cfg, many ? paged_combine_kernel<D, QBF16, 8> : paged_combine_kernel<D, QBF16, 1>,
+                            p, static_cast<int>(C::kSub), 8 * NT * TEAM);
 }
 
 // Rows of a team and how it is made up: one warp for 8 or 16 rows, two or four

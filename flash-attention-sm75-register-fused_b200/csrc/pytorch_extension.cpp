@@ -12,6 +12,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <cmath>
+
 #include "fa_b200.h"
 
 namespace {
@@ -470,7 +472,8 @@ fa_paged_cache paged_cache(const torch::Tensor& k, const torch::Tensor& v,
                            torch::ScalarType dtype) {
   TORCH_CHECK(k.is_cuda() && k.device() == device && v.device() == device,
               "k_cache and v_cache must be on the inputs' CUDA device");
-  TORCH_CHECK(k.dim() == 4, "k_cache must be [num_pages, Hkv, page_size, D]");
+  TORCH_CHECK_VALUE(k.dim() == 4 && v.dim() == 4,
+                    "k_cache and v_cache must be 4D [num_pages, H_kv, page_size, D]");
   TORCH_CHECK(k.sizes() == v.sizes() && k.scalar_type() == v.scalar_type(),
               "k_cache and v_cache must share shape and dtype");
   TORCH_CHECK(k.size(3) == 64 || k.size(3) == 128,
@@ -532,6 +535,13 @@ fa_paged_cache paged_cache(const torch::Tensor& k, const torch::Tensor& v,
   return c;
 }
 
+// int32 tensor with contiguous rows on `device`: x itself where it is one.
+torch::Tensor as_ints(const torch::Tensor& x, const torch::Device& device) {
+  const bool rows = x.dim() == 0 || x.size(-1) <= 1 || x.stride(-1) == 1;
+  if (x.scalar_type() == torch::kInt32 && x.device() == device && rows) return x;
+  return x.to(torch::TensorOptions().dtype(torch::kInt32).device(device)).contiguous();
+}
+
 // Number of sequences; checks cu_seqlens [B + 1] and seqlens_k [B] against the table.
 int paged_batch(const torch::Tensor& cu, const torch::Tensor& lens, const torch::Tensor& table,
                 const torch::Device& device) {
@@ -548,10 +558,10 @@ int paged_batch(const torch::Tensor& cu, const torch::Tensor& lens, const torch:
 
 // New rows [total, H, D], f16 / bf16, any token and head strides of 16 bytes.
 void check_new_rows(const torch::Tensor& t, const char* name) {
-  TORCH_CHECK(t.is_cuda(), std::string(name) + " must be a CUDA tensor");
-  TORCH_CHECK(t.scalar_type() == torch::kFloat16 || t.scalar_type() == torch::kBFloat16,
-              std::string(name) + " must be FP16 or BF16");
-  TORCH_CHECK(t.dim() == 3, std::string(name) + " must be [total, H, D]");
+  TORCH_CHECK_VALUE(t.dim() == 3, name, " must be 3D [total, H, D]");
+  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
+  TORCH_CHECK(t.scalar_type() == torch::kFloat16 || t.scalar_type() == torch::kBFloat16, name,
+              " must be FP16 or BF16");
   TORCH_CHECK(t.size(0) <= INT32_MAX && t.size(1) <= INT32_MAX, "size exceeds int32");
 }
 
@@ -566,11 +576,13 @@ torch::Tensor readable_rows(const torch::Tensor& t) {
 
 void kvcache_write_paged(const torch::Tensor& k_in, const torch::Tensor& v_in,
                          const torch::Tensor& k_cache, const torch::Tensor& v_cache,
-                         const torch::Tensor& table, const torch::Tensor& cu,
-                         const torch::Tensor& lens, const c10::optional<torch::Tensor>& ks,
+                         const torch::Tensor& table_in, const torch::Tensor& cu_in,
+                         const torch::Tensor& lens_in, const c10::optional<torch::Tensor>& ks,
                          const c10::optional<torch::Tensor>& vs) {
   check_new_rows(k_in, "k");
   check_new_rows(v_in, "v");
+  const auto table = as_ints(table_in, k_in.device());
+  const auto cu = as_ints(cu_in, k_in.device()), lens = as_ints(lens_in, k_in.device());
   TORCH_CHECK(k_in.sizes() == v_in.sizes() && k_in.scalar_type() == v_in.scalar_type() &&
                   k_in.device() == v_in.device(),
               "k and v must share shape, dtype and device");
@@ -589,9 +601,11 @@ void kvcache_write_paged(const torch::Tensor& k_in, const torch::Tensor& v_in,
 }
 
 std::tuple<torch::Tensor, torch::Tensor> kvcache_read_paged(
-    const torch::Tensor& k_cache, const torch::Tensor& v_cache, const torch::Tensor& table,
-    const torch::Tensor& cu, const torch::Tensor& lens, int64_t total,
+    const torch::Tensor& k_cache, const torch::Tensor& v_cache, const torch::Tensor& table_in,
+    const torch::Tensor& cu_in, const torch::Tensor& lens_in, int64_t total,
     const c10::optional<torch::Tensor>& ks, const c10::optional<torch::Tensor>& vs, bool bf16) {
+  const auto table = as_ints(table_in, k_cache.device());
+  const auto cu = as_ints(cu_in, k_cache.device()), lens = as_ints(lens_in, k_cache.device());
   const auto dtype = bf16 ? torch::kBFloat16 : torch::kFloat16;
   const auto c = paged_cache(k_cache, v_cache, table, ks, vs, k_cache.device(), dtype);
   TORCH_CHECK(total >= 0 && total <= INT32_MAX, "total must be a count of rows, got ", total);
@@ -612,10 +626,14 @@ std::tuple<torch::Tensor, torch::Tensor> kvcache_read_paged(
 // O [total_q, Hq, d] and, if asked for, LSE fp32 [Hq, total_q].
 std::tuple<torch::Tensor, c10::optional<torch::Tensor>> flash_attention_forward_paged(
     const torch::Tensor& q_in, const torch::Tensor& k_cache, const torch::Tensor& v_cache,
-    const torch::Tensor& table, const torch::Tensor& cu, const torch::Tensor& lens,
-    int64_t max_seqlen_q, int64_t max_seqlen_k, int64_t causal, float scale, bool want_lse,
-    const c10::optional<torch::Tensor>& ks, const c10::optional<torch::Tensor>& vs) {
+    const torch::Tensor& table_in, const torch::Tensor& cu_in, const torch::Tensor& lens_in,
+    int64_t max_seqlen_q, int64_t max_seqlen_k, int64_t causal, c10::optional<double> scale_in,
+    bool want_lse, const c10::optional<torch::Tensor>& ks, const c10::optional<torch::Tensor>& vs) {
   check_new_rows(q_in, "q");
+  const auto table = as_ints(table_in, q_in.device());
+  const auto cu = as_ints(cu_in, q_in.device()), lens = as_ints(lens_in, q_in.device());
+  const float scale = static_cast<float>(
+      scale_in.has_value() ? *scale_in : 1.0 / std::sqrt(static_cast<double>(q_in.size(2))));
   const auto c = paged_cache(k_cache, v_cache, table, ks, vs, q_in.device(), q_in.scalar_type());
   TORCH_CHECK(q_in.size(2) == c.head_dim, "head_dim mismatch");
   TORCH_CHECK(c.kv_heads > 0 && q_in.size(1) % c.kv_heads == 0, "GQA: Q heads (", q_in.size(1),

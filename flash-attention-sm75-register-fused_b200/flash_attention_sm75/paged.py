@@ -14,29 +14,17 @@ packed rows ``[cu_seqlens[b], cu_seqlens[b + 1])``, and the last of them is
 position ``seqlens_k[b] - 1``.  A serving step writes its tokens' K and V, then
 attends, with one set of ``block_table``, ``cu_seqlens`` and ``seqlens_k``.
 """
-import math
-
 import torch
 
 import flash_attn_sm75_cuda as _C
 
-from .ops import _CAUSAL_MODES, _check_gqa
+from .ops import _CAUSAL_MODES
 
 
-def _ints(x, device):
-    """int32 device tensor with contiguous rows from a tensor or a sequence of ints."""
-    if not (isinstance(x, torch.Tensor) and x.dtype is torch.int32 and x.device == device):
-        x = torch.as_tensor(x, dtype=torch.int32, device=device)
-    return x if x.dim() == 0 or x.size(-1) <= 1 or x.stride(-1) == 1 else x.contiguous()
-
-
-def _check_pages(k_cache, v_cache):
-    if k_cache.dim() != 4 or v_cache.dim() != 4:
-        raise ValueError("k_cache and v_cache must be 4D [num_pages, H_kv, page_size, D]")
-    if k_cache.size(-1) not in (64, 128):
-        raise RuntimeError(
-            f"flash_attention_sm75 supports head_dim=64 or 128, got {k_cache.size(-1)}"
-        )
+# The binding checks the arguments, and takes integer tensors of any type and
+# device; what it gets as int32 on the inputs' device is used in place.
+def _ints(x):
+    return x if isinstance(x, torch.Tensor) else torch.as_tensor(x, dtype=torch.int32)
 
 
 def kvcache_write_paged(k, v, k_cache, v_cache, block_table, cu_seqlens, seqlens_k, k_scale=None,
@@ -58,12 +46,8 @@ def kvcache_write_paged(k, v, k_cache, v_cache, block_table, cu_seqlens, seqlens
     448 (e4m3).  Tokens without a place (position below 0 or past the table,
     a table entry outside the cache) are not stored.
     """
-    if k.dim() != 3 or v.dim() != 3:
-        raise ValueError("k and v must be 3D [total, H_kv, D]")
-    _check_pages(k_cache, v_cache)
-    dev = k.device
-    _C.kvcache_write_paged(k, v, k_cache, v_cache, _ints(block_table, dev), _ints(cu_seqlens, dev),
-                           _ints(seqlens_k, dev), k_scale, v_scale)
+    _C.kvcache_write_paged(k, v, k_cache, v_cache, _ints(block_table), _ints(cu_seqlens),
+                           _ints(seqlens_k), k_scale, v_scale)
 
 
 def kvcache_read_paged(k_cache, v_cache, block_table, cu_seqlens, seqlens_k, total, k_scale=None,
@@ -82,14 +66,12 @@ def kvcache_read_paged(k_cache, v_cache, block_table, cu_seqlens, seqlens_k, tot
         k, v: [total, H_kv, D], the layout ``flash_attention_varlen_forward``
         takes.  Rows of tokens without a place, and of no sequence, are zero.
     """
-    _check_pages(k_cache, v_cache)
     if dtype is None:
         dtype = k_cache.dtype if k_cache.element_size() == 2 else torch.bfloat16
     if dtype not in (torch.float16, torch.bfloat16):
         raise ValueError(f"dtype must be torch.float16 or torch.bfloat16, got {dtype}")
-    dev = k_cache.device
-    return _C.kvcache_read_paged(k_cache, v_cache, _ints(block_table, dev), _ints(cu_seqlens, dev),
-                                 _ints(seqlens_k, dev), int(total), k_scale, v_scale,
+    return _C.kvcache_read_paged(k_cache, v_cache, _ints(block_table), _ints(cu_seqlens),
+                                 _ints(seqlens_k), int(total), k_scale, v_scale,
                                  dtype is torch.bfloat16)
 
 
@@ -116,18 +98,12 @@ def flash_attention_forward_paged(q, k_cache, v_cache, block_table, cu_seqlens_q
 
     Rows that see no key, and rows of no sequence, return O = 0, LSE = -inf.
     """
-    if q.dim() != 3:
-        raise ValueError("q must be 3D [total_q, H_q, D]")
-    _check_pages(k_cache, v_cache)
-    if causal and causal_alignment not in _CAUSAL_MODES:
-        raise ValueError(f"causal_alignment must be one of {sorted(_CAUSAL_MODES)}")
-    _check_gqa(q.size(1), k_cache.size(1))
-    if scale is None:
-        scale = 1.0 / math.sqrt(q.size(-1))
-    dev = q.device
-    mode = _CAUSAL_MODES[causal_alignment] if causal else 0
+    mode = 0
+    if causal:
+        mode = _CAUSAL_MODES.get(causal_alignment)
+        if mode is None:
+            raise ValueError(f"causal_alignment must be one of {sorted(_CAUSAL_MODES)}")
     out, lse = _C.flash_attention_forward_paged(
-        q, k_cache, v_cache, _ints(block_table, dev), _ints(cu_seqlens_q, dev),
-        _ints(seqlens_k, dev), int(max_seqlen_q), int(max_seqlen_k), mode, float(scale),
-        bool(return_lse), k_scale, v_scale)
+        q, k_cache, v_cache, _ints(block_table), _ints(cu_seqlens_q), _ints(seqlens_k),
+        int(max_seqlen_q), int(max_seqlen_k), mode, scale, bool(return_lse), k_scale, v_scale)
     return (out, lse) if return_lse else out
