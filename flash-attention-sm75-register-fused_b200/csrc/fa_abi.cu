@@ -715,9 +715,9 @@ bool host_tensor_map(CUtensorMap* map, const TiledMap& t) {
   }
   auto fn = encode_fn();
   if (fn == nullptr) return false;
-  cuuint64_t dims[4], strides[3];
-  cuuint32_t box[4];
-  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  cuuint64_t dims[5], strides[4];
+  cuuint32_t box[5];
+  const cuuint32_t ones[5] = {1, 1, 1, 1, 1};
   for (int i = 0; i < t.rank; ++i) {
     dims[i] = t.dims[i];
     box[i] = t.box[i];

@@ -21,8 +21,8 @@ struct TiledMap {
   enum { kF16, kBf16, kBytes };
   const void* base;
   int type, rank;
-  unsigned long long dims[4], strides[3];
-  unsigned box[4];
+  unsigned long long dims[5], strides[4];
+  unsigned box[5];
 };
 bool host_tensor_map(CUtensorMap* map, const TiledMap& t);
 

@@ -68,14 +68,26 @@ struct PagedAttn {
 
 struct alignas(64) ChunkParams {
   CUtensorMap tm_q;  // (d, Hq, T), box (64, G, tq)
-  CUtensorMap tm_k;  // (d, page rows, heads, pages), box (64, box_rows, 1, 1)
+  // (64 columns, 8 rows, d / 64, row groups of 8, planes), box (64, 8, d / 64,
+  // box_rows / 8, 1): a plane is a head of a page, at page * page_step + head *
+  // head_step; 8-bit pages: a head's expanded rows
+  CUtensorMap tm_k;
   CUtensorMap tm_v;
   PagedAttn a;
   int tq;            // tokens of a 128-row tile: 128 / group
   int box_rows;
+  int page_step, head_step;
+  int stale;         // tiles may end in stale rows (pages do, the expanded rows do not)
   int skip_rows;     // sequences with at most this many rows per KV head are not ours
   int n_splits;
   int fill_outside;  // write the rows of no sequence
+  int head0, n_heads;  // KV heads of this launch
+  // 8-bit pages: f16 rows and scales of the launch's heads (paged_expand_kernel)
+  long long exp_rows;
+  uint16_t* exp_k;   // [n_heads][exp_rows][d]
+  uint16_t* exp_v;
+  float* exp_ks;     // [n_heads][exp_rows], f16 results only
+  float* exp_vs;
   float* ws_o;       // [n_splits][total * Hq][d] fp32, normalised
   float* ws_lse;     // [n_splits][total * Hq], natural log
   unsigned epoch;
@@ -105,8 +117,10 @@ int paged_decode_rows();
 size_t paged_decode_ws_bytes(int max_rows, int head_dim, int sms);
 cudaError_t launch_paged_decode(DecodeParams p, int head_dim, int cache_dtype, bool bf16, int sms,
                                 cudaStream_t stream);
-// Chunk kernel and, for n_splits > 1, the join of its key splits.
+// Chunk kernel (after the expansion of 8-bit pages) over the KV heads of p, and
+// the join of its key splits once all heads are done.
 cudaError_t launch_paged_chunk(const ChunkParams& p, int head_dim, int cache_dtype, bool bf16,
-                               int grid, cudaStream_t stream);
+                               int grid, int sms, cudaStream_t stream);
+cudaError_t launch_paged_join(const ChunkParams& p, int head_dim, bool bf16, cudaStream_t stream);
 
 }  // namespace fa

@@ -86,10 +86,20 @@ struct PagedPlan {
   int tq = 0;           // chunk kernel: tokens of a query tile
   int slots = 0;        // ... pairs of tiles there may be
   int n_splits = 1;
-  size_t ws_decode = 0, ws_o = 0, ws_bytes = 16;
+  // 8-bit pages: rows of the expanded keys, KV heads expanded at a time, and
+  // bytes of one head's K (or V) rows and scales
+  long long exp_rows = 0;
+  int exp_heads = 0;
+  size_t exp_row_bytes = 0, exp_scale_bytes = 0;
+  size_t ws_decode = 0, ws_o = 0, ws_lse = 0, ws_bytes = 16;
 };
 
-PagedPlan make_paged_plan(int B, int heads, int group, int head_dim, int total, int max_q, int max_k) {
+// Expanded keys and values are at most this large where several KV heads would
+// make them larger: the heads then go through the chunk kernel in groups.
+constexpr size_t kExpandBytes = size_t{1} << 30;
+
+PagedPlan make_paged_plan(int B, int heads, int group, int head_dim, bool eight, int total, int max_q,
+                          int max_k) {
   PagedPlan k;
   const int sms = fa::host_sm_count();
   const long long rows = static_cast<long long>(max_q) * group;
@@ -107,11 +117,21 @@ PagedPlan make_paged_plan(int B, int heads, int group, int head_dim, int total, 
     const long long n_seq = total / least < B ? total / least : B;
     const long long slots = total / pair + n_seq;
     k.slots = slots < 1 ? 1 : static_cast<int>(slots);
+    k.exp_heads = heads;
+    if (eight) {
+      k.exp_rows = (n_seq < 1 ? 1 : n_seq) * ((static_cast<long long>(max_k) + 127) / 128 * 128);
+      if (k.exp_rows < 128) k.exp_rows = 128;
+      k.exp_row_bytes = static_cast<size_t>(k.exp_rows) * head_dim * 2;
+      k.exp_scale_bytes = static_cast<size_t>(k.exp_rows) * sizeof(float);
+      const size_t per_head = 2 * (k.exp_row_bytes + k.exp_scale_bytes);
+      const size_t fit = kExpandBytes / per_head;
+      if (fit < static_cast<size_t>(heads)) k.exp_heads = fit < 1 ? 1 : static_cast<int>(fit);
+    }
     // One CTA per (pair, head, split): the split with the fewest waves x (key
     // tiles per split + 4 tiles of start-up and join), as for chunked prefill
     // over a contiguous cache; the number of pairs is estimated from the rows.
     const long long pairs = B <= 1 ? (total + pair - 1) / pair : total / pair + (n_seq + 1) / 2;
-    const long long items = (pairs < 1 ? 1 : pairs) * heads;
+    const long long items = (pairs < 1 ? 1 : pairs) * k.exp_heads;
     const long long n = (static_cast<long long>(max_k) + 127) / 128;
     long long best = -1;
     for (long long ns = 1; ns <= 32 && ns <= (n < 1 ? 1 : n); ++ns) {
@@ -122,11 +142,14 @@ PagedPlan make_paged_plan(int B, int heads, int group, int head_dim, int total, 
         k.n_splits = static_cast<int>(ns);
       }
     }
-    if (k.n_splits > 1)
-      k.ws_o = static_cast<size_t>(k.n_splits) * total * heads * group * head_dim * sizeof(float);
+    if (k.n_splits > 1) {
+      const size_t rows_all = static_cast<size_t>(k.n_splits) * total * heads * group;
+      k.ws_o = rows_all * head_dim * sizeof(float);
+      k.ws_lse = (rows_all * sizeof(float) + 127) / 128 * 128;
+    }
   }
   const size_t chunk_bytes =
-      k.n_splits > 1 ? k.ws_o + static_cast<size_t>(k.n_splits) * total * heads * group * sizeof(float) : 0;
+      k.ws_o + k.ws_lse + 2 * static_cast<size_t>(k.exp_heads) * (k.exp_row_bytes + k.exp_scale_bytes);
   // (the kernels run one after another, so they share the workspace)
   k.ws_bytes = k.ws_decode > chunk_bytes ? k.ws_decode : chunk_bytes;
   if (k.ws_bytes < 16) k.ws_bytes = 16;
@@ -163,6 +186,64 @@ bool page_maps(const fa_paged_cache& c, int rows, CUtensorMap* k, CUtensorMap* v
   if (!fa::host_tensor_map(k, t)) return false;
   t.base = c.v;
   return fa::host_tensor_map(v, t);
+}
+
+// Tensor map of 128-byte column halves by groups of 8 rows (see ChunkParams):
+// `planes` planes of `rows` rows, `plane` and `row` bytes apart.
+bool tile_map(const void* base, int type, int head_dim, long long rows, unsigned long long row,
+              long long planes, unsigned long long plane, int box_rows, CUtensorMap* map) {
+  fa::TiledMap t{};
+  t.type = type;
+  t.base = base;
+  t.rank = 5;
+  t.dims[0] = 64;
+  t.dims[1] = 8;
+  t.dims[2] = head_dim / 64;
+  t.dims[3] = rows / 8;
+  t.dims[4] = planes;
+  t.strides[0] = row;
+  t.strides[1] = 128;
+  t.strides[2] = 8 * row;
+  t.strides[3] = plane;
+  t.box[0] = 64;
+  t.box[1] = 8;
+  t.box[2] = head_dim / 64;
+  t.box[3] = box_rows / 8;
+  t.box[4] = 1;
+  return fa::host_tensor_map(map, t);
+}
+
+// Maps of 16-bit pages for the chunk kernel.  Heads and pages share the last
+// dimension, whose stride is the greatest common divisor of theirs (the head
+// stride itself in head-major and token-major pages).
+bool chunk_maps(const fa_paged_cache& c, fa::ChunkParams* p) {
+  const unsigned long long row = 2ull * c.head_dim;
+  const unsigned long long rs = c.row_stride > 0 ? 2ull * c.row_stride : row;
+  const unsigned long long hs = c.kv_heads > 1 ? 2ull * c.head_stride : 0;
+  const unsigned long long ps = c.num_pages > 1 ? 2ull * c.page_stride : 0;
+  unsigned long long g = hs, x = ps;
+  while (x != 0) {
+    const unsigned long long r = g % x;
+    g = x;
+    x = r;
+  }
+  if (g == 0) g = row;  // one head of one page (or strides of zero)
+  const unsigned long long planes = (c.num_pages > 1 ? (c.num_pages - 1ull) * (ps / g) : 0ull) +
+                                    (c.kv_heads - 1ull) * (hs / g) + 1ull;
+  if (planes > 0x7fffffffull || ps / g > 0x7fffffffull || hs / g > 0x7fffffffull) return false;
+  p->page_step = static_cast<int>(ps / g);
+  p->head_step = static_cast<int>(hs / g);
+  const int type = c.dtype == FA_DTYPE_BF16 ? fa::TiledMap::kBf16 : fa::TiledMap::kF16;
+  return tile_map(c.k, type, c.head_dim, c.page_size, rs, planes, g, p->box_rows, &p->tm_k) &&
+         tile_map(c.v, type, c.head_dim, c.page_size, rs, planes, g, p->box_rows, &p->tm_v);
+}
+
+// Maps of the expanded rows of 8-bit pages.
+bool rows_maps(fa::ChunkParams& p, int head_dim, int heads) {
+  const unsigned long long row = 2ull * head_dim;
+  const int type = fa::TiledMap::kF16;
+  return tile_map(p.exp_k, type, head_dim, p.exp_rows, row, heads, row * p.exp_rows, 128, &p.tm_k) &&
+         tile_map(p.exp_v, type, head_dim, p.exp_rows, row, heads, row * p.exp_rows, 128, &p.tm_v);
 }
 
 // Tensor map of the queries: boxes of a query tile, `tq` tokens x the heads of
@@ -238,8 +319,8 @@ size_t fa_fwd_paged_workspace_bytes(const fa_paged_cache* cache, int B, int Hq, 
   if (!cache || cache->kv_heads <= 0 || Hq <= 0 || total_q <= 0) return 16;
   const int group = Hq / cache->kv_heads > 0 ? Hq / cache->kv_heads : 1;
   if (group > 128 || B < 0 || max_seqlen_q < 0 || max_seqlen_k < 0) return 16;  // refused sizes
-  return make_paged_plan(B, cache->kv_heads, group, cache->head_dim, total_q, max_seqlen_q,
-                         max_seqlen_k)
+  return make_paged_plan(B, cache->kv_heads, group, cache->head_dim, is_8bit(cache->dtype), total_q,
+                         max_seqlen_q, max_seqlen_k)
       .ws_bytes;
 }
 
@@ -262,10 +343,11 @@ int fa_fwd_paged(const fa_paged_cache* cache, const void* Q, long long q_token_s
       ((q_token_stride | q_head_stride) & 7) || (reinterpret_cast<uintptr_t>(lse) & 3u))
     return FA_ERR_ALIGNMENT;
   const int group = Hq / a.c.heads;
-  const PagedPlan k = make_paged_plan(B, a.c.heads, group, cache->head_dim, total_q, max_seqlen_q,
+  const bool eight = is_8bit(cache->dtype);
+  const PagedPlan k = make_paged_plan(B, a.c.heads, group, cache->head_dim, eight, total_q, max_seqlen_q,
                                       max_seqlen_k);
   if (workspace_bytes < k.ws_bytes) return FA_ERR_INVALID_ARG;
-  const long long grid = static_cast<long long>(k.slots) * a.c.heads * k.n_splits;
+  const long long grid = static_cast<long long>(k.slots) * a.c.heads * k.n_splits;  // of all heads
   if (grid > 0x7fffffffLL || static_cast<long long>(B) * a.c.heads > 0x7fffffffLL ||
       static_cast<long long>(total_q) * Hq > (1LL << 33))
     return FA_ERR_TOO_LARGE;
@@ -299,20 +381,35 @@ int fa_fwd_paged(const fa_paged_cache* cache, const void* Q, long long q_token_s
     fa::ChunkParams p;
     p.a = a;
     p.tq = k.tq;
-    p.box_rows = gcd_128(cache->page_size);
+    p.box_rows = eight ? 128 : gcd_128(cache->page_size);
+    p.stale = eight ? 0 : 1;
+    p.page_step = p.head_step = 0;
     p.skip_rows = k.decode ? k.decode_rows : 0;
     p.n_splits = k.n_splits;
-    p.fill_outside = k.decode ? 0 : 1;
-    p.ws_o = static_cast<float*>(workspace);
-    p.ws_lse = reinterpret_cast<float*>(static_cast<char*>(workspace) + k.ws_o);
-    p.epoch = fa::host_next_epoch();
+    char* ws = static_cast<char*>(workspace);
+    p.ws_o = reinterpret_cast<float*>(ws);
+    p.ws_lse = reinterpret_cast<float*>(ws + k.ws_o);
+    ws += k.ws_o + k.ws_lse;
+    p.exp_rows = k.exp_rows;
+    p.exp_k = reinterpret_cast<uint16_t*>(ws);
+    p.exp_v = reinterpret_cast<uint16_t*>(ws + k.exp_heads * k.exp_row_bytes);
+    ws += 2 * k.exp_heads * k.exp_row_bytes;
+    p.exp_ks = reinterpret_cast<float*>(ws);
+    p.exp_vs = reinterpret_cast<float*>(ws + k.exp_heads * k.exp_scale_bytes);
     p.timeout_ns = fa::host_timeout_ns();
-    if (!is_8bit(cache->dtype) &&
-        (!page_maps(*cache, p.box_rows, &p.tm_k, &p.tm_v) ||
-         !query_map(*cache, p.tq, Q, q_token_stride, q_head_stride, Hq, total_q, bf16, &p.tm_q)))
-      return FA_ERR_TENSOR_MAP;
-    if (fa::launch_paged_chunk(p, cache->head_dim, cache->dtype, bf16, static_cast<int>(grid), st) !=
-        cudaSuccess)
+    const bool maps =
+        (eight ? rows_maps(p, cache->head_dim, k.exp_heads) : chunk_maps(*cache, &p)) &&
+        query_map(*cache, p.tq, Q, q_token_stride, q_head_stride, Hq, total_q, bf16, &p.tm_q);
+    if (!maps) return FA_ERR_TENSOR_MAP;
+    for (p.head0 = 0; p.head0 < a.c.heads; p.head0 += k.exp_heads) {
+      p.n_heads = a.c.heads - p.head0 < k.exp_heads ? a.c.heads - p.head0 : k.exp_heads;
+      p.fill_outside = !k.decode && p.head0 == 0 ? 1 : 0;
+      p.epoch = fa::host_next_epoch();
+      if (fa::launch_paged_chunk(p, cache->head_dim, cache->dtype, bf16, k.slots * p.n_heads * k.n_splits,
+                                 fa::host_sm_count(), st) != cudaSuccess)
+        return FA_ERR_LAUNCH;
+    }
+    if (k.n_splits > 1 && fa::launch_paged_join(p, cache->head_dim, bf16, st) != cudaSuccess)
       return FA_ERR_LAUNCH;
   }
   return FA_OK;

@@ -16,15 +16,22 @@
 //          rows can hold, and a CTA without one leaves at once.  Pairs of a
 //          sequence run from its end, the longest causal rows first.
 //   pages  16-bit pages: a 128-key tile is a set of TMA boxes of gcd(page, 128)
-//          rows, one per lane of the producer warp.  The rows behind the last
-//          visible key in its box are stale; V's are set to zero before the
-//          tile is released, K's are masked as scores.
-//          8-bit pages: three warps read 16-key groups into registers, widen
-//          them to f16 (exact) and store them in the swizzled layout the
-//          products read.  For bf16 results they also multiply by the row's
-//          scale (two f16 roundings, 8 times finer than the result's); for f16
-//          results the softmax applies the scales in fp32: K's to the scores,
-//          V's to P relative to a power of two that follows the largest scale.
+//          rows, one per lane of the producer warp.  A box brings whole rows: the
+//          maps split d into halves of 128 bytes, laid out per 8 rows (8 rows x
+//          128 bytes of one half, then of the other), which the products'
+//          descriptors take like any swizzled tile.  (With a box per half, 32
+//          per tile at page 16, the loads bounded the kernel: 551 us against 420
+//          from 128-row pages at B=2, 2048 over 8192 keys, d = 128.)  The rows
+//          behind the last visible key in its box are stale; V's are set to zero
+//          before the tile is released, K's are masked as scores.
+//          8-bit pages: paged_expand_kernel first writes the visible keys and
+//          values once as f16 rows into the workspace (exactly, with the scales
+//          beside them, for f16 results; multiplied by their scale and rounded,
+//          8 times finer than the result, for bf16 ones), so that the pairs of a
+//          chunk do not widen the same keys again and again, and the kernel
+//          reads plain 128-row tiles.  For f16 results the softmax applies the
+//          scales in fp32: K's to the scores; V's is split into a power of two,
+//          which the rows take (exactly), and a rest in [1, 2) for P.
 //   joins  With few items the keys are split; partial O and LSE go to the
 //          workspace and paged_join_kernel merges them.
 #include "fa_paged.h"
@@ -33,23 +40,32 @@
 namespace fa {
 namespace {
 
-template <int D, bool k8>
+// What the kernel reads.
+enum { kPagesF16 = 0, kPagesBf16 = 1, kExpanded = 2 };
+
+template <int D, bool kScaled>
 struct ChunkLayout {
+  // register split; the scales' multiplications take 16 more in the softmax
+  static constexpr int kRegsSoft = kScaled ? 208 : kRegsSoftmax;
+  static constexpr int kRegsRest = kScaled ? 88 : kRegsOther;
+  static_assert(256 * kRegsSoft + 128 * kRegsRest <= kThreads * kLaunchRegs,
+                "register split exceeds the launch allocation");
   static constexpr int kColBlocks = D / 64;
-  static constexpr int kBlockBytes = 128 * 128;
+  static constexpr int kBlockBytes = 128 * 128;           // Q: 64 columns of a tile
+  static constexpr int kGroupBytes = 1024 * kColBlocks;   // K, V: 8 rows of a tile
   static constexpr int kTile = 128 * D * 2;
-  static constexpr int kSlots = D == 64 ? 8 : (k8 ? 4 : 5);
+  static constexpr int kSlots = D == 64 ? 8 : (kScaled ? 4 : 5);
   static constexpr int kOffQ = 0;
   static constexpr int kOffKV = 2 * kTile;
   static constexpr int kOffScale = kOffKV + kSlots * kTile;
-  // scales of tile j at entry j % kScaleRing: K's 128, V's 128, V's maximum per
-  // 16 keys.  K_j's slot is free only after the scores of tile
-  // j - kSlots / 2 were issued for both groups, i.e. after both finished the
-  // softmax of the tile before it, so entry j - kScaleRing is no longer read.
+  // scales of tile j at entry j % kScaleRing: K's 128, V's 128, loaded with
+  // K_j.  K_j's slot is free only after the scores of tile j - kSlots / 2 were
+  // issued for both groups, i.e. after both finished the softmax of the tile
+  // before it, so entry j - kScaleRing is no longer read.
   static constexpr int kScaleRing = D == 64 ? 8 : 4;
-  static constexpr int kScaleEntry = (128 + 128 + 8) * 4;
+  static constexpr int kScaleEntry = 2 * 128 * 4;
   static_assert(kScaleRing >= kSlots / 2 + 1, "a scale entry outlives its tile");
-  static constexpr int kOffBar = kOffScale + (k8 ? kScaleRing * kScaleEntry : 0);
+  static constexpr int kOffBar = kOffScale + (kScaled ? kScaleRing * kScaleEntry : 0);
   static constexpr int kBarQ = 0;                       // 2
   static constexpr int kBarFull = 2;                    // kSlots
   static constexpr int kBarEmpty = kBarFull + kSlots;   // kSlots
@@ -72,18 +88,28 @@ struct ChunkLayout {
   static_assert(kDynBytes <= 227 * 1024, "shared memory budget");
 };
 
-// exp_tile (fa_fwd_sm100.cu) with P multiplied by V's scales: e = 2^(x sl - m)
-// is summed as it is, e * vs goes to tensor memory.
+// Four scales from shared memory; volatile, so that the loads stay where they
+// are used (hoisted over the 128 scores of a row they spill).
+__device__ __forceinline__ float4 load_scales(uint32_t addr) {
+  float4 f;
+  asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(f.x), "=f"(f.y), "=f"(f.z), "=f"(f.w)
+               : "r"(addr));
+  return f;
+}
+
+// exp_tile (fa_fwd_sm100.cu) with P multiplied by the rest of V's scales: e =
+// 2^(x sl - m) is summed as it is, e * vs goes to tensor memory.
 template <bool kEmulate, int kPeriod, typename Announce>
 __device__ __forceinline__ float exp_tile_scaled(const float (&x)[kBlockN], float sl, float neg_m,
-                                                 const float* vs, uint32_t tP, Announce announce) {
+                                                 uint32_t vs, uint32_t tP, Announce announce) {
   float a0 = 0.f, a1 = 0.f, b0 = 0.f, b1 = 0.f;
 #pragma unroll
   for (int h = 0; h < 4; ++h) {
     uint32_t pk[16];
 #pragma unroll
     for (int c = 0; c < 16; c += 2) {
-      const float4 f = *reinterpret_cast<const float4*>(vs + 32 * h + 2 * c);
+      const float4 f = load_scales(vs + 4 * (32 * h + 2 * c));
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
         const int i = 32 * h + 2 * (c + y);
@@ -108,6 +134,9 @@ __device__ __forceinline__ float exp_tile_scaled(const float (&x)[kBlockN], floa
   return a0 + a1;
 }
 
+// 128-row blocks of a sequence in the expanded rows.
+__device__ __forceinline__ int expand_blocks(const Seq& s) { return (s.vis + kBlockN - 1) / kBlockN; }
+
 // The work item of a CTA.
 struct ChunkItem {
   Seq s;
@@ -115,20 +144,20 @@ struct ChunkItem {
   int n_kv[2], jb, n_loop;  // key tiles of either query tile, from tile jb
 };
 
-// KV: type of the pages (FA_DTYPE_*); QBF16: type of Q and O.
-template <int D, int KV, bool QBF16>
+// SRC: what is read; QBF16: type of Q and O.
+template <int D, int SRC, bool QBF16>
 __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_constant__ ChunkParams p) {
-  constexpr bool k8 = KV >= FA_DTYPE_INT8;
-  constexpr bool kBf16 = KV == FA_DTYPE_BF16;  // type of the products
-  constexpr bool kFold = k8 && QBF16;          // scales go into the widened values
-  constexpr bool kScaled = k8 && !QBF16;       // ... are applied by the softmax
-  using L = ChunkLayout<D, k8>;
+  constexpr bool kExp = SRC == kExpanded;
+  constexpr bool kBf16 = SRC == kPagesBf16;   // type of the products
+  constexpr bool kScaled = kExp && !QBF16;    // the softmax applies the scales
+  constexpr bool kCastQ = kExp && QBF16;      // Q becomes f16
+  using L = ChunkLayout<D, kScaled>;
   const PagedAttn& a = p.a;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
   __shared__ long long sh_scan[kThreads / 32];
-  __shared__ int sh_item[2];  // sequence, pair (-1: none)
+  __shared__ int sh_item[3];  // sequence, pair (-1: none), first block of the expanded rows
   const uint32_t sbase = ptx::smem_u32(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kOffMisc);
@@ -138,11 +167,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
 
   // ---- which (sequence, pair) is this CTA's?
   const int w = static_cast<int>(blockIdx.x);
-  const int slot_id = w / (p.n_splits * a.c.heads);
+  const int slot_id = w / (p.n_splits * p.n_heads);
   {
-    auto pairs_of = [&](int b) {
+    // low word: pairs of a sequence; high word: its 128-row blocks in the
+    // expanded rows
+    auto pairs_of = [&](int b) -> long long {
       const Seq s = load_seq(a, b);
-      return static_cast<long long>(s.nq) * a.group <= p.skip_rows ? 0 : (s.nq + 2 * p.tq - 1) / (2 * p.tq);
+      if (static_cast<long long>(s.nq) * a.group <= p.skip_rows) return 0;
+      return (s.nq + 2 * p.tq - 1) / (2 * p.tq) + (static_cast<long long>(expand_blocks(s)) << 32);
     };
     const int share = (a.r.B + kThreads - 1) / kThreads;
     const int b0 = min(static_cast<int>(threadIdx.x) * share, a.r.B), b1 = min(b0 + share, a.r.B);
@@ -150,12 +182,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
     long long sum = 0, total;
     for (int b = b0; b < b1; ++b) sum += pairs_of(b);
     long long x = block_scan<kThreads>(sum, sh_scan, &total);
-    if (slot_id >= x && slot_id < x + sum)
+    const int lo = static_cast<int>(x), hi = lo + static_cast<int>(sum);
+    if (slot_id >= lo && slot_id < hi)
       for (int b = b0; b < b1; ++b) {
-        const int n = pairs_of(b);
-        if (slot_id < x + n) {
+        const long long n = pairs_of(b);
+        const int first = static_cast<int>(x), pairs = static_cast<int>(n);
+        if (slot_id < first + pairs) {
           sh_item[0] = b;
-          sh_item[1] = n - 1 - static_cast<int>(slot_id - x);  // from the sequence's end
+          sh_item[1] = first + pairs - 1 - slot_id;  // from the sequence's end
+          sh_item[2] = static_cast<int>(x >> 32);
           break;
         }
         x += n;
@@ -179,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
   it.pair = sh_item[1];
   if (it.pair < 0) return;
   it.b = sh_item[0];
-  it.h = (w / p.n_splits) % a.c.heads;
+  it.h = p.head0 + (w / p.n_splits) % p.n_heads;
   it.sp = w % p.n_splits;
   it.s = load_seq(a, it.b);
   const int tok0 = it.pair * 2 * p.tq;  // first token of tile 0
@@ -206,9 +241,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
     *abort_flag = ((st >> 32) == p.epoch && (st & 0xffffffffull) != 0ull) ? 1 : 0;
     for (int i = 0; i < L::kNumBars; ++i) {
       const bool all = (i >= L::kBarP && i < L::kBarP + 2) || (i >= L::kBarPH && i < L::kBarPH + 2) ||
-                       (k8 && i < 2);
-      const bool full = i >= L::kBarFull && i < L::kBarFull + L::kSlots;
-      ptx::mbar_init(bar(i), all ? 128u : (k8 && full) ? 8u : 1u);
+                       (kCastQ && i < 2);
+      ptx::mbar_init(bar(i), all ? 128u : 1u);
     }
     ptx::fence_barrier_init();
   }
@@ -226,16 +260,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
   const int n_items = 2 * it.n_loop;  // K_0 V_0 K_1 V_1 ...
 
   if (warp >= 8) {
-    ptx::setmaxnreg_dec<kRegsOther>();
-    if (!k8 && warp == kWarpLoad) {
-      // =================================================== TMA producer (16-bit pages)
+    ptx::setmaxnreg_dec<L::kRegsRest>();
+    if (warp == kWarpLoad) {
+      // =================================================== TMA producer
       const uint64_t pol_q = ptx::policy_evict_first();
       const uint64_t pol_kv = ptx::policy_evict_last();
       if (lane == 0) {
         ptx::prefetch_tmap(&p.tm_q);
         ptx::prefetch_tmap(&p.tm_k);
         ptx::prefetch_tmap(&p.tm_v);
-        for (int g = 0; g < 2; ++g) {
+        for (int g = 0; g < 2 && !kCastQ; ++g) {
           if (it.n_kv[g] == 0) continue;
           ptx::mbar_arrive_expect_tx(bar(L::kBarQ + g), L::kColBlocks * n_rows * 128);
 #pragma unroll
@@ -246,14 +280,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
         }
       }
       __syncwarp();
-      // lane = column block * 8 + box; a box starts at key tile * 128 + box * box_rows
-      const int col = lane >> 3, box = lane & 7;
-      const bool issues = col < L::kColBlocks && box * p.box_rows < kBlockN;
-      const uint32_t dst_off = col * L::kBlockBytes + box * p.box_rows * 128;
-      auto page_at = [&](int tile) {  // page of this lane's box; -1 reads as zeros
+      // lane = box of the tile (the expanded rows have one of 128 rows)
+      const int box = lane;
+      const bool issues = box * p.box_rows < kBlockN;
+      const uint32_t dst_off = box * p.box_rows * (2 * D);
+      // place of this lane's box in the map's last dimension; -1 reads as zeros
+      auto page_at = [&](int tile) {
+        if (kExp) return it.h - p.head0;
         const int pos = tile * kBlockN + box * p.box_rows;
-        return issues && pos < it.s.vis ? a.c.lookup(it.b, pos) : -1;
+        const int page = issues && pos < it.s.vis ? a.c.lookup(it.b, pos) : -1;
+        return page >= 0 ? page * p.page_step + it.h * p.head_step : -1;
       };
+      const int exp_row0 = sh_item[2] * kBlockN;  // of the sequence in the expanded rows
       int next_page = page_at(it.jb), page = -1;
       bool ok = true, tail_used = false;
       int i = 0;
@@ -271,21 +309,33 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
         // stale V rows of the tile: [r0, r1)
         const int r0 = it.s.vis - tile * kBlockN;
         const int r1 = (r0 + p.box_rows - 1) / p.box_rows * p.box_rows;
-        const bool tail = (i & 1) && r0 < kBlockN && r0 != r1;
+        // (a run-time flag, though the expanded rows never have any: with the
+        // branch compiled out the softmax spills, 874 instead of 449 us)
+        const bool tail = p.stale && (i & 1) && r0 < kBlockN && r0 != r1;
         const uint32_t full = tail ? bar(L::kBarTail) : bar(L::kBarFull + slot);
-        if (lane == 0) ptx::mbar_arrive_expect_tx(full, L::kTile);
+        const bool scales = kScaled && !(i & 1);
+        if (lane == 0) ptx::mbar_arrive_expect_tx(full, L::kTile + (scales ? L::kScaleEntry : 0));
         __syncwarp();
         const uint32_t dst = sbase + L::kOffKV + slot * L::kTile;
+        // first row: in the page, or in the expanded rows (kept inside them)
+        const int row = kExp ? min(exp_row0 + tile * kBlockN, static_cast<int>(p.exp_rows) - kBlockN)
+                             : a.c.row_in_page(tile * kBlockN + box * p.box_rows);
         if (issues)
-          ptx::tma_load_4d(dst + dst_off, (i & 1) ? &p.tm_v : &p.tm_k, full, col * 64,
-                      a.c.row_in_page(tile * kBlockN + box * p.box_rows), it.h, page, pol_kv);
+          ptx::tma_load_5d(dst + dst_off, (i & 1) ? &p.tm_v : &p.tm_k, full, 0, 0, 0, row >> 3, page, pol_kv);
+        if (scales && lane < 2) {
+          const float* src = (lane ? p.exp_vs : p.exp_ks) +
+                             static_cast<long long>(it.h - p.head0) * p.exp_rows + row;
+          ptx::bulk_load(sbase + L::kOffScale + ((i >> 1) % L::kScaleRing) * L::kScaleEntry + lane * 512, src,
+                         512, full);
+        }
         if (tail) {
           tail_used = true;
           if (!(ok = __all_sync(0xffffffffu, bar_wait(bar(L::kBarTail), 0, wc, 7)))) break;
           for (int x = lane; x < (r1 - r0) * 8 * L::kColBlocks; x += 32) {
             const int r = r0 + x / (8 * L::kColBlocks), c = x % (8 * L::kColBlocks);
-            *reinterpret_cast<uint4*>(smem + L::kOffKV + slot * L::kTile + (c >> 3) * L::kBlockBytes +
-                                      r * 128 + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+            *reinterpret_cast<uint4*>(smem + L::kOffKV + slot * L::kTile + (r >> 3) * L::kGroupBytes +
+                                      (c >> 3) * 1024 + (r & 7) * 128 + (c & 7) * 16) =
+                make_uint4(0u, 0u, 0u, 0u);
           }
           ptx::fence_proxy_async_smem();
           __syncwarp();
@@ -296,155 +346,34 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
       for (int r = max(0, i - L::kSlots); r < i; ++r)
         bar_wait(bar(L::kBarFull + r % L::kSlots), (r / L::kSlots) & 1, wc, 2, false);
       if (tail_used && !ok) bar_wait(bar(L::kBarTail), 0, wc, 2, false);
-      for (int g = 0; g < 2; ++g)
+      for (int g = 0; g < 2 && !kCastQ; ++g)
         if (it.n_kv[g] > 0) bar_wait(bar(L::kBarQ + g), 0, wc, 2, false);
-    } else if (k8 && warp != kWarpMma) {
-      // =================================================== widening warps (8-bit pages)
-      // Groups of 16 keys, 8 per ring item, dealt to warps 8, 10 and 11 in turn.
-      // A lane takes 16 values of a row at a time: D / 16 lanes a row.
-      constexpr int kLanesRow = D / 16;
-      constexpr int kLoads = 16 / (32 / kLanesRow);  // rows of the group per lane
-      const int cw = warp == kWarpLoad ? 0 : warp - kWarpLoad - 1;
-      const int n_groups = 8 * n_items;
-      const int lr = lane / kLanesRow, lx = lane % kLanesRow;
-      struct Raw {
-        uint4 v[kLoads];
-        float sc, sc2;  // lane < 16: scale of row `lane` (kScaled, K items: K's and V's)
-      };
-      auto lookup = [&](int n) {
-        const int pos = (it.jb + (n >> 4)) * kBlockN + 16 * (n & 7);
-        return n < n_groups && pos < it.s.vis ? a.c.lookup(it.b, pos) : -1;
-      };
-      auto load = [&](Raw& r, int n, int page) {
-        const int pos = (it.jb + (n >> 4)) * kBlockN + 16 * (n & 7);
-        const bool is_v = (n >> 3) & 1;
-        const int left = page >= 0 ? it.s.vis - pos : 0;  // rows that exist
-        const long long prow = a.c.row_in_page(pos);
-        const uint8_t* src = (is_v ? a.c.v : a.c.k) + page * a.c.page_stride + it.h * a.c.head_stride +
-                             prow * a.c.row_stride + 16 * lx;
-#pragma unroll
-        for (int y = 0; y < kLoads; ++y) {
-          const int row = y * (32 / kLanesRow) + lr;
-          r.v[y] = make_uint4(0u, 0u, 0u, 0u);
-          if (row < left) r.v[y] = __ldg(reinterpret_cast<const uint4*>(src + row * a.c.row_stride));
-        }
-        r.sc = r.sc2 = 0.f;
-        if (lane < 16 && lane < left) {
-          const long long so = page * a.c.s_page + it.h * a.c.s_head + (prow + lane) * a.c.s_row;
-          if constexpr (kFold) {
-            r.sc = __ldg((is_v ? a.c.vs : a.c.ks) + so);
-          } else if (!is_v) {
-            r.sc = __ldg(a.c.ks + so);
-            r.sc2 = __ldg(a.c.vs + so);
-          }
-        }
-      };
-      auto store = [&](const Raw& r, int n) -> bool {
-        const int item = n >> 3, grp = n & 7;
-        const int slot = item % L::kSlots;
-        if (item >= L::kSlots &&
-            !__all_sync(0xffffffffu, bar_wait(bar(L::kBarEmpty + slot), ((item / L::kSlots) - 1) & 1, wc, 1)))
-          return false;
-        uint8_t* dst = smem + L::kOffKV + slot * L::kTile;
-        // f16 products of a scale below 2^-14 would lose its bits, and one above
-        // 128 could overflow: such groups multiply in two steps
-        bool wide = false;
-        if constexpr (kFold)
-          wide = __any_sync(0xffffffffu, lane < 16 && (r.sc != 0.f && (r.sc < 6.103515625e-5f || !(r.sc <= 128.f))));
-#pragma unroll
-        for (int y = 0; y < kLoads; ++y) {
-          const int row = y * (32 / kLanesRow) + lr;
-          const uint32_t in[4] = {r.v[y].x, r.v[y].y, r.v[y].z, r.v[y].w};
-          uint32_t o[8];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) widen<KV, false>(in[i], o[2 * i], o[2 * i + 1]);
-          if constexpr (kFold) {
-            const float sc = __shfl_sync(0xffffffffu, r.sc, row);
-            __half2 s1, s2;
-            if (!wide) {
-              s1 = __float2half2_rn(sc);
-            } else {
-              // sc = m * 2^e, 2^e in f16's range (2^-23 .. 2^7), m in [1, 2) as far as that goes
-              const uint32_t eb = min(max(__float_as_uint(sc) & 0x7f800000u, 0x34000000u), 0x43000000u);
-              const float e = __uint_as_float(eb), mant = sc / e;
-              s1 = __float2half2_rn(mant > 65504.f ? 65504.f : mant);
-              s2 = __float2half2_rn(e);
-            }
-            const __half2 top = __half2half2(__ushort_as_half(0x7bff));  // 65504
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              __half2 x = __hmul2(*reinterpret_cast<__half2*>(&o[i]), s1);
-              if (wide) x = __hmax2_nan(__hmin2_nan(__hmul2(x, s2), top), __hneg2(top));
-              o[i] = *reinterpret_cast<uint32_t*>(&x);
-            }
-          }
-          // 16 values = 16-byte pieces 2 lx and 2 lx + 1 of the row; the right half
-          // of a 128-wide row stores its odd piece first, so that the eight lanes of
-          // a row hit eight bank groups
-          const int row_t = 16 * grp + row;
-          const int cb = D == 128 ? lx >> 2 : 0;
-          const int c = (2 * lx) & 7;
-          uint8_t* base = dst + cb * L::kBlockBytes + row_t * 128;
-          const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
-          const bool odd = cb != 0;
-          *reinterpret_cast<uint4*>(base + (((c + (odd ? 1 : 0)) ^ (row_t & 7)) << 4)) = odd ? hi : lo;
-          *reinterpret_cast<uint4*>(base + (((c + (odd ? 0 : 1)) ^ (row_t & 7)) << 4)) = odd ? lo : hi;
-        }
-        if constexpr (kScaled) {
-          if (!(item & 1)) {
-            float* e = reinterpret_cast<float*>(smem + L::kOffScale + ((item >> 1) % L::kScaleRing) * L::kScaleEntry);
-            float mx = r.sc2;
-#pragma unroll
-            for (int x = 8; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-            if (lane < 16) {
-              e[16 * grp + lane] = r.sc;
-              e[128 + 16 * grp + lane] = r.sc2;
-            }
-            if (lane == 0) e[256 + grp] = mx;
-          }
-        }
-        ptx::fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(bar(L::kBarFull + slot));
-        return true;
-      };
-      // two groups in flight, their pages looked up one step earlier
-      Raw ra, rb;
-      int n = cw;
-      load(ra, n, lookup(n));
-      load(rb, n + 3, lookup(n + 3));
-      int pa = lookup(n + 6), pb = lookup(n + 9);
-      for (; n < n_groups; n += 6) {
-        if (!store(ra, n)) break;
-        load(ra, n + 6, pa);
-        pa = lookup(n + 12);
-        if (n + 3 < n_groups && !store(rb, n + 3)) break;
-        load(rb, n + 9, pb);
-        pb = lookup(n + 15);
-      }
     } else if (warp == kWarpMma) {
       // =================================================== MMA issuer (see fa_fwd_kernel)
       constexpr uint32_t fmt = kBf16 ? 1u : 0u;
       constexpr uint32_t idesc_qk = ptx::make_idesc_f16(kBlockM, kBlockN, fmt, 0, 0);
       constexpr uint32_t idesc_pv = ptx::make_idesc_f16(kBlockM, D, fmt, 0, 1);
-      const uint64_t k_desc0 = ptx::smem_desc_sw128(sbase + L::kOffKV, 16, 1024);
-      const uint64_t v_desc0 = ptx::smem_desc_sw128(sbase + L::kOffKV, L::kBlockBytes, 1024);
-      const uint32_t d_hi = static_cast<uint32_t>(k_desc0 >> 32);
-      const uint32_t v_hi = static_cast<uint32_t>(v_desc0 >> 32);
+      const uint64_t k_desc0 = ptx::smem_desc_sw128(sbase + L::kOffKV, 16, L::kGroupBytes);
+      const uint64_t v_desc0 = ptx::smem_desc_sw128(sbase + L::kOffKV, 1024, L::kGroupBytes);
+      const uint64_t q_desc0 = ptx::smem_desc_sw128(sbase + L::kOffQ, 16, 1024);
+      const uint32_t kv_hi = static_cast<uint32_t>(k_desc0 >> 32);  // (the same for K and V)
+      const uint32_t q_hi = static_cast<uint32_t>(q_desc0 >> 32);
       const uint32_t k_lo0 = static_cast<uint32_t>(k_desc0);
       const uint32_t v_lo0 = static_cast<uint32_t>(v_desc0);
-      const uint32_t q_lo0 = static_cast<uint32_t>(ptx::smem_desc_sw128(sbase + L::kOffQ, 16, 1024));
+      const uint32_t q_lo0 = static_cast<uint32_t>(q_desc0);
       const uint32_t q_lo1 =
           static_cast<uint32_t>(ptx::smem_desc_sw128(sbase + L::kOffQ + L::kTile, 16, 1024));
       constexpr uint32_t kSlotStep = L::kTile >> 4;
+      constexpr uint32_t kVStep = 2 * L::kGroupBytes >> 4;  // 16 keys
       auto issue_s = [&](int g, int ks, uint32_t q_lo) {
         const uint32_t k_lo = k_lo0 + static_cast<uint32_t>(ks) * kSlotStep;
         if (ptx::elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
-            const uint32_t off = static_cast<uint32_t>(((kk / 4) * L::kBlockBytes + (kk % 4) * 32) >> 4);
-            ptx::mma_ss(tmem + L::tS(g), ptx::make_desc(q_lo + off, d_hi),
-                        ptx::make_desc(k_lo + off, d_hi), idesc_qk, kk > 0 ? 1u : 0u);
+            const uint32_t q_off = static_cast<uint32_t>(((kk / 4) * L::kBlockBytes + (kk % 4) * 32) >> 4);
+            const uint32_t k_off = static_cast<uint32_t>(((kk / 4) * 1024 + (kk % 4) * 32) >> 4);
+            ptx::mma_ss(tmem + L::tS(g), ptx::make_desc(q_lo + q_off, q_hi),
+                        ptx::make_desc(k_lo + k_off, kv_hi), idesc_qk, kk > 0 ? 1u : 0u);
           }
           ptx::mma_commit(bar(L::kBarS + g));
         }
@@ -465,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
 #pragma unroll
           for (int kk = 0; kk < 2 * kPEarlyQuarters; ++kk)
             ptx::mma_ts(tmem + L::tO(g), tmem + L::tP(g) + kk * 8,
-                        ptx::make_desc(v_lo + kk * 128u, v_hi), idesc_pv, (!first || kk > 0) ? 1u : 0u);
+                        ptx::make_desc(v_lo + kk * kVStep, kv_hi), idesc_pv, (!first || kk > 0) ? 1u : 0u);
         }
         __syncwarp();
         if (!wait(bar(L::kBarP + g), ph, 13 + 3 * g)) return false;
@@ -474,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
 #pragma unroll
           for (int kk = 2 * kPEarlyQuarters; kk < kBlockN / 16; ++kk)
             ptx::mma_ts(tmem + L::tO(g), tmem + L::tP(g) + kk * 8,
-                        ptx::make_desc(v_lo + kk * 128u, v_hi), idesc_pv, 1u);
+                        ptx::make_desc(v_lo + kk * kVStep, kv_hi), idesc_pv, 1u);
           ptx::mma_commit(bar(L::kBarO + g));
         }
         __syncwarp();
@@ -536,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
     }
   } else {
     // ===================================================== softmax groups
-    ptx::setmaxnreg_inc<kRegsSoftmax>();
+    ptx::setmaxnreg_inc<L::kRegsSoft>();
     const int g = warp >> 2;
     const int wq = warp & 3;
     const int r = wq * 32 + lane;  // row of the tile == TMEM lane
@@ -551,7 +480,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
     const bool row_ok = r < n_rows && tok < it.s.nq;
     float sl = a.scale_log2;
     bool ok = true;
-    if constexpr (k8) {
+    if constexpr (kCastQ) {
       // Q as f16 in the swizzled layout, one row per thread; a bf16 row is
       // scaled by a power of two into f16's range, undone in sl
       if (n_tiles > 0) {
@@ -564,7 +493,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
 #pragma unroll
           for (int c = 0; c < D / 8; ++c) q[c] = __ldg(src + c);
         }
-        if constexpr (QBF16) {
+        {
           auto f2 = [](uint32_t u) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&u)); };
           float mx = 0.f;
 #pragma unroll
@@ -596,10 +525,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
     const int row_end = row_limit(a, it.s, tok);
     const int tile_end = row_limit(a, it.s, tok_lo);
 
-    constexpr float kGrow = kScaled ? 8.0f : kRescaleThreshold;
+    // (kScaled: P is multiplied by up to 2 and must stay in f16's range)
+    constexpr float kGrow = kScaled ? kRescaleThreshold - 1.0f : kRescaleThreshold;
     float m = -INFINITY;  // running max of the scaled scores (log2 units)
-    float l = 0.f;        // running sum of exp2(s - m) (kScaled: times 2^-lv)
-    float lv = 0.f;       // kScaled: log2 of the power of two V's scales are relative to
+    float l = 0.f;        // running sum of exp2(s - m)
     for (int j = 0; ok && j < n_tiles; ++j) {
       ok = __all_sync(0xffffffffu, bar_wait(bar(L::kBarS + g), j & 1, wc, 20 + g));
       if (!ok) break;
@@ -624,24 +553,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
           x[96 + c] = __uint_as_float(u3[c]);
         }
       }
-      const float* entry = reinterpret_cast<const float*>(
-          smem + L::kOffScale + (k8 ? (j % L::kScaleRing) * L::kScaleEntry : 0));
-      float lv_new = lv;
+      const uint32_t entry = sbase + L::kOffScale + (kScaled ? (j % L::kScaleRing) * L::kScaleEntry : 0);
       if constexpr (kScaled) {
 #pragma unroll
         for (int c = 0; c < kBlockN; c += 4) {
-          const float4 f = *reinterpret_cast<const float4*>(entry + c);
+          const float4 f = load_scales(entry + 4 * c);
           ptx::fmul2(x[c], x[c + 1], x[c], x[c + 1], f.x, f.y);
           ptx::fmul2(x[c + 2], x[c + 3], x[c + 2], x[c + 3], f.z, f.w);
         }
-        // P * vs stays below 2^8 * 2^6: lv follows V's largest scale (the same for
-        // all threads); the first tile sets it
-        const float4 f0 = *reinterpret_cast<const float4*>(entry + 256);
-        const float4 f1 = *reinterpret_cast<const float4*>(entry + 260);
-        const float vm = fmaxf(fmaxf(fmaxf(f0.x, f0.y), fmaxf(f0.z, f0.w)),
-                               fmaxf(fmaxf(f1.x, f1.y), fmaxf(f1.z, f1.w)));
-        const float e = static_cast<float>(static_cast<int>(__float_as_uint(vm) >> 23) - 127);
-        if (j == 0 || e > lv + 5.f) lv_new = fmaxf(fminf(e, 100.f), -50.f);
       }
 
       const int key0 = (it.jb + j) * kBlockN;
@@ -666,11 +585,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
       const bool grow = m_new > m + kGrow;
       if (j == 0) {
         m = m_new;
-        lv = lv_new;
       } else {
-        if (__any_sync(0xffffffffu, grow) || (kScaled && lv_new != lv)) {
-          float alpha = grow ? ptx::ex2_approx(m - m_new) : 1.0f;
-          if constexpr (kScaled) alpha *= ptx::ex2_approx(lv - lv_new);
+        if (__any_sync(0xffffffffu, grow)) {
+          const float alpha = grow ? ptx::ex2_approx(m - m_new) : 1.0f;
 #pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
             uint32_t o[32];
@@ -688,17 +605,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
           }
           ptx::tmem_wait_st();
           l *= alpha;
-          lv = lv_new;
         }
         if (grow) m = m_new;
       }
-      const float neg_m = ((m == -INFINITY) ? 0.f : -m) - lv;
+      const float neg_m = (m == -INFINITY) ? 0.f : -m;
       const uint32_t half_bar = bar(L::kBarPH + g);
       auto announce = [half_bar] { ptx::mbar_arrive(half_bar); };
       float tile_sum;
       if constexpr (kScaled) {
-        tile_sum = masked ? exp_tile_scaled<false, kEmuPeriod>(x, sl_eff, neg_m, entry + 128, tP, announce)
-                          : exp_tile_scaled<true, kPairEmuPeriod<D>>(x, sl_eff, neg_m, entry + 128, tP, announce);
+        tile_sum = masked ? exp_tile_scaled<false, kEmuPeriod>(x, sl_eff, neg_m, entry + 512, tP, announce)
+                          : exp_tile_scaled<true, kPairEmuPeriod<D>>(x, sl_eff, neg_m, entry + 512, tP, announce);
       } else {
         tile_sum = masked ? exp_tile<kBf16, false>(x, sl_eff, neg_m, tP, announce)
                           : exp_tile<kBf16, true, kPairEmuPeriod<D>>(x, sl_eff, neg_m, tP, announce);
@@ -731,7 +647,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
         const float inv_l = (l > 0.f) ? 1.0f / l : (l == 0.f ? 0.f : l);  // (a NaN stays one)
         const float m_use = (m == -INFINITY) ? 0.f : m;
         const float lse_row =
-            l == 0.f ? -INFINITY : (m_use + lv + __log2f(l)) * 0.69314718055994530942f;
+            l == 0.f ? -INFINITY : (m_use + __log2f(l)) * 0.69314718055994530942f;
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           uint32_t o[32];
@@ -819,10 +735,123 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__
     a.lse[row % a.Hq * a.r.total + row / a.Hq] = sum == 0.f ? -INFINITY : mx + logf(sum);
 }
 
-template <int D, int KV, bool QBF16>
+// The visible keys and values of the chunk kernel's sequences as f16 rows:
+// sequence after sequence, each padded to 128 rows (the padding is zeros),
+// [n_heads][exp_rows][d] for K and for V, with the scales [n_heads][exp_rows] or,
+// for kFold, multiplied by them.  A warp takes groups of 16 keys of one head.
+constexpr int kExpandThreads = 128;
+
+template <int D, int KV, bool kFold>
+__global__ void __launch_bounds__(kExpandThreads) paged_expand_kernel(const __grid_constant__ ChunkParams p) {
+  const PagedAttn& a = p.a;
+  constexpr int L = D / 16;            // lanes per row: 8 bytes at 8 part and at d / 2 + 8 part
+  constexpr int kRows = 32 / L;        // rows per pass
+  constexpr int kPasses = 16 / kRows;
+  __shared__ long long sh_scan[kExpandThreads / 32];
+  __shared__ int sh_first[kExpandThreads];  // blocks before each thread's share of the sequences
+  const int lane = threadIdx.x & 31, part = lane % L;
+  const int share = (a.r.B + kExpandThreads - 1) / kExpandThreads;
+  auto blocks_of = [&](int b) {
+    const Seq s = load_seq(a, b);
+    return static_cast<long long>(s.nq) * a.group <= p.skip_rows ? 0 : expand_blocks(s);
+  };
+  long long total;
+  {
+    const int b0 = min(static_cast<int>(threadIdx.x) * share, a.r.B), b1 = min(b0 + share, a.r.B);
+    long long sum = 0;
+    for (int b = b0; b < b1; ++b) sum += blocks_of(b);
+    sh_first[threadIdx.x] = static_cast<int>(block_scan<kExpandThreads>(sum, sh_scan, &total));
+    __syncthreads();
+  }
+  // units: (block, group of 16 rows in it, head), heads fastest
+  const long long n_units = min(total * 8, p.exp_rows / 16) * p.n_heads;
+  for (long long u = static_cast<long long>(blockIdx.x) * (kExpandThreads / 32) + (threadIdx.x >> 5);
+       u < n_units; u += static_cast<long long>(gridDim.x) * (kExpandThreads / 32)) {
+    const int h = static_cast<int>(u % p.n_heads);
+    const long long grp = u / p.n_heads;
+    const int block = static_cast<int>(grp >> 3);
+    // its sequence: the last share that starts at or before the block, then on from there
+    int lo = 0;
+#pragma unroll
+    for (int step = kExpandThreads / 2; step > 0; step >>= 1)
+      if (sh_first[lo + step] <= block) lo += step;
+    int b = lo * share, first = sh_first[lo];
+    for (int n = blocks_of(b); b + 1 < a.r.B && block >= first + n; n = blocks_of(b)) {
+      first += n;
+      ++b;
+    }
+    const Seq s = load_seq(a, b);
+    const int pos = (block - first) * kBlockN + 16 * static_cast<int>(grp & 7);
+    const int left = s.vis - pos;  // rows that exist
+    const int page = left > 0 ? a.c.lookup(b, pos) : -1;
+    const long long prow = a.c.row_in_page(pos);
+    const int head = p.head0 + h;
+    const long long src0 = page * a.c.page_stride + head * a.c.head_stride + prow * a.c.row_stride;
+    const long long dst0 = static_cast<long long>(h) * p.exp_rows + static_cast<long long>(grp) * 16;
+    const long long sc0 = page * a.c.s_page + head * a.c.s_head + prow * a.c.s_row;
+    uint2 x[2][kPasses][2];
+    float sc[2][kPasses];
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+      for (int y = 0; y < kPasses; ++y) {
+        const int r = y * kRows + lane / L;
+        x[kv][y][0] = x[kv][y][1] = make_uint2(0u, 0u);
+        sc[kv][y] = 0.f;
+        if (page >= 0 && r < left) {
+          const uint2* src = reinterpret_cast<const uint2*>((kv ? a.c.v : a.c.k) + src0 + r * a.c.row_stride);
+          x[kv][y][0] = __ldg(src + part);
+          x[kv][y][1] = __ldg(src + D / 16 + part);
+          sc[kv][y] = __ldg((kv ? a.c.vs : a.c.ks) + sc0 + r * a.c.s_row);
+        }
+      }
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+      for (int y = 0; y < kPasses; ++y) {
+        const long long row = dst0 + y * kRows + lane / L;
+        uint4* dst = reinterpret_cast<uint4*>((kv ? p.exp_v : p.exp_k) + row * D) + part;
+        // V's scale = power * rest, rest in [1, 2) where power is in range
+        const float power = __uint_as_float(
+            min(max(__float_as_uint(sc[kv][y]) & 0x7f800000u, 0x33800000u), 0x43000000u));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          uint32_t w[4];
+          widen<KV, false>(x[kv][y][i].x, w[0], w[1]);
+          widen<KV, false>(x[kv][y][i].y, w[2], w[3]);
+          if (!kFold && kv) {
+            // exact: f16 holds 8-bit values times 2^-24 .. 2^7 (below 2^-24 they
+            // are smaller than any f16 result)
+            const __half2 p2 = __float2half2_rn(power);
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+              const __half2 f = __hmul2(*reinterpret_cast<__half2*>(&w[z]), p2);
+              w[z] = *reinterpret_cast<const uint32_t*>(&f);
+            }
+          }
+          if constexpr (kFold) {
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+              // beyond f16's range: its largest value
+              const float2 f = __half22float2(*reinterpret_cast<__half2*>(&w[z]));
+              const float f0 = f.x * sc[kv][y], f1 = f.y * sc[kv][y];
+              auto clamp = [](float v) { return v > 65504.f ? 65504.f : v < -65504.f ? -65504.f : v; };
+              w[z] = pack2<false>(clamp(f0), clamp(f1));
+            }
+          }
+          dst[i * (D / 16)] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        if constexpr (!kFold) {
+          if (part == 0) (kv ? p.exp_vs : p.exp_ks)[row] = kv ? sc[kv][y] / power : sc[kv][y];
+        }
+      }
+  }
+}
+
+template <int D, int SRC, bool QBF16>
 cudaError_t launch_chunk_impl(const ChunkParams& p, int grid, cudaStream_t stream) {
-  auto kern = paged_chunk_kernel<D, KV, QBF16>;
-  constexpr int kSmem = ChunkLayout<D, (KV >= FA_DTYPE_INT8)>::kDynBytes;
+  auto kern = paged_chunk_kernel<D, SRC, QBF16>;
+  using L = ChunkLayout<D, SRC == kExpanded && !QBF16>;
   static int attr_done[64] = {0};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -831,15 +860,58 @@ cudaError_t launch_chunk_impl(const ChunkParams& p, int grid, cudaStream_t strea
     cudaFuncAttributes fa{};
     cudaError_t e = cudaFuncGetAttributes(&fa, kern);
     if (e != cudaSuccess) return e;
-    if (fa.numRegs != kLaunchRegs || fa.maxThreadsPerBlock < kThreads)
-      return cudaErrorInvalidConfiguration;
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (fa.numRegs != kLaunchRegs || fa.maxThreadsPerBlock < kThreads) return cudaErrorInvalidConfiguration;
+    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kDynBytes);
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) attr_done[dev] = 1;
   }
-  kern<<<grid, kThreads, kSmem, stream>>>(p);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess || p.n_splits == 1) return e;
+  kern<<<grid, kThreads, L::kDynBytes, stream>>>(p);
+  return cudaGetLastError();
+}
+
+template <int D>
+cudaError_t launch_chunk_d(const ChunkParams& p, int kv, bool bf16, int grid, cudaStream_t s) {
+  switch (kv) {
+    case FA_DTYPE_INT8:
+    case FA_DTYPE_E4M3:
+      return bf16 ? launch_chunk_impl<D, kExpanded, true>(p, grid, s)
+                  : launch_chunk_impl<D, kExpanded, false>(p, grid, s);
+    case FA_DTYPE_BF16: return launch_chunk_impl<D, kPagesBf16, true>(p, grid, s);
+    default: return launch_chunk_impl<D, kPagesF16, false>(p, grid, s);
+  }
+}
+
+template <int D>
+cudaError_t launch_expand_d(const ChunkParams& p, int kv, bool fold, int grid, cudaStream_t s) {
+  if (kv == FA_DTYPE_INT8) {
+    if (fold) paged_expand_kernel<D, FA_DTYPE_INT8, true><<<grid, kExpandThreads, 0, s>>>(p);
+    else paged_expand_kernel<D, FA_DTYPE_INT8, false><<<grid, kExpandThreads, 0, s>>>(p);
+  } else {
+    if (fold) paged_expand_kernel<D, FA_DTYPE_E4M3, true><<<grid, kExpandThreads, 0, s>>>(p);
+    else paged_expand_kernel<D, FA_DTYPE_E4M3, false><<<grid, kExpandThreads, 0, s>>>(p);
+  }
+  return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_paged_chunk(const ChunkParams& p, int head_dim, int kv, bool bf16, int grid, int sms,
+                               cudaStream_t stream) {
+  if (kv >= FA_DTYPE_INT8) {
+    // enough warps to fill the GPU; they walk the rows there are
+    const long long units = p.exp_rows / 16 * p.n_heads;
+    const long long most = static_cast<long long>(sms) * 12;
+    const long long blocks = (units + kExpandThreads / 32 - 1) / (kExpandThreads / 32);
+    const int g = static_cast<int>(blocks < most ? blocks : most);
+    const cudaError_t e = head_dim == 64 ? launch_expand_d<64>(p, kv, bf16, g, stream)
+                                         : launch_expand_d<128>(p, kv, bf16, g, stream);
+    if (e != cudaSuccess) return e;
+  }
+  return head_dim == 64 ? launch_chunk_d<64>(p, kv, bf16, grid, stream)
+                        : launch_chunk_d<128>(p, kv, bf16, grid, stream);
+}
+
+cudaError_t launch_paged_join(const ChunkParams& p, int head_dim, bool bf16, cudaStream_t stream) {
   cudaLaunchConfig_t cfg{};
   const long long n_all = static_cast<long long>(p.a.r.total) * p.a.Hq;
   cfg.gridDim = dim3(static_cast<unsigned>((n_all + 7) / 8));
@@ -850,29 +922,11 @@ cudaError_t launch_chunk_impl(const ChunkParams& p, int grid, cudaStream_t strea
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_join_kernel<D, QBF16>, p);
-}
-
-template <int D>
-cudaError_t launch_chunk_d(const ChunkParams& p, int kv, bool bf16, int grid, cudaStream_t s) {
-  switch (kv) {
-    case FA_DTYPE_INT8:
-      return bf16 ? launch_chunk_impl<D, FA_DTYPE_INT8, true>(p, grid, s)
-                  : launch_chunk_impl<D, FA_DTYPE_INT8, false>(p, grid, s);
-    case FA_DTYPE_E4M3:
-      return bf16 ? launch_chunk_impl<D, FA_DTYPE_E4M3, true>(p, grid, s)
-                  : launch_chunk_impl<D, FA_DTYPE_E4M3, false>(p, grid, s);
-    case FA_DTYPE_BF16: return launch_chunk_impl<D, FA_DTYPE_BF16, true>(p, grid, s);
-    default: return launch_chunk_impl<D, FA_DTYPE_F16, false>(p, grid, s);
-  }
-}
-
-}  // namespace
-
-cudaError_t launch_paged_chunk(const ChunkParams& p, int head_dim, int kv, bool bf16, int grid,
-                               cudaStream_t stream) {
-  return head_dim == 64 ? launch_chunk_d<64>(p, kv, bf16, grid, stream)
-                        : launch_chunk_d<128>(p, kv, bf16, grid, stream);
+  if (head_dim == 64)
+    return bf16 ? cudaLaunchKernelEx(&cfg, paged_join_kernel<64, true>, p)
+                : cudaLaunchKernelEx(&cfg, paged_join_kernel<64, false>, p);
+  return bf16 ? cudaLaunchKernelEx(&cfg, paged_join_kernel<128, true>, p)
+              : cudaLaunchKernelEx(&cfg, paged_join_kernel<128, false>, p);
 }
 
 }  // namespace fa
