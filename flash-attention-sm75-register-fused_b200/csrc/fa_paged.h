@@ -104,7 +104,9 @@ struct alignas(64) DecodeParams {
   CUtensorMap tm_v;
   PagedAttn a;
   float* ws;
-  int n_teams;   // teams of the launch, set by launch_paged_decode
+  // set by launch_paged_decode: teams of the launch, one CTA per (sequence,
+  // head), ring stages per warp
+  int n_teams, solo, stages;
   int max_rows;  // query rows per KV head of the sequences handled
   unsigned epoch;
   unsigned long long timeout_ns;
@@ -114,7 +116,7 @@ struct alignas(64) DecodeParams {
 // rows (new tokens x group) per KV head, and the rows of sequences without
 // visible keys or of no sequence.  Sequences with more rows are left alone.
 int paged_decode_rows();
-size_t paged_decode_ws_bytes(int max_rows, int head_dim, int sms);
+size_t paged_decode_ws_bytes(int max_rows, int max_k, int head_dim, int cache_dtype, int sms);
 cudaError_t launch_paged_decode(DecodeParams p, int head_dim, int cache_dtype, bool bf16, int sms,
                                 cudaStream_t stream);
 // Chunk kernel (after the expansion of 8-bit pages) over the KV heads of p, and

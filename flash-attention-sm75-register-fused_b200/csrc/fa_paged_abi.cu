@@ -91,15 +91,16 @@ struct PagedPlan {
   long long exp_rows = 0;
   int exp_heads = 0;
   size_t exp_row_bytes = 0, exp_scale_bytes = 0;
-  size_t ws_decode = 0, ws_o = 0, ws_lse = 0, ws_bytes = 16;
+  size_t ws_decode = 0, ws_o = 0, ws_lse = 0, ws_bytes = 0;
 };
 
 // Expanded keys and values are at most this large where several KV heads would
 // make them larger: the heads then go through the chunk kernel in groups.
 constexpr size_t kExpandBytes = size_t{1} << 30;
 
-PagedPlan make_paged_plan(int B, int heads, int group, int head_dim, bool eight, int total, int max_q,
+PagedPlan make_paged_plan(int B, int heads, int group, int head_dim, int dtype, int total, int max_q,
                           int max_k) {
+  const bool eight = is_8bit(dtype);
   PagedPlan k;
   const int sms = fa::host_sm_count();
   const long long rows = static_cast<long long>(max_q) * group;
@@ -108,7 +109,7 @@ PagedPlan make_paged_plan(int B, int heads, int group, int head_dim, bool eight,
   k.decode = !k.chunk || (rows > cap && B > 1 && group <= kMixedRows &&
                           total < static_cast<long long>(B) * max_q);
   k.decode_rows = k.chunk ? (kMixedRows / group) * group : static_cast<int>(rows);
-  if (k.decode) k.ws_decode = fa::paged_decode_ws_bytes(k.decode_rows, head_dim, sms);
+  if (k.decode) k.ws_decode = fa::paged_decode_ws_bytes(k.decode_rows, max_k, head_dim, dtype, sms);
   if (k.chunk) {
     k.tq = 128 / group;
     const int pair = 2 * k.tq;
@@ -152,7 +153,6 @@ PagedPlan make_paged_plan(int B, int heads, int group, int head_dim, bool eight,
       k.ws_o + k.ws_lse + 2 * static_cast<size_t>(k.exp_heads) * (k.exp_row_bytes + k.exp_scale_bytes);
   // (the kernels run one after another, so they share the workspace)
   k.ws_bytes = k.ws_decode > chunk_bytes ? k.ws_decode : chunk_bytes;
-  if (k.ws_bytes < 16) k.ws_bytes = 16;
   return k;
 }
 
@@ -316,10 +316,10 @@ int fa_kvcache_read(const fa_paged_cache* cache, void* K, void* V, const int* cu
 
 size_t fa_fwd_paged_workspace_bytes(const fa_paged_cache* cache, int B, int Hq, int total_q,
                                     int max_seqlen_q, int max_seqlen_k) {
-  if (!cache || cache->kv_heads <= 0 || Hq <= 0 || total_q <= 0) return 16;
+  if (!cache || cache->kv_heads <= 0 || Hq <= 0 || total_q <= 0) return 0;
   const int group = Hq / cache->kv_heads > 0 ? Hq / cache->kv_heads : 1;
-  if (group > 128 || B < 0 || max_seqlen_q < 0 || max_seqlen_k < 0) return 16;  // refused sizes
-  return make_paged_plan(B, cache->kv_heads, group, cache->head_dim, is_8bit(cache->dtype), total_q,
+  if (group > 128 || B < 0 || max_seqlen_q < 0 || max_seqlen_k < 0) return 0;  // refused sizes
+  return make_paged_plan(B, cache->kv_heads, group, cache->head_dim, cache->dtype, total_q,
                          max_seqlen_q, max_seqlen_k)
       .ws_bytes;
 }
@@ -338,15 +338,15 @@ int fa_fwd_paged(const fa_paged_cache* cache, const void* Q, long long q_token_s
   if (Hq == 0 || total_q == 0) return FA_OK;
   if (Hq % a.c.heads != 0) return FA_ERR_GQA_DIVISIBILITY;
   if (Hq / a.c.heads > 128) return FA_ERR_GROUP;
-  if (!Q || !O || !workspace) return FA_ERR_INVALID_ARG;
+  if (!Q || !O) return FA_ERR_INVALID_ARG;
   if (!aligned16(Q) || !aligned16(O) || !aligned16(workspace) ||
       ((q_token_stride | q_head_stride) & 7) || (reinterpret_cast<uintptr_t>(lse) & 3u))
     return FA_ERR_ALIGNMENT;
   const int group = Hq / a.c.heads;
   const bool eight = is_8bit(cache->dtype);
-  const PagedPlan k = make_paged_plan(B, a.c.heads, group, cache->head_dim, eight, total_q, max_seqlen_q,
+  const PagedPlan k = make_paged_plan(B, a.c.heads, group, cache->head_dim, cache->dtype, total_q, max_seqlen_q,
                                       max_seqlen_k);
-  if (workspace_bytes < k.ws_bytes) return FA_ERR_INVALID_ARG;
+  if (k.ws_bytes > 0 && (!workspace || workspace_bytes < k.ws_bytes)) return FA_ERR_INVALID_ARG;
   const long long grid = static_cast<long long>(k.slots) * a.c.heads * k.n_splits;  // of all heads
   if (grid > 0x7fffffffLL || static_cast<long long>(B) * a.c.heads > 0x7fffffffLL ||
       static_cast<long long>(total_q) * Hq > (1LL << 33))

@@ -34,6 +34,10 @@
 // its unnormalised O, m and l go to one of its two workspace slots (its run's
 // first part, which continues a head of the team before, or its last, which
 // the next team continues) and paged_combine_kernel joins them in order.
+//
+// Short caches (DecodeParams::solo: at most 8 units per team) take one CTA per
+// (sequence, head) instead, whose teams share its units and join in shared
+// memory: one launch, no workspace, no plan over the batch.
 #include "fa_paged.h"
 #include "fa_paged_dev.cuh"
 
@@ -48,9 +52,11 @@ constexpr int kCombineThreads = 256;
 // maxima are never NaN, and below any score.
 constexpr float kNoMax = -1e30f;
 
-// NT: 8-row column blocks of a warp.
+// NT: 8-row column blocks of a warp.  Ring stages per warp: as many as the CTAs
+// that share an SM leave room for.
+constexpr int kMaxStages = 6;
 __host__ __device__ constexpr int ctas_per_sm(int nt) { return nt == 1 ? 3 : 2; }
-__host__ __device__ constexpr int stages_per_warp(int nt) { return nt == 1 ? 2 : 3; }
+constexpr int stages_per_warp(int nt) { return nt == 1 ? 2 : 3; }
 
 template <int D, int KV>
 struct Cfg {
@@ -64,9 +70,7 @@ struct Cfg {
   static constexpr int kBoxes = 2 * kCols * kMT;       // of a unit: (K, V) x columns x groups
   static constexpr int kKS = D / 16;                   // 16-column steps of d
   static constexpr int kScaleBytes = k8 ? kSub * 8 : 0;
-  __host__ __device__ static constexpr int smem(int nt) {
-    return 1024 + kWarps * stages_per_warp(nt) * (8192 + kScaleBytes);
-  }
+  static constexpr int smem(int stages) { return 1024 + kWarps * stages * (8192 + kScaleBytes); }
   // Address of 16-byte piece c of row r of a K or V half stage: boxes of 16
   // rows in the TMA swizzle (128-byte rows: piece ^ row % 8; 64-byte rows:
   // piece ^ (row / 2) % 4), so eight rows at one piece hit eight bank groups.
@@ -163,6 +167,52 @@ __host__ __device__ constexpr long long slot_floats(int rows, int d) {
   return static_cast<long long>(rows) * (d + 2);
 }
 
+// O = 0, LSE = -inf in the packed rows of no sequence (before the first and
+// after the last), dealt over the grid's blocks.
+__device__ __forceinline__ void fill_outside(const PagedAttn& a, int d, int block, int n_blocks) {
+  const int head = min(max(__ldg(a.r.cu), 0), a.r.total);
+  const int tail = min(max(__ldg(a.r.cu + a.r.B), head), a.r.total);
+  const int n_out = head + a.r.total - tail;
+  const int n = static_cast<int>(blockDim.x), words = a.Hq * d / 2;
+  for (int x = block; x < n_out; x += n_blocks) {
+    const int t = x < head ? x : tail + x - head;
+    for (int i = threadIdx.x; i < words; i += n)
+      static_cast<uint32_t*>(a.o)[static_cast<long long>(t) * words + i] = 0u;
+    if (a.lse != nullptr)
+      for (int i = threadIdx.x; i < a.Hq; i += n)
+        a.lse[static_cast<long long>(i) * a.r.total + t] = -INFINITY;
+  }
+}
+
+// Partial result of a row over a lane's D / 32 columns.
+template <int D>
+struct Partial {
+  static constexpr int E = D / 32;
+  float m = kNoMax, l = 0.f, o[E] = {};
+  __device__ __forceinline__ void add(float mi, float li, const float (&v)[E]) {
+    const float mn = fmaxf(m, mi);
+    const float f0 = exp2f(m - mn), f1 = exp2f(mi - mn);
+    m = mn;
+    l = l * f0 + li * f1;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = o[e] * f0 + v[e] * f1;
+  }
+  // the warp writes the row
+  template <bool BF16>
+  __device__ __forceinline__ void write(const PagedAttn& a, int tok, int hq) const {
+    const int lane = threadIdx.x & 31;
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.o) +
+                                                (static_cast<long long>(tok) * a.Hq + hq) * D) +
+                    lane * (E / 2);
+#pragma unroll
+    for (int e = 0; e < E; e += 2) dst[e / 2] = pack2<BF16>(o[e] * inv, o[e + 1] * inv);
+    if (lane == 0 && a.lse != nullptr)
+      a.lse[static_cast<long long>(hq) * a.r.total + tok] =
+          l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
+  }
+};
+
 // Place of a team in its run: unit t of n of (sequence b, head h), position v.
 struct Cursor {
   Seq s;
@@ -174,14 +224,14 @@ template <int D, int KV, bool QBF16, int NT, int TEAM>
 __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
     paged_decode_kernel(const __grid_constant__ DecodeParams p) {
   using C = Cfg<D, KV>;
-  constexpr int kStages = stages_per_warp(NT) * TEAM;
+  const int stages = p.stages * TEAM;  // of a team
   constexpr int kTeams = kWarps / TEAM;
   const PagedAttn& a = p.a;
   extern __shared__ uint8_t smem_raw[];
   __shared__ long long sh_scan[kWarps];
   __shared__ int sh_b[kTeams];
   __shared__ long long sh_rel[kTeams];
-  __shared__ __align__(8) unsigned long long sh_bar[kTeams * kStages];
+  __shared__ __align__(8) unsigned long long sh_bar[kWarps * kMaxStages];
   __shared__ int sh_abort;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, j = lane & 3;
@@ -197,13 +247,23 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
     sh_abort = ((st >> 32) == p.epoch && (st & 0xffffffffull) != 0ull) ? 1 : 0;
     // a stage is full when its boxes have landed (and, 8-bit pages, the 32
     // lanes' scales)
-    for (int i = 0; i < kTeams * kStages; ++i)
+    for (int i = 0; i < kTeams * stages; ++i)
       ptx::mbar_init(ptx::smem_u32(&sh_bar[i]), C::k8 ? 33u : 1u);
     ptx::fence_barrier_init();
   }
   long long v1, rel;
   int b_first;
-  {
+  if (p.solo) {
+    // the teams take equal parts of the units of (sequence, head) blockIdx.x
+    fill_outside(a, D, static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
+    b_first = static_cast<int>(blockIdx.x) / H;
+    const int n = (load_short(a, b_first, p.max_rows).vis + C::kSub - 1) / C::kSub;
+    const long long base = static_cast<long long>(static_cast<int>(blockIdx.x) % H) * (n + kSegCost) + kSegCost;
+    rel = base + static_cast<long long>(n) * team / kTeams;
+    v1 = base + static_cast<long long>(n) * (team + 1) / kTeams;
+    __syncthreads();
+    if (*abort_flag) return;
+  } else {
     const int share = (a.r.B + 32 * kWarps - 1) / (32 * kWarps);
     const int s0 = min(static_cast<int>(threadIdx.x) * share, a.r.B), s1 = min(s0 + share, a.r.B);
     long long sum = 0, total;
@@ -265,8 +325,15 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
     seek(c, c.b + 1);
   };
   Cursor cc;  // unit being computed
-  seek(cc, b_first);
-  {
+  if (p.solo) {
+    cc.s = load_short(a, b_first, p.max_rows);
+    cc.n = (cc.s.vis + C::kSub - 1) / C::kSub;
+    cc.b = b_first;
+    cc.h = static_cast<int>(blockIdx.x) % H;
+    cc.t = static_cast<int>(static_cast<long long>(cc.n) * team / kTeams);
+    cc.v = rel;
+  } else {
+    seek(cc, b_first);
     const long long seg = cc.n + kSegCost;
     cc.h = static_cast<int>(rel / seg);
     cc.t = max(static_cast<int>(rel % seg) - kSegCost, 0);
@@ -278,28 +345,45 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
   // ---- loads
   uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                                    ~static_cast<uintptr_t>(1023)) +
-                        team * kStages * 8192;
+                        team * stages * 8192;
   const uint32_t ring = ptx::smem_u32(smem);
   // scales of all stages behind the data of all teams: per key K's, V's
-  const uint32_t sring = ring + (kWarps * stages_per_warp(NT) - team * kStages) * 8192 +
-                         team * kStages * C::kScaleBytes;
-  const uint32_t bars = ptx::smem_u32(&sh_bar[team * kStages]);
+  const uint32_t sring = ring + (kWarps * p.stages - team * stages) * 8192 +
+                         team * stages * C::kScaleBytes;
+  const uint32_t bars = ptx::smem_u32(&sh_bar[team * stages]);
   const uint64_t policy = ptx::policy_evict_first();  // every key is read once
   // lane = (group * kCols + column) * 2 + (0: K, 1: V)
   const int bgrp = lane / (2 * C::kCols), bcol = (lane >> 1) % C::kCols;
   const bool boxes = lane < C::kBoxes;
   const uint32_t box_dst = (lane & 1) * 4096 + (C::kCols == 2 ? bcol * 2048 : bgrp * 16 * C::kRowBytes);
   const void* const box_map = (lane & 1) ? &p.tm_v : &p.tm_k;
-  auto page_of_box = [&] {  // -1 (no key any row may see, or no page) reads as zeros
-    const int pos = ci.t * C::kSub + 16 * bgrp;
-    return boxes && pos < ci.s.vis ? a.c.lookup(ci.b, pos) : -1;
+  // Pages of the 16-key groups around ci: lane l holds that of group wbase + l
+  // in `win` and of group wbase + 32 + l in `win_next`, loaded 32 groups ahead,
+  // so a unit's pages are shuffles.  -1 (no key any row may see, or no page)
+  // reads as zeros.
+  int wbase = 0, win = -1, win_next = -1;
+  auto load_window = [&](int first) {
+    const int pos = 16 * (first + lane);
+    return pos < ci.s.vis ? a.c.lookup(ci.b, pos) : -1;
   };
-  int page = -1;
+  auto start_window = [&] {  // at the first unit of the run in a segment
+    wbase = ci.t * C::kMT;
+    win = load_window(wbase);
+    win_next = load_window(wbase + 32);
+  };
   int wstage = 0;
   auto issue = [&] {
     if (ci.v >= v1) return;
     const uint32_t bar = bars + 8 * wstage;
     const int key0 = ci.t * C::kSub;
+    int g0 = ci.t * C::kMT - wbase;  // the unit's first group in the window
+    if (g0 >= 32) {
+      g0 -= 32;
+      wbase += 32;
+      win = win_next;
+      win_next = load_window(wbase + 32);
+    }
+    const int page = __shfl_sync(0xffffffffu, win, g0 + (boxes ? bgrp : 0));
     if (lane == 0) ptx::mbar_arrive_expect_tx(bar, 8192);
     __syncwarp();
     if (boxes)
@@ -310,7 +394,7 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
 #pragma unroll
       for (int x = 0; x < C::kSub / 32; ++x) {
         const int r = x * 32 + lane;
-        const int pg = __shfl_sync(0xffffffffu, page, (r >> 4) * 2);
+        const int pg = __shfl_sync(0xffffffffu, win, g0 + (r >> 4));
         const bool ok = r < left && pg >= 0;
         const long long o =
             ok ? static_cast<long long>(pg) * a.c.s_page + ci.h * a.c.s_head +
@@ -322,13 +406,13 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
       }
       ptx::cp_async_arrive(bar);
     }
-    if (++wstage == kStages) wstage = 0;
+    if (++wstage == stages) wstage = 0;
     advance(ci);
-    if (ci.v < v1) page = page_of_box();
+    if (ci.t == 0 && ci.v < v1) start_window();
   };
   if (trank == 0) {
-    page = page_of_box();
-    for (int x = 0; x < kStages - 1; ++x) issue();
+    start_window();
+    for (int x = 0; x < stages - 1; ++x) issue();
   }
 
   // ---- the segments (sequence, head) of the run
@@ -426,14 +510,21 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
     int lv = C::k8 ? -60 : 0;
 
     for (int t = t_begin; t < t_end; ++t) {
-      ok = bar_wait(bars + 8 * rstage, rphase, wc, 50);
-      // (also: every warp is done with the stage before, which is refilled now)
-      if (!(ok = team_ok(ok))) break;
+      // Every warp is done with the stage before, which is refilled now, before
+      // the wait for this one: two units are in flight while the team waits.
+      // (A warp whose wait fails releases the others once, at their next
+      // barrier, and after a barrier that reports it no warp calls another.)
+      if (!(ok = team_ok(true))) break;
       if (trank == 0) issue();
+      if (!__all_sync(0xffffffffu, bar_wait(bars + 8 * rstage, rphase, wc, 50))) {
+        team_ok(false);
+        ok = false;
+        break;
+      }
       const uint32_t st = ring + rstage * 8192;
       const uint32_t sst = sring + rstage * C::kScaleBytes;
       uint8_t* const stage = smem + rstage * 8192;
-      if (++rstage == kStages) {
+      if (++rstage == stages) {
         rstage = 0;
         rphase ^= 1u;
       }
@@ -462,15 +553,23 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
 #pragma unroll
           for (int i = 0; i < 4; ++i) sc[nt][mt][i] = 0.f;
         if constexpr (!C::k8) {
+          // (two accumulation chains: a unit of one key group would wait for
+          // every product in turn)
           const int r = mt * 16 + (lane & 15);
+          float odd[NT][4] = {};
 #pragma unroll
           for (int k = 0; k < C::kKS; ++k) {
             uint32_t f[4];
             ldsm4(st + C::piece(r, 2 * k + (lane >> 4)), f);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              mma16816<C::kBf16>(sc[nt][mt], f[0], f[1], f[2], f[3], q[nt][k][0], q[nt][k][1]);
+              mma16816<C::kBf16>((k & 1) ? odd[nt] : sc[nt][mt], f[0], f[1], f[2], f[3], q[nt][k][0],
+                                 q[nt][k][1]);
           }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sc[nt][mt][i] += odd[nt][i];
         } else {
           // two 16-column steps per ldmatrix: keys 0-7 and 8-15 of pieces k, k + 1
           const int r = mt * 16 + (lane & 15);
@@ -621,6 +720,11 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
 
     // ---- the segment's result
     const bool first = t_begin == 0, last = t_end == n_units;
+    constexpr int kSlotRows = 8 * NT * TEAM;
+    // (solo: the team's part of the ring, once all its warps have read it)
+    float* const slot = p.solo ? reinterpret_cast<float*>(smem)
+                               : p.ws + (2ll * tid + (first ? 1 : 0)) * slot_floats(kSlotRows, D);
+    if (p.solo && !(ok = team_ok(true))) break;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -640,7 +744,7 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
       for (int c = 0; c < 2; ++c) {
         const int r = row0 + nt * 8 + 2 * j + c;
         if (r >= rows) continue;
-        if (first && last) {
+        if (first && last && !p.solo) {
           const int tok = s.c0 + r / a.group, hq = cc.h * a.group + r % a.group;
           const float inv = l[nt][c] == 0.f ? 0.f : 1.f / l[nt][c];
           uint16_t* dst = static_cast<uint16_t*>(a.o) + (static_cast<long long>(tok) * a.Hq + hq) * D;
@@ -659,8 +763,6 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
                 l[nt][c] == 0.f ? -INFINITY : (m[nt][c] + __log2f(l[nt][c])) * 0.69314718055994530942f;
         } else {
           // slot 0: continues the head of an earlier team; slot 1: begins one
-          constexpr int kSlotRows = 8 * NT * TEAM;
-          float* slot = p.ws + (2ll * tid + (first ? 1 : 0)) * slot_floats(kSlotRows, D);
 #pragma unroll
           for (int k = 0; k < C::kKS; ++k) {
             slot[r * D + col(k, 0)] = o[nt][k][c];
@@ -677,17 +779,37 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
     cc.t = t_end - 1;
     advance(cc);
   }
+  if (ok) ok = team_ok(true);  // (the barrier a failed last wait releases)
   // after a failed wait: copies in flight land before the CTA exits
   if (!ok && trank == 0) {
-    for (int x = 0; x < kStages; ++x) {
+    for (int x = 0; x < stages; ++x) {
       bar_wait(bars + 8 * rstage, rphase, wc, 51, false);
-      if (++rstage == kStages) {
+      if (++rstage == stages) {
         rstage = 0;
         rphase ^= 1u;
       }
       if (rstage == wstage) break;
     }
     ptx::cp_async_wait_all();
+  }
+  if (p.solo) {
+    if (__syncthreads_and(ok ? 1 : 0) == 0) return;
+    // one warp joins a row of the teams' slots
+    constexpr int kSlotRows = 8 * NT * TEAM;
+    const Seq s = load_short(a, b_first, p.max_rows);
+    const int n = (s.vis + C::kSub - 1) / C::kSub, h = static_cast<int>(blockIdx.x) % H;
+    for (int row = warp; row < s.nq * a.group; row += kWarps) {
+      Partial<D> all;
+      for (int w = 0; w < kTeams; ++w) {
+        if (static_cast<long long>(n) * w / kTeams == static_cast<long long>(n) * (w + 1) / kTeams) continue;
+        const float* sl = reinterpret_cast<const float*>(smem + (w - team) * (stages * 8192));
+        float v[Partial<D>::E];
+#pragma unroll
+        for (int e = 0; e < Partial<D>::E; ++e) v[e] = sl[row * D + lane * Partial<D>::E + e];
+        all.add(sl[kSlotRows * D + row], sl[kSlotRows * D + kSlotRows + row], v);
+      }
+      all.template write<QBF16>(a, s.c0 + row / a.group, h * a.group + row % a.group);
+    }
   }
 }
 
@@ -702,20 +824,6 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
 // sequences without visible keys and packed rows of no sequence.
 constexpr int kManySlots = 32;
 
-template <int D>
-struct Partial {
-  static constexpr int E = D / 32;  // columns of a lane
-  float m = kNoMax, l = 0.f, o[E] = {};
-  __device__ __forceinline__ void add(float mi, float li, const float (&v)[E]) {
-    const float mn = fmaxf(m, mi);
-    const float f0 = exp2f(m - mn), f1 = exp2f(mi - mn);
-    m = mn;
-    l = l * f0 + li * f1;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = o[e] * f0 + v[e] * f1;
-  }
-};
-
 template <int D, bool BF16, int kRows>
 __global__ void __launch_bounds__(kCombineThreads)
     paged_combine_kernel(const __grid_constant__ DecodeParams p, int sub, int slot_rows) {
@@ -727,22 +835,8 @@ __global__ void __launch_bounds__(kCombineThreads)
   __shared__ float sh_m[kW], sh_l[kW];
   const int b = blockIdx.x / a.c.heads, h = blockIdx.x % a.c.heads;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  uint16_t* out = static_cast<uint16_t*>(a.o);
-  // rows of no sequence: before the first and after the last
-  {
-    const int head = min(max(__ldg(a.r.cu), 0), a.r.total);
-    const int tail = min(max(__ldg(a.r.cu + a.r.B), head), a.r.total);
-    const int n_out = head + a.r.total - tail;
-    const int id = static_cast<int>(blockIdx.y * gridDim.x + blockIdx.x);
-    for (int x = id; x < n_out; x += static_cast<int>(gridDim.x * gridDim.y)) {
-      const int t = x < head ? x : tail + x - head;
-      for (int i = threadIdx.x; i < a.Hq * D / 2; i += kCombineThreads)
-        reinterpret_cast<uint32_t*>(out)[static_cast<long long>(t) * (a.Hq * D / 2) + i] = 0u;
-      if (a.lse != nullptr)
-        for (int i = threadIdx.x; i < a.Hq; i += kCombineThreads)
-          a.lse[static_cast<long long>(i) * a.r.total + t] = -INFINITY;
-    }
-  }
+  fill_outside(a, D, static_cast<int>(blockIdx.y * gridDim.x + blockIdx.x),
+               static_cast<int>(gridDim.x * gridDim.y));
   const Seq s = load_short(a, b, p.max_rows);
   const Spot sp = find_spot<kCombineThreads>(a, sub, p.max_rows, b, sh);
   // the decode kernel's results are complete and visible after this
@@ -794,17 +888,8 @@ __global__ void __launch_bounds__(kCombineThreads)
     }
     return acc;
   };
-  // one warp writes a row
   auto finish = [&](int row, const Partial<D>& r) {
-    const int tok = s.c0 + row / a.group, hq = h * a.group + row % a.group;
-    const float inv = r.l == 0.f ? 0.f : 1.f / r.l;
-    uint32_t* dst =
-        reinterpret_cast<uint32_t*>(out + (static_cast<long long>(tok) * a.Hq + hq) * D) + lane * (E / 2);
-#pragma unroll
-    for (int e = 0; e < E; e += 2) dst[e / 2] = pack2<BF16>(r.o[e] * inv, r.o[e + 1] * inv);
-    if (lane == 0 && a.lse != nullptr)
-      a.lse[static_cast<long long>(hq) * a.r.total + tok] =
-          r.l == 0.f ? -INFINITY : (r.m + log2f(r.l)) * 0.69314718055994530942f;
+    r.template write<BF16>(a, s.c0 + row / a.group, h * a.group + row % a.group);
   };
   if (kRows > 1 && w1 - w0 < kManySlots) {
     for (int r = warp; r < rows; r += kW) finish(row0 + r, gather(row0 + r, 0, 1));
@@ -843,13 +928,13 @@ cudaError_t launch_impl(const DecodeParams& p, int n_ctas, cudaStream_t stream) 
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !attr_done[dev]) {
     const cudaError_t e =
-        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::smem(NT));
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::smem(kMaxStages));
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) attr_done[dev] = 1;
   }
-  kern<<<n_ctas, 32 * kWarps, C::smem(NT), stream>>>(p);
+  kern<<<n_ctas, 32 * kWarps, C::smem(p.stages), stream>>>(p);
   cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
+  if (e != cudaSuccess || p.solo) return e;
   // the combine may start while the last teams finish; it waits for them
   // before it reads a slot
   cudaLaunchConfig_t cfg{};
@@ -903,7 +988,18 @@ cudaError_t launch_d(const DecodeParams& p, int kv, bool bf16, int n_ctas, cudaS
 
 int paged_decode_rows() { return pdec::kRowsMax; }
 
-size_t paged_decode_ws_bytes(int max_rows, int head_dim, int sms) {
+namespace {
+namespace pdec {
+// Few units per (sequence, head): one CTA each, joined in shared memory.
+bool is_solo(int max_rows, int max_k, int head_dim, int kv) {
+  const int sub = 4096 / (head_dim * (kv >= FA_DTYPE_INT8 ? 1 : 2));
+  return (static_cast<long long>(max_k) + sub - 1) / sub <= 8 * (kWarps / team_for(max_rows).warps);
+}
+}  // namespace pdec
+}  // namespace
+
+size_t paged_decode_ws_bytes(int max_rows, int max_k, int head_dim, int kv, int sms) {
+  if (pdec::is_solo(max_rows, max_k, head_dim, kv)) return 0;
   const pdec::Team t = pdec::team_for(max_rows);
   const size_t teams = static_cast<size_t>(sms) * pdec::ctas_per_sm(t.nt) * (pdec::kWarps / t.warps);
   return 2 * teams * static_cast<size_t>(pdec::slot_floats(8 * t.nt * t.warps, head_dim)) * sizeof(float);
@@ -921,6 +1017,13 @@ cudaError_t launch_paged_decode(DecodeParams p, int head_dim, int kv, bool bf16,
   const long long most = static_cast<long long>(sms) * pdec::ctas_per_sm(t.nt);
   ctas = ctas > most ? most : ctas < 1 ? 1 : ctas;
   p.n_teams = static_cast<int>(ctas) * per_cta;
+  p.solo = pdec::is_solo(p.max_rows, p.a.max_k, head_dim, kv) ? 1 : 0;
+  p.stages = pdec::stages_per_warp(t.nt);
+  if (p.solo) {
+    ctas = static_cast<long long>(p.a.r.B) * p.a.c.heads;
+    if (ctas <= sms) p.stages = pdec::kMaxStages;
+    else if (ctas <= 2LL * sms) p.stages = 3;
+  }
   return head_dim == 64 ? pdec::launch_d<64>(p, kv, bf16, static_cast<int>(ctas), stream)
                         : pdec::launch_d<128>(p, kv, bf16, static_cast<int>(ctas), stream);
 }

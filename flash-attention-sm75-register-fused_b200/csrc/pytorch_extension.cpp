@@ -651,14 +651,15 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> flash_attention_forward_
   if (q.numel() == 0) return {O, lse};
   const int mq = static_cast<int>(max_seqlen_q), mk = static_cast<int>(max_seqlen_k);
   const size_t ws_bytes = fa_fwd_paged_workspace_bytes(&c, B, Hq, total, mq, mk);
-  auto ws = torch::empty({static_cast<int64_t>(ws_bytes > 0 ? ws_bytes : 16)},
-                         q.options().dtype(torch::kUInt8));
+  torch::Tensor ws;
+  if (ws_bytes > 0)
+    ws = torch::empty({static_cast<int64_t>(ws_bytes)}, q.options().dtype(torch::kUInt8));
   const int rc = fa_fwd_paged(&c, q.data_ptr(), stride_of(q, 0), stride_of(q, 1), O.data_ptr(),
                               want_lse ? lse->data_ptr<float>() : nullptr, cu.data_ptr<int>(),
                               B > 0 ? lens.data_ptr<int>() : nullptr, B, Hq, total, mq, mk, scale,
                               static_cast<int>(causal),
                               q.scalar_type() == torch::kBFloat16 ? FA_DTYPE_BF16 : FA_DTYPE_F16,
-                              ws.data_ptr(), ws_bytes, stream_of(q));
+                              ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes, stream_of(q));
   TORCH_CHECK(rc == FA_OK, "flash_attention_forward_paged: ", fa_error_string(rc));
   return {O, lse};
 }

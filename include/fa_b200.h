@@ -301,8 +301,8 @@ int fa_kvcache_read(const fa_paged_cache* cache, void* K, void* V, const int* cu
  * `dtype` (f16 / bf16) is that of Q and O; a 16-bit cache has the same.
  * max_seqlen_q / max_seqlen_k bound n_b and seqlens_k (tokens and keys beyond
  * them are not computed / not seen).  Hq / kv_heads is at most 128.
- * `workspace` (16-byte aligned) needs fa_fwd_paged_workspace_bytes() bytes.
- * Asynchronous on `stream`.
+ * `workspace` (16-byte aligned) needs fa_fwd_paged_workspace_bytes() bytes (may
+ * be NULL where that is 0).  Asynchronous on `stream`.
  *
  * No reference counterpart (reference llama_attention_replacement.py:63-65).
  */
@@ -312,7 +312,10 @@ int fa_fwd_paged(const fa_paged_cache* cache, const void* Q, long long q_token_s
                  int max_seqlen_k, float scale, int causal, int dtype, void* workspace,
                  size_t workspace_bytes, void* stream);
 
-/* Workspace bytes of fa_fwd_paged (a function of its sizes alone). */
+/* Workspace bytes of fa_fwd_paged (a function of its sizes alone): partial
+ * results of split keys, and for chunks over 8-bit pages the keys and values as
+ * f16 (at most about 1 GiB, or one KV head's if that is more); 0 for a few new
+ * tokens over short caches. */
 size_t fa_fwd_paged_workspace_bytes(const fa_paged_cache* cache, int B, int Hq, int total_q,
                                     int max_seqlen_q, int max_seqlen_k);
 

@@ -34,9 +34,9 @@ def _read(c, total=3, dtype=0, K=P16):
 
 
 def _attend(c, total=3, dtype=0, Q=P16, Hq=4, scale=1.0, causal=1, ws=P16, nbytes=1 << 62, qs=256,
-            max_q=3):
+            max_q=3, max_k=64):
     return abi.load().fa_fwd_paged(ctypes.byref(c) if c else None, Q, qs, 64, P16, None, P16, P16, 1, Hq,
-                                   total, max_q, 64, scale, causal, dtype, ws, nbytes, None)
+                                   total, max_q, max_k, scale, causal, dtype, ws, nbytes, None)
 
 
 @pytest.mark.parametrize("call", [_write, _read, _attend])
@@ -74,9 +74,9 @@ def test_call_argument_errors():
     assert _attend(_cache(), causal=3) == 1
     assert _attend(_cache(), Q=0) == 1
     assert _attend(_cache(), qs=260) == 4
-    assert _attend(_cache(), ws=0) == 1
+    assert _attend(_cache(), ws=0, max_q=99, total=99, max_k=8192) == 1
     assert _attend(_cache(), ws=P16 + 4) == 4
-    assert _attend(_cache(), nbytes=0) == 1
+    assert _attend(_cache(), nbytes=0, max_q=99, total=99, max_k=8192) == 1
     assert _attend(_cache(), max_q=-1) == 1
     for code in (12, 13, 14):
         assert abi.load().fa_error_string(code) not in (b"ok", b"unknown error")
@@ -84,13 +84,20 @@ def test_call_argument_errors():
 
 def test_workspace_depends_on_sizes_alone():
     f = abi.load().fa_fwd_paged_workspace_bytes
-    for args in ((1, 4, 1, 1, 64), (8, 4, 8, 1, 8192), (3, 4, 700, 512, 4096), (0, 4, 5, 1, 1)):
+    # a short cache needs none; splits, and chunks over 8-bit pages, do
+    for args, some in (((1, 4, 1, 1, 64), False), ((8, 4, 8, 1, 8192), True),
+                       ((3, 4, 700, 512, 4096), True), ((0, 4, 5, 1, 1), False)):
         n = f(ctypes.byref(_cache()), *args)
-        assert 0 < n == f(ctypes.byref(_cache(k=P16 * 2, block_table=P16 * 4)), *args)
-    # sizes that the call itself refuses
+        assert (n > 0) == some
+        assert n == f(ctypes.byref(_cache(k=P16 * 2, block_table=P16 * 4)), *args)
+    eight = dict(dtype=2, k_scale=P16, v_scale=P16)
+    assert f(ctypes.byref(_cache(**eight)), 1, 4, 700, 700, 700) >= 2 * 2 * 768 * 64 * 2
+    # a batch whose expanded keys pass 1 GiB goes head by head
+    assert f(ctypes.byref(_cache(kv_heads=16, **eight)), 64, 64, 1 << 16, 1024, 1 << 14) < 2 << 30
+    # sizes that the call itself refuses: no crash
     for args in ((1, 258, 9, 9, 64), (-1, 4, 9, 9, 64), (1, 4, -9, 9, 64), (1, 4, 9, -1, 64)):
-        assert f(ctypes.byref(_cache()), *args) > 0
-    assert f(None, 1, 4, 9, 9, 64) > 0 and f(ctypes.byref(_cache(kv_heads=0)), 1, 4, 9, 9, 64) > 0
+        assert f(ctypes.byref(_cache()), *args) == 0
+    assert f(None, 1, 4, 9, 9, 64) == 0 and f(ctypes.byref(_cache(kv_heads=0)), 1, 4, 9, 9, 64) == 0
 
 
 @pytest.mark.parametrize("mode", [0, 1, 2])
