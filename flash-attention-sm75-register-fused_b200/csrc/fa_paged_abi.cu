@@ -129,15 +129,16 @@ PagedPlan make_paged_plan(int B, int heads, int group, int head_dim, int dtype, 
       if (fit < static_cast<size_t>(heads)) k.exp_heads = fit < 1 ? 1 : static_cast<int>(fit);
     }
     // One CTA per (pair, head, split): the split with the fewest waves x (key
-    // tiles per split + 4 tiles of start-up and join), as for chunked prefill
-    // over a contiguous cache; the number of pairs is estimated from the rows.
+    // tiles per split + 4 tiles of start-up), as for chunked prefill over a
+    // contiguous cache, where a join's launch costs another 4 tiles (about 2 us
+    // each); the number of pairs is estimated from the rows.
     const long long pairs = B <= 1 ? (total + pair - 1) / pair : total / pair + (n_seq + 1) / 2;
     const long long items = (pairs < 1 ? 1 : pairs) * k.exp_heads;
     const long long n = (static_cast<long long>(max_k) + 127) / 128;
     long long best = -1;
     for (long long ns = 1; ns <= 32 && ns <= (n < 1 ? 1 : n); ++ns) {
       const long long waves = (items * ns + sms - 1) / sms;
-      const long long cost = waves * ((n + ns - 1) / ns + 4) + (ns > 1 ? 2 : 0);
+      const long long cost = waves * ((n + ns - 1) / ns + 4) + (ns > 1 ? 4 : 0);
       if (best < 0 || cost < best) {
         best = cost;
         k.n_splits = static_cast<int>(ns);

@@ -16,14 +16,14 @@
 //          rows can hold, and a CTA without one leaves at once.  Pairs of a
 //          sequence run from its end, the longest causal rows first.
 //   pages  16-bit pages: a 128-key tile is a set of TMA boxes of gcd(page, 128)
-//          rows, one per lane of the producer warp.  A box brings whole rows: the
-//          maps split d into halves of 128 bytes, laid out per 8 rows (8 rows x
-//          128 bytes of one half, then of the other), which the products'
-//          descriptors take like any swizzled tile.  (With a box per half, 32
-//          per tile at page 16, the loads bounded the kernel: 551 us against 420
-//          from 128-row pages at B=2, 2048 over 8192 keys, d = 128.)  The rows
-//          behind the last visible key in its box are stale; V's are set to zero
-//          before the tile is released, K's are masked as scores.
+//          rows, one per lane of a producer warp (one warp for K, one for V).  A
+//          box brings whole rows: the maps split d into halves of 128 bytes, laid
+//          out per 8 rows (8 rows x 128 bytes of one half, then of the other),
+//          which the products' descriptors take like any swizzled tile.  At B=2,
+//          2048 over 8192 keys, d = 128, pages of 16: a box per half from one warp
+//          551 us, whole rows 448, two warps 411 (1171 TFLOPS, as with pages of
+//          128).  The rows behind the last visible key in its box are stale; V's
+//          are set to zero before the tile is released, K's are masked as scores.
 //          8-bit pages: paged_expand_kernel first writes the visible keys and
 //          values once as f16 rows into the workspace (exactly, with the scales
 //          beside them, for f16 results; multiplied by their scale and rounded,
@@ -261,11 +261,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
 
   if (warp >= 8) {
     ptx::setmaxnreg_dec<L::kRegsRest>();
-    if (warp == kWarpLoad) {
-      // =================================================== TMA producer
+    if (warp == kWarpLoad || warp == kWarpMma + 1) {
+      // ================================================ TMA producers: K (and Q), V
+      const int second = warp == kWarpLoad ? 0 : 1;
       const uint64_t pol_q = ptx::policy_evict_first();
       const uint64_t pol_kv = ptx::policy_evict_last();
-      if (lane == 0) {
+      if (lane == 0 && second == 0) {
         ptx::prefetch_tmap(&p.tm_q);
         ptx::prefetch_tmap(&p.tm_k);
         ptx::prefetch_tmap(&p.tm_v);
@@ -294,13 +295,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
       const int exp_row0 = sh_item[2] * kBlockN;  // of the sequence in the expanded rows
       int next_page = page_at(it.jb), page = -1;
       bool ok = true, tail_used = false;
-      int i = 0;
-      for (; i < n_items; ++i) {
+      int i = second;
+      for (; i < n_items; i += 2) {
         const int tile = it.jb + (i >> 1);
-        if (!(i & 1)) {
-          page = next_page;
-          if (i + 2 < n_items) next_page = page_at(tile + 1);
-        }
+        page = next_page;
+        if (i + 2 < n_items) next_page = page_at(tile + 1);
         const int slot = i % L::kSlots;
         if (i >= L::kSlots &&
             !(ok = __all_sync(0xffffffffu, bar_wait(bar(L::kBarEmpty + slot),
@@ -343,10 +342,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
         }
       }
       // every copy started lands before the CTA exits
-      for (int r = max(0, i - L::kSlots); r < i; ++r)
-        bar_wait(bar(L::kBarFull + r % L::kSlots), (r / L::kSlots) & 1, wc, 2, false);
+      for (int r = second; r < i; r += 2)
+        if (r >= i - L::kSlots) bar_wait(bar(L::kBarFull + r % L::kSlots), (r / L::kSlots) & 1, wc, 2, false);
       if (tail_used && !ok) bar_wait(bar(L::kBarTail), 0, wc, 2, false);
-      for (int g = 0; g < 2 && !kCastQ; ++g)
+      for (int g = 0; g < 2 && !kCastQ && second == 0; ++g)
         if (it.n_kv[g] > 0) bar_wait(bar(L::kBarQ + g), 0, wc, 2, false);
     } else if (warp == kWarpMma) {
       // =================================================== MMA issuer (see fa_fwd_kernel)

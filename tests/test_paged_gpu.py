@@ -132,6 +132,30 @@ def test_rows_of_no_sequence(sm100, nq):
     _check(P, q, 4, 1, again)
 
 
+@pytest.mark.parametrize("io", [F16, BF16])
+def test_expanded_keys_go_head_group_by_head_group(sm100, io):
+    """A bound on the lengths whose expanded 8-bit keys would pass 1 GiB for all
+    heads: the chunk kernel runs a few heads at a time, with the same result."""
+    P = Paged([(150, 700), (90, 90)], 6, 128, 32, I8, io=io, seed=21)
+    q = P.new(12)
+    c = P.cuda()
+    args = (q.cuda(), c["k_cache"], c["v_cache"], c["table"], c["cu"], c["lens"], 150)
+    kw = dict(causal=True, k_scale=c["k_scale"], v_scale=c["v_scale"], return_lse=True)
+    got = fa.flash_attention_forward_paged(*args, 1 << 18, **kw)
+    _check(P, q, 12, 1, got)
+
+
+def test_single_token_calls_without_workspace(sm100):
+    """Short caches: one kernel, also for more (sequence, head) pairs than SMs and
+    more ring stages than units."""
+    for B, nk, cache in ((1, 300, F16), (40, 90, I8), (70, 512, BF16)):
+        io = BF16 if cache == BF16 else F16
+        P = Paged([(1, 1 + (nk * (b + 1)) // B) for b in range(B - 1)] + [(1, nk)], 4, 128, 16, cache,
+                  io=io, seed=B)
+        q = P.new(8)
+        _check(P, q, 8, 1, _attend(P, q, 8, 1))
+
+
 def test_max_seqlen_k_limits_the_keys(sm100):
     """Keys past max_seqlen_k are not seen (no causal rule here)."""
     for nq in (1, 40):
