@@ -9,6 +9,7 @@
 // (Nq != Nk: decode and chunked prefill), the paged KV cache (write, read back,
 // attention), and diagnostics.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -535,8 +536,15 @@ fa_paged_cache paged_cache(const torch::Tensor& k, const torch::Tensor& v,
   return c;
 }
 
-// int32 tensor with contiguous rows on `device`: x itself where it is one.
-torch::Tensor as_ints(const torch::Tensor& x, const torch::Device& device) {
+// int32 tensor with contiguous rows on `device` from a tensor (itself where it
+// is one) or a sequence of ints.
+torch::Tensor as_ints(pybind11::handle h, const torch::Device& device) {
+  torch::Tensor x;
+  if (THPVariable_Check(h.ptr())) {
+    x = THPVariable_Unpack(h.ptr());
+  } else {
+    x = pybind11::module_::import("torch").attr("as_tensor")(h).cast<torch::Tensor>();
+  }
   const bool rows = x.dim() == 0 || x.size(-1) <= 1 || x.stride(-1) == 1;
   if (x.scalar_type() == torch::kInt32 && x.device() == device && rows) return x;
   return x.to(torch::TensorOptions().dtype(torch::kInt32).device(device)).contiguous();
@@ -565,6 +573,12 @@ void check_new_rows(const torch::Tensor& t, const char* name) {
   TORCH_CHECK(t.size(0) <= INT32_MAX && t.size(1) <= INT32_MAX, "size exceeds int32");
 }
 
+// Uninitialised result (without the dispatcher: small calls
+// are bound by host time).
+torch::Tensor new_result(at::IntArrayRef sizes, torch::ScalarType dtype, const torch::Device& device) {
+  return at::detail::empty_cuda(sizes, torch::TensorOptions().dtype(dtype).device(device));
+}
+
 // `t` itself if the kernels can read it in place (contiguous rows, token and
 // head strides and base multiples of 16 bytes), else a contiguous copy.
 torch::Tensor readable_rows(const torch::Tensor& t) {
@@ -576,8 +590,8 @@ torch::Tensor readable_rows(const torch::Tensor& t) {
 
 void kvcache_write_paged(const torch::Tensor& k_in, const torch::Tensor& v_in,
                          const torch::Tensor& k_cache, const torch::Tensor& v_cache,
-                         const torch::Tensor& table_in, const torch::Tensor& cu_in,
-                         const torch::Tensor& lens_in, const c10::optional<torch::Tensor>& ks,
+                         pybind11::handle table_in, pybind11::handle cu_in,
+                         pybind11::handle lens_in, const c10::optional<torch::Tensor>& ks,
                          const c10::optional<torch::Tensor>& vs) {
   check_new_rows(k_in, "k");
   check_new_rows(v_in, "v");
@@ -601,8 +615,8 @@ void kvcache_write_paged(const torch::Tensor& k_in, const torch::Tensor& v_in,
 }
 
 std::tuple<torch::Tensor, torch::Tensor> kvcache_read_paged(
-    const torch::Tensor& k_cache, const torch::Tensor& v_cache, const torch::Tensor& table_in,
-    const torch::Tensor& cu_in, const torch::Tensor& lens_in, int64_t total,
+    const torch::Tensor& k_cache, const torch::Tensor& v_cache, pybind11::handle table_in,
+    pybind11::handle cu_in, pybind11::handle lens_in, int64_t total,
     const c10::optional<torch::Tensor>& ks, const c10::optional<torch::Tensor>& vs, bool bf16) {
   const auto table = as_ints(table_in, k_cache.device());
   const auto cu = as_ints(cu_in, k_cache.device()), lens = as_ints(lens_in, k_cache.device());
@@ -611,9 +625,8 @@ std::tuple<torch::Tensor, torch::Tensor> kvcache_read_paged(
   TORCH_CHECK(total >= 0 && total <= INT32_MAX, "total must be a count of rows, got ", total);
   const int B = paged_batch(cu, lens, table, k_cache.device());
   const c10::cuda::CUDAGuard guard(k_cache.device());
-  const auto opt = k_cache.options().dtype(dtype);
-  auto k = torch::empty({total, c.kv_heads, c.head_dim}, opt);
-  auto v = torch::empty({total, c.kv_heads, c.head_dim}, opt);
+  auto k = new_result({total, c.kv_heads, c.head_dim}, dtype, k_cache.device());
+  auto v = new_result({total, c.kv_heads, c.head_dim}, dtype, k_cache.device());
   if (total == 0) return {k, v};
   const int rc = fa_kvcache_read(&c, k.data_ptr(), v.data_ptr(), cu.data_ptr<int>(),
                                  B > 0 ? lens.data_ptr<int>() : nullptr, B,
@@ -623,10 +636,10 @@ std::tuple<torch::Tensor, torch::Tensor> kvcache_read_paged(
   return {k, v};
 }
 
-// O [total_q, Hq, d] and, if asked for, LSE fp32 [Hq, total_q].
-std::tuple<torch::Tensor, c10::optional<torch::Tensor>> flash_attention_forward_paged(
+// O [total_q, Hq, d], or with want_lse (O, LSE fp32 [Hq, total_q]).
+pybind11::object flash_attention_forward_paged(
     const torch::Tensor& q_in, const torch::Tensor& k_cache, const torch::Tensor& v_cache,
-    const torch::Tensor& table_in, const torch::Tensor& cu_in, const torch::Tensor& lens_in,
+    pybind11::handle table_in, pybind11::handle cu_in, pybind11::handle lens_in,
     int64_t max_seqlen_q, int64_t max_seqlen_k, int64_t causal, c10::optional<double> scale_in,
     bool want_lse, const c10::optional<torch::Tensor>& ks, const c10::optional<torch::Tensor>& vs) {
   check_new_rows(q_in, "q");
@@ -645,23 +658,26 @@ std::tuple<torch::Tensor, c10::optional<torch::Tensor>> flash_attention_forward_
   const c10::cuda::CUDAGuard guard(q_in.device());
   const auto q = readable_rows(q_in);
   const int Hq = static_cast<int>(q.size(1)), total = static_cast<int>(q.size(0));
-  auto O = torch::empty(q.sizes(), q.options());
-  c10::optional<torch::Tensor> lse;
-  if (want_lse) lse = torch::empty({Hq, total}, q.options().dtype(torch::kFloat32));
-  if (q.numel() == 0) return {O, lse};
+  auto O = new_result(q.sizes(), q.scalar_type(), q.device());
+  torch::Tensor lse;
+  if (want_lse) lse = new_result({Hq, total}, torch::kFloat32, q.device());
+  auto result = [&]() -> pybind11::object {
+    if (!want_lse) return pybind11::cast(O);
+    return pybind11::make_tuple(O, lse);
+  };
+  if (q.numel() == 0) return result();
   const int mq = static_cast<int>(max_seqlen_q), mk = static_cast<int>(max_seqlen_k);
   const size_t ws_bytes = fa_fwd_paged_workspace_bytes(&c, B, Hq, total, mq, mk);
   torch::Tensor ws;
-  if (ws_bytes > 0)
-    ws = torch::empty({static_cast<int64_t>(ws_bytes)}, q.options().dtype(torch::kUInt8));
+  if (ws_bytes > 0) ws = new_result({static_cast<int64_t>(ws_bytes)}, torch::kUInt8, q.device());
   const int rc = fa_fwd_paged(&c, q.data_ptr(), stride_of(q, 0), stride_of(q, 1), O.data_ptr(),
-                              want_lse ? lse->data_ptr<float>() : nullptr, cu.data_ptr<int>(),
+                              want_lse ? lse.data_ptr<float>() : nullptr, cu.data_ptr<int>(),
                               B > 0 ? lens.data_ptr<int>() : nullptr, B, Hq, total, mq, mk, scale,
                               static_cast<int>(causal),
                               q.scalar_type() == torch::kBFloat16 ? FA_DTYPE_BF16 : FA_DTYPE_F16,
                               ws_bytes > 0 ? ws.data_ptr() : nullptr, ws_bytes, stream_of(q));
   TORCH_CHECK(rc == FA_OK, "flash_attention_forward_paged: ", fa_error_string(rc));
-  return {O, lse};
+  return result();
 }
 
 int device_status(bool reset) { return fa_device_status(reset ? 1 : 0); }
@@ -695,7 +711,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("kvcache_read_paged", &kvcache_read_paged,
         "(K, V) packed 16-bit rows of the described tokens");
   m.def("flash_attention_forward_paged", &flash_attention_forward_paged,
-        "(O [total_q, Hq, d], LSE [Hq, total_q] or None) of new tokens over a paged cache");
+        "O [total_q, Hq, d], or (O, LSE [Hq, total_q]), of new tokens over a paged cache");
   m.def("device_status", &device_status, pybind11::arg("reset") = false,
         "Error code recorded by the in-kernel watchdog (0 = none)");
   m.def("set_watchdog_ns", &fa_set_watchdog_ns);

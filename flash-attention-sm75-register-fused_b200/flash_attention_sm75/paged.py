@@ -21,10 +21,9 @@ import flash_attn_sm75_cuda as _C
 from .ops import _CAUSAL_MODES
 
 
-# The binding checks the arguments, and takes integer tensors of any type and
-# device; what it gets as int32 on the inputs' device is used in place.
-def _ints(x):
-    return x if isinstance(x, torch.Tensor) else torch.as_tensor(x, dtype=torch.int32)
+# The binding checks the arguments; integer arguments may be tensors of any type
+# and device or sequences, and are used in place where they are int32 on the
+# inputs' device.
 
 
 def kvcache_write_paged(k, v, k_cache, v_cache, block_table, cu_seqlens, seqlens_k, k_scale=None,
@@ -46,8 +45,8 @@ def kvcache_write_paged(k, v, k_cache, v_cache, block_table, cu_seqlens, seqlens
     448 (e4m3).  Tokens without a place (position below 0 or past the table,
     a table entry outside the cache) are not stored.
     """
-    _C.kvcache_write_paged(k, v, k_cache, v_cache, _ints(block_table), _ints(cu_seqlens),
-                           _ints(seqlens_k), k_scale, v_scale)
+    _C.kvcache_write_paged(k, v, k_cache, v_cache, block_table, cu_seqlens,
+                           seqlens_k, k_scale, v_scale)
 
 
 def kvcache_read_paged(k_cache, v_cache, block_table, cu_seqlens, seqlens_k, total, k_scale=None,
@@ -70,8 +69,8 @@ def kvcache_read_paged(k_cache, v_cache, block_table, cu_seqlens, seqlens_k, tot
         dtype = k_cache.dtype if k_cache.element_size() == 2 else torch.bfloat16
     if dtype not in (torch.float16, torch.bfloat16):
         raise ValueError(f"dtype must be torch.float16 or torch.bfloat16, got {dtype}")
-    return _C.kvcache_read_paged(k_cache, v_cache, _ints(block_table), _ints(cu_seqlens),
-                                 _ints(seqlens_k), int(total), k_scale, v_scale,
+    return _C.kvcache_read_paged(k_cache, v_cache, block_table, cu_seqlens,
+                                 seqlens_k, total, k_scale, v_scale,
                                  dtype is torch.bfloat16)
 
 
@@ -103,7 +102,6 @@ def flash_attention_forward_paged(q, k_cache, v_cache, block_table, cu_seqlens_q
         mode = _CAUSAL_MODES.get(causal_alignment)
         if mode is None:
             raise ValueError(f"causal_alignment must be one of {sorted(_CAUSAL_MODES)}")
-    out, lse = _C.flash_attention_forward_paged(
-        q, k_cache, v_cache, _ints(block_table), _ints(cu_seqlens_q), _ints(seqlens_k),
-        int(max_seqlen_q), int(max_seqlen_k), mode, scale, bool(return_lse), k_scale, v_scale)
-    return (out, lse) if return_lse else out
+    return _C.flash_attention_forward_paged(q, k_cache, v_cache, block_table, cu_seqlens_q, seqlens_k,
+                                            max_seqlen_q, max_seqlen_k, mode, scale, return_lse,
+                                            k_scale, v_scale)
