@@ -236,9 +236,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
   const int n_rows = p.tq * a.group;  // rows of a tile in use
 
   // ---- set-up
+  int dead = 0;  // this launch failed elsewhere
   if (threadIdx.x == 0) {
     const unsigned long long st = *reinterpret_cast<volatile unsigned long long*>(&g_fa_status);
-    *abort_flag = ((st >> 32) == p.epoch && (st & 0xffffffffull) != 0ull) ? 1 : 0;
+    dead = ((st >> 32) == p.epoch && (st & 0xffffffffull) != 0ull) ? 1 : 0;
+    *abort_flag = 0;
     for (int i = 0; i < L::kNumBars; ++i) {
       const bool all = (i >= L::kBarP && i < L::kBarP + 2) || (i >= L::kBarPH && i < L::kBarPH + 2) ||
                        (kCastQ && i < 2);
@@ -246,8 +248,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
     }
     ptx::fence_barrier_init();
   }
-  __syncthreads();
-  if (*abort_flag) return;
+  if (__syncthreads_or(dead)) return;
   if (warp == kWarpMma) {
     ptx::tmem_alloc(ptx::smem_u32(tmem_slot), L::kTmemCols);
     ptx::tmem_relinquish();

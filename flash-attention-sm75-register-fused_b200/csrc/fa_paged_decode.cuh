@@ -242,9 +242,11 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
   ptx::launch_dependents();
 
   // ---- set-up, and the team's run [v0, v1) of the batch's positions
+  int dead = 0;  // this launch failed elsewhere
   if (threadIdx.x == 0) {
     const unsigned long long st = *reinterpret_cast<volatile unsigned long long*>(&g_fa_status);
-    sh_abort = ((st >> 32) == p.epoch && (st & 0xffffffffull) != 0ull) ? 1 : 0;
+    dead = ((st >> 32) == p.epoch && (st & 0xffffffffull) != 0ull) ? 1 : 0;
+    sh_abort = 0;
     // a stage is full when its boxes have landed (and, 8-bit pages, the 32
     // lanes' scales)
     for (int i = 0; i < kTeams * stages; ++i)
@@ -261,8 +263,7 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
     const long long base = static_cast<long long>(static_cast<int>(blockIdx.x) % H) * (n + kSegCost) + kSegCost;
     rel = base + static_cast<long long>(n) * team / kTeams;
     v1 = base + static_cast<long long>(n) * (team + 1) / kTeams;
-    __syncthreads();
-    if (*abort_flag) return;
+    if (__syncthreads_or(dead)) return;
   } else {
     const int share = (a.r.B + 32 * kWarps - 1) / (32 * kWarps);
     const int s0 = min(static_cast<int>(threadIdx.x) * share, a.r.B), s1 = min(s0 + share, a.r.B);
@@ -288,10 +289,10 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
         }
       }
     }
-    __syncthreads();
+    if (__syncthreads_or(dead)) return;  // (one answer for the block)
     const long long v0 = min(per * tid, total);
     v1 = min(v0 + per, total);
-    if (v0 >= v1 || *abort_flag) return;
+    if (v0 >= v1) return;
     b_first = sh_b[team];
     rel = sh_rel[team];
     v1 -= v0 - rel;  // relative to the first sequence's first position, like rel
@@ -507,7 +508,7 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
     }
     // V's scales are relative to 2^lv: p = exp2(s - m - lv) is summed, and
     // p * vs multiplies V's 8-bit values
-    int lv = C::k8 ? -60 : 0;
+    int lv = C::k8 ? -95 : 0;  // (below any scale a row is stored with, and l stays finite)
 
     for (int t = t_begin; t < t_end; ++t) {
       ok = bar_wait(bars + 8 * rstage, rphase, wc, 50);
