@@ -115,8 +115,9 @@ struct alignas(64) DecodeParams {
 // Decode kernel: sequences with at most max_rows <= paged_decode_rows() query
 // rows (new tokens x group) per KV head, and the rows of sequences without
 // visible keys or of no sequence.  Sequences with more rows are left alone.
-int paged_decode_rows();
-size_t paged_decode_ws_bytes(int max_rows, int max_k, int head_dim, int cache_dtype, int sms);
+// heads: sequences x KV heads.
+int paged_decode_rows(long long heads, int head_dim, int cache_dtype, int sms);
+size_t paged_decode_ws_bytes(long long heads, int max_rows, int max_k, int head_dim, int cache_dtype, int sms);
 cudaError_t launch_paged_decode(DecodeParams p, int head_dim, int cache_dtype, bool bf16, int sms,
                                 cudaStream_t stream);
 // Chunk kernel (after the expansion of 8-bit pages) over the KV heads of p, and

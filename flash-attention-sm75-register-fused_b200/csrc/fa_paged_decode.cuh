@@ -35,7 +35,7 @@
 // first part, which continues a head of the team before, or its last, which
 // the next team continues) and paged_combine_kernel joins them in order.
 //
-// Short caches (DecodeParams::solo: at most 8 units per team) take one CTA per
+// Short caches (DecodeParams::solo, at most 3 to 8 units per team) take one CTA per
 // (sequence, head) instead, whose teams share its units and join in shared
 // memory: one launch, no workspace, no plan over the batch.
 #include "fa_paged.h"
@@ -926,6 +926,9 @@ cudaError_t launch_impl(const DecodeParams& p, int n_ctas, cudaStream_t stream) 
   // before it reads a slot
   cudaLaunchConfig_t cfg{};
   const unsigned segments = static_cast<unsigned>(p.a.r.B) * p.a.c.heads;
+  // blocks of one row fill the device with few segments (8 heads x 64 rows: 38
+  // us for the call instead of 50; 64 x 4: 86 / 90), blocks of eight with many
+  // (256 x 4: 91 / 86; 128 x 64: 155 / 113)
   const bool many = static_cast<long long>(segments) * p.max_rows > 4 * 148;
   cfg.gridDim = dim3(segments, many ? (p.max_rows + 7) / 8 : p.max_rows);
   cfg.blockDim = dim3(kCombineThreads);
@@ -952,8 +955,10 @@ template <int D, int KV, bool QBF16>
 cudaError_t launch_rows(const DecodeParams& p, int n_ctas, cudaStream_t s) {
   if (p.max_rows <= 8) return launch_impl<D, KV, QBF16, 1, 1>(p, n_ctas, s);
   if (p.max_rows <= 16) return launch_impl<D, KV, QBF16, 2, 1>(p, n_ctas, s);
-  if (p.max_rows <= 32) return launch_impl<D, KV, QBF16, 2, 2>(p, n_ctas, s);
-  return launch_impl<D, KV, QBF16, 2, 4>(p, n_ctas, s);
+  if constexpr (D == 64 || KV >= FA_DTYPE_INT8) {
+    if (p.max_rows > 32) return launch_impl<D, KV, QBF16, 2, 4>(p, n_ctas, s);
+  }
+  return launch_impl<D, KV, QBF16, 2, 2>(p, n_ctas, s);  // (paged_decode_rows)
 }
 
 template <int D>
@@ -973,20 +978,46 @@ cudaError_t launch_d(const DecodeParams& p, int kv, bool bf16, int n_ctas, cudaS
 }  // namespace pdec
 }  // namespace
 
-int paged_decode_rows() { return pdec::kRowsMax; }
+// Query rows per (sequence, KV head) up to which this kernel is taken.  Over
+// 8-bit pages always kRowsMax, for the chunk kernel has to expand them first
+// (B=8, 8192 keys, 8 KV heads, d = 128, 64 rows: 105 us here, 155 there; 32
+// rows: 60 / 152).  16-bit pages: up to 32 rows (16: 54 / 70 us, 32: 61 / 85);
+// above, teams of four warps read a unit four times from shared memory and are
+// slower (48 rows: 106 / 87, 32 x 4096 keys: 210 / 137), except at d = 64 with
+// less than half a CTA of the chunk kernel per SM (4 x 8 heads x 4096 keys, 48
+// rows: 25 / 28 us, but 128 heads x 2048: 38 / 29).
+int paged_decode_rows(long long heads, int head_dim, int kv, int sms) {
+  return kv >= FA_DTYPE_INT8 || (head_dim == 64 && 2 * heads < sms) ? pdec::kRowsMax : 32;
+}
 
 namespace {
 namespace pdec {
-// Few units per (sequence, head): one CTA each, joined in shared memory.
-bool is_solo(int max_rows, int max_k, int head_dim, int kv) {
-  const int sub = 4096 / (head_dim * (kv >= FA_DTYPE_INT8 ? 1 : 2));
-  return (static_cast<long long>(max_k) + sub - 1) / sub <= 8 * (kWarps / team_for(max_rows).warps);
+// Few units per (sequence, head): one CTA each, joined in shared memory.  What
+// it saves is the join (one launch); what it costs is that few CTAs run and
+// none helps another.  Time of either way, d = 128, by units per team (us, runs /
+// one CTA each):
+//   heads of all sequences      8          64          152         1024
+//   f16  3 units            8.4 / 6.5   9.6 / 6.9  10.0 / 7.4  27.9 / 25.4
+//        5                  8.5 / 8.1   9.7 / 8.2  12.1 / 8.9  37.7 / 35.4
+//        8                  8.6 / 10.2 10.6 / 10.4 15.0 / 11.4 53.3 / 49.7
+//        16                 9.2 / 15.7 13.1 / 15.9 20.7 / 17.3 91.5 / 87.3
+//   int8 3                  9.7 / 8.3  10.5 / 8.4  12.0 / 9.3  29.9 / 29.8
+//        4                  9.5 / 9.4  11.1 / 9.6  13.6 / 10.9 34.5 / 35.3
+//        8                  9.6 / 14.1 12.1 / 14.4 16.7 / 16.4 54.1 / 58.6
+// With a CTA for half the SMs or more 8 units, though equal lengths would allow
+// 16: in a ragged batch the longest sequence has one CTA too (152 heads, lengths
+// of 1 to 16 units per team: 17.1 / 16.9, mostly short ones 15.8 / 16.1).
+bool is_solo(long long heads, int max_rows, int max_k, int head_dim, int kv, int sms) {
+  const bool k8 = kv >= FA_DTYPE_INT8;
+  const int sub = 4096 / (head_dim * (k8 ? 1 : 2));
+  const int most = 2 * heads < sms ? (k8 ? 4 : 5) : !k8 || heads <= 3LL * sms ? 8 : 3;
+  return (static_cast<long long>(max_k) + sub - 1) / sub <= most * (kWarps / team_for(max_rows).warps);
 }
 }  // namespace pdec
 }  // namespace
 
-size_t paged_decode_ws_bytes(int max_rows, int max_k, int head_dim, int kv, int sms) {
-  if (pdec::is_solo(max_rows, max_k, head_dim, kv)) return 0;
+size_t paged_decode_ws_bytes(long long heads, int max_rows, int max_k, int head_dim, int kv, int sms) {
+  if (pdec::is_solo(heads, max_rows, max_k, head_dim, kv, sms)) return 0;
   const pdec::Team t = pdec::team_for(max_rows);
   const size_t teams = static_cast<size_t>(sms) * pdec::ctas_per_sm(t.nt) * (pdec::kWarps / t.warps);
   return 2 * teams * static_cast<size_t>(pdec::slot_floats(8 * t.nt * t.warps, head_dim)) * sizeof(float);
@@ -998,16 +1029,16 @@ cudaError_t launch_paged_decode(DecodeParams p, int head_dim, int kv, bool bf16,
   const int per_cta = pdec::kWarps / t.warps;
   // no more teams than units there can be
   const int sub = 4096 / (head_dim * (kv >= FA_DTYPE_INT8 ? 1 : 2));
-  const long long units = static_cast<long long>(p.a.r.B) * p.a.c.heads *
-                          ((static_cast<long long>(p.a.max_k) + sub - 1) / sub);
+  const long long heads = static_cast<long long>(p.a.r.B) * p.a.c.heads;
+  const long long units = heads * ((static_cast<long long>(p.a.max_k) + sub - 1) / sub);
   long long ctas = (units + per_cta - 1) / per_cta;
   const long long most = static_cast<long long>(sms) * pdec::ctas_per_sm(t.nt);
   ctas = ctas > most ? most : ctas < 1 ? 1 : ctas;
   p.n_teams = static_cast<int>(ctas) * per_cta;
-  p.solo = pdec::is_solo(p.max_rows, p.a.max_k, head_dim, kv) ? 1 : 0;
+  p.solo = pdec::is_solo(heads, p.max_rows, p.a.max_k, head_dim, kv, sms) ? 1 : 0;
   p.stages = pdec::stages_per_warp(t.nt);
   if (p.solo) {
-    ctas = static_cast<long long>(p.a.r.B) * p.a.c.heads;
+    ctas = heads;
     if (ctas <= sms) p.stages = pdec::kMaxStages;
     else if (ctas <= 2LL * sms) p.stages = 3;
   }
