@@ -66,6 +66,12 @@ struct PagedAttn {
   float scale_log2;           // scale * log2(e)
 };
 
+// An item of the chunk kernel that the end of a run cuts: its sequence's first row
+// and tokens, its first token, KV head and parts (0: none is cut).
+struct alignas(16) PagedCut {
+  int c0, nq, tok0, h, parts, pad[3];
+};
+
 struct alignas(64) ChunkParams {
   CUtensorMap tm_q;  // (d, Hq, T), box (64, G, tq)
   // (64 columns, 8 rows, d / 64, row groups of 8, planes), box (64, 8, d / 64,
@@ -79,7 +85,8 @@ struct alignas(64) ChunkParams {
   int page_step, head_step;
   int stale;         // tiles may end in stale rows (pages do, the expanded rows do not)
   int skip_rows;     // sequences with at most this many rows per KV head are not ours
-  int n_splits;
+  int runs;          // 1: CTAs take equal runs of the work order, 0: a (pair, head) each
+  int n_ctas;
   int fill_outside;  // write the rows of no sequence
   int head0, n_heads;  // KV heads of this launch
   // 8-bit pages: f16 rows and scales of the launch's heads (paged_expand_kernel)
@@ -88,8 +95,11 @@ struct alignas(64) ChunkParams {
   uint16_t* exp_v;
   float* exp_ks;     // [n_heads][exp_rows], f16 results only
   float* exp_vs;
-  float* ws_o;       // [n_splits][total * Hq][d] fp32, normalised
-  float* ws_lse;     // [n_splits][total * Hq], natural log
+  // parts of cut items, two slots per run: [2 n_ctas][2 query tiles][d / 4][128
+  // rows][4] fp32, normalised, and [2 n_ctas][2][128], natural log
+  float* ws_o;
+  float* ws_lse;
+  PagedCut* ws_cuts;  // [n_ctas]
   unsigned epoch;
   unsigned long long timeout_ns;
 };
@@ -121,9 +131,8 @@ size_t paged_decode_ws_bytes(long long heads, int max_rows, int max_k, int head_
 cudaError_t launch_paged_decode(DecodeParams p, int head_dim, int cache_dtype, bool bf16, int sms,
                                 cudaStream_t stream);
 // Chunk kernel (after the expansion of 8-bit pages) over the KV heads of p, and
-// the join of its key splits once all heads are done.
-cudaError_t launch_paged_chunk(const ChunkParams& p, int head_dim, int cache_dtype, bool bf16,
-                               int grid, int sms, cudaStream_t stream);
-cudaError_t launch_paged_join(const ChunkParams& p, int head_dim, bool bf16, cudaStream_t stream);
+// the join of the items that its runs cut.
+cudaError_t launch_paged_chunk(const ChunkParams& p, int head_dim, int cache_dtype, bool bf16, int sms,
+                               cudaStream_t stream);
 
 }  // namespace fa

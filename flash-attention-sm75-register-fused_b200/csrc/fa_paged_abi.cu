@@ -87,13 +87,14 @@ struct PagedPlan {
   int decode_rows = 0;  // rows per KV head the decode kernel takes at most
   int tq = 0;           // chunk kernel: tokens of a query tile
   int slots = 0;        // ... pairs of tiles there may be
-  int n_splits = 1;
+  bool runs = false;    // ... equal runs, or one CTA per (pair, head)
+  int n_ctas = 0;       // ... runs
   // 8-bit pages: rows of the expanded keys, KV heads expanded at a time, and
   // bytes of one head's K (or V) rows and scales
   long long exp_rows = 0;
   int exp_heads = 0;
   size_t exp_row_bytes = 0, exp_scale_bytes = 0;
-  size_t ws_decode = 0, ws_o = 0, ws_lse = 0, ws_bytes = 0;
+  size_t ws_decode = 0, ws_o = 0, ws_lse = 0, ws_cuts = 0, ws_bytes = 0;
 };
 
 // Expanded keys and values are at most this large where several KV heads would
@@ -131,30 +132,43 @@ PagedPlan make_paged_plan(int B, int heads, int group, int head_dim, int dtype, 
       const size_t fit = kExpandBytes / per_head;
       if (fit < static_cast<size_t>(heads)) k.exp_heads = fit < 1 ? 1 : static_cast<int>(fit);
     }
-    // One CTA per (pair, head, split): the split with the fewest waves x (key
-    // tiles per split + 4 tiles of start-up), as for chunked prefill over a
-    // contiguous cache, where a join's launch costs another 4 tiles (about 2 us
-    // each); the number of pairs is estimated from the rows.
+    // A CTA per (pair, head), or equal runs of all of them: estimated in key
+    // tiles of an SM, from bounds.  An item costs its tiles (from `least_t` to `tiles`
+    // of a causal chunk's pairs, longest first) and 5 for its start, 3 in a run,
+    // where the next item's tiles are loaded meanwhile; runs cost another 12 (parts
+    // written and joined).  With all SMs at work a tile takes 15/14 of its time, and
+    // runs another 9/8 where the keys outgrow the L2: the CTAs are at different
+    // places of them.
+    const long long tiles = max_k < 1 ? 1 : (static_cast<long long>(max_k) + 127) / 128;
+    const long long drop = (max_q < max_k ? max_q : max_k) / 128;
+    const long long least_t = tiles - drop, mean_t = tiles - drop / 2;
     const long long pairs = B <= 1 ? (total + pair - 1) / pair : total / pair + (n_seq + 1) / 2;
     const long long items = (pairs < 1 ? 1 : pairs) * k.exp_heads;
-    const long long n = (static_cast<long long>(max_k) + 127) / 128;
-    long long best = -1;
-    for (long long ns = 1; ns <= 32 && ns <= (n < 1 ? 1 : n); ++ns) {
-      const long long waves = (items * ns + sms - 1) / sms;
-      const long long cost = waves * ((n + ns - 1) / ns + 4) + (ns > 1 ? 4 : 0);
-      if (best < 0 || cost < best) {
-        best = cost;
-        k.n_splits = static_cast<int>(ns);
-      }
+    long long by_item = tiles + 5, by_run = items * (mean_t + 3) * 15 / 14 / sms + 12;
+    if (items > sms) {
+      const long long in_waves = (items + sms - 1) / sms * (mean_t + 5);
+      const long long in_order = items * (mean_t + 5) / sms + least_t + 5;
+      by_item = (in_waves < in_order ? in_waves : in_order) * 15 / 14;
+      // (in a ragged batch a sequence's keys are taken to go with its tokens)
+      const long long keys = static_cast<long long>(total) * max_k / (max_q < 1 ? 1 : max_q);
+      if (keys > (100 << 20) / 4 / heads / head_dim) by_run = by_run * 9 / 8;
     }
-    if (k.n_splits > 1) {
-      const size_t rows_all = static_cast<size_t>(k.n_splits) * total * heads * group;
-      k.ws_o = rows_all * head_dim * sizeof(float);
-      k.ws_lse = (rows_all * sizeof(float) + 127) / 128 * 128;
+    k.runs = by_run < by_item;
+    if (k.runs) {
+      // no more runs than key tiles there can be, nor parts of an item than a
+      // join reads in a few rounds
+      const long long most = items * (tiles > 32 ? 32 : tiles);
+      k.n_ctas = static_cast<int>(most < sms ? most : sms);
+      if (k.n_ctas > 1) {
+        const size_t rows = static_cast<size_t>(2 * k.n_ctas) * 256;
+        k.ws_o = rows * head_dim * sizeof(float);
+        k.ws_lse = rows * sizeof(float);
+        k.ws_cuts = (k.n_ctas * sizeof(fa::PagedCut) + 127) / 128 * 128;
+      }
     }
   }
   const size_t chunk_bytes =
-      k.ws_o + k.ws_lse + 2 * static_cast<size_t>(k.exp_heads) * (k.exp_row_bytes + k.exp_scale_bytes);
+      k.ws_o + k.ws_lse + k.ws_cuts + 2 * static_cast<size_t>(k.exp_heads) * (k.exp_row_bytes + k.exp_scale_bytes);
   // (the kernels run one after another, so they share the workspace)
   k.ws_bytes = k.ws_decode > chunk_bytes ? k.ws_decode : chunk_bytes;
   return k;
@@ -351,7 +365,7 @@ int fa_fwd_paged(const fa_paged_cache* cache, const void* Q, long long q_token_s
   const PagedPlan k = make_paged_plan(B, a.c.heads, group, cache->head_dim, cache->dtype, total_q, max_seqlen_q,
                                       max_seqlen_k);
   if (k.ws_bytes > 0 && (!workspace || workspace_bytes < k.ws_bytes)) return FA_ERR_INVALID_ARG;
-  const long long grid = static_cast<long long>(k.slots) * a.c.heads * k.n_splits;  // of all heads
+  const long long grid = static_cast<long long>(k.slots) * a.c.heads;  // of all heads
   if (grid > 0x7fffffffLL || static_cast<long long>(B) * a.c.heads > 0x7fffffffLL ||
       static_cast<long long>(total_q) * Hq > (1LL << 33))
     return FA_ERR_TOO_LARGE;
@@ -389,11 +403,12 @@ int fa_fwd_paged(const fa_paged_cache* cache, const void* Q, long long q_token_s
     p.stale = eight ? 0 : 1;
     p.page_step = p.head_step = 0;
     p.skip_rows = k.decode ? k.decode_rows : 0;
-    p.n_splits = k.n_splits;
+    p.runs = k.runs ? 1 : 0;
     char* ws = static_cast<char*>(workspace);
     p.ws_o = reinterpret_cast<float*>(ws);
     p.ws_lse = reinterpret_cast<float*>(ws + k.ws_o);
-    ws += k.ws_o + k.ws_lse;
+    p.ws_cuts = reinterpret_cast<fa::PagedCut*>(ws + k.ws_o + k.ws_lse);
+    ws += k.ws_o + k.ws_lse + k.ws_cuts;
     p.exp_rows = k.exp_rows;
     p.exp_k = reinterpret_cast<uint16_t*>(ws);
     p.exp_v = reinterpret_cast<uint16_t*>(ws + k.exp_heads * k.exp_row_bytes);
@@ -409,12 +424,11 @@ int fa_fwd_paged(const fa_paged_cache* cache, const void* Q, long long q_token_s
       p.n_heads = a.c.heads - p.head0 < k.exp_heads ? a.c.heads - p.head0 : k.exp_heads;
       p.fill_outside = !k.decode && p.head0 == 0 ? 1 : 0;
       p.epoch = fa::host_next_epoch();
-      if (fa::launch_paged_chunk(p, cache->head_dim, cache->dtype, bf16, k.slots * p.n_heads * k.n_splits,
-                                 fa::host_sm_count(), st) != cudaSuccess)
+      p.n_ctas = k.runs ? k.n_ctas : k.slots * p.n_heads;
+      if (fa::launch_paged_chunk(p, cache->head_dim, cache->dtype, bf16, fa::host_sm_count(), st) !=
+          cudaSuccess)
         return FA_ERR_LAUNCH;
     }
-    if (k.n_splits > 1 && fa::launch_paged_join(p, cache->head_dim, bf16, st) != cudaSuccess)
-      return FA_ERR_LAUNCH;
   }
   return FA_OK;
 }

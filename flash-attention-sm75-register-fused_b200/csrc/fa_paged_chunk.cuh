@@ -11,10 +11,19 @@
 //          token * G + head), for every length: K and V are read once per
 //          group, and short chunks fill their tiles.  G need not divide 128
 //          (G = 7: 18 tokens, 126 rows).
-//   items  (sequence, pair of tiles, KV head, key split), found from the
-//          lengths on the device: the grid has room for every pair the packed
-//          rows can hold, and a CTA without one leaves at once.  Pairs of a
-//          sequence run from its end, the longest causal rows first.
+//   items  (sequence, KV head, pair of tiles), found from the lengths on the device
+//          in one of two ways (chosen on the host by an estimate of both).  One CTA
+//          per item: the grid has room for every pair the packed rows can hold,
+//          a CTA without one leaves at once, and pairs of a sequence run from its
+//          end, the longest causal rows first.  Or equal runs: the key tiles of
+//          all items in a row are cut into one run per SM, whatever the lengths
+//          (SeqWork gives positions in closed form), one warp hands the
+//          run's segments to the others through a ring, K and V of the next segment
+//          load while the last one ends, and cut items are joined.  Items / runs,
+//          d = 128, GQA 4, 8 KV heads: 512 tokens over 8192 keys 116 / 70 us (two
+//          splits of each item, 128 CTAs: 76), over 1024 keys 23.5 / 25.3; 2 x 2048
+//          over 8192 460 / 433; 200 over 200 14.3 / 22.1; 8 x 1024 over 1024 124 /
+//          115; 8 x 2048 over 8192 (keys twice the L2) 1780 / 2000.
 //   pages  16-bit pages: a 128-key tile is a set of TMA boxes of gcd(page, 128)
 //          rows, one per lane of a producer warp (one warp for K, one for V).  A
 //          box brings whole rows: the maps split d into halves of 128 bytes, laid
@@ -32,8 +41,15 @@
 //          reads plain 128-row tiles.  For f16 results the softmax applies the
 //          scales in fp32: K's to the scores; V's is split into a power of two,
 //          which the rows take (exactly), and a rest in [1, 2) for P.
-//   joins  With few items the keys are split; partial O and LSE go to the
-//          workspace and paged_join_kernel merges them.
+//   joins  The parts of a cut item go to the workspace as fp32 (four columns of all
+//          rows side by side, so that stores and the join's loads are whole
+//          lines: 77 -> 70 us for 512 tokens over 8192 keys), and paged_join_kernel
+//          merges them by a table that the runs leave.
+//
+// Bound by the tensor cores and what feeds them: with all SMs at work a pair's key
+// tile takes 1.8 us (1.5 at the rate of a large library product), so 2 x 2048
+// tokens over 8192 keys run at 1230 TFLOPS; then by the start of the work: a
+// call with one item per SM costs 11 us beyond its tiles, one of equal runs 21.
 #include "fa_paged.h"
 #include "fa_paged_dev.cuh"
 
@@ -42,6 +58,19 @@ namespace {
 
 // What the kernel reads.
 enum { kPagesF16 = 0, kPagesBf16 = 1, kExpanded = 2 };
+
+// A part of a work item that a CTA computes.
+struct Segment {
+  int b, h;              // sequence (-1: the run ends), KV head
+  int c0, nq, nk, off, vis;  // of the sequence (Seq)
+  int tok0;              // first token of query tile 0
+  int jb, n0, n1;        // first key tile; key tiles of either query tile
+  int slot;              // of the workspace, -1: the segment is the whole item
+  int exp_row0;          // sequence's first row in the expanded rows
+  int tiles, parity;     // key tiles before it; bit g: those of query tile g, mod 2
+  int pad;
+};
+constexpr int kSegRing = 4;
 
 template <int D, bool kScaled>
 struct ChunkLayout {
@@ -75,8 +104,12 @@ struct ChunkLayout {
   static constexpr int kBarO = kBarPH + 2;              // 2
   static constexpr int kBarDrain = kBarO + 2;           // 1
   static constexpr int kBarTail = kBarDrain + 1;        // 1: the V tile with stale rows landed
-  static constexpr int kNumBars = kBarTail + 1;
-  static constexpr int kOffMisc = kOffBar + 8 * kNumBars;
+  static constexpr int kBarQFree = kBarTail + 1;        // 2: Q read by its last scores
+  static constexpr int kBarSegFull = kBarQFree + 2;     // kSegRing
+  static constexpr int kBarSegEmpty = kBarSegFull + kSegRing;  // kSegRing
+  static constexpr int kNumBars = kBarSegEmpty + kSegRing;
+  static constexpr int kOffSeg = kOffBar + (8 * kNumBars + 15) / 16 * 16;
+  static constexpr int kOffMisc = kOffSeg + kSegRing * static_cast<int>(sizeof(Segment));
   static constexpr int kBytes = kOffMisc + 16;
   static constexpr int kDynBytes = kBytes + 1024;
   static constexpr uint32_t kTmemCols = 512;
@@ -137,11 +170,112 @@ __device__ __forceinline__ float exp_tile_scaled(const float (&x)[kBlockN], floa
 // 128-row blocks of a sequence in the expanded rows.
 __device__ __forceinline__ int expand_blocks(const Seq& s) { return (s.vis + kBlockN - 1) / kBlockN; }
 
-// The work item of a CTA.
+// The pairs of query tiles of a sequence, and what they cost.  Pair i (of one
+// head) sees keys [0, lim(i)), lim(i) = clamp(off + (i + 1) c, 0, vis) for c tokens
+// a pair; it takes kItemCost + lim(i) positions of the work order, the key tile
+// that starts at key k the one at kItemCost + k.
+// (kItemCost: six ragged chunks over e4m3 pages take 271 us with 256, 263 with 384
+// or 512, 275 with 1024.  kMinRun, the shortest run: 64 tokens over 8192 keys take 37.9
+// us with 128, 35.5 with 512; 512 over 1024 26.9 with 128, 27.3 with 512, 31.8 with 1024)
+constexpr int kItemCost = 384;
+constexpr int kMinRun = 512;
+struct SeqWork {
+  long long off;
+  int c, vis, n;  // n pairs
+  int z, s;       // pairs [0, z) see no key, pairs [s, n) all of them
+  __device__ __forceinline__ int lim(int i) const {
+    return static_cast<int>(min(max(off + static_cast<long long>(i + 1) * c, 0ll), static_cast<long long>(vis)));
+  }
+  __device__ __forceinline__ int tiles(int i) const { return (lim(i) + kBlockN - 1) / kBlockN; }
+  // positions of pairs [0, i)
+  __device__ __forceinline__ long long before(int i) const {
+    const long long s1 = min(i, s), z1 = min(i, z);
+    return static_cast<long long>(i) * kItemCost + (s1 - z1) * off + c * ((s1 * (s1 + 1) - z1 * (z1 + 1)) / 2) +
+           (i - s1) * vis;
+  }
+  // the last pair that starts at or before position x
+  __device__ __forceinline__ int pair_at(long long x) const {
+    int lo = 0;
+    for (int hi = n; hi - lo > 1;) {
+      const int mid = (lo + hi) >> 1;
+      if (before(mid) <= x) lo = mid;
+      else hi = mid;
+    }
+    return lo;
+  }
+};
+__device__ __forceinline__ SeqWork work_of(const ChunkParams& p, const Seq& s) {
+  SeqWork w;
+  w.c = 2 * p.tq;
+  w.vis = s.vis;
+  w.off = p.a.causal == FA_CAUSAL_NONE ? s.vis : s.off;
+  w.n = static_cast<long long>(s.nq) * p.a.group <= p.skip_rows ? 0 : (s.nq + w.c - 1) / w.c;
+  const unsigned n = w.n, c = w.c, off = w.off;  // (differences below fit 32 bits)
+  w.z = w.off < 0 ? static_cast<int>(min((0u - off) / c, n)) : 0;
+  w.s = w.off < w.vis ? static_cast<int>(min((static_cast<unsigned>(w.vis) - off) / c, n)) : 0;
+  w.s = max(w.s, w.z);
+  return w;
+}
+
+// Where a CTA starts in the work order.
+struct WorkStart {
+  long long per;   // positions of a run
+  long long base;  // of sequence b (p.runs: positions, else pairs)
+  int b;           // -1: past the end
+  int blocks;      // 128-row blocks before the sequence in the expanded rows
+  Seq s;
+};
+// Called by all threads.  p.runs: CTA x starts at position x * per, else at pair x.
+template <bool kExp>
+__device__ __forceinline__ void find_start(const ChunkParams& p, int x, WorkStart* out, long long* scan_a,
+                                           long long* scan_b) {
+  const PagedAttn& a = p.a;
+  const int share = (a.r.B + kThreads - 1) / kThreads;
+  const int b0 = min(static_cast<int>(threadIdx.x) * share, a.r.B), b1 = min(b0 + share, a.r.B);
+  Seq s{};  // the last one looked at
+  int blocks = 0;
+  auto weight = [&](int b) -> long long {
+    s = load_seq(a, b);
+    const bool ours = static_cast<long long>(s.nq) * a.group > p.skip_rows;
+    blocks = ours ? expand_blocks(s) : 0;
+    if (!p.runs) return ours ? (s.nq + 2 * p.tq - 1) / (2 * p.tq) : 0;
+    const SeqWork w = work_of(p, s);
+    return p.n_heads * w.before(w.n);
+  };
+  if (threadIdx.x == 0) out->b = -1;
+  long long sum = 0, sum_blocks = 0, total, unused;
+  for (int b = b0; b < b1; ++b) {
+    sum += weight(b);
+    sum_blocks += blocks;
+  }
+  long long at = block_scan<kThreads>(sum, scan_a, &total);
+  long long at_blocks = kExp ? block_scan<kThreads>(sum_blocks, scan_b, &unused) : 0;
+  const long long per =
+      p.runs ? max((total + p.n_ctas - 1) / p.n_ctas, static_cast<long long>(kMinRun)) : 1;
+  const long long v = x * per;
+  if (v >= at && v < at + sum) {
+    int b = b0;
+    if (share > 1)
+      for (;; ++b) {
+        const long long w = weight(b);
+        if (v < at + w) break;
+        at += w;
+        at_blocks += blocks;
+      }
+    out->per = per;
+    out->base = at;
+    out->blocks = static_cast<int>(at_blocks);
+    out->b = b;
+    out->s = s;
+  }
+  __syncthreads();
+}
+
+// A segment as the softmax of query tile g sees it.
 struct ChunkItem {
   Seq s;
-  int b, h, pair, sp;
-  int n_kv[2], jb, n_loop;  // key tiles of either query tile, from tile jb
+  int h, tok_lo, jb, n_tiles, slot, tiles, par;
+  bool last;
 };
 
 // SRC: what is read; QBF16: type of Q and O.
@@ -156,8 +290,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~static_cast<uintptr_t>(1023));
-  __shared__ long long sh_scan[kThreads / 32];
-  __shared__ int sh_item[3];  // sequence, pair (-1: none), first block of the expanded rows
+  __shared__ long long sh_scan[2][kThreads / 32];
+  __shared__ WorkStart start;
   const uint32_t sbase = ptx::smem_u32(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kOffMisc);
@@ -165,41 +299,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
   auto bar = [&](int i) -> uint32_t { return sbase + L::kOffBar + 8u * static_cast<uint32_t>(i); };
   ptx::launch_dependents();
 
-  // ---- which (sequence, pair) is this CTA's?
-  const int w = static_cast<int>(blockIdx.x);
-  const int slot_id = w / (p.n_splits * p.n_heads);
+  // ---- where does this CTA's work start?
+  const int cta = static_cast<int>(blockIdx.x);
+  find_start<kExp>(p, p.runs ? cta : cta / p.n_heads, &start, sh_scan[0], sh_scan[1]);
   {
-    // low word: pairs of a sequence; high word: its 128-row blocks in the
-    // expanded rows
-    auto pairs_of = [&](int b) -> long long {
-      const Seq s = load_seq(a, b);
-      if (static_cast<long long>(s.nq) * a.group <= p.skip_rows) return 0;
-      return (s.nq + 2 * p.tq - 1) / (2 * p.tq) + (static_cast<long long>(expand_blocks(s)) << 32);
-    };
-    const int share = (a.r.B + kThreads - 1) / kThreads;
-    const int b0 = min(static_cast<int>(threadIdx.x) * share, a.r.B), b1 = min(b0 + share, a.r.B);
-    if (threadIdx.x == 0) sh_item[1] = -1;
-    long long sum = 0, total;
-    for (int b = b0; b < b1; ++b) sum += pairs_of(b);
-    long long x = block_scan<kThreads>(sum, sh_scan, &total);
-    const int lo = static_cast<int>(x), hi = lo + static_cast<int>(sum);
-    if (slot_id >= lo && slot_id < hi)
-      for (int b = b0; b < b1; ++b) {
-        const long long n = pairs_of(b);
-        const int first = static_cast<int>(x), pairs = static_cast<int>(n);
-        if (slot_id < first + pairs) {
-          sh_item[0] = b;
-          sh_item[1] = first + pairs - 1 - slot_id;  // from the sequence's end
-          sh_item[2] = static_cast<int>(x >> 32);
-          break;
-        }
-        x += n;
-      }
     if (p.fill_outside) {
       const int head = a.r.B > 0 ? min(max(__ldg(a.r.cu), 0), a.r.total) : a.r.total;
       const int tail = a.r.B > 0 ? min(max(__ldg(a.r.cu + a.r.B), head), a.r.total) : a.r.total;
       const int n_out = head + a.r.total - tail;
-      for (int y = w; y < n_out; y += static_cast<int>(gridDim.x)) {
+      for (int y = cta; y < n_out; y += static_cast<int>(gridDim.x)) {
         const int t = y < head ? y : tail + y - head;
         for (int i = threadIdx.x; i < a.Hq * D / 2; i += kThreads)
           static_cast<uint32_t*>(a.o)[static_cast<long long>(t) * (a.Hq * D / 2) + i] = 0u;
@@ -208,30 +316,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
             a.lse[static_cast<long long>(i) * a.r.total + t] = -INFINITY;
       }
     }
-    __syncthreads();
   }
-  ChunkItem it;
-  it.pair = sh_item[1];
-  if (it.pair < 0) return;
-  it.b = sh_item[0];
-  it.h = p.head0 + (w / p.n_splits) % p.n_heads;
-  it.sp = w % p.n_splits;
-  it.s = load_seq(a, it.b);
-  const int tok0 = it.pair * 2 * p.tq;  // first token of tile 0
-#pragma unroll
-  for (int g = 0; g < 2; ++g) {
-    const int lo = tok0 + g * p.tq;
-    const int lim = lo < it.s.nq ? row_limit(a, it.s, min(lo + p.tq, it.s.nq) - 1) : 0;
-    it.n_kv[g] = (lim + kBlockN - 1) / kBlockN;
-  }
-  {
-    // the pair's key tiles, in equal parts
-    const int n = max(it.n_kv[0], it.n_kv[1]);
-    const int tps = (n + p.n_splits - 1) / p.n_splits;
-    it.jb = it.sp * tps;
-#pragma unroll
-    for (int g = 0; g < 2; ++g) it.n_kv[g] = max(min(it.n_kv[g] - it.jb, tps), 0);
-    it.n_loop = max(it.n_kv[0], it.n_kv[1]);
+  if (start.b < 0) {
+    if (p.runs && p.n_ctas > 1 && threadIdx.x == 0) p.ws_cuts[cta].parts = 0;
+    return;
   }
   const int n_rows = p.tq * a.group;  // rows of a tile in use
 
@@ -244,7 +332,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
     for (int i = 0; i < L::kNumBars; ++i) {
       const bool all = (i >= L::kBarP && i < L::kBarP + 2) || (i >= L::kBarPH && i < L::kBarPH + 2) ||
                        (kCastQ && i < 2);
-      ptx::mbar_init(bar(i), all ? 128u : 1u);
+      const bool seg = i >= L::kBarSegEmpty;  // one arrival per warp that reads segments
+      ptx::mbar_init(bar(i), all ? 128u : seg ? 11u : 1u);
     }
     ptx::fence_barrier_init();
   }
@@ -258,11 +347,113 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
   ptx::tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
   const WaitCtl wc{abort_flag, p.timeout_ns, p.epoch};
-  const int n_items = 2 * it.n_loop;  // K_0 V_0 K_1 V_1 ...
+  volatile Segment* const segs = reinterpret_cast<volatile Segment*>(smem + L::kOffSeg);
+  // Every reading warp waits for segment n, reads it and releases it.
+  auto seg_ready = [&](int n) {
+    return __all_sync(0xffffffffu, bar_wait(bar(L::kBarSegFull + n % kSegRing), (n / kSegRing) & 1, wc, 3));
+  };
+  auto seg_done = [&](int n) {
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(bar(L::kBarSegEmpty + n % kSegRing));
+  };
 
   if (warp >= 8) {
     ptx::setmaxnreg_dec<L::kRegsRest>();
-    if (warp == kWarpLoad || warp == kWarpMma + 1) {
+    if (warp == kWarpMma + 2) {
+      // =================================================== the run's segments
+      int b = start.b, n_seg = 0, tiles = 0, par = 0;
+      int exp_row0 = start.blocks * kBlockN;
+      bool ok = true;
+      auto push = [&](const Seq& s, int h, int tok0, int jb, int n0, int n1, int slot) {
+        const int e = n_seg % kSegRing;
+        if (n_seg >= kSegRing &&
+            !(ok = __all_sync(0xffffffffu, bar_wait(bar(L::kBarSegEmpty + e), ((n_seg / kSegRing) - 1) & 1, wc, 4))))
+          return;
+        if (lane == 0) {
+          volatile Segment& g = segs[e];
+          g.b = b;
+          g.h = h;
+          g.c0 = s.c0;
+          g.nq = s.nq;
+          g.nk = s.nk;
+          g.off = s.off;
+          g.vis = s.vis;
+          g.tok0 = tok0;
+          g.jb = jb;
+          g.n0 = n0;
+          g.n1 = n1;
+          g.slot = slot;
+          g.exp_row0 = exp_row0;
+          g.tiles = tiles;
+          g.parity = par;
+          ptx::mbar_arrive(bar(L::kBarSegFull + e));
+        }
+        __syncwarp();
+        ++n_seg;
+        tiles += max(n0, n1);
+        par ^= (n0 & 1) | ((n1 & 1) << 1);
+      };
+      // tiles [lo, hi) of pair i of head h
+      auto take = [&](const Seq& s, int h, int i, int lo, int hi, int slot) {
+        int n[2];
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          const int tok = (2 * i + g) * p.tq;
+          const int lim = tok < s.nq ? row_limit(a, s, min(tok + p.tq, s.nq) - 1) : 0;
+          n[g] = max(min((lim + kBlockN - 1) / kBlockN, hi) - lo, 0);
+        }
+        push(s, h, 2 * i * p.tq, lo, n[0], n[1], slot);
+      };
+      Seq s = start.s;
+      SeqWork w = work_of(p, s);
+      if (!p.runs) {
+        // pairs of a sequence from its end, the longest causal rows first
+        const int i = static_cast<int>(start.base) + w.n - 1 - cta / p.n_heads;
+        take(s, p.head0 + cta % p.n_heads, i, 0, w.tiles(i), -1);
+      } else {
+        const long long v0 = cta * start.per, v1 = v0 + start.per;
+        const long long all = w.before(w.n);
+        PagedCut cut{};  // the item that this run's end cuts first
+        int h = static_cast<int>((v0 - start.base) / all);
+        long long at = start.base + h * all;  // of pair 0, then of pair i
+        int i = w.pair_at(v0 - at);
+        at += w.before(i);
+        while (ok && at < v1) {
+          const int n = w.tiles(i);
+          const long long key0 = at + kItemCost;
+          auto from = [&](long long v) {  // first tile that starts at or after v
+            const long long k = v - key0;
+            return k <= 0 ? 0 : static_cast<int>(min((k + kBlockN - 1) / kBlockN, static_cast<long long>(n)));
+          };
+          const int lo = from(v0), hi = from(v1);
+          if (lo == 0 && hi > 0 && hi < n) {
+            const long long last = (key0 + static_cast<long long>(n - 1) * kBlockN) / start.per;  // its last run
+            cut = PagedCut{s.c0, s.nq, 2 * i * p.tq, p.head0 + h, static_cast<int>(last) - cta + 1, {0, 0, 0}};
+          }
+          if (lo < hi) take(s, p.head0 + h, i, lo, hi, lo > 0 ? 2 * cta : hi < n ? 2 * cta + 1 : -1);
+          else if (n == 0 && at >= v0) take(s, p.head0 + h, i, 0, 0, -1);
+          at = key0 + w.lim(i);
+          if (++i == w.n) {
+            i = 0;
+            if (++h == p.n_heads) {
+              h = 0;
+              if (w.n > 0) exp_row0 += expand_blocks(s) * kBlockN;
+              do {
+                if (++b >= a.r.B) break;
+                s = load_seq(a, b);
+                w = work_of(p, s);
+              } while (w.n == 0);
+              if (b >= a.r.B) break;
+            }
+          }
+        }
+        if (lane == 0 && p.n_ctas > 1) p.ws_cuts[cta] = cut;
+      }
+      if (ok) {
+        b = -1;
+        push(s, 0, 0, 0, 0, 0, -1);
+      }
+    } else if (warp == kWarpLoad || warp == kWarpMma + 1) {
       // ================================================ TMA producers: K (and Q), V
       const int second = warp == kWarpLoad ? 0 : 1;
       const uint64_t pol_q = ptx::policy_evict_first();
@@ -271,83 +462,103 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
         ptx::prefetch_tmap(&p.tm_q);
         ptx::prefetch_tmap(&p.tm_k);
         ptx::prefetch_tmap(&p.tm_v);
-        for (int g = 0; g < 2 && !kCastQ; ++g) {
-          if (it.n_kv[g] == 0) continue;
-          ptx::mbar_arrive_expect_tx(bar(L::kBarQ + g), L::kColBlocks * n_rows * 128);
-#pragma unroll
-          for (int c = 0; c < L::kColBlocks; ++c)
-            ptx::tma_load_3d(sbase + L::kOffQ + g * L::kTile + c * L::kBlockBytes, &p.tm_q,
-                             bar(L::kBarQ + g), c * 64, it.h * a.group, it.s.c0 + tok0 + g * p.tq,
-                             pol_q);
-        }
       }
       __syncwarp();
       // lane = box of the tile (the expanded rows have one of 128 rows)
       const int box = lane;
       const bool issues = box * p.box_rows < kBlockN;
       const uint32_t dst_off = box * p.box_rows * (2 * D);
-      // place of this lane's box in the map's last dimension; -1 reads as zeros
-      auto page_at = [&](int tile) {
-        if (kExp) return it.h - p.head0;
-        const int pos = tile * kBlockN + box * p.box_rows;
-        const int page = issues && pos < it.s.vis ? a.c.lookup(it.b, pos) : -1;
-        return page >= 0 ? page * p.page_step + it.h * p.head_step : -1;
-      };
-      const int exp_row0 = sh_item[2] * kBlockN;  // of the sequence in the expanded rows
-      int next_page = page_at(it.jb), page = -1;
-      bool ok = true, tail_used = false;
-      int i = second;
-      for (; i < n_items; i += 2) {
-        const int tile = it.jb + (i >> 1);
-        page = next_page;
-        if (i + 2 < n_items) next_page = page_at(tile + 1);
-        const int slot = i % L::kSlots;
-        if (i >= L::kSlots &&
-            !(ok = __all_sync(0xffffffffu, bar_wait(bar(L::kBarEmpty + slot),
-                                                    ((i / L::kSlots) - 1) & 1, wc, 1))))
-          break;
-        // stale V rows of the tile: [r0, r1)
-        const int r0 = it.s.vis - tile * kBlockN;
-        const int r1 = (r0 + p.box_rows - 1) / p.box_rows * p.box_rows;
-        // (a run-time flag, though the expanded rows never have any: with the
-        // branch compiled out the softmax spills, 874 instead of 449 us)
-        const bool tail = p.stale && (i & 1) && r0 < kBlockN && r0 != r1;
-        const uint32_t full = tail ? bar(L::kBarTail) : bar(L::kBarFull + slot);
-        const bool scales = kScaled && !(i & 1);
-        if (lane == 0) ptx::mbar_arrive_expect_tx(full, L::kTile + (scales ? L::kScaleEntry : 0));
-        __syncwarp();
-        const uint32_t dst = sbase + L::kOffKV + slot * L::kTile;
-        // first row: in the page, or in the expanded rows (kept inside them)
-        const int row = kExp ? min(exp_row0 + tile * kBlockN, static_cast<int>(p.exp_rows) - kBlockN)
-                             : a.c.row_in_page(tile * kBlockN + box * p.box_rows);
-        if (issues)
-          ptx::tma_load_5d(dst + dst_off, (i & 1) ? &p.tm_v : &p.tm_k, full, 0, 0, 0, row >> 3, page, pol_kv);
-        if (scales && lane < 2) {
-          const float* src = (lane ? p.exp_vs : p.exp_ks) +
-                             static_cast<long long>(it.h - p.head0) * p.exp_rows + row;
-          ptx::bulk_load(sbase + L::kOffScale + ((i >> 1) % L::kScaleRing) * L::kScaleEntry + lane * 512, src,
-                         512, full);
-        }
-        if (tail) {
-          tail_used = true;
-          if (!(ok = __all_sync(0xffffffffu, bar_wait(bar(L::kBarTail), 0, wc, 7)))) break;
-          for (int x = lane; x < (r1 - r0) * 8 * L::kColBlocks; x += 32) {
-            const int r = r0 + x / (8 * L::kColBlocks), c = x % (8 * L::kColBlocks);
-            *reinterpret_cast<uint4*>(smem + L::kOffKV + slot * L::kTile + (r >> 3) * L::kGroupBytes +
-                                      (c >> 3) * 1024 + (r & 7) * 128 + (c & 7) * 16) =
-                make_uint4(0u, 0u, 0u, 0u);
+      bool ok = true;
+      int i = second;                   // ring entry: K_0 V_0 K_1 V_1 ..., over all segments
+      int n_tail = 0, n_q[2] = {0, 0};  // stale V tiles, Q tiles loaded so far
+      for (int n = 0; (ok = seg_ready(n)); ++n) {
+        const volatile Segment& sg = segs[n % kSegRing];
+        const int b = sg.b, h = sg.h, c0 = sg.c0, vis = sg.vis, tok0 = sg.tok0, jb = sg.jb;
+        const int n_kv[2] = {sg.n0, sg.n1}, exp_row0 = sg.exp_row0;
+        seg_done(n);
+        if (b < 0) break;
+        const int n_loop = max(n_kv[0], n_kv[1]);
+        // place of this lane's box in the map's last dimension; -1 reads as zeros
+        auto page_at = [&](int tile) {
+          if (kExp) return h - p.head0;
+          const int pos = tile * kBlockN + box * p.box_rows;
+          const int page = issues && pos < vis ? a.c.lookup(b, pos) : -1;
+          return page >= 0 ? page * p.page_step + h * p.head_step : -1;
+        };
+        int next_page = n_loop > 0 ? page_at(jb) : -1, page = -1;
+        for (int g = 0; ok && g < 2 && !kCastQ && second == 0; ++g) {
+          if (n_kv[g] == 0) continue;
+          if (n_q[g] > 0 &&
+              !(ok = __all_sync(0xffffffffu, bar_wait(bar(L::kBarQFree + g), (n_q[g] - 1) & 1, wc, 8))))
+            break;
+          ++n_q[g];
+          if (lane == 0) {
+            ptx::mbar_arrive_expect_tx(bar(L::kBarQ + g), L::kColBlocks * n_rows * 128);
+#pragma unroll
+            for (int c = 0; c < L::kColBlocks; ++c)
+              ptx::tma_load_3d(sbase + L::kOffQ + g * L::kTile + c * L::kBlockBytes, &p.tm_q,
+                               bar(L::kBarQ + g), c * 64, h * a.group, c0 + tok0 + g * p.tq, pol_q);
           }
-          ptx::fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) ptx::mbar_arrive(bar(L::kBarFull + slot));
         }
+        for (int x = 0; ok && x < n_loop; ++x) {
+          const int tile = jb + x;
+          page = next_page;
+          if (x + 1 < n_loop) next_page = page_at(tile + 1);
+          const int slot = i % L::kSlots;
+          if (i >= L::kSlots &&
+              !(ok = __all_sync(0xffffffffu, bar_wait(bar(L::kBarEmpty + slot),
+                                                      ((i / L::kSlots) - 1) & 1, wc, 1))))
+            break;
+          // stale V rows of the tile: [r0, r1)
+          const int r0 = vis - tile * kBlockN;
+          const int r1 = (r0 + p.box_rows - 1) / p.box_rows * p.box_rows;
+          // (a run-time flag, though the expanded rows never have any: with the
+          // branch compiled out the softmax spills, 874 instead of 449 us)
+          const bool tail = p.stale && second && r0 < kBlockN && r0 != r1;
+          const uint32_t full = tail ? bar(L::kBarTail) : bar(L::kBarFull + slot);
+          const bool scales = kScaled && !second;
+          if (lane == 0) ptx::mbar_arrive_expect_tx(full, L::kTile + (scales ? L::kScaleEntry : 0));
+          __syncwarp();
+          const uint32_t dst = sbase + L::kOffKV + slot * L::kTile;
+          // first row: in the page, or in the expanded rows (kept inside them)
+          const int row = kExp ? min(exp_row0 + tile * kBlockN, static_cast<int>(p.exp_rows) - kBlockN)
+                               : a.c.row_in_page(tile * kBlockN + box * p.box_rows);
+          if (issues)
+            ptx::tma_load_5d(dst + dst_off, second ? &p.tm_v : &p.tm_k, full, 0, 0, 0, row >> 3, page, pol_kv);
+          if (scales && lane < 2) {
+            const float* src = (lane ? p.exp_vs : p.exp_ks) +
+                               static_cast<long long>(h - p.head0) * p.exp_rows + row;
+            ptx::bulk_load(sbase + L::kOffScale + ((i >> 1) % L::kScaleRing) * L::kScaleEntry + lane * 512, src,
+                           512, full);
+          }
+          i += 2;
+          if (tail) {
+            const bool here = __all_sync(0xffffffffu, bar_wait(bar(L::kBarTail), n_tail & 1, wc, 7));
+            ++n_tail;
+            if (!(ok = here)) {
+              i -= 2;  // (its slot is not announced)
+              break;
+            }
+            for (int y = lane; y < (r1 - r0) * 8 * L::kColBlocks; y += 32) {
+              const int r = r0 + y / (8 * L::kColBlocks), c = y % (8 * L::kColBlocks);
+              *reinterpret_cast<uint4*>(smem + L::kOffKV + slot * L::kTile + (r >> 3) * L::kGroupBytes +
+                                        (c >> 3) * 1024 + (r & 7) * 128 + (c & 7) * 16) =
+                  make_uint4(0u, 0u, 0u, 0u);
+            }
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(bar(L::kBarFull + slot));
+          }
+        }
+        if (!ok) break;
       }
       // every copy started lands before the CTA exits
-      for (int r = second; r < i; r += 2)
-        if (r >= i - L::kSlots) bar_wait(bar(L::kBarFull + r % L::kSlots), (r / L::kSlots) & 1, wc, 2, false);
-      if (tail_used && !ok) bar_wait(bar(L::kBarTail), 0, wc, 2, false);
-      for (int g = 0; g < 2 && !kCastQ && second == 0; ++g)
-        if (it.n_kv[g] > 0) bar_wait(bar(L::kBarQ + g), 0, wc, 2, false);
+      for (int r = i - 2; r >= 0 && r >= i - L::kSlots; r -= 2)
+        bar_wait(bar(L::kBarFull + r % L::kSlots), (r / L::kSlots) & 1, wc, 2, false);
+      if (n_tail > 0 && !ok) bar_wait(bar(L::kBarTail), (n_tail - 1) & 1, wc, 2, false);
+      for (int g = 0; g < 2; ++g)
+        if (n_q[g] > 0) bar_wait(bar(L::kBarQ + g), (n_q[g] - 1) & 1, wc, 2, false);
     } else if (warp == kWarpMma) {
       // =================================================== MMA issuer (see fa_fwd_kernel)
       constexpr uint32_t fmt = kBf16 ? 1u : 0u;
@@ -365,7 +576,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
           static_cast<uint32_t>(ptx::smem_desc_sw128(sbase + L::kOffQ + L::kTile, 16, 1024));
       constexpr uint32_t kSlotStep = L::kTile >> 4;
       constexpr uint32_t kVStep = 2 * L::kGroupBytes >> 4;  // 16 keys
-      auto issue_s = [&](int g, int ks, uint32_t q_lo) {
+      auto issue_s = [&](int g, int ks, uint32_t q_lo, bool last) {
         const uint32_t k_lo = k_lo0 + static_cast<uint32_t>(ks) * kSlotStep;
         if (ptx::elect_one()) {
 #pragma unroll
@@ -376,6 +587,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                         ptx::make_desc(k_lo + k_off, kv_hi), idesc_qk, kk > 0 ? 1u : 0u);
           }
           ptx::mma_commit(bar(L::kBarS + g));
+          if (last) ptx::mma_commit(bar(L::kBarQFree + g));
         }
         __syncwarp();
       };
@@ -409,54 +621,64 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
         __syncwarp();
         return true;
       };
-      const int n0 = it.n_kv[0], n1 = it.n_kv[1];
       bool ok = true;
-      int ks = 0;
+      int ks = 0;                      // ring slot of the next K, its phase
       uint32_t kph = 0;
+      uint32_t cnt[2] = {0, 0};        // key tiles of query tile g so far
+      uint32_t n_q[2] = {0, 0};        // Q tiles used so far
       auto adv = [](int& sl, uint32_t& ph) {
         if (++sl == L::kSlots) {
           sl = 0;
           ph ^= 1u;
         }
       };
-      if (it.n_loop > 0) {
-        if (n0 > 0) ok = wait(bar(L::kBarQ), 0, 10);
-        if (ok && n1 > 0) ok = wait(bar(L::kBarQ + 1), 0, 10);
-        if (ok) ok = wait(bar(L::kBarFull), 0, 11);
-        if (ok) {
-          ptx::tc_fence_after();
-          if (n0 > 0) issue_s(0, ks, q_lo0);
-          if (n1 > 0) issue_s(1, ks, q_lo1);
-          commit(bar(L::kBarEmpty + ks));
-        }
-      }
-      for (int j = 0; ok && j < it.n_loop; ++j) {
-        int vs = ks;
-        uint32_t vph = kph;
-        adv(vs, vph);
-        int ns = vs;
-        uint32_t nph = vph;
-        adv(ns, nph);
-        ks = ns;
-        kph = nph;
-        const bool next0 = j + 1 < n0, next1 = j + 1 < n1;
-        if (!(ok = wait(bar(L::kBarFull + vs), vph, 12))) break;
-        if ((next0 || next1) && !(ok = wait(bar(L::kBarFull + ns), nph, 14))) break;
-        if (j < n0) {
-          if (!(ok = issue_pv(0, vs, j == 0, j & 1))) break;
-          if (next0) {
-            issue_s(0, ns, q_lo0);
-            if (!next1) commit(bar(L::kBarEmpty + ns));
+      for (int n = 0; ok && (ok = seg_ready(n)); ++n) {
+        const volatile Segment& sg = segs[n % kSegRing];
+        const int b = sg.b, n0 = sg.n0, n1 = sg.n1;
+        seg_done(n);
+        if (b < 0) break;
+        const int n_loop = max(n0, n1);
+        if (n_loop > 0) {
+          if (n0 > 0) ok = wait(bar(L::kBarQ), n_q[0]++ & 1, 10);
+          if (ok && n1 > 0) ok = wait(bar(L::kBarQ + 1), n_q[1]++ & 1, 10);
+          if (ok) ok = wait(bar(L::kBarFull + ks), kph, 11);
+          if (ok) {
+            ptx::tc_fence_after();
+            if (n0 > 0) issue_s(0, ks, q_lo0, n0 == 1);
+            if (n1 > 0) issue_s(1, ks, q_lo1, n1 == 1);
+            commit(bar(L::kBarEmpty + ks));
           }
         }
-        if (j < n1) {
-          if (!(ok = issue_pv(1, vs, j == 0, j & 1))) break;
+        for (int j = 0; ok && j < n_loop; ++j) {
+          int vs = ks;
+          uint32_t vph = kph;
+          adv(vs, vph);
+          int ns = vs;
+          uint32_t nph = vph;
+          adv(ns, nph);
+          ks = ns;
+          kph = nph;
+          const bool next0 = j + 1 < n0, next1 = j + 1 < n1;
+          if (!(ok = wait(bar(L::kBarFull + vs), vph, 12))) break;
+          if ((next0 || next1) && !(ok = wait(bar(L::kBarFull + ns), nph, 14))) break;
+          if (j < n0) {
+            if (!(ok = issue_pv(0, vs, j == 0, (cnt[0] + j) & 1))) break;
+            if (next0) {
+              issue_s(0, ns, q_lo0, j + 2 == n0);
+              if (!next1) commit(bar(L::kBarEmpty + ns));
+            }
+          }
+          if (j < n1) {
+            if (!(ok = issue_pv(1, vs, j == 0, (cnt[1] + j) & 1))) break;
+          }
+          commit(bar(L::kBarEmpty + vs));
+          if (next1) {
+            issue_s(1, ns, q_lo1, j + 2 == n1);
+            commit(bar(L::kBarEmpty + ns));
+          }
         }
-        commit(bar(L::kBarEmpty + vs));
-        if (next1) {
-          issue_s(1, ns, q_lo1);
-          commit(bar(L::kBarEmpty + ns));
-        }
+        cnt[0] += n0;
+        cnt[1] += n1;
       }
       // all products complete before tensor memory is released
       commit(bar(L::kBarDrain));
@@ -473,13 +695,32 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
     const uint32_t tS = tmem + lane_off + L::tS(g);
     const uint32_t tP = tmem + lane_off + L::tP(g);
     const uint32_t tO = tmem + lane_off + L::tO(g);
-    const int n_tiles = g ? it.n_kv[1] : it.n_kv[0];
-    const int tok_lo = tok0 + g * p.tq;
+    bool ok = true;
+    for (int n_seg = 0; ok && (ok = seg_ready(n_seg)); ++n_seg) {
+    ChunkItem it;
+    {
+      const volatile Segment& sg = segs[n_seg % kSegRing];
+      it.last = sg.b < 0;
+      it.h = sg.h;
+      it.s.c0 = sg.c0;
+      it.s.nq = sg.nq;
+      it.s.nk = sg.nk;
+      it.s.off = sg.off;
+      it.tok_lo = sg.tok0 + g * p.tq;
+      it.jb = sg.jb;
+      it.n_tiles = g ? sg.n1 : sg.n0;
+      it.slot = sg.slot;
+      it.tiles = sg.tiles;
+      it.par = (sg.parity >> g) & 1;
+    }
+    seg_done(n_seg);
+    if (it.last) break;
+    const int n_tiles = it.n_tiles;
+    const int tok_lo = it.tok_lo;
     const int tok = tok_lo + r / a.group;      // token of the sequence
     const int hq = it.h * a.group + r % a.group;
     const bool row_ok = r < n_rows && tok < it.s.nq;
     float sl = a.scale_log2;
-    bool ok = true;
     if constexpr (kCastQ) {
       // Q as f16 in the swizzled layout, one row per thread; a bf16 row is
       // scaled by a power of two into f16's range, undone in sl
@@ -530,7 +771,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
     float m = -INFINITY;  // running max of the scaled scores (log2 units)
     float l = 0.f;        // running sum of exp2(s - m)
     for (int j = 0; ok && j < n_tiles; ++j) {
-      ok = __all_sync(0xffffffffu, bar_wait(bar(L::kBarS + g), j & 1, wc, 20 + g));
+      ok = __all_sync(0xffffffffu, bar_wait(bar(L::kBarS + g), (it.par + j) & 1, wc, 20 + g));
       if (!ok) break;
       ptx::tc_fence_after();
       float x[kBlockN];
@@ -553,7 +794,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
           x[96 + c] = __uint_as_float(u3[c]);
         }
       }
-      const uint32_t entry = sbase + L::kOffScale + (kScaled ? (j % L::kScaleRing) * L::kScaleEntry : 0);
+      const uint32_t entry = sbase + L::kOffScale + (kScaled ? ((it.tiles + j) % L::kScaleRing) * L::kScaleEntry : 0);
       if constexpr (kScaled) {
 #pragma unroll
         for (int c = 0; c < kBlockN; c += 4) {
@@ -628,9 +869,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
     // ---- epilogue
     using T = typename std::conditional<QBF16, __nv_bfloat16, __half>::type;
     const long long row_id = static_cast<long long>(it.s.c0 + tok) * a.Hq + hq;
-    const long long n_all = static_cast<long long>(a.r.total) * a.Hq;
-    const bool partial = p.n_splits > 1;
-    float* lse_dst = partial ? p.ws_lse + it.sp * n_all + row_id
+    const bool partial = it.slot >= 0;
+    const long long ws_row = (static_cast<long long>(it.slot) * 2 + g) * kBlockM + r;
+    float* lse_dst = partial ? p.ws_lse + ws_row
                      : a.lse ? a.lse + static_cast<long long>(hq) * a.r.total + it.s.c0 + tok
                              : nullptr;
     if (n_tiles == 0) {
@@ -641,7 +882,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
       }
       if (row_ok && lse_dst) *lse_dst = -INFINITY;
     } else {
-      if (ok) ok = __all_sync(0xffffffffu, bar_wait(bar(L::kBarO + g), (n_tiles - 1) & 1, wc, 22 + g));
+      if (ok) ok = __all_sync(0xffffffffu, bar_wait(bar(L::kBarO + g), (it.par + n_tiles - 1) & 1, wc, 22 + g));
       if (ok) {
         ptx::tc_fence_after();
         const float inv_l = (l > 0.f) ? 1.0f / l : (l == 0.f ? 0.f : l);  // (a NaN stays one)
@@ -666,16 +907,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                 dst[i] = make_uint4(hv[4 * i], hv[4 * i + 1], hv[4 * i + 2], hv[4 * i + 3]);
             }
           } else if (row_ok) {
-            float4* dst = reinterpret_cast<float4*>(p.ws_o + (it.sp * n_all + row_id) * D + c * 32);
+            // four columns of all rows side by side: a warp's stores are 512 bytes
+            float4* dst = reinterpret_cast<float4*>(p.ws_o + (ws_row - r) * D) + c * 8 * kBlockM + r;
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-              dst[i] = make_float4(__uint_as_float(o[4 * i]) * inv_l, __uint_as_float(o[4 * i + 1]) * inv_l,
-                                   __uint_as_float(o[4 * i + 2]) * inv_l, __uint_as_float(o[4 * i + 3]) * inv_l);
+              dst[i * kBlockM] =
+                  make_float4(__uint_as_float(o[4 * i]) * inv_l, __uint_as_float(o[4 * i + 1]) * inv_l,
+                              __uint_as_float(o[4 * i + 2]) * inv_l, __uint_as_float(o[4 * i + 3]) * inv_l);
           }
         }
         if (row_ok && lse_dst) *lse_dst = lse_row;
       }
     }
+    }  // segments
   }
 
   // ---- teardown
@@ -688,51 +932,58 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
   }
 }
 
-// Joins the key splits of the chunk kernel's rows, one warp per (token, query
-// head): LSE = log sum_s exp(LSE_s), O = sum_s exp(LSE_s - LSE) O_s.
+// Joins the parts of the items that the chunk kernel's runs cut: LSE = log sum_s
+// exp(LSE_s), O = sum_s exp(LSE_s - LSE) O_s, parts in the order of their keys.
+// Block x is for the item that the end of run x cuts first; a thread has 16
+// columns of one of its 256 rows, a warp 32 rows.
+constexpr int kJoinThreads = 256;
 template <int D, bool BF16>
-__global__ void __launch_bounds__(256) paged_join_kernel(const __grid_constant__ ChunkParams p) {
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ ChunkParams p) {
   const PagedAttn& a = p.a;
-  constexpr int E = D / 32;
-  __shared__ int sh_mine[8];  // per row of the block: a sequence of the chunk kernel holds its token
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long n_all = static_cast<long long>(a.r.total) * a.Hq;
-  const long long row0 = static_cast<long long>(blockIdx.x) * 8;
-  if (threadIdx.x < 8) sh_mine[threadIdx.x] = 0;
-  __syncthreads();
-  for (int b = threadIdx.x; b < a.r.B; b += 256) {
-    const Seq s = load_seq(a, b);
-    if (static_cast<long long>(s.nq) * a.group <= p.skip_rows) continue;
-    const long long lo = max(static_cast<long long>(s.c0) * a.Hq, row0);
-    const long long hi = min((static_cast<long long>(s.c0) + s.nq) * a.Hq, row0 + 8);
-    for (long long x = lo; x < hi; ++x) sh_mine[x - row0] = 1;
-  }
-  __syncthreads();
   ptx::grid_dep_wait();
-  const long long row = row0 + warp;
-  if (row >= n_all || !sh_mine[warp]) return;
-  const float ls = lane < p.n_splits ? __ldcg(p.ws_lse + lane * n_all + row) : -INFINITY;
-  float mx = ls;
+  const PagedCut c = p.ws_cuts[blockIdx.x];
+  if (c.parts == 0) return;
+  const int y = static_cast<int>(blockIdx.y * kJoinThreads + threadIdx.x);
+  const int r = y % kBlockM, col = y / kBlockM % (D / 16) * 16, g = y / (kBlockM * (D / 16));
+  const int tok = c.tok0 + g * p.tq + r / a.group;
+  if (r >= p.tq * a.group || tok >= c.nq) return;
+  // first row of query tile g in part x
+  auto tile_row = [&](int x) {
+    return ((x == 0 ? 2ll * blockIdx.x + 1 : 2ll * (blockIdx.x + x)) * 2 + g) * kBlockM;
+  };
+  float mx = -INFINITY;
+#pragma unroll 4
+  for (int x = 0; x < c.parts; ++x) mx = fmaxf(mx, __ldcg(p.ws_lse + tile_row(x) + r));
+  float acc[16] = {}, sum = 0.f;
+#pragma unroll 2
+  for (int x = 0; x < c.parts; ++x) {
+    const float4* src = reinterpret_cast<const float4*>(p.ws_o + tile_row(x) * D) + (col >> 2) * kBlockM + r;
+    float4 o[4];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-  float wgt = ls == -INFINITY ? 0.f : expf(ls - mx);  // (a NaN stays one)
-  float sum = wgt;
+    for (int e = 0; e < 4; ++e) o[e] = __ldcg(src + e * kBlockM);
+    const float ls = __ldcg(p.ws_lse + tile_row(x) + r);
+    // (a part without a key for this row has no O; a NaN stays one)
+    const float f = ls == -INFINITY ? 0.f : expf(ls - mx);
+    sum += f;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  float acc[E] = {};
-  for (int s = 0; s < p.n_splits; ++s) {
-    const float f = __shfl_sync(0xffffffffu, wgt, s);
-    if (f == 0.f) continue;
-    const float* src = p.ws_o + (s * n_all + row) * D + lane * E;
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = fmaf(f, __ldcg(src + e), acc[e]);
+    for (int e = 0; e < 4; ++e) {
+      acc[4 * e] = f == 0.f ? acc[4 * e] : fmaf(f, o[e].x, acc[4 * e]);
+      acc[4 * e + 1] = f == 0.f ? acc[4 * e + 1] : fmaf(f, o[e].y, acc[4 * e + 1]);
+      acc[4 * e + 2] = f == 0.f ? acc[4 * e + 2] : fmaf(f, o[e].z, acc[4 * e + 2]);
+      acc[4 * e + 3] = f == 0.f ? acc[4 * e + 3] : fmaf(f, o[e].w, acc[4 * e + 3]);
+    }
   }
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
-  uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.o) + row * D + lane * E);
+  const int hq = c.h * a.group + r % a.group;
+  const long long out = static_cast<long long>(c.c0 + tok) * a.Hq + hq;
+  uint32_t w[8];
 #pragma unroll
-  for (int e = 0; e < E / 2; ++e) dst[e] = pack2<BF16>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
-  if (lane == 0 && a.lse != nullptr)
-    a.lse[row % a.Hq * a.r.total + row / a.Hq] = sum == 0.f ? -INFINITY : mx + logf(sum);
+  for (int e = 0; e < 8; ++e) w[e] = pack2<BF16>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+  uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.o) + out * D + col);
+  dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  if (col == 0 && a.lse != nullptr)
+    a.lse[static_cast<long long>(hq) * a.r.total + c.c0 + tok] = sum == 0.f ? -INFINITY : mx + logf(sum);
 }
 
 // The visible keys and values of the chunk kernel's sequences as f16 rows:
@@ -895,7 +1146,7 @@ cudaError_t launch_expand_d(const ChunkParams& p, int kv, bool fold, int grid, c
 
 }  // namespace
 
-cudaError_t launch_paged_chunk(const ChunkParams& p, int head_dim, int kv, bool bf16, int grid, int sms,
+cudaError_t launch_paged_chunk(const ChunkParams& p, int head_dim, int kv, bool bf16, int sms,
                                cudaStream_t stream) {
   if (kv >= FA_DTYPE_INT8) {
     // enough warps to fill the GPU; they walk the rows there are
@@ -907,15 +1158,13 @@ cudaError_t launch_paged_chunk(const ChunkParams& p, int head_dim, int kv, bool 
                                          : launch_expand_d<128>(p, kv, bf16, g, stream);
     if (e != cudaSuccess) return e;
   }
-  return head_dim == 64 ? launch_chunk_d<64>(p, kv, bf16, grid, stream)
-                        : launch_chunk_d<128>(p, kv, bf16, grid, stream);
-}
-
-cudaError_t launch_paged_join(const ChunkParams& p, int head_dim, bool bf16, cudaStream_t stream) {
+  const cudaError_t e = head_dim == 64 ? launch_chunk_d<64>(p, kv, bf16, p.n_ctas, stream)
+                                       : launch_chunk_d<128>(p, kv, bf16, p.n_ctas, stream);
+  if (e != cudaSuccess || !p.runs || p.n_ctas == 1) return e;
+  // may start while the last runs finish; it waits for them before it reads
   cudaLaunchConfig_t cfg{};
-  const long long n_all = static_cast<long long>(p.a.r.total) * p.a.Hq;
-  cfg.gridDim = dim3(static_cast<unsigned>((n_all + 7) / 8));
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = dim3(p.n_ctas - 1, 2 * kBlockM * (head_dim / 16) / kJoinThreads);
+  cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

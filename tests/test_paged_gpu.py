@@ -443,3 +443,32 @@ def test_empty_calls(sm100):
     assert (o == 0).all() and (lse == -math.inf).all()
     k, v = fa.kvcache_read_paged(c["k_cache"], c["v_cache"], t0, zero[:1], e, 2)
     assert (k == 0).all() and (v == 0).all()
+
+
+@pytest.mark.parametrize("mode", [0, 1, 2])
+@pytest.mark.parametrize("kind", [(BF16, BF16), (F16, E4M3)], ids=["bf16", "f16-e4m3"])
+def test_key_tiles_of_many_items_in_equal_runs(sm100, kind, mode):
+    """A few long sequences between short, empty and keyless ones, more query
+    rows than the decode kernel takes: runs that cover several items, items that
+    several runs cut, items without keys, pairs whose second tile is empty."""
+    lens = [(90, 3000), (0, 0), (70, 70), (300, 100), (129, 129), (65, 5000), (40, 0), (257, 2300)]
+    P = Paged(lens, 2, 128, 32, kind[1], io=kind[0], seed=31)
+    q = P.new(2 * 2)
+    got = _attend(P, q, 4, mode)
+    _check(P, q, 4, mode, got)
+    again = _attend(P, q, 4, mode)
+    assert all(torch.equal(x, y) for x, y in zip(got, again))
+
+
+def test_one_long_item_cut_by_many_runs(sm100):
+    """One KV head, one pair of query tiles, 150 key tiles: parts of a few tiles."""
+    P = Paged([(70, 19111)], 1, 64, 64, F16, seed=33)
+    q = P.new(1)
+    _check(P, q, 1, 1, _attend(P, q, 1, 1))
+
+
+def test_many_sequences_without_keys(sm100):
+    """A batch bound to hold no keys at all: O = 0, LSE = -inf everywhere."""
+    P = Paged([(70, 0)] * 200, 2, 64, 16, F16, seed=35)
+    q = P.new(4)
+    _check(P, q, 4, 0, _attend(P, q, 4, 0))
