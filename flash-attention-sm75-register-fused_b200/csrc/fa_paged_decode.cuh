@@ -38,6 +38,11 @@
 // Short caches (DecodeParams::solo, at most 3 to 8 units per team) take one CTA per
 // (sequence, head) instead, whose teams share its units and join in shared
 // memory: one launch, no workspace, no plan over the batch.
+//
+// Measured with the join, 8 KV heads, d = 128, GQA 4, one token: 8 sequences x 8192
+// keys of f16 pages 47.1 us (5.7 TB/s; a plain copy runs at 6.5), one of 65536 over
+// e4m3 pages 32.7 us (4.2 TB/s): loads at HBM's rate between about 5 us until the
+// first unit and 3 to 6 for the join.
 #include "fa_paged.h"
 #include "fa_paged_dev.cuh"
 
@@ -131,7 +136,8 @@ __device__ __forceinline__ Seq load_short(const PagedAttn& a, int b, int max_row
 // The runs are cut from positions, not units: a segment (sequence, head) of n
 // units has kSegCost positions before its units' n, for what a team spends on a
 // segment besides its units (queries, results).  Without them the teams that
-// get many short sequences finish last.
+// get many short sequences finish last (32 ragged sequences over int8 pages: 37 us
+// without, 30 with, the kernel alone).
 constexpr int kSegCost = 1;
 __device__ __forceinline__ int positions_of(const PagedAttn& a, int b, int sub, int max_rows) {
   const int n = (load_short(a, b, max_rows).vis + sub - 1) / sub;
