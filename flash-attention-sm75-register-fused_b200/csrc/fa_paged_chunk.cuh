@@ -317,10 +317,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
       }
     }
   }
-  if (start.b < 0) {
-    if (p.runs && p.n_ctas > 1 && threadIdx.x == 0) p.ws_cuts[cta].parts = 0;
-    return;
-  }
+  // (whatever ends this CTA early, the join finds nothing to do for it)
+  if (p.runs && p.n_ctas > 1 && threadIdx.x == 0) p.ws_cuts[cta].parts = 0;
+  if (start.b < 0) return;
   const int n_rows = p.tq * a.group;  // rows of a tile in use
 
   // ---- set-up
@@ -447,7 +446,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
             }
           }
         }
-        if (lane == 0 && p.n_ctas > 1) p.ws_cuts[cta] = cut;
+        if (ok && lane == 0 && p.n_ctas > 1) p.ws_cuts[cta] = cut;
       }
       if (ok) {
         b = -1;
