@@ -1,5 +1,5 @@
 // Device-side view of a paged KV cache and of the new tokens of a call, and
-// the launchers of the paged kernels (fa_paged_cache.cu, fa_paged_decode.cu).
+// the launchers of the paged kernels (fa_paged_cache.cu, fa_paged_decode.cuh, fa_paged_chunk.cuh).
 #pragma once
 #include <cuda.h>
 #include <cuda_runtime.h>

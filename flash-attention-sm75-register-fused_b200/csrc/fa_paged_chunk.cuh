@@ -513,7 +513,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
           const int r0 = vis - tile * kBlockN;
           const int r1 = (r0 + p.box_rows - 1) / p.box_rows * p.box_rows;
           // (a run-time flag, though the expanded rows never have any: with the
-          // branch compiled out the softmax spills, 874 instead of 449 us)
+          // branch compiled out ptxas schedules the softmax of f16 results worse,
+          // 2 x 2048 tokens over 8192 keys take 487 us instead of 471, 421 instead
+          // of 394 at d = 64; bf16 results gain 2 %)
           const bool tail = p.stale && second && r0 < kBlockN && r0 != r1;
           const uint32_t full = tail ? bar(L::kBarTail) : bar(L::kBarFull + slot);
           const bool scales = kScaled && !second;
@@ -696,229 +698,229 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
     const uint32_t tO = tmem + lane_off + L::tO(g);
     bool ok = true;
     for (int n_seg = 0; ok && (ok = seg_ready(n_seg)); ++n_seg) {
-    ChunkItem it;
-    {
-      const volatile Segment& sg = segs[n_seg % kSegRing];
-      it.last = sg.b < 0;
-      it.h = sg.h;
-      it.s.c0 = sg.c0;
-      it.s.nq = sg.nq;
-      it.s.nk = sg.nk;
-      it.s.off = sg.off;
-      it.tok_lo = sg.tok0 + g * p.tq;
-      it.jb = sg.jb;
-      it.n_tiles = g ? sg.n1 : sg.n0;
-      it.slot = sg.slot;
-      it.tiles = sg.tiles;
-      it.par = (sg.parity >> g) & 1;
-    }
-    seg_done(n_seg);
-    if (it.last) break;
-    const int n_tiles = it.n_tiles;
-    const int tok_lo = it.tok_lo;
-    const int tok = tok_lo + r / a.group;      // token of the sequence
-    const int hq = it.h * a.group + r % a.group;
-    const bool row_ok = r < n_rows && tok < it.s.nq;
-    float sl = a.scale_log2;
-    if constexpr (kCastQ) {
-      // Q as f16 in the swizzled layout, one row per thread; a bf16 row is
-      // scaled by a power of two into f16's range, undone in sl
-      if (n_tiles > 0) {
-        uint4 q[D / 8];
-#pragma unroll
-        for (int c = 0; c < D / 8; ++c) q[c] = make_uint4(0u, 0u, 0u, 0u);
-        if (row_ok) {
-          const uint4* src = reinterpret_cast<const uint4*>(
-              a.q + static_cast<long long>(it.s.c0 + tok) * a.q_token + hq * a.q_head);
-#pragma unroll
-          for (int c = 0; c < D / 8; ++c) q[c] = __ldg(src + c);
-        }
-        {
-          auto f2 = [](uint32_t u) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&u)); };
-          float mx = 0.f;
-#pragma unroll
-          for (int c = 0; c < D / 8; ++c) {
-            const uint32_t u[4] = {q[c].x, q[c].y, q[c].z, q[c].w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) mx = fmaxf(mx, fmaxf(fabsf(f2(u[i]).x), fabsf(f2(u[i]).y)));
-          }
-          const uint32_t e = __float_as_uint(mx) & 0x7f800000u;
-          const bool plain = e == 0u || e >= 0x7e800000u;
-          const float inv = plain ? 1.f : __uint_as_float(0x7f000000u - e);
-          if (!plain) sl *= __uint_as_float(e);
-#pragma unroll
-          for (int c = 0; c < D / 8; ++c) {
-            uint32_t* u = reinterpret_cast<uint32_t*>(&q[c]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) u[i] = pack2<false>(f2(u[i]).x * inv, f2(u[i]).y * inv);
-          }
-        }
-        uint8_t* dst = smem + L::kOffQ + g * L::kTile + r * 128;
-#pragma unroll
-        for (int c = 0; c < D / 8; ++c)
-          *reinterpret_cast<uint4*>(dst + (c >> 3) * L::kBlockBytes + (((c & 7) ^ (r & 7)) << 4)) = q[c];
-        ptx::fence_proxy_async_smem();
-        ptx::mbar_arrive(bar(L::kBarQ + g));
-      }
-    }
-    // key limit of this row, and the smallest of the tile's rows
-    const int row_end = row_limit(a, it.s, tok);
-    const int tile_end = row_limit(a, it.s, tok_lo);
-
-    // (kScaled: P is multiplied by up to 2 and must stay in f16's range)
-    constexpr float kGrow = kScaled ? kRescaleThreshold - 1.0f : kRescaleThreshold;
-    float m = -INFINITY;  // running max of the scaled scores (log2 units)
-    float l = 0.f;        // running sum of exp2(s - m)
-    for (int j = 0; ok && j < n_tiles; ++j) {
-      ok = __all_sync(0xffffffffu, bar_wait(bar(L::kBarS + g), (it.par + j) & 1, wc, 20 + g));
-      if (!ok) break;
-      ptx::tc_fence_after();
-      float x[kBlockN];
+      ChunkItem it;
       {
-        uint32_t u0[32], u1[32], u2[32], u3[32];
-        ptx::tmem_ld32(tS + 0, u0);
-        ptx::tmem_ld32(tS + 32, u1);
-        ptx::tmem_ld32(tS + 64, u2);
-        ptx::tmem_ld32(tS + 96, u3);
-        ptx::tmem_wait_ld();
-        pin_after_wait<32>(u0);
-        pin_after_wait<32>(u1);
-        pin_after_wait<32>(u2);
-        pin_after_wait<32>(u3);
+        const volatile Segment& sg = segs[n_seg % kSegRing];
+        it.last = sg.b < 0;
+        it.h = sg.h;
+        it.s.c0 = sg.c0;
+        it.s.nq = sg.nq;
+        it.s.nk = sg.nk;
+        it.s.off = sg.off;
+        it.tok_lo = sg.tok0 + g * p.tq;
+        it.jb = sg.jb;
+        it.n_tiles = g ? sg.n1 : sg.n0;
+        it.slot = sg.slot;
+        it.tiles = sg.tiles;
+        it.par = (sg.parity >> g) & 1;
+      }
+      seg_done(n_seg);
+      if (it.last) break;
+      const int n_tiles = it.n_tiles;
+      const int tok_lo = it.tok_lo;
+      const int tok = tok_lo + r / a.group;      // token of the sequence
+      const int hq = it.h * a.group + r % a.group;
+      const bool row_ok = r < n_rows && tok < it.s.nq;
+      float sl = a.scale_log2;
+      if constexpr (kCastQ) {
+        // Q as f16 in the swizzled layout, one row per thread; a bf16 row is
+        // scaled by a power of two into f16's range, undone in sl
+        if (n_tiles > 0) {
+          uint4 q[D / 8];
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          x[c] = __uint_as_float(u0[c]);
-          x[32 + c] = __uint_as_float(u1[c]);
-          x[64 + c] = __uint_as_float(u2[c]);
-          x[96 + c] = __uint_as_float(u3[c]);
+          for (int c = 0; c < D / 8; ++c) q[c] = make_uint4(0u, 0u, 0u, 0u);
+          if (row_ok) {
+            const uint4* src = reinterpret_cast<const uint4*>(
+                a.q + static_cast<long long>(it.s.c0 + tok) * a.q_token + hq * a.q_head);
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c) q[c] = __ldg(src + c);
+          }
+          {
+            auto f2 = [](uint32_t u) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&u)); };
+            float mx = 0.f;
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c) {
+              const uint32_t u[4] = {q[c].x, q[c].y, q[c].z, q[c].w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i) mx = fmaxf(mx, fmaxf(fabsf(f2(u[i]).x), fabsf(f2(u[i]).y)));
+            }
+            const uint32_t e = __float_as_uint(mx) & 0x7f800000u;
+            const bool plain = e == 0u || e >= 0x7e800000u;
+            const float inv = plain ? 1.f : __uint_as_float(0x7f000000u - e);
+            if (!plain) sl *= __uint_as_float(e);
+#pragma unroll
+            for (int c = 0; c < D / 8; ++c) {
+              uint32_t* u = reinterpret_cast<uint32_t*>(&q[c]);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) u[i] = pack2<false>(f2(u[i]).x * inv, f2(u[i]).y * inv);
+            }
+          }
+          uint8_t* dst = smem + L::kOffQ + g * L::kTile + r * 128;
+#pragma unroll
+          for (int c = 0; c < D / 8; ++c)
+            *reinterpret_cast<uint4*>(dst + (c >> 3) * L::kBlockBytes + (((c & 7) ^ (r & 7)) << 4)) = q[c];
+          ptx::fence_proxy_async_smem();
+          ptx::mbar_arrive(bar(L::kBarQ + g));
         }
       }
-      const uint32_t entry = sbase + L::kOffScale + (kScaled ? ((it.tiles + j) % L::kScaleRing) * L::kScaleEntry : 0);
-      if constexpr (kScaled) {
+      // key limit of this row, and the smallest of the tile's rows
+      const int row_end = row_limit(a, it.s, tok);
+      const int tile_end = row_limit(a, it.s, tok_lo);
+
+      // (kScaled: P is multiplied by up to 2 and must stay in f16's range)
+      constexpr float kGrow = kScaled ? kRescaleThreshold - 1.0f : kRescaleThreshold;
+      float m = -INFINITY;  // running max of the scaled scores (log2 units)
+      float l = 0.f;        // running sum of exp2(s - m)
+      for (int j = 0; ok && j < n_tiles; ++j) {
+        ok = __all_sync(0xffffffffu, bar_wait(bar(L::kBarS + g), (it.par + j) & 1, wc, 20 + g));
+        if (!ok) break;
+        ptx::tc_fence_after();
+        float x[kBlockN];
+        {
+          uint32_t u0[32], u1[32], u2[32], u3[32];
+          ptx::tmem_ld32(tS + 0, u0);
+          ptx::tmem_ld32(tS + 32, u1);
+          ptx::tmem_ld32(tS + 64, u2);
+          ptx::tmem_ld32(tS + 96, u3);
+          ptx::tmem_wait_ld();
+          pin_after_wait<32>(u0);
+          pin_after_wait<32>(u1);
+          pin_after_wait<32>(u2);
+          pin_after_wait<32>(u3);
 #pragma unroll
-        for (int c = 0; c < kBlockN; c += 4) {
-          const float4 f = load_scales(entry + 4 * c);
-          ptx::fmul2(x[c], x[c + 1], x[c], x[c + 1], f.x, f.y);
-          ptx::fmul2(x[c + 2], x[c + 3], x[c + 2], x[c + 3], f.z, f.w);
+          for (int c = 0; c < 32; ++c) {
+            x[c] = __uint_as_float(u0[c]);
+            x[32 + c] = __uint_as_float(u1[c]);
+            x[64 + c] = __uint_as_float(u2[c]);
+            x[96 + c] = __uint_as_float(u3[c]);
+          }
         }
+        const uint32_t entry = sbase + L::kOffScale + (kScaled ? ((it.tiles + j) % L::kScaleRing) * L::kScaleEntry : 0);
+        if constexpr (kScaled) {
+#pragma unroll
+          for (int c = 0; c < kBlockN; c += 4) {
+            const float4 f = load_scales(entry + 4 * c);
+            ptx::fmul2(x[c], x[c + 1], x[c], x[c + 1], f.x, f.y);
+            ptx::fmul2(x[c + 2], x[c + 3], x[c + 2], x[c + 3], f.z, f.w);
+          }
+        }
+
+        const int key0 = (it.jb + j) * kBlockN;
+        const bool masked = key0 + kBlockN > tile_end;
+        float m_tile;
+        float sl_eff = sl;
+        if (masked) {
+          const int lim = row_end - key0;
+#pragma unroll
+          for (int c = 0; c < kBlockN; c += 2) ptx::fmul2(x[c], x[c + 1], x[c], x[c + 1], sl, sl);
+#pragma unroll
+          for (int c = 0; c < kBlockN; ++c)
+            if (c >= lim) x[c] = -INFINITY;
+          m_tile = row_extreme<kBlockN, false>(x);
+          sl_eff = 1.0f;
+        } else if (sl >= 0.f) {
+          m_tile = row_extreme<kBlockN, false>(x) * sl;
+        } else {
+          m_tile = row_extreme<kBlockN, true>(x) * sl;
+        }
+        const float m_new = fmaxf(m, m_tile);
+        const bool grow = m_new > m + kGrow;
+        if (j == 0) {
+          m = m_new;
+        } else {
+          if (__any_sync(0xffffffffu, grow)) {
+            const float alpha = grow ? ptx::ex2_approx(m - m_new) : 1.0f;
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+              uint32_t o[32];
+              ptx::tmem_ld32(tO + c * 32, o);
+              ptx::tmem_wait_ld();
+              pin_after_wait<32>(o);
+#pragma unroll
+              for (int i = 0; i < 32; i += 2) {
+                float a0 = __uint_as_float(o[i]), a1 = __uint_as_float(o[i + 1]);
+                ptx::fmul2(a0, a1, a0, a1, alpha, alpha);
+                o[i] = __float_as_uint(a0);
+                o[i + 1] = __float_as_uint(a1);
+              }
+              ptx::tmem_st32(tO + c * 32, o);
+            }
+            ptx::tmem_wait_st();
+            l *= alpha;
+          }
+          if (grow) m = m_new;
+        }
+        const float neg_m = (m == -INFINITY) ? 0.f : -m;
+        const uint32_t half_bar = bar(L::kBarPH + g);
+        auto announce = [half_bar] { ptx::mbar_arrive(half_bar); };
+        float tile_sum;
+        if constexpr (kScaled) {
+          tile_sum = masked ? exp_tile_scaled<false, kEmuPeriod>(x, sl_eff, neg_m, entry + 512, tP, announce)
+                            : exp_tile_scaled<true, kPairEmuPeriod<D>>(x, sl_eff, neg_m, entry + 512, tP, announce);
+        } else {
+          tile_sum = masked ? exp_tile<kBf16, false>(x, sl_eff, neg_m, tP, announce)
+                            : exp_tile<kBf16, true, kPairEmuPeriod<D>>(x, sl_eff, neg_m, tP, announce);
+        }
+        ptx::tmem_wait_st();
+        ptx::tc_fence_before();
+        ptx::mbar_arrive(bar(L::kBarP + g));
+        l += tile_sum;
       }
 
-      const int key0 = (it.jb + j) * kBlockN;
-      const bool masked = key0 + kBlockN > tile_end;
-      float m_tile;
-      float sl_eff = sl;
-      if (masked) {
-        const int lim = row_end - key0;
+      // ---- epilogue
+      using T = typename std::conditional<QBF16, __nv_bfloat16, __half>::type;
+      const long long row_id = static_cast<long long>(it.s.c0 + tok) * a.Hq + hq;
+      const bool partial = it.slot >= 0;
+      const long long ws_row = (static_cast<long long>(it.slot) * 2 + g) * kBlockM + r;
+      float* lse_dst = partial ? p.ws_lse + ws_row
+                       : a.lse ? a.lse + static_cast<long long>(hq) * a.r.total + it.s.c0 + tok
+                               : nullptr;
+      if (n_tiles == 0) {
+        if (row_ok && !partial) {
+          uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.o) + row_id * D);
 #pragma unroll
-        for (int c = 0; c < kBlockN; c += 2) ptx::fmul2(x[c], x[c + 1], x[c], x[c + 1], sl, sl);
+          for (int i = 0; i < D / 8; ++i) dst[i] = make_uint4(0u, 0u, 0u, 0u);
+        }
+        if (row_ok && lse_dst) *lse_dst = -INFINITY;
+      } else {
+        if (ok) ok = __all_sync(0xffffffffu, bar_wait(bar(L::kBarO + g), (it.par + n_tiles - 1) & 1, wc, 22 + g));
+        if (ok) {
+          ptx::tc_fence_after();
+          const float inv_l = (l > 0.f) ? 1.0f / l : (l == 0.f ? 0.f : l);  // (a NaN stays one)
+          const float m_use = (m == -INFINITY) ? 0.f : m;
+          const float lse_row =
+              l == 0.f ? -INFINITY : (m_use + __log2f(l)) * 0.69314718055994530942f;
 #pragma unroll
-        for (int c = 0; c < kBlockN; ++c)
-          if (c >= lim) x[c] = -INFINITY;
-        m_tile = row_extreme<kBlockN, false>(x);
-        sl_eff = 1.0f;
-      } else if (sl >= 0.f) {
-        m_tile = row_extreme<kBlockN, false>(x) * sl;
-      } else {
-        m_tile = row_extreme<kBlockN, true>(x) * sl;
-      }
-      const float m_new = fmaxf(m, m_tile);
-      const bool grow = m_new > m + kGrow;
-      if (j == 0) {
-        m = m_new;
-      } else {
-        if (__any_sync(0xffffffffu, grow)) {
-          const float alpha = grow ? ptx::ex2_approx(m - m_new) : 1.0f;
-#pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
             uint32_t o[32];
             ptx::tmem_ld32(tO + c * 32, o);
             ptx::tmem_wait_ld();
             pin_after_wait<32>(o);
+            if (!partial) {
+              uint32_t hv[16];
 #pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              float a0 = __uint_as_float(o[i]), a1 = __uint_as_float(o[i + 1]);
-              ptx::fmul2(a0, a1, a0, a1, alpha, alpha);
-              o[i] = __float_as_uint(a0);
-              o[i + 1] = __float_as_uint(a1);
+              for (int i = 0; i < 16; ++i)
+                hv[i] = pack2<QBF16>(__uint_as_float(o[2 * i]) * inv_l, __uint_as_float(o[2 * i + 1]) * inv_l);
+              if (row_ok) {
+                uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.o) + row_id * D + c * 32);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  dst[i] = make_uint4(hv[4 * i], hv[4 * i + 1], hv[4 * i + 2], hv[4 * i + 3]);
+              }
+            } else if (row_ok) {
+              // four columns of all rows side by side: a warp's stores are 512 bytes
+              float4* dst = reinterpret_cast<float4*>(p.ws_o + (ws_row - r) * D) + c * 8 * kBlockM + r;
+#pragma unroll
+              for (int i = 0; i < 8; ++i)
+                dst[i * kBlockM] =
+                    make_float4(__uint_as_float(o[4 * i]) * inv_l, __uint_as_float(o[4 * i + 1]) * inv_l,
+                                __uint_as_float(o[4 * i + 2]) * inv_l, __uint_as_float(o[4 * i + 3]) * inv_l);
             }
-            ptx::tmem_st32(tO + c * 32, o);
           }
-          ptx::tmem_wait_st();
-          l *= alpha;
+          if (row_ok && lse_dst) *lse_dst = lse_row;
         }
-        if (grow) m = m_new;
-      }
-      const float neg_m = (m == -INFINITY) ? 0.f : -m;
-      const uint32_t half_bar = bar(L::kBarPH + g);
-      auto announce = [half_bar] { ptx::mbar_arrive(half_bar); };
-      float tile_sum;
-      if constexpr (kScaled) {
-        tile_sum = masked ? exp_tile_scaled<false, kEmuPeriod>(x, sl_eff, neg_m, entry + 512, tP, announce)
-                          : exp_tile_scaled<true, kPairEmuPeriod<D>>(x, sl_eff, neg_m, entry + 512, tP, announce);
-      } else {
-        tile_sum = masked ? exp_tile<kBf16, false>(x, sl_eff, neg_m, tP, announce)
-                          : exp_tile<kBf16, true, kPairEmuPeriod<D>>(x, sl_eff, neg_m, tP, announce);
-      }
-      ptx::tmem_wait_st();
-      ptx::tc_fence_before();
-      ptx::mbar_arrive(bar(L::kBarP + g));
-      l += tile_sum;
-    }
-
-    // ---- epilogue
-    using T = typename std::conditional<QBF16, __nv_bfloat16, __half>::type;
-    const long long row_id = static_cast<long long>(it.s.c0 + tok) * a.Hq + hq;
-    const bool partial = it.slot >= 0;
-    const long long ws_row = (static_cast<long long>(it.slot) * 2 + g) * kBlockM + r;
-    float* lse_dst = partial ? p.ws_lse + ws_row
-                     : a.lse ? a.lse + static_cast<long long>(hq) * a.r.total + it.s.c0 + tok
-                             : nullptr;
-    if (n_tiles == 0) {
-      if (row_ok && !partial) {
-        uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.o) + row_id * D);
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) dst[i] = make_uint4(0u, 0u, 0u, 0u);
-      }
-      if (row_ok && lse_dst) *lse_dst = -INFINITY;
-    } else {
-      if (ok) ok = __all_sync(0xffffffffu, bar_wait(bar(L::kBarO + g), (it.par + n_tiles - 1) & 1, wc, 22 + g));
-      if (ok) {
-        ptx::tc_fence_after();
-        const float inv_l = (l > 0.f) ? 1.0f / l : (l == 0.f ? 0.f : l);  // (a NaN stays one)
-        const float m_use = (m == -INFINITY) ? 0.f : m;
-        const float lse_row =
-            l == 0.f ? -INFINITY : (m_use + __log2f(l)) * 0.69314718055994530942f;
-#pragma unroll
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t o[32];
-          ptx::tmem_ld32(tO + c * 32, o);
-          ptx::tmem_wait_ld();
-          pin_after_wait<32>(o);
-          if (!partial) {
-            uint32_t hv[16];
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              hv[i] = pack2<QBF16>(__uint_as_float(o[2 * i]) * inv_l, __uint_as_float(o[2 * i + 1]) * inv_l);
-            if (row_ok) {
-              uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.o) + row_id * D + c * 32);
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                dst[i] = make_uint4(hv[4 * i], hv[4 * i + 1], hv[4 * i + 2], hv[4 * i + 3]);
-            }
-          } else if (row_ok) {
-            // four columns of all rows side by side: a warp's stores are 512 bytes
-            float4* dst = reinterpret_cast<float4*>(p.ws_o + (ws_row - r) * D) + c * 8 * kBlockM + r;
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              dst[i * kBlockM] =
-                  make_float4(__uint_as_float(o[4 * i]) * inv_l, __uint_as_float(o[4 * i + 1]) * inv_l,
-                              __uint_as_float(o[4 * i + 2]) * inv_l, __uint_as_float(o[4 * i + 3]) * inv_l);
-          }
-        }
-        if (row_ok && lse_dst) *lse_dst = lse_row;
       }
     }
-    }  // segments
   }
 
   // ---- teardown
