@@ -1058,6 +1058,8 @@ const char* fa_error_string(int code) {
     case FA_ERR_PAGE_SIZE: return "page_size must be a positive multiple of 16";
     case FA_ERR_GROUP: return "at most 128 query heads per KV head";
     case FA_ERR_SCALES: return "8-bit caches need k_scale and v_scale, 16-bit caches take none";
+    case FA_ERR_STRIDE:
+      return "strides must be positive (0 only for heads and pages that are read, not written)";
     default: break;
   }
   if (code >= FA_ERR_TIMEOUT_BASE) return "device watchdog: an in-kernel wait timed out";

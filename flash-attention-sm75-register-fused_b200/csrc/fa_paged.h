@@ -112,6 +112,7 @@ cudaError_t launch_cache_read(const PagedCache& c, const PagedRows& r, void* k, 
 struct alignas(64) DecodeParams {
   CUtensorMap tm_k;  // (d, page rows, heads, pages), box (min(row, 128 bytes), 16, 1, 1)
   CUtensorMap tm_v;
+  int page_step, head_step;  // 1, or 0 where the map has one entry for all of them
   PagedAttn a;
   float* ws;
   // set by launch_paged_decode: teams of the launch, one CTA per (sequence,

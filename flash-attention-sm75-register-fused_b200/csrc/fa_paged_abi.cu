@@ -16,8 +16,8 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 bool is_8bit(int dtype) { return dtype == FA_DTYPE_INT8 || dtype == FA_DTYPE_E4M3; }
 
 // Checks the cache's description and the call's 16-bit type; fills the
-// device-side view.
-int check_cache(const fa_paged_cache* c, int dtype, fa::PagedCache* out) {
+// device-side view.  `writes`: no two entries may share memory.
+int check_cache(const fa_paged_cache* c, int dtype, bool writes, fa::PagedCache* out) {
   if (!c) return FA_ERR_INVALID_ARG;
   if (c->head_dim != 64 && c->head_dim != 128) return FA_ERR_UNSUPPORTED_HEAD_DIM;
   if (dtype != FA_DTYPE_F16 && dtype != FA_DTYPE_BF16) return FA_ERR_DTYPE;
@@ -35,6 +35,14 @@ int check_cache(const fa_paged_cache* c, int dtype, fa::PagedCache* out) {
       (reinterpret_cast<uintptr_t>(c->block_table) & 3u) ||
       (reinterpret_cast<uintptr_t>(c->k_scale) & 3u) || (reinterpret_cast<uintptr_t>(c->v_scale) & 3u))
     return FA_ERR_ALIGNMENT;
+  const long long least = writes ? 1 : 0;
+  if (c->row_stride <= 0 || (c->num_pages > 1 && c->page_stride < least) ||
+      (c->kv_heads > 1 && c->head_stride < least))
+    return FA_ERR_STRIDE;
+  if (writes && is_8bit(c->dtype) &&
+      (c->scale_row_stride == 0 || (c->num_pages > 1 && c->scale_page_stride == 0) ||
+       (c->kv_heads > 1 && c->scale_head_stride == 0)))
+    return FA_ERR_STRIDE;
   // positions are int32
   if (static_cast<long long>(c->max_pages) * c->page_size > (1LL << 30) || c->kv_heads > (1 << 14))
     return FA_ERR_TOO_LARGE;
@@ -180,30 +188,32 @@ int gcd_128(int x) {  // of x (a multiple of 16) and 128
   return g;
 }
 
-// Tensor maps of the pages, for boxes of `rows` rows (and 64 columns, or a
-// whole 8-bit row).  The stride of a dimension with one entry is free: any
-// valid one serves.
-bool page_maps(const fa_paged_cache& c, int rows, CUtensorMap* k, CUtensorMap* v) {
+// Tensor maps of the pages for the decode kernel, for boxes of `rows` rows (and
+// 64 columns, or a whole 8-bit row).  Heads or pages with a stride of 0 become
+// one entry, and the kernel's coordinate stays at 0; the stride of a dimension
+// with one entry is free: any valid one serves.
+bool page_maps(const fa_paged_cache& c, int rows, fa::DecodeParams* p) {
   const int es = is_8bit(c.dtype) ? 1 : 2;
   const unsigned long long row = static_cast<unsigned long long>(es) * c.head_dim;
-  auto st = [row, es](long long elems) { return elems > 0 ? static_cast<unsigned long long>(es) * elems : row; };
+  p->page_step = c.num_pages > 1 && c.page_stride > 0 ? 1 : 0;
+  p->head_step = c.kv_heads > 1 && c.head_stride > 0 ? 1 : 0;
   fa::TiledMap t{};
   t.type = es == 1 ? fa::TiledMap::kBytes : c.dtype == FA_DTYPE_BF16 ? fa::TiledMap::kBf16 : fa::TiledMap::kF16;
   t.rank = 4;
   t.dims[0] = c.head_dim;
   t.dims[1] = c.page_size;
-  t.dims[2] = c.kv_heads;
-  t.dims[3] = c.num_pages > 0 ? c.num_pages : 1;
-  t.strides[0] = st(c.row_stride);
-  t.strides[1] = st(c.head_stride);
-  t.strides[2] = st(c.page_stride);
+  t.dims[2] = p->head_step ? c.kv_heads : 1;
+  t.dims[3] = p->page_step ? c.num_pages : 1;
+  t.strides[0] = static_cast<unsigned long long>(es) * c.row_stride;
+  t.strides[1] = p->head_step ? static_cast<unsigned long long>(es) * c.head_stride : row;
+  t.strides[2] = p->page_step ? static_cast<unsigned long long>(es) * c.page_stride : row;
   t.box[0] = es == 1 ? c.head_dim : 64;
   t.box[1] = rows;
   t.box[2] = t.box[3] = 1;
   t.base = c.k;
-  if (!fa::host_tensor_map(k, t)) return false;
+  if (!fa::host_tensor_map(&p->tm_k, t)) return false;
   t.base = c.v;
-  return fa::host_tensor_map(v, t);
+  return fa::host_tensor_map(&p->tm_v, t);
 }
 
 // Tensor map of 128-byte column halves by groups of 8 rows (see ChunkParams):
@@ -236,7 +246,7 @@ bool tile_map(const void* base, int type, int head_dim, long long rows, unsigned
 // stride itself in head-major and token-major pages).
 bool chunk_maps(const fa_paged_cache& c, fa::ChunkParams* p) {
   const unsigned long long row = 2ull * c.head_dim;
-  const unsigned long long rs = c.row_stride > 0 ? 2ull * c.row_stride : row;
+  const unsigned long long rs = 2ull * c.row_stride;
   const unsigned long long hs = c.kv_heads > 1 ? 2ull * c.head_stride : 0;
   const unsigned long long ps = c.num_pages > 1 ? 2ull * c.page_stride : 0;
   unsigned long long g = hs, x = ps;
@@ -245,7 +255,7 @@ bool chunk_maps(const fa_paged_cache& c, fa::ChunkParams* p) {
     g = x;
     x = r;
   }
-  if (g == 0) g = row;  // one head of one page (or strides of zero)
+  if (g == 0) g = row;  // one head of one page, or all of them the same
   const unsigned long long planes = (c.num_pages > 1 ? (c.num_pages - 1ull) * (ps / g) : 0ull) +
                                     (c.kv_heads - 1ull) * (hs / g) + 1ull;
   if (planes > 0x7fffffffull || ps / g > 0x7fffffffull || hs / g > 0x7fffffffull) return false;
@@ -269,7 +279,6 @@ bool rows_maps(fa::ChunkParams& p, int head_dim, int heads) {
 bool query_map(const fa_paged_cache& c, int tq, const void* q, long long q_token, long long q_head,
                int Hq, int total, bool bf16, CUtensorMap* map) {
   const unsigned long long row = 2ull * c.head_dim;
-  auto st = [row](long long elems) { return elems > 0 ? 2ull * elems : row; };
   fa::TiledMap t{};
   t.type = bf16 ? fa::TiledMap::kBf16 : fa::TiledMap::kF16;
   t.base = q;
@@ -277,8 +286,8 @@ bool query_map(const fa_paged_cache& c, int tq, const void* q, long long q_token
   t.dims[0] = c.head_dim;
   t.dims[1] = Hq;
   t.dims[2] = total;
-  t.strides[0] = st(q_head);
-  t.strides[1] = st(q_token);
+  t.strides[0] = Hq > 1 ? 2ull * q_head : row;  // (free where there is one)
+  t.strides[1] = total > 1 ? 2ull * q_token : row;
   t.box[0] = 64;
   t.box[1] = Hq / c.kv_heads;
   t.box[2] = tq;
@@ -295,7 +304,7 @@ int fa_kvcache_write(const fa_paged_cache* cache, const void* K, const void* V,
                      const int* seqlens_k, int B, int total, int dtype, void* stream) {
   fa::PagedCache c;
   fa::PagedRows r;
-  if (int rc = check_cache(cache, dtype, &c)) return rc;
+  if (int rc = check_cache(cache, dtype, true, &c)) return rc;
   if (int rc = check_rows(cu_seqlens, seqlens_k, B, total, &r)) return rc;
   if (B == 0 || total == 0) return FA_OK;
   if (!K || !V) return FA_ERR_INVALID_ARG;
@@ -318,7 +327,7 @@ int fa_kvcache_read(const fa_paged_cache* cache, void* K, void* V, const int* cu
                     const int* seqlens_k, int B, int total, int dtype, void* stream) {
   fa::PagedCache c;
   fa::PagedRows r;
-  if (int rc = check_cache(cache, dtype, &c)) return rc;
+  if (int rc = check_cache(cache, dtype, false, &c)) return rc;
   if (int rc = check_rows(cu_seqlens, seqlens_k, B, total, &r)) return rc;
   if (total == 0) return FA_OK;
   if (!K || !V) return FA_ERR_INVALID_ARG;
@@ -348,7 +357,7 @@ int fa_fwd_paged(const fa_paged_cache* cache, const void* Q, long long q_token_s
                  int max_seqlen_k, float scale, int causal, int dtype, void* workspace,
                  size_t workspace_bytes, void* stream) {
   fa::PagedAttn a;
-  if (int rc = check_cache(cache, dtype, &a.c)) return rc;
+  if (int rc = check_cache(cache, dtype, false, &a.c)) return rc;
   if (int rc = check_rows(cu_seqlens_q, seqlens_k, B, total_q, &a.r)) return rc;
   if (Hq < 0 || max_seqlen_q < 0 || max_seqlen_k < 0) return FA_ERR_INVALID_ARG;
   if (causal < FA_CAUSAL_NONE || causal > FA_CAUSAL_TOP_LEFT) return FA_ERR_INVALID_ARG;
@@ -360,6 +369,7 @@ int fa_fwd_paged(const fa_paged_cache* cache, const void* Q, long long q_token_s
   if (!aligned16(Q) || !aligned16(O) || !aligned16(workspace) ||
       ((q_token_stride | q_head_stride) & 7) || (reinterpret_cast<uintptr_t>(lse) & 3u))
     return FA_ERR_ALIGNMENT;
+  if ((total_q > 1 && q_token_stride <= 0) || (Hq > 1 && q_head_stride <= 0)) return FA_ERR_STRIDE;
   const int group = Hq / a.c.heads;
   const bool eight = is_8bit(cache->dtype);
   const PagedPlan k = make_paged_plan(B, a.c.heads, group, cache->head_dim, cache->dtype, total_q, max_seqlen_q,
@@ -390,7 +400,7 @@ int fa_fwd_paged(const fa_paged_cache* cache, const void* Q, long long q_token_s
     p.max_rows = k.decode_rows;
     p.epoch = fa::host_next_epoch();
     p.timeout_ns = fa::host_timeout_ns();
-    if (!page_maps(*cache, 16, &p.tm_k, &p.tm_v)) return FA_ERR_TENSOR_MAP;
+    if (!page_maps(*cache, 16, &p)) return FA_ERR_TENSOR_MAP;
     if (fa::launch_paged_decode(p, cache->head_dim, cache->dtype, bf16, fa::host_sm_count(), st) !=
         cudaSuccess)
       return FA_ERR_LAUNCH;

@@ -395,7 +395,8 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
     __syncwarp();
     if (boxes)
       ptx::tma_load_4d(ring + wstage * 8192 + box_dst, box_map, bar, bcol * (C::kBoxBytes / (C::k8 ? 1 : 2)),
-                       a.c.row_in_page(key0 + 16 * bgrp), ci.h, page, policy);
+                       a.c.row_in_page(key0 + 16 * bgrp), ci.h * p.head_step,
+                       page < 0 ? -1 : page * p.page_step, policy);
     if constexpr (C::k8) {
       const int left = ci.s.vis - key0;
 #pragma unroll

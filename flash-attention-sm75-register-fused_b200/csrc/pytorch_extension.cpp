@@ -470,7 +470,7 @@ int64_t stride_of(const torch::Tensor& t, int64_t dim) {
 fa_paged_cache paged_cache(const torch::Tensor& k, const torch::Tensor& v,
                            const torch::Tensor& table, const c10::optional<torch::Tensor>& ks,
                            const c10::optional<torch::Tensor>& vs, const torch::Device& device,
-                           torch::ScalarType dtype) {
+                           torch::ScalarType dtype, bool writes = false) {
   TORCH_CHECK(k.is_cuda() && k.device() == device && v.device() == device,
               "k_cache and v_cache must be on the inputs' CUDA device");
   TORCH_CHECK_VALUE(k.dim() == 4 && v.dim() == 4,
@@ -496,6 +496,9 @@ fa_paged_cache paged_cache(const torch::Tensor& k, const torch::Tensor& v,
     TORCH_CHECK(st == stride_of(v, i), "k_cache and v_cache must have the same strides");
     TORCH_CHECK(st * static_cast<int64_t>(k.element_size()) % 16 == 0,
                 "the pages' strides must be multiples of 16 bytes");
+    TORCH_CHECK(k.size(i) <= 1 || st > 0 || (i < 2 && !writes),
+                writes ? "pages that are written cannot be broadcast tensors"
+                       : "the rows of a page cannot be a broadcast dimension");
   }
   TORCH_CHECK(k.size(0) <= INT32_MAX && k.size(1) <= INT32_MAX && k.size(2) <= INT32_MAX,
               "size exceeds int32");
@@ -514,6 +517,8 @@ fa_paged_cache paged_cache(const torch::Tensor& k, const torch::Tensor& v,
       for (int64_t i = 0; i < 3; ++i)
         TORCH_CHECK(stride_of(*t, i) == stride_of(*ks, i),
                     "k_scale and v_scale must have the same strides");
+      for (int64_t i = 0; writes && i < 3; ++i)
+        TORCH_CHECK(t->size(i) <= 1 || t->stride(i) > 0, "scales that are written cannot be broadcast tensors");
     }
     c.k_scale = ks->data_ptr<float>();
     c.v_scale = vs->data_ptr<float>();
@@ -580,10 +585,12 @@ torch::Tensor new_result(at::IntArrayRef sizes, torch::ScalarType dtype, const t
 }
 
 // `t` itself if the kernels can read it in place (contiguous rows, token and
-// head strides and base multiples of 16 bytes), else a contiguous copy.
-torch::Tensor readable_rows(const torch::Tensor& t) {
+// head strides and base multiples of 16 bytes; no broadcast dimension where a
+// tensor map describes it), else a contiguous copy.
+torch::Tensor readable_rows(const torch::Tensor& t, bool mapped = false) {
   if (t.numel() == 0) return t;
-  const bool ok = t.stride(2) == 1 && stride_of(t, 0) % 8 == 0 && stride_of(t, 1) % 8 == 0 &&
+  const bool repeats = (t.size(0) > 1 && t.stride(0) == 0) || (t.size(1) > 1 && t.stride(1) == 0);
+  const bool ok = t.stride(2) == 1 && !(mapped && repeats) && stride_of(t, 0) % 8 == 0 && stride_of(t, 1) % 8 == 0 &&
                   reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
   return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
@@ -600,7 +607,7 @@ void kvcache_write_paged(const torch::Tensor& k_in, const torch::Tensor& v_in,
   TORCH_CHECK(k_in.sizes() == v_in.sizes() && k_in.scalar_type() == v_in.scalar_type() &&
                   k_in.device() == v_in.device(),
               "k and v must share shape, dtype and device");
-  const auto c = paged_cache(k_cache, v_cache, table, ks, vs, k_in.device(), k_in.scalar_type());
+  const auto c = paged_cache(k_cache, v_cache, table, ks, vs, k_in.device(), k_in.scalar_type(), /*writes=*/true);
   TORCH_CHECK(k_in.size(1) == c.kv_heads && k_in.size(2) == c.head_dim,
               "k and v must be [total, ", c.kv_heads, ", ", c.head_dim, "] for these pages");
   const int B = paged_batch(cu, lens, table, k_in.device());
@@ -656,7 +663,7 @@ pybind11::object flash_attention_forward_paged(
                   max_seqlen_k <= INT32_MAX,
               "max_seqlen_q and max_seqlen_k must be lengths");
   const c10::cuda::CUDAGuard guard(q_in.device());
-  const auto q = readable_rows(q_in);
+  const auto q = readable_rows(q_in, /*mapped=*/true);
   const int Hq = static_cast<int>(q.size(1)), total = static_cast<int>(q.size(0));
   auto O = new_result(q.sizes(), q.scalar_type(), q.device());
   torch::Tensor lse;

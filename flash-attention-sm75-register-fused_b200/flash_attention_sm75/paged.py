@@ -7,7 +7,8 @@ values, in any memory order with contiguous rows (token-major pages are passed
 as ``pages.transpose(1, 2)``), of fp16 / bf16, or of int8 / float8_e4m3fn with
 fp32 scales ``[num_pages, H_kv, page_size]`` (one per token and head, any
 strides).  Position ``p`` of sequence ``b`` is row ``p % page_size`` of page
-``block_table[b, p // page_size]``.
+``block_table[b, p // page_size]``.  Pages (and scales) broadcast over heads can
+be read and attended over, not written.
 
 All three functions describe tokens in the same way: sequence ``b`` has the
 packed rows ``[cu_seqlens[b], cu_seqlens[b + 1])``, and the last of them is

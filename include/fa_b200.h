@@ -43,6 +43,7 @@ enum {
   FA_ERR_PAGE_SIZE = 12,           /* paged cache: page_size not a positive multiple of 16 */
   FA_ERR_GROUP = 13,               /* paged attention: more than 128 query heads per KV head */
   FA_ERR_SCALES = 14,              /* 8-bit cache without scales, or a 16-bit cache with them */
+  FA_ERR_STRIDE = 15,              /* paged cache or its queries: a stride that cannot be used */
   FA_ERR_TIMEOUT_BASE = 100        /* device watchdog: 100 + wait site id */
 };
 
@@ -221,7 +222,11 @@ int fa_bwd_varlen(const void* Q, const void* K, const void* V, const void* O, co
  * row * row_stride + c] (strides in elements; V the same from v), so head-major
  * pages [num_pages, kv_heads, page_size, d], token-major pages
  * [num_pages, page_size, kv_heads, d] and slices of a larger array all fit.
- * Pointers are 16-byte aligned and the strides multiples of 16 bytes.
+ * Pointers are 16-byte aligned and the strides multiples of 16 bytes; the row
+ * stride is positive, the others not negative (where a dimension has one entry,
+ * its stride is not used).  A head or page stride of 0, the same rows seen as
+ * several heads or pages, is for reading alone: writes refuse it, and a scale
+ * stride of 0, with FA_ERR_STRIDE.
  *
  * Position p of sequence b is row p % page_size of page
  * block_table[b * table_stride + p / page_size] (int32, on the device).  Table
@@ -292,7 +297,8 @@ int fa_kvcache_read(const fa_paged_cache* cache, void* K, void* V, const int* cu
 /*
  * fa_fwd_paged — attention of new tokens over a paged cache that already holds
  * their own keys and values: Q row (t, h) at t * q_token_stride +
- * h * q_head_stride (elements, multiples of 8; 16-byte aligned), O
+ * h * q_head_stride (elements, multiples of 8, positive where there is more than
+ * one token / head; 16-byte aligned), O
  * [total_q, Hq, d] contiguous, LSE (may be NULL) fp32 [Hq, total_q].  Sequence
  * b's queries see keys j < seqlens_k[b], with `causal` FA_CAUSAL_BOTTOM_RIGHT
  * those with j <= i + seqlens_k[b] - n_b, with FA_CAUSAL_TOP_LEFT j <= i.  Rows

@@ -1,0 +1,94 @@
+"""Paged KV cache on the GPU, at the edges: broadcast tensors, loose and tight
+bounds, scales of very different size, large caches, many heads and sequences,
+captured graphs, and the C entry points.  Compared with the plain 64-bit forms
+and tolerances of tests/paged_plain.py."""
+import pytest
+import torch
+
+import flash_attention_sm75 as fa
+from tests.paged_plain import Paged
+from tests.test_paged_gpu import BF16, E4M3, F16, I8, _attend, _check
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------ broadcast tensors
+
+@pytest.mark.parametrize("nq", [1, 40])
+@pytest.mark.parametrize("kind", [(F16, F16), (BF16, BF16), (F16, I8), (BF16, E4M3)],
+                         ids=["f16", "bf16", "f16-int8", "bf16-e4m3"])
+def test_queries_broadcast_over_heads_and_tokens(sm100, nq, kind):
+    """Queries expanded over heads, over tokens, and over both."""
+    P = Paged([(nq, 300), (nq, 77)], 2, 64, 16, kind[1], io=kind[0], seed=41)
+    one = (torch.randn(P.total, 8, 64, generator=P.g)).to(kind[0]).cuda()
+    for q in (one[:, :1].expand(-1, 8, -1), one[:1].expand(P.total, -1, -1),
+              one[:1, :1].expand(P.total, 8, -1)):
+        _check(P, q.cpu(), 8, 1, _attend(P, q, 8, 1))
+
+
+@pytest.mark.parametrize("nq", [1, 40])
+@pytest.mark.parametrize("kind", [(F16, F16), (BF16, BF16), (F16, E4M3), (BF16, I8)],
+                         ids=["f16", "bf16", "f16-e4m3", "bf16-int8"])
+def test_pages_broadcast_over_heads(sm100, nq, kind):
+    """One KV head of pages seen as several: attention and reading back."""
+    P = Paged([(nq, 300), (nq, 77)], 1, 128, 32, kind[1], io=kind[0], seed=42)
+    c = P.cuda()
+    for name in ("k_cache", "v_cache"):
+        c[name] = c[name].expand(-1, 3, -1, -1)
+    for name in ("k_scale", "v_scale"):
+        c[name] = None if c[name] is None else c[name].expand(-1, 3, -1)
+    q = P.new(6)
+    got = _attend(P, q, 6, 1, c=c)
+    _check(P, q, 6, 1, got)  # (the same values under one head)
+    n = [x for _, x in P.lens]
+    k, _ = fa.kvcache_read_paged(c["k_cache"], c["v_cache"], c["table"], [0, n[0], sum(n)], c["lens"], sum(n),
+                                 k_scale=c["k_scale"], v_scale=c["v_scale"], dtype=kind[0])
+    want = torch.cat([P.held("k", b, n[b]) for b in range(2)]).float().to(kind[0])
+    assert torch.equal(k.cpu(), want.expand(-1, 3, -1))
+
+
+@pytest.mark.parametrize("nq", [1, 40])
+def test_pages_broadcast_over_pages(sm100, nq):
+    """One page seen as several."""
+    P = Paged([(nq, 16)], 2, 64, 16, F16, seed=43, spare=0)
+    c = P.cuda()
+    c["k_cache"], c["v_cache"] = c["k_cache"].expand(9, -1, -1, -1), c["v_cache"].expand(9, -1, -1, -1)
+    c["table"] = torch.tensor([[0, 7, 3, 8, -1, 2]], dtype=torch.int32, device="cuda")
+    c["lens"].fill_(90)
+    P.table, P.lens = torch.tensor([[0, 0, 0, 0, 1, 0]], dtype=torch.int32), [(nq, 90)]
+    P.k, P.v = (torch.cat([x, torch.zeros_like(x)]) for x in (P.k, P.v))  # (no page: zeros)
+    q = P.new(4)
+    _check(P, q, 4, 1, _attend(P, q, 4, 1, c=c))
+
+
+def test_new_rows_broadcast_into_the_cache(sm100):
+    """New keys and values expanded over heads are written as any others."""
+    P = Paged([(5, 40), (3, 3)], 4, 64, 16, F16, seed=44)
+    c = P.cuda()
+    x = torch.randn(P.total, 1, 64, generator=P.g).half().cuda()
+    fa.kvcache_write_paged(x.expand(-1, 4, -1), x.expand(-1, 4, -1), c["k_cache"], c["v_cache"], c["table"],
+                           c["cu"], c["lens"])
+    for got in fa.kvcache_read_paged(c["k_cache"], c["v_cache"], c["table"], c["cu"], c["lens"], P.total):
+        assert torch.equal(got, x.expand(-1, 4, -1))
+
+
+def test_writes_into_broadcast_pages_are_refused(sm100):
+    P = Paged([(2, 20)], 1, 64, 16, I8, seed=45)
+    c = P.cuda()
+    x = P.new(2).cuda()
+
+    def write(heads_c, heads_s, x):
+        fa.kvcache_write_paged(x, x, c["k_cache"].expand(-1, heads_c, -1, -1), c["v_cache"].expand(-1, heads_c, -1, -1),
+                               c["table"], c["cu"], c["lens"], k_scale=c["k_scale"].expand(-1, heads_s, -1),
+                               v_scale=c["v_scale"].expand(-1, heads_s, -1))
+
+    with pytest.raises(RuntimeError, match="pages that are written"):
+        write(2, 2, x)
+    own = [c[n].expand(-1, 2, -1, -1).contiguous() for n in ("k_cache", "v_cache")]
+    c["k_cache"], c["v_cache"] = own
+    with pytest.raises(RuntimeError, match="scales that are written"):
+        fa.kvcache_write_paged(x, x, *own, c["table"], c["cu"], c["lens"], k_scale=c["k_scale"].expand(-1, 2, -1),
+                               v_scale=c["v_scale"].expand(-1, 2, -1))
+    row = torch.zeros(3, 2, 1, 64, dtype=F16, device="cuda").expand(-1, -1, 16, -1)
+    with pytest.raises(RuntimeError, match="rows of a page"):
+        fa.flash_attention_forward_paged(x, row, row, c["table"], c["cu"], c["lens"], 2, 20)
