@@ -15,6 +15,8 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 
 bool is_8bit(int dtype) { return dtype == FA_DTYPE_INT8 || dtype == FA_DTYPE_E4M3; }
 
+constexpr int kMaxHeads = 1 << 14, kMaxBatch = 1 << 20, kMaxRows = 1 << 28;
+
 // Checks the cache's description and the call's 16-bit type; fills the
 // device-side view.  `writes`: no two entries may share memory.
 int check_cache(const fa_paged_cache* c, int dtype, bool writes, fa::PagedCache* out) {
@@ -44,7 +46,7 @@ int check_cache(const fa_paged_cache* c, int dtype, bool writes, fa::PagedCache*
        (c->kv_heads > 1 && c->scale_head_stride == 0)))
     return FA_ERR_STRIDE;
   // positions are int32
-  if (static_cast<long long>(c->max_pages) * c->page_size > (1LL << 30) || c->kv_heads > (1 << 14))
+  if (static_cast<long long>(c->max_pages) * c->page_size > (1LL << 30) || c->kv_heads > kMaxHeads)
     return FA_ERR_TOO_LARGE;
   out->k = static_cast<const uint8_t*>(c->k);
   out->v = static_cast<const uint8_t*>(c->v);
@@ -70,7 +72,7 @@ int check_cache(const fa_paged_cache* c, int dtype, bool writes, fa::PagedCache*
 
 int check_rows(const int* cu, const int* lens, int B, int total, fa::PagedRows* out) {
   if (B < 0 || total < 0) return FA_ERR_INVALID_ARG;
-  if (B > (1 << 20) || total > (1 << 28)) return FA_ERR_TOO_LARGE;
+  if (B > kMaxBatch || total > kMaxRows) return FA_ERR_TOO_LARGE;
   if (B > 0 && total > 0 && (!cu || !lens)) return FA_ERR_INVALID_ARG;
   if ((reinterpret_cast<uintptr_t>(cu) & 3u) || (reinterpret_cast<uintptr_t>(lens) & 3u))
     return FA_ERR_ALIGNMENT;
@@ -344,8 +346,12 @@ int fa_kvcache_read(const fa_paged_cache* cache, void* K, void* V, const int* cu
 size_t fa_fwd_paged_workspace_bytes(const fa_paged_cache* cache, int B, int Hq, int total_q,
                                     int max_seqlen_q, int max_seqlen_k) {
   if (!cache || cache->kv_heads <= 0 || Hq <= 0 || total_q <= 0) return 0;
-  const int group = Hq / cache->kv_heads > 0 ? Hq / cache->kv_heads : 1;
-  if (group > 128 || B < 0 || max_seqlen_q < 0 || max_seqlen_k < 0) return 0;  // refused sizes
+  const int group = Hq / cache->kv_heads;
+  // what the call refuses
+  if (group * cache->kv_heads != Hq || group > 128 || B < 0 || max_seqlen_q < 0 || max_seqlen_k < 0 ||
+      (cache->head_dim != 64 && cache->head_dim != 128) || cache->dtype < FA_DTYPE_F16 ||
+      cache->dtype > FA_DTYPE_E4M3 || cache->kv_heads > kMaxHeads || B > kMaxBatch || total_q > kMaxRows)
+    return 0;
   return make_paged_plan(B, cache->kv_heads, group, cache->head_dim, cache->dtype, total_q,
                          max_seqlen_q, max_seqlen_k)
       .ws_bytes;

@@ -324,7 +324,7 @@ int fa_fwd_paged(const fa_paged_cache* cache, const void* Q, long long q_token_s
 /* Workspace bytes of fa_fwd_paged (a function of its sizes alone): partial
  * results of split keys, and for chunks over 8-bit pages the keys and values as
  * f16 (at most about 1 GiB, or one KV head's if that is more); 0 for a few new
- * tokens over short caches. */
+ * tokens over short caches, and for what the call refuses. */
 size_t fa_fwd_paged_workspace_bytes(const fa_paged_cache* cache, int B, int Hq, int total_q,
                                     int max_seqlen_q, int max_seqlen_k);
 

@@ -1,5 +1,5 @@
 """Paged KV cache, host side, at the edges: strides that the C entry points
-refuse (no GPU is touched)."""
+refuse, and the workspace query (no GPU is touched)."""
 import ctypes
 
 from tests import abi_ctypes as abi
@@ -36,3 +36,15 @@ def test_unusable_strides_are_refused():
 
     assert attend(256, 0) == STRIDE and attend(0, 64) == STRIDE and attend(-256, 64) == STRIDE
     assert abi.load().fa_error_string(STRIDE) not in (b"ok", b"unknown error")
+
+
+def test_workspace_query_answers_0_for_what_the_call_refuses():
+    f = abi.load().fa_fwd_paged_workspace_bytes
+    eight = dict(k_scale=P16, v_scale=P16)
+    for kw in (dict(head_dim=0), dict(head_dim=96), dict(head_dim=8192), dict(head_dim=-64), dict(dtype=-1),
+               dict(dtype=4, **eight), dict(kv_heads=3), dict(kv_heads=1 << 20)):
+        for args in ((1, 4, 1, 1, 8192), (8, 4, 8, 1, 1 << 20), (1, 4, 99, 99, 64)):
+            assert f(ctypes.byref(_cache(**kw)), *args) == 0, (kw, args)
+    assert f(ctypes.byref(abi.PagedCache(kv_heads=1)), 1, 4, 9, 9, 64) == 0  # all else zero
+    assert f(ctypes.byref(_cache()), 1 << 21, 4, 9, 9, 64) == 0
+    assert f(ctypes.byref(_cache()), 1, 4, 1 << 29, 9, 64) == 0
