@@ -114,6 +114,7 @@ constexpr size_t kExpandBytes = size_t{1} << 30;
 PagedPlan make_paged_plan(int B, int heads, int group, int head_dim, int dtype, int total, int max_q,
                           int max_k) {
   const bool eight = is_8bit(dtype);
+  if (max_q > total) max_q = total;  // (a bound that is looser than it can be)
   PagedPlan k;
   const int sms = fa::host_sm_count();
   const long long rows = static_cast<long long>(max_q) * group;

@@ -13,6 +13,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "fa_b200.h"
@@ -673,7 +674,10 @@ pybind11::object flash_attention_forward_paged(
     return pybind11::make_tuple(O, lse);
   };
   if (q.numel() == 0) return result();
-  const int mq = static_cast<int>(max_seqlen_q), mk = static_cast<int>(max_seqlen_k);
+  // no sequence is longer than its row of the table, whatever bound was given:
+  // the plan and the workspace go by what can be
+  const int mq = static_cast<int>(max_seqlen_q);
+  const int mk = static_cast<int>(std::min(max_seqlen_k, static_cast<int64_t>(c.max_pages) * c.page_size));
   const size_t ws_bytes = fa_fwd_paged_workspace_bytes(&c, B, Hq, total, mq, mk);
   torch::Tensor ws;
   if (ws_bytes > 0) ws = new_result({static_cast<int64_t>(ws_bytes)}, torch::kUInt8, q.device());

@@ -89,7 +89,8 @@ def flash_attention_forward_paged(q, k_cache, v_cache, block_table, cu_seqlens_q
         cu_seqlens_q: B + 1 row offsets of q (int32 tensor or ints); one
             token per sequence, a few, chunks, or any mixture
         max_seqlen_q, max_seqlen_k: upper bounds of the new tokens and of
-            seqlens_k
+            seqlens_k (loose ones cost: over 8-bit pages the workspace of a
+            chunk grows with B x max_seqlen_k, up to what the table can hold)
         causal, causal_alignment: "bottom_right" (token i of a sequence sees
             keys j <= i + n_k - n_q: the tokens are the cache's last ones) or
             "top_left" (j <= i)

@@ -309,7 +309,9 @@ int fa_kvcache_read(const fa_paged_cache* cache, void* K, void* V, const int* cu
  * values of 8-bit pages may be read as f16: with bf16 results magnitudes above
  * 65504 then count as 65504 and those below 2^-24 as 0.
  * max_seqlen_q / max_seqlen_k bound n_b and seqlens_k (tokens and keys beyond
- * them are not computed / not seen).  Hq / kv_heads is at most 128.
+ * them are not computed / not seen).  The kernels and the workspace are chosen by
+ * max_seqlen_k as it is given, so it should be no more than the longest sequence
+ * there may be, and never more than max_pages * page_size.  Hq / kv_heads is at most 128.
  * `workspace` (16-byte aligned) needs fa_fwd_paged_workspace_bytes() bytes (may
  * be NULL where that is 0).  Asynchronous on `stream`.
  *

@@ -92,3 +92,37 @@ def test_writes_into_broadcast_pages_are_refused(sm100):
     row = torch.zeros(3, 2, 1, 64, dtype=F16, device="cuda").expand(-1, -1, 16, -1)
     with pytest.raises(RuntimeError, match="rows of a page"):
         fa.flash_attention_forward_paged(x, row, row, c["table"], c["cu"], c["lens"], 2, 20)
+
+
+# ------------------------------------------------------------------ lengths and their bounds
+
+@pytest.mark.parametrize("nq", [1, 40])
+@pytest.mark.parametrize("cache", [F16, I8], ids=["f16", "int8"])
+def test_loose_bounds_cost_no_memory(sm100, nq, cache):
+    """Bounds far above what the batch and its table can hold."""
+    P = Paged([(nq, 300), (nq, 77)], 2, 128, 16, cache, seed=50)
+    q = P.new(8).cuda()
+    c = P.cuda()
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = fa.flash_attention_forward_paged(q, c["k_cache"], c["v_cache"], c["table"], c["cu"], c["lens"], 1 << 30,
+                                           1 << 30, causal=True, k_scale=c["k_scale"], v_scale=c["v_scale"],
+                                           return_lse=True)
+    assert torch.cuda.max_memory_allocated() - before < 256 << 20
+    _check(P, q.cpu(), 8, 1, got)
+
+
+@pytest.mark.parametrize("io", [F16, BF16])
+def test_wide_tables_go_head_group_by_head_group(sm100, io):
+    """A table whose sequences' expanded 8-bit keys would pass 1 GiB for all heads: the
+    chunk kernel runs a few heads at a time."""
+    P = Paged([(150, 700), (90, 90)], 6, 128, 32, I8, io=io, seed=21)
+    q = P.new(12)
+    c = P.cuda()
+    wide = torch.full((2, 1 << 13), -1, dtype=torch.int32, device="cuda")
+    wide[:, :c["table"].size(1)] = c["table"]
+    got = fa.flash_attention_forward_paged(q.cuda(), c["k_cache"], c["v_cache"], wide, c["cu"], c["lens"], 150,
+                                           1 << 18, causal=True, k_scale=c["k_scale"], v_scale=c["v_scale"],
+                                           return_lse=True)
+    _check(P, q, 12, 1, got)
