@@ -39,7 +39,8 @@ __device__ __forceinline__ void widen(uint32_t w, uint32_t& p0, uint32_t& p1) {
 // What a sequence brings to a call.
 struct Seq {
   int c0, nq;    // first packed row; new tokens
-  int nk, off;   // visible keys: key j < lim(i) = min(nk, i + off + 1) (causal) or nk
+  int nk, off;   // visible keys: key j < lim(i) = min(nk, i + off + 1) (causal) or nk;
+                 // off goes by the whole length, also where bounds cut nk
   int vis;       // keys any of its rows may see
 };
 
@@ -51,12 +52,13 @@ __device__ __forceinline__ Seq load_seq(const PagedAttn& a, int b) {
   Seq s;
   const int c0 = min(max(__ldg(a.r.cu + b), 0), a.r.total);
   const int c1 = min(max(__ldg(a.r.cu + b + 1), c0), a.r.total);
-  const int len = __ldg(a.r.lens + b);
+  // (beyond 2^30 keys and 2^28 new tokens every token sees all keys a table can hold)
+  const int len = min(max(__ldg(a.r.lens + b), 0), 3 << 29);
   const int n = c1 - c0;
   s.c0 = c0;
   s.nq = min(n, a.max_q);
-  s.nk = max(min(min(len, a.max_k), a.c.max_pages * a.c.page_size), 0);
-  s.off = a.causal == FA_CAUSAL_BOTTOM_RIGHT ? s.nk - n : 0;
+  s.nk = min(min(len, a.max_k), a.c.max_pages * a.c.page_size);
+  s.off = a.causal == FA_CAUSAL_BOTTOM_RIGHT ? len - n : 0;
   s.vis = s.nq > 0 ? row_limit(a, s, s.nq - 1) : 0;
   return s;
 }

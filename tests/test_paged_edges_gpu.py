@@ -2,11 +2,13 @@
 bounds, scales of very different size, large caches, many heads and sequences,
 captured graphs, and the C entry points.  Compared with the plain 64-bit forms
 and tolerances of tests/paged_plain.py."""
+import math
+
 import pytest
 import torch
 
 import flash_attention_sm75 as fa
-from tests.paged_plain import Paged
+from tests.paged_plain import UNIT, Paged
 from tests.test_paged_gpu import BF16, E4M3, F16, I8, _attend, _check
 
 pytestmark = pytest.mark.gpu
@@ -126,3 +128,50 @@ def test_wide_tables_go_head_group_by_head_group(sm100, io):
                                            1 << 18, causal=True, k_scale=c["k_scale"], v_scale=c["v_scale"],
                                            return_lse=True)
     _check(P, q, 12, 1, got)
+
+
+def _plain_rows(P, q, Hq, limits):
+    """O and LSE in 64 bits where token i of sequence b sees its keys j < limits[b][i]."""
+    o = torch.zeros(P.total, Hq, P.d, dtype=torch.float64)
+    lse = torch.full((Hq, P.total), -math.inf, dtype=torch.float64)
+    for b, lim in enumerate(limits):
+        for i, n in enumerate(lim):
+            if n <= 0:
+                continue
+            t = P.cu[b] + i
+            k, v = (P.held(x, b, n).repeat_interleave(Hq // P.Hkv, 1).transpose(0, 1) for x in ("k", "v"))
+            s = (k @ q[t].double().unsqueeze(-1)).squeeze(-1) / math.sqrt(P.d)
+            lse[:, t] = torch.logsumexp(s, -1)
+            o[t] = (torch.softmax(s, -1).unsqueeze(1) @ v).squeeze(1)
+    return o, lse
+
+
+def _close(got, want, io):
+    """Values of a few units: P and O are each rounded once to 11 or 8 bits, and the
+    exponential is good to 1e-4; |V| and |O| stay below 6 here."""
+    o, lse = want
+    assert (got[0].double().cpu() - o).abs().max() <= 6 * (3 * UNIT[io] + 2e-4)
+    fin = torch.isfinite(lse)
+    gl = got[1].double().cpu()
+    assert torch.equal(gl == -math.inf, ~fin) and (gl - lse).abs()[fin].max() <= 2e-4
+    assert (got[0].cpu()[(~fin).T] == 0).all()
+
+
+@pytest.mark.parametrize("nq", [1, 5, 40])
+@pytest.mark.parametrize("kind", [(F16, F16), (BF16, BF16)], ids=["f16", "bf16"])
+def test_key_bounds_do_not_move_the_causal_rule(sm100, nq, kind):
+    """Keys that max_seqlen_k or the table's width leaves out are not seen; which of the
+    others a token sees goes by its own position."""
+    P = Paged([(nq, 200), (nq, 60)], 2, 64, 16, kind[1], io=kind[0], seed=51)
+    q = P.new(4)
+    c = P.cuda()
+
+    def limits(most):
+        return [[min(n - nq + i + 1, most) for i in range(nq)] for n in (200, 60)]
+
+    def call(table, max_k):
+        return fa.flash_attention_forward_paged(q.cuda(), c["k_cache"], c["v_cache"], table, c["cu"], c["lens"],
+                                                nq, max_k, causal=True, return_lse=True)
+
+    _close(call(c["table"], 170), _plain_rows(P, q, 4, limits(170)), kind[0])
+    _close(call(c["table"][:, :11], 200), _plain_rows(P, q, 4, limits(176)), kind[0])
