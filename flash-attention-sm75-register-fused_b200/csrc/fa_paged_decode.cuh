@@ -26,9 +26,12 @@
 // tenth of their rate to keep up with HBM, and they take operands converted in
 // registers, which 8-bit pages need: int8 and e4m3 both become f16 exactly, K's
 // scale multiplies the score and V's scale the probability.  Because f16 has
-// few exponent bits, V's scales are taken relative to a power of two per warp
-// that follows the largest one seen; bf16 queries over 8-bit pages are scaled
-// per row by a power of two likewise.
+// few exponent bits, the weights w_ij = p_ij vs_j that multiply V's 8-bit values
+// have a reference of their own: with p_ij = 2^(s_ij - m_i), O_i is the sum of
+// 2^(m_i - r_i) w_ij v_j, and m_i + log2 w_ij moves r_i as s_ij moves m_i.  A row
+// then holds the value rows that make up its result, however large others are
+// that it gives no weight to.  bf16 queries over 8-bit pages are scaled per row
+// by a power of two.
 //
 // A team whose run covers a whole (sequence, head) writes O and LSE; otherwise
 // its unnormalised O, m and l go to one of its two workspace slots (its run's
@@ -53,9 +56,12 @@ namespace pdec {
 constexpr int kWarps = 4;  // per CTA
 constexpr int kRowsMax = 64;
 constexpr int kCombineThreads = 256;
-// Score maximum of a row that has seen no key: finite, so that differences of
-// maxima are never NaN, and below any score.
+// Reference of a row that has seen no key (no value, for r): finite, so that
+// differences are never NaN, and below any score.
 constexpr float kNoMax = -1e30f;
+// V's scales are taken times 2^-kScaleDown, so that w stays finite for the
+// largest bf16 values (p grows to 2^8).
+constexpr int kScaleDown = 10;
 
 // NT: 8-row column blocks of a warp.  Ring stages per warp: as many as the CTAs
 // that share an SM leave room for.
@@ -168,7 +174,9 @@ __device__ Spot find_spot(const PagedAttn& a, int sub, int max_rows, int b, long
   return sp;
 }
 
-// Workspace slots: floats [rows][D] of O, then m[rows], l[rows].
+// Workspace slots: floats [rows][D] of O, then m[rows], l[rows].  16-bit pages:
+// O and l relative to 2^m; 8-bit pages: the part's own result times
+// 2^-kScaleDown, with l = 1 and m the log2 of its sum of exponentials.
 __host__ __device__ constexpr long long slot_floats(int rows, int d) {
   return static_cast<long long>(rows) * (d + 2);
 }
@@ -203,11 +211,11 @@ struct Partial {
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = o[e] * f0 + v[e] * f1;
   }
-  // the warp writes the row
+  // the warp writes the row, times `up`
   template <bool BF16>
-  __device__ __forceinline__ void write(const PagedAttn& a, int tok, int hq) const {
+  __device__ __forceinline__ void write(const PagedAttn& a, int tok, int hq, float up) const {
     const int lane = threadIdx.x & 31;
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = l == 0.f ? 0.f : up / l;
     uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.o) +
                                                 (static_cast<long long>(tok) * a.Hq + hq) * D) +
                     lane * (E / 2);
@@ -232,6 +240,7 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
   using C = Cfg<D, KV>;
   const int stages = p.stages * TEAM;  // of a team
   constexpr int kTeams = kWarps / TEAM;
+  constexpr float kUp = C::k8 ? 1 << kScaleDown : 1;  // of a stored O
   const PagedAttn& a = p.a;
   extern __shared__ uint8_t smem_raw[];
   __shared__ long long sh_scan[kWarps];
@@ -504,18 +513,16 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
 
     float o[NT][C::kKS][4];
     float m[NT][2], l[NT][2];
+    float ref[NT][2];  // r of 8-bit pages (16-bit pages: m)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int k = 0; k < C::kKS; ++k)
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[nt][k][i] = 0.f;
-      m[nt][0] = m[nt][1] = kNoMax;
+      m[nt][0] = m[nt][1] = ref[nt][0] = ref[nt][1] = kNoMax;
       l[nt][0] = l[nt][1] = 0.f;
     }
-    // V's scales are relative to 2^lv: p = exp2(s - m - lv) is summed, and
-    // p * vs multiplies V's 8-bit values
-    int lv = C::k8 ? -95 : 0;  // (below any scale a row is stored with, and l stays finite)
 
     for (int t = t_begin; t < t_end; ++t) {
       ok = bar_wait(bars + 8 * rstage, rphase, wc, 50);
@@ -597,8 +604,8 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
                          : "=f"(f.x), "=f"(f.y)
                          : "r"(sst + 8 * (mt * 16 + g + 8 * hh))
                          : "memory");
-            vsc[mt][hh] = f.y;
-            vmax = fmaxf(vmax, f.y);
+            vsc[mt][hh] = f.y * (1.f / (1 << kScaleDown));
+            vmax = fmaxf(vmax, fabsf(vsc[mt][hh]));
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               sc[nt][mt][2 * hh] *= f.x;
@@ -615,8 +622,9 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
             for (int i = 0; i < 4; ++i)
               if (key0 + mt * 16 + g + 8 * (i >> 1) >= lim[nt][i & 1]) sc[nt][mt][i] = -INFINITY;
       }
-      bool grow = C::k8 && __float_as_int(vmax) >= (lv + 127 + 6) << 23;
+      bool grow = false;
       float top[NT][2];
+      const float vlog = C::k8 ? __log2f(vmax) : 0.f;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -626,28 +634,34 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
           for (int mt = 1; mt < C::kMT; ++mt) x = fmaxf(x, fmaxf(sc[nt][mt][c], sc[nt][mt][2 + c]));
           top[nt][c] = x;
           grow |= fmaf(x, cs[nt][c], -m[nt][c]) > kGrow;
+          // (a bound of m + log2 w: the thread's largest score and scale may be different keys')
+          if constexpr (C::k8) grow |= fmaf(x, cs[nt][c], vlog) - ref[nt][c] > kGrow;
         }
       if (__any_sync(0xffffffffu, grow)) {
-        float fv = 1.f;
-        if constexpr (C::k8) {
-          // vmax < 2^(lv + 1) now; p * vs stays below 2^8 * 2^6 until lv moves again
-          const int e = (__reduce_max_sync(0xffffffffu, __float_as_int(vmax)) >> 23) - 127;
-          const int nlv = max(lv, min(e, 100));
-          fv = ptx::ex2_approx(static_cast<float>(lv - nlv));
-          lv = nlv;
-        }
+        auto over_keys = [](float x) {
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+          x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+          return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+        };
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float x = top[nt][c];
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-            x = fmaxf(m[nt][c], x * cs[nt][c]);
-            const float f = ptx::ex2_approx(m[nt][c] - x) * fv;
+            float x = fmaxf(m[nt][c], over_keys(top[nt][c]) * cs[nt][c]);
+            float f = ptx::ex2_approx(m[nt][c] - x);
             m[nt][c] = x;
             l[nt][c] *= f;
+            if constexpr (C::k8) {
+              float y = -INFINITY;  // the largest log2 w + m
+#pragma unroll
+              for (int mt = 0; mt < C::kMT; ++mt)
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh)
+                  y = fmaxf(y, fmaf(sc[nt][mt][2 * hh + c], cs[nt][c], __log2f(fabsf(vsc[mt][hh]))));
+              x = fmaxf(ref[nt][c], over_keys(y));
+              f = ptx::ex2_approx(ref[nt][c] - x);
+              ref[nt][c] = x;
+            }
 #pragma unroll
             for (int k = 0; k < C::kKS; ++k) {
               o[nt][k][c] *= f;
@@ -659,18 +673,20 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
       uint32_t pb[NT][C::kMT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const float n0 = -(m[nt][0] + static_cast<float>(lv)), n1 = -(m[nt][1] + static_cast<float>(lv));
+        // (126: no value yet, all w are 0)
+        const float f0 = C::k8 ? ptx::ex2_approx(fminf(m[nt][0] - ref[nt][0], 126.f)) : 1.f;
+        const float f1 = C::k8 ? ptx::ex2_approx(fminf(m[nt][1] - ref[nt][1], 126.f)) : 1.f;
 #pragma unroll
         for (int mt = 0; mt < C::kMT; ++mt)
 #pragma unroll
           for (int hh = 0; hh < 2; ++hh) {
-            float p0 = ptx::ex2_approx(fmaf(sc[nt][mt][2 * hh], cs[nt][0], n0));
-            float p1 = ptx::ex2_approx(fmaf(sc[nt][mt][2 * hh + 1], cs[nt][1], n1));
+            float p0 = ptx::ex2_approx(fmaf(sc[nt][mt][2 * hh], cs[nt][0], -m[nt][0]));
+            float p1 = ptx::ex2_approx(fmaf(sc[nt][mt][2 * hh + 1], cs[nt][1], -m[nt][1]));
             l[nt][0] += p0;
             l[nt][1] += p1;
             if constexpr (C::k8) {
-              p0 *= vsc[mt][hh];
-              p1 *= vsc[mt][hh];
+              ptx::fmul2(p0, p1, p0, p1, vsc[mt][hh], vsc[mt][hh]);  // w
+              ptx::fmul2(p0, p1, p0, p1, f0, f1);
             }
             pb[nt][mt][hh] = transpose8(pack2<C::kBf16>(p0, p1));
           }
@@ -729,7 +745,19 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
         x += __shfl_xor_sync(0xffffffffu, x, 8);
         x += __shfl_xor_sync(0xffffffffu, x, 16);
         l[nt][c] = x;
-        m[nt][c] += static_cast<float>(lv);
+        if constexpr (C::k8) {
+          // O becomes the result times 2^-kScaleDown (one exponent: 2^(r - m) alone
+          // may pass fp32's range)
+          const float lg = log2f(x);
+          const float f = x == 0.f ? 0.f : exp2f(ref[nt][c] - m[nt][c] - lg);
+#pragma unroll
+          for (int k = 0; k < C::kKS; ++k) {
+            o[nt][k][c] *= f;
+            o[nt][k][2 + c] *= f;
+          }
+          m[nt][c] = x == 0.f ? kNoMax : m[nt][c] + lg;
+          l[nt][c] = x == 0.f ? 0.f : 1.f;
+        }
       }
     // column of o[..][k][2 hh + c]
     auto col = [&](int k, int hh) { return C::k8 ? 16 * k + 2 * g + hh : 16 * k + g + 8 * hh; };
@@ -741,7 +769,7 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
         if (r >= rows) continue;
         if (first && last && !p.solo) {
           const int tok = s.c0 + r / a.group, hq = cc.h * a.group + r % a.group;
-          const float inv = l[nt][c] == 0.f ? 0.f : 1.f / l[nt][c];
+          const float inv = l[nt][c] == 0.f ? 0.f : kUp / l[nt][c];
           uint16_t* dst = static_cast<uint16_t*>(a.o) + (static_cast<long long>(tok) * a.Hq + hq) * D;
 #pragma unroll
           for (int k = 0; k < C::kKS; ++k) {
@@ -755,7 +783,7 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
           }
           if (g == 0 && a.lse != nullptr)
             a.lse[static_cast<long long>(hq) * a.r.total + tok] =
-                l[nt][c] == 0.f ? -INFINITY : (m[nt][c] + __log2f(l[nt][c])) * 0.69314718055994530942f;
+                l[nt][c] == 0.f ? -INFINITY : (m[nt][c] + (C::k8 ? 0.f : __log2f(l[nt][c]))) * 0.69314718055994530942f;
         } else {
           // slot 0: continues the head of an earlier team; slot 1: begins one
 #pragma unroll
@@ -802,14 +830,14 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
         for (int e = 0; e < Partial<D>::E; ++e) v[e] = sl[row * D + lane * Partial<D>::E + e];
         all.add(sl[kSlotRows * D + row], sl[kSlotRows * D + kSlotRows + row], v);
       }
-      all.template write<QBF16>(a, s.c0 + row / a.group, h * a.group + row % a.group);
+      all.template write<QBF16>(a, s.c0 + row / a.group, h * a.group + row % a.group, kUp);
     }
   }
 }
 
 // Joins the partial results of (sequence, KV head) blockIdx.x, query rows
 // blockIdx.y * kRows ..: with M = max m_s over the segment's slots,
-//   O = sum 2^(m_s - M) O_s / sum 2^(m_s - M) l_s,
+//   O = up sum 2^(m_s - M) O_s / sum 2^(m_s - M) l_s,
 // slots in the order of their teams (so the result does not depend on timing).
 // kRows = 8 (many rows to join, few slots each): one warp per row.  kRows = 1
 // (few rows, many slots), or a segment of more than kManySlots: the block's
@@ -820,7 +848,7 @@ constexpr int kManySlots = 32;
 
 template <int D, bool BF16, int kRows>
 __global__ void __launch_bounds__(kCombineThreads)
-    paged_combine_kernel(const __grid_constant__ DecodeParams p, int sub, int slot_rows) {
+    paged_combine_kernel(const __grid_constant__ DecodeParams p, int sub, int slot_rows, float up) {
   constexpr int kW = kCombineThreads / 32;
   constexpr int E = D / 32;
   const PagedAttn& a = p.a;
@@ -883,7 +911,7 @@ __global__ void __launch_bounds__(kCombineThreads)
     return acc;
   };
   auto finish = [&](int row, const Partial<D>& r) {
-    r.template write<BF16>(a, s.c0 + row / a.group, h * a.group + row % a.group);
+    r.template write<BF16>(a, s.c0 + row / a.group, h * a.group + row % a.group, up);
   };
   if (kRows > 1 && w1 - w0 < kManySlots) {
     for (int r = warp; r < rows; r += kW) finish(row0 + r, gather(row0 + r, 0, 1));
@@ -946,7 +974,8 @@ cudaError_t launch_impl(const DecodeParams& p, int n_ctas, cudaStream_t stream) 
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, many ? paged_combine_kernel<D, QBF16, 8> : paged_combine_kernel<D, QBF16, 1>,
-                            p, static_cast<int>(C::kSub), 8 * NT * TEAM);
+                            p, static_cast<int>(C::kSub), 8 * NT * TEAM,
+                            C::k8 ? static_cast<float>(1 << kScaleDown) : 1.f);
 }
 
 // Rows of a team and how it is made up: one warp for 8 or 16 rows, two or four

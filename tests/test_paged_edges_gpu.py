@@ -8,7 +8,7 @@ import pytest
 import torch
 
 import flash_attention_sm75 as fa
-from tests.paged_plain import UNIT, Paged
+from tests.paged_plain import UNIT, Paged, attention, quantise
 from tests.test_paged_gpu import BF16, E4M3, F16, I8, _attend, _check
 
 pytestmark = pytest.mark.gpu
@@ -175,3 +175,91 @@ def test_key_bounds_do_not_move_the_causal_rule(sm100, nq, kind):
 
     _close(call(c["table"], 170), _plain_rows(P, q, 4, limits(170)), kind[0])
     _close(call(c["table"][:, :11], 200), _plain_rows(P, q, 4, limits(176)), kind[0])
+
+
+# ------------------------------------------------------------------ scales of very different size
+
+def _check_relative(P, q, Hq, mode, got):
+    """_check without an absolute term, for 8-bit pages whose keys and queries are used
+    exactly: with A = sum p |v| an element of O is off by at most
+        u_out |O| + A (2 u + 4e-4),   u = 2^-11 (P is f16; the exponential, the scores in fp32),
+    and by P's smallest step: p times a row's scale is an f16 relative to a largest one
+    W = max_j p_j scale_j, good to 2^-25 W, so 2^-25 W sum_j |v_j / scale_j| (and half a step of
+    f16 results below 2^-14)."""
+    d, io = P.d, P.io
+    go, gl = got[0].double().cpu(), got[1].double().cpu()
+    assert torch.isfinite(go).all()
+    for b, (m, n) in enumerate(P.lens):
+        rows = slice(P.cu[b], P.cu[b + 1])
+        k, v = (P.held(x, b, n).repeat_interleave(Hq // P.Hkv, 1).transpose(0, 1) for x in ("k", "v"))
+        pos = torch.arange(n)
+        vs = P.vs[P.table[b].long()[pos // P.page], :, pos % P.page].double()
+        vs = vs.repeat_interleave(Hq // P.Hkv, 1).transpose(0, 1)              # [Hq, n]
+        s = q[rows].double().transpose(0, 1) @ k.transpose(1, 2) / math.sqrt(d)
+        see = torch.arange(n)[None] <= torch.arange(m)[:, None] + n - m if mode else torch.ones(m, n, dtype=bool)
+        s = s.masked_fill(~see, -math.inf)
+        z = torch.logsumexp(s, -1)
+        p = torch.exp(s - z[..., None])
+        o, a = p @ v, p @ v.abs()
+        w = (p * vs[:, None]).amax(-1, keepdim=True)
+        v8 = (v / vs.clamp(min=1e-300)[..., None]).abs()
+        steps = w * (see.double() @ v8)
+        tol = UNIT[io] * o.abs() + a * (2 * UNIT[F16] + 4e-4) + 2.0 ** -25 * steps
+        if io == F16:
+            tol = tol + 2.0 ** -25
+        off = (go[rows].transpose(0, 1) - o).abs()
+        assert (off <= tol).all(), (off / tol).max().item()
+        assert ((gl[:, rows] - z).abs() <= 1e-4 + z.abs() * 2.0 ** -20).all()
+
+
+@pytest.mark.parametrize("nq", [1, 6])
+@pytest.mark.parametrize("kind", [(F16, I8), (F16, E4M3), (BF16, I8), (BF16, E4M3)],
+                         ids=["f16-int8", "f16-e4m3", "bf16-int8", "bf16-e4m3"])
+@pytest.mark.parametrize("late", [True, False], ids=["late", "early"])
+def test_small_value_row_takes_the_weight(sm100, nq, kind, late):
+    """A key whose value row is millions of times smaller than others' takes nearly all
+    the weight, behind the large ones and before them, alone and within one tile."""
+    io, cache = kind
+    P = Paged([(nq, 700), (nq, 90)], 1, 64, 16, cache, io=io, seed=61)
+    q0 = torch.randn(64, generator=P.g)
+    q = (q0 + 0.01 * torch.randn(P.total, 4, 64, generator=P.g)).to(io)
+    big, small = (3e3, 2e-3) if io == F16 else (1e7, 1e-6)
+    for b, (_, n) in enumerate(P.lens):
+        k = torch.randn(n, 1, 64, generator=P.g) * 0.1
+        v = torch.randn(n, 1, 64, generator=P.g) * small
+        at = n - nq - 5 if late else 3
+        other = 20 if late else n - nq - 9
+        k[at, 0] = q0 * 8          # its score is about 64 above the others'
+        v[other] = torch.randn(1, 64, generator=P.g) * big
+        v[at + 1] = torch.randn(1, 64, generator=P.g) * big
+        for name, x in (("k", k), ("v", v)):
+            P.put(name, b, range(n), *quantise(x, cache))
+    _check_relative(P, q, 4, 1, _attend(P, q, 4, 1))
+
+
+@pytest.mark.parametrize("nq", [1])
+@pytest.mark.parametrize("cache", [I8, E4M3], ids=["int8", "e4m3"])
+@pytest.mark.parametrize("size", [2e-30, 1e-20, 1e-7, 1e-4, 1e6, 1e20, 1e36])
+def test_bf16_results_hold_their_range(sm100, nq, cache, size):
+    """Values (and keys, with queries to match) far outside f16's range."""
+    P = Paged([(nq, 300), (nq, 50)], 2, 128, 16, cache, io=BF16, seed=62)
+    for b, (_, n) in enumerate(P.lens):
+        for name in ("k", "v"):
+            P.put(name, b, range(n), *quantise(torch.randn(n, 2, 128, generator=P.g) * size, cache))
+    q = P.new(8, spread=1 / size)
+    _check_relative(P, q, 8, 1, _attend(P, q, 8, 1))
+
+
+@pytest.mark.parametrize("nq", [1])
+def test_lse_over_8_bit_pages_is_held_in_32_bits(sm100, nq):
+    """Scores come from the stored bits and their fp32 scales: the LSE of bf16 results is
+    as good as that of f16 ones."""
+    for io in (F16, BF16):
+        for cache in (I8, E4M3):
+            P = Paged([(nq, 2000)], 2, 128, 32, cache, io=io, seed=63)
+            q = P.new(8)
+            gl = _attend(P, q, 8, 1)[1].double().cpu()
+            lse = attention(P, q, 8, 1)[1]
+            # one exponential is good to 2^-13 at worst (its approximation's error has both
+            # signs over the sum), fp32 sums and scores to 1e-6: 2e-5 is a tenth of what f16 keys cost
+            assert (gl - lse).abs().max() <= 2e-5
