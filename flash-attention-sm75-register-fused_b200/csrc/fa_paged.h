@@ -89,12 +89,14 @@ struct alignas(64) ChunkParams {
   int n_ctas;
   int fill_outside;  // write the rows of no sequence
   int head0, n_heads;  // KV heads of this launch
-  // 8-bit pages: f16 rows and scales of the launch's heads (paged_expand_kernel)
+  // 8-bit pages: 16-bit rows and scales of the launch's heads (paged_expand_kernel)
   long long exp_rows;
-  uint16_t* exp_k;   // [n_heads][exp_rows][d]
-  uint16_t* exp_v;
-  float* exp_ks;     // [n_heads][exp_rows], f16 results only
-  float* exp_vs;
+  uint16_t* exp_k;   // [n_heads][exp_rows][d], the type of the queries
+  uint16_t* exp_v;   // f16
+  float* exp_ks;     // [n_heads][exp_rows]
+  float* exp_vs;     // ... times 2^-kScaleShift
+  float* exp_vl;     // ... log2 of its magnitude
+  float* exp_vm;     // [n_heads][exp_rows / 16], the largest exp_vl of 16 rows
   // parts of cut items, two slots per run: [2 n_ctas][2 query tiles][d / 4][128
   // rows][4] fp32, normalised, and [2 n_ctas][2][128], natural log
   float* ws_o;

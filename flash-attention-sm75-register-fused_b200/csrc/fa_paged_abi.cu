@@ -100,10 +100,10 @@ struct PagedPlan {
   bool runs = false;    // ... equal runs, or one CTA per (pair, head)
   int n_ctas = 0;       // ... runs
   // 8-bit pages: rows of the expanded keys, KV heads expanded at a time, and
-  // bytes of one head's K (or V) rows and scales
+  // bytes of one head's K (or V) rows, of a scale of every row, of their maxima
   long long exp_rows = 0;
   int exp_heads = 0;
-  size_t exp_row_bytes = 0, exp_scale_bytes = 0;
+  size_t exp_row_bytes = 0, exp_scale_bytes = 0, exp_max_bytes = 0;
   size_t ws_decode = 0, ws_o = 0, ws_lse = 0, ws_cuts = 0, ws_bytes = 0;
 };
 
@@ -139,7 +139,8 @@ PagedPlan make_paged_plan(int B, int heads, int group, int head_dim, int dtype, 
       if (k.exp_rows < 128) k.exp_rows = 128;
       k.exp_row_bytes = static_cast<size_t>(k.exp_rows) * head_dim * 2;
       k.exp_scale_bytes = static_cast<size_t>(k.exp_rows) * sizeof(float);
-      const size_t per_head = 2 * (k.exp_row_bytes + k.exp_scale_bytes);
+      k.exp_max_bytes = static_cast<size_t>(k.exp_rows / 16) * sizeof(float);
+      const size_t per_head = 2 * k.exp_row_bytes + 3 * k.exp_scale_bytes + k.exp_max_bytes;
       const size_t fit = kExpandBytes / per_head;
       if (fit < static_cast<size_t>(heads)) k.exp_heads = fit < 1 ? 1 : static_cast<int>(fit);
     }
@@ -179,7 +180,8 @@ PagedPlan make_paged_plan(int B, int heads, int group, int head_dim, int dtype, 
     }
   }
   const size_t chunk_bytes =
-      k.ws_o + k.ws_lse + k.ws_cuts + 2 * static_cast<size_t>(k.exp_heads) * (k.exp_row_bytes + k.exp_scale_bytes);
+      k.ws_o + k.ws_lse + k.ws_cuts +
+      static_cast<size_t>(k.exp_heads) * (2 * k.exp_row_bytes + 3 * k.exp_scale_bytes + k.exp_max_bytes);
   // (the kernels run one after another, so they share the workspace)
   k.ws_bytes = k.ws_decode > chunk_bytes ? k.ws_decode : chunk_bytes;
   return k;
@@ -269,7 +271,7 @@ bool chunk_maps(const fa_paged_cache& c, fa::ChunkParams* p) {
          tile_map(c.v, type, c.head_dim, c.page_size, rs, planes, g, p->box_rows, &p->tm_v);
 }
 
-// Maps of the expanded rows of 8-bit pages.
+// Maps of the expanded rows of 8-bit pages (a copy is the same for f16 and bf16).
 bool rows_maps(fa::ChunkParams& p, int head_dim, int heads) {
   const unsigned long long row = 2ull * head_dim;
   const int type = fa::TiledMap::kF16;
@@ -432,6 +434,8 @@ int fa_fwd_paged(const fa_paged_cache* cache, const void* Q, long long q_token_s
     ws += 2 * k.exp_heads * k.exp_row_bytes;
     p.exp_ks = reinterpret_cast<float*>(ws);
     p.exp_vs = reinterpret_cast<float*>(ws + k.exp_heads * k.exp_scale_bytes);
+    p.exp_vl = reinterpret_cast<float*>(ws + 2 * k.exp_heads * k.exp_scale_bytes);
+    p.exp_vm = reinterpret_cast<float*>(ws + 3 * k.exp_heads * k.exp_scale_bytes);
     p.timeout_ns = fa::host_timeout_ns();
     const bool maps =
         (eight ? rows_maps(p, cache->head_dim, k.exp_heads) : chunk_maps(*cache, &p)) &&

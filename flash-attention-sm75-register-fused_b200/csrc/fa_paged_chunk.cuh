@@ -34,13 +34,17 @@
 //          128).  The rows behind the last visible key in its box are stale; V's
 //          are set to zero before the tile is released, K's are masked as scores.
 //          8-bit pages: paged_expand_kernel first writes the visible keys and
-//          values once as f16 rows into the workspace (exactly, with the scales
-//          beside them, for f16 results; multiplied by their scale and rounded,
-//          8 times finer than the result, for bf16 ones), so that the pairs of a
-//          chunk do not widen the same keys again and again, and the kernel
-//          reads plain 128-row tiles.  For f16 results the softmax applies the
-//          scales in fp32: K's to the scores; V's is split into a power of two,
-//          which the rows take (exactly), and a rest in [1, 2) for P.
+//          values once as 16-bit rows into the workspace (exactly, K in the
+//          queries' type, V in f16, the scales beside them), so that the pairs of
+//          a chunk do not widen the same keys again and again, and the kernel
+//          reads plain 128-row tiles.  The softmax applies the scales in fp32:
+//          K's to the scores, V's to P.
+//   P      over 8-bit pages is 2^(s_ij - r_i) vs_j with a reference r_i that follows
+//          the largest s_ij + log2 vs_j instead of the largest score: f16 then holds
+//          the value rows that make up a result, however large or small they and
+//          others are.  The row sum of exponentials is kept relative to the largest
+//          score, m_i.  A bound, the tile's largest score and largest scale, says
+//          where r may have to grow; only then is the maximum taken key by key.
 //   joins  The parts of a cut item go to the workspace as fp32 (four columns of all
 //          rows side by side, so that stores and the join's loads are whole
 //          lines: 77 -> 70 us for 512 tokens over 8192 keys), and paged_join_kernel
@@ -56,7 +60,7 @@
 namespace fa {
 namespace {
 
-// What the kernel reads.
+// What the kernel reads: pages, or the expanded rows of 8-bit pages.
 enum { kPagesF16 = 0, kPagesBf16 = 1, kExpanded = 2 };
 
 // A part of a work item that a CTA computes.
@@ -87,12 +91,13 @@ struct ChunkLayout {
   static constexpr int kOffQ = 0;
   static constexpr int kOffKV = 2 * kTile;
   static constexpr int kOffScale = kOffKV + kSlots * kTile;
-  // scales of tile j at entry j % kScaleRing: K's 128, V's 128, loaded with
-  // K_j.  K_j's slot is free only after the scores of tile j - kSlots / 2 were
-  // issued for both groups, i.e. after both finished the softmax of the tile
-  // before it, so entry j - kScaleRing is no longer read.
+  // scales of tile j at entry j % kScaleRing: K's 128, V's 128, the 128 logarithms
+  // of V's and 8 maxima of those, loaded with K_j.  K_j's slot is free only after
+  // the scores of tile j - kSlots / 2 were issued for both groups, i.e. after both
+  // finished the softmax of the tile before it, so entry j - kScaleRing is no
+  // longer read.
   static constexpr int kScaleRing = D == 64 ? 8 : 4;
-  static constexpr int kScaleEntry = 2 * 128 * 4;
+  static constexpr int kScaleEntry = (3 * 128 + 8) * 4;
   static_assert(kScaleRing >= kSlots / 2 + 1, "a scale entry outlives its tile");
   static constexpr int kOffBar = kOffScale + (kScaled ? kScaleRing * kScaleEntry : 0);
   static constexpr int kBarQ = 0;                       // 2
@@ -131,10 +136,10 @@ __device__ __forceinline__ float4 load_scales(uint32_t addr) {
   return f;
 }
 
-// exp_tile (fa_fwd_sm100.cu) with P multiplied by the rest of V's scales: e =
-// 2^(x sl - m) is summed as it is, e * vs goes to tensor memory.
+// exp_tile (fa_fwd_sm100.cu) with P multiplied by V's scales: e = 2^(x sl - ref)
+// is summed as it is, e * vs goes to tensor memory.
 template <bool kEmulate, int kPeriod, typename Announce>
-__device__ __forceinline__ float exp_tile_scaled(const float (&x)[kBlockN], float sl, float neg_m,
+__device__ __forceinline__ float exp_tile_scaled(const float (&x)[kBlockN], float sl, float neg_ref,
                                                  uint32_t vs, uint32_t tP, Announce announce) {
   float a0 = 0.f, a1 = 0.f, b0 = 0.f, b1 = 0.f;
 #pragma unroll
@@ -147,7 +152,7 @@ __device__ __forceinline__ float exp_tile_scaled(const float (&x)[kBlockN], floa
       for (int y = 0; y < 2; ++y) {
         const int i = 32 * h + 2 * (c + y);
         float e0, e1;
-        exp2_pair<kEmulate, kPeriod>(c + y, x[i], x[i + 1], sl, neg_m, e0, e1);
+        exp2_pair<kEmulate, kPeriod>(c + y, x[i], x[i + 1], sl, neg_ref, e0, e1);
         if (y)
           ptx::fadd2(b0, b1, b0, b1, e0, e1);
         else
@@ -271,6 +276,15 @@ __device__ __forceinline__ void find_start(const ChunkParams& p, int x, WorkStar
   __syncthreads();
 }
 
+// The reference of P over 8-bit pages (log2): none yet; how far P may pass it until
+// O is rescaled; and how far it may be above and below the largest score, so that
+// the exponentials relative to it stay in fp32's range.  V's scales, 2^-109 to 2^121
+// in what the write stores, are taken times 2^-kScaleShift: within the range from
+// kRefBelow below to kRefAbove above, but for the largest ones, whose P is then up to
+// 2^15, still in f16's range.
+constexpr float kNoRef = -1e30f, kRefLag = 14.f, kRefAbove = 100.f, kRefBelow = 116.f;
+constexpr float kScaleShift = 6.f;
+
 // A segment as the softmax of query tile g sees it.
 struct ChunkItem {
   Seq s;
@@ -281,11 +295,9 @@ struct ChunkItem {
 // SRC: what is read; QBF16: type of Q and O.
 template <int D, int SRC, bool QBF16>
 __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_constant__ ChunkParams p) {
-  constexpr bool kExp = SRC == kExpanded;
-  constexpr bool kBf16 = SRC == kPagesBf16;   // type of the products
-  constexpr bool kScaled = kExp && !QBF16;    // the softmax applies the scales
-  constexpr bool kCastQ = kExp && QBF16;      // Q becomes f16
-  using L = ChunkLayout<D, kScaled>;
+  constexpr bool kExp = SRC == kExpanded;     // the softmax applies the scales
+  constexpr bool kBf16 = SRC == kPagesBf16;   // type of P and V (Q and K: QBF16)
+  using L = ChunkLayout<D, kExp>;
   const PagedAttn& a = p.a;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -329,8 +341,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
     dead = ((st >> 32) == p.epoch && (st & 0xffffffffull) != 0ull) ? 1 : 0;
     *abort_flag = 0;
     for (int i = 0; i < L::kNumBars; ++i) {
-      const bool all = (i >= L::kBarP && i < L::kBarP + 2) || (i >= L::kBarPH && i < L::kBarPH + 2) ||
-                       (kCastQ && i < 2);
+      const bool all = (i >= L::kBarP && i < L::kBarP + 2) || (i >= L::kBarPH && i < L::kBarPH + 2);
       const bool seg = i >= L::kBarSegEmpty;  // one arrival per warp that reads segments
       ptx::mbar_init(bar(i), all ? 128u : seg ? 11u : 1u);
     }
@@ -485,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
           return page >= 0 ? page * p.page_step + h * p.head_step : -1;
         };
         int next_page = n_loop > 0 ? page_at(jb) : -1, page = -1;
-        for (int g = 0; ok && g < 2 && !kCastQ && second == 0; ++g) {
+        for (int g = 0; ok && g < 2 && second == 0; ++g) {
           if (n_kv[g] == 0) continue;
           if (n_q[g] > 0 &&
               !(ok = __all_sync(0xffffffffu, bar_wait(bar(L::kBarQFree + g), (n_q[g] - 1) & 1, wc, 8))))
@@ -513,12 +524,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
           const int r0 = vis - tile * kBlockN;
           const int r1 = (r0 + p.box_rows - 1) / p.box_rows * p.box_rows;
           // (a run-time flag, though the expanded rows never have any: with the
-          // branch compiled out ptxas schedules the softmax of f16 results worse,
-          // 2 x 2048 tokens over 8192 keys take 487 us instead of 471, 421 instead
-          // of 394 at d = 64; bf16 results gain 2 %)
+          // branch compiled out ptxas schedules the softmax over 8-bit pages worse, 2
+          // x 2048 tokens over 8192 keys take 3 % longer at d = 128, 4 % at d = 64)
           const bool tail = p.stale && second && r0 < kBlockN && r0 != r1;
           const uint32_t full = tail ? bar(L::kBarTail) : bar(L::kBarFull + slot);
-          const bool scales = kScaled && !second;
+          const bool scales = kExp && !second;
           if (lane == 0) ptx::mbar_arrive_expect_tx(full, L::kTile + (scales ? L::kScaleEntry : 0));
           __syncwarp();
           const uint32_t dst = sbase + L::kOffKV + slot * L::kTile;
@@ -527,11 +537,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                                : a.c.row_in_page(tile * kBlockN + box * p.box_rows);
           if (issues)
             ptx::tma_load_5d(dst + dst_off, second ? &p.tm_v : &p.tm_k, full, 0, 0, 0, row >> 3, page, pol_kv);
-          if (scales && lane < 2) {
-            const float* src = (lane ? p.exp_vs : p.exp_ks) +
-                               static_cast<long long>(h - p.head0) * p.exp_rows + row;
+          if (scales && lane < 4) {
+            const long long at = static_cast<long long>(h - p.head0) * p.exp_rows + row;
+            const float* src = lane == 0   ? p.exp_ks + at
+                               : lane == 1 ? p.exp_vs + at
+                               : lane == 2 ? p.exp_vl + at
+                                           : p.exp_vm + at / 16;
             ptx::bulk_load(sbase + L::kOffScale + ((i >> 1) % L::kScaleRing) * L::kScaleEntry + lane * 512, src,
-                           512, full);
+                           lane < 3 ? 512 : 32, full);
           }
           i += 2;
           if (tail) {
@@ -562,9 +575,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
         if (n_q[g] > 0) bar_wait(bar(L::kBarQ + g), (n_q[g] - 1) & 1, wc, 2, false);
     } else if (warp == kWarpMma) {
       // =================================================== MMA issuer (see fa_fwd_kernel)
-      constexpr uint32_t fmt = kBf16 ? 1u : 0u;
-      constexpr uint32_t idesc_qk = ptx::make_idesc_f16(kBlockM, kBlockN, fmt, 0, 0);
-      constexpr uint32_t idesc_pv = ptx::make_idesc_f16(kBlockM, D, fmt, 0, 1);
+      constexpr uint32_t idesc_qk = ptx::make_idesc_f16(kBlockM, kBlockN, QBF16 ? 1u : 0u, 0, 0);
+      constexpr uint32_t idesc_pv = ptx::make_idesc_f16(kBlockM, D, kBf16 ? 1u : 0u, 0, 1);
       const uint64_t k_desc0 = ptx::smem_desc_sw128(sbase + L::kOffKV, 16, L::kGroupBytes);
       const uint64_t v_desc0 = ptx::smem_desc_sw128(sbase + L::kOffKV, 1024, L::kGroupBytes);
       const uint64_t q_desc0 = ptx::smem_desc_sw128(sbase + L::kOffQ, 16, 1024);
@@ -721,56 +733,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
       const int tok = tok_lo + r / a.group;      // token of the sequence
       const int hq = it.h * a.group + r % a.group;
       const bool row_ok = r < n_rows && tok < it.s.nq;
-      float sl = a.scale_log2;
-      if constexpr (kCastQ) {
-        // Q as f16 in the swizzled layout, one row per thread; a bf16 row is
-        // scaled by a power of two into f16's range, undone in sl
-        if (n_tiles > 0) {
-          uint4 q[D / 8];
-#pragma unroll
-          for (int c = 0; c < D / 8; ++c) q[c] = make_uint4(0u, 0u, 0u, 0u);
-          if (row_ok) {
-            const uint4* src = reinterpret_cast<const uint4*>(
-                a.q + static_cast<long long>(it.s.c0 + tok) * a.q_token + hq * a.q_head);
-#pragma unroll
-            for (int c = 0; c < D / 8; ++c) q[c] = __ldg(src + c);
-          }
-          {
-            auto f2 = [](uint32_t u) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&u)); };
-            float mx = 0.f;
-#pragma unroll
-            for (int c = 0; c < D / 8; ++c) {
-              const uint32_t u[4] = {q[c].x, q[c].y, q[c].z, q[c].w};
-#pragma unroll
-              for (int i = 0; i < 4; ++i) mx = fmaxf(mx, fmaxf(fabsf(f2(u[i]).x), fabsf(f2(u[i]).y)));
-            }
-            const uint32_t e = __float_as_uint(mx) & 0x7f800000u;
-            const bool plain = e == 0u || e >= 0x7e800000u;
-            const float inv = plain ? 1.f : __uint_as_float(0x7f000000u - e);
-            if (!plain) sl *= __uint_as_float(e);
-#pragma unroll
-            for (int c = 0; c < D / 8; ++c) {
-              uint32_t* u = reinterpret_cast<uint32_t*>(&q[c]);
-#pragma unroll
-              for (int i = 0; i < 4; ++i) u[i] = pack2<false>(f2(u[i]).x * inv, f2(u[i]).y * inv);
-            }
-          }
-          uint8_t* dst = smem + L::kOffQ + g * L::kTile + r * 128;
-#pragma unroll
-          for (int c = 0; c < D / 8; ++c)
-            *reinterpret_cast<uint4*>(dst + (c >> 3) * L::kBlockBytes + (((c & 7) ^ (r & 7)) << 4)) = q[c];
-          ptx::fence_proxy_async_smem();
-          ptx::mbar_arrive(bar(L::kBarQ + g));
-        }
-      }
+      const float sl = a.scale_log2;
       // key limit of this row, and the smallest of the tile's rows
       const int row_end = row_limit(a, it.s, tok);
       const int tile_end = row_limit(a, it.s, tok_lo);
 
-      // (kScaled: P is multiplied by up to 2 and must stay in f16's range)
-      constexpr float kGrow = kScaled ? kRescaleThreshold - 1.0f : kRescaleThreshold;
       float m = -INFINITY;  // running max of the scaled scores (log2 units)
       float l = 0.f;        // running sum of exp2(s - m)
+      float ref = kNoRef;   // kExp: reference of P and O (else m)
       for (int j = 0; ok && j < n_tiles; ++j) {
         ok = __all_sync(0xffffffffu, bar_wait(bar(L::kBarS + g), (it.par + j) & 1, wc, 20 + g));
         if (!ok) break;
@@ -795,8 +765,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
             x[96 + c] = __uint_as_float(u3[c]);
           }
         }
-        const uint32_t entry = sbase + L::kOffScale + (kScaled ? ((it.tiles + j) % L::kScaleRing) * L::kScaleEntry : 0);
-        if constexpr (kScaled) {
+        const uint32_t entry = sbase + L::kOffScale + (kExp ? ((it.tiles + j) % L::kScaleRing) * L::kScaleEntry : 0);
+        if constexpr (kExp) {
 #pragma unroll
           for (int c = 0; c < kBlockN; c += 4) {
             const float4 f = load_scales(entry + 4 * c);
@@ -824,40 +794,64 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
           m_tile = row_extreme<kBlockN, true>(x) * sl;
         }
         const float m_new = fmaxf(m, m_tile);
-        const bool grow = m_new > m + kGrow;
-        if (j == 0) {
-          m = m_new;
-        } else {
-          if (__any_sync(0xffffffffu, grow)) {
-            const float alpha = grow ? ptx::ex2_approx(m - m_new) : 1.0f;
+        auto scale_o = [&](float alpha) {
 #pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-              uint32_t o[32];
-              ptx::tmem_ld32(tO + c * 32, o);
-              ptx::tmem_wait_ld();
-              pin_after_wait<32>(o);
+          for (int c = 0; c < D / 32; ++c) {
+            uint32_t o[32];
+            ptx::tmem_ld32(tO + c * 32, o);
+            ptx::tmem_wait_ld();
+            pin_after_wait<32>(o);
 #pragma unroll
-              for (int i = 0; i < 32; i += 2) {
-                float a0 = __uint_as_float(o[i]), a1 = __uint_as_float(o[i + 1]);
-                ptx::fmul2(a0, a1, a0, a1, alpha, alpha);
-                o[i] = __float_as_uint(a0);
-                o[i + 1] = __float_as_uint(a1);
-              }
-              ptx::tmem_st32(tO + c * 32, o);
+            for (int i = 0; i < 32; i += 2) {
+              float a0 = __uint_as_float(o[i]), a1 = __uint_as_float(o[i + 1]);
+              ptx::fmul2(a0, a1, a0, a1, alpha, alpha);
+              o[i] = __float_as_uint(a0);
+              o[i + 1] = __float_as_uint(a1);
             }
-            ptx::tmem_wait_st();
-            l *= alpha;
+            ptx::tmem_st32(tO + c * 32, o);
           }
-          if (grow) m = m_new;
+          ptx::tmem_wait_st();
+        };
+        if constexpr (kExp) {
+          if (m_new > m) l *= ptx::ex2_approx(m - m_new);
+          m = m_new;
+          const float4 v0 = load_scales(entry + 1536), v1 = load_scales(entry + 1552);
+          const float vm = fmax3(fmax3(fmaxf(v0.x, v0.y), v0.z, v0.w), fmaxf(v1.x, v1.y), fmaxf(v1.z, v1.w));
+          if (__any_sync(0xffffffffu, m_tile + vm > ref + kRefLag || m > ref + kRefBelow)) {
+            float y = -INFINITY;  // the largest s + log2 vs
+#pragma unroll
+            for (int c = 0; c < kBlockN; c += 4) {
+              const float4 f = load_scales(entry + 1024 + 4 * c);
+              y = fmax3(y, fmaf(x[c], sl_eff, f.x), fmaf(x[c + 1], sl_eff, f.y));
+              y = fmax3(y, fmaf(x[c + 2], sl_eff, f.z), fmaf(x[c + 3], sl_eff, f.w));
+            }
+            y = fmaxf(fminf(y, m + kRefAbove), m - kRefBelow);
+            const bool grow = y > ref + kRefLag || m > ref + kRefBelow;
+            if (j > 0 && __any_sync(0xffffffffu, grow)) scale_o(grow ? ptx::ex2_approx(ref - y) : 1.0f);
+            if (grow) ref = y;
+          }
+        } else {
+          const bool grow = m_new > m + kRescaleThreshold;
+          if (j == 0) {
+            m = m_new;
+          } else {
+            if (__any_sync(0xffffffffu, grow)) {
+              const float alpha = grow ? ptx::ex2_approx(m - m_new) : 1.0f;
+              scale_o(alpha);
+              l *= alpha;
+            }
+            if (grow) m = m_new;
+          }
         }
-        const float neg_m = (m == -INFINITY) ? 0.f : -m;
         const uint32_t half_bar = bar(L::kBarPH + g);
         auto announce = [half_bar] { ptx::mbar_arrive(half_bar); };
         float tile_sum;
-        if constexpr (kScaled) {
-          tile_sum = masked ? exp_tile_scaled<false, kEmuPeriod>(x, sl_eff, neg_m, entry + 512, tP, announce)
-                            : exp_tile_scaled<true, kPairEmuPeriod<D>>(x, sl_eff, neg_m, entry + 512, tP, announce);
+        if constexpr (kExp) {
+          tile_sum = masked ? exp_tile_scaled<false, kEmuPeriod>(x, sl_eff, -ref, entry + 512, tP, announce)
+                            : exp_tile_scaled<true, kPairEmuPeriod<D>>(x, sl_eff, -ref, entry + 512, tP, announce);
+          tile_sum *= m == -INFINITY ? 1.f : ptx::ex2_approx(ref - m);  // (1: no key so far, or NaN)
         } else {
+          const float neg_m = (m == -INFINITY) ? 0.f : -m;
           tile_sum = masked ? exp_tile<kBf16, false>(x, sl_eff, neg_m, tP, announce)
                             : exp_tile<kBf16, true, kPairEmuPeriod<D>>(x, sl_eff, neg_m, tP, announce);
         }
@@ -886,7 +880,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
         if (ok) ok = __all_sync(0xffffffffu, bar_wait(bar(L::kBarO + g), (it.par + n_tiles - 1) & 1, wc, 22 + g));
         if (ok) {
           ptx::tc_fence_after();
-          const float inv_l = (l > 0.f) ? 1.0f / l : (l == 0.f ? 0.f : l);  // (a NaN stays one)
+          // (a NaN stays one; 2^(ref - m) / l as one exponent, for its parts may pass fp32's range)
+          const float inv_l = l == 0.f ? 0.f : kExp ? exp2f(ref - m - __log2f(l) + kScaleShift) : l > 0.f ? 1.0f / l : l;
           const float m_use = (m == -INFINITY) ? 0.f : m;
           const float lse_row =
               l == 0.f ? -INFINITY : (m_use + __log2f(l)) * 0.69314718055994530942f;
@@ -988,14 +983,15 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
     a.lse[static_cast<long long>(hq) * a.r.total + c.c0 + tok] = sum == 0.f ? -INFINITY : mx + logf(sum);
 }
 
-// The visible keys and values of the chunk kernel's sequences as f16 rows:
+// The visible keys and values of the chunk kernel's sequences as 16-bit rows:
 // sequence after sequence, each padded to 128 rows (the padding is zeros),
-// [n_heads][exp_rows][d] for K and for V, with the scales [n_heads][exp_rows] or,
-// for kFold, multiplied by them.  A warp takes groups of 16 keys of one head.
+// [n_heads][exp_rows][d] for K (in the type of the queries) and for V (f16), with
+// the scales [n_heads][exp_rows], V's logarithms and the largest of every 16 rows.
+// Both types hold 8-bit values exactly.  A warp takes groups of 16 keys of one head.
 // Bound by memory, much of it L2: 39 MB of e4m3 pages become 79 MB in 19 us.
 constexpr int kExpandThreads = 128;
 
-template <int D, int KV, bool kFold>
+template <int D, int KV, bool kKBf16>
 __global__ void __launch_bounds__(kExpandThreads) paged_expand_kernel(const __grid_constant__ ChunkParams p) {
   const PagedAttn& a = p.a;
   constexpr int L = D / 16;            // lanes per row: 8 bytes at 8 part and at d / 2 + 8 part
@@ -1057,6 +1053,7 @@ __global__ void __launch_bounds__(kExpandThreads) paged_expand_kernel(const __gr
           x[kv][y][0] = __ldg(src + part);
           x[kv][y][1] = __ldg(src + D / 16 + part);
           sc[kv][y] = __ldg((kv ? a.c.vs : a.c.ks) + sc0 + r * a.c.s_row);
+          if (kv) sc[kv][y] *= 1.f / (1 << static_cast<int>(kScaleShift));
         }
       }
 #pragma unroll
@@ -1065,47 +1062,39 @@ __global__ void __launch_bounds__(kExpandThreads) paged_expand_kernel(const __gr
       for (int y = 0; y < kPasses; ++y) {
         const long long row = dst0 + y * kRows + lane / L;
         uint4* dst = reinterpret_cast<uint4*>((kv ? p.exp_v : p.exp_k) + row * D) + part;
-        // V's scale = power * rest, rest in [1, 2) where power is in range
-        const float power = __uint_as_float(
-            min(max(__float_as_uint(sc[kv][y]) & 0x7f800000u, 0x33800000u), 0x43000000u));
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           uint32_t w[4];
           widen<KV, false>(x[kv][y][i].x, w[0], w[1]);
           widen<KV, false>(x[kv][y][i].y, w[2], w[3]);
-          if (!kFold && kv) {
-            // exact: f16 holds 8-bit values times 2^-24 .. 2^7 (below 2^-24 they
-            // are smaller than any f16 result)
-            const __half2 p2 = __float2half2_rn(power);
+          if (kKBf16 && !kv) {
 #pragma unroll
             for (int z = 0; z < 4; ++z) {
-              const __half2 f = __hmul2(*reinterpret_cast<__half2*>(&w[z]), p2);
-              w[z] = *reinterpret_cast<const uint32_t*>(&f);
-            }
-          }
-          if constexpr (kFold) {
-#pragma unroll
-            for (int z = 0; z < 4; ++z) {
-              // beyond f16's range: its largest value
               const float2 f = __half22float2(*reinterpret_cast<__half2*>(&w[z]));
-              const float f0 = f.x * sc[kv][y], f1 = f.y * sc[kv][y];
-              auto clamp = [](float v) { return v > 65504.f ? 65504.f : v < -65504.f ? -65504.f : v; };
-              w[z] = pack2<false>(clamp(f0), clamp(f1));
+              w[z] = pack2<true>(f.x, f.y);
             }
           }
           dst[i * (D / 16)] = make_uint4(w[0], w[1], w[2], w[3]);
         }
-        if constexpr (!kFold) {
-          if (part == 0) (kv ? p.exp_vs : p.exp_ks)[row] = kv ? sc[kv][y] / power : sc[kv][y];
-        }
+        if (part == 0) (kv ? p.exp_vs : p.exp_ks)[row] = sc[kv][y];
       }
+    float vm = -INFINITY;
+#pragma unroll
+    for (int y = 0; y < kPasses; ++y) {
+      const float lg = __log2f(fabsf(sc[1][y]));
+      if (part == 0) p.exp_vl[dst0 + y * kRows + lane / L] = lg;
+      vm = fmaxf(vm, lg);
+    }
+#pragma unroll
+    for (int o = L; o < 32; o <<= 1) vm = fmaxf(vm, __shfl_xor_sync(0xffffffffu, vm, o));
+    if (lane == 0) p.exp_vm[dst0 / 16] = vm;
   }
 }
 
 template <int D, int SRC, bool QBF16>
 cudaError_t launch_chunk_impl(const ChunkParams& p, int grid, cudaStream_t stream) {
   auto kern = paged_chunk_kernel<D, SRC, QBF16>;
-  using L = ChunkLayout<D, SRC == kExpanded && !QBF16>;
+  using L = ChunkLayout<D, SRC == kExpanded>;
   static int attr_done[64] = {0};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -1136,12 +1125,12 @@ cudaError_t launch_chunk_d(const ChunkParams& p, int kv, bool bf16, int grid, cu
 }
 
 template <int D>
-cudaError_t launch_expand_d(const ChunkParams& p, int kv, bool fold, int grid, cudaStream_t s) {
+cudaError_t launch_expand_d(const ChunkParams& p, int kv, bool bf16, int grid, cudaStream_t s) {
   if (kv == FA_DTYPE_INT8) {
-    if (fold) paged_expand_kernel<D, FA_DTYPE_INT8, true><<<grid, kExpandThreads, 0, s>>>(p);
+    if (bf16) paged_expand_kernel<D, FA_DTYPE_INT8, true><<<grid, kExpandThreads, 0, s>>>(p);
     else paged_expand_kernel<D, FA_DTYPE_INT8, false><<<grid, kExpandThreads, 0, s>>>(p);
   } else {
-    if (fold) paged_expand_kernel<D, FA_DTYPE_E4M3, true><<<grid, kExpandThreads, 0, s>>>(p);
+    if (bf16) paged_expand_kernel<D, FA_DTYPE_E4M3, true><<<grid, kExpandThreads, 0, s>>>(p);
     else paged_expand_kernel<D, FA_DTYPE_E4M3, false><<<grid, kExpandThreads, 0, s>>>(p);
   }
   return cudaGetLastError();

@@ -748,7 +748,7 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
         if constexpr (C::k8) {
           // O becomes the result times 2^-kScaleDown (one exponent: 2^(r - m) alone
           // may pass fp32's range)
-          const float lg = log2f(x);
+          const float lg = __log2f(x);
           const float f = x == 0.f ? 0.f : exp2f(ref[nt][c] - m[nt][c] - lg);
 #pragma unroll
           for (int k = 0; k < C::kKS; ++k) {

@@ -503,7 +503,7 @@ __device__ __forceinline__ void fmul2(float& d0, float& d1, float a0, float a1, 
   unpack_f2(d, d0, d1);
 }
 
-// 2^t for two lanes on the FMA pipe (no MUFU), t <= 64.
+// 2^t for two lanes on the FMA pipe (no MUFU), t <= 126.
 // Method: t = n + f with n = round-to-nearest(t) obtained by adding and
 // subtracting 1.5*2^23 (the addition leaves n in the low mantissa bits),
 // f in [-0.5, 0.5]; 2^f from a degree-3 polynomial fitted here by a Remez

@@ -305,9 +305,11 @@ int fa_kvcache_read(const fa_paged_cache* cache, void* K, void* V, const int* cu
  * that see no key, and rows of no sequence, get O = 0, LSE = -inf.  Keys that
  * no query may see have no effect, whatever their rows of the pages hold.
  * `dtype` (f16 / bf16) is that of Q and O; a 16-bit cache has the same.
- * For more than 16 query rows (n_b x Hq / kv_heads) per KV head the keys and
- * values of 8-bit pages may be read as f16: with bf16 results magnitudes above
- * 65504 then count as 65504 and those below 2^-24 as 0.
+ * 8-bit keys and values are used exactly, with their scales in fp32.  The
+ * probabilities are rounded to f16 (16-bit pages: to their type), over 8-bit pages
+ * after their product with the value's scale and relative to a row's largest one.
+ * For few tokens bf16 queries over 8-bit pages are rounded to f16 relative to the
+ * row's largest magnitude (exact down to 2^-17 of it).
  * max_seqlen_q / max_seqlen_k bound n_b and seqlens_k (tokens and keys beyond
  * them are not computed / not seen).  The kernels and the workspace are chosen by
  * max_seqlen_k as it is given, so it should be no more than the longest sequence

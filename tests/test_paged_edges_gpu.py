@@ -212,7 +212,7 @@ def _check_relative(P, q, Hq, mode, got):
         assert ((gl[:, rows] - z).abs() <= 1e-4 + z.abs() * 2.0 ** -20).all()
 
 
-@pytest.mark.parametrize("nq", [1, 6])
+@pytest.mark.parametrize("nq", [1, 6, 40])
 @pytest.mark.parametrize("kind", [(F16, I8), (F16, E4M3), (BF16, I8), (BF16, E4M3)],
                          ids=["f16-int8", "f16-e4m3", "bf16-int8", "bf16-e4m3"])
 @pytest.mark.parametrize("late", [True, False], ids=["late", "early"])
@@ -237,7 +237,7 @@ def test_small_value_row_takes_the_weight(sm100, nq, kind, late):
     _check_relative(P, q, 4, 1, _attend(P, q, 4, 1))
 
 
-@pytest.mark.parametrize("nq", [1])
+@pytest.mark.parametrize("nq", [1, 40])
 @pytest.mark.parametrize("cache", [I8, E4M3], ids=["int8", "e4m3"])
 @pytest.mark.parametrize("size", [2e-30, 1e-20, 1e-7, 1e-4, 1e6, 1e20, 1e36])
 def test_bf16_results_hold_their_range(sm100, nq, cache, size):
@@ -250,7 +250,7 @@ def test_bf16_results_hold_their_range(sm100, nq, cache, size):
     _check_relative(P, q, 8, 1, _attend(P, q, 8, 1))
 
 
-@pytest.mark.parametrize("nq", [1])
+@pytest.mark.parametrize("nq", [1, 40])
 def test_lse_over_8_bit_pages_is_held_in_32_bits(sm100, nq):
     """Scores come from the stored bits and their fp32 scales: the LSE of bf16 results is
     as good as that of f16 ones."""
