@@ -87,7 +87,7 @@ struct alignas(64) ChunkParams {
   int skip_rows;     // sequences with at most this many rows per KV head are not ours
   int runs;          // 1: CTAs take equal runs of the work order, 0: a (pair, head) each
   int n_ctas;
-  int fill_outside;  // write the rows of no sequence
+  int fill;          // write the rows that no kernel computes
   int head0, n_heads;  // KV heads of this launch
   // 8-bit pages: 16-bit rows and scales of the launch's heads (paged_expand_kernel)
   long long exp_rows;

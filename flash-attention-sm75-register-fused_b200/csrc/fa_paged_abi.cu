@@ -443,7 +443,7 @@ int fa_fwd_paged(const fa_paged_cache* cache, const void* Q, long long q_token_s
     if (!maps) return FA_ERR_TENSOR_MAP;
     for (p.head0 = 0; p.head0 < a.c.heads; p.head0 += k.exp_heads) {
       p.n_heads = a.c.heads - p.head0 < k.exp_heads ? a.c.heads - p.head0 : k.exp_heads;
-      p.fill_outside = !k.decode && p.head0 == 0 ? 1 : 0;
+      p.fill = !k.decode && p.head0 == 0 ? 1 : 0;
       p.epoch = fa::host_next_epoch();
       p.n_ctas = k.runs ? k.n_ctas : k.slots * p.n_heads;
       if (fa::launch_paged_chunk(p, cache->head_dim, cache->dtype, bf16, fa::host_sm_count(), st) !=

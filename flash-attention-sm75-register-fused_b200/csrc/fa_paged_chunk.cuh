@@ -314,20 +314,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
   // ---- where does this CTA's work start?
   const int cta = static_cast<int>(blockIdx.x);
   find_start<kExp>(p, p.runs ? cta : cta / p.n_heads, &start, sh_scan[0], sh_scan[1]);
-  {
-    if (p.fill_outside) {
-      const int head = a.r.B > 0 ? min(max(__ldg(a.r.cu), 0), a.r.total) : a.r.total;
-      const int tail = a.r.B > 0 ? min(max(__ldg(a.r.cu + a.r.B), head), a.r.total) : a.r.total;
-      const int n_out = head + a.r.total - tail;
-      for (int y = cta; y < n_out; y += static_cast<int>(gridDim.x)) {
-        const int t = y < head ? y : tail + y - head;
-        for (int i = threadIdx.x; i < a.Hq * D / 2; i += kThreads)
-          static_cast<uint32_t*>(a.o)[static_cast<long long>(t) * (a.Hq * D / 2) + i] = 0u;
-        if (a.lse != nullptr)
-          for (int i = threadIdx.x; i < a.Hq; i += kThreads)
-            a.lse[static_cast<long long>(i) * a.r.total + t] = -INFINITY;
-      }
-    }
+  if (p.fill) {
+    fill_outside(a, D, cta, static_cast<int>(gridDim.x));
+    if (a.max_q < a.r.total)
+      for (int b = cta; b < a.r.B; b += static_cast<int>(gridDim.x)) fill_beyond(a, D, load_seq(a, b));
   }
   // (whatever ends this CTA early, the join finds nothing to do for it)
   if (p.runs && p.n_ctas > 1 && threadIdx.x == 0) p.ws_cuts[cta].parts = 0;

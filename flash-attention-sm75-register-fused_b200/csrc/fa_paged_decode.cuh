@@ -181,23 +181,6 @@ __host__ __device__ constexpr long long slot_floats(int rows, int d) {
   return static_cast<long long>(rows) * (d + 2);
 }
 
-// O = 0, LSE = -inf in the packed rows of no sequence (before the first and
-// after the last), dealt over the grid's blocks.
-__device__ __forceinline__ void fill_outside(const PagedAttn& a, int d, int block, int n_blocks) {
-  const int head = min(max(__ldg(a.r.cu), 0), a.r.total);
-  const int tail = min(max(__ldg(a.r.cu + a.r.B), head), a.r.total);
-  const int n_out = head + a.r.total - tail;
-  const int n = static_cast<int>(blockDim.x), words = a.Hq * d / 2;
-  for (int x = block; x < n_out; x += n_blocks) {
-    const int t = x < head ? x : tail + x - head;
-    for (int i = threadIdx.x; i < words; i += n)
-      static_cast<uint32_t*>(a.o)[static_cast<long long>(t) * words + i] = 0u;
-    if (a.lse != nullptr)
-      for (int i = threadIdx.x; i < a.Hq; i += n)
-        a.lse[static_cast<long long>(i) * a.r.total + t] = -INFINITY;
-  }
-}
-
 // Partial result of a row over a lane's D / 32 columns.
 template <int D>
 struct Partial {
@@ -274,7 +257,9 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
     // the teams take equal parts of the units of (sequence, head) blockIdx.x
     fill_outside(a, D, static_cast<int>(blockIdx.x), static_cast<int>(gridDim.x));
     b_first = static_cast<int>(blockIdx.x) / H;
-    const int n = (load_short(a, b_first, p.max_rows).vis + C::kSub - 1) / C::kSub;
+    const Seq s = load_short(a, b_first, p.max_rows);
+    if (static_cast<int>(blockIdx.x) % H == 0) fill_beyond(a, D, s);
+    const int n = (s.vis + C::kSub - 1) / C::kSub;
     const long long base = static_cast<long long>(static_cast<int>(blockIdx.x) % H) * (n + kSegCost) + kSegCost;
     rel = base + static_cast<long long>(n) * team / kTeams;
     v1 = base + static_cast<long long>(n) * (team + 1) / kTeams;
@@ -843,7 +828,7 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
 // (few rows, many slots), or a segment of more than kManySlots: the block's
 // warps share a row's slots and are joined at the end.
 // Also writes the rows that no team of the decode kernel computes: rows of
-// sequences without visible keys and packed rows of no sequence.
+// sequences without visible keys or beyond max_q, and packed rows of no sequence.
 constexpr int kManySlots = 32;
 
 template <int D, bool BF16, int kRows>
@@ -860,6 +845,7 @@ __global__ void __launch_bounds__(kCombineThreads)
   fill_outside(a, D, static_cast<int>(blockIdx.y * gridDim.x + blockIdx.x),
                static_cast<int>(gridDim.x * gridDim.y));
   const Seq s = load_short(a, b, p.max_rows);
+  if (h == 0 && blockIdx.y == 0) fill_beyond(a, D, s);
   const Spot sp = find_spot<kCombineThreads>(a, sub, p.max_rows, b, sh);
   // the decode kernel's results are complete and visible after this
   ptx::grid_dep_wait();

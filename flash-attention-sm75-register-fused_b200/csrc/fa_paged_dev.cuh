@@ -38,7 +38,7 @@ __device__ __forceinline__ void widen(uint32_t w, uint32_t& p0, uint32_t& p1) {
 
 // What a sequence brings to a call.
 struct Seq {
-  int c0, nq;    // first packed row; new tokens
+  int c0, n, nq; // first packed row; new tokens; those of them that are computed
   int nk, off;   // visible keys: key j < lim(i) = min(nk, i + off + 1) (causal) or nk;
                  // off goes by the whole length, also where bounds cut nk
   int vis;       // keys any of its rows may see
@@ -56,11 +56,34 @@ __device__ __forceinline__ Seq load_seq(const PagedAttn& a, int b) {
   const int len = min(max(__ldg(a.r.lens + b), 0), 3 << 29);
   const int n = c1 - c0;
   s.c0 = c0;
+  s.n = n;
   s.nq = min(n, a.max_q);
   s.nk = min(min(len, a.max_k), a.c.max_pages * a.c.page_size);
   s.off = a.causal == FA_CAUSAL_BOTTOM_RIGHT ? len - n : 0;
   s.vis = s.nq > 0 ? row_limit(a, s, s.nq - 1) : 0;
   return s;
+}
+
+// O = 0, LSE = -inf in packed row t, which no kernel computes.  (Also below: all
+// threads of a block call it.)
+__device__ __forceinline__ void fill_row(const PagedAttn& a, int d, int t) {
+  const int n = static_cast<int>(blockDim.x), words = a.Hq * d / 2;
+  for (int i = threadIdx.x; i < words; i += n)
+    static_cast<uint32_t*>(a.o)[static_cast<long long>(t) * words + i] = 0u;
+  if (a.lse != nullptr)
+    for (int i = threadIdx.x; i < a.Hq; i += n) a.lse[static_cast<long long>(i) * a.r.total + t] = -INFINITY;
+}
+// The rows of no sequence (before the first and after the last), dealt over the
+// grid's blocks.
+__device__ __forceinline__ void fill_outside(const PagedAttn& a, int d, int block, int n_blocks) {
+  const int head = a.r.B > 0 ? min(max(__ldg(a.r.cu), 0), a.r.total) : a.r.total;
+  const int tail = a.r.B > 0 ? min(max(__ldg(a.r.cu + a.r.B), head), a.r.total) : a.r.total;
+  const int n_out = head + a.r.total - tail;
+  for (int x = block; x < n_out; x += n_blocks) fill_row(a, d, x < head ? x : tail + x - head);
+}
+// The tokens of a sequence beyond max_q.
+__device__ __forceinline__ void fill_beyond(const PagedAttn& a, int d, const Seq& s) {
+  for (int i = a.max_q; i < s.n; ++i) fill_row(a, d, s.c0 + i);
 }
 
 // Exclusive prefix sum of `sum` over the block's threads; *total its sum.

@@ -97,7 +97,8 @@ def flash_attention_forward_paged(q, k_cache, v_cache, block_table, cu_seqlens_q
         scale: float (default 1/sqrt(D))
         return_lse: also return LSE [H_q, total_q] fp32 (natural log)
 
-    Rows that see no key, and rows of no sequence, return O = 0, LSE = -inf.
+    Rows that see no key, rows of no sequence and tokens beyond max_seqlen_q
+    return O = 0, LSE = -inf.
     """
     mode = 0
     if causal:

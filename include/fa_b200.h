@@ -310,8 +310,8 @@ int fa_kvcache_read(const fa_paged_cache* cache, void* K, void* V, const int* cu
  * after their product with the value's scale and relative to a row's largest one.
  * For few tokens bf16 queries over 8-bit pages are rounded to f16 relative to the
  * row's largest magnitude (exact down to 2^-17 of it).
- * max_seqlen_q / max_seqlen_k bound n_b and seqlens_k (tokens and keys beyond
- * them are not computed / not seen).  The kernels and the workspace are chosen by
+ * max_seqlen_q / max_seqlen_k bound n_b and seqlens_k: tokens beyond them get O =
+ * 0, LSE = -inf, keys beyond them are not seen.  The kernels and the workspace are chosen by
  * max_seqlen_k as it is given, so it should be no more than the longest sequence
  * there may be, and never more than max_pages * page_size.  Hq / kv_heads is at most 128.
  * `workspace` (16-byte aligned) needs fa_fwd_paged_workspace_bytes() bytes (may

@@ -177,6 +177,44 @@ def test_key_bounds_do_not_move_the_causal_rule(sm100, nq, kind):
     _close(call(c["table"][:, :11], 200), _plain_rows(P, q, 4, limits(176)), kind[0])
 
 
+@pytest.mark.parametrize("B,nq", [(3, 4), (2, 90), (40, 3)])
+def test_rows_beyond_max_seqlen_q(sm100, B, nq):
+    """Tokens past max_seqlen_q are not computed: O = 0, LSE = -inf; the others' results
+    are those of the whole call."""
+    P = Paged([(nq, 100 + b) for b in range(B)], 2, 64, 16, F16, seed=52, first=1, tail=2)
+    q = P.new(8)
+    c = P.cuda()
+    full = _attend(P, q, 8, 1)
+    for most in (nq - 1, 1, 0):
+        junk = [torch.full((P.total, 8, 64), float("nan"), dtype=F16, device="cuda") for _ in range(3)]
+        del junk  # (memory that a result may get is not zero)
+        o, lse = fa.flash_attention_forward_paged(q.cuda(), c["k_cache"], c["v_cache"], c["table"], c["cu"],
+                                                  c["lens"], most, 200, causal=True, return_lse=True)
+        i = torch.arange(P.total, device="cuda") - 1
+        keep = (i >= 0) & (i < B * nq) & (i % nq < most)
+        assert (o[~keep] == 0).all() and (lse[:, ~keep] == -math.inf).all()
+        # (other kernels may take the shorter sequences: two roundings of P and O, values below 6)
+        assert keep.sum() == B * most
+        if most:
+            assert (o[keep].float() - full[0][keep].float()).abs().max() <= 6 * 6 * UNIT[F16]
+
+
+def test_rows_beyond_max_seqlen_q_in_a_mixed_batch(sm100):
+    """The same where both kernels run: a chunk is cut, single tokens are whole."""
+    lens = [(300, 400), (1, 50), (2, 60), (250, 250)]
+    P = Paged(lens, 2, 64, 16, F16, seed=53)
+    q = P.new(8)
+    c = P.cuda()
+    full = _attend(P, q, 8, 1)
+    junk = [torch.full((P.total, 8, 64), float("nan"), dtype=F16, device="cuda") for _ in range(3)]
+    del junk
+    o, lse = fa.flash_attention_forward_paged(q.cuda(), c["k_cache"], c["v_cache"], c["table"], c["cu"], c["lens"],
+                                              200, 400, causal=True, return_lse=True)
+    keep = torch.cat([torch.arange(m) < 200 for m, _ in lens]).cuda()
+    assert (o[~keep] == 0).all() and (lse[:, ~keep] == -math.inf).all()
+    assert (o[keep].float() - full[0][keep].float()).abs().max() <= 6 * 6 * UNIT[F16]
+
+
 # ------------------------------------------------------------------ scales of very different size
 
 def _check_relative(P, q, Hq, mode, got):
