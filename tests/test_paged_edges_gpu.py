@@ -8,7 +8,8 @@ import pytest
 import torch
 
 import flash_attention_sm75 as fa
-from tests.paged_plain import UNIT, Paged, attention, quantise
+from tests import abi_ctypes as abi
+from tests.paged_plain import QMAX, UNIT, Paged, attention, quantise
 from tests.test_paged_gpu import BF16, E4M3, F16, I8, _attend, _check
 
 pytestmark = pytest.mark.gpu
@@ -301,3 +302,152 @@ def test_lse_over_8_bit_pages_is_held_in_32_bits(sm100, nq):
             # one exponential is good to 2^-13 at worst (its approximation's error has both
             # signs over the sum), fp32 sums and scores to 1e-6: 2e-5 is a tenth of what f16 keys cost
             assert (gl - lse).abs().max() <= 2e-5
+
+
+# ------------------------------------------------------------------ many heads, many sequences, large caches
+
+@pytest.mark.parametrize("mode", [0, 1])
+@pytest.mark.parametrize("kind", [(F16, F16), (BF16, BF16), (F16, I8), (BF16, E4M3)],
+                         ids=["f16", "bf16", "f16-int8", "bf16-e4m3"])
+@pytest.mark.parametrize("G,d", [(64, 64), (65, 128), (100, 64), (128, 128), (128, 64)])
+def test_groups_up_to_128_heads(sm100, G, d, kind, mode):
+    """Query tiles of one token (more than 64 heads per KV head), full and not, and of two."""
+    P = Paged([(1, 150), (5, 5), (0, 9), (2, 300), (1, 0)], 2, d, 16, kind[1], io=kind[0], seed=71)
+    q = P.new(2 * G)
+    _check(P, q, 2 * G, mode, _attend(P, q, 2 * G, mode))
+
+
+def test_one_token_of_128_heads(sm100):
+    """A decode step with a full one-token tile, keys split between many CTAs."""
+    P = Paged([(1, 6000)], 1, 128, 64, BF16, io=BF16, seed=72)
+    q = P.new(128)
+    _check(P, q, 128, 1, _attend(P, q, 128, 1))
+
+
+@pytest.mark.parametrize("cache", [F16, I8], ids=["f16", "int8"])
+@pytest.mark.parametrize("B", [33, 100, 1500])
+def test_write_and_read_many_sequences(sm100, B, cache):
+    """More sequences than one warp looks at at once, some of them without tokens."""
+    g = torch.Generator().manual_seed(B)
+    new = [int(x) for x in torch.randint(0, 4, (B,), generator=g)]
+    new[B // 2:B // 2 + 20] = [0] * len(new[B // 2:B // 2 + 20])
+    new[3] = 70
+    P = Paged([(m, m + b % 5) for b, m in enumerate(new)], 1, 64, 16, cache, seed=73, first=2, tail=1, poison=False)
+    c = P.cuda()
+    x = torch.randn(P.total, 2, 64, generator=P.g).half()
+    xd = x.cuda()
+    fa.kvcache_write_paged(xd[:, :1], xd[:, 1:], c["k_cache"], c["v_cache"], c["table"], c["cu"], c["lens"],
+                           k_scale=c["k_scale"], v_scale=c["v_scale"])
+    got = fa.kvcache_read_paged(c["k_cache"], c["v_cache"], c["table"], c["cu"], c["lens"], P.total,
+                                k_scale=c["k_scale"], v_scale=c["v_scale"], dtype=F16)
+    pages = [c["k_cache"].cpu(), c["v_cache"].cpu()]
+    inside = torch.zeros(P.total, dtype=torch.bool)
+    inside[P.cu[0]:P.cu[-1]] = True
+    for kv in range(2):
+        want = x[:, kv:kv + 1]
+        if cache == I8:
+            y, s = quantise(want, I8)
+            want = (y.float() * s.unsqueeze(-1)).half()
+        back = got[kv].cpu()
+        assert torch.equal(back[inside], want[inside]) and (back[~inside] == 0).all()
+        for b in (0, 3, 31, 32, B - 1):  # and the right pages hold them
+            m, n = P.lens[b]
+            for i in range(m):
+                pg, row = P.place(b, n - m + i)
+                stored = y[P.cu[b] + i] if cache == I8 else want[P.cu[b] + i]
+                assert torch.equal(pages[kv][pg, :, row], stored)
+
+
+@pytest.mark.parametrize("cache", [F16, I8], ids=["f16", "int8"])
+def test_byte_offsets_pass_32_bits(sm100, cache):
+    """Pages that lie more than 2^32 bytes into each tensor: written, read back, and
+    attended over by both kernels."""
+    page, Hkv, d = 128, 8, 128
+    pages = (1 << 32) // (page * Hkv * d * (1 if cache == I8 else 2)) + 40
+    kc = torch.zeros(pages, Hkv, page, d, dtype=cache, device="cuda")
+    vc = torch.zeros_like(kc)
+    assert (pages - 5) * kc.stride(0) * kc.element_size() > 1 << 32
+    s = {n: torch.zeros(pages, Hkv, page, device="cuda") for n in ("k_scale", "v_scale")} if cache == I8 else {}
+    table = torch.tensor([[pages - 1, 3, pages - 3], [pages - 2, pages - 5, 7]], dtype=torch.int32, device="cuda")
+    g = torch.Generator().manual_seed(0)
+    n = [300, 270]
+    x = torch.randn(sum(n), 2 * Hkv, d, generator=g).half()
+    xd = x.cuda()
+    cu = [0, n[0], sum(n)]
+    fa.kvcache_write_paged(xd[:, :Hkv], xd[:, Hkv:], kc, vc, table, cu, n, **s)
+    k, v = fa.kvcache_read_paged(kc, vc, table, cu, n, sum(n), dtype=F16, **s)
+    for got, want in ((k, x[:, :Hkv]), (v, x[:, Hkv:])):
+        if cache == I8:
+            y, sc = quantise(want, I8)
+            want = (y.float() * sc.unsqueeze(-1)).half()
+        assert torch.equal(got.cpu(), want)
+    # the rows' own bytes are where the table says, and nowhere 2^32 bytes before
+    assert torch.equal(kc[pages - 1, :, 0].cpu(), (quantise(x[0, :Hkv], I8)[0] if cache == I8 else x[0, :Hkv]))
+    assert not kc[39].any() and not kc[35].any()
+    for nq in (1, 40):
+        q = torch.randn(2 * nq, 32, d, generator=g).half().cuda()
+        o = fa.flash_attention_forward_paged(q, kc, vc, table, [0, nq, 2 * nq], n, nq, 300, causal=True, **s)
+        ref = fa.flash_attention_varlen_forward(q, k, v, [0, nq, 2 * nq], cu, nq, 300, causal=True)
+        # two kernels on values of at most ~3, each within 2^-11 relative of the sums they round
+        assert (o.float() - ref.float()).abs().max().item() <= 4e-3
+
+
+# ------------------------------------------------------------------ captured graphs, C entry points
+
+@pytest.mark.parametrize("kind", [(F16, F16), (BF16, E4M3), (F16, I8)], ids=["f16", "bf16-e4m3", "f16-int8"])
+def test_chunks_in_a_cuda_graph(sm100, kind):
+    """Captured once, replayed on other lengths and another split of the rows within the same
+    bounds: chunks beside single tokens, more keys, fewer rows in use."""
+    lens = [(120, 1500), (1, 900), (29, 400)]
+    P = Paged(lens, 2, 128, 16, kind[1], io=kind[0], seed=81)
+    q = P.new(8)
+    c = P.cuda()
+    qd = q.cuda()
+    call = lambda: fa.flash_attention_forward_paged(  # noqa: E731
+        qd, c["k_cache"], c["v_cache"], c["table"], c["cu"], c["lens"], 120, 1500, causal=True,
+        k_scale=c["k_scale"], v_scale=c["v_scale"], return_lse=True)
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for now in (lens, [(1, 1), (1, 900), (100, 400)], [(0, 3), (2, 2), (3, 3)], [(100, 1500), (20, 20), (30, 31)], lens):
+        P.lens = now
+        P.cu = [0, now[0][0], now[0][0] + now[1][0], sum(m for m, _ in now)]
+        c["lens"].copy_(torch.tensor([n for _, n in now], dtype=torch.int32))
+        c["cu"].copy_(torch.tensor(P.cu, dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        _check(P, q, 8, 1, out)
+
+
+@pytest.mark.parametrize("nq", [1, 50])
+@pytest.mark.parametrize("kind", [(F16, F16), (BF16, I8)], ids=["f16", "bf16-int8"])
+def test_c_entry_points(sm100, nq, kind):
+    """The same calls through the C ABI: write, read back, attend."""
+    io, cache = kind
+    P = Paged([(nq, 170), (nq, nq)], 2, 64, 16, cache, io=io, order="token", seed=91)
+    c = P.cuda()
+    pc = abi.paged_cache(c["k_cache"], c["v_cache"], c["table"], c["k_scale"], c["v_scale"])
+    new = torch.randn(P.total, 5, 64, generator=P.g).to(io)
+    nd = new.cuda()
+    assert abi.fa_kvcache_write(pc, nd[:, :2], nd[:, 2:4], c["cu"], c["lens"]) == 0
+    k, v = (torch.full((P.total, 2, 64), float("nan"), dtype=io, device="cuda") for _ in range(2))
+    assert abi.fa_kvcache_read(pc, k, v, c["cu"], c["lens"]) == 0
+    for got, name, x in ((k, "k", new[:, :2]), (v, "v", new[:, 2:4])):
+        y, s = quantise(x, cache) if cache in QMAX else (x, None)
+        for b, (m, n) in enumerate(P.lens):
+            rows = slice(P.cu[b], P.cu[b + 1])
+            P.put(name, b, range(n - m, n), y[rows], s[rows] if s is not None else None)
+        want = (y.float() * s.unsqueeze(-1)).to(io) if s is not None else x
+        assert torch.equal(got.cpu(), want)
+    q = P.new(6)
+    o = torch.full((P.total, 6, 64), float("nan"), dtype=io, device="cuda")
+    lse = torch.full((6, P.total), float("nan"), device="cuda")
+    for causal in (1, 2):
+        assert abi.fa_fwd_paged(pc, q.cuda(), o, lse, c["cu"], c["lens"], nq, 170, causal=causal) == 0
+        torch.cuda.synchronize()
+        _check(P, q, 6, causal, (o, lse))
+    o2 = torch.empty_like(o)
+    assert abi.fa_fwd_paged(pc, q.cuda(), o2, None, c["cu"], c["lens"], nq, 170, causal=2) == 0
+    assert torch.equal(o, o2) and abi.load().fa_device_status(1) == 0
