@@ -16,9 +16,9 @@
 // loads for up to 32 sequences, which overlap the source rows' own loads when
 // writing) and keeps U independent 16-byte loads per lane in flight.
 //
-// Measured: 48 MB of bf16 rows of ragged prompts copied into pages 9.7 us (7.4 at
-// the rate of a plain copy, 6.5 TB/s); 217 MB of int8 prefixes read back as bf16 38.6
-// us (5.6 TB/s); eight tokens written and read back 4.5 us (two launches).
+// Measured: 48 MB of bf16 rows of ragged prompts copied into pages 9.9 us (7.4 at
+// the rate of a plain copy, 6.5 TB/s); 217 MB of int8 prefixes read back as bf16 38.3
+// us (5.7 TB/s); eight tokens written and read back 4.8 us (two launches).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -307,6 +307,10 @@ RowMap row_map(const PagedCache& c, const PagedRows& r) {
   return {static_cast<unsigned>(r.total) * heads2,
           static_cast<unsigned>(((1ull << 32) + heads2 - 1) / heads2)};
 }
+// Few rows: up to 64 for each of the 148 SMs.  One row per lane group / more, bf16
+// rows written (us): at d = 128 1024 rows 2.1 / 2.3, 9472 2.8 / 2.9, 18944 3.6 / 3.3,
+// 75776 9.8 / 7.4 (int8: 2.6 / 2.9, 2.9 / 3.2, 3.6 / 3.5, 8.6 / 7.9); at d = 64 9472 2.6 /
+// 2.7, 37888 3.7 / 3.3 (int8: 2.7 / 2.9, 3.5 / 3.5); reading is alike.
 bool few_rows(unsigned n_rows) { return n_rows <= 148u * 64u; }
 
 template <int D, bool BF16, int KIND>

@@ -179,8 +179,8 @@ __device__ __forceinline__ int expand_blocks(const Seq& s) { return (s.vis + kBl
 // head) sees keys [0, lim(i)), lim(i) = clamp(off + (i + 1) c, 0, vis) for c tokens
 // a pair; it takes kItemCost + lim(i) positions of the work order, the key tile
 // that starts at key k the one at kItemCost + k.
-// (kItemCost: six ragged chunks over e4m3 pages take 271 us with 256, 263 with 384
-// or 512, 275 with 1024.  kMinRun, the shortest run: 64 tokens over 8192 keys take 37.9
+// (kItemCost: six ragged chunks over e4m3 pages take 271 us with 256, 260 with 384,
+// 262 with 512, 273 with 1024.  kMinRun, the shortest run: 64 tokens over 8192 keys take 37.9
 // us with 128, 35.5 with 512; 512 over 1024 26.9 with 128, 27.3 with 512, 31.8 with 1024)
 constexpr int kItemCost = 384;
 constexpr int kMinRun = 512;
@@ -978,7 +978,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
 // [n_heads][exp_rows][d] for K (in the type of the queries) and for V (f16), with
 // the scales [n_heads][exp_rows], V's logarithms and the largest of every 16 rows.
 // Both types hold 8-bit values exactly.  A warp takes groups of 16 keys of one head.
-// Bound by memory, much of it L2: 39 MB of e4m3 pages become 79 MB in 19 us.
+// Bound by memory, much of it L2: 39 MB of e4m3 pages become 79 MB in 20 us.
 constexpr int kExpandThreads = 128;
 
 template <int D, int KV, bool kKBf16>

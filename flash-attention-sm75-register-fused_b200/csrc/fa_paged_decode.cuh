@@ -43,8 +43,8 @@
 // memory: one launch, no workspace, no plan over the batch.
 //
 // Measured with the join, 8 KV heads, d = 128, GQA 4, one token: 8 sequences x 8192
-// keys of f16 pages 47.1 us (5.7 TB/s; a plain copy runs at 6.5), one of 65536 over
-// e4m3 pages 32.7 us (4.2 TB/s): loads at HBM's rate between about 5 us until the
+// keys of f16 pages 47.5 us (5.7 TB/s; a plain copy runs at 6.5), one of 65536 over
+// e4m3 pages 33.1 us (4.2 TB/s): loads at HBM's rate between about 5 us until the
 // first unit and 3 to 6 for the join.
 #include "fa_paged.h"
 #include "fa_paged_dev.cuh"
@@ -142,8 +142,8 @@ __device__ __forceinline__ Seq load_short(const PagedAttn& a, int b, int max_row
 // The runs are cut from positions, not units: a segment (sequence, head) of n
 // units has kSegCost positions before its units' n, for what a team spends on a
 // segment besides its units (queries, results).  Without them the teams that
-// get many short sequences finish last (32 ragged sequences over int8 pages: 37 us
-// without, 30 with, the kernel alone).
+// get many short sequences finish last (32 ragged sequences over int8 pages: 42 us
+// without, 32 with, the kernel alone).
 constexpr int kSegCost = 1;
 __device__ __forceinline__ int positions_of(const PagedAttn& a, int b, int sub, int max_rows) {
   const int n = (load_short(a, b, max_rows).vis + sub - 1) / sub;
@@ -949,7 +949,8 @@ cudaError_t launch_impl(const DecodeParams& p, int n_ctas, cudaStream_t stream) 
   const unsigned segments = static_cast<unsigned>(p.a.r.B) * p.a.c.heads;
   // blocks of one row fill the device with few segments (8 heads x 64 rows: 38
   // us for the call instead of 50; 64 x 4: 86 / 90), blocks of eight with many
-  // (256 x 4: 91 / 86; 128 x 64: 155 / 113)
+  // (256 x 4: 91 / 86; 128 x 64: 155 / 113); the line is at four rows for each of
+  // the 148 SMs
   const bool many = static_cast<long long>(segments) * p.max_rows > 4 * 148;
   cfg.gridDim = dim3(segments, many ? (p.max_rows + 7) / 8 : p.max_rows);
   cfg.blockDim = dim3(kCombineThreads);
@@ -1002,8 +1003,8 @@ cudaError_t launch_d(const DecodeParams& p, int kv, bool bf16, int n_ctas, cudaS
 
 // Query rows per (sequence, KV head) up to which this kernel is taken.  Over
 // 8-bit pages always kRowsMax, for the chunk kernel has to expand them first
-// (B=8, 8192 keys, 8 KV heads, d = 128, 64 rows: 105 us here, 155 there; 32
-// rows: 60 / 152).  16-bit pages: up to 32 rows (16: 54 / 70 us, 32: 61 / 85);
+// (B=8, 8192 keys, 8 KV heads, d = 128, int8, 64 rows: 106 us here, 150 there; 32
+// rows: 60 / 151).  16-bit pages: up to 32 rows (16: 54 / 70 us, 32: 61 / 85);
 // above, teams of four warps read a unit four times from shared memory and are
 // slower (48 rows: 106 / 87, 32 x 4096 keys: 210 / 137), except at d = 64 with
 // less than half a CTA of the chunk kernel per SM (4 x 8 heads x 4096 keys, 48
@@ -1023,9 +1024,9 @@ namespace pdec {
 //        5                  8.5 / 8.1   9.7 / 8.2  12.1 / 8.9  37.7 / 35.4
 //        8                  8.6 / 10.2 10.6 / 10.4 15.0 / 11.4 53.3 / 49.7
 //        16                 9.2 / 15.7 13.1 / 15.9 20.7 / 17.3 91.5 / 87.3
-//   int8 3                  9.7 / 8.3  10.5 / 8.4  12.0 / 9.3  29.9 / 29.8
-//        4                  9.5 / 9.4  11.1 / 9.6  13.6 / 10.9 34.5 / 35.3
-//        8                  9.6 / 14.1 12.1 / 14.4 16.7 / 16.4 54.1 / 58.6
+//   int8 3                  9.5 / 8.6  10.8 / 8.9  12.5 / 9.8  30.8 / 31.3
+//        4                  9.8 / 9.8  11.4 / 10.1 13.5 / 11.3 35.7 / 36.9
+//        8                  9.7 / 14.6 12.4 / 14.9 17.1 / 17.2 55.5 / 59.8
 // With a CTA for half the SMs or more 8 units, though equal lengths would allow
 // 16: in a ragged batch the longest sequence has one CTA too (152 heads, lengths
 // of 1 to 16 units per team: 17.1 / 16.9, mostly short ones 15.8 / 16.1).
