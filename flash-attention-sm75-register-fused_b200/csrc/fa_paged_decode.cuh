@@ -34,7 +34,8 @@
 // by a power of two.
 //
 // A team whose run covers a whole (sequence, head) writes O and LSE; otherwise
-// its unnormalised O, m and l go to one of its two workspace slots (its run's
+// its unnormalised O, m and l (8-bit pages: its result and the logarithm of its
+// sum) go to one of its two workspace slots (its run's
 // first part, which continues a head of the team before, or its last, which
 // the next team continues) and paged_combine_kernel joins them in order.
 //
