@@ -64,7 +64,14 @@ struct PagedAttn {
   int max_q, max_k;
   int causal;                 // FA_CAUSAL_*
   float scale_log2;           // scale * log2(e)
+  // Attention over two sets of keys in two passes: the first stores its results here
+  // as fp32 (part = kPartFirst; o and lse are not used), the second joins its own
+  // with them (kPartSecond).
+  int part;                   // kPart*
+  float* part_o;              // [total, Hq, d]
+  float* part_lse;            // [total, Hq], natural log
 };
+enum { kPartNone = 0, kPartFirst = 1, kPartSecond = 2 };
 
 // An item of the chunk kernel that the end of a run cuts: its sequence's first row
 // and tokens, its first token, KV head and parts (0: none is cut).
@@ -110,6 +117,30 @@ cudaError_t launch_cache_write(const PagedCache& c, const PagedRows& r, const Pa
                                int head_dim, int cache_dtype, bool bf16, cudaStream_t stream);
 cudaError_t launch_cache_read(const PagedCache& c, const PagedRows& r, void* k, void* v,
                               int head_dim, int cache_dtype, bool bf16, cudaStream_t stream);
+
+// Summed attention weights (fa_paged_weights.cu): a.lse is read; row (b, h) of the
+// sums at w + b * w_seq + h * w_head.
+struct PagedWeights {
+  PagedAttn a;
+  float* w;
+  long long w_seq, w_head;
+  int mode;  // FA_WEIGHTS_*
+};
+cudaError_t launch_paged_weights(const PagedWeights& p, int head_dim, int cache_dtype, bool bf16, int sms,
+                                 cudaStream_t stream);
+
+// Eviction (fa_paged_evict.cu).
+struct PagedEvict {
+  PagedCache c;
+  float* w;
+  long long w_seq, w_head;
+  const int* lens;
+  const int* keep;  // [B], or nullptr: keep_all
+  int keep_all, first, recent;
+  int* new_lens;
+  int B;
+};
+cudaError_t launch_paged_evict(const PagedEvict& p, int row_bytes, bool scales, int sms, cudaStream_t stream);
 
 struct alignas(64) DecodeParams {
   CUtensorMap tm_k;  // (d, page rows, heads, pages), box (min(row, 128 bytes), 16, 1, 1)

@@ -18,8 +18,9 @@ bool is_8bit(int dtype) { return dtype == FA_DTYPE_INT8 || dtype == FA_DTYPE_E4M
 constexpr int kMaxHeads = 1 << 14, kMaxBatch = 1 << 20, kMaxRows = 1 << 28;
 
 // Checks the cache's description and the call's 16-bit type; fills the
-// device-side view.  `writes`: no two entries may share memory.
-int check_cache(const fa_paged_cache* c, int dtype, bool writes, fa::PagedCache* out) {
+// device-side view.  `writes`: no two entries may share memory.  `values`: V and its
+// scales are used too.
+int check_cache(const fa_paged_cache* c, int dtype, bool writes, fa::PagedCache* out, bool values = true) {
   if (!c) return FA_ERR_INVALID_ARG;
   if (c->head_dim != 64 && c->head_dim != 128) return FA_ERR_UNSUPPORTED_HEAD_DIM;
   if (dtype != FA_DTYPE_F16 && dtype != FA_DTYPE_BF16) return FA_ERR_DTYPE;
@@ -27,10 +28,10 @@ int check_cache(const fa_paged_cache* c, int dtype, bool writes, fa::PagedCache*
   if (!is_8bit(c->dtype) && c->dtype != dtype) return FA_ERR_DTYPE;
   if (c->page_size <= 0 || c->page_size % 16 != 0) return FA_ERR_PAGE_SIZE;
   if (c->num_pages < 0 || c->max_pages < 0 || c->kv_heads <= 0) return FA_ERR_INVALID_ARG;
-  const bool scales = c->k_scale != nullptr && c->v_scale != nullptr;
+  const bool scales = c->k_scale != nullptr && (c->v_scale != nullptr || !values);
   if (is_8bit(c->dtype) ? !scales : (c->k_scale != nullptr || c->v_scale != nullptr))
     return FA_ERR_SCALES;
-  if (!c->k || !c->v || !c->block_table) return FA_ERR_INVALID_ARG;
+  if (!c->k || (values && !c->v) || !c->block_table) return FA_ERR_INVALID_ARG;
   const int es = is_8bit(c->dtype) ? 1 : 2;
   if (!aligned16(c->k) || !aligned16(c->v) || (c->page_stride * es) % 16 != 0 ||
       (c->head_stride * es) % 16 != 0 || (c->row_stride * es) % 16 != 0 ||
@@ -299,6 +300,137 @@ bool query_map(const fa_paged_cache& c, int tq, const void* q, long long q_token
   return fa::host_tensor_map(map, t);
 }
 
+// What attention calls have in common: head counts and bounds, queries, their strides.
+int check_attention(int Hq, int max_q, int max_k, float scale, int causal) {
+  if (Hq < 0 || max_q < 0 || max_k < 0) return FA_ERR_INVALID_ARG;
+  if (causal < FA_CAUSAL_NONE || causal > FA_CAUSAL_TOP_LEFT) return FA_ERR_INVALID_ARG;
+  return std::isfinite(scale) ? FA_OK : FA_ERR_INVALID_ARG;
+}
+
+// `other`: the call's result, or the other input by row, on `align` bytes.
+int check_queries(const fa::PagedCache& c, int Hq, int total, const void* Q, const void* other,
+                  long long q_token, long long q_head, unsigned align = 16) {
+  if (Hq % c.heads != 0) return FA_ERR_GQA_DIVISIBILITY;
+  if (Hq / c.heads > 128) return FA_ERR_GROUP;
+  if (total > 0 && (!Q || !other)) return FA_ERR_INVALID_ARG;
+  if (!aligned16(Q) || (reinterpret_cast<uintptr_t>(other) & (align - 1)) || ((q_token | q_head) & 7))
+    return FA_ERR_ALIGNMENT;
+  return FA_OK;
+}
+
+int check_query_strides(int Hq, int total, long long q_token, long long q_head) {
+  return (total > 1 && q_token <= 0) || (Hq > 1 && q_head <= 0) ? FA_ERR_STRIDE : FA_OK;
+}
+
+// Summed weights: fp32 rows of at least `need` positions that do not overlap.
+int check_sums(const float* w, long long seq, long long head, int len, int need, int B, int heads) {
+  if (len < need || len < 0 || (B > 0 && len > 0 && !w)) return FA_ERR_INVALID_ARG;
+  if (reinterpret_cast<uintptr_t>(w) & 3u) return FA_ERR_ALIGNMENT;
+  if ((B > 1 && seq < len) || (heads > 1 && head < len)) return FA_ERR_STRIDE;
+  return FA_OK;
+}
+
+void set_queries(fa::PagedAttn* a, const fa_paged_cache* cache, const void* Q, long long q_token, long long q_head,
+                 int Hq, int max_q, int max_k, float scale, int causal) {
+  a->q = static_cast<const uint8_t*>(Q);
+  a->q_token = 2 * q_token;
+  a->q_head = 2 * q_head;
+  a->o = nullptr;
+  a->lse = nullptr;
+  a->Hq = Hq;
+  a->group = Hq / cache->kv_heads;
+  a->max_q = max_q;
+  a->max_k = max_k;
+  a->causal = causal;
+  a->scale_log2 = scale * 1.4426950408889634f;
+  a->part = fa::kPartNone;
+  a->part_o = a->part_lse = nullptr;
+}
+
+PagedPlan plan_of(const fa::PagedAttn& a, const fa_paged_cache& c) {
+  return make_paged_plan(a.r.B, a.c.heads, a.group, c.head_dim, c.dtype, a.r.total, a.max_q, a.max_k);
+}
+
+int check_grid(const PagedPlan& k, const fa::PagedAttn& a) {
+  const long long grid = static_cast<long long>(k.slots) * a.c.heads;  // of all heads
+  return grid > 0x7fffffffLL || static_cast<long long>(a.r.B) * a.c.heads > 0x7fffffffLL ||
+                 static_cast<long long>(a.r.total) * a.Hq > (1LL << 33)
+             ? FA_ERR_TOO_LARGE
+             : FA_OK;
+}
+
+// Sizes whose plan can be made (what the calls refuse has none).
+bool sizes_ok(const fa_paged_cache* c, int B, int Hq, int total, int max_q, int max_k) {
+  if (!c || c->kv_heads <= 0 || Hq <= 0 || total <= 0) return false;
+  const int group = Hq / c->kv_heads;
+  return group * c->kv_heads == Hq && group <= 128 && B >= 0 && max_q >= 0 && max_k >= 0 &&
+         (c->head_dim == 64 || c->head_dim == 128) && c->dtype >= FA_DTYPE_F16 && c->dtype <= FA_DTYPE_E4M3 &&
+         c->kv_heads <= kMaxHeads && B <= kMaxBatch && total <= kMaxRows;
+}
+
+// fp32 results of a first pass: O and LSE.
+size_t part_bytes(int total, int Hq, int head_dim) {
+  return (static_cast<size_t>(total) * Hq * (head_dim + 1) * sizeof(float) + 127) / 128 * 128;
+}
+
+// The kernels of one pass.
+int run_paged(const fa::PagedAttn& a, const fa_paged_cache& cache, const PagedPlan& k, const void* Q,
+              long long q_token_stride, long long q_head_stride, int dtype, void* workspace, void* stream) {
+  const bool eight = is_8bit(cache.dtype);
+  const bool bf16 = dtype == FA_DTYPE_BF16;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (k.decode) {
+    fa::DecodeParams p;
+    p.a = a;
+    p.ws = static_cast<float*>(workspace);
+    p.max_rows = k.decode_rows;
+    p.epoch = fa::host_next_epoch();
+    p.timeout_ns = fa::host_timeout_ns();
+    if (!page_maps(cache, 16, &p)) return FA_ERR_TENSOR_MAP;
+    if (fa::launch_paged_decode(p, cache.head_dim, cache.dtype, bf16, fa::host_sm_count(), st) !=
+        cudaSuccess)
+      return FA_ERR_LAUNCH;
+  }
+  if (k.chunk) {
+    fa::ChunkParams p;
+    p.a = a;
+    p.tq = k.tq;
+    p.box_rows = eight ? 128 : gcd_128(cache.page_size);
+    p.stale = eight ? 0 : 1;
+    p.page_step = p.head_step = 0;
+    p.skip_rows = k.decode ? k.decode_rows : 0;
+    p.runs = k.runs ? 1 : 0;
+    char* ws = static_cast<char*>(workspace);
+    p.ws_o = reinterpret_cast<float*>(ws);
+    p.ws_lse = reinterpret_cast<float*>(ws + k.ws_o);
+    p.ws_cuts = reinterpret_cast<fa::PagedCut*>(ws + k.ws_o + k.ws_lse);
+    ws += k.ws_o + k.ws_lse + k.ws_cuts;
+    p.exp_rows = k.exp_rows;
+    p.exp_k = reinterpret_cast<uint16_t*>(ws);
+    p.exp_v = reinterpret_cast<uint16_t*>(ws + k.exp_heads * k.exp_row_bytes);
+    ws += 2 * k.exp_heads * k.exp_row_bytes;
+    p.exp_ks = reinterpret_cast<float*>(ws);
+    p.exp_vs = reinterpret_cast<float*>(ws + k.exp_heads * k.exp_scale_bytes);
+    p.exp_vl = reinterpret_cast<float*>(ws + 2 * k.exp_heads * k.exp_scale_bytes);
+    p.exp_vm = reinterpret_cast<float*>(ws + 3 * k.exp_heads * k.exp_scale_bytes);
+    p.timeout_ns = fa::host_timeout_ns();
+    const bool maps =
+        (eight ? rows_maps(p, cache.head_dim, k.exp_heads) : chunk_maps(cache, &p)) &&
+        query_map(cache, p.tq, Q, q_token_stride, q_head_stride, a.Hq, a.r.total, bf16, &p.tm_q);
+    if (!maps) return FA_ERR_TENSOR_MAP;
+    for (p.head0 = 0; p.head0 < a.c.heads; p.head0 += k.exp_heads) {
+      p.n_heads = a.c.heads - p.head0 < k.exp_heads ? a.c.heads - p.head0 : k.exp_heads;
+      p.fill = !k.decode && p.head0 == 0 ? 1 : 0;
+      p.epoch = fa::host_next_epoch();
+      p.n_ctas = k.runs ? k.n_ctas : k.slots * p.n_heads;
+      if (fa::launch_paged_chunk(p, cache.head_dim, cache.dtype, bf16, fa::host_sm_count(), st) !=
+          cudaSuccess)
+        return FA_ERR_LAUNCH;
+    }
+  }
+  return FA_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -348,14 +480,8 @@ int fa_kvcache_read(const fa_paged_cache* cache, void* K, void* V, const int* cu
 
 size_t fa_fwd_paged_workspace_bytes(const fa_paged_cache* cache, int B, int Hq, int total_q,
                                     int max_seqlen_q, int max_seqlen_k) {
-  if (!cache || cache->kv_heads <= 0 || Hq <= 0 || total_q <= 0) return 0;
-  const int group = Hq / cache->kv_heads;
-  // what the call refuses
-  if (group * cache->kv_heads != Hq || group > 128 || B < 0 || max_seqlen_q < 0 || max_seqlen_k < 0 ||
-      (cache->head_dim != 64 && cache->head_dim != 128) || cache->dtype < FA_DTYPE_F16 ||
-      cache->dtype > FA_DTYPE_E4M3 || cache->kv_heads > kMaxHeads || B > kMaxBatch || total_q > kMaxRows)
-    return 0;
-  return make_paged_plan(B, cache->kv_heads, group, cache->head_dim, cache->dtype, total_q,
+  if (!sizes_ok(cache, B, Hq, total_q, max_seqlen_q, max_seqlen_k)) return 0;
+  return make_paged_plan(B, cache->kv_heads, Hq / cache->kv_heads, cache->head_dim, cache->dtype, total_q,
                          max_seqlen_q, max_seqlen_k)
       .ws_bytes;
 }
@@ -368,90 +494,147 @@ int fa_fwd_paged(const fa_paged_cache* cache, const void* Q, long long q_token_s
   fa::PagedAttn a;
   if (int rc = check_cache(cache, dtype, false, &a.c)) return rc;
   if (int rc = check_rows(cu_seqlens_q, seqlens_k, B, total_q, &a.r)) return rc;
-  if (Hq < 0 || max_seqlen_q < 0 || max_seqlen_k < 0) return FA_ERR_INVALID_ARG;
-  if (causal < FA_CAUSAL_NONE || causal > FA_CAUSAL_TOP_LEFT) return FA_ERR_INVALID_ARG;
-  if (!std::isfinite(scale)) return FA_ERR_INVALID_ARG;
+  if (int rc = check_attention(Hq, max_seqlen_q, max_seqlen_k, scale, causal)) return rc;
   if (Hq == 0 || total_q == 0) return FA_OK;
-  if (Hq % a.c.heads != 0) return FA_ERR_GQA_DIVISIBILITY;
-  if (Hq / a.c.heads > 128) return FA_ERR_GROUP;
-  if (!Q || !O) return FA_ERR_INVALID_ARG;
-  if (!aligned16(Q) || !aligned16(O) || !aligned16(workspace) ||
-      ((q_token_stride | q_head_stride) & 7) || (reinterpret_cast<uintptr_t>(lse) & 3u))
-    return FA_ERR_ALIGNMENT;
-  if ((total_q > 1 && q_token_stride <= 0) || (Hq > 1 && q_head_stride <= 0)) return FA_ERR_STRIDE;
-  const int group = Hq / a.c.heads;
-  const bool eight = is_8bit(cache->dtype);
-  const PagedPlan k = make_paged_plan(B, a.c.heads, group, cache->head_dim, cache->dtype, total_q, max_seqlen_q,
-                                      max_seqlen_k);
-  if (k.ws_bytes > 0 && (!workspace || workspace_bytes < k.ws_bytes)) return FA_ERR_INVALID_ARG;
-  const long long grid = static_cast<long long>(k.slots) * a.c.heads;  // of all heads
-  if (grid > 0x7fffffffLL || static_cast<long long>(B) * a.c.heads > 0x7fffffffLL ||
-      static_cast<long long>(total_q) * Hq > (1LL << 33))
-    return FA_ERR_TOO_LARGE;
-  if (int rc = fa::host_check_device()) return rc;
-  a.q = static_cast<const uint8_t*>(Q);
-  a.q_token = 2 * q_token_stride;
-  a.q_head = 2 * q_head_stride;
+  if (int rc = check_queries(a.c, Hq, total_q, Q, O, q_token_stride, q_head_stride)) return rc;
+  if (!aligned16(workspace) || (reinterpret_cast<uintptr_t>(lse) & 3u)) return FA_ERR_ALIGNMENT;
+  if (int rc = check_query_strides(Hq, total_q, q_token_stride, q_head_stride)) return rc;
+  set_queries(&a, cache, Q, q_token_stride, q_head_stride, Hq, max_seqlen_q, max_seqlen_k, scale, causal);
   a.o = O;
   a.lse = lse;
-  a.Hq = Hq;
-  a.group = group;
-  a.max_q = max_seqlen_q;
-  a.max_k = max_seqlen_k;
-  a.causal = causal;
-  a.scale_log2 = scale * 1.4426950408889634f;
-  const bool bf16 = dtype == FA_DTYPE_BF16;
-  const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (k.decode) {
-    fa::DecodeParams p;
-    p.a = a;
-    p.ws = static_cast<float*>(workspace);
-    p.max_rows = k.decode_rows;
-    p.epoch = fa::host_next_epoch();
-    p.timeout_ns = fa::host_timeout_ns();
-    if (!page_maps(*cache, 16, &p)) return FA_ERR_TENSOR_MAP;
-    if (fa::launch_paged_decode(p, cache->head_dim, cache->dtype, bf16, fa::host_sm_count(), st) !=
-        cudaSuccess)
-      return FA_ERR_LAUNCH;
-  }
-  if (k.chunk) {
-    fa::ChunkParams p;
-    p.a = a;
-    p.tq = k.tq;
-    p.box_rows = eight ? 128 : gcd_128(cache->page_size);
-    p.stale = eight ? 0 : 1;
-    p.page_step = p.head_step = 0;
-    p.skip_rows = k.decode ? k.decode_rows : 0;
-    p.runs = k.runs ? 1 : 0;
-    char* ws = static_cast<char*>(workspace);
-    p.ws_o = reinterpret_cast<float*>(ws);
-    p.ws_lse = reinterpret_cast<float*>(ws + k.ws_o);
-    p.ws_cuts = reinterpret_cast<fa::PagedCut*>(ws + k.ws_o + k.ws_lse);
-    ws += k.ws_o + k.ws_lse + k.ws_cuts;
-    p.exp_rows = k.exp_rows;
-    p.exp_k = reinterpret_cast<uint16_t*>(ws);
-    p.exp_v = reinterpret_cast<uint16_t*>(ws + k.exp_heads * k.exp_row_bytes);
-    ws += 2 * k.exp_heads * k.exp_row_bytes;
-    p.exp_ks = reinterpret_cast<float*>(ws);
-    p.exp_vs = reinterpret_cast<float*>(ws + k.exp_heads * k.exp_scale_bytes);
-    p.exp_vl = reinterpret_cast<float*>(ws + 2 * k.exp_heads * k.exp_scale_bytes);
-    p.exp_vm = reinterpret_cast<float*>(ws + 3 * k.exp_heads * k.exp_scale_bytes);
-    p.timeout_ns = fa::host_timeout_ns();
-    const bool maps =
-        (eight ? rows_maps(p, cache->head_dim, k.exp_heads) : chunk_maps(*cache, &p)) &&
-        query_map(*cache, p.tq, Q, q_token_stride, q_head_stride, Hq, total_q, bf16, &p.tm_q);
-    if (!maps) return FA_ERR_TENSOR_MAP;
-    for (p.head0 = 0; p.head0 < a.c.heads; p.head0 += k.exp_heads) {
-      p.n_heads = a.c.heads - p.head0 < k.exp_heads ? a.c.heads - p.head0 : k.exp_heads;
-      p.fill = !k.decode && p.head0 == 0 ? 1 : 0;
-      p.epoch = fa::host_next_epoch();
-      p.n_ctas = k.runs ? k.n_ctas : k.slots * p.n_heads;
-      if (fa::launch_paged_chunk(p, cache->head_dim, cache->dtype, bf16, fa::host_sm_count(), st) !=
-          cudaSuccess)
-        return FA_ERR_LAUNCH;
-    }
-  }
-  return FA_OK;
+  const PagedPlan k = plan_of(a, *cache);
+  if (k.ws_bytes > 0 && (!workspace || workspace_bytes < k.ws_bytes)) return FA_ERR_INVALID_ARG;
+  if (int rc = check_grid(k, a)) return rc;
+  if (int rc = fa::host_check_device()) return rc;
+  return run_paged(a, *cache, k, Q, q_token_stride, q_head_stride, dtype, workspace, stream);
+}
+
+size_t fa_fwd_paged_prefix_workspace_bytes(const fa_paged_cache* cache, int n_prefixes,
+                                           int max_prefix_q, int max_prefix_k, int B, int Hq,
+                                           int total_q, int max_seqlen_q, int max_seqlen_k) {
+  if (!sizes_ok(cache, B, Hq, total_q, max_seqlen_q, max_seqlen_k) ||
+      !sizes_ok(cache, n_prefixes, Hq, total_q, max_prefix_q, max_prefix_k))
+    return 0;
+  const int group = Hq / cache->kv_heads;
+  const size_t first = make_paged_plan(n_prefixes, cache->kv_heads, group, cache->head_dim, cache->dtype,
+                                       total_q, max_prefix_q, max_prefix_k).ws_bytes;
+  const size_t second = make_paged_plan(B, cache->kv_heads, group, cache->head_dim, cache->dtype, total_q,
+                                        max_seqlen_q, max_seqlen_k).ws_bytes;
+  return part_bytes(total_q, Hq, cache->head_dim) + (first > second ? first : second);
+}
+
+int fa_fwd_paged_prefix(const fa_paged_cache* cache, const int* prefix_table,
+                        long long prefix_table_stride, int prefix_max_pages, int n_prefixes,
+                        const int* cu_prefix_q, const int* prefix_lens, int max_prefix_q,
+                        int max_prefix_k, const void* Q, long long q_token_stride,
+                        long long q_head_stride, void* O, float* lse, const int* cu_seqlens_q,
+                        const int* seqlens_k, int B, int Hq, int total_q, int max_seqlen_q,
+                        int max_seqlen_k, float scale, int causal, int dtype, void* workspace,
+                        size_t workspace_bytes, void* stream) {
+  fa::PagedAttn a, first;
+  if (int rc = check_cache(cache, dtype, false, &a.c)) return rc;
+  fa_paged_cache of_prefixes = *cache;
+  of_prefixes.block_table = prefix_table;
+  of_prefixes.table_stride = prefix_table_stride;
+  of_prefixes.max_pages = prefix_max_pages;
+  if (int rc = check_cache(&of_prefixes, dtype, false, &first.c)) return rc;
+  if (int rc = check_rows(cu_seqlens_q, seqlens_k, B, total_q, &a.r)) return rc;
+  if (int rc = check_rows(cu_prefix_q, prefix_lens, n_prefixes, total_q, &first.r)) return rc;
+  if (int rc = check_attention(Hq, max_seqlen_q, max_seqlen_k, scale, causal)) return rc;
+  if (int rc = check_attention(Hq, max_prefix_q, max_prefix_k, scale, FA_CAUSAL_NONE)) return rc;
+  if (Hq == 0 || total_q == 0) return FA_OK;
+  if (int rc = check_queries(a.c, Hq, total_q, Q, O, q_token_stride, q_head_stride)) return rc;
+  if (!aligned16(workspace) || (reinterpret_cast<uintptr_t>(lse) & 3u)) return FA_ERR_ALIGNMENT;
+  if (int rc = check_query_strides(Hq, total_q, q_token_stride, q_head_stride)) return rc;
+  set_queries(&a, cache, Q, q_token_stride, q_head_stride, Hq, max_seqlen_q, max_seqlen_k, scale, causal);
+  set_queries(&first, cache, Q, q_token_stride, q_head_stride, Hq, max_prefix_q, max_prefix_k, scale,
+              FA_CAUSAL_NONE);
+  a.o = O;
+  a.lse = lse;
+  const PagedPlan k1 = plan_of(first, of_prefixes), k2 = plan_of(a, *cache);
+  const size_t part = part_bytes(total_q, Hq, cache->head_dim);
+  const size_t need = part + (k1.ws_bytes > k2.ws_bytes ? k1.ws_bytes : k2.ws_bytes);
+  if (!workspace || workspace_bytes < need) return FA_ERR_INVALID_ARG;
+  if (int rc = check_grid(k1, first)) return rc;
+  if (int rc = check_grid(k2, a)) return rc;
+  if (int rc = fa::host_check_device()) return rc;
+  char* const ws = static_cast<char*>(workspace) + part;  // of either pass, one after the other
+  a.part_o = static_cast<float*>(workspace);
+  a.part_lse = a.part_o + static_cast<size_t>(total_q) * Hq * cache->head_dim;
+  a.part = fa::kPartSecond;
+  first.part_o = a.part_o;
+  first.part_lse = a.part_lse;
+  first.part = fa::kPartFirst;
+  if (int rc = run_paged(first, of_prefixes, k1, Q, q_token_stride, q_head_stride, dtype, ws, stream)) return rc;
+  return run_paged(a, *cache, k2, Q, q_token_stride, q_head_stride, dtype, ws, stream);
+}
+
+int fa_kvcache_weights(const fa_paged_cache* cache, const void* Q, long long q_token_stride,
+                       long long q_head_stride, const float* lse, const int* cu_seqlens_q,
+                       const int* seqlens_k, int B, int Hq, int total_q, int max_seqlen_q,
+                       int max_seqlen_k, float* weights, long long w_seq_stride,
+                       long long w_head_stride, int weights_len, int mode, float scale, int causal,
+                       int dtype, void* stream) {
+  fa::PagedWeights p;
+  if (int rc = check_cache(cache, dtype, false, &p.a.c, /*values=*/false)) return rc;
+  if (int rc = check_rows(cu_seqlens_q, seqlens_k, B, total_q, &p.a.r)) return rc;
+  // (a sequence without new tokens has sums too)
+  if (B > 0 && (!cu_seqlens_q || !seqlens_k)) return FA_ERR_INVALID_ARG;
+  if (int rc = check_attention(Hq, max_seqlen_q, max_seqlen_k, scale, causal)) return rc;
+  if (mode < FA_WEIGHTS_SET || mode > FA_WEIGHTS_APPEND) return FA_ERR_INVALID_ARG;
+  const long long held = static_cast<long long>(cache->max_pages) * cache->page_size;
+  const int keys = static_cast<int>(max_seqlen_k < held ? max_seqlen_k : held);
+  if (int rc = check_sums(weights, w_seq_stride, w_head_stride, weights_len, keys, B, p.a.c.heads)) return rc;
+  if (B == 0 || keys == 0 || Hq == 0) return FA_OK;
+  if (int rc = check_queries(p.a.c, Hq, total_q, Q, lse, q_token_stride, q_head_stride, 4)) return rc;
+  if (int rc = check_query_strides(Hq, total_q, q_token_stride, q_head_stride)) return rc;
+  if (static_cast<long long>(B) * p.a.c.heads > 0x7fffffffLL || static_cast<long long>(total_q) * Hq > (1LL << 33))
+    return FA_ERR_TOO_LARGE;
+  if (int rc = fa::host_check_device()) return rc;
+  set_queries(&p.a, cache, Q, q_token_stride, q_head_stride, Hq, max_seqlen_q, keys, scale, causal);
+  p.a.o = nullptr;
+  p.a.lse = const_cast<float*>(lse);
+  p.w = weights;
+  p.w_seq = w_seq_stride;
+  p.w_head = w_head_stride;
+  p.mode = mode;
+  const cudaError_t e = fa::launch_paged_weights(p, cache->head_dim, cache->dtype, dtype == FA_DTYPE_BF16,
+                                                 fa::host_sm_count(), static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
+}
+
+int fa_kvcache_evict(const fa_paged_cache* cache, float* weights, long long w_seq_stride,
+                     long long w_head_stride, int weights_len, const int* seqlens_k,
+                     const int* keep, int keep_all, int first, int recent, int* new_lens, int B,
+                     void* stream) {
+  fa::PagedEvict p;
+  if (!cache) return FA_ERR_INVALID_ARG;
+  const bool eight = is_8bit(cache->dtype);
+  if (int rc = check_cache(cache, eight ? FA_DTYPE_F16 : cache->dtype, true, &p.c)) return rc;
+  if (B < 0 || first < 0 || recent < 0) return FA_ERR_INVALID_ARG;
+  if (B > kMaxBatch || static_cast<long long>(B) * p.c.heads > 0x7fffffffLL) return FA_ERR_TOO_LARGE;
+  if (B == 0) return FA_OK;
+  if (!seqlens_k || !new_lens || new_lens == seqlens_k || new_lens == keep) return FA_ERR_INVALID_ARG;
+  if (((reinterpret_cast<uintptr_t>(seqlens_k) | reinterpret_cast<uintptr_t>(keep) |
+        reinterpret_cast<uintptr_t>(new_lens)) & 3u) != 0)
+    return FA_ERR_ALIGNMENT;
+  if (int rc = check_sums(weights, w_seq_stride, w_head_stride, weights_len, p.c.max_pages * p.c.page_size, B,
+                          p.c.heads))
+    return rc;
+  if (int rc = fa::host_check_device()) return rc;
+  p.w = weights;
+  p.w_seq = w_seq_stride;
+  p.w_head = w_head_stride;
+  p.lens = seqlens_k;
+  p.keep = keep;
+  p.keep_all = keep_all;
+  p.first = first;
+  p.recent = recent;
+  p.new_lens = new_lens;
+  p.B = B;
+  const cudaError_t e = fa::launch_paged_evict(p, cache->head_dim * (eight ? 1 : 2), eight, fa::host_sm_count(),
+                                               static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
 
 }  // extern "C"

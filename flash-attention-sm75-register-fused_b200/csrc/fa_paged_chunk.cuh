@@ -856,10 +856,31 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
       const long long row_id = static_cast<long long>(it.s.c0 + tok) * a.Hq + hq;
       const bool partial = it.slot >= 0;
       const long long ws_row = (static_cast<long long>(it.slot) * 2 + g) * kBlockM + r;
-      float* lse_dst = partial ? p.ws_lse + ws_row
-                       : a.lse ? a.lse + static_cast<long long>(hq) * a.r.total + it.s.c0 + tok
-                               : nullptr;
+      float* lse_dst = partial                  ? p.ws_lse + ws_row
+                       : a.part == kPartFirst ? a.part_lse + row_id
+                       : a.lse                ? a.lse + static_cast<long long>(hq) * a.r.total + it.s.c0 + tok
+                                              : nullptr;
+      // of two passes: where the first one's row goes, or is
+      float4* const first_o =
+          !partial && a.part != kPartNone ? reinterpret_cast<float4*>(a.part_o + row_id * D) : nullptr;
       if (n_tiles == 0) {
+        if (first_o != nullptr) {
+          if (row_ok) {
+            const float lse_first = a.part == kPartSecond ? __ldcg(a.part_lse + row_id) : -INFINITY;
+#pragma unroll 1
+            for (int i = 0; i < D / 4; ++i) {
+              if (a.part == kPartFirst) {
+                first_o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+              } else {
+                const float4 f = __ldcg(first_o + i);  // (zeros without any key)
+                reinterpret_cast<uint2*>(static_cast<T*>(a.o) + row_id * D)[i] =
+                    make_uint2(pack2<QBF16>(f.x, f.y), pack2<QBF16>(f.z, f.w));
+              }
+            }
+            if (lse_dst) *lse_dst = lse_first;
+          }
+          continue;
+        }
         if (row_ok && !partial) {
           uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.o) + row_id * D);
 #pragma unroll
@@ -875,6 +896,38 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
           const float m_use = (m == -INFINITY) ? 0.f : m;
           const float lse_row =
               l == 0.f ? -INFINITY : (m_use + __log2f(l)) * 0.69314718055994530942f;
+          if (first_o != nullptr) {
+            const Joined jn = a.part == kPartFirst || !row_ok
+                                  ? Joined{1.f, 0.f, lse_row}
+                                  : join_passes(__ldcg(a.part_lse + row_id), lse_row);
+            const float f_own = jn.own == 0.f ? 0.f : inv_l * jn.own;
+#pragma unroll 1
+            for (int c = 0; c < D / 16; ++c) {
+              uint32_t o[16];
+              ptx::tmem_ld16(tO + c * 16, o);
+              ptx::tmem_wait_ld();
+              pin_after_wait<16>(o);
+#pragma unroll
+              for (int i = 0; row_ok && i < 4; ++i) {
+                float4 x = make_float4(__uint_as_float(o[4 * i]) * f_own, __uint_as_float(o[4 * i + 1]) * f_own,
+                                       __uint_as_float(o[4 * i + 2]) * f_own, __uint_as_float(o[4 * i + 3]) * f_own);
+                if (jn.own == 0.f) x = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (a.part == kPartFirst) {
+                  first_o[4 * c + i] = x;
+                } else {
+                  if (jn.first != 0.f) {
+                    const float4 f = __ldcg(first_o + 4 * c + i);
+                    x = make_float4(fmaf(f.x, jn.first, x.x), fmaf(f.y, jn.first, x.y), fmaf(f.z, jn.first, x.z),
+                                    fmaf(f.w, jn.first, x.w));
+                  }
+                  reinterpret_cast<uint2*>(static_cast<T*>(a.o) + row_id * D)[4 * c + i] =
+                      make_uint2(pack2<QBF16>(x.x, x.y), pack2<QBF16>(x.z, x.w));
+                }
+              }
+            }
+            if (row_ok && lse_dst) *lse_dst = jn.lse;
+            continue;
+          }
 #pragma unroll
           for (int c = 0; c < D / 32; ++c) {
             uint32_t o[32];
@@ -964,6 +1017,33 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
   const int hq = c.h * a.group + r % a.group;
   const long long out = static_cast<long long>(c.c0 + tok) * a.Hq + hq;
   uint32_t w[8];
+  if (a.part != kPartNone) {
+    const float lse = sum == 0.f ? -INFINITY : mx + logf(sum);
+    float4* const first_o = reinterpret_cast<float4*>(a.part_o + out * D + col);
+    if (a.part == kPartFirst) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        first_o[e] = make_float4(acc[4 * e] * inv, acc[4 * e + 1] * inv, acc[4 * e + 2] * inv, acc[4 * e + 3] * inv);
+      if (col == 0) a.part_lse[out] = lse;
+      return;
+    }
+    const Joined jn = join_passes(__ldcg(a.part_lse + out), lse);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float4 f = __ldcg(first_o + e);
+      const float y[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        acc[4 * e + x] = (jn.own == 0.f ? 0.f : acc[4 * e + x] * inv * jn.own) + (jn.first == 0.f ? 0.f : y[x] * jn.first);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w[e] = pack2<BF16>(acc[2 * e], acc[2 * e + 1]);
+    uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.o) + out * D + col);
+    dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
+    dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+    if (col == 0 && a.lse != nullptr) a.lse[static_cast<long long>(hq) * a.r.total + c.c0 + tok] = jn.lse;
+    return;
+  }
 #pragma unroll
   for (int e = 0; e < 8; ++e) w[e] = pack2<BF16>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
   uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.o) + out * D + col);

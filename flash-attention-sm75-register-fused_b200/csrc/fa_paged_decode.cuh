@@ -200,6 +200,28 @@ struct Partial {
   __device__ __forceinline__ void write(const PagedAttn& a, int tok, int hq, float up) const {
     const int lane = threadIdx.x & 31;
     const float inv = l == 0.f ? 0.f : up / l;
+    if (a.part != kPartNone) {
+      const long long row = static_cast<long long>(tok) * a.Hq + hq;
+      const float lse = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
+      float x[E];
+      if (a.part == kPartFirst) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) a.part_o[row * D + lane * E + e] = o[e] * inv;
+        if (lane == 0) a.part_lse[row] = lse;
+        return;
+      }
+      const Joined j = join_passes(__ldcg(a.part_lse + row), lse);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float f = __ldcg(a.part_o + row * D + lane * E + e);
+        x[e] = (j.own == 0.f ? 0.f : o[e] * inv * j.own) + (j.first == 0.f ? 0.f : f * j.first);
+      }
+      uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.o) + row * D) + lane * (E / 2);
+#pragma unroll
+      for (int e = 0; e < E; e += 2) dst[e / 2] = pack2<BF16>(x[e], x[e + 1]);
+      if (lane == 0 && a.lse != nullptr) a.lse[static_cast<long long>(hq) * a.r.total + tok] = j.lse;
+      return;
+    }
     uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.o) +
                                                 (static_cast<long long>(tok) * a.Hq + hq) * D) +
                     lane * (E / 2);
@@ -756,6 +778,32 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
         if (first && last && !p.solo) {
           const int tok = s.c0 + r / a.group, hq = cc.h * a.group + r % a.group;
           const float inv = l[nt][c] == 0.f ? 0.f : kUp / l[nt][c];
+          const float lse_row =
+              l[nt][c] == 0.f ? -INFINITY : (m[nt][c] + (C::k8 ? 0.f : __log2f(l[nt][c]))) * 0.69314718055994530942f;
+          if (a.part != kPartNone) {
+            const long long row = static_cast<long long>(tok) * a.Hq + hq;
+            float* const first_o = a.part_o + row * D;
+            const Joined jn = a.part == kPartFirst ? Joined{1.f, 0.f, lse_row}
+                                                   : join_passes(__ldcg(a.part_lse + row), lse_row);
+#pragma unroll
+            for (int k = 0; k < C::kKS; ++k)
+#pragma unroll
+              for (int hh = 0; hh < 2; ++hh) {
+                const float x = jn.own == 0.f ? 0.f : o[nt][k][2 * hh + c] * inv * jn.own;
+                if (a.part == kPartFirst) {
+                  first_o[col(k, hh)] = x;
+                } else {
+                  const float y = jn.first == 0.f ? x : fmaf(__ldcg(first_o + col(k, hh)), jn.first, x);
+                  static_cast<uint16_t*>(a.o)[row * D + col(k, hh)] =
+                      static_cast<uint16_t>(pack2<QBF16>(y, 0.f) & 0xffffu);
+                }
+              }
+            if (g == 0) {
+              if (a.part == kPartFirst) a.part_lse[row] = lse_row;
+              else if (a.lse != nullptr) a.lse[static_cast<long long>(hq) * a.r.total + tok] = jn.lse;
+            }
+            continue;
+          }
           uint16_t* dst = static_cast<uint16_t*>(a.o) + (static_cast<long long>(tok) * a.Hq + hq) * D;
 #pragma unroll
           for (int k = 0; k < C::kKS; ++k) {
@@ -767,9 +815,7 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
               dst[col(k, 1)] = static_cast<uint16_t>(w >> 16);
             }
           }
-          if (g == 0 && a.lse != nullptr)
-            a.lse[static_cast<long long>(hq) * a.r.total + tok] =
-                l[nt][c] == 0.f ? -INFINITY : (m[nt][c] + (C::k8 ? 0.f : __log2f(l[nt][c]))) * 0.69314718055994530942f;
+          if (g == 0 && a.lse != nullptr) a.lse[static_cast<long long>(hq) * a.r.total + tok] = lse_row;
         } else {
           // slot 0: continues the head of an earlier team; slot 1: begins one
 #pragma unroll

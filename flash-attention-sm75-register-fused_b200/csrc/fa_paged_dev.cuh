@@ -64,10 +64,29 @@ __device__ __forceinline__ Seq load_seq(const PagedAttn& a, int b) {
   return s;
 }
 
+// Result of a row of the second pass with that of the first: O = own O_2 + first
+// O_1, LSE.  (Without keys in a set its weight is 0; without any, all are.)
+struct Joined {
+  float own, first, lse;
+};
+__device__ __forceinline__ Joined join_passes(float lse_first, float lse_own) {
+  const float m = fmaxf(lse_first, lse_own);
+  if (m == -INFINITY) return {0.f, 0.f, -INFINITY};
+  const float f1 = expf(lse_first - m), f2 = expf(lse_own - m);
+  const float sum = f1 + f2;
+  return {f2 / sum, f1 / sum, m + logf(sum)};
+}
+
 // O = 0, LSE = -inf in packed row t, which no kernel computes.  (Also below: all
 // threads of a block call it.)
 __device__ __forceinline__ void fill_row(const PagedAttn& a, int d, int t) {
-  const int n = static_cast<int>(blockDim.x), words = a.Hq * d / 2;
+  const int n = static_cast<int>(blockDim.x);
+  if (a.part == kPartFirst) {
+    for (int i = threadIdx.x; i < a.Hq * d; i += n) a.part_o[static_cast<long long>(t) * a.Hq * d + i] = 0.f;
+    for (int i = threadIdx.x; i < a.Hq; i += n) a.part_lse[static_cast<long long>(t) * a.Hq + i] = -INFINITY;
+    return;
+  }
+  const int words = a.Hq * d / 2;
   for (int i = threadIdx.x; i < words; i += n)
     static_cast<uint32_t*>(a.o)[static_cast<long long>(t) * words + i] = 0u;
   if (a.lse != nullptr)

@@ -7,7 +7,7 @@
 // Additions: native GQA (K/V may have fewer heads than Q), bf16 inputs,
 // flash_attention_forward_lse returning (O, LSE), flash_attention_forward_kvcache
 // (Nq != Nk: decode and chunked prefill), the paged KV cache (write, read back,
-// attention), and diagnostics.
+// attention, also behind shared prefixes, summed weights, eviction), and diagnostics.
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -468,6 +468,7 @@ int64_t stride_of(const torch::Tensor& t, int64_t dim) {
 // any strides with d contiguous, block_table int32 [B, max_pages], scales fp32
 // [num_pages, Hkv, page_size] for 8-bit pages.  `like` (new tokens or results)
 // fixes the device and, for 16-bit pages, the type.
+// (The keys alone: v = k, vs = ks.)
 fa_paged_cache paged_cache(const torch::Tensor& k, const torch::Tensor& v,
                            const torch::Tensor& table, const c10::optional<torch::Tensor>& ks,
                            const c10::optional<torch::Tensor>& vs, const torch::Device& device,
@@ -558,15 +559,16 @@ torch::Tensor as_ints(pybind11::handle h, const torch::Device& device) {
 
 // Number of sequences; checks cu_seqlens [B + 1] and seqlens_k [B] against the table.
 int paged_batch(const torch::Tensor& cu, const torch::Tensor& lens, const torch::Tensor& table,
-                const torch::Device& device) {
+                const torch::Device& device,
+                const char* agree = "block_table [B, max_pages], seqlens_k [B] and cu_seqlens [B + 1] must agree, "
+                                    "got B = ") {
   TORCH_CHECK(cu.device() == device && lens.device() == device,
               "cu_seqlens and seqlens_k must be on the inputs' device");
   TORCH_CHECK(cu.scalar_type() == torch::kInt32 && lens.scalar_type() == torch::kInt32 &&
                   cu.is_contiguous() && lens.is_contiguous() && cu.dim() == 1 && lens.dim() == 1,
               "cu_seqlens and seqlens_k must be contiguous 1-D int32 tensors");
   TORCH_CHECK(lens.size(0) == table.size(0) && cu.size(0) == table.size(0) + 1,
-              "block_table [B, max_pages], seqlens_k [B] and cu_seqlens [B + 1] must agree, got B = ",
-              table.size(0), ", ", lens.size(0), ", ", cu.size(0) - 1);
+              agree, table.size(0), ", ", lens.size(0), ", ", cu.size(0) - 1);
   return static_cast<int>(table.size(0));
 }
 
@@ -691,6 +693,150 @@ pybind11::object flash_attention_forward_paged(
   return result();
 }
 
+// O [total_q, Hq, d], or with want_lse (O, LSE fp32 [Hq, total_q]).
+pybind11::object flash_attention_forward_paged_prefix(
+    const torch::Tensor& q_in, const torch::Tensor& k_cache, const torch::Tensor& v_cache,
+    pybind11::handle prefix_table_in, pybind11::handle cu_prefix_in, pybind11::handle prefix_lens_in,
+    pybind11::handle table_in, pybind11::handle cu_in, pybind11::handle lens_in, int64_t max_prefix_q,
+    int64_t max_prefix_k, int64_t max_seqlen_q, int64_t max_seqlen_k, int64_t causal,
+    c10::optional<double> scale_in, bool want_lse, const c10::optional<torch::Tensor>& ks,
+    const c10::optional<torch::Tensor>& vs) {
+  check_new_rows(q_in, "q");
+  const auto prefix_table = as_ints(prefix_table_in, q_in.device());
+  const auto cu_prefix = as_ints(cu_prefix_in, q_in.device());
+  const auto prefix_lens = as_ints(prefix_lens_in, q_in.device());
+  const auto table = as_ints(table_in, q_in.device());
+  const auto cu = as_ints(cu_in, q_in.device()), lens = as_ints(lens_in, q_in.device());
+  const float scale = static_cast<float>(
+      scale_in.has_value() ? *scale_in : 1.0 / std::sqrt(static_cast<double>(q_in.size(2))));
+  const auto cp = paged_cache(k_cache, v_cache, prefix_table, ks, vs, q_in.device(), q_in.scalar_type());
+  const auto c = paged_cache(k_cache, v_cache, table, ks, vs, q_in.device(), q_in.scalar_type());
+  TORCH_CHECK(q_in.size(2) == c.head_dim, "head_dim mismatch");
+  TORCH_CHECK(c.kv_heads > 0 && q_in.size(1) % c.kv_heads == 0, "GQA: Q heads (", q_in.size(1),
+              ") not divisible by K/V heads (", c.kv_heads, ")");
+  const int P = paged_batch(cu_prefix, prefix_lens, prefix_table, q_in.device(), "prefix_table [P, max_pages], "
+                            "prefix_lens [P] and cu_prefix_q [P + 1] must agree, got P = ");
+  const int B = paged_batch(cu, lens, table, q_in.device());
+  for (const int64_t x : {max_prefix_q, max_prefix_k, max_seqlen_q, max_seqlen_k})
+    TORCH_CHECK(x >= 0 && x <= INT32_MAX,
+                "max_prefix_q, max_prefix_k, max_seqlen_q and max_seqlen_k must be lengths");
+  const c10::cuda::CUDAGuard guard(q_in.device());
+  const auto q = readable_rows(q_in, /*mapped=*/true);
+  const int Hq = static_cast<int>(q.size(1)), total = static_cast<int>(q.size(0));
+  auto O = new_result(q.sizes(), q.scalar_type(), q.device());
+  torch::Tensor lse;
+  if (want_lse) lse = new_result({Hq, total}, torch::kFloat32, q.device());
+  auto result = [&]() -> pybind11::object {
+    if (!want_lse) return pybind11::cast(O);
+    return pybind11::make_tuple(O, lse);
+  };
+  if (q.numel() == 0) return result();
+  // bounds that are looser than the tables are cut to what these hold
+  const int mpq = static_cast<int>(max_prefix_q), mq = static_cast<int>(max_seqlen_q);
+  const int mpk = static_cast<int>(std::min(max_prefix_k, static_cast<int64_t>(cp.max_pages) * c.page_size));
+  const int mk = static_cast<int>(std::min(max_seqlen_k, static_cast<int64_t>(c.max_pages) * c.page_size));
+  const size_t ws_bytes = fa_fwd_paged_prefix_workspace_bytes(&c, P, mpq, mpk, B, Hq, total, mq, mk);
+  const auto ws = new_result({static_cast<int64_t>(ws_bytes)}, torch::kUInt8, q.device());
+  const int rc = fa_fwd_paged_prefix(
+      &c, cp.block_table, cp.table_stride, cp.max_pages, P, cu_prefix.data_ptr<int>(),
+      P > 0 ? prefix_lens.data_ptr<int>() : nullptr, mpq, mpk, q.data_ptr(), stride_of(q, 0), stride_of(q, 1),
+      O.data_ptr(), want_lse ? lse.data_ptr<float>() : nullptr, cu.data_ptr<int>(),
+      B > 0 ? lens.data_ptr<int>() : nullptr, B, Hq, total, mq, mk, scale, static_cast<int>(causal),
+      q.scalar_type() == torch::kBFloat16 ? FA_DTYPE_BF16 : FA_DTYPE_F16, ws.data_ptr(), ws_bytes, stream_of(q));
+  TORCH_CHECK(rc == FA_OK, "flash_attention_forward_paged_prefix: ", fa_error_string(rc));
+  return result();
+}
+
+// Summed weights [B, Hkv, L] fp32 whose rows do not overlap, for B sequences and the cache's heads.
+void check_weights(const torch::Tensor& w, int B, const fa_paged_cache& c, const torch::Device& device) {
+  TORCH_CHECK(w.device() == device && w.scalar_type() == torch::kFloat32,
+              "weights must be fp32 on the pages' device");
+  TORCH_CHECK_VALUE(w.dim() == 3 && w.size(0) == B && w.size(1) == c.kv_heads, "weights must be [", B, ", ",
+                    c.kv_heads, ", L] for this cache");
+  TORCH_CHECK(w.size(2) <= INT32_MAX, "size exceeds int32");
+  TORCH_CHECK((w.size(2) <= 1 || w.stride(2) == 1) && (w.size(0) <= 1 || w.stride(0) >= w.size(2)) &&
+                  (w.size(1) <= 1 || w.stride(1) >= w.size(2)),
+              "the rows of weights must be contiguous and must not overlap");
+}
+
+void kvcache_weights_paged(const torch::Tensor& q_in, const torch::Tensor& lse_in, const torch::Tensor& k_cache,
+                           pybind11::handle table_in, pybind11::handle cu_in, pybind11::handle lens_in,
+                           int64_t max_seqlen_q, int64_t max_seqlen_k, const torch::Tensor& weights, int64_t causal,
+                           c10::optional<double> scale_in, int64_t mode, const c10::optional<torch::Tensor>& ks) {
+  check_new_rows(q_in, "q");
+  const auto table = as_ints(table_in, q_in.device());
+  const auto cu = as_ints(cu_in, q_in.device()), lens = as_ints(lens_in, q_in.device());
+  const float scale = static_cast<float>(
+      scale_in.has_value() ? *scale_in : 1.0 / std::sqrt(static_cast<double>(q_in.size(2))));
+  auto c = paged_cache(k_cache, k_cache, table, ks, ks, q_in.device(), q_in.scalar_type());
+  c.v = nullptr;
+  c.v_scale = nullptr;
+  TORCH_CHECK(q_in.size(2) == c.head_dim, "head_dim mismatch");
+  TORCH_CHECK(c.kv_heads > 0 && q_in.size(1) > 0 && q_in.size(1) % c.kv_heads == 0, "GQA: Q heads (",
+              q_in.size(1), ") not divisible by K/V heads (", c.kv_heads, ")");
+  TORCH_CHECK(lse_in.device() == q_in.device() && lse_in.scalar_type() == torch::kFloat32 && lse_in.dim() == 2 &&
+                  lse_in.size(0) == q_in.size(1) && lse_in.size(1) == q_in.size(0),
+              "lse must be fp32 [H_q, total_q] on q's device");
+  const int B = paged_batch(cu, lens, table, q_in.device());
+  check_weights(weights, B, c, q_in.device());
+  TORCH_CHECK(max_seqlen_q >= 0 && max_seqlen_k >= 0 && max_seqlen_q <= INT32_MAX &&
+                  max_seqlen_k <= INT32_MAX,
+              "max_seqlen_q and max_seqlen_k must be lengths");
+  const int mk = static_cast<int>(std::min(max_seqlen_k, static_cast<int64_t>(c.max_pages) * c.page_size));
+  TORCH_CHECK_VALUE(weights.size(2) >= mk, "weights has ", weights.size(2), " positions, fewer than the ", mk,
+                    " that max_seqlen_k and the table allow");
+  if (B == 0 || mk == 0) return;
+  const c10::cuda::CUDAGuard guard(q_in.device());
+  const auto q = readable_rows(q_in, /*mapped=*/true);
+  const auto lse = lse_in.contiguous();
+  const int rc = fa_kvcache_weights(
+      &c, q.data_ptr(), stride_of(q, 0), stride_of(q, 1), lse.data_ptr<float>(), cu.data_ptr<int>(),
+      lens.data_ptr<int>(), B, static_cast<int>(q.size(1)), static_cast<int>(q.size(0)),
+      static_cast<int>(max_seqlen_q), mk, weights.data_ptr<float>(), stride_of(weights, 0), stride_of(weights, 1),
+      static_cast<int>(weights.size(2)), static_cast<int>(mode), scale, static_cast<int>(causal),
+      q.scalar_type() == torch::kBFloat16 ? FA_DTYPE_BF16 : FA_DTYPE_F16, stream_of(q));
+  TORCH_CHECK(rc == FA_OK, "kvcache_weights_paged: ", fa_error_string(rc));
+}
+
+// New lengths int32 [B].  keep: an int, or B of them.
+torch::Tensor kvcache_evict_paged(const torch::Tensor& k_cache, const torch::Tensor& v_cache,
+                                  const torch::Tensor& weights, pybind11::handle table_in, pybind11::handle lens_in,
+                                  pybind11::handle keep_in, int64_t recent, int64_t first,
+                                  const c10::optional<torch::Tensor>& ks, const c10::optional<torch::Tensor>& vs) {
+  const auto device = k_cache.device();
+  const auto table = as_ints(table_in, device), lens = as_ints(lens_in, device);
+  const auto kind = k_cache.scalar_type() == torch::kBFloat16 ? torch::kBFloat16 : torch::kFloat16;
+  const auto c = paged_cache(k_cache, v_cache, table, ks, vs, device, kind, /*writes=*/true);
+  TORCH_CHECK(lens.device() == device && lens.is_contiguous() && lens.dim() == 1 && lens.size(0) == table.size(0),
+              "seqlens_k must be [B] for block_table [B, max_pages], got B = ", table.size(0));
+  const int B = static_cast<int>(table.size(0));
+  check_weights(weights, B, c, device);
+  const int64_t held = static_cast<int64_t>(c.max_pages) * c.page_size;
+  TORCH_CHECK_VALUE(weights.size(2) >= held, "weights has ", weights.size(2), " positions, fewer than the ", held,
+                    " of the table");
+  torch::Tensor keep;
+  int64_t keep_all = 0;
+  if (pybind11::isinstance<pybind11::int_>(keep_in)) {
+    keep_all = keep_in.cast<int64_t>();
+  } else {
+    keep = as_ints(keep_in, device);
+    if (keep.dim() == 0) keep = keep.expand({B}).contiguous();
+    TORCH_CHECK(keep.is_contiguous() && keep.dim() == 1 && keep.size(0) == B,
+                "keep must be one number of positions, or one for each sequence");
+  }
+  TORCH_CHECK_VALUE(keep_all >= 0 && first >= 0 && recent >= 0, "keep, first and recent must not be negative");
+  const auto most = [](int64_t x) { return static_cast<int>(std::min<int64_t>(x, INT32_MAX)); };
+  const c10::cuda::CUDAGuard guard(device);
+  auto new_lens = new_result({B}, torch::kInt32, device);
+  if (B == 0) return new_lens;
+  const int rc = fa_kvcache_evict(
+      &c, weights.data_ptr<float>(), stride_of(weights, 0), stride_of(weights, 1),
+      static_cast<int>(weights.size(2)), lens.data_ptr<int>(), keep.defined() ? keep.data_ptr<int>() : nullptr,
+      most(keep_all), most(first), most(recent), new_lens.data_ptr<int>(), B, stream_of(k_cache));
+  TORCH_CHECK(rc == FA_OK, "kvcache_evict_paged: ", fa_error_string(rc));
+  return new_lens;
+}
+
 int device_status(bool reset) { return fa_device_status(reset ? 1 : 0); }
 
 }  // namespace
@@ -723,6 +869,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "(K, V) packed 16-bit rows of the described tokens");
   m.def("flash_attention_forward_paged", &flash_attention_forward_paged,
         "O [total_q, Hq, d], or (O, LSE [Hq, total_q]), of new tokens over a paged cache");
+  m.def("flash_attention_forward_paged_prefix", &flash_attention_forward_paged_prefix,
+        "O [total_q, Hq, d], or (O, LSE [Hq, total_q]), of new tokens over shared prefixes and their own keys");
+  m.def("kvcache_weights_paged", &kvcache_weights_paged,
+        "Attention weight of the cached keys, summed over the new tokens, into weights [B, Hkv, L]");
+  m.def("kvcache_evict_paged", &kvcache_evict_paged,
+        "Cuts the sequences of a paged cache to a budget by their summed weights; new lengths [B]");
   m.def("device_status", &device_status, pybind11::arg("reset") = false,
         "Error code recorded by the in-kernel watchdog (0 = none)");
   m.def("set_watchdog_ns", &fa_set_watchdog_ns);

@@ -8,12 +8,15 @@ Same public surface as the reference package
 ``flash_attention_forward_padded`` (padded batches with per-entry row ranges)
 ``flash_attention`` / ``flash_attention_padded`` / ``flash_attention_varlen``
 (forward + backward), and the paged KV cache (``kvcache_write_paged``,
-``kvcache_read_paged``, ``flash_attention_forward_paged``) are additions.
+``kvcache_read_paged``, ``flash_attention_forward_paged``,
+``flash_attention_forward_paged_prefix``, ``kvcache_weights_paged``,
+``kvcache_evict_paged``) are additions.
 """
 from .ops import (flash_attention, flash_attention_forward, flash_attention_forward_host,
                   flash_attention_forward_kvcache, flash_attention_forward_padded,
                   flash_attention_padded, flash_attention_varlen, flash_attention_varlen_forward)
-from .paged import (flash_attention_forward_paged, kvcache_read_paged,  # noqa: F401
+from .paged import (flash_attention_forward_paged, flash_attention_forward_paged_prefix,  # noqa: F401
+                    kvcache_evict_paged, kvcache_read_paged, kvcache_weights_paged,
                     kvcache_write_paged)
 
 __version__ = "0.1.0"

@@ -36,6 +36,16 @@ SIGNATURES = {
                              ctypes.c_size_t, c_vp]),
     "fa_fwd_paged_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(PagedCache), c_int, c_int,
                                                        c_int, c_int, c_int]),
+    "fa_fwd_paged_prefix": (c_int, [ctypes.POINTER(PagedCache), c_vp, c_ll, c_int, c_int, c_vp, c_vp,
+                                    c_int, c_int, c_vp, c_ll, c_ll, c_vp, c_vp, c_vp, c_vp, c_int,
+                                    c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_vp,
+                                    ctypes.c_size_t, c_vp]),
+    "fa_fwd_paged_prefix_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(PagedCache)] + [c_int] * 8),
+    "fa_kvcache_weights": (c_int, [ctypes.POINTER(PagedCache), c_vp, c_ll, c_ll, c_vp, c_vp, c_vp, c_int,
+                                   c_int, c_int, c_int, c_int, c_vp, c_ll, c_ll, c_int, c_int, c_float,
+                                   c_int, c_int, c_vp]),
+    "fa_kvcache_evict": (c_int, [ctypes.POINTER(PagedCache), c_vp, c_ll, c_ll, c_int, c_vp, c_vp, c_int,
+                                 c_int, c_int, c_vp, c_int, c_vp]),
     "fa_fwd": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_int, c_float,
                        c_int, c_int, c_vp]),
     "fa_fwd_kvcache": (c_int, [c_vp, c_vp, c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_int,
@@ -290,3 +300,58 @@ def fa_fwd_paged(cache, q, o, lse, cu_seqlens_q, seqlens_k, max_seqlen_q, max_se
                             int(max_seqlen_k), float(scale), int(causal),
                             1 if q.dtype == torch.bfloat16 else 0, ptr(ws), nbytes,
                             stream_ptr(stream))
+
+
+def fa_fwd_paged_prefix(cache, prefix_table, cu_prefix_q, prefix_lens, max_prefix_q, max_prefix_k, q, o,
+                        lse, cu_seqlens_q, seqlens_k, max_seqlen_q, max_seqlen_k, causal=CAUSAL_NONE,
+                        scale=None, stream=None, workspace=None):
+    """Call fa_fwd_paged_prefix on torch CUDA tensors (prefix_table int32 [P,
+    pages], the rest as fa_fwd_paged); allocates the workspace unless one is
+    given.  Returns the status."""
+    import math
+    import torch
+    T, Hq, d = q.shape
+    if scale is None:
+        scale = 1.0 / math.sqrt(d)
+    lib = load()
+    B, P = seqlens_k.numel(), prefix_lens.numel()
+    if workspace is None:
+        nbytes = lib.fa_fwd_paged_prefix_workspace_bytes(
+            ctypes.byref(cache), P, int(max_prefix_q), int(max_prefix_k), B, Hq, T, int(max_seqlen_q),
+            int(max_seqlen_k))
+        workspace = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=q.device)
+    return lib.fa_fwd_paged_prefix(
+        ctypes.byref(cache), ptr(prefix_table), prefix_table.stride(0), prefix_table.size(1), P,
+        ptr(cu_prefix_q), ptr(prefix_lens), int(max_prefix_q), int(max_prefix_k), ptr(q), q.stride(0),
+        q.stride(1), ptr(o), ptr(lse), ptr(cu_seqlens_q), ptr(seqlens_k), B, Hq, T, int(max_seqlen_q),
+        int(max_seqlen_k), float(scale), int(causal), 1 if q.dtype == torch.bfloat16 else 0,
+        ptr(workspace), workspace.numel(), stream_ptr(stream))
+
+
+WEIGHTS_SET, WEIGHTS_ADD, WEIGHTS_APPEND = 0, 1, 2
+
+
+def fa_kvcache_weights(cache, q, lse, cu_seqlens_q, seqlens_k, max_seqlen_q, max_seqlen_k, weights,
+                       mode=WEIGHTS_APPEND, causal=CAUSAL_NONE, scale=None, stream=None):
+    """Call fa_kvcache_weights on torch CUDA tensors (q [total_q, Hq, d], lse
+    [Hq, total_q], weights fp32 [B, Hkv, L]).  Returns the status."""
+    import math
+    import torch
+    T, Hq, d = q.shape
+    if scale is None:
+        scale = 1.0 / math.sqrt(d)
+    return load().fa_kvcache_weights(
+        ctypes.byref(cache), ptr(q), q.stride(0), q.stride(1), ptr(lse), ptr(cu_seqlens_q), ptr(seqlens_k),
+        seqlens_k.numel(), Hq, T, int(max_seqlen_q), int(max_seqlen_k), ptr(weights), weights.stride(0),
+        weights.stride(1), weights.size(2), int(mode), float(scale), int(causal),
+        1 if q.dtype == torch.bfloat16 else 0, stream_ptr(stream))
+
+
+def fa_kvcache_evict(cache, weights, seqlens_k, keep, new_lens, first=0, recent=0, stream=None):
+    """Call fa_kvcache_evict on torch CUDA tensors (weights fp32 [B, Hkv, L], keep
+    an int or an int32 tensor [B], new_lens int32 [B]).  Returns the status."""
+    each = not isinstance(keep, int)
+    return load().fa_kvcache_evict(
+        ctypes.byref(cache), ptr(weights), weights.stride(0), weights.stride(1), weights.size(2),
+        ptr(seqlens_k), ptr(keep if each else None), 0 if each else keep, int(first), int(recent),
+        ptr(new_lens), seqlens_k.numel(), stream_ptr(stream))

@@ -1,5 +1,6 @@
-"""Paged KV cache: writing new tokens, reading them back, and attention over it
-(no reference counterpart; the reference leaves cached decode to PyTorch SDPA,
+"""Paged KV cache: writing new tokens, reading them back, attention over it (also
+for batches behind shared prefixes), the attention weight its keys receive, and
+eviction of those that receive little (no reference counterpart; the reference leaves cached decode to PyTorch SDPA,
 llama_attention_replacement.py:63-65).
 
 A cache is a pair of tensors ``[num_pages, H_kv, page_size, D]`` for keys and
@@ -10,7 +11,7 @@ strides).  Position ``p`` of sequence ``b`` is row ``p % page_size`` of page
 ``block_table[b, p // page_size]``.  Pages (and scales) broadcast over heads can
 be read and attended over, not written.
 
-All three functions describe tokens in the same way: sequence ``b`` has the
+The functions describe tokens in the same way: sequence ``b`` has the
 packed rows ``[cu_seqlens[b], cu_seqlens[b + 1])``, and the last of them is
 position ``seqlens_k[b] - 1``.  A serving step writes its tokens' K and V, then
 attends, with one set of ``block_table``, ``cu_seqlens`` and ``seqlens_k``.
@@ -108,3 +109,106 @@ def flash_attention_forward_paged(q, k_cache, v_cache, block_table, cu_seqlens_q
     return _C.flash_attention_forward_paged(q, k_cache, v_cache, block_table, cu_seqlens_q, seqlens_k,
                                             max_seqlen_q, max_seqlen_k, mode, scale, return_lse,
                                             k_scale, v_scale)
+
+
+def flash_attention_forward_paged_prefix(q, k_cache, v_cache, prefix_table, cu_prefix_q, prefix_lens,
+                                         block_table, cu_seqlens_q, seqlens_k, max_prefix_q,
+                                         max_prefix_k, max_seqlen_q, max_seqlen_k, causal=False,
+                                         scale=None, return_lse=False,
+                                         causal_alignment="bottom_right", k_scale=None, v_scale=None):
+    """``flash_attention_forward_paged`` of a batch whose sequences share long
+    prefixes (a system prompt, a document): each prefix is computed once for all
+    the tokens behind it, instead of once per sequence; forward only.
+
+    Args:
+        q, k_cache, v_cache, k_scale, v_scale, block_table, cu_seqlens_q,
+            seqlens_k, max_seqlen_q, max_seqlen_k, causal, causal_alignment,
+            scale, return_lse: as ``flash_attention_forward_paged``; the block
+            table and the lengths are those of what follows the prefix
+        prefix_table: int32 [P, max_pages], the pages of the prefixes in the
+            same cache
+        cu_prefix_q: P + 1 row offsets (int32 tensor or ints): the tokens in
+            rows [cu_prefix_q[g], cu_prefix_q[g + 1]) see prefix g; rows
+            outside have none
+        prefix_lens: P lengths of the prefixes
+        max_prefix_q, max_prefix_k: upper bounds of a prefix's tokens and keys
+            (tokens beyond do not see it, keys beyond are not seen)
+
+    A token sees all keys of its prefix, and those of its own sequence that
+    ``causal`` leaves.  Rows that see no key, rows of no sequence and tokens
+    beyond max_seqlen_q return O = 0, LSE = -inf.
+    """
+    mode = 0
+    if causal:
+        mode = _CAUSAL_MODES.get(causal_alignment)
+        if mode is None:
+            raise ValueError(f"causal_alignment must be one of {sorted(_CAUSAL_MODES)}")
+    return _C.flash_attention_forward_paged_prefix(q, k_cache, v_cache, prefix_table, cu_prefix_q,
+                                                   prefix_lens, block_table, cu_seqlens_q, seqlens_k,
+                                                   max_prefix_q, max_prefix_k, max_seqlen_q,
+                                                   max_seqlen_k, mode, scale, return_lse, k_scale,
+                                                   v_scale)
+
+
+_WEIGHT_MODES = {"set": 0, "add": 1, "append": 2}
+
+
+def kvcache_weights_paged(q, lse, k_cache, block_table, cu_seqlens_q, seqlens_k, max_seqlen_q,
+                          max_seqlen_k, weights, causal=False, scale=None, mode="append",
+                          causal_alignment="bottom_right", k_scale=None):
+    """Attention weight that cached keys received from new tokens, summed over
+    these and over the query heads of a KV head, in place in ``weights``.
+
+    Args:
+        q: [total_q, H_q, D]  float16 / bfloat16, cuda
+        lse: fp32 [H_q, total_q], what ``flash_attention_forward_paged`` (or
+            ``..._paged_prefix``) returned for these queries
+        k_cache, k_scale, block_table, cu_seqlens_q, seqlens_k, max_seqlen_q,
+            max_seqlen_k, causal, causal_alignment, scale: as that call's (the
+            weight of prefix keys: its prefix_table, cu_prefix_q, prefix_lens,
+            max_prefix_q and max_prefix_k, with causal=False and mode="add")
+        weights: fp32 [B, H_kv, L], L at least max_seqlen_k or the positions of
+            a table row, with contiguous rows; weights[b, h, j] is the sum of
+            position j of sequence b
+        mode: "append" (added to the sums there, but the new tokens' own
+            positions, which have none yet, are set), "add" or "set" (all of a
+            sequence's positions)
+
+    Positions from a sequence's length (or max_seqlen_k) on are left as they are.
+    """
+    if mode not in _WEIGHT_MODES:
+        raise ValueError(f"mode must be one of {sorted(_WEIGHT_MODES)}, got {mode!r}")
+    rule = 0
+    if causal:
+        rule = _CAUSAL_MODES.get(causal_alignment)
+        if rule is None:
+            raise ValueError(f"causal_alignment must be one of {sorted(_CAUSAL_MODES)}")
+    _C.kvcache_weights_paged(q, lse, k_cache, block_table, cu_seqlens_q, seqlens_k, max_seqlen_q,
+                             max_seqlen_k, weights, rule, scale, _WEIGHT_MODES[mode], k_scale)
+
+
+def kvcache_evict_paged(k_cache, v_cache, weights, block_table, seqlens_k, keep, recent=0, first=0,
+                        k_scale=None, v_scale=None):
+    """Cut the sequences of a paged cache to ``keep`` positions, in place, each KV
+    head by its own weights; returns the new lengths.
+
+    Args:
+        k_cache, v_cache, k_scale, v_scale, block_table, seqlens_k: as
+            ``kvcache_write_paged``; no page may belong to two sequences
+        weights: fp32 [B, H_kv, L] (``kvcache_weights_paged``), L at least the
+            positions of a table row
+        keep: positions that stay, one int for all or B of them
+        recent, first: the last `recent` and the first `first` positions stay
+            whatever their weight (`first` comes first where keep is too small)
+
+    Of the others those of the largest weight stay (equal weights: the lower
+    position; a NaN is less than every number).  Keys, values, scales and
+    weights of what stays move to positions 0 .. keep - 1 in their order;
+    positions behind keep what they hold.
+
+    Returns:
+        int32 [B]: min(seqlens_k, keep), the lengths from now on (the next
+        tokens are written behind them).
+    """
+    return _C.kvcache_evict_paged(k_cache, v_cache, weights, block_table, seqlens_k, keep, recent, first,
+                                  k_scale, v_scale)

@@ -332,6 +332,90 @@ int fa_fwd_paged(const fa_paged_cache* cache, const void* Q, long long q_token_s
 size_t fa_fwd_paged_workspace_bytes(const fa_paged_cache* cache, int B, int Hq, int total_q,
                                     int max_seqlen_q, int max_seqlen_k);
 
+/*
+ * fa_fwd_paged_prefix — fa_fwd_paged for a batch whose sequences share long
+ * prefixes, each computed once for all its tokens.  Prefix g of n_prefixes has
+ * prefix_lens[g] keys in the pages of row g of `prefix_table` (rows of
+ * prefix_max_pages entries, prefix_table_stride apart; the same pages as the
+ * sequences', which hold what follows the prefix), and packed rows
+ * [cu_prefix_q[g], cu_prefix_q[g+1]) see all of them besides their own
+ * sequence's keys, for which `causal` and everything else is as in fa_fwd_paged.
+ * cu_prefix_q (n_prefixes + 1 entries, non-decreasing) and prefix_lens are int32
+ * DEVICE arrays, clamped to their bounds; rows outside every range have no prefix.
+ * max_prefix_q / max_prefix_k bound the tokens and keys of a prefix: tokens beyond
+ * the first max_prefix_q of a range do not see it, keys beyond max_prefix_k are not seen.
+ * The two sets of keys are computed one after the other and joined in fp32; the
+ * result is rounded once.  `workspace` (16-byte aligned) needs
+ * fa_fwd_paged_prefix_workspace_bytes() bytes.  Asynchronous on `stream`.
+ *
+ * No reference counterpart (reference llama_attention_replacement.py:63-65).
+ */
+int fa_fwd_paged_prefix(const fa_paged_cache* cache, const int* prefix_table,
+                        long long prefix_table_stride, int prefix_max_pages, int n_prefixes,
+                        const int* cu_prefix_q, const int* prefix_lens, int max_prefix_q,
+                        int max_prefix_k, const void* Q, long long q_token_stride,
+                        long long q_head_stride, void* O, float* lse, const int* cu_seqlens_q,
+                        const int* seqlens_k, int B, int Hq, int total_q, int max_seqlen_q,
+                        int max_seqlen_k, float scale, int causal, int dtype, void* workspace,
+                        size_t workspace_bytes, void* stream);
+
+/* Workspace bytes of fa_fwd_paged_prefix (a function of its sizes alone): the fp32
+ * results of the prefixes, and the larger of the two passes' needs; 0 for what the
+ * call refuses. */
+size_t fa_fwd_paged_prefix_workspace_bytes(const fa_paged_cache* cache, int n_prefixes,
+                                           int max_prefix_q, int max_prefix_k, int B, int Hq,
+                                           int total_q, int max_seqlen_q, int max_seqlen_k);
+
+/* What fa_kvcache_weights does with the sums of earlier calls. */
+enum {
+  FA_WEIGHTS_SET = 0,   /* they are replaced */
+  FA_WEIGHTS_ADD = 1,   /* added to */
+  FA_WEIGHTS_APPEND = 2 /* added to, but the new tokens' own positions, which have none, are set */
+};
+
+/*
+ * fa_kvcache_weights — the attention weight that cached keys received: for the
+ * positions j < min(seqlens_k[b], max_seqlen_k) of every sequence b and KV head h
+ *   weights[b * w_seq_stride + h * w_head_stride + j]  = or +=
+ *     sum over its new tokens i and the query heads of h of exp(scale q_i.k_j - LSE_i),
+ * keys that a row may not see (`causal`) adding 0.  Q, cu_seqlens_q, seqlens_k,
+ * the bounds, scale and causal are those of the attention call whose LSE (fp32
+ * [Hq, total_q]) is given; a row whose LSE is -inf adds nothing.  Only the keys of
+ * `cache` are read (v and v_scale may be NULL).  `weights` is fp32, a row holds
+ * weights_len >= min(max_seqlen_k, max_pages * page_size) positions and rows do not
+ * overlap; positions from there on, and those of other rows, are left as they are.
+ * All sums are fp32, in an order that does not depend on timing.  Asynchronous
+ * on `stream`.
+ *
+ * No reference counterpart (reference llama_attention_replacement.py:63-65).
+ */
+int fa_kvcache_weights(const fa_paged_cache* cache, const void* Q, long long q_token_stride,
+                       long long q_head_stride, const float* lse, const int* cu_seqlens_q,
+                       const int* seqlens_k, int B, int Hq, int total_q, int max_seqlen_q,
+                       int max_seqlen_k, float* weights, long long w_seq_stride,
+                       long long w_head_stride, int weights_len, int mode, float scale, int causal,
+                       int dtype, void* stream);
+
+/*
+ * fa_kvcache_evict — cuts every sequence of a cache to its budget, for each KV
+ * head by itself.  Of a sequence of n = seqlens_k[b] > keep positions (keep[b], an
+ * int32 DEVICE array, or keep_all for all where keep is NULL; negative: 0) stay
+ * the first f = min(first, keep), the last r = min(recent, keep - f) and, of those
+ * between, the keep - f - r with the largest weights (equal weights: the lower
+ * position; a NaN is less than every number).  Their rows of K and V, scales and
+ * weights move together in order of position to positions 0 .. keep - 1, in place;
+ * what lies behind is left as it is.  new_lens[b] (int32 DEVICE array, not
+ * seqlens_k) = min(n, keep).  `weights` as in fa_kvcache_weights, with weights_len >=
+ * max_pages * page_size.  No page may belong to two sequences, nor twice to one.
+ * Rows without a page read as zeros, and are not written.  Asynchronous on `stream`.
+ *
+ * No reference counterpart (reference llama_attention_replacement.py:63-65).
+ */
+int fa_kvcache_evict(const fa_paged_cache* cache, float* weights, long long w_seq_stride,
+                     long long w_head_stride, int weights_len, const int* seqlens_k,
+                     const int* keep, int keep_all, int first, int recent, int* new_lens, int B,
+                     void* stream);
+
 /* ---- reference-compatible launchers (void, fp16, blocking) ----
  * Same signatures and conventions as the reference: errors are printed to
  * stderr, the work runs on the legacy default stream and the call ends with
