@@ -186,8 +186,305 @@ __global__ void __launch_bounds__(kWeightThreads) paged_weights_kernel(const Pag
   }
 }
 
+// ---- few query rows (decode, drafts)
+//
+// Bound by the keys' bytes.  All steps of 16 keys (32 of 8-bit pages) of the batch, in
+// order of sequence, head and key, are cut into equal runs, one per warp, whatever the
+// sequences' lengths.  A warp has its query rows in registers, the page ids of 32 groups of
+// 16 keys in one register a lane, loaded a window ahead, and the next step's keys on
+// their way while it computes this one's; nothing waits for another warp.
+//
+// bf16 queries over 8-bit pages are taken as f16, q / 2^e with 2^e the size of
+// the row's largest element: bf16's 8 bits fit f16's 11, and elements below 2^-14 of
+// the largest lose at most 2^-25 of it, no more than the sum in fp32 does.
+constexpr int kRowsFew = 32;
+
+// Positions of the work order that a (sequence, head) takes besides its steps: its
+// queries, and the wait for its first keys.
+constexpr int kSegmentCost = 2;
+
+template <int D, int KV>
+struct Stream {
+  static constexpr bool k8 = KV >= FA_DTYPE_INT8;
+  static constexpr int kRowBytes = k8 ? D : 2 * D;
+  static constexpr int kChunks = kRowBytes / 64;  // 16-byte pieces of a lane per key
+  static constexpr int kTiles = k8 ? 2 : 1;       // of 16 keys in a step
+  static constexpr int kKeys = 16 * kTiles;
+  static constexpr int kPairs = D / 8;            // 32-bit operands of a lane per query row
+};
+
+template <int D, int KV>
+struct KeyStep {
+  using S = Stream<D, KV>;
+  uint4 x[S::kTiles][2][S::kChunks];  // keys g, g + 8 of a tile
+  float ks[S::kTiles][2];
+  float old[S::kTiles];               // earlier sum of key g + 8 j (lanes j < 2)
+};
+
+__device__ __forceinline__ uint4 load_once(const uint8_t* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+
+__host__ __device__ constexpr int few_ctas_per_sm(int nt) { return nt == 1 ? 4 : nt == 2 ? 3 : 2; }
+
+template <int D, int KV, bool QBF16, int NT>
+__global__ void __launch_bounds__(kWeightThreads, few_ctas_per_sm(NT))
+    paged_weights_few_kernel(const PagedWeights p, int n_warps) {
+  using S = Stream<D, KV>;
+  constexpr bool kBf16 = !S::k8 && QBF16;  // type of the products
+  constexpr int kWarps = kWeightThreads / 32;
+  const PagedAttn& a = p.a;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, j = lane & 3;
+  const int H = a.c.heads;
+
+  // ---- the warp's run [v, v1), relative to sequence b's first position
+  __shared__ long long sh_scan[kWarps];
+  __shared__ int sh_b[kWarps];
+  __shared__ long long sh_rel[kWarps];
+  auto steps_of = [&](const Seq& s) { return (s.nk + S::kKeys - 1) / S::kKeys; };
+  auto positions = [&](int b) -> long long {
+    const int n = steps_of(load_seq(a, b));
+    return n > 0 ? static_cast<long long>(n + kSegmentCost) * H : 0;
+  };
+  long long v, v1;
+  int b;
+  {
+    const int share = (a.r.B + kWeightThreads - 1) / kWeightThreads;
+    const int s0 = min(static_cast<int>(threadIdx.x) * share, a.r.B), s1 = min(s0 + share, a.r.B);
+    long long sum = 0, total;
+    for (int i = s0; i < s1; ++i) sum += positions(i);
+    const long long lo = block_scan<kWeightThreads>(sum, sh_scan, &total);
+    const long long per = (total + n_warps - 1) / n_warps;
+    for (int w = 0; w < kWarps; ++w) {
+      const long long first = per * (static_cast<long long>(blockIdx.x) * kWarps + w);
+      if (first < total && first >= lo && first < lo + sum) {
+        long long x = lo;
+        for (int i = s0; i < s1; ++i) {
+          const long long n = positions(i);
+          if (first < x + n) {
+            sh_b[w] = i;
+            sh_rel[w] = first - x;
+            break;
+          }
+          x += n;
+        }
+      }
+    }
+    __syncthreads();
+    const long long v0 = per * (static_cast<long long>(blockIdx.x) * kWarps + warp);
+    if (v0 >= total) return;
+    b = sh_b[warp];
+    v = sh_rel[warp];
+    v1 = min(v0 + per, total) - v0 + v;
+  }
+
+  for (Seq s = load_seq(a, b);;) {
+    const int n_all = steps_of(s), seg = n_all + kSegmentCost;
+    const int h = static_cast<int>(v / seg);
+    const long long at = static_cast<long long>(h) * seg + kSegmentCost;  // of the head's first step
+    const int t0 = static_cast<int>(max(v - at, 0ll)), t1 = static_cast<int>(min(v1 - at, static_cast<long long>(n_all)));
+    if (t0 < t1) {
+      const int fresh0 = p.mode == FA_WEIGHTS_SET      ? 0
+                         : p.mode == FA_WEIGHTS_APPEND ? min(__ldg(a.r.lens + b), 3 << 29) - s.n
+                                                       : 0x7fffffff;
+      float* const w = p.w + b * p.w_seq + h * p.w_head;
+      const uint8_t* const k_head = a.c.k + h * a.c.head_stride;
+      const float* const ks_head = S::k8 ? a.c.ks + h * a.c.s_head : nullptr;
+      // pages of the 16-key groups: lane l has that of group wbase + l, and of wbase + 32 + l
+      int wbase = t0 * S::kTiles;
+      auto window = [&](int first) {
+        const int pos = 16 * (first + lane);
+        return first + lane < t1 * S::kTiles && pos < s.vis ? a.c.lookup(b, pos) : -1;
+      };
+      int win = window(wbase), win_next = window(wbase + 32);
+
+      auto load = [&](KeyStep<D, KV>& st, int t) {
+        if (t * S::kTiles >= wbase + 32) {
+          wbase += 32;
+          win = win_next;
+          win_next = window(wbase + 32);
+        }
+#pragma unroll
+        for (int m = 0; m < S::kTiles; ++m) {
+          const int key0 = t * S::kKeys + 16 * m;
+          const int page = __shfl_sync(0xffffffffu, win, t * S::kTiles + m - wbase);
+          const int row0 = a.c.row_in_page(key0);
+          const uint8_t* const base = k_head + page * a.c.page_stride;
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const int r = g + 8 * y;
+            const bool ok = page >= 0 && key0 + r < s.vis;
+            const uint8_t* src = base + static_cast<long long>(row0 + r) * a.c.row_stride + 16 * j;
+#pragma unroll
+            for (int c = 0; c < S::kChunks; ++c)
+              st.x[m][y][c] = ok ? load_once(src + 64 * c) : make_uint4(0u, 0u, 0u, 0u);
+            if constexpr (S::k8)
+              st.ks[m][y] = ok ? __ldg(ks_head + page * a.c.s_page + static_cast<long long>(row0 + r) * a.c.s_row) : 0.f;
+          }
+          const int key = key0 + g + 8 * j;
+          st.old[m] = j < 2 && key < s.nk && key < fresh0 ? w[key] : 0.f;
+        }
+      };
+
+      KeyStep<D, KV> cur, next;
+      load(cur, t0);
+
+      // ---- query rows: operands, LSE and key limit of this thread's two rows per block of 8
+      const int rows = s.nq * a.group;
+      uint32_t q[NT][S::kPairs];
+      float cs[NT][2], lse[NT][2];
+      int lim[NT][2];
+    #pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int r = nt * 8 + g;
+        const QueryRow qr = query_row(a, s, h, r);
+        const uint8_t* const src = a.q + static_cast<long long>(qr.tok) * a.q_token + qr.hq * a.q_head;
+    #pragma unroll
+        for (int i = 0; i < S::kPairs / 4; ++i) {
+          // 16-bit keys: the piece of 8 columns at 32 i + 8 j; 8-bit keys: the half i % 2 of the
+          // 16 columns at 64 (i / 2) + 16 j
+          const int byte = S::k8 ? 128 * (i / 2) + 32 * j + 16 * (i % 2) : 64 * i + 16 * j;
+          const uint4 v = r < rows ? __ldg(reinterpret_cast<const uint4*>(src + byte)) : make_uint4(0u, 0u, 0u, 0u);
+          q[nt][4 * i] = v.x;
+          q[nt][4 * i + 1] = v.y;
+          q[nt][4 * i + 2] = v.z;
+          q[nt][4 * i + 3] = v.w;
+        }
+        float unit = 1.f;
+        if constexpr (S::k8 && QBF16) {
+          float mx = 0.f;
+    #pragma unroll
+          for (int i = 0; i < S::kPairs; ++i) {
+            const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&q[nt][i]));
+            mx = fmaxf(mx, fmaxf(fabsf(f.x), fabsf(f.y)));
+          }
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          const uint32_t e = __float_as_uint(mx) & 0x7f800000u;
+          const bool plain = e == 0u || e >= 0x7e800000u;
+          unit = plain ? 1.f : __uint_as_float(e);
+          const float inv = plain ? 1.f : __uint_as_float(0x7f000000u - e);
+    #pragma unroll
+          for (int i = 0; i < S::kPairs; ++i) {
+            const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&q[nt][i]));
+            const __half2 x = __floats2half2_rn(f.x * inv, f.y * inv);
+            q[nt][i] = *reinterpret_cast<const uint32_t*>(&x);
+          }
+        }
+    #pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int rc = nt * 8 + 2 * j + c;
+          const QueryRow qc = query_row(a, s, h, rc);
+          float l = -INFINITY;
+          if (rc < rows) l = a.lse[static_cast<long long>(qc.hq) * a.r.total + qc.tok];
+          lim[nt][c] = l == -INFINITY ? 0 : row_limit(a, s, rc / a.group);
+          lse[nt][c] = l == -INFINITY ? 0.f : l * 1.4426950408889634f;
+          cs[nt][c] = a.scale_log2;
+          if constexpr (S::k8 && QBF16) cs[nt][c] *= __shfl_sync(0xffffffffu, unit, (2 * j + c) * 4);
+        }
+      }
+      int all = 0x7fffffff;  // every row sees the keys below
+    #pragma unroll
+      for (int nt = 0; nt < NT; ++nt) all = min(all, min(lim[nt][0], lim[nt][1]));
+      all = __reduce_min_sync(0xffffffffu, all);
+      auto compute = [&](const KeyStep<D, KV>& st, int t) {
+#pragma unroll
+        for (int m = 0; m < S::kTiles; ++m) {
+          const int key0 = t * S::kKeys + 16 * m;
+          float c[NT][4];
+    #pragma unroll
+          for (int nt = 0; nt < NT; ++nt) c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.f;
+    #pragma unroll
+          for (int i = 0; i < S::kChunks; ++i) {
+            const uint32_t k0[4] = {st.x[m][0][i].x, st.x[m][0][i].y, st.x[m][0][i].z, st.x[m][0][i].w};
+            const uint32_t k1[4] = {st.x[m][1][i].x, st.x[m][1][i].y, st.x[m][1][i].z, st.x[m][1][i].w};
+            if constexpr (!S::k8) {
+    #pragma unroll
+              for (int e = 0; e < 2; ++e)
+    #pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                  mma_16816<kBf16>(c[nt], k0[2 * e], k1[2 * e], k0[2 * e + 1], k1[2 * e + 1], q[nt][4 * i + 2 * e],
+                                   q[nt][4 * i + 2 * e + 1]);
+            } else {
+    #pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                uint32_t a0, a1, a2, a3;
+                widen<KV, false>(k0[e], a0, a2);
+                widen<KV, false>(k1[e], a1, a3);
+    #pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+                  mma_16816<false>(c[nt], a0, a1, a2, a3, q[nt][8 * i + 2 * e], q[nt][8 * i + 2 * e + 1]);
+              }
+            }
+          }
+          float sum[2] = {0.f, 0.f};
+          const bool masked = key0 + 16 > all;
+    #pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+    #pragma unroll
+            for (int y = 0; y < 2; ++y)
+    #pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float x = S::k8 ? c[nt][2 * y + e] * st.ks[m][y] : c[nt][2 * y + e];
+                const float v = ptx::ex2_approx(fmaf(x, cs[nt][e], -lse[nt][e]));
+                if (!masked || key0 + g + 8 * y < lim[nt][e]) sum[y] += v;
+              }
+    #pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            sum[y] += __shfl_xor_sync(0xffffffffu, sum[y], 1);
+            sum[y] += __shfl_xor_sync(0xffffffffu, sum[y], 2);
+          }
+          const int key = key0 + g + 8 * j;
+          if (j < 2 && key < s.nk) w[key] = st.old[m] + (j == 0 ? sum[0] : sum[1]);
+        }
+      };
+      for (int t = t0; t < t1; t += 2) {
+        if (t + 1 < t1) load(next, t + 1);
+        compute(cur, t);
+        if (t + 1 >= t1) break;
+        if (t + 2 < t1) load(cur, t + 2);
+        compute(next, t + 1);
+      }
+    }
+    // ---- the next segment
+    v = at + n_all;
+    if (v >= v1) break;
+    if (h + 1 == H) {
+      v1 -= v;
+      v = 0;
+      do {
+        if (++b >= a.r.B) return;
+        s = load_seq(a, b);
+      } while (s.nk <= 0);
+    }
+  }
+}
+
+template <int D, int KV, bool QBF16, int NT>
+cudaError_t few_impl(const PagedWeights& p, int sms, cudaStream_t stream) {
+  using S = Stream<D, KV>;
+  constexpr int kWarps = kWeightThreads / 32;
+  // no more warps than steps there can be
+  const long long heads = static_cast<long long>(p.a.r.B) * p.a.c.heads;
+  const long long steps = heads * ((static_cast<long long>(p.a.max_k) + S::kKeys - 1) / S::kKeys);
+  const long long most = static_cast<long long>(sms) * few_ctas_per_sm(NT);
+  const long long ctas = (steps + kWarps - 1) / kWarps;
+  const int grid = static_cast<int>(ctas < most ? ctas : most);
+  paged_weights_few_kernel<D, KV, QBF16, NT><<<grid, kWeightThreads, 0, stream>>>(p, grid * kWarps);
+  return cudaGetLastError();
+}
+
 template <int D, int KV, bool QBF16>
-cudaError_t weights_impl(const PagedWeights& p, cudaStream_t stream) {
+cudaError_t weights_impl(const PagedWeights& p, int sms, cudaStream_t stream) {
+  const long long rows = static_cast<long long>(p.a.max_q < p.a.r.total ? p.a.max_q : p.a.r.total) * p.a.group;
+  if (rows <= 8) return few_impl<D, KV, QBF16, 1>(p, sms, stream);
+  if (rows <= 16) return few_impl<D, KV, QBF16, 2>(p, sms, stream);
+  if (rows <= kRowsFew) return few_impl<D, KV, QBF16, 4>(p, sms, stream);
   const int n_blocks = (p.a.max_k + kWeightKeys - 1) / kWeightKeys;
   const long long grid = static_cast<long long>(n_blocks) * p.a.r.B * p.a.c.heads;
   if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;
@@ -197,23 +494,23 @@ cudaError_t weights_impl(const PagedWeights& p, cudaStream_t stream) {
 }
 
 template <int D>
-cudaError_t weights_d(const PagedWeights& p, int kv, bool bf16, cudaStream_t s) {
+cudaError_t weights_d(const PagedWeights& p, int kv, bool bf16, int sms, cudaStream_t s) {
   switch (kv) {
     case FA_DTYPE_INT8:
-      return bf16 ? weights_impl<D, FA_DTYPE_INT8, true>(p, s) : weights_impl<D, FA_DTYPE_INT8, false>(p, s);
+      return bf16 ? weights_impl<D, FA_DTYPE_INT8, true>(p, sms, s) : weights_impl<D, FA_DTYPE_INT8, false>(p, sms, s);
     case FA_DTYPE_E4M3:
-      return bf16 ? weights_impl<D, FA_DTYPE_E4M3, true>(p, s) : weights_impl<D, FA_DTYPE_E4M3, false>(p, s);
-    case FA_DTYPE_BF16: return weights_impl<D, FA_DTYPE_BF16, true>(p, s);
-    default: return weights_impl<D, FA_DTYPE_F16, false>(p, s);
+      return bf16 ? weights_impl<D, FA_DTYPE_E4M3, true>(p, sms, s) : weights_impl<D, FA_DTYPE_E4M3, false>(p, sms, s);
+    case FA_DTYPE_BF16: return weights_impl<D, FA_DTYPE_BF16, true>(p, sms, s);
+    default: return weights_impl<D, FA_DTYPE_F16, false>(p, sms, s);
   }
 }
 
 }  // namespace
 
-cudaError_t launch_paged_weights(const PagedWeights& p, int head_dim, int cache_dtype, bool bf16, int,
+cudaError_t launch_paged_weights(const PagedWeights& p, int head_dim, int cache_dtype, bool bf16, int sms,
                                  cudaStream_t stream) {
-  return head_dim == 64 ? weights_d<64>(p, cache_dtype, bf16, stream)
-                        : weights_d<128>(p, cache_dtype, bf16, stream);
+  return head_dim == 64 ? weights_d<64>(p, cache_dtype, bf16, sms, stream)
+                        : weights_d<128>(p, cache_dtype, bf16, sms, stream);
 }
 
 }  // namespace fa
