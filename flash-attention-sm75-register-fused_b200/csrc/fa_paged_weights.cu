@@ -213,12 +213,18 @@ struct Stream {
   static constexpr int kPairs = D / 8;            // 32-bit operands of a lane per query row
 };
 
+__device__ __forceinline__ long long shfl64(long long x, int src) {
+  const int lo = __shfl_sync(0xffffffffu, static_cast<int>(x), src);
+  const int hi = __shfl_sync(0xffffffffu, static_cast<int>(x >> 32), src);
+  return (static_cast<long long>(hi) << 32) | static_cast<unsigned>(lo);
+}
+
 template <int D, int KV>
 struct KeyStep {
   using S = Stream<D, KV>;
   uint4 x[S::kTiles][2][S::kChunks];  // keys g, g + 8 of a tile
   float ks[S::kTiles][2];
-  float old[S::kTiles];               // earlier sum of key g + 8 j (lanes j < 2)
+  float old;                          // earlier sum of this lane's key (key_of)
 };
 
 __device__ __forceinline__ uint4 load_once(const uint8_t* p) {
@@ -293,42 +299,60 @@ __global__ void __launch_bounds__(kWeightThreads, few_ctas_per_sm(NT))
                          : p.mode == FA_WEIGHTS_APPEND ? min(__ldg(a.r.lens + b), 3 << 29) - s.n
                                                        : 0x7fffffff;
       float* const w = p.w + b * p.w_seq + h * p.w_head;
-      const uint8_t* const k_head = a.c.k + h * a.c.head_stride;
-      const float* const ks_head = S::k8 ? a.c.ks + h * a.c.s_head : nullptr;
-      // pages of the 16-key groups: lane l has that of group wbase + l, and of wbase + 32 + l
+      // the key of a step whose sum this lane gets: with one tile, lanes j and j + 2 the same
+      auto key_of = [&](int t) { return t * S::kKeys + (S::kTiles == 2 ? 8 * j : 8 * (j & 1)) + g; };
+      // Offsets of the 16-key groups' first rows and scales (-1: no page, or no key any row may
+      // see): lane l has those of group wbase + l, and the page of group wbase + 32 + l.
       int wbase = t0 * S::kTiles;
-      auto window = [&](int first) {
+      auto page_at = [&](int first) {
         const int pos = 16 * (first + lane);
         return first + lane < t1 * S::kTiles && pos < s.vis ? a.c.lookup(b, pos) : -1;
       };
-      int win = window(wbase), win_next = window(wbase + 32);
+      long long win, win_scale = 0;
+      int next_page = page_at(wbase);
+      auto next_window = [&] {
+        const int page = next_page, row = a.c.row_in_page(16 * (wbase + lane));
+        win = page < 0 ? -1 : page * a.c.page_stride + row * a.c.row_stride;
+        if constexpr (S::k8) win_scale = page * a.c.s_page + row * a.c.s_row;
+        next_page = page_at(wbase + 32);
+      };
+      next_window();
+            const uint8_t* const k_lane = a.c.k + h * a.c.head_stride + g * a.c.row_stride + 16 * j;
+      const long long row8 = 8 * a.c.row_stride;
+      const float* const ks_lane = S::k8 ? a.c.ks + h * a.c.s_head + g * a.c.s_row : nullptr;
 
       auto load = [&](KeyStep<D, KV>& st, int t) {
         if (t * S::kTiles >= wbase + 32) {
           wbase += 32;
-          win = win_next;
-          win_next = window(wbase + 32);
+          next_window();
         }
 #pragma unroll
         for (int m = 0; m < S::kTiles; ++m) {
           const int key0 = t * S::kKeys + 16 * m;
-          const int page = __shfl_sync(0xffffffffu, win, t * S::kTiles + m - wbase);
-          const int row0 = a.c.row_in_page(key0);
-          const uint8_t* const base = k_head + page * a.c.page_stride;
+          const long long off = shfl64(win, t * S::kTiles + m - wbase);
+          const uint8_t* const src = k_lane + off;
+          const float* sc = nullptr;
+          if constexpr (S::k8) sc = ks_lane + shfl64(win_scale, t * S::kTiles + m - wbase);
+          if (off >= 0 && key0 + 16 <= s.vis) {
 #pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const int r = g + 8 * y;
-            const bool ok = page >= 0 && key0 + r < s.vis;
-            const uint8_t* src = base + static_cast<long long>(row0 + r) * a.c.row_stride + 16 * j;
+            for (int y = 0; y < 2; ++y) {
 #pragma unroll
-            for (int c = 0; c < S::kChunks; ++c)
-              st.x[m][y][c] = ok ? load_once(src + 64 * c) : make_uint4(0u, 0u, 0u, 0u);
-            if constexpr (S::k8)
-              st.ks[m][y] = ok ? __ldg(ks_head + page * a.c.s_page + static_cast<long long>(row0 + r) * a.c.s_row) : 0.f;
+              for (int c = 0; c < S::kChunks; ++c) st.x[m][y][c] = load_once(src + y * row8 + 64 * c);
+              if constexpr (S::k8) st.ks[m][y] = __ldg(sc + 8 * y * a.c.s_row);
+            }
+          } else {
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              const bool ok = off >= 0 && key0 + g + 8 * y < s.vis;
+#pragma unroll
+              for (int c = 0; c < S::kChunks; ++c)
+                st.x[m][y][c] = ok ? load_once(src + y * row8 + 64 * c) : make_uint4(0u, 0u, 0u, 0u);
+              if constexpr (S::k8) st.ks[m][y] = ok ? __ldg(sc + 8 * y * a.c.s_row) : 0.f;
+            }
           }
-          const int key = key0 + g + 8 * j;
-          st.old[m] = j < 2 && key < s.nk && key < fresh0 ? w[key] : 0.f;
         }
+        const int key = key_of(t);
+        st.old = key < min(s.nk, fresh0) ? w[key] : 0.f;
       };
 
       KeyStep<D, KV> cur, next;
@@ -337,7 +361,7 @@ __global__ void __launch_bounds__(kWeightThreads, few_ctas_per_sm(NT))
       // ---- query rows: operands, LSE and key limit of this thread's two rows per block of 8
       const int rows = s.nq * a.group;
       uint32_t q[NT][S::kPairs];
-      float cs[NT][2], lse[NT][2];
+      float cs[NT][2], nlse[NT][2];
       int lim[NT][2];
     #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -383,7 +407,7 @@ __global__ void __launch_bounds__(kWeightThreads, few_ctas_per_sm(NT))
           float l = -INFINITY;
           if (rc < rows) l = a.lse[static_cast<long long>(qc.hq) * a.r.total + qc.tok];
           lim[nt][c] = l == -INFINITY ? 0 : row_limit(a, s, rc / a.group);
-          lse[nt][c] = l == -INFINITY ? 0.f : l * 1.4426950408889634f;
+          nlse[nt][c] = l == -INFINITY ? 0.f : l * -1.4426950408889634f;
           cs[nt][c] = a.scale_log2;
           if constexpr (S::k8 && QBF16) cs[nt][c] *= __shfl_sync(0xffffffffu, unit, (2 * j + c) * 4);
         }
@@ -393,55 +417,73 @@ __global__ void __launch_bounds__(kWeightThreads, few_ctas_per_sm(NT))
       for (int nt = 0; nt < NT; ++nt) all = min(all, min(lim[nt][0], lim[nt][1]));
       all = __reduce_min_sync(0xffffffffu, all);
       auto compute = [&](const KeyStep<D, KV>& st, int t) {
+        float sum[S::kTiles][2];
 #pragma unroll
         for (int m = 0; m < S::kTiles; ++m) {
           const int key0 = t * S::kKeys + 16 * m;
           float c[NT][4];
-    #pragma unroll
+#pragma unroll
           for (int nt = 0; nt < NT; ++nt) c[nt][0] = c[nt][1] = c[nt][2] = c[nt][3] = 0.f;
-    #pragma unroll
+#pragma unroll
           for (int i = 0; i < S::kChunks; ++i) {
             const uint32_t k0[4] = {st.x[m][0][i].x, st.x[m][0][i].y, st.x[m][0][i].z, st.x[m][0][i].w};
             const uint32_t k1[4] = {st.x[m][1][i].x, st.x[m][1][i].y, st.x[m][1][i].z, st.x[m][1][i].w};
             if constexpr (!S::k8) {
-    #pragma unroll
+#pragma unroll
               for (int e = 0; e < 2; ++e)
-    #pragma unroll
+#pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
                   mma_16816<kBf16>(c[nt], k0[2 * e], k1[2 * e], k0[2 * e + 1], k1[2 * e + 1], q[nt][4 * i + 2 * e],
                                    q[nt][4 * i + 2 * e + 1]);
             } else {
-    #pragma unroll
+#pragma unroll
               for (int e = 0; e < 4; ++e) {
                 uint32_t a0, a1, a2, a3;
                 widen<KV, false>(k0[e], a0, a2);
                 widen<KV, false>(k1[e], a1, a3);
-    #pragma unroll
+#pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
                   mma_16816<false>(c[nt], a0, a1, a2, a3, q[nt][8 * i + 2 * e], q[nt][8 * i + 2 * e + 1]);
               }
             }
           }
-          float sum[2] = {0.f, 0.f};
-          const bool masked = key0 + 16 > all;
-    #pragma unroll
+          float v[NT][4];
+#pragma unroll
           for (int nt = 0; nt < NT; ++nt)
-    #pragma unroll
-            for (int y = 0; y < 2; ++y)
-    #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const float x = S::k8 ? c[nt][2 * y + e] * st.ks[m][y] : c[nt][2 * y + e];
-                const float v = ptx::ex2_approx(fmaf(x, cs[nt][e], -lse[nt][e]));
-                if (!masked || key0 + g + 8 * y < lim[nt][e]) sum[y] += v;
-              }
-    #pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            sum[y] += __shfl_xor_sync(0xffffffffu, sum[y], 1);
-            sum[y] += __shfl_xor_sync(0xffffffffu, sum[y], 2);
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+              float x0 = c[nt][2 * y], x1 = c[nt][2 * y + 1];
+              if constexpr (S::k8) ptx::fmul2(x0, x1, x0, x1, st.ks[m][y], st.ks[m][y]);
+              ptx::ffma2(x0, x1, x0, x1, cs[nt][0], cs[nt][1], nlse[nt][0], nlse[nt][1]);
+              v[nt][2 * y] = ptx::ex2_approx(x0);
+              v[nt][2 * y + 1] = ptx::ex2_approx(x1);
+            }
+          if (key0 + 16 > all) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (key0 + g + 8 * (i >> 1) >= lim[nt][i & 1]) v[nt][i] = 0.f;
           }
-          const int key = key0 + g + 8 * j;
-          if (j < 2 && key < s.nk) w[key] = st.old[m] + (j == 0 ? sum[0] : sum[1]);
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            sum[m][y] = v[0][2 * y] + v[0][2 * y + 1];
+#pragma unroll
+            for (int nt = 1; nt < NT; ++nt) sum[m][y] += v[nt][2 * y] + v[nt][2 * y + 1];
+          }
         }
+        // over the quad's lanes: each keeps the half it needs and hands on the other
+        float mine[S::kTiles];
+#pragma unroll
+        for (int m = 0; m < S::kTiles; ++m)
+          mine[m] = (j & 1 ? sum[m][1] : sum[m][0]) + __shfl_xor_sync(0xffffffffu, j & 1 ? sum[m][0] : sum[m][1], 1);
+        float total;
+        if constexpr (S::kTiles == 2)
+          total = (j & 2 ? mine[1] : mine[0]) + __shfl_xor_sync(0xffffffffu, j & 2 ? mine[0] : mine[1], 2);
+        else
+          total = mine[0] + __shfl_xor_sync(0xffffffffu, mine[0], 2);
+        const int key = key_of(t);
+        if ((S::kTiles == 2 || j < 2) && key < s.nk) w[key] = st.old + total;
       };
       for (int t = t0; t < t1; t += 2) {
         if (t + 1 < t1) load(next, t + 1);
