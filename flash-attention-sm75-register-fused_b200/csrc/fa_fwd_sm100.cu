@@ -1485,3 +1485,4 @@ cudaError_t read_status(unsigned long long* out, bool reset) {
 #include "fa_bwd_sm100.cuh"
 #include "fa_paged_chunk.cuh"
 #include "fa_paged_decode.cuh"
+#include "fa_paged_weights_chunk.cuh"

@@ -126,8 +126,26 @@ struct PagedWeights {
   long long w_seq, w_head;
   int mode;  // FA_WEIGHTS_*
 };
-cudaError_t launch_paged_weights(const PagedWeights& p, int head_dim, int cache_dtype, bool bf16, int sms,
-                                 cudaStream_t stream);
+// Sequences of at most max_rows <= paged_weights_rows() query rows (new tokens x group) per
+// KV head; the others are left alone.
+constexpr int paged_weights_rows() { return 32; }
+cudaError_t launch_paged_weights(const PagedWeights& p, int max_rows, int head_dim, int cache_dtype, bool bf16,
+                                 int sms, cudaStream_t stream);
+
+// ... and those of more than skip_rows rows (fa_paged_weights_chunk.cuh).
+struct alignas(64) WeightsChunkParams {
+  CUtensorMap tm_q;  // (d, Hq, T), box (64, G, tq)
+  PagedWeights w;
+  int tq;            // tokens of a 128-row tile: 128 / group
+  int skip_rows;
+  unsigned epoch;
+  unsigned long long timeout_ns;
+  // set by launch_paged_weights_chunk: key blocks of a (sequence, head), CTAs that share one
+  int n_blocks, split;
+};
+cudaError_t launch_paged_weights_chunk(WeightsChunkParams p, int head_dim, int cache_dtype, bool bf16, int sms,
+                                       cudaStream_t stream);
+
 
 // Eviction (fa_paged_evict.cu).
 struct PagedEvict {

@@ -598,9 +598,30 @@ int fa_kvcache_weights(const fa_paged_cache* cache, const void* Q, long long q_t
   p.w_seq = w_seq_stride;
   p.w_head = w_head_stride;
   p.mode = mode;
-  const cudaError_t e = fa::launch_paged_weights(p, cache->head_dim, cache->dtype, dtype == FA_DTYPE_BF16,
-                                                 fa::host_sm_count(), static_cast<cudaStream_t>(stream));
-  return e == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
+  // Sequences of few query rows are streamed, the others go through the tensor cores; both
+  // where the bounds allow both (see kMixedRows).
+  const bool bf16 = dtype == FA_DTYPE_BF16;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int most = max_seqlen_q < total_q ? max_seqlen_q : total_q, group = p.a.group;
+  const bool chunk = static_cast<long long>(most) * group > fa::paged_weights_rows();
+  const bool few = !chunk || (B > 1 && group <= kMixedRows && total_q < static_cast<long long>(B) * most);
+  const int few_rows = chunk ? kMixedRows / group * group : most * group;
+  if (few && fa::launch_paged_weights(p, few_rows, cache->head_dim, cache->dtype, bf16, fa::host_sm_count(), st) !=
+                 cudaSuccess)
+    return FA_ERR_LAUNCH;
+  if (chunk) {
+    fa::WeightsChunkParams c;
+    c.w = p;
+    c.tq = 128 / group;
+    c.skip_rows = few ? few_rows : -1;
+    c.epoch = fa::host_next_epoch();
+    c.timeout_ns = fa::host_timeout_ns();
+    if (!query_map(*cache, c.tq, Q, q_token_stride, q_head_stride, Hq, total_q, bf16, &c.tm_q))
+      return FA_ERR_TENSOR_MAP;
+    if (fa::launch_paged_weights_chunk(c, cache->head_dim, cache->dtype, bf16, fa::host_sm_count(), st) != cudaSuccess)
+      return FA_ERR_LAUNCH;
+  }
+  return FA_OK;
 }
 
 int fa_kvcache_evict(const fa_paged_cache* cache, float* weights, long long w_seq_stride,

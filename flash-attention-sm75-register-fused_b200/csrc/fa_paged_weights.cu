@@ -6,12 +6,24 @@
 // with the LSE the attention returned, zero where row i does not see key j, added
 // to (or replacing) the sums of earlier calls.
 //
-// A warp takes 16 keys and multiplies them by blocks of 32 query rows (m16n8k16,
-// keys on M): S^T, one exponential per score, a sum over the rows.  Keys are
+// This file streams the keys for few query rows (decode, drafts);
+// fa_paged_weights_chunk.cuh takes chunks.  A warp multiplies 16 keys by its query rows
+// (m16n8k16, keys on M): S^T, one exponential per score, a sum over the rows.  Keys are
 // independent of one another, so nothing is joined between warps and no sum
 // depends on timing.  The columns of a row may come in any order as long as keys and
 // queries agree, so a lane reads its part of a key row with 16-byte loads straight
 // into the operand's registers.
+//
+// Bound by the keys' bytes.  All steps of 16 keys (32 of 8-bit pages) of the batch, in
+// order of sequence, head and key, are cut into equal runs, one per warp, whatever the
+// sequences' lengths.  A warp has its query rows in registers, the page ids of 32 groups of
+// 16 keys in one register a lane, loaded a window ahead, and the next step's keys on
+// their way while it computes this one's; nothing waits for another warp.
+//
+// Measured, 8 KV heads, d = 128, GQA 4: 16 sequences x 8192 keys of bf16 pages, one token,
+// 48.1 us (5.8 TB/s; a plain copy runs at 6.5; one CTA per 64 keys and 32 rows, with the queries
+// in shared memory, 82).  32 ragged sequences over int8 pages, 3 tokens, 26.7 us (3.6 TB/s: 290
+// instructions per 16 keys, a third of them widening, at half the issue rate).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -26,8 +38,6 @@ namespace fa {
 namespace {
 
 constexpr int kWeightThreads = 128;
-constexpr int kWeightRows = 32;                    // query rows of a block
-constexpr int kWeightKeys = kWeightThreads / 2;    // keys of a CTA
 
 template <bool BF16>
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -45,18 +55,6 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a
   }
 }
 
-// An f16 pair (of 8-bit values, which both types hold exactly) in the queries' type.
-template <bool BF16>
-__device__ __forceinline__ uint32_t as_query_type(uint32_t x) {
-  if constexpr (BF16) {
-    const float2 f = __half22float2(*reinterpret_cast<__half2*>(&x));
-    const __nv_bfloat162 v = __floats2bfloat162_rn(f.x, f.y);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  } else {
-    return x;
-  }
-}
-
 // Row r of (sequence, KV head): its packed token and query head.
 struct QueryRow {
   int tok, hq;
@@ -65,140 +63,9 @@ __device__ __forceinline__ QueryRow query_row(const PagedAttn& a, const Seq& s, 
   return {s.c0 + r / a.group, h * a.group + r % a.group};
 }
 
-template <int D, int KV, bool QBF16>
-__global__ void __launch_bounds__(kWeightThreads) paged_weights_kernel(const PagedWeights p, int n_blocks) {
-  constexpr bool k8 = KV >= FA_DTYPE_INT8;
-  constexpr int kRowBytes = k8 ? D : 2 * D;
-  constexpr int kChunks = kRowBytes / 64;          // 16-byte pieces of a lane per key
-  constexpr int kNT = kWeightRows / 8;
-  constexpr int kPitch = 2 * D + (k8 ? 16 : 64);   // bytes of a query row: no bank conflicts
-  const PagedAttn& a = p.a;
-  __shared__ __align__(16) uint8_t sh_q[kWeightRows * kPitch];
-  __shared__ float sh_lse[kWeightRows];
-  __shared__ int sh_lim[kWeightRows];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int g = lane >> 2, j = lane & 3;
-  const int b = static_cast<int>(blockIdx.x / n_blocks) / a.c.heads;
-  const int h = static_cast<int>(blockIdx.x / n_blocks) % a.c.heads;
-  const int cta_key0 = static_cast<int>(blockIdx.x % n_blocks) * kWeightKeys;
-  const Seq s = load_seq(a, b);
-  if (cta_key0 >= s.nk) return;
-  const int key0 = cta_key0 + warp * 16;
-  const int rows = s.nq * a.group;
-  // the new tokens' own positions, which have no earlier sum
-  const int fresh0 = p.mode == FA_WEIGHTS_SET      ? 0
-                     : p.mode == FA_WEIGHTS_APPEND ? min(__ldg(a.r.lens + b), 3 << 29) - s.n
-                                                   : 0x7fffffff;
-
-  // keys key0 + g, key0 + 8 + g: this lane's pieces
-  uint4 x[2][kChunks];
-  float ks[2] = {1.f, 1.f};
-  const int page = key0 < s.vis ? a.c.lookup(b, key0) : -1;
-#pragma unroll
-  for (int y = 0; y < 2; ++y) {
-    const int r = g + 8 * y;
-    const bool ok = page >= 0 && key0 + r < s.vis;
-    const long long row = a.c.row_in_page(key0) + r;
-    const uint8_t* src = a.c.k + page * a.c.page_stride + h * a.c.head_stride + row * a.c.row_stride;
-#pragma unroll
-    for (int c = 0; c < kChunks; ++c)
-      x[y][c] = ok ? __ldg(reinterpret_cast<const uint4*>(src + 64 * c) + j) : make_uint4(0u, 0u, 0u, 0u);
-    if constexpr (k8) ks[y] = ok ? __ldg(a.c.ks + page * a.c.s_page + h * a.c.s_head + row * a.c.s_row) : 0.f;
-  }
-
-  float sum[2] = {0.f, 0.f};
-  for (int r0 = 0; r0 < rows; r0 += kWeightRows) {
-    // (no row of the block sees a key of the CTA)
-    if (row_limit(a, s, (min(r0 + kWeightRows, rows) - 1) / a.group) <= cta_key0) continue;
-    __syncthreads();
-    for (int i = threadIdx.x; i < kWeightRows * (D / 8); i += kWeightThreads) {
-      const int r = i / (D / 8), c = i % (D / 8);
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (r0 + r < rows) {
-        const QueryRow q = query_row(a, s, h, r0 + r);
-        v = __ldg(reinterpret_cast<const uint4*>(a.q + q.tok * a.q_token + q.hq * a.q_head) + c);
-      }
-      *reinterpret_cast<uint4*>(sh_q + r * kPitch + 16 * c) = v;
-    }
-    if (threadIdx.x < kWeightRows) {
-      const int r = r0 + threadIdx.x;
-      float l = 0.f;
-      int lim = 0;
-      if (r < rows) {
-        const QueryRow q = query_row(a, s, h, r);
-        l = a.lse[static_cast<long long>(q.hq) * a.r.total + q.tok];
-        lim = l == -INFINITY ? 0 : row_limit(a, s, r / a.group);
-      }
-      sh_lse[threadIdx.x] = lim > 0 ? l * 1.4426950408889634f : 0.f;
-      sh_lim[threadIdx.x] = lim;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int nt = 0; nt < kNT; ++nt) {
-      float c[4] = {0.f, 0.f, 0.f, 0.f};
-      const uint8_t* qrow = sh_q + (nt * 8 + g) * kPitch;
-#pragma unroll
-      for (int i = 0; i < kChunks; ++i) {
-        const uint32_t k0[4] = {x[0][i].x, x[0][i].y, x[0][i].z, x[0][i].w};
-        const uint32_t k1[4] = {x[1][i].x, x[1][i].y, x[1][i].z, x[1][i].w};
-        if constexpr (!k8) {
-          const uint4 q = *reinterpret_cast<const uint4*>(qrow + 64 * i + 16 * j);
-          mma_16816<QBF16>(c, k0[0], k1[0], k0[1], k1[1], q.x, q.y);
-          mma_16816<QBF16>(c, k0[2], k1[2], k0[3], k1[3], q.z, q.w);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint4 q = *reinterpret_cast<const uint4*>(qrow + 128 * i + 32 * j + 16 * e);
-            uint32_t w0[4], w1[4];
-            widen<KV, false>(k0[2 * e], w0[0], w0[1]);
-            widen<KV, false>(k0[2 * e + 1], w0[2], w0[3]);
-            widen<KV, false>(k1[2 * e], w1[0], w1[1]);
-            widen<KV, false>(k1[2 * e + 1], w1[2], w1[3]);
-#pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              w0[y] = as_query_type<QBF16>(w0[y]);
-              w1[y] = as_query_type<QBF16>(w1[y]);
-            }
-            mma_16816<QBF16>(c, w0[0], w1[0], w0[1], w1[1], q.x, q.y);
-            mma_16816<QBF16>(c, w0[2], w1[2], w0[3], w1[3], q.z, q.w);
-          }
-        }
-      }
-#pragma unroll
-      for (int y = 0; y < 2; ++y)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int r = nt * 8 + 2 * j + e;
-          const float t = fmaf(c[2 * y + e], a.scale_log2 * ks[y], -sh_lse[r]);
-          if (key0 + g + 8 * y < sh_lim[r]) sum[y] += ptx::ex2_approx(t);
-        }
-    }
-  }
-#pragma unroll
-  for (int y = 0; y < 2; ++y) {
-    sum[y] += __shfl_xor_sync(0xffffffffu, sum[y], 1);
-    sum[y] += __shfl_xor_sync(0xffffffffu, sum[y], 2);
-    const int key = key0 + g + 8 * y;
-    if (j == 0 && key < s.nk) {
-      float* dst = p.w + b * p.w_seq + h * p.w_head + key;
-      *dst = key >= fresh0 ? sum[y] : *dst + sum[y];
-    }
-  }
-}
-
-// ---- few query rows (decode, drafts)
-//
-// Bound by the keys' bytes.  All steps of 16 keys (32 of 8-bit pages) of the batch, in
-// order of sequence, head and key, are cut into equal runs, one per warp, whatever the
-// sequences' lengths.  A warp has its query rows in registers, the page ids of 32 groups of
-// 16 keys in one register a lane, loaded a window ahead, and the next step's keys on
-// their way while it computes this one's; nothing waits for another warp.
-//
 // bf16 queries over 8-bit pages are taken as f16, q / 2^e with 2^e the size of
 // the row's largest element: bf16's 8 bits fit f16's 11, and elements below 2^-14 of
 // the largest lose at most 2^-25 of it, no more than the sum in fp32 does.
-constexpr int kRowsFew = 32;
-
 // Positions of the work order that a (sequence, head) takes besides its steps: its
 // queries, and the wait for its first keys.
 constexpr int kSegmentCost = 2;
@@ -239,7 +106,7 @@ __host__ __device__ constexpr int few_ctas_per_sm(int nt) { return nt == 1 ? 4 :
 
 template <int D, int KV, bool QBF16, int NT>
 __global__ void __launch_bounds__(kWeightThreads, few_ctas_per_sm(NT))
-    paged_weights_few_kernel(const PagedWeights p, int n_warps) {
+    paged_weights_few_kernel(const PagedWeights p, int max_rows, int n_warps) {
   using S = Stream<D, KV>;
   constexpr bool kBf16 = !S::k8 && QBF16;  // type of the products
   constexpr int kWarps = kWeightThreads / 32;
@@ -252,7 +119,9 @@ __global__ void __launch_bounds__(kWeightThreads, few_ctas_per_sm(NT))
   __shared__ long long sh_scan[kWarps];
   __shared__ int sh_b[kWarps];
   __shared__ long long sh_rel[kWarps];
-  auto steps_of = [&](const Seq& s) { return (s.nk + S::kKeys - 1) / S::kKeys; };
+  auto steps_of = [&](const Seq& s) {
+    return static_cast<long long>(s.nq) * a.group > max_rows ? 0 : (s.nk + S::kKeys - 1) / S::kKeys;
+  };
   auto positions = [&](int b) -> long long {
     const int n = steps_of(load_seq(a, b));
     return n > 0 ? static_cast<long long>(n + kSegmentCost) * H : 0;
@@ -502,13 +371,13 @@ __global__ void __launch_bounds__(kWeightThreads, few_ctas_per_sm(NT))
       do {
         if (++b >= a.r.B) return;
         s = load_seq(a, b);
-      } while (s.nk <= 0);
+      } while (steps_of(s) == 0);
     }
   }
 }
 
 template <int D, int KV, bool QBF16, int NT>
-cudaError_t few_impl(const PagedWeights& p, int sms, cudaStream_t stream) {
+cudaError_t few_impl(const PagedWeights& p, int max_rows, int sms, cudaStream_t stream) {
   using S = Stream<D, KV>;
   constexpr int kWarps = kWeightThreads / 32;
   // no more warps than steps there can be
@@ -517,42 +386,35 @@ cudaError_t few_impl(const PagedWeights& p, int sms, cudaStream_t stream) {
   const long long most = static_cast<long long>(sms) * few_ctas_per_sm(NT);
   const long long ctas = (steps + kWarps - 1) / kWarps;
   const int grid = static_cast<int>(ctas < most ? ctas : most);
-  paged_weights_few_kernel<D, KV, QBF16, NT><<<grid, kWeightThreads, 0, stream>>>(p, grid * kWarps);
+  paged_weights_few_kernel<D, KV, QBF16, NT><<<grid, kWeightThreads, 0, stream>>>(p, max_rows, grid * kWarps);
   return cudaGetLastError();
 }
 
 template <int D, int KV, bool QBF16>
-cudaError_t weights_impl(const PagedWeights& p, int sms, cudaStream_t stream) {
-  const long long rows = static_cast<long long>(p.a.max_q < p.a.r.total ? p.a.max_q : p.a.r.total) * p.a.group;
-  if (rows <= 8) return few_impl<D, KV, QBF16, 1>(p, sms, stream);
-  if (rows <= 16) return few_impl<D, KV, QBF16, 2>(p, sms, stream);
-  if (rows <= kRowsFew) return few_impl<D, KV, QBF16, 4>(p, sms, stream);
-  const int n_blocks = (p.a.max_k + kWeightKeys - 1) / kWeightKeys;
-  const long long grid = static_cast<long long>(n_blocks) * p.a.r.B * p.a.c.heads;
-  if (grid > 0x7fffffffLL) return cudaErrorInvalidValue;
-  if (grid == 0) return cudaSuccess;
-  paged_weights_kernel<D, KV, QBF16><<<static_cast<unsigned>(grid), kWeightThreads, 0, stream>>>(p, n_blocks);
-  return cudaGetLastError();
+cudaError_t weights_impl(const PagedWeights& p, int max_rows, int sms, cudaStream_t stream) {
+  if (max_rows <= 8) return few_impl<D, KV, QBF16, 1>(p, max_rows, sms, stream);
+  if (max_rows <= 16) return few_impl<D, KV, QBF16, 2>(p, max_rows, sms, stream);
+  return few_impl<D, KV, QBF16, 4>(p, max_rows, sms, stream);
 }
 
 template <int D>
-cudaError_t weights_d(const PagedWeights& p, int kv, bool bf16, int sms, cudaStream_t s) {
+cudaError_t weights_d(const PagedWeights& p, int n, int kv, bool bf16, int sms, cudaStream_t s) {
   switch (kv) {
     case FA_DTYPE_INT8:
-      return bf16 ? weights_impl<D, FA_DTYPE_INT8, true>(p, sms, s) : weights_impl<D, FA_DTYPE_INT8, false>(p, sms, s);
+      return bf16 ? weights_impl<D, FA_DTYPE_INT8, true>(p, n, sms, s) : weights_impl<D, FA_DTYPE_INT8, false>(p, n, sms, s);
     case FA_DTYPE_E4M3:
-      return bf16 ? weights_impl<D, FA_DTYPE_E4M3, true>(p, sms, s) : weights_impl<D, FA_DTYPE_E4M3, false>(p, sms, s);
-    case FA_DTYPE_BF16: return weights_impl<D, FA_DTYPE_BF16, true>(p, sms, s);
-    default: return weights_impl<D, FA_DTYPE_F16, false>(p, sms, s);
+      return bf16 ? weights_impl<D, FA_DTYPE_E4M3, true>(p, n, sms, s) : weights_impl<D, FA_DTYPE_E4M3, false>(p, n, sms, s);
+    case FA_DTYPE_BF16: return weights_impl<D, FA_DTYPE_BF16, true>(p, n, sms, s);
+    default: return weights_impl<D, FA_DTYPE_F16, false>(p, n, sms, s);
   }
 }
 
 }  // namespace
 
-cudaError_t launch_paged_weights(const PagedWeights& p, int head_dim, int cache_dtype, bool bf16, int sms,
+cudaError_t launch_paged_weights(const PagedWeights& p, int max_rows, int head_dim, int cache_dtype, bool bf16, int sms,
                                  cudaStream_t stream) {
-  return head_dim == 64 ? weights_d<64>(p, cache_dtype, bf16, sms, stream)
-                        : weights_d<128>(p, cache_dtype, bf16, sms, stream);
+  return head_dim == 64 ? weights_d<64>(p, max_rows, cache_dtype, bf16, sms, stream)
+                        : weights_d<128>(p, max_rows, cache_dtype, bf16, sms, stream);
 }
 
 }  // namespace fa
