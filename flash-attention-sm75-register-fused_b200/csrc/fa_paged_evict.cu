@@ -8,13 +8,14 @@
 //   select  The weight of the last one that stays, by radix selection over
 //           order-preserving integers, 11 bits a pass, without a sort: every CTA counts
 //           its positions in shared memory, and all add up the cluster's counts.
-//   place   The cluster walks the positions, 1024 per CTA and step; two ranks (of
+//   place   The cluster walks the positions, 2048 per CTA and step; two ranks (of
 //           equal weights, of what stays) and the CTAs' counts give every kept one
-//           its place, and its position goes to the CTA that moves that place.
-//   move    Places in ascending order, as many at a time as the cluster holds in
-//           registers: all are loaded before any is stored, and as the i-th kept
-//           position is at least i, nothing is overwritten that a later group reads.
-// Bound by memory: the weights are read once (the first kCacheSteps x 1024 of a CTA stay in
+//           its place, and its page and row go to the list of the CTA that moves it.
+//   move    Places in ascending order, a group at a time: all of a group are loaded
+//           before any is stored, and as the i-th kept position is at least i, nothing
+//           is overwritten that a later group reads.  So the next group's loads are on
+//           their way while this one is stored.
+// Bound by memory: the weights are read once (the first kCacheSteps x 2048 of a CTA stay in
 // shared memory), rows that move are read and written once.  @@
 #include <cuda_runtime.h>
 
@@ -26,10 +27,14 @@
 namespace fa {
 namespace {
 
-constexpr int kEvictThreads = 1024;
+constexpr int kEvictThreads = 512;
 constexpr int kBins = 2048;
-constexpr int kCacheSteps = 16;
+constexpr int kEach = 4;                          // positions of a thread and step
+constexpr int kChunk = kEach * kEvictThreads;     // ... of a CTA
+constexpr int kCacheSteps = 6;
+constexpr int kList = 4096;                       // places of a CTA
 constexpr int kMaxCluster = 8;
+constexpr long long kClusterLoad = 4;
 
 // Integer that orders as the weights do: -0 as 0, a NaN below all.
 __device__ __forceinline__ uint32_t order_key(float f) {
@@ -38,10 +43,19 @@ __device__ __forceinline__ uint32_t order_key(float f) {
   return u ^ (static_cast<uint32_t>(static_cast<int>(u) >> 31) | 0x80000000u);
 }
 
-__device__ __forceinline__ int load_cluster(const void* p, int rank) {
-  int x;
-  asm volatile("ld.shared::cluster.s32 %0, [%1];"
-               : "=r"(x)
+// From and to the shared memory of another CTA of the cluster.
+__device__ __forceinline__ int4 load_cluster4(const void* p, int rank) {
+  int4 x;
+  asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+               : "r"(ptx::mapa(ptx::smem_u32(p), static_cast<uint32_t>(rank)))
+               : "memory");
+  return x;
+}
+__device__ __forceinline__ int2 load_cluster2(const void* p, int rank) {
+  int2 x;
+  asm volatile("ld.shared::cluster.v2.s32 {%0,%1}, [%2];"
+               : "=r"(x.x), "=r"(x.y)
                : "r"(ptx::mapa(ptx::smem_u32(p), static_cast<uint32_t>(rank)))
                : "memory");
   return x;
@@ -51,7 +65,7 @@ __device__ __forceinline__ void store_cluster(const void* p, int rank, int x) {
                : "memory");
 }
 
-// Sum of `x` over the block's threads before this one; *total over all.  sh: 32 entries.
+// Sum of `x` over the block's threads before this one; *total over all.  sh: one entry a warp.
 __device__ __forceinline__ int block_sum_before(int x, int* sh, int* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int incl = x;
@@ -62,7 +76,7 @@ __device__ __forceinline__ int block_sum_before(int x, int* sh, int* total) {
   }
   if (lane == 31) sh[warp] = incl;
   __syncthreads();
-  const int mine = sh[lane];
+  const int mine = lane < kEvictThreads / 32 ? sh[lane] : 0;
   int all = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -75,13 +89,19 @@ __device__ __forceinline__ int block_sum_before(int x, int* sh, int* total) {
   return before + incl - x;
 }
 
-template <int RB, bool kScales>
-__global__ void __launch_bounds__(kEvictThreads) paged_evict_kernel(const PagedEvict p, int C) {
-  extern __shared__ float cache[];  // [kCacheSteps][kEvictThreads]
-  __shared__ int sh_hist[2][kBins];
-  __shared__ int sh_list[kEvictThreads];
+struct Source {
+  int page, row;  // page -1: none
+};
+
+// kUnits: rows of a thread in a group.
+template <int RB, bool kScales, int kUnits>
+__global__ void __launch_bounds__(kEvictThreads, kUnits == 2 ? 2 : 1) paged_evict_kernel(const PagedEvict p, int C) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  Source* const list = reinterpret_cast<Source*>(smem_raw);                    // [kList]
+  float* const cache = reinterpret_cast<float*>(smem_raw + kList * sizeof(Source));  // [kCacheSteps][kChunk]
+  __shared__ __align__(16) int sh_hist[2][kBins];
   __shared__ int sh_warp[32];
-  __shared__ int sh_count[2][2];
+  __shared__ __align__(8) int sh_count[2][2];
   __shared__ int sh_bin, sh_want;
   const int tid = threadIdx.x;
   const int rank = static_cast<int>(blockIdx.x) % C, item = static_cast<int>(blockIdx.x) / C;
@@ -93,18 +113,36 @@ __global__ void __launch_bounds__(kEvictThreads) paged_evict_kernel(const PagedE
   const int first = min(p.first, keep), recent = min(p.recent, keep - first);
   const int lo = first, hi = n - recent;
   float* const w = p.w + b * p.w_seq + h * p.w_head;
-  // positions of step s: [s P, (s + 1) P), this CTA's from s P + 1024 rank
-  const int P = C * kEvictThreads;
+  // Up to kChunk positions every CTA selects by itself, and the cluster shares the move alone.
+  const bool alone = n <= kChunk;
+  const int R = alone ? 1 : C, me = alone ? 0 : rank;
+  auto sync_select = [&] {
+    if (alone) __syncthreads();
+    else ptx::cluster_sync();
+  };
+  // positions of step s: [s P, (s + 1) P), this CTA's from s P + me kChunk, a thread's four of them
+  const int P = R * kChunk;
   const int n_steps = (n - 1) / P + 1;
-  auto pos_of = [&](int s) { return s * P + rank * kEvictThreads + tid; };
-  for (int s = 0; s < n_steps && s < kCacheSteps; ++s) {
-    const int pos = pos_of(s);
-    cache[s * kEvictThreads + tid] = pos < n ? __ldcg(w + pos) : 0.f;
-  }
-  auto weight = [&](int s) {  // (a thread reads back its own)
-    if (s < kCacheSteps) return cache[s * kEvictThreads + tid];
-    const int pos = pos_of(s);
-    return pos < n ? __ldcg(w + pos) : 0.f;
+  auto pos_of = [&](int s) { return s * P + me * kChunk + kEach * tid; };
+  for (int s = 0; s < n_steps && s < kCacheSteps; ++s)
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int x = i * kEvictThreads + tid, pos = s * P + me * kChunk + x;
+      cache[s * kChunk + x] = pos < n ? __ldcg(w + pos) : 0.f;
+    }
+  if (alone) ptx::cluster_sync();  // (all have read the weights that the first one moves)
+  else __syncthreads();
+  auto weights = [&](int s, float (&x)[kEach]) {
+    if (s < kCacheSteps) {
+      const float4 v = *reinterpret_cast<const float4*>(cache + s * kChunk + kEach * tid);
+      x[0] = v.x;
+      x[1] = v.y;
+      x[2] = v.z;
+      x[3] = v.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) x[i] = pos_of(s) + i < n ? __ldcg(w + pos_of(s) + i) : 0.f;
+    }
   };
 
   // ---- the smallest key that stays, and how many of that value do
@@ -117,27 +155,46 @@ __global__ void __launch_bounds__(kEvictThreads) paged_evict_kernel(const PagedE
       const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
       const uint32_t digit = pass == 2 ? 1023u : 2047u;
       int* const hist = sh_hist[pass & 1];
-      hist[tid] = hist[kEvictThreads + tid] = 0;
+#pragma unroll
+      for (int i = tid; i < kBins; i += kEvictThreads) hist[i] = 0;
       __syncthreads();
       for (int s = 0; s < n_steps; ++s) {
-        const int pos = pos_of(s);
-        const uint32_t u = order_key(weight(s));
-        if (pos >= lo && pos < hi && (u & mask) == key) atomicAdd(&hist[(u >> shift) & digit], 1);
+        float x[kEach];
+        weights(s, x);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+          const int pos = pos_of(s) + i;
+          const uint32_t u = order_key(x[i]);
+          if (pos >= lo && pos < hi && (u & mask) == key) atomicAdd(&hist[(u >> shift) & digit], 1);
+        }
       }
-      ptx::cluster_sync();
-      // thread t has bins 2047 - 2 t and 2046 - 2 t: from the top down
-      int c0 = 0, c1 = 0;
-      const int bin = kBins - 1 - 2 * tid;
-      for (int r = 0; r < C; ++r) {
-        c0 += load_cluster(&hist[bin], r);
-        c1 += load_cluster(&hist[bin - 1], r);
+      sync_select();
+      // thread t has the four bins from 2047 - 4 t down
+      static_assert(kBins == 4 * kEvictThreads, "bins of a thread");
+      const int bin = kBins - 1 - 4 * tid;
+      int4 part[kMaxCluster];
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; ++r)
+        part[r] = r < R ? load_cluster4(&hist[bin - 3], alone ? rank : r) : make_int4(0, 0, 0, 0);
+      int c[4] = {}, sum = 0;
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; ++r) {
+        c[0] += part[r].w;
+        c[1] += part[r].z;
+        c[2] += part[r].y;
+        c[3] += part[r].x;
       }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum += c[i];
       int total;
-      const int before = block_sum_before(c0 + c1, sh_warp, &total);
-      if (before < want && before + c0 + c1 >= want) {
-        const bool second = before + c0 < want;
-        sh_bin = second ? bin - 1 : bin;
-        sh_want = want - before - (second ? c0 : 0);
+      int before = block_sum_before(sum, sh_warp, &total);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (before < want && before + c[i] >= want) {
+          sh_bin = bin - i;
+          sh_want = want - before;
+        }
+        before += c[i];
       }
       __syncthreads();
       key |= static_cast<uint32_t>(sh_bin) << shift;
@@ -149,119 +206,168 @@ __global__ void __launch_bounds__(kEvictThreads) paged_evict_kernel(const PagedE
 
   // ---- the places of what stays, and the move
   constexpr int kLanes = RB / 16;                         // threads of a row
-  constexpr int kUnits = 2;                               // rows of a thread in flight
-  constexpr int kRows = kUnits * kEvictThreads / kLanes;  // ... of a CTA
-  static_assert(kRows <= kEvictThreads, "list");
+  constexpr int kStride = kEvictThreads / kLanes;         // rows of a unit
+  constexpr int kRows = kUnits * kStride;                 // ... of a group, in a CTA
+  static_assert(kList % kRows == 0, "list");
   const int W = C * kRows;
+  const int part = tid % kLanes;
   int kept = 0, ties = 0;  // in the steps before
-  for (int s = 0; s < n_steps && kept < keep; ++s) {
-    const int pos = pos_of(s);
-    const float wt = weight(s);
-    const uint32_t u = order_key(wt);
-    const bool sure = pos < n && (pos < lo || pos >= hi || u > key);
-    const bool tie = pos >= lo && pos < hi && u == key;
-    // both counts in one scan
-    int both;
-    const int before = block_sum_before((sure ? 1 : 0) | (tie ? 1 << 16 : 0), sh_warp, &both);
-    if (tid == 0) {
-      sh_count[s & 1][0] = both & 0xffff;
-      sh_count[s & 1][1] = both >> 16;
-    }
-    ptx::cluster_sync();
-    int base = 0, mine = 0, n_step = 0, tie_at = ties;  // kept before this CTA, ties before it
-    int t = ties;
-    for (int r = 0; r < C; ++r) {
-      const int g = load_cluster(&sh_count[s & 1][0], r), e = load_cluster(&sh_count[s & 1][1], r);
-      if (r == rank) {
-        tie_at = t;
-        base = n_step;
+  for (int s = 0; s < n_steps && kept < keep;) {
+    // places kept .. of the next steps, as many as the lists take
+    int place0 = kept, filled = 0;
+    for (; s < n_steps && kept < keep && filled + P <= C * kList; ++s) {
+      const int pos0 = pos_of(s);
+      float x[kEach];
+      weights(s, x);
+      unsigned sure = 0, tie = 0;  // bit i: position pos0 + i
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const int pos = pos0 + i;
+        const uint32_t u = order_key(x[i]);
+        const bool between = pos >= lo && pos < hi;
+        sure |= (pos < n && (!between || u > key) ? 1u : 0u) << i;
+        tie |= (between && u == key ? 1u : 0u) << i;
       }
-      n_step += g + min(max(want - t, 0), e);
-      t += e;
-    }
-    mine = tie_at + (before >> 16);  // equal weights before this one
-    const bool stays = sure || (tie && mine < want);
-    // kept ones of this CTA before it: the sure ones, and the ties that stay
-    const int q = base + (before & 0xffff) + min(max(want - tie_at, 0), before >> 16);
-    const bool still = kept == s * P && n_step == min(P, n - s * P);  // nothing has moved so far
-    if (stays && !still) {
-      const int sub = q / W, in = q % W;
-      store_cluster(&sh_list[sub * kRows + in % kRows], in / kRows, pos);
-      w[kept + q] = wt;
+      // both counts in one scan
+      int both;
+      const int before = block_sum_before(__popc(sure) | __popc(tie) << 16, sh_warp, &both);
+      if (tid == 0) {
+        sh_count[s & 1][0] = both & 0xffff;
+        sh_count[s & 1][1] = both >> 16;
+      }
+      sync_select();
+      // lane r has CTA r's counts; prefix sums over the lanes
+      const int lane = tid & 31;
+      const int2 counts = lane < R ? load_cluster2(sh_count[s & 1], alone ? rank : lane) : make_int2(0, 0);
+      auto prefix = [&](int x) {
+#pragma unroll
+        for (int o = 1; o < kMaxCluster; o <<= 1) {
+          const int up = __shfl_up_sync(0xffffffffu, x, o);
+          if (lane >= o) x += up;
+        }
+        return x;
+      };
+      const int ties_end = ties + prefix(counts.y);
+      const int stay = counts.x + min(max(want - (ties_end - counts.y), 0), counts.y);
+      const int stay_end = prefix(stay);
+      const int n_step = __shfl_sync(0xffffffffu, stay_end, kMaxCluster - 1);
+      const int base = __shfl_sync(0xffffffffu, stay_end - stay, me);          // kept, equal weights
+      const int tie_at = __shfl_sync(0xffffffffu, ties_end - counts.y, me);  // before this CTA
+      ties = __shfl_sync(0xffffffffu, ties_end, kMaxCluster - 1);
+      if (filled == 0 && kept == s * P && n_step == min(P, n - s * P)) {  // nothing has moved so far
+        kept += n_step;
+        place0 = kept;
+        continue;
+      }
+      const int left = max(want - tie_at, 0);  // equal weights of this CTA that stay
+      int q = filled + base + (before & 0xffff) + min(left, before >> 16), rest = left - (before >> 16);
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) {
+        const bool t = (tie >> i) & 1u;
+        if (((sure >> i) & 1u) || (t && rest > 0)) {
+          const int in = q % W, to = in / kRows;
+          Source* const at = &list[q / W * kRows + in % kRows];
+          if (!alone || to == rank) {
+            store_cluster(&at->page, to, p.c.lookup(b, pos0 + i));
+            store_cluster(&at->row, to, p.c.row_in_page(pos0 + i));
+          }
+          if (!alone || rank == 0) w[place0 + q] = x[i];
+          ++q;
+        }
+        if (t) --rest;
+      }
+      filled += n_step;
+      kept += n_step;
     }
     ptx::cluster_sync();
-    for (int q0 = 0; q0 < n_step && !still; q0 += W) {
+
+    struct Group {
       uint4 k[kUnits], v[kUnits];
       float ks[kUnits], vs[kUnits];
       int to[kUnits];
+    };
+    auto load = [&](Group& x, int q0) {
 #pragma unroll
-      for (int x = 0; x < kUnits; ++x) {
-        const int r = x * (kEvictThreads / kLanes) + tid / kLanes, part = tid % kLanes;
-        const int place = q0 + rank * kRows + r;
-        const int src = place < n_step ? sh_list[q0 / C + r] : 0;
-        to[x] = place < n_step && src != kept + place ? p.c.lookup(b, kept + place) : -1;
-        const int from = to[x] >= 0 ? p.c.lookup(b, src) : -1;
-        k[x] = v[x] = make_uint4(0u, 0u, 0u, 0u);
-        ks[x] = vs[x] = 0.f;
-        if (from >= 0) {
-          const long long row = p.c.row_in_page(src);
-          const long long o = from * p.c.page_stride + h * p.c.head_stride + row * p.c.row_stride;
-          k[x] = __ldcg(reinterpret_cast<const uint4*>(p.c.k + o) + part);
-          v[x] = __ldcg(reinterpret_cast<const uint4*>(p.c.v + o) + part);
-          if (kScales && part == 0) {
-            const long long so = from * p.c.s_page + h * p.c.s_head + row * p.c.s_row;
-            ks[x] = __ldcg(p.c.ks + so);
-            vs[x] = __ldcg(p.c.vs + so);
+      for (int i = 0; i < kUnits; ++i) {
+        const int r = i * kStride + tid / kLanes, q = q0 + rank * kRows + r;
+        x.to[i] = -1;
+        x.k[i] = x.v[i] = make_uint4(0u, 0u, 0u, 0u);
+        x.ks[i] = x.vs[i] = 0.f;
+        if (q < filled) {
+          const Source src = list[q0 / C + r];
+          x.to[i] = p.c.lookup(b, place0 + q);
+          if (src.page >= 0) {
+            const long long o = src.page * p.c.page_stride + h * p.c.head_stride + src.row * p.c.row_stride;
+            x.k[i] = __ldcg(reinterpret_cast<const uint4*>(p.c.k + o) + part);
+            x.v[i] = __ldcg(reinterpret_cast<const uint4*>(p.c.v + o) + part);
+            if (kScales && part == 0) {
+              const long long so = src.page * p.c.s_page + h * p.c.s_head + src.row * p.c.s_row;
+              x.ks[i] = __ldcg(p.c.ks + so);
+              x.vs[i] = __ldcg(p.c.vs + so);
+            }
           }
         }
       }
-      ptx::cluster_sync();
+    };
+    auto store = [&](const Group& x, int q0) {
 #pragma unroll
-      for (int x = 0; x < kUnits; ++x) {
-        if (to[x] < 0) continue;
-        const int r = x * (kEvictThreads / kLanes) + tid / kLanes, part = tid % kLanes;
-        const long long row = p.c.row_in_page(kept + q0 + rank * kRows + r);
-        const long long o = to[x] * p.c.page_stride + h * p.c.head_stride + row * p.c.row_stride;
-        reinterpret_cast<uint4*>(const_cast<uint8_t*>(p.c.k) + o)[part] = k[x];
-        reinterpret_cast<uint4*>(const_cast<uint8_t*>(p.c.v) + o)[part] = v[x];
+      for (int i = 0; i < kUnits; ++i) {
+        if (x.to[i] < 0) continue;
+        const int row = p.c.row_in_page(place0 + q0 + rank * kRows + i * kStride + tid / kLanes);
+        const long long o = x.to[i] * p.c.page_stride + h * p.c.head_stride + row * p.c.row_stride;
+        reinterpret_cast<uint4*>(const_cast<uint8_t*>(p.c.k) + o)[part] = x.k[i];
+        reinterpret_cast<uint4*>(const_cast<uint8_t*>(p.c.v) + o)[part] = x.v[i];
         if (kScales && part == 0) {
-          const long long so = to[x] * p.c.s_page + h * p.c.s_head + row * p.c.s_row;
-          p.c.ks[so] = ks[x];
-          p.c.vs[so] = vs[x];
+          const long long so = x.to[i] * p.c.s_page + h * p.c.s_head + row * p.c.s_row;
+          p.c.ks[so] = x.ks[i];
+          p.c.vs[so] = x.vs[i];
         }
       }
+    };
+    // (the compiler may not wait for a load before the barrier: what it returns is pinned)
+    auto landed = [&](Group& x) {
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i)
+        asm volatile("" : "+r"(x.k[i].x), "+r"(x.k[i].y), "+r"(x.k[i].z), "+r"(x.k[i].w), "+r"(x.v[i].x),
+                          "+r"(x.v[i].y), "+r"(x.v[i].z), "+r"(x.v[i].w), "+f"(x.ks[i]), "+f"(x.vs[i]));
+    };
+    Group x, y;
+    if (filled > 0) load(x, 0);
+    for (int q0 = 0; q0 < filled; q0 += 2 * W) {
+      load(y, q0 + W);
+      landed(x);
+      ptx::cluster_sync();
+      store(x, q0);
+      if (q0 + W >= filled) break;
+      load(x, q0 + 2 * W);
+      landed(y);
+      ptx::cluster_sync();
+      store(y, q0 + W);
     }
-    kept += n_step;
-    ties = t;
   }
   ptx::cluster_sync();  // (nobody reads the shared memory of a CTA that is gone)
 }
 
-template <int RB, bool kScales>
-cudaError_t evict_impl(const PagedEvict& p, int sms, cudaStream_t stream) {
-  auto kern = paged_evict_kernel<RB, kScales>;
-  constexpr int kDyn = kCacheSteps * kEvictThreads * static_cast<int>(sizeof(float));
+template <int RB, bool kScales, int kUnits>
+cudaError_t evict_units(const PagedEvict& p, int C, cudaStream_t stream) {
+  auto kern = paged_evict_kernel<RB, kScales, kUnits>;
+  constexpr int kListBytes = kList * static_cast<int>(sizeof(Source));
+  constexpr int kStepBytes = kChunk * static_cast<int>(sizeof(float));
   static int attr_done[64] = {0};
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !attr_done[dev]) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kDyn);
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               kListBytes + kCacheSteps * kStepBytes);
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) attr_done[dev] = 1;
   }
-  // CTAs of a cluster: as many as there are SMs and positions for
-  const long long items = static_cast<long long>(p.B) * p.c.heads;
-  const long long held = static_cast<long long>(p.c.max_pages) * p.c.page_size;
-  int C = 1;
-  while (C < kMaxCluster && items * 2 * C <= sms && held > static_cast<long long>(C) * kEvictThreads) C *= 2;
-  if (items * C > 0x7fffffffLL) return cudaErrorInvalidValue;
+  const long long P = static_cast<long long>(C) * kChunk;
+  const long long steps = (static_cast<long long>(p.c.max_pages) * p.c.page_size + P - 1) / P;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(items * C));
+  cfg.gridDim = dim3(static_cast<unsigned>(static_cast<long long>(p.B) * p.c.heads * C));
   cfg.blockDim = dim3(kEvictThreads);
-  cfg.dynamicSmemBytes = static_cast<size_t>(
-      sizeof(float) * kEvictThreads * (held > static_cast<long long>(C) * kEvictThreads * kCacheSteps
-                                           ? kCacheSteps
-                                           : (held + C * kEvictThreads - 1) / (C * kEvictThreads)));
+  cfg.dynamicSmemBytes = static_cast<size_t>(kListBytes + kStepBytes * (steps < kCacheSteps ? steps : kCacheSteps));
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -270,6 +376,16 @@ cudaError_t evict_impl(const PagedEvict& p, int sms, cudaStream_t stream) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kern, p, C);
+}
+
+template <int RB, bool kScales>
+cudaError_t evict_impl(const PagedEvict& p, int sms, cudaStream_t stream) {
+  const long long items = static_cast<long long>(p.B) * p.c.heads;
+  const long long held = static_cast<long long>(p.c.max_pages) * p.c.page_size;
+  int C = 1;
+  while (C < kMaxCluster && items * 2 * C <= kClusterLoad * sms && held > 128LL * C) C *= 2;
+  if (items * C > 0x7fffffffLL) return cudaErrorInvalidValue;
+  return items * C <= sms ? evict_units<RB, kScales, 4>(p, C, stream) : evict_units<RB, kScales, 2>(p, C, stream);
 }
 
 }  // namespace
