@@ -90,7 +90,7 @@ __device__ __forceinline__ int block_sum_before(int x, int* sh, int* total) {
 }
 
 struct Source {
-  int page, row;  // page -1: none
+  int page, pos;  // page -1: none
 };
 
 // kUnits: rows of a thread in a group.
@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(kEvictThreads, kUnits == 2 ? 2 : 1) paged_evic
           Source* const at = &list[q / W * kRows + in % kRows];
           if (!alone || to == rank) {
             store_cluster(&at->page, to, p.c.lookup(b, pos0 + i));
-            store_cluster(&at->row, to, p.c.row_in_page(pos0 + i));
+            store_cluster(&at->pos, to, pos0 + i);
           }
           if (!alone || rank == 0) w[place0 + q] = x[i];
           ++q;
@@ -295,13 +295,15 @@ __global__ void __launch_bounds__(kEvictThreads, kUnits == 2 ? 2 : 1) paged_evic
         x.ks[i] = x.vs[i] = 0.f;
         if (q < filled) {
           const Source src = list[q0 / C + r];
+          if (src.pos == place0 + q) continue;  // (nothing before it went)
           x.to[i] = p.c.lookup(b, place0 + q);
           if (src.page >= 0) {
-            const long long o = src.page * p.c.page_stride + h * p.c.head_stride + src.row * p.c.row_stride;
+            const int row = p.c.row_in_page(src.pos);
+            const long long o = src.page * p.c.page_stride + h * p.c.head_stride + row * p.c.row_stride;
             x.k[i] = __ldcg(reinterpret_cast<const uint4*>(p.c.k + o) + part);
             x.v[i] = __ldcg(reinterpret_cast<const uint4*>(p.c.v + o) + part);
             if (kScales && part == 0) {
-              const long long so = src.page * p.c.s_page + h * p.c.s_head + src.row * p.c.s_row;
+              const long long so = src.page * p.c.s_page + h * p.c.s_head + row * p.c.s_row;
               x.ks[i] = __ldcg(p.c.ks + so);
               x.vs[i] = __ldcg(p.c.vs + so);
             }
