@@ -64,14 +64,29 @@ struct PagedAttn {
   int max_q, max_k;
   int causal;                 // FA_CAUSAL_*
   float scale_log2;           // scale * log2(e)
-  // Attention over two sets of keys in two passes: the first stores its results here
-  // as fp32 (part = kPartFirst; o and lse are not used), the second joins its own
-  // with them (kPartSecond).
+  // Attention over two sets of keys in two passes: where its results go, and (kPartJoin)
+  // the first pass's, which they are joined with.
   int part;                   // kPart*
   float* part_o;              // [total, Hq, d]
   float* part_lse;            // [total, Hq], natural log
 };
-enum { kPartNone = 0, kPartFirst = 1, kPartSecond = 2 };
+// kPartNone: o and lse.  kPartFirst, kPartSecond: part_o and part_lse, as fp32; rows that
+// no kernel computes get O = 0 and LSE = -inf, in the second pass kNoRow.  kPartJoin: o and
+// lse, joined with part_o and part_lse (chunk kernel alone).
+enum { kPartNone = 0, kPartFirst = 1, kPartSecond = 2, kPartJoin = 3 };
+constexpr unsigned kNoRow = 0x7fffdeadu;  // bits of an LSE: the row belongs to no sequence
+
+// Joins the rows of two passes (fa_paged_merge.cu).
+struct PagedMerge {
+  const float* o1;
+  const float* lse1;
+  const float* o2;
+  const float* lse2;
+  void* o;      // [total, Hq, d]
+  float* lse;   // [Hq, total] or nullptr
+  int total, Hq;
+};
+cudaError_t launch_paged_merge(const PagedMerge& p, int head_dim, bool bf16, cudaStream_t stream);
 
 // An item of the chunk kernel that the end of a run cuts: its sequence's first row
 // and tokens, its first token, KV head and parts (0: none is cut).
@@ -170,6 +185,7 @@ struct alignas(64) DecodeParams {
   // head), ring stages per warp
   int n_teams, solo, stages;
   int max_rows;  // query rows per KV head of the sequences handled
+  int early;     // may run beside the kernels before it, whose results it does not read; ends after them
   unsigned epoch;
   unsigned long long timeout_ns;
 };

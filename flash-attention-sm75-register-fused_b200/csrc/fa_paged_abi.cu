@@ -373,9 +373,16 @@ size_t part_bytes(int total, int Hq, int head_dim) {
   return (static_cast<size_t>(total) * Hq * (head_dim + 1) * sizeof(float) + 127) / 128 * 128;
 }
 
-// The kernels of one pass.
+// Of two passes over chunks alone the second joins its rows with the first's as it writes them
+// (4096 tokens, 32 heads: @@).  A kernel that ends many short segments would wait there for what it reads
+// (64 tokens over 64 sequences: 60 us instead of 30 for the pass), so its results go to the
+// workspace and a kernel of its own joins them.
+bool joins_itself(const PagedPlan& k) { return k.chunk && !k.decode; }
+
+// The kernels of one pass.  `early`: it may start while the kernels before it end.
 int run_paged(const fa::PagedAttn& a, const fa_paged_cache& cache, const PagedPlan& k, const void* Q,
-              long long q_token_stride, long long q_head_stride, int dtype, void* workspace, void* stream) {
+              long long q_token_stride, long long q_head_stride, int dtype, void* workspace, void* stream,
+              bool early = false) {
   const bool eight = is_8bit(cache.dtype);
   const bool bf16 = dtype == FA_DTYPE_BF16;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -384,6 +391,7 @@ int run_paged(const fa::PagedAttn& a, const fa_paged_cache& cache, const PagedPl
     p.a = a;
     p.ws = static_cast<float*>(workspace);
     p.max_rows = k.decode_rows;
+    p.early = early ? 1 : 0;
     p.epoch = fa::host_next_epoch();
     p.timeout_ns = fa::host_timeout_ns();
     if (!page_maps(cache, 16, &p)) return FA_ERR_TENSOR_MAP;
@@ -516,11 +524,11 @@ size_t fa_fwd_paged_prefix_workspace_bytes(const fa_paged_cache* cache, int n_pr
       !sizes_ok(cache, n_prefixes, Hq, total_q, max_prefix_q, max_prefix_k))
     return 0;
   const int group = Hq / cache->kv_heads;
-  const size_t first = make_paged_plan(n_prefixes, cache->kv_heads, group, cache->head_dim, cache->dtype,
-                                       total_q, max_prefix_q, max_prefix_k).ws_bytes;
-  const size_t second = make_paged_plan(B, cache->kv_heads, group, cache->head_dim, cache->dtype, total_q,
-                                        max_seqlen_q, max_seqlen_k).ws_bytes;
-  return part_bytes(total_q, Hq, cache->head_dim) + (first > second ? first : second);
+  const PagedPlan first = make_paged_plan(n_prefixes, cache->kv_heads, group, cache->head_dim, cache->dtype,
+                                          total_q, max_prefix_q, max_prefix_k);
+  const PagedPlan second = make_paged_plan(B, cache->kv_heads, group, cache->head_dim, cache->dtype, total_q,
+                                           max_seqlen_q, max_seqlen_k);
+  return (joins_itself(second) ? 1 : 2) * part_bytes(total_q, Hq, cache->head_dim) + first.ws_bytes + second.ws_bytes;
 }
 
 int fa_fwd_paged_prefix(const fa_paged_cache* cache, const int* prefix_table,
@@ -553,20 +561,35 @@ int fa_fwd_paged_prefix(const fa_paged_cache* cache, const int* prefix_table,
   a.lse = lse;
   const PagedPlan k1 = plan_of(first, of_prefixes), k2 = plan_of(a, *cache);
   const size_t part = part_bytes(total_q, Hq, cache->head_dim);
-  const size_t need = part + (k1.ws_bytes > k2.ws_bytes ? k1.ws_bytes : k2.ws_bytes);
+  const size_t parts = joins_itself(k2) ? part : 2 * part;
+  const size_t need = parts + k1.ws_bytes + k2.ws_bytes;
   if (!workspace || workspace_bytes < need) return FA_ERR_INVALID_ARG;
   if (int rc = check_grid(k1, first)) return rc;
   if (int rc = check_grid(k2, a)) return rc;
   if (int rc = fa::host_check_device()) return rc;
-  char* const ws = static_cast<char*>(workspace) + part;  // of either pass, one after the other
-  a.part_o = static_cast<float*>(workspace);
-  a.part_lse = a.part_o + static_cast<size_t>(total_q) * Hq * cache->head_dim;
-  a.part = fa::kPartSecond;
-  first.part_o = a.part_o;
-  first.part_lse = a.part_lse;
+  char* const ws = static_cast<char*>(workspace) + parts;
+  const size_t rows = static_cast<size_t>(total_q) * Hq;
+  first.part_o = static_cast<float*>(workspace);
+  first.part_lse = first.part_o + rows * cache->head_dim;
   first.part = fa::kPartFirst;
+  if (joins_itself(k2)) {
+    a.part_o = first.part_o;
+    a.part_lse = first.part_lse;
+    a.part = fa::kPartJoin;
+  } else {
+    a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + part);
+    a.part_lse = a.part_o + rows * cache->head_dim;
+    a.part = fa::kPartSecond;
+  }
   if (int rc = run_paged(first, of_prefixes, k1, Q, q_token_stride, q_head_stride, dtype, ws, stream)) return rc;
-  return run_paged(a, *cache, k2, Q, q_token_stride, q_head_stride, dtype, ws, stream);
+  if (int rc = run_paged(a, *cache, k2, Q, q_token_stride, q_head_stride, dtype, ws + k1.ws_bytes, stream,
+                         /*early=*/true))
+    return rc;
+  if (joins_itself(k2)) return FA_OK;
+  const fa::PagedMerge m{first.part_o, first.part_lse, a.part_o, a.part_lse, O, lse, total_q, Hq};
+  const cudaError_t e = fa::launch_paged_merge(m, cache->head_dim, dtype == FA_DTYPE_BF16,
+                                               static_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? FA_OK : FA_ERR_LAUNCH;
 }
 
 int fa_kvcache_weights(const fa_paged_cache* cache, const void* Q, long long q_token_stride,

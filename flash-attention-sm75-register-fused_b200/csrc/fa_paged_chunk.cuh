@@ -856,20 +856,20 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
       const long long row_id = static_cast<long long>(it.s.c0 + tok) * a.Hq + hq;
       const bool partial = it.slot >= 0;
       const long long ws_row = (static_cast<long long>(it.slot) * 2 + g) * kBlockM + r;
-      float* lse_dst = partial                  ? p.ws_lse + ws_row
-                       : a.part == kPartFirst ? a.part_lse + row_id
-                       : a.lse                ? a.lse + static_cast<long long>(hq) * a.r.total + it.s.c0 + tok
-                                              : nullptr;
-      // of two passes: where the first one's row goes, or is
+      const bool stores = a.part == kPartFirst || a.part == kPartSecond;
+      float* lse_dst = partial  ? p.ws_lse + ws_row
+                       : stores ? a.part_lse + row_id
+                       : a.lse  ? a.lse + static_cast<long long>(hq) * a.r.total + it.s.c0 + tok
+                                : nullptr;
+      // of two passes: where this one's row goes, or the first one's is
       float4* const first_o =
           !partial && a.part != kPartNone ? reinterpret_cast<float4*>(a.part_o + row_id * D) : nullptr;
       if (n_tiles == 0) {
         if (first_o != nullptr) {
           if (row_ok) {
-            const float lse_first = a.part == kPartSecond ? __ldcg(a.part_lse + row_id) : -INFINITY;
-#pragma unroll 1
+#pragma unroll 8
             for (int i = 0; i < D / 4; ++i) {
-              if (a.part == kPartFirst) {
+              if (stores) {
                 first_o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
               } else {
                 const float4 f = __ldcg(first_o + i);  // (zeros without any key)
@@ -877,7 +877,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                     make_uint2(pack2<QBF16>(f.x, f.y), pack2<QBF16>(f.z, f.w));
               }
             }
-            if (lse_dst) *lse_dst = lse_first;
+            if (lse_dst) *lse_dst = stores ? -INFINITY : __ldcg(a.part_lse + row_id);
           }
           continue;
         }
@@ -897,31 +897,33 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
           const float lse_row =
               l == 0.f ? -INFINITY : (m_use + __log2f(l)) * 0.69314718055994530942f;
           if (first_o != nullptr) {
-            const Joined jn = a.part == kPartFirst || !row_ok
-                                  ? Joined{1.f, 0.f, lse_row}
-                                  : join_passes(__ldcg(a.part_lse + row_id), lse_row);
+            Joined jn{1.f, 0.f, lse_row};
+            if (!stores && row_ok) jn = join_passes(__ldcg(a.part_lse + row_id), lse_row);
             const float f_own = jn.own == 0.f ? 0.f : inv_l * jn.own;
 #pragma unroll 1
-            for (int c = 0; c < D / 16; ++c) {
-              uint32_t o[16];
-              ptx::tmem_ld16(tO + c * 16, o);
-              ptx::tmem_wait_ld();
-              pin_after_wait<16>(o);
+            for (int c = 0; c < D / 32; ++c) {
+              float4 f[8] = {};
+              if (!stores && row_ok) {
 #pragma unroll
-              for (int i = 0; row_ok && i < 4; ++i) {
+                for (int i = 0; i < 8; ++i) f[i] = __ldcg(first_o + 8 * c + i);
+              }
+              uint32_t o[32];
+              ptx::tmem_ld32(tO + c * 32, o);
+              ptx::tmem_wait_ld();
+              pin_after_wait<32>(o);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
                 float4 x = make_float4(__uint_as_float(o[4 * i]) * f_own, __uint_as_float(o[4 * i + 1]) * f_own,
                                        __uint_as_float(o[4 * i + 2]) * f_own, __uint_as_float(o[4 * i + 3]) * f_own);
                 if (jn.own == 0.f) x = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (a.part == kPartFirst) {
-                  first_o[4 * c + i] = x;
-                } else {
-                  if (jn.first != 0.f) {
-                    const float4 f = __ldcg(first_o + 4 * c + i);
-                    x = make_float4(fmaf(f.x, jn.first, x.x), fmaf(f.y, jn.first, x.y), fmaf(f.z, jn.first, x.z),
-                                    fmaf(f.w, jn.first, x.w));
-                  }
-                  reinterpret_cast<uint2*>(static_cast<T*>(a.o) + row_id * D)[4 * c + i] =
-                      make_uint2(pack2<QBF16>(x.x, x.y), pack2<QBF16>(x.z, x.w));
+                if (jn.first != 0.f)
+                  x = make_float4(fmaf(f[i].x, jn.first, x.x), fmaf(f[i].y, jn.first, x.y),
+                                  fmaf(f[i].z, jn.first, x.z), fmaf(f[i].w, jn.first, x.w));
+                if (row_ok) {
+                  if (stores) first_o[8 * c + i] = x;
+                  else
+                    reinterpret_cast<uint2*>(static_cast<T*>(a.o) + row_id * D)[8 * c + i] =
+                        make_uint2(pack2<QBF16>(x.x, x.y), pack2<QBF16>(x.z, x.w));
                 }
               }
             }
@@ -973,18 +975,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
 
 // Joins the parts of the items that the chunk kernel's runs cut: LSE = log sum_s
 // exp(LSE_s), O = sum_s exp(LSE_s - LSE) O_s, parts in the order of their keys.
-// Bound by latency, a dependent read of the table and of the parts: 4 to 5 us of a
-// call.  Block x is for the item that the end of run x cuts first; a thread has 16
-// columns of one of its 256 rows, a warp 32 rows.
+// Bound by latency, a dependent read of the table and of the parts.  Block x is for the
+// item that the end of run x cuts first; a thread has four columns of one of its 256
+// rows, a warp 32 rows, and eight parts are on their way at a time (@@).
 constexpr int kJoinThreads = 256;
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ ChunkParams p) {
   const PagedAttn& a = p.a;
+  ptx::launch_dependents();
   ptx::grid_dep_wait();
   const PagedCut c = p.ws_cuts[blockIdx.x];
   if (c.parts == 0) return;
   const int y = static_cast<int>(blockIdx.y * kJoinThreads + threadIdx.x);
-  const int r = y % kBlockM, col = y / kBlockM % (D / 16) * 16, g = y / (kBlockM * (D / 16));
+  const int r = y % kBlockM, col = y / kBlockM % (D / 4) * 4, g = y / (kBlockM * (D / 4));
   const int tok = c.tok0 + g * p.tq + r / a.group;
   if (r >= p.tq * a.group || tok >= c.nq) return;
   // first row of query tile g in part x
@@ -992,65 +995,45 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
     return ((x == 0 ? 2ll * blockIdx.x + 1 : 2ll * (blockIdx.x + x)) * 2 + g) * kBlockM;
   };
   float mx = -INFINITY;
-#pragma unroll 4
+#pragma unroll 8
   for (int x = 0; x < c.parts; ++x) mx = fmaxf(mx, __ldcg(p.ws_lse + tile_row(x) + r));
-  float acc[16] = {}, sum = 0.f;
-#pragma unroll 2
+  float acc[4] = {}, sum = 0.f;
+#pragma unroll 8
   for (int x = 0; x < c.parts; ++x) {
-    const float4* src = reinterpret_cast<const float4*>(p.ws_o + tile_row(x) * D) + (col >> 2) * kBlockM + r;
-    float4 o[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] = __ldcg(src + e * kBlockM);
+    const float4 o = __ldcg(reinterpret_cast<const float4*>(p.ws_o + tile_row(x) * D) + (col >> 2) * kBlockM + r);
     const float ls = __ldcg(p.ws_lse + tile_row(x) + r);
     // (a part without a key for this row has no O; a NaN stays one)
     const float f = ls == -INFINITY ? 0.f : expf(ls - mx);
     sum += f;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      acc[4 * e] = f == 0.f ? acc[4 * e] : fmaf(f, o[e].x, acc[4 * e]);
-      acc[4 * e + 1] = f == 0.f ? acc[4 * e + 1] : fmaf(f, o[e].y, acc[4 * e + 1]);
-      acc[4 * e + 2] = f == 0.f ? acc[4 * e + 2] : fmaf(f, o[e].z, acc[4 * e + 2]);
-      acc[4 * e + 3] = f == 0.f ? acc[4 * e + 3] : fmaf(f, o[e].w, acc[4 * e + 3]);
-    }
+    acc[0] = f == 0.f ? acc[0] : fmaf(f, o.x, acc[0]);
+    acc[1] = f == 0.f ? acc[1] : fmaf(f, o.y, acc[1]);
+    acc[2] = f == 0.f ? acc[2] : fmaf(f, o.z, acc[2]);
+    acc[3] = f == 0.f ? acc[3] : fmaf(f, o.w, acc[3]);
   }
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
   const int hq = c.h * a.group + r % a.group;
   const long long out = static_cast<long long>(c.c0 + tok) * a.Hq + hq;
-  uint32_t w[8];
-  if (a.part != kPartNone) {
-    const float lse = sum == 0.f ? -INFINITY : mx + logf(sum);
-    float4* const first_o = reinterpret_cast<float4*>(a.part_o + out * D + col);
-    if (a.part == kPartFirst) {
+  float lse = sum == 0.f ? -INFINITY : mx + logf(sum);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        first_o[e] = make_float4(acc[4 * e] * inv, acc[4 * e + 1] * inv, acc[4 * e + 2] * inv, acc[4 * e + 3] * inv);
+  for (int e = 0; e < 4; ++e) acc[e] *= inv;
+  if (a.part != kPartNone) {
+    float4* const first_o = reinterpret_cast<float4*>(a.part_o + out * D + col);
+    if (a.part != kPartJoin) {
+      *first_o = make_float4(acc[0], acc[1], acc[2], acc[3]);
       if (col == 0) a.part_lse[out] = lse;
       return;
     }
     const Joined jn = join_passes(__ldcg(a.part_lse + out), lse);
+    const float4 f = __ldcg(first_o);
+    const float y4[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float4 f = __ldcg(first_o + e);
-      const float y[4] = {f.x, f.y, f.z, f.w};
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-        acc[4 * e + x] = (jn.own == 0.f ? 0.f : acc[4 * e + x] * inv * jn.own) + (jn.first == 0.f ? 0.f : y[x] * jn.first);
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = pack2<BF16>(acc[2 * e], acc[2 * e + 1]);
-    uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.o) + out * D + col);
-    dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
-    dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
-    if (col == 0 && a.lse != nullptr) a.lse[static_cast<long long>(hq) * a.r.total + c.c0 + tok] = jn.lse;
-    return;
+    for (int e = 0; e < 4; ++e)
+      acc[e] = (jn.own == 0.f ? 0.f : acc[e] * jn.own) + (jn.first == 0.f ? 0.f : y4[e] * jn.first);
+    lse = jn.lse;
   }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) w[e] = pack2<BF16>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
-  uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.o) + out * D + col);
-  dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
-  dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
-  if (col == 0 && a.lse != nullptr)
-    a.lse[static_cast<long long>(hq) * a.r.total + c.c0 + tok] = sum == 0.f ? -INFINITY : mx + logf(sum);
+  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + out * D + col) =
+      make_uint2(pack2<BF16>(acc[0], acc[1]), pack2<BF16>(acc[2], acc[3]));
+  if (col == 0 && a.lse != nullptr) a.lse[static_cast<long long>(hq) * a.r.total + c.c0 + tok] = lse;
 }
 
 // The visible keys and values of the chunk kernel's sequences as 16-bit rows:
@@ -1225,7 +1208,7 @@ cudaError_t launch_paged_chunk(const ChunkParams& p, int head_dim, int kv, bool 
   if (e != cudaSuccess || !p.runs || p.n_ctas == 1) return e;
   // may start while the last runs finish; it waits for them before it reads
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(p.n_ctas - 1, 2 * kBlockM * (head_dim / 16) / kJoinThreads);
+  cfg.gridDim = dim3(p.n_ctas - 1, 2 * kBlockM * (head_dim / 4) / kJoinThreads);
   cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];

@@ -202,24 +202,9 @@ struct Partial {
     const float inv = l == 0.f ? 0.f : up / l;
     if (a.part != kPartNone) {
       const long long row = static_cast<long long>(tok) * a.Hq + hq;
-      const float lse = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
-      float x[E];
-      if (a.part == kPartFirst) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) a.part_o[row * D + lane * E + e] = o[e] * inv;
-        if (lane == 0) a.part_lse[row] = lse;
-        return;
-      }
-      const Joined j = join_passes(__ldcg(a.part_lse + row), lse);
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const float f = __ldcg(a.part_o + row * D + lane * E + e);
-        x[e] = (j.own == 0.f ? 0.f : o[e] * inv * j.own) + (j.first == 0.f ? 0.f : f * j.first);
-      }
-      uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.o) + row * D) + lane * (E / 2);
-#pragma unroll
-      for (int e = 0; e < E; e += 2) dst[e / 2] = pack2<BF16>(x[e], x[e + 1]);
-      if (lane == 0 && a.lse != nullptr) a.lse[static_cast<long long>(hq) * a.r.total + tok] = j.lse;
+      for (int e = 0; e < E; ++e) a.part_o[row * D + lane * E + e] = o[e] * inv;
+      if (lane == 0) a.part_lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
       return;
     }
     uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.o) +
@@ -241,8 +226,7 @@ struct Cursor {
 };
 
 template <int D, int KV, bool QBF16, int NT, int TEAM>
-__global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
-    paged_decode_kernel(const __grid_constant__ DecodeParams p) {
+__device__ __forceinline__ void paged_decode_body(const DecodeParams& p) {
   using C = Cfg<D, KV>;
   const int stages = p.stages * TEAM;  // of a team
   constexpr int kTeams = kWarps / TEAM;
@@ -782,26 +766,12 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
               l[nt][c] == 0.f ? -INFINITY : (m[nt][c] + (C::k8 ? 0.f : __log2f(l[nt][c]))) * 0.69314718055994530942f;
           if (a.part != kPartNone) {
             const long long row = static_cast<long long>(tok) * a.Hq + hq;
-            float* const first_o = a.part_o + row * D;
-            const Joined jn = a.part == kPartFirst ? Joined{1.f, 0.f, lse_row}
-                                                   : join_passes(__ldcg(a.part_lse + row), lse_row);
 #pragma unroll
-            for (int k = 0; k < C::kKS; ++k)
-#pragma unroll
-              for (int hh = 0; hh < 2; ++hh) {
-                const float x = jn.own == 0.f ? 0.f : o[nt][k][2 * hh + c] * inv * jn.own;
-                if (a.part == kPartFirst) {
-                  first_o[col(k, hh)] = x;
-                } else {
-                  const float y = jn.first == 0.f ? x : fmaf(__ldcg(first_o + col(k, hh)), jn.first, x);
-                  static_cast<uint16_t*>(a.o)[row * D + col(k, hh)] =
-                      static_cast<uint16_t>(pack2<QBF16>(y, 0.f) & 0xffffu);
-                }
-              }
-            if (g == 0) {
-              if (a.part == kPartFirst) a.part_lse[row] = lse_row;
-              else if (a.lse != nullptr) a.lse[static_cast<long long>(hq) * a.r.total + tok] = jn.lse;
+            for (int k = 0; k < C::kKS; ++k) {
+              a.part_o[row * D + col(k, 0)] = o[nt][k][c] * inv;
+              a.part_o[row * D + col(k, 1)] = o[nt][k][2 + c] * inv;
             }
+            if (g == 0) a.part_lse[row] = lse_row;
             continue;
           }
           uint16_t* dst = static_cast<uint16_t*>(a.o) + (static_cast<long long>(tok) * a.Hq + hq) * D;
@@ -867,6 +837,13 @@ __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
   }
 }
 
+template <int D, int KV, bool QBF16, int NT, int TEAM>
+__global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
+    paged_decode_kernel(const __grid_constant__ DecodeParams p) {
+  paged_decode_body<D, KV, QBF16, NT, TEAM>(p);
+  if (p.early) ptx::grid_dep_wait();
+}
+
 // Joins the partial results of (sequence, KV head) blockIdx.x, query rows
 // blockIdx.y * kRows ..: with M = max m_s over the segment's slots,
 //   O = up sum 2^(m_s - M) O_s / sum 2^(m_s - M) l_s,
@@ -889,6 +866,7 @@ __global__ void __launch_bounds__(kCombineThreads)
   __shared__ float sh_m[kW], sh_l[kW];
   const int b = blockIdx.x / a.c.heads, h = blockIdx.x % a.c.heads;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  ptx::launch_dependents();
   fill_outside(a, D, static_cast<int>(blockIdx.y * gridDim.x + blockIdx.x),
                static_cast<int>(gridDim.x * gridDim.y));
   const Seq s = load_short(a, b, p.max_rows);
@@ -987,8 +965,17 @@ cudaError_t launch_impl(const DecodeParams& p, int n_ctas, cudaStream_t stream) 
     if (e != cudaSuccess) return e;
     if (dev >= 0 && dev < 64) attr_done[dev] = 1;
   }
-  kern<<<n_ctas, 32 * kWarps, C::smem(p.stages), stream>>>(p);
-  cudaError_t e = cudaGetLastError();
+  cudaLaunchConfig_t first{};
+  cudaLaunchAttribute early[1];
+  early[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early[0].val.programmaticStreamSerializationAllowed = 1;
+  first.gridDim = dim3(n_ctas);
+  first.blockDim = dim3(32 * kWarps);
+  first.dynamicSmemBytes = C::smem(p.stages);
+  first.stream = stream;
+  first.attrs = early;
+  first.numAttrs = p.early ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&first, kern, p);
   if (e != cudaSuccess || p.solo) return e;
   // the combine may start while the last teams finish; it waits for them
   // before it reads a slot

@@ -84,9 +84,10 @@ def test_prefix_workspace_depends_on_sizes_alone():
         assert n == f(ctypes.byref(_cache(k=P16 * 2, block_table=P16 * 4)), *first, *second)
         B, Hq, total, max_q, max_k = second
         part = total * Hq * 65 * 4
-        either = max(plain(ctypes.byref(_cache()), first[0], Hq, total, first[1], first[2]),
-                     plain(ctypes.byref(_cache()), *second))
-        assert part + either <= n < part + either + 128
+        passes = (plain(ctypes.byref(_cache()), first[0], Hq, total, first[1], first[2]) +
+                  plain(ctypes.byref(_cache()), *second))
+        # the results of the first pass, and of the second unless it joins them as it writes
+        assert any(0 <= n - passes - x * part < 256 for x in (1, 2))
     for first, second in (((-1, 1, 64), (1, 4, 1, 1, 64)), ((1, -1, 64), (1, 4, 1, 1, 64)),
                           ((1, 1, 64), (1, 258, 9, 9, 64)), ((1, 1, 64), (1, 4, -9, 9, 64)),
                           ((1, 1, -64), (1, 4, 9, 9, 64)), ((1 << 21, 1, 64), (1, 4, 9, 9, 64))):
