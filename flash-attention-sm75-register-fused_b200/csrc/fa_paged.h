@@ -67,8 +67,12 @@ struct PagedAttn {
   // Attention over two sets of keys in two passes: where its results go, and (kPartJoin)
   // the first pass's, which they are joined with.
   int part;                   // kPart*
-  float* part_o;              // [total, Hq, d]
+  float* part_o;              // column c of row (token, head) at part_at(row, c)
   float* part_lse;            // [total, Hq], natural log
+  long long part_row, part_block;  // elements from row to row, from four columns to the next four
+  __device__ __forceinline__ float* part_at(long long row, int c) const {
+    return part_o + row * part_row + (c >> 2) * part_block + (c & 3);
+  }
 };
 // kPartNone: o and lse.  kPartFirst, kPartSecond: part_o and part_lse, as fp32; rows that
 // no kernel computes get O = 0 and LSE = -inf, in the second pass kNoRow.  kPartJoin: o and

@@ -345,6 +345,7 @@ void set_queries(fa::PagedAttn* a, const fa_paged_cache* cache, const void* Q, l
   a->scale_log2 = scale * 1.4426950408889634f;
   a->part = fa::kPartNone;
   a->part_o = a->part_lse = nullptr;
+  a->part_row = a->part_block = 0;
 }
 
 PagedPlan plan_of(const fa::PagedAttn& a, const fa_paged_cache& c) {
@@ -572,7 +573,12 @@ int fa_fwd_paged_prefix(const fa_paged_cache* cache, const int* prefix_table,
   first.part_o = static_cast<float*>(workspace);
   first.part_lse = first.part_o + rows * cache->head_dim;
   first.part = fa::kPartFirst;
+  first.part_row = a.part_row = cache->head_dim;
+  first.part_block = a.part_block = 4;
   if (joins_itself(k2)) {
+    // a thread of the chunk kernel has a row: the same columns of the rows side by side
+    first.part_row = a.part_row = 4;
+    first.part_block = a.part_block = 4 * static_cast<long long>(rows);
     a.part_o = first.part_o;
     a.part_lse = first.part_lse;
     a.part = fa::kPartJoin;
@@ -608,7 +614,8 @@ int fa_kvcache_weights(const fa_paged_cache* cache, const void* Q, long long q_t
   const long long held = static_cast<long long>(cache->max_pages) * cache->page_size;
   const int keys = static_cast<int>(max_seqlen_k < held ? max_seqlen_k : held);
   if (int rc = check_sums(weights, w_seq_stride, w_head_stride, weights_len, keys, B, p.a.c.heads)) return rc;
-  if (B == 0 || keys == 0 || Hq == 0) return FA_OK;
+  if (Hq == 0) return FA_ERR_INVALID_ARG;
+  if (B == 0 || keys == 0) return FA_OK;
   if (int rc = check_queries(p.a.c, Hq, total_q, Q, lse, q_token_stride, q_head_stride, 4)) return rc;
   if (int rc = check_query_strides(Hq, total_q, q_token_stride, q_head_stride)) return rc;
   if (static_cast<long long>(B) * p.a.c.heads > 0x7fffffffLL || static_cast<long long>(total_q) * Hq > (1LL << 33))

@@ -863,16 +863,17 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                                 : nullptr;
       // of two passes: where this one's row goes, or the first one's is
       float4* const first_o =
-          !partial && a.part != kPartNone ? reinterpret_cast<float4*>(a.part_o + row_id * D) : nullptr;
+          !partial && a.part != kPartNone ? reinterpret_cast<float4*>(a.part_at(row_id, 0)) : nullptr;
+      const long long step_o = a.part_block / 4;
       if (n_tiles == 0) {
         if (first_o != nullptr) {
           if (row_ok) {
 #pragma unroll 8
             for (int i = 0; i < D / 4; ++i) {
               if (stores) {
-                first_o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                first_o[i * step_o] = make_float4(0.f, 0.f, 0.f, 0.f);
               } else {
-                const float4 f = __ldcg(first_o + i);  // (zeros without any key)
+                const float4 f = __ldcg(first_o + i * step_o);  // (zeros without any key)
                 reinterpret_cast<uint2*>(static_cast<T*>(a.o) + row_id * D)[i] =
                     make_uint2(pack2<QBF16>(f.x, f.y), pack2<QBF16>(f.z, f.w));
               }
@@ -905,7 +906,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
               float4 f[8] = {};
               if (!stores && row_ok) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) f[i] = __ldcg(first_o + 8 * c + i);
+                for (int i = 0; i < 8; ++i) f[i] = __ldcg(first_o + (8 * c + i) * step_o);
               }
               uint32_t o[32];
               ptx::tmem_ld32(tO + c * 32, o);
@@ -920,7 +921,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                   x = make_float4(fmaf(f[i].x, jn.first, x.x), fmaf(f[i].y, jn.first, x.y),
                                   fmaf(f[i].z, jn.first, x.z), fmaf(f[i].w, jn.first, x.w));
                 if (row_ok) {
-                  if (stores) first_o[8 * c + i] = x;
+                  if (stores) first_o[(8 * c + i) * step_o] = x;
                   else
                     reinterpret_cast<uint2*>(static_cast<T*>(a.o) + row_id * D)[8 * c + i] =
                         make_uint2(pack2<QBF16>(x.x, x.y), pack2<QBF16>(x.z, x.w));
@@ -1017,7 +1018,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
 #pragma unroll
   for (int e = 0; e < 4; ++e) acc[e] *= inv;
   if (a.part != kPartNone) {
-    float4* const first_o = reinterpret_cast<float4*>(a.part_o + out * D + col);
+    float4* const first_o = reinterpret_cast<float4*>(a.part_at(out, col));
     if (a.part != kPartJoin) {
       *first_o = make_float4(acc[0], acc[1], acc[2], acc[3]);
       if (col == 0) a.part_lse[out] = lse;

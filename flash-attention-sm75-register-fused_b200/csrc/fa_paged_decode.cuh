@@ -203,7 +203,7 @@ struct Partial {
     if (a.part != kPartNone) {
       const long long row = static_cast<long long>(tok) * a.Hq + hq;
 #pragma unroll
-      for (int e = 0; e < E; ++e) a.part_o[row * D + lane * E + e] = o[e] * inv;
+      for (int e = 0; e < E; ++e) *a.part_at(row, lane * E + e) = o[e] * inv;
       if (lane == 0) a.part_lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
       return;
     }
@@ -768,8 +768,8 @@ __device__ __forceinline__ void paged_decode_body(const DecodeParams& p) {
             const long long row = static_cast<long long>(tok) * a.Hq + hq;
 #pragma unroll
             for (int k = 0; k < C::kKS; ++k) {
-              a.part_o[row * D + col(k, 0)] = o[nt][k][c] * inv;
-              a.part_o[row * D + col(k, 1)] = o[nt][k][2 + c] * inv;
+              *a.part_at(row, col(k, 0)) = o[nt][k][c] * inv;
+              *a.part_at(row, col(k, 1)) = o[nt][k][2 + c] * inv;
             }
             if (g == 0) a.part_lse[row] = lse_row;
             continue;

@@ -97,7 +97,8 @@ def test_prefix_workspace_depends_on_sizes_alone():
 
 def test_weights_argument_errors():
     for kw in (dict(mode=-1), dict(mode=3), dict(causal=3), dict(scale=math.inf), dict(max_q=-1), dict(max_k=-1),
-               dict(w=0), dict(L=63), dict(L=-1), dict(Q=0), dict(lse=0), dict(cu=0)):
+               dict(w=0), dict(L=63), dict(L=-1), dict(Q=0), dict(lse=0), dict(cu=0),
+               dict(Hq=0)):
         assert _weights(_cache(), **kw) == 1, kw
     assert _weights(_cache(), dtype=2) == 5
     assert _weights(_cache(), Hq=3) == 3 and _weights(_cache(), Hq=258) == 13

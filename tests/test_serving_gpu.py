@@ -317,6 +317,15 @@ def test_weights_modes_bounds_and_rows_of_no_sequence(sm100, nq):
                        max_k=mk)
 
 
+def test_weights_without_queries(sm100):
+    """A step without tokens: the sums stay, or are set to 0."""
+    P = Paged([(0, 130), (0, 7), (0, 0)], 2, 64, 16, F16, seed=2)
+    q, lse, old = P.new(8), torch.zeros(8, 0), _old(P)
+    assert q.size(0) == 0
+    for how in ("append", "add", "set"):
+        _check_weights(P, q, lse, 8, 1, old, how, _weights(P, q, lse, old, 1, how))
+
+
 @pytest.mark.parametrize("nq", [1, 150])
 def test_weights_masked_rows_and_places(sm100, nq):
     """Rows whose LSE is -inf add nothing, whatever keys hold; NaN keys that no row may see do
