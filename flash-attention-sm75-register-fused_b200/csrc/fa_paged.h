@@ -73,11 +73,15 @@ struct PagedAttn {
   __device__ __forceinline__ float* part_at(long long row, int c) const {
     return part_o + row * part_row + (c >> 2) * part_block + (c & 3);
   }
+  const float* first_o;       // kPartRuns: the first pass's, [total, Hq, d] and [total, Hq]
+  const float* first_lse;
 };
 // kPartNone: o and lse.  kPartFirst, kPartSecond: part_o and part_lse, as fp32; rows that
 // no kernel computes get O = 0 and LSE = -inf, in the second pass kNoRow.  kPartJoin: o and
-// lse, joined with part_o and part_lse (chunk kernel alone).
-enum { kPartNone = 0, kPartFirst = 1, kPartSecond = 2, kPartJoin = 3 };
+// lse, joined with the first pass's rows in part_o and part_lse (chunk kernel alone, or
+// decode with one CTA per (sequence, head)).  kPartRuns: decode whose runs are combined: rows
+// that one team has go to part_o and part_lse, and the combine joins all with first_o.
+enum { kPartNone = 0, kPartFirst = 1, kPartSecond = 2, kPartJoin = 3, kPartRuns = 4 };
 constexpr unsigned kNoRow = 0x7fffdeadu;  // bits of an LSE: the row belongs to no sequence
 
 // Joins the rows of two passes (fa_paged_merge.cu).

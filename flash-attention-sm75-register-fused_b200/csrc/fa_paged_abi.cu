@@ -346,6 +346,7 @@ void set_queries(fa::PagedAttn* a, const fa_paged_cache* cache, const void* Q, l
   a->part = fa::kPartNone;
   a->part_o = a->part_lse = nullptr;
   a->part_row = a->part_block = 0;
+  a->first_o = a->first_lse = nullptr;
 }
 
 PagedPlan plan_of(const fa::PagedAttn& a, const fa_paged_cache& c) {
@@ -374,11 +375,16 @@ size_t part_bytes(int total, int Hq, int head_dim) {
   return (static_cast<size_t>(total) * Hq * (head_dim + 1) * sizeof(float) + 127) / 128 * 128;
 }
 
-// Of two passes over chunks alone the second joins its rows with the first's as it writes them
-// (4096 tokens, 32 heads: @@).  A kernel that ends many short segments would wait there for what it reads
-// (64 tokens over 64 sequences: 60 us instead of 30 for the pass), so its results go to the
-// workspace and a kernel of its own joins them.
-bool joins_itself(const PagedPlan& k) { return k.chunk && !k.decode; }
+// How the second of two passes joins its rows with the first's.  The chunk kernel does it as it
+// writes them, and the decode kernel where a CTA has one (sequence, head).  Where teams end
+// many short segments they would wait there for what they read (64 tokens over 64 sequences: 60
+// us instead of 30 for the pass), so the combine does it; and where both kernels run their
+// results go to the workspace and a kernel of its own joins them.
+int join_mode(const PagedPlan& k) {
+  if (k.chunk) return k.decode ? fa::kPartSecond : fa::kPartJoin;
+  return k.ws_decode == 0 ? fa::kPartJoin : fa::kPartRuns;
+}
+int part_buffers(const PagedPlan& second) { return join_mode(second) == fa::kPartJoin ? 1 : 2; }
 
 // The kernels of one pass.  `early`: it may start while the kernels before it end.
 int run_paged(const fa::PagedAttn& a, const fa_paged_cache& cache, const PagedPlan& k, const void* Q,
@@ -529,7 +535,7 @@ size_t fa_fwd_paged_prefix_workspace_bytes(const fa_paged_cache* cache, int n_pr
                                           total_q, max_prefix_q, max_prefix_k);
   const PagedPlan second = make_paged_plan(B, cache->kv_heads, group, cache->head_dim, cache->dtype, total_q,
                                            max_seqlen_q, max_seqlen_k);
-  return (joins_itself(second) ? 1 : 2) * part_bytes(total_q, Hq, cache->head_dim) + first.ws_bytes + second.ws_bytes;
+  return part_buffers(second) * part_bytes(total_q, Hq, cache->head_dim) + first.ws_bytes + second.ws_bytes;
 }
 
 int fa_fwd_paged_prefix(const fa_paged_cache* cache, const int* prefix_table,
@@ -562,7 +568,7 @@ int fa_fwd_paged_prefix(const fa_paged_cache* cache, const int* prefix_table,
   a.lse = lse;
   const PagedPlan k1 = plan_of(first, of_prefixes), k2 = plan_of(a, *cache);
   const size_t part = part_bytes(total_q, Hq, cache->head_dim);
-  const size_t parts = joins_itself(k2) ? part : 2 * part;
+  const size_t parts = part_buffers(k2) * part;
   const size_t need = parts + k1.ws_bytes + k2.ws_bytes;
   if (!workspace || workspace_bytes < need) return FA_ERR_INVALID_ARG;
   if (int rc = check_grid(k1, first)) return rc;
@@ -575,23 +581,25 @@ int fa_fwd_paged_prefix(const fa_paged_cache* cache, const int* prefix_table,
   first.part = fa::kPartFirst;
   first.part_row = a.part_row = cache->head_dim;
   first.part_block = a.part_block = 4;
-  if (joins_itself(k2)) {
-    // a thread of the chunk kernel has a row: the same columns of the rows side by side
-    first.part_row = a.part_row = 4;
-    first.part_block = a.part_block = 4 * static_cast<long long>(rows);
+  a.part = join_mode(k2);
+  a.first_o = first.part_o;
+  a.first_lse = first.part_lse;
+  if (a.part == fa::kPartJoin) {
     a.part_o = first.part_o;
     a.part_lse = first.part_lse;
-    a.part = fa::kPartJoin;
+    if (k2.chunk) {  // a thread of the chunk kernel has a row: the same columns of the rows side by side
+      first.part_row = a.part_row = 4;
+      first.part_block = a.part_block = 4 * static_cast<long long>(rows);
+    }
   } else {
     a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + part);
     a.part_lse = a.part_o + rows * cache->head_dim;
-    a.part = fa::kPartSecond;
   }
   if (int rc = run_paged(first, of_prefixes, k1, Q, q_token_stride, q_head_stride, dtype, ws, stream)) return rc;
   if (int rc = run_paged(a, *cache, k2, Q, q_token_stride, q_head_stride, dtype, ws + k1.ws_bytes, stream,
                          /*early=*/true))
     return rc;
-  if (joins_itself(k2)) return FA_OK;
+  if (a.part != fa::kPartSecond) return FA_OK;
   const fa::PagedMerge m{first.part_o, first.part_lse, a.part_o, a.part_lse, O, lse, total_q, Hq};
   const cudaError_t e = fa::launch_paged_merge(m, cache->head_dim, dtype == FA_DTYPE_BF16,
                                                static_cast<cudaStream_t>(stream));

@@ -202,9 +202,25 @@ struct Partial {
     const float inv = l == 0.f ? 0.f : up / l;
     if (a.part != kPartNone) {
       const long long row = static_cast<long long>(tok) * a.Hq + hq;
+      const float lse = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
+      if (a.part == kPartFirst || a.part == kPartSecond) {
 #pragma unroll
-      for (int e = 0; e < E; ++e) *a.part_at(row, lane * E + e) = o[e] * inv;
-      if (lane == 0) a.part_lse[row] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
+        for (int e = 0; e < E; ++e) *a.part_at(row, lane * E + e) = o[e] * inv;
+        if (lane == 0) a.part_lse[row] = lse;
+        return;
+      }
+      const bool runs = a.part == kPartRuns;
+      const Joined j = join_passes(__ldcg((runs ? a.first_lse : a.part_lse) + row), lse);
+      float x[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float f = __ldcg(runs ? a.first_o + row * D + lane * E + e : a.part_at(row, lane * E + e));
+        x[e] = (j.own == 0.f ? 0.f : o[e] * inv * j.own) + (j.first == 0.f ? 0.f : f * j.first);
+      }
+      uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.o) + row * D) + lane * (E / 2);
+#pragma unroll
+      for (int e = 0; e < E; e += 2) dst[e / 2] = pack2<BF16>(x[e], x[e + 1]);
+      if (lane == 0 && a.lse != nullptr) a.lse[static_cast<long long>(hq) * a.r.total + tok] = j.lse;
       return;
     }
     uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.o) +
@@ -818,6 +834,7 @@ __device__ __forceinline__ void paged_decode_body(const DecodeParams& p) {
   }
   if (p.solo) {
     if (__syncthreads_and(ok ? 1 : 0) == 0) return;
+    if (p.early) ptx::grid_dep_wait();  // (the first pass's rows are read)
     // one warp joins a row of the teams' slots
     constexpr int kSlotRows = 8 * NT * TEAM;
     const Seq s = load_short(a, b_first, p.max_rows);
@@ -883,7 +900,7 @@ __global__ void __launch_bounds__(kCombineThreads)
   const long long t0 = sp.before * a.c.heads + static_cast<long long>(h) * (n + kSegCost) + kSegCost;
   const int w0 = n > 0 ? static_cast<int>(t0 / per) : 0;
   const int w1 = n > 0 ? static_cast<int>((t0 + n - 1) / per) : -1;
-  if (w0 == w1) return;  // one team had it all
+  if (w0 == w1 && a.part != kPartRuns) return;  // one team had it all
   const long long stride = slot_floats(slot_rows, D);
   // slots first, first + step, ... of row `row`
   auto gather = [&](int row, int first, int step) {
@@ -924,6 +941,22 @@ __global__ void __launch_bounds__(kCombineThreads)
   auto finish = [&](int row, const Partial<D>& r) {
     r.template write<BF16>(a, s.c0 + row / a.group, h * a.group + row % a.group, up);
   };
+  if (w0 == w1) {  // ... and left it as a result
+    for (int r = warp; r < rows; r += kW) {
+      const int y = row0 + r;
+      const long long row = static_cast<long long>(s.c0 + y / a.group) * a.Hq + h * a.group + y % a.group;
+      const float lse = __ldcg(a.part_lse + row);
+      Partial<D> x;
+      if (lse != -INFINITY) {
+        x.m = lse * 1.4426950408889634f;
+        x.l = 1.f;
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) x.o[e] = __ldcg(a.part_at(row, lane * E + e)) / up;
+      finish(y, x);
+    }
+    return;
+  }
   if (kRows > 1 && w1 - w0 < kManySlots) {
     for (int r = warp; r < rows; r += kW) finish(row0 + r, gather(row0 + r, 0, 1));
     return;
