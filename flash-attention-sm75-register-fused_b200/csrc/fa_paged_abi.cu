@@ -438,6 +438,8 @@ int run_paged(const fa::PagedAttn& a, const fa_paged_cache& cache, const PagedPl
       p.fill = !k.decode && p.head0 == 0 ? 1 : 0;
       p.epoch = fa::host_next_epoch();
       p.n_ctas = k.runs ? k.n_ctas : k.slots * p.n_heads;
+      const long long most = static_cast<long long>(k.slots) * p.n_heads;
+      p.max_items = most < 0x7fffffffLL ? static_cast<int>(most) : 0x7fffffff;
       if (fa::launch_paged_chunk(p, cache.head_dim, cache.dtype, bf16, fa::host_sm_count(), st) !=
           cudaSuccess)
         return FA_ERR_LAUNCH;

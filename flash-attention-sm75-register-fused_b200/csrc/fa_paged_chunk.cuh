@@ -976,16 +976,34 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
 
 // Joins the parts of the items that the chunk kernel's runs cut: LSE = log sum_s
 // exp(LSE_s), O = sum_s exp(LSE_s - LSE) O_s, parts in the order of their keys.
-// Bound by latency, a dependent read of the table and of the parts.  Block x is for the
-// item that the end of run x cuts first; a thread has four columns of one of its 256
-// rows, a warp 32 rows, and eight parts are on their way at a time (@@).
+// Bound by latency, a dependent read of the table and of the parts.  Blocks x are for the
+// item that the end of run x cuts first, or, where there are fewer items than runs, for the
+// x-th item that is cut (256 blocks instead of 4700 for a step behind one prefix; those
+// without an item kept the next kernel from starting).  A thread has four columns of one
+// of its item's 256 rows, a warp 32 rows, and eight parts are on their way at a time.
 constexpr int kJoinThreads = 256;
 template <int D, bool BF16>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ ChunkParams p) {
   const PagedAttn& a = p.a;
   ptx::launch_dependents();
   ptx::grid_dep_wait();
-  const PagedCut c = p.ws_cuts[blockIdx.x];
+  int run = static_cast<int>(blockIdx.x);
+  if (static_cast<int>(gridDim.x) < p.n_ctas - 1) {
+    __shared__ int sh_before[kJoinThreads / 32], sh_run;
+    const int tid = static_cast<int>(threadIdx.x);
+    const bool is_cut = tid < p.n_ctas - 1 && __ldcg(&p.ws_cuts[tid].parts) != 0;
+    const unsigned cuts = __ballot_sync(0xffffffffu, is_cut);
+    if (tid == 0) sh_run = -1;
+    if ((tid & 31) == 0) sh_before[tid >> 5] = __popc(cuts);
+    __syncthreads();
+    int n = __popc(cuts & ((1u << (tid & 31)) - 1u));
+    for (int w = 0; w < tid >> 5; ++w) n += sh_before[w];
+    if (is_cut && n == run) sh_run = tid;
+    __syncthreads();
+    run = sh_run;
+    if (run < 0) return;
+  }
+  const PagedCut c = p.ws_cuts[run];
   if (c.parts == 0) return;
   const int y = static_cast<int>(blockIdx.y * kJoinThreads + threadIdx.x);
   const int r = y % kBlockM, col = y / kBlockM % (D / 4) * 4, g = y / (kBlockM * (D / 4));
@@ -993,7 +1011,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_c
   if (r >= p.tq * a.group || tok >= c.nq) return;
   // first row of query tile g in part x
   auto tile_row = [&](int x) {
-    return ((x == 0 ? 2ll * blockIdx.x + 1 : 2ll * (blockIdx.x + x)) * 2 + g) * kBlockM;
+    return ((x == 0 ? 2ll * run + 1 : 2ll * (run + x)) * 2 + g) * kBlockM;
   };
   float mx = -INFINITY;
 #pragma unroll 8
@@ -1209,7 +1227,8 @@ cudaError_t launch_paged_chunk(const ChunkParams& p, int head_dim, int kv, bool 
   if (e != cudaSuccess || !p.runs || p.n_ctas == 1) return e;
   // may start while the last runs finish; it waits for them before it reads
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(p.n_ctas - 1, 2 * kBlockM * (head_dim / 4) / kJoinThreads);
+  const bool few = p.max_items < p.n_ctas - 1 && p.n_ctas - 1 <= kJoinThreads;
+  cfg.gridDim = dim3(few ? p.max_items : p.n_ctas - 1, 2 * kBlockM * (head_dim / 4) / kJoinThreads);
   cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];

@@ -607,6 +607,85 @@ def test_evict_refusals(sm100):
 
 # ---------------------------------------------------------------- together
 
+@pytest.mark.parametrize("kind", KINDS, ids=KIND_IDS)
+def test_weights_of_prefix_and_own_keys_sum_to_the_rows(sm100, kind):
+    """Each row's weights over its prefix and its own keys sum to 1: the LSE of the two passes and
+    the sums of two calls belong together."""
+    io, cache = kind
+    P = with_prefixes([(1, 60), (40, 70), (3, 3)], [200, 77], 2, 128, 16, cache, io=io, seed=12)
+    q = P.new(8).cuda()
+    c = P.cuda()
+    s = split(P, c)
+    cup = torch.tensor([0, P.cu[2], P.total], dtype=torch.int32, device="cuda")
+    _, lse = _attend(P, q, cup.tolist(), 1, c)
+    own = torch.zeros(3, 2, P.width * 16, device="cuda")
+    pre = torch.zeros(2, 2, P.width * 16, device="cuda")
+    fa.kvcache_weights_paged(q, lse, c["k_cache"], s["table"], s["cu"], s["lens"], 40, 70, own, causal=True,
+                             k_scale=c["k_scale"])
+    fa.kvcache_weights_paged(q, lse, c["k_cache"], s["prefix_table"], cup, s["prefix_lens"], P.cu[2], 200, pre,
+                             mode="add", k_scale=c["k_scale"])
+    o, p = own.sum(-1).cpu(), pre.sum(-1).cpu()
+    # (LSE is good to 1e-4 and, 8-bit pages, f16 rounding of a score of about 10; 164 rows)
+    assert torch.allclose(o[0] + o[1] + p[0], torch.full((2,), 4.0 * 41), rtol=2e-3)
+    assert torch.allclose(o[2] + p[1], torch.full((2,), 4.0 * 3), rtol=2e-3)
+
+
+@pytest.mark.parametrize("cache", [F16, I8])
+def test_byte_offsets_past_4_gib(sm100, cache):
+    """The same pages at the end of a cache of more than 2^32 bytes: equal bits."""
+    P = with_prefixes([(1, 300), (60, 90), (2, 40)], [150], 2, 128, 16, cache, seed=13)
+    q = P.new(8).cuda()
+    c = P.cuda()
+    s = split(P, c)
+    n, size = P.pages, 2 * 16 * 128 * c["k_cache"].element_size()
+    big = (1 << 32) // size + 1000
+
+    def far(x):
+        if x is None:
+            return None
+        y = torch.empty((big + n, *x.shape[1:]), dtype=x.dtype, device="cuda")
+        bits(y)[big:] = bits(x)
+        return y
+
+    b = dict(c, **{k: far(c[k]) for k in ("k_cache", "v_cache", "k_scale", "v_scale")})
+    b["table"] = torch.where((c["table"] >= 0) & (c["table"] < n), c["table"] + big, c["table"])
+    P.pages += big
+    rows = [0, P.total]
+    near, there = _attend(P, q, rows, 1, c), _attend(P, q, rows, 1, b)
+    assert torch.equal(near[0], there[0]) and torch.equal(near[1], there[1])
+    out = []
+    for x in (c, b):
+        t = x["table"][:3].contiguous()
+        w = torch.ones(3, 2, P.width * 16, device="cuda")
+        fa.kvcache_weights_paged(q, near[1], x["k_cache"], t, s["cu"], s["lens"], 60, 300, w, causal=True,
+                                 k_scale=x["k_scale"])
+        lens = fa.kvcache_evict_paged(x["k_cache"], x["v_cache"], w, t, s["lens"], 70, recent=9, **_scales(x))
+        out.append((w, lens, bits(x["k_cache"])[-n:], bits(x["v_cache"])[-n:]))
+    for x, y in zip(*out):
+        assert torch.equal(x.contiguous().view(torch.uint8), y.contiguous().view(torch.uint8))
+
+
+@pytest.mark.parametrize("kind", [F16, I8])
+def test_many_sequences(sm100, kind):
+    """More sequences than threads of a block; ragged, some without tokens or keys."""
+    g = torch.Generator().manual_seed(5)
+    n = torch.randint(0, 30, (700,), generator=g).tolist()
+    lens = [(min(x, int(torch.randint(0, 4, (1,), generator=g))), x) for x in n]
+    P = with_prefixes(lens, [33, 0, 100], 1, 64, 16, kind, seed=14)
+    q = P.new(3)
+    rows = [P.cu[10], P.cu[300], P.cu[310], P.cu[650]]
+    c = P.cuda()
+    got = _attend(P, q, rows, 1, c)
+    _check(P, q, 3, rows, 1, got)
+    P.lens, P.cu, P.nk = P.lens[:700], P.cu[:701], P.nk[:700]
+    c["table"], c["cu"], c["lens"] = c["table"][:700].contiguous(), c["cu"][:701].contiguous(), c["lens"][:700].contiguous()
+    old = _old(P)
+    lse = got[1].cpu()
+    _check_weights(P, q, lse, 3, 1, old, "append", _weights(P, q, lse, old, 1, "append", c))
+    w = _sums(P, seed=15)
+    _check_evict(P, w, 9, 2, 1, _evict(P, w, 9, 2, 1, c))
+
+
 @pytest.mark.parametrize("kind", [F16, I8], ids=["f16", "int8"])
 def test_a_serving_run(sm100, kind):
     """Steps of two requests behind one prompt as they would be served: write, attend, sum the
