@@ -29,8 +29,8 @@ NVCC = os.path.join(CUDA_HOME, "bin", "nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 KERNEL_SOURCES = ["fa_fwd_sm100.cu", "fa_abi.cu", "fa_paged_abi.cu", "fa_paged_cache.cu",
-                  "fa_paged_weights.cu", "fa_paged_evict.cu", "fa_paged_merge.cu"]
-KERNEL_HEADERS = ["fa_host.h", "fa_paged.h", "sm100_ptx.cuh", "fa_softmax.cuh", "fa_fwd.h", "fa_bwd_sm100.cuh",
+                  "fa_paged_prefix.cu", "fa_paged_weights.cu", "fa_paged_evict.cu", "fa_paged_merge.cu"]
+KERNEL_HEADERS = ["fa_host.h", "fa_paged.h", "fa_device.cuh", "sm100_ptx.cuh", "fa_softmax.cuh", "fa_fwd.h", "fa_bwd_sm100.cuh",
                   "fa_decode_sm100.cuh", "fa_fwd_tile.cuh", "fa_fwd_pair2.cuh",
                   "fa_paged_dev.cuh", "fa_paged_chunk.cuh", "fa_paged_decode.cuh",
                   "fa_paged_weights_chunk.cuh"]

@@ -169,5 +169,7 @@ int bwd_smem_bytes_for(int head_dim);
 cudaError_t launch_combine(const FwdParams& p, int head_dim, bool bf16, cudaStream_t stream);
 int smem_bytes_for(int head_dim);
 cudaError_t read_status(unsigned long long* out, bool reset);
+// ... of fa_paged_prefix.cu alone
+cudaError_t read_status_prefix(unsigned long long* out, bool reset);
 
 }  // namespace fa

@@ -81,6 +81,11 @@ struct PagedAttn {
 // lse, joined with the first pass's rows in part_o and part_lse (chunk kernel alone, or
 // decode with one CTA per (sequence, head)).  kPartRuns: decode whose runs are combined: rows
 // that one team has go to part_o and part_lse, and the combine joins all with first_o.
+// (The kernels of a translation unit without FA_PART_ROWS know kPartNone alone.)
+#ifndef FA_PART_ROWS
+#define FA_PART_ROWS 0
+#endif
+constexpr bool kPartRows = FA_PART_ROWS != 0;
 enum { kPartNone = 0, kPartFirst = 1, kPartSecond = 2, kPartJoin = 3, kPartRuns = 4 };
 constexpr unsigned kNoRow = 0x7fffdeadu;  // bits of an LSE: the row belongs to no sequence
 
@@ -207,9 +212,14 @@ int paged_decode_rows(long long heads, int head_dim, int cache_dtype, int sms);
 size_t paged_decode_ws_bytes(long long heads, int max_rows, int max_k, int head_dim, int cache_dtype, int sms);
 cudaError_t launch_paged_decode(DecodeParams p, int head_dim, int cache_dtype, bool bf16, int sms,
                                 cudaStream_t stream);
+cudaError_t launch_paged_decode_part(DecodeParams p, int head_dim, int cache_dtype, bool bf16, int sms,
+                                     cudaStream_t stream);
 // Chunk kernel (after the expansion of 8-bit pages) over the KV heads of p, and
 // the join of the items that its runs cut.
 cudaError_t launch_paged_chunk(const ChunkParams& p, int head_dim, int cache_dtype, bool bf16, int sms,
                                cudaStream_t stream);
+// The same of a pass of two (p.a.part).
+cudaError_t launch_paged_chunk_part(const ChunkParams& p, int head_dim, int cache_dtype, bool bf16, int sms,
+                                    cudaStream_t stream);
 
 }  // namespace fa

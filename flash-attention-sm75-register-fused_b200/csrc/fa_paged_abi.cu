@@ -402,9 +402,8 @@ int run_paged(const fa::PagedAttn& a, const fa_paged_cache& cache, const PagedPl
     p.epoch = fa::host_next_epoch();
     p.timeout_ns = fa::host_timeout_ns();
     if (!page_maps(cache, 16, &p)) return FA_ERR_TENSOR_MAP;
-    if (fa::launch_paged_decode(p, cache.head_dim, cache.dtype, bf16, fa::host_sm_count(), st) !=
-        cudaSuccess)
-      return FA_ERR_LAUNCH;
+    const auto launch = a.part == fa::kPartNone ? fa::launch_paged_decode : fa::launch_paged_decode_part;
+    if (launch(p, cache.head_dim, cache.dtype, bf16, fa::host_sm_count(), st) != cudaSuccess) return FA_ERR_LAUNCH;
   }
   if (k.chunk) {
     fa::ChunkParams p;
@@ -440,9 +439,8 @@ int run_paged(const fa::PagedAttn& a, const fa_paged_cache& cache, const PagedPl
       p.n_ctas = k.runs ? k.n_ctas : k.slots * p.n_heads;
       const long long most = static_cast<long long>(k.slots) * p.n_heads;
       p.max_items = most < 0x7fffffffLL ? static_cast<int>(most) : 0x7fffffff;
-      if (fa::launch_paged_chunk(p, cache.head_dim, cache.dtype, bf16, fa::host_sm_count(), st) !=
-          cudaSuccess)
-        return FA_ERR_LAUNCH;
+      const auto launch = a.part == fa::kPartNone ? fa::launch_paged_chunk : fa::launch_paged_chunk_part;
+      if (launch(p, cache.head_dim, cache.dtype, bf16, fa::host_sm_count(), st) != cudaSuccess) return FA_ERR_LAUNCH;
     }
   }
   return FA_OK;

@@ -1,7 +1,7 @@
 // Attention of chunks of new tokens over a paged KV cache (more query rows per
 // (sequence, KV head) than the decode kernel takes).  Included by
-// fa_fwd_sm100.cu, whose helpers (bounded mbarrier waits, the device status
-// word, exp_tile, the register split) it uses.
+// fa_fwd_sm100.cu and fa_paged_prefix.cu; fa_device.cuh has the helpers (bounded mbarrier
+// waits, the device status word, exp_tile, the register split).
 //
 // The pair kernel's arrangement (fa_fwd_kernel): two 128-row query tiles per
 // CTA ping-pong on one tcgen05 issuer, S and P in tensor memory, lazy rescale.
@@ -856,14 +856,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
       const long long row_id = static_cast<long long>(it.s.c0 + tok) * a.Hq + hq;
       const bool partial = it.slot >= 0;
       const long long ws_row = (static_cast<long long>(it.slot) * 2 + g) * kBlockM + r;
-      const bool stores = a.part == kPartFirst || a.part == kPartSecond;
+      const bool stores = kPartRows && (a.part == kPartFirst || a.part == kPartSecond);
       float* lse_dst = partial  ? p.ws_lse + ws_row
                        : stores ? a.part_lse + row_id
                        : a.lse  ? a.lse + static_cast<long long>(hq) * a.r.total + it.s.c0 + tok
                                 : nullptr;
       // of two passes: where this one's row goes, or the first one's is
       float4* const first_o =
-          !partial && a.part != kPartNone ? reinterpret_cast<float4*>(a.part_at(row_id, 0)) : nullptr;
+          kPartRows && !partial && a.part != kPartNone ? reinterpret_cast<float4*>(a.part_at(row_id, 0)) : nullptr;
       const long long step_o = a.part_block / 4;
       if (n_tiles == 0) {
         if (first_o != nullptr) {
@@ -976,14 +976,67 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
 
 // Joins the parts of the items that the chunk kernel's runs cut: LSE = log sum_s
 // exp(LSE_s), O = sum_s exp(LSE_s - LSE) O_s, parts in the order of their keys.
-// Bound by latency, a dependent read of the table and of the parts.  Blocks x are for the
+// Bound by latency, a dependent read of the table and of the parts: 4 to 5 us of a
+// call.  Block x is for the item that the end of run x cuts first; a thread has 16
+// columns of one of its 256 rows, a warp 32 rows.
+constexpr int kJoinThreads = 256;
+template <int D, bool BF16>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ ChunkParams p) {
+  const PagedAttn& a = p.a;
+  ptx::grid_dep_wait();
+  const PagedCut c = p.ws_cuts[blockIdx.x];
+  if (c.parts == 0) return;
+  const int y = static_cast<int>(blockIdx.y * kJoinThreads + threadIdx.x);
+  const int r = y % kBlockM, col = y / kBlockM % (D / 16) * 16, g = y / (kBlockM * (D / 16));
+  const int tok = c.tok0 + g * p.tq + r / a.group;
+  if (r >= p.tq * a.group || tok >= c.nq) return;
+  // first row of query tile g in part x
+  auto tile_row = [&](int x) {
+    return ((x == 0 ? 2ll * blockIdx.x + 1 : 2ll * (blockIdx.x + x)) * 2 + g) * kBlockM;
+  };
+  float mx = -INFINITY;
+#pragma unroll 4
+  for (int x = 0; x < c.parts; ++x) mx = fmaxf(mx, __ldcg(p.ws_lse + tile_row(x) + r));
+  float acc[16] = {}, sum = 0.f;
+#pragma unroll 2
+  for (int x = 0; x < c.parts; ++x) {
+    const float4* src = reinterpret_cast<const float4*>(p.ws_o + tile_row(x) * D) + (col >> 2) * kBlockM + r;
+    float4 o[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] = __ldcg(src + e * kBlockM);
+    const float ls = __ldcg(p.ws_lse + tile_row(x) + r);
+    // (a part without a key for this row has no O; a NaN stays one)
+    const float f = ls == -INFINITY ? 0.f : expf(ls - mx);
+    sum += f;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      acc[4 * e] = f == 0.f ? acc[4 * e] : fmaf(f, o[e].x, acc[4 * e]);
+      acc[4 * e + 1] = f == 0.f ? acc[4 * e + 1] : fmaf(f, o[e].y, acc[4 * e + 1]);
+      acc[4 * e + 2] = f == 0.f ? acc[4 * e + 2] : fmaf(f, o[e].z, acc[4 * e + 2]);
+      acc[4 * e + 3] = f == 0.f ? acc[4 * e + 3] : fmaf(f, o[e].w, acc[4 * e + 3]);
+    }
+  }
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  const int hq = c.h * a.group + r % a.group;
+  const long long out = static_cast<long long>(c.c0 + tok) * a.Hq + hq;
+  uint32_t w[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w[e] = pack2<BF16>(acc[2 * e] * inv, acc[2 * e + 1] * inv);
+  uint4* dst = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.o) + out * D + col);
+  dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+  if (col == 0 && a.lse != nullptr)
+    a.lse[static_cast<long long>(hq) * a.r.total + c.c0 + tok] = sum == 0.f ? -INFINITY : mx + logf(sum);
+}
+
+// The same in a pass of two, whose rows go to the workspace or are joined with the
+// first pass's.  Blocks x are for the
 // item that the end of run x cuts first, or, where there are fewer items than runs, for the
 // x-th item that is cut (256 blocks instead of 4700 for a step behind one prefix; those
 // without an item kept the next kernel from starting).  A thread has four columns of one
 // of its item's 256 rows, a warp 32 rows, and eight parts are on their way at a time.
-constexpr int kJoinThreads = 256;
 template <int D, bool BF16>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const __grid_constant__ ChunkParams p) {
+__global__ void __launch_bounds__(kJoinThreads) paged_part_join_kernel(const __grid_constant__ ChunkParams p) {
   const PagedAttn& a = p.a;
   ptx::launch_dependents();
   ptx::grid_dep_wait();
@@ -1208,10 +1261,32 @@ cudaError_t launch_expand_d(const ChunkParams& p, int kv, bool bf16, int grid, c
   return cudaGetLastError();
 }
 
+// PART: one of paged_part_join_kernel, else paged_join_kernel.
+template <int D, bool BF16, bool PART>
+cudaError_t launch_join(const ChunkParams& p, cudaStream_t stream) {
+  // may start while the last runs finish; it waits for them before it reads
+  cudaLaunchConfig_t cfg{};
+  const bool few = PART && p.max_items < p.n_ctas - 1 && p.n_ctas - 1 <= kJoinThreads;
+  cfg.gridDim = dim3(few ? p.max_items : p.n_ctas - 1, 2 * kBlockM * (D / (PART ? 4 : 16)) / kJoinThreads);
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if constexpr (PART) return cudaLaunchKernelEx(&cfg, paged_part_join_kernel<D, BF16>, p);
+  else return cudaLaunchKernelEx(&cfg, paged_join_kernel<D, BF16>, p);
+}
+
 }  // namespace
 
-cudaError_t launch_paged_chunk(const ChunkParams& p, int head_dim, int kv, bool bf16, int sms,
-                               cudaStream_t stream) {
+#if FA_PART_ROWS
+cudaError_t launch_paged_chunk_part(
+#else
+cudaError_t launch_paged_chunk(
+#endif
+    const ChunkParams& p, int head_dim, int kv, bool bf16, int sms, cudaStream_t stream) {
   if (kv >= FA_DTYPE_INT8) {
     // enough warps to fill the GPU; they walk the rows there are
     const long long units = p.exp_rows / 16 * p.n_heads;
@@ -1225,22 +1300,8 @@ cudaError_t launch_paged_chunk(const ChunkParams& p, int head_dim, int kv, bool 
   const cudaError_t e = head_dim == 64 ? launch_chunk_d<64>(p, kv, bf16, p.n_ctas, stream)
                                        : launch_chunk_d<128>(p, kv, bf16, p.n_ctas, stream);
   if (e != cudaSuccess || !p.runs || p.n_ctas == 1) return e;
-  // may start while the last runs finish; it waits for them before it reads
-  cudaLaunchConfig_t cfg{};
-  const bool few = p.max_items < p.n_ctas - 1 && p.n_ctas - 1 <= kJoinThreads;
-  cfg.gridDim = dim3(few ? p.max_items : p.n_ctas - 1, 2 * kBlockM * (head_dim / 4) / kJoinThreads);
-  cfg.blockDim = dim3(kJoinThreads);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (head_dim == 64)
-    return bf16 ? cudaLaunchKernelEx(&cfg, paged_join_kernel<64, true>, p)
-                : cudaLaunchKernelEx(&cfg, paged_join_kernel<64, false>, p);
-  return bf16 ? cudaLaunchKernelEx(&cfg, paged_join_kernel<128, true>, p)
-              : cudaLaunchKernelEx(&cfg, paged_join_kernel<128, false>, p);
+  if (head_dim == 64) return bf16 ? launch_join<64, true, kPartRows>(p, stream) : launch_join<64, false, kPartRows>(p, stream);
+  return bf16 ? launch_join<128, true, kPartRows>(p, stream) : launch_join<128, false, kPartRows>(p, stream);
 }
 
 }  // namespace fa

@@ -200,7 +200,7 @@ struct Partial {
   __device__ __forceinline__ void write(const PagedAttn& a, int tok, int hq, float up) const {
     const int lane = threadIdx.x & 31;
     const float inv = l == 0.f ? 0.f : up / l;
-    if (a.part != kPartNone) {
+    if (kPartRows && a.part != kPartNone) {
       const long long row = static_cast<long long>(tok) * a.Hq + hq;
       const float lse = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
       if (a.part == kPartFirst || a.part == kPartSecond) {
@@ -778,9 +778,9 @@ __device__ __forceinline__ void paged_decode_body(const DecodeParams& p) {
         if (first && last && !p.solo) {
           const int tok = s.c0 + r / a.group, hq = cc.h * a.group + r % a.group;
           const float inv = l[nt][c] == 0.f ? 0.f : kUp / l[nt][c];
-          const float lse_row =
-              l[nt][c] == 0.f ? -INFINITY : (m[nt][c] + (C::k8 ? 0.f : __log2f(l[nt][c]))) * 0.69314718055994530942f;
-          if (a.part != kPartNone) {
+          if (kPartRows && a.part != kPartNone) {
+            const float lse_row =
+                l[nt][c] == 0.f ? -INFINITY : (m[nt][c] + (C::k8 ? 0.f : __log2f(l[nt][c]))) * 0.69314718055994530942f;
             const long long row = static_cast<long long>(tok) * a.Hq + hq;
 #pragma unroll
             for (int k = 0; k < C::kKS; ++k) {
@@ -801,7 +801,9 @@ __device__ __forceinline__ void paged_decode_body(const DecodeParams& p) {
               dst[col(k, 1)] = static_cast<uint16_t>(w >> 16);
             }
           }
-          if (g == 0 && a.lse != nullptr) a.lse[static_cast<long long>(hq) * a.r.total + tok] = lse_row;
+          if (g == 0 && a.lse != nullptr)
+            a.lse[static_cast<long long>(hq) * a.r.total + tok] =
+                l[nt][c] == 0.f ? -INFINITY : (m[nt][c] + (C::k8 ? 0.f : __log2f(l[nt][c]))) * 0.69314718055994530942f;
         } else {
           // slot 0: continues the head of an earlier team; slot 1: begins one
 #pragma unroll
@@ -834,7 +836,7 @@ __device__ __forceinline__ void paged_decode_body(const DecodeParams& p) {
   }
   if (p.solo) {
     if (__syncthreads_and(ok ? 1 : 0) == 0) return;
-    if (p.early) ptx::grid_dep_wait();  // (the first pass's rows are read)
+    if (kPartRows && p.early) ptx::grid_dep_wait();  // (the first pass's rows are read)
     // one warp joins a row of the teams' slots
     constexpr int kSlotRows = 8 * NT * TEAM;
     const Seq s = load_short(a, b_first, p.max_rows);
@@ -858,7 +860,7 @@ template <int D, int KV, bool QBF16, int NT, int TEAM>
 __global__ void __launch_bounds__(32 * kWarps, ctas_per_sm(NT))
     paged_decode_kernel(const __grid_constant__ DecodeParams p) {
   paged_decode_body<D, KV, QBF16, NT, TEAM>(p);
-  if (p.early) ptx::grid_dep_wait();
+  if (kPartRows && p.early) ptx::grid_dep_wait();
 }
 
 // Joins the partial results of (sequence, KV head) blockIdx.x, query rows
@@ -883,7 +885,7 @@ __global__ void __launch_bounds__(kCombineThreads)
   __shared__ float sh_m[kW], sh_l[kW];
   const int b = blockIdx.x / a.c.heads, h = blockIdx.x % a.c.heads;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  ptx::launch_dependents();
+  if (kPartRows) ptx::launch_dependents();
   fill_outside(a, D, static_cast<int>(blockIdx.y * gridDim.x + blockIdx.x),
                static_cast<int>(gridDim.x * gridDim.y));
   const Seq s = load_short(a, b, p.max_rows);
@@ -900,7 +902,7 @@ __global__ void __launch_bounds__(kCombineThreads)
   const long long t0 = sp.before * a.c.heads + static_cast<long long>(h) * (n + kSegCost) + kSegCost;
   const int w0 = n > 0 ? static_cast<int>(t0 / per) : 0;
   const int w1 = n > 0 ? static_cast<int>((t0 + n - 1) / per) : -1;
-  if (w0 == w1 && a.part != kPartRuns) return;  // one team had it all
+  if (w0 == w1 && (!kPartRows || a.part != kPartRuns)) return;  // one team had it all
   const long long stride = slot_floats(slot_rows, D);
   // slots first, first + step, ... of row `row`
   auto gather = [&](int row, int first, int step) {
@@ -941,7 +943,7 @@ __global__ void __launch_bounds__(kCombineThreads)
   auto finish = [&](int row, const Partial<D>& r) {
     r.template write<BF16>(a, s.c0 + row / a.group, h * a.group + row % a.group, up);
   };
-  if (w0 == w1) {  // ... and left it as a result
+  if (kPartRows && w0 == w1) {  // ... and left it as a result
     for (int r = warp; r < rows; r += kW) {
       const int y = row0 + r;
       const long long row = static_cast<long long>(s.c0 + y / a.group) * a.Hq + h * a.group + y % a.group;
@@ -1007,7 +1009,7 @@ cudaError_t launch_impl(const DecodeParams& p, int n_ctas, cudaStream_t stream) 
   first.dynamicSmemBytes = C::smem(p.stages);
   first.stream = stream;
   first.attrs = early;
-  first.numAttrs = p.early ? 1 : 0;
+  first.numAttrs = kPartRows && p.early ? 1 : 0;
   const cudaError_t e = cudaLaunchKernelEx(&first, kern, p);
   if (e != cudaSuccess || p.solo) return e;
   // the combine may start while the last teams finish; it waits for them
@@ -1068,6 +1070,7 @@ cudaError_t launch_d(const DecodeParams& p, int kv, bool bf16, int n_ctas, cudaS
 }  // namespace pdec
 }  // namespace
 
+#if !FA_PART_ROWS
 // Query rows per (sequence, KV head) up to which this kernel is taken.  Over
 // 8-bit pages always kRowsMax, for the chunk kernel has to expand them first
 // (B=8, 8192 keys, 8 KV heads, d = 128, int8, 64 rows: 106 us here, 150 there; 32
@@ -1079,6 +1082,7 @@ cudaError_t launch_d(const DecodeParams& p, int kv, bool bf16, int n_ctas, cudaS
 int paged_decode_rows(long long heads, int head_dim, int kv, int sms) {
   return kv >= FA_DTYPE_INT8 || (head_dim == 64 && 2 * heads < sms) ? pdec::kRowsMax : 32;
 }
+#endif
 
 namespace {
 namespace pdec {
@@ -1106,15 +1110,21 @@ bool is_solo(long long heads, int max_rows, int max_k, int head_dim, int kv, int
 }  // namespace pdec
 }  // namespace
 
+#if !FA_PART_ROWS
 size_t paged_decode_ws_bytes(long long heads, int max_rows, int max_k, int head_dim, int kv, int sms) {
   if (pdec::is_solo(heads, max_rows, max_k, head_dim, kv, sms)) return 0;
   const pdec::Team t = pdec::team_for(max_rows);
   const size_t teams = static_cast<size_t>(sms) * pdec::ctas_per_sm(t.nt) * (pdec::kWarps / t.warps);
   return 2 * teams * static_cast<size_t>(pdec::slot_floats(8 * t.nt * t.warps, head_dim)) * sizeof(float);
 }
+#endif
 
-cudaError_t launch_paged_decode(DecodeParams p, int head_dim, int kv, bool bf16, int sms,
-                                cudaStream_t stream) {
+#if FA_PART_ROWS
+cudaError_t launch_paged_decode_part(
+#else
+cudaError_t launch_paged_decode(
+#endif
+    DecodeParams p, int head_dim, int kv, bool bf16, int sms, cudaStream_t stream) {
   const pdec::Team t = pdec::team_for(p.max_rows);
   const int per_cta = pdec::kWarps / t.warps;
   // no more teams than units there can be

@@ -81,7 +81,7 @@ __device__ __forceinline__ Joined join_passes(float lse_first, float lse_own) {
 // threads of a block call it.)
 __device__ __forceinline__ void fill_row(const PagedAttn& a, int d, int t) {
   const int n = static_cast<int>(blockDim.x);
-  if (a.part == kPartFirst || a.part == kPartSecond) {
+  if (kPartRows && (a.part == kPartFirst || a.part == kPartSecond)) {
     const float none = a.part == kPartFirst ? -INFINITY : __uint_as_float(kNoRow);
     for (int i = threadIdx.x; i < a.Hq * d; i += n) *a.part_at(static_cast<long long>(t) * a.Hq + i / d, i % d) = 0.f;
     for (int i = threadIdx.x; i < a.Hq; i += n) a.part_lse[static_cast<long long>(t) * a.Hq + i] = none;
