@@ -136,7 +136,7 @@ __device__ __forceinline__ float4 load_scales(uint32_t addr) {
   return f;
 }
 
-// exp_tile (fa_fwd_sm100.cu) with P multiplied by V's scales: e = 2^(x sl - ref)
+// exp_tile (fa_device.cuh) with P multiplied by V's scales: e = 2^(x sl - ref)
 // is summed as it is, e * vs goes to tensor memory.
 template <bool kEmulate, int kPeriod, typename Announce>
 __device__ __forceinline__ float exp_tile_scaled(const float (&x)[kBlockN], float sl, float neg_ref,

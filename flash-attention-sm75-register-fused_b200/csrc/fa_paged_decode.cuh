@@ -1,6 +1,7 @@
 // Attention of a few new tokens per sequence over a paged KV cache: at most 64
 // query rows per (sequence, KV head), i.e. new tokens x query heads of a group.
-// Included by fa_fwd_sm100.cu (bounded mbarrier waits, device status word).
+// Included by fa_fwd_sm100.cu and fa_paged_prefix.cu (fa_device.cuh has the bounded
+// mbarrier waits and the device status word).
 //
 //   s_ij = scale q_i . k_j,   O_i = sum_j softmax(s_i)_j v_j,
 //   LSE_i = log sum_j exp(s_ij)

@@ -10,13 +10,18 @@
 //           its positions in shared memory, and all add up the cluster's counts.
 //   place   The cluster walks the positions, 2048 per CTA and step; two ranks (of
 //           equal weights, of what stays) and the CTAs' counts give every kept one
-//           its place, and its page and row go to the list of the CTA that moves it.
+//           its place, and its page and position go to the list of the CTA that moves it.
 //   move    Places in ascending order, a group at a time: all of a group are loaded
 //           before any is stored, and as the i-th kept position is at least i, nothing
 //           is overwritten that a later group reads.  So the next group's loads are on
 //           their way while this one is stored.
 // Bound by memory: the weights are read once (the first kCacheSteps x 2048 of a CTA stay in
-// shared memory), rows that move are read and written once.  @@
+// shared memory), rows that move are read and written once.  Measured, 8 KV heads, d = 128:
+// 32 ragged caches of up to 8192 bf16 positions cut to 2048, 187 MB moved, 74 us (29 at the
+// rate of a plain copy: three passes of selection and the places take 16, and the clusters run
+// in two rounds); 2 x 65536 int8 positions to 16384, 173 MB, 122 us (16 clusters of 8 on 128
+// SMs, 4 TB/s while rows move); 1 x 1024 to 512 16 us, all latency.  A CTA alone per head, with
+// 1024 positions' rows moved as they are found, took 80, 328 and 19 us.
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -34,6 +39,8 @@ constexpr int kChunk = kEach * kEvictThreads;     // ... of a CTA
 constexpr int kCacheSteps = 6;
 constexpr int kList = 4096;                       // places of a CTA
 constexpr int kMaxCluster = 8;
+// CTAs that share a head: up to this many for every SM in all (a ragged batch's short sequences
+// leave at once).  32 ragged sequences x 8 heads with 2 / 4 / 8: 119 / 74 / 79 us.
 constexpr long long kClusterLoad = 4;
 
 // Integer that orders as the weights do: -0 as 0, a NaN below all.

@@ -1,6 +1,6 @@
 // Attention weight that cached keys receive from chunks of new tokens (more query
-// rows per KV head than fa_paged_weights.cu streams).  Included by fa_fwd_sm100.cu, whose
-// bounded mbarrier waits and device status word it uses.
+// rows per KV head than fa_paged_weights.cu streams).  Included by fa_paged_prefix.cu;
+// fa_device.cuh has the bounded mbarrier waits and the device status word.
 //
 //   w_j = sum_i 2^(s'_ij - L'_i)    s' = scale log2(e) q_i . k_j,  L' = log2(e) LSE_i
 //
@@ -23,7 +23,7 @@
 // Bound by the exponentials: 128 x 256 of them take the special-function unit 2048 cycles,
 // the two products about 1100.  kFmaPairs of 16 pairs go to the FMA pipe instead (0 / 2 / 4
 // / 6 of 16: 239 / 226 / 216 / 235 us for 2 x 1024 tokens over 8192 keys, bf16, d = 128, GQA
-// 4).  Now 207 us there: the unit is busy for 51 %, the issue slots for 52 %; what is left
+// 4).  Now 207 us there: the unit is busy for 54 %, the issue slots for 55 %; what is left
 // is the latency between a tile's arrival and its last sum.  CTAs that walk several key
 // blocks, with the next one's keys loaded by a warp of their own, took as long (the
 // registers that this takes spill), and so did two CTAs of one key tile per SM.

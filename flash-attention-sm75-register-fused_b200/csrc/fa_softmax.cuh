@@ -1,5 +1,5 @@
 // Register-softmax building blocks of the attention forward, shared by the
-// kernel (fa_fwd_sm100.cu) and the stage tests (fa_selftest.cu): the
+// kernels (by fa_device.cuh) and the stage tests (fa_selftest.cu): the
 // three-input row max, and exp2(s * scale_log2 - m) for a pair of scores with
 // a fixed fraction of the pairs on the FMA-pipe polynomial instead of MUFU.
 //

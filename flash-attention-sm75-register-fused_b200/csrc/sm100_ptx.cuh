@@ -4,7 +4,7 @@
 //
 // Every wait in this file is bounded: callers pass a WaitCtl whose deadline
 // (ns of %globaltimer) turns a lost arrival into an error code instead of a
-// hang.  See fa_fwd_sm100.cu for how the error is propagated and drained.
+// hang.  See fa_device.cuh for how the error is propagated and drained.
 #pragma once
 #include <cstdint>
 #include <cuda_runtime.h>

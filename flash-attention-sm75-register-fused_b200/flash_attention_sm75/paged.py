@@ -134,6 +134,12 @@ def flash_attention_forward_paged_prefix(q, k_cache, v_cache, prefix_table, cu_p
         max_prefix_q, max_prefix_k: upper bounds of a prefix's tokens and keys
             (tokens beyond do not see it, keys beyond are not seen)
 
+    It pays where many sequences of few tokens share a long prefix (64 tokens
+    behind 8192 keys: 63 us instead of 143 with the prefix's pages at the head
+    of every table); a few sequences behind a short one (8 behind 1024: 21 / 16),
+    and chunks that fill tiles by themselves (8 x 512 behind 8192: 540 / 498),
+    are a little faster with tables that begin with the prefix's (whole) pages.
+
     A token sees all keys of its prefix, and those of its own sequence that
     ``causal`` leaves.  Rows that see no key, rows of no sequence and tokens
     beyond max_seqlen_q return O = 0, LSE = -inf.
