@@ -3,7 +3,12 @@ leave one batch, prompts are prefilled in chunks beside the decode steps of the
 others, and every step is two calls for the whole batch: write the new tokens'
 keys and values, then attend.
 
-    python examples/paged_serving.py [--pages same|int8|e4m3] [--steps N]
+    python examples/paged_serving.py [--pages same|int8|e4m3] [--steps N] [--budget N]
+
+With a budget every request's cache is cut to that many tokens whenever it has grown
+a quarter beyond: the attention weight that each key received is summed over the
+steps (``kvcache_weights_paged``), and those with the least go
+(``kvcache_evict_paged``), but for the first four and the most recent.
 
 The "model" is one attention layer with random projections and a token drawn
 from its output, enough to have real data flow through the cache.  At the end
@@ -55,6 +60,7 @@ class Request:
         self.length = 0           # tokens in the cache
         self.pages = []
         self.drawn = []
+        self.sums = None          # attention weight of its keys, where a budget asks for it
 
 
 class Layer:
@@ -74,7 +80,43 @@ class Layer:
         return x[:, :HQ], x[:, HQ:HQ + HKV], x[:, HQ + HKV:]
 
 
-def step(layer, cache, batch, chunk):
+def add_weights(cache, batch, q, lse, table, cu, lens, new):
+    """Adds what the step's tokens gave to the batch's keys to the requests' sums."""
+    held = table.size(1) * PAGE
+    sums = torch.zeros(len(batch), HKV, held, device=q.device)
+    for i, r in enumerate(batch):
+        if r.sums is not None:
+            n = min(held, r.sums.size(1))
+            sums[i, :, :n] = r.sums[:, :n]
+    fa.kvcache_weights_paged(q, lse, cache.k, table, cu, lens, max(len(n) for n in new),
+                             max(r.length for r in batch), sums, causal=True,
+                             k_scale=cache.scales.get("k_scale"))
+    for i, r in enumerate(batch):
+        r.sums = sums[i]
+
+
+def evict(cache, batch, budget):
+    """Cuts the caches that have grown a quarter beyond the budget."""
+    full = [r for r in batch if r.length > budget + budget // 4]
+    if not full:
+        return
+    dev = cache.k.device
+    width = max(len(r.pages) for r in full)
+    table = torch.tensor([r.pages + [-1] * (width - len(r.pages)) for r in full], dtype=torch.int32).to(dev)
+    sums = torch.zeros(len(full), HKV, width * PAGE, device=dev)
+    for i, r in enumerate(full):
+        n = min(width * PAGE, r.sums.size(1))
+        sums[i, :, :n] = r.sums[:, :n]
+    lens = fa.kvcache_evict_paged(cache.k, cache.v, sums, table, [r.length for r in full], budget,
+                                  recent=budget // 4, first=4, **cache.scales).tolist()
+    for i, r in enumerate(full):
+        r.length, r.sums = lens[i], sums[i]
+        keep = -(-r.length // PAGE)
+        cache.free.extend(r.pages[keep:])
+        del r.pages[keep:]
+
+
+def step(layer, cache, batch, chunk, budget=0):
     """One step of a batch: up to `chunk` prompt tokens, or one drawn token, of
     every request.  Returns the tokens drawn."""
     dev = cache.k.device
@@ -93,9 +135,11 @@ def step(layer, cache, batch, chunk):
     cu_dev = torch.tensor(cu, dtype=torch.int32).to(dev)
     q, k, v = layer.project(torch.tensor([t for n in new for t in n]).to(dev))
     fa.kvcache_write_paged(k, v, cache.k, cache.v, table, cu_dev, lens, **cache.scales)
-    o = fa.flash_attention_forward_paged(q, cache.k, cache.v, table, cu_dev, lens,
-                                         max(len(n) for n in new), max(r.length for r in batch),
-                                         causal=True, **cache.scales)
+    o, lse = fa.flash_attention_forward_paged(q, cache.k, cache.v, table, cu_dev, lens,
+                                              max(len(n) for n in new), max(r.length for r in batch),
+                                              causal=True, return_lse=True, **cache.scales)
+    if budget:
+        add_weights(cache, batch, q, lse, table, cu_dev, lens, new)
     last = o[torch.tensor(cu[1:]).to(dev) - 1].reshape(len(batch), HQ * D)
     drawn = (last @ layer.out).argmax(-1).tolist()
     for r, t in zip(batch, drawn):
@@ -119,7 +163,7 @@ def check(cache, batch, q, o, table, lens, cu):
     return (ref.float() - o[rows].float()).abs().max().item()
 
 
-def serve(pages="int8", steps=40, chunk=96, device="cuda", verbose=True):
+def serve(pages="int8", steps=40, chunk=96, device="cuda", verbose=True, budget=0):
     """Runs the loop; returns (tokens drawn per request, largest difference seen)."""
     cache = PagedCache(512, PAGES[pages], device)
     layer = Layer(device)
@@ -133,11 +177,13 @@ def serve(pages="int8", steps=40, chunk=96, device="cuda", verbose=True):
     for i in range(steps):
         if waiting and len(batch) < 4:
             batch.append(waiting.pop(0))
-        state = step(layer, cache, batch, chunk)
+        state = step(layer, cache, batch, chunk, budget)
         worst = max(worst, check(cache, batch, *state))
         if verbose:
             print(f"step {i:2d}: {len(batch)} requests, {state[4][-1]:3d} new tokens, "
                   f"{sum(r.length for r in batch):4d} cached")
+        if budget:
+            evict(cache, batch, budget)
         for r in [r for r in batch if not r.todo]:
             batch.remove(r)
             cache.release(r.pages)
@@ -153,5 +199,6 @@ if __name__ == "__main__":
     ap = argparse.ArgumentParser(description=__doc__.splitlines()[0])
     ap.add_argument("--pages", choices=sorted(PAGES), default="int8")
     ap.add_argument("--steps", type=int, default=60)
+    ap.add_argument("--budget", type=int, default=0)
     args = ap.parse_args()
-    serve(args.pages, args.steps)
+    serve(args.pages, args.steps, budget=args.budget)
