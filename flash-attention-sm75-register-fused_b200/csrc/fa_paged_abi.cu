@@ -322,11 +322,17 @@ int check_query_strides(int Hq, int total, long long q_token, long long q_head) 
   return (total > 1 && q_token <= 0) || (Hq > 1 && q_head <= 0) ? FA_ERR_STRIDE : FA_OK;
 }
 
-// Summed weights: fp32 rows of at least `need` positions that do not overlap.
+// Summed weights: fp32 rows of at least `need` positions that do not overlap: all
+// heads of a sequence before the next sequence, or all sequences of a head before
+// the next head.
 int check_sums(const float* w, long long seq, long long head, int len, int need, int B, int heads) {
   if (len < need || len < 0 || (B > 0 && len > 0 && !w)) return FA_ERR_INVALID_ARG;
   if (reinterpret_cast<uintptr_t>(w) & 3u) return FA_ERR_ALIGNMENT;
   if ((B > 1 && seq < len) || (heads > 1 && head < len)) return FA_ERR_STRIDE;
+  const __int128 n = len;
+  if (B > 1 && heads > 1 && len > 0 && seq < (heads - 1) * static_cast<__int128>(head) + n &&
+      head < (B - 1) * static_cast<__int128>(seq) + n)
+    return FA_ERR_STRIDE;
   return FA_OK;
 }
 

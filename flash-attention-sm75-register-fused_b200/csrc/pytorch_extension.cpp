@@ -754,8 +754,13 @@ void check_weights(const torch::Tensor& w, int B, const fa_paged_cache& c, const
   TORCH_CHECK_VALUE(w.dim() == 3 && w.size(0) == B && w.size(1) == c.kv_heads, "weights must be [", B, ", ",
                     c.kv_heads, ", L] for this cache");
   TORCH_CHECK(w.size(2) <= INT32_MAX, "size exceeds int32");
+  // (all heads of a sequence before the next sequence, or all sequences of a head before the next head)
+  const int64_t last_seq = std::max<int64_t>(w.size(0) - 1, 0) * w.stride(0);
+  const int64_t last_head = std::max<int64_t>(w.size(1) - 1, 0) * w.stride(1);
   TORCH_CHECK((w.size(2) <= 1 || w.stride(2) == 1) && (w.size(0) <= 1 || w.stride(0) >= w.size(2)) &&
-                  (w.size(1) <= 1 || w.stride(1) >= w.size(2)),
+                  (w.size(1) <= 1 || w.stride(1) >= w.size(2)) &&
+                  (w.size(0) <= 1 || w.size(1) <= 1 || w.stride(0) >= last_head + w.size(2) ||
+                   w.stride(1) >= last_seq + w.size(2)),
               "the rows of weights must be contiguous and must not overlap");
 }
 

@@ -178,3 +178,16 @@ def test_plain_eviction():
     for i, j in enumerate(at):
         (pg, row), (dpg, drow) = P.place(0, j), P.place(0, i)
         assert torch.equal(v[dpg, 0, drow], P.v[pg, 0, row])
+
+
+@pytest.mark.parametrize("call", [_weights, _evict])
+def test_rows_of_sums_that_overlap(call):
+    """Strides of at least a row, but rows of one sequence on those of another: refused.  One after
+    the other, in either order, they are accepted (no work here: no sequences)."""
+    for ws, wh in ((64, 64), (100, 64), (64, 100), (127, 64), (64, 127), (1 << 62, 1 << 62)):
+        overlap = not (ws >= wh + 64 or wh >= ws + 64)
+        assert overlap and call(_cache(kv_heads=2), ws=ws, wh=wh) == 15, (ws, wh)
+    assert call(_cache(kv_heads=2), ws=64, wh=64, B=0) == 0
+    if not torch.cuda.is_available():  # (the check of the device comes after that of the strides)
+        for ws, wh in ((128, 64), (64, 128), (1 << 62, 64)):
+            assert call(_cache(kv_heads=2), ws=ws, wh=wh) not in (0, 15), (ws, wh)
