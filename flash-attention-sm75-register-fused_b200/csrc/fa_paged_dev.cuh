@@ -65,13 +65,15 @@ __device__ __forceinline__ Seq load_seq(const PagedAttn& a, int b) {
 }
 
 // Result of a row of the second pass with that of the first: O = own O_2 + first
-// O_1, LSE.  (Without keys in a set its weight is 0; without any, all are.)
+// O_1, LSE.  (Without keys in a set its weight is 0; without any, all are.  A NaN of either
+// set stays one, also beside a set without keys: the maximum of NaN and -inf is -inf, so
+// it does not tell rows without keys.)
 struct Joined {
   float own, first, lse;
 };
 __device__ __forceinline__ Joined join_passes(float lse_first, float lse_own) {
+  if (lse_first == -INFINITY && lse_own == -INFINITY) return {0.f, 0.f, -INFINITY};
   const float m = fmaxf(lse_first, lse_own);
-  if (m == -INFINITY) return {0.f, 0.f, -INFINITY};
   const float f1 = expf(lse_first - m), f2 = expf(lse_own - m);
   const float sum = f1 + f2;
   return {f2 / sum, f1 / sum, m + logf(sum)};

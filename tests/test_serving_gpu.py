@@ -776,3 +776,39 @@ def test_example_with_a_budget(sm100, pages):
     assert max(seen) <= 80 and 64 in seen
     # values of a few units: bf16 results and bf16 keys read back differ by a few roundings of 2^-8
     assert worst <= 0.06
+
+
+# ---------------------------------------------------------------- what is not a number
+
+# tokens: some behind the prefix alone, behind both, with own keys alone, without any
+NAN = [
+    ([(1, 0), (1, 200), (1, 200), (1, 0)], [0, 2], [300], 8, 2),                                # a CTA per head joins
+    ([(1, 0), (1, 200)] * 40 + [(1, 200), (1, 0)] * 40, [0, 80], [700], 8, 2),                  # runs, combined
+    ([(200, 200), (1, 0), (200, 0), (200, 200), (1, 0), (200, 0)], [0, 3], [300], 8, 2),        # chunks
+    ([(200, 200), (1, 0), (1, 200), (200, 200), (1, 0), (1, 200), (9, 0)], [0, 3], [300], 8, 2),  # both kernels, merged
+]
+
+
+@pytest.mark.parametrize("kind", KINDS, ids=KIND_IDS)
+@pytest.mark.parametrize("case", NAN, ids=["solo", "runs", "chunks", "both"])
+def test_prefix_passes_nan_on(sm100, case, kind):
+    """A NaN query returns NaN from whichever set of keys it sees, as from the plain call; without any
+    key it returns O = 0, LSE = -inf; the other rows do not change."""
+    lens, cuts, prefixes, Hq, Hkv = case
+    io, cache = kind
+    P = with_prefixes(lens, prefixes, Hkv, 128, 16, cache, io=io, seed=21)
+    q = P.new(Hq)
+    rows = [P.cu[x] for x in cuts]
+    c = P.cuda()
+    clean = _attend(P, q, rows, 0, c)
+    _check(P, q, Hq, rows, 0, clean)
+    q[:, 1] = math.nan
+    q[::2, 5, 7] = math.nan
+    o, lse = _attend(P, q, rows, 0, c)
+    sees = torch.isfinite(clean[1]).cpu()                              # [Hq, total]
+    bad = q.isnan().any(-1).T & sees
+    assert bad.any() and (~sees).any()
+    assert torch.equal(lse.isnan().cpu(), bad)
+    assert o.isnan().all(-1).cpu()[bad.T].all()
+    ok = ~bad.cuda()
+    assert torch.equal(lse[ok], clean[1][ok]) and torch.equal(o[ok.T], clean[0][ok.T])
