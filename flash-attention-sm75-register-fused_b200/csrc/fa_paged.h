@@ -161,7 +161,9 @@ constexpr int paged_weights_rows() { return 32; }
 cudaError_t launch_paged_weights(const PagedWeights& p, int max_rows, int head_dim, int cache_dtype, bool bf16,
                                  int sms, cudaStream_t stream);
 
-// ... and those of more than skip_rows rows (fa_paged_weights_chunk.cuh).
+// ... and those of more than skip_rows rows (fa_paged_weights_chunk.cuh), a CTA or a cluster per
+// paged_weights_chunk_keys() keys of a (sequence, head): at most 2^31 - 1 of them.
+constexpr int paged_weights_chunk_keys() { return 256; }
 struct alignas(64) WeightsChunkParams {
   CUtensorMap tm_q;  // (d, Hq, T), box (64, G, tq)
   PagedWeights w;

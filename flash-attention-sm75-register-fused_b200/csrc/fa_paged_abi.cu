@@ -634,27 +634,27 @@ int fa_kvcache_weights(const fa_paged_cache* cache, const void* Q, long long q_t
   if (int rc = check_query_strides(Hq, total_q, q_token_stride, q_head_stride)) return rc;
   if (static_cast<long long>(B) * p.a.c.heads > 0x7fffffffLL || static_cast<long long>(total_q) * Hq > (1LL << 33))
     return FA_ERR_TOO_LARGE;
+  // Sequences of few query rows are streamed, the others go through the tensor cores; both
+  // where the bounds allow both (see kMixedRows).
+  const int most = max_seqlen_q < total_q ? max_seqlen_q : total_q, group = Hq / p.a.c.heads;
+  const bool chunk = static_cast<long long>(most) * group > fa::paged_weights_rows();
+  const bool few = !chunk || (B > 1 && group <= kMixedRows && total_q < static_cast<long long>(B) * most);
+  const int few_rows = chunk ? kMixedRows / group * group : most * group;
+  const long long blocks = (static_cast<long long>(keys) + fa::paged_weights_chunk_keys() - 1) / fa::paged_weights_chunk_keys();
+  if (chunk && blocks * B * p.a.c.heads > 0x7fffffffLL) return FA_ERR_TOO_LARGE;
   if (int rc = fa::host_check_device()) return rc;
   set_queries(&p.a, cache, Q, q_token_stride, q_head_stride, Hq, max_seqlen_q, keys, scale, causal);
-  p.a.o = nullptr;
   p.a.lse = const_cast<float*>(lse);
   p.w = weights;
   p.w_seq = w_seq_stride;
   p.w_head = w_head_stride;
   p.mode = mode;
-  // Sequences of few query rows are streamed, the others go through the tensor cores; both
-  // where the bounds allow both (see kMixedRows).
   const bool bf16 = dtype == FA_DTYPE_BF16;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int most = max_seqlen_q < total_q ? max_seqlen_q : total_q, group = p.a.group;
-  const bool chunk = static_cast<long long>(most) * group > fa::paged_weights_rows();
-  const bool few = !chunk || (B > 1 && group <= kMixedRows && total_q < static_cast<long long>(B) * most);
-  const int few_rows = chunk ? kMixedRows / group * group : most * group;
-  if (few && fa::launch_paged_weights(p, few_rows, cache->head_dim, cache->dtype, bf16, fa::host_sm_count(), st) !=
-                 cudaSuccess)
-    return FA_ERR_LAUNCH;
+  // (everything that can be refused is, before the first kernel changes a sum: with "add" or
+  // "append" the call could not be made again)
+  fa::WeightsChunkParams c;
   if (chunk) {
-    fa::WeightsChunkParams c;
     c.w = p;
     c.tq = 128 / group;
     c.skip_rows = few ? few_rows : -1;
@@ -662,9 +662,13 @@ int fa_kvcache_weights(const fa_paged_cache* cache, const void* Q, long long q_t
     c.timeout_ns = fa::host_timeout_ns();
     if (!query_map(*cache, c.tq, Q, q_token_stride, q_head_stride, Hq, total_q, bf16, &c.tm_q))
       return FA_ERR_TENSOR_MAP;
-    if (fa::launch_paged_weights_chunk(c, cache->head_dim, cache->dtype, bf16, fa::host_sm_count(), st) != cudaSuccess)
-      return FA_ERR_LAUNCH;
   }
+  if (few && fa::launch_paged_weights(p, few_rows, cache->head_dim, cache->dtype, bf16, fa::host_sm_count(), st) !=
+                 cudaSuccess)
+    return FA_ERR_LAUNCH;
+  if (chunk &&
+      fa::launch_paged_weights_chunk(c, cache->head_dim, cache->dtype, bf16, fa::host_sm_count(), st) != cudaSuccess)
+    return FA_ERR_LAUNCH;
   return FA_OK;
 }
 

@@ -35,7 +35,7 @@ namespace {
 namespace pwc {
 
 constexpr int kThreads = 608;
-constexpr int kKeys = 256;   // of a CTA
+constexpr int kKeys = paged_weights_chunk_keys();  // of a CTA
 constexpr int kExps = 512;   // threads of the exponentials: two per key, for half of a tile's rows each
 constexpr int kWarpTma = 16, kWarpMma = 17, kWarpRows = 18;
 constexpr int kRowRing = 4;
@@ -478,14 +478,14 @@ cudaError_t launch_paged_weights_chunk(WeightsChunkParams p, int head_dim, int c
   const int max_q = p.w.a.max_q < p.w.a.r.total ? p.w.a.max_q : p.w.a.r.total;
   const int tiles = (max_q + p.tq - 1) / p.tq;
   long long best = 0;
-  for (int x = 1; x <= pwc::kMaxSplit && x <= tiles; x *= 2) {
+  for (int x = 1; x <= pwc::kMaxSplit && x <= tiles && items * x <= 0x7fffffffLL; x *= 2) {
     const long long cost = (items * x + sms - 1) / sms * (6 + (tiles + x - 1) / x);
     if (x == 1 || cost < best) {
       best = cost;
       p.split = x;
     }
   }
-  if (items * p.split > 0x7fffffffLL) return cudaErrorInvalidValue;
+  if (items > 0x7fffffffLL) return cudaErrorInvalidValue;  // (refused before)
   return head_dim == 64 ? pwc::launch_d<64>(p, cache_dtype, bf16, stream)
                         : pwc::launch_d<128>(p, cache_dtype, bf16, stream);
 }

@@ -191,3 +191,16 @@ def test_rows_of_sums_that_overlap(call):
     if not torch.cuda.is_available():  # (the check of the device comes after that of the strides)
         for ws, wh in ((128, 64), (64, 128), (1 << 62, 64)):
             assert call(_cache(kv_heads=2), ws=ws, wh=wh) not in (0, 15), (ws, wh)
+
+
+def test_weights_of_more_key_blocks_than_a_grid_has():
+    """2^20 sequences x 16 heads x 2^16 keys (or one head of 2^30): chunks would take 2^32 blocks of 256
+    keys.  Refused before any kernel runs (single tokens come first where a batch has both)."""
+    many = dict(B=1 << 20, L=1 << 16, max_k=1 << 16, ws=1 << 40, wh=1 << 17)
+    big = dict(kv_heads=16, max_pages=1 << 12)
+    assert _weights(_cache(**big), Hq=64, total=3000, max_q=1000, **many) == 10
+    assert _weights(_cache(**big), Hq=64, total=1000, max_q=1000, **many) == 10
+    one = dict(B=1 << 10, L=1 << 30, max_k=1 << 30, ws=1 << 40, wh=1 << 31)
+    assert _weights(_cache(kv_heads=1, max_pages=1 << 26), Hq=4, total=3000, max_q=1000, **one) == 10
+    if not torch.cuda.is_available():  # streams of few rows have no such limit (the device is checked afterwards)
+        assert _weights(_cache(**big), Hq=64, total=1 << 20, max_q=1, **many) not in (0, 10)
