@@ -544,14 +544,16 @@ fa_paged_cache paged_cache(const torch::Tensor& k, const torch::Tensor& v,
 }
 
 // int32 tensor with contiguous rows on `device` from a tensor (itself where it
-// is one) or a sequence of ints.
-torch::Tensor as_ints(pybind11::handle h, const torch::Device& device) {
+// is one) or a sequence of ints.  `counts`: numbers that int32 does not hold become
+// the largest or the least that it does (else they wrap).
+torch::Tensor as_ints(pybind11::handle h, const torch::Device& device, bool counts = false) {
   torch::Tensor x;
   if (THPVariable_Check(h.ptr())) {
     x = THPVariable_Unpack(h.ptr());
   } else {
     x = pybind11::module_::import("torch").attr("as_tensor")(h).cast<torch::Tensor>();
   }
+  if (counts && x.scalar_type() == torch::kInt64) x = x.clamp(INT32_MIN, INT32_MAX);
   const bool rows = x.dim() == 0 || x.size(-1) <= 1 || x.stride(-1) == 1;
   if (x.scalar_type() == torch::kInt32 && x.device() == device && rows) return x;
   return x.to(torch::TensorOptions().dtype(torch::kInt32).device(device)).contiguous();
@@ -824,7 +826,7 @@ torch::Tensor kvcache_evict_paged(const torch::Tensor& k_cache, const torch::Ten
   if (pybind11::isinstance<pybind11::int_>(keep_in)) {
     keep_all = keep_in.cast<int64_t>();
   } else {
-    keep = as_ints(keep_in, device);
+    keep = as_ints(keep_in, device, /*counts=*/true);
     if (keep.dim() == 0) keep = keep.expand({B}).contiguous();
     TORCH_CHECK(keep.is_contiguous() && keep.dim() == 1 && keep.size(0) == B,
                 "keep must be one number of positions, or one for each sequence");

@@ -203,7 +203,8 @@ def kvcache_evict_paged(k_cache, v_cache, weights, block_table, seqlens_k, keep,
             ``kvcache_write_paged``; no page may belong to two sequences
         weights: fp32 [B, H_kv, L] (``kvcache_weights_paged``), L at least the
             positions of a table row
-        keep: positions that stay, one int for all or B of them
+        keep: positions that stay, one int for all or B of them (of these a
+            negative one counts as 0)
         recent, first: the last `recent` and the first `first` positions stay
             whatever their weight (`first` comes first where keep is too small)
 

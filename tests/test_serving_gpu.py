@@ -812,3 +812,20 @@ def test_prefix_passes_nan_on(sm100, case, kind):
     assert o.isnan().all(-1).cpu()[bad.T].all()
     ok = ~bad.cuda()
     assert torch.equal(lse[ok], clean[1][ok]) and torch.equal(o[ok.T], clean[0][ok.T])
+
+
+@pytest.mark.parametrize("where", ["list", "cpu", "cuda"])
+def test_evict_budgets_beyond_int32(sm100, where):
+    """A number of positions that int32 does not hold keeps everything, alone or for each sequence."""
+    P = Paged([(0, 40), (0, 90), (0, 33)], 2, 64, 16, F16, seed=2)
+    w = _sums(P, seed=2)
+    for big in (1 << 31, 1 << 32, (1 << 32) + 5, 1 << 62):
+        keep = [big, 20, big]
+        c = P.cuda()
+        wd = w.cuda()
+        lens = fa.kvcache_evict_paged(c["k_cache"], c["v_cache"], wd, c["table"], c["lens"],
+                                      keep if where == "list" else torch.tensor(keep, device=where), recent=3)
+        _check_evict(P, w, keep, 3, 0, (c, wd, lens))
+        c = P.cuda()
+        lens = fa.kvcache_evict_paged(c["k_cache"], c["v_cache"], wd, c["table"], c["lens"], big)
+        assert lens.tolist() == [40, 90, 33]
