@@ -157,3 +157,31 @@ def evicted(P, weights, keep, recent, first):
                     x[dpg, h, drow] = held[pg, h, row]
             w[b, h, :kp] = weights[b, h, at]
     return (*out, w, lens)
+
+
+def evicted_whole(c, table, w, lens, keep, recent, first, page):
+    """The same for long caches: whole sequences at a time, bit by bit.  c: name -> [pages, Hkv, page,
+    ...] (or None) on any device; returns (caches, weights)."""
+    out = {x: None if y is None else y.clone() for x, y in c.items()}
+    w2 = w.clone()
+    h = torch.arange(w.size(1), device=w.device)[:, None]
+    for b, n in enumerate(lens):
+        if n <= keep:
+            continue
+        f = min(first, keep)
+        r = min(recent, keep - f)
+        x = w[b, :, :n].double() + 0.0  # (-0 is 0)
+        # (beyond every fp32 number: what stays whatever its weight above +inf, a NaN below -inf)
+        x = torch.where(x == math.inf, 1e39, torch.where(x == -math.inf, -1e39, x))
+        x = torch.where(x.isnan(), -math.inf, x)
+        x[:, :f] = math.inf
+        x[:, n - r:] = math.inf
+        best = torch.sort(x, dim=-1, descending=True, stable=True).indices[:, :keep]
+        at = torch.sort(best, dim=-1).values
+        dst = torch.arange(keep, device=w.device)
+        pg = table[b].long()
+        for name, src in c.items():
+            if src is not None:
+                out[name][pg[dst // page], h, dst % page] = src[pg[at // page], h, at % page]
+        w2[b, :, :keep] = w[b].gather(1, at)
+    return out, w2

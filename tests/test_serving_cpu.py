@@ -10,7 +10,7 @@ import torch
 import flash_attention_sm75 as fa
 from tests import abi_ctypes as abi
 from tests.paged_plain import Paged, attention
-from tests.serving_plain import evicted, prefix_attention, summed_weights, with_prefixes
+from tests.serving_plain import evicted, evicted_whole, prefix_attention, summed_weights, with_prefixes
 from tests.test_paged_cpu import P16, _cache
 
 EIGHT = dict(dtype=2, k_scale=P16, v_scale=P16, scale_page_stride=32, scale_head_stride=16, scale_row_stride=1)
@@ -204,3 +204,20 @@ def test_weights_of_more_key_blocks_than_a_grid_has():
     assert _weights(_cache(kv_heads=1, max_pages=1 << 26), Hq=4, total=3000, max_q=1000, **one) == 10
     if not torch.cuda.is_available():  # streams of few rows have no such limit (the device is checked afterwards)
         assert _weights(_cache(**big), Hq=64, total=1 << 20, max_q=1, **many) not in (0, 10)
+
+
+@pytest.mark.parametrize("keep,recent,first", [(64, 10, 2), (1, 0, 0), (0, 3, 3), (150, 400, 20), (299, 0, 1)])
+def test_plain_evictions_agree(keep, recent, first):
+    """The vectorised form against the one that goes row by row, with every kind of weight."""
+    P = Paged([(0, 300), (0, 77), (0, 0)], 2, 64, 16, torch.int8, seed=5)
+    g = torch.Generator().manual_seed(keep)
+    w = torch.randn(3, 2, P.width * P.page, generator=g)
+    r = torch.rand(w.shape, generator=g)
+    for i, x in enumerate((0.0, -0.0, 1.5, math.nan, math.inf, -math.inf)):
+        w[(r > i / 10) & (r < (i + 1) / 10)] = x
+    k, v, ks, vs, w2, _ = evicted(P, w, keep, recent, first)
+    got, w3 = evicted_whole(dict(k=P.k, v=P.v, ks=P.ks, vs=P.vs), P.table, w, P.nk, keep, recent, first, P.page)
+    assert torch.equal(w2.view(torch.int32), w3.view(torch.int32))
+    for a, b in ((got["k"].view(torch.uint8), k), (got["v"].view(torch.uint8), v),
+                 (got["ks"].view(torch.int32), ks.view(torch.int32)), (got["vs"].view(torch.int32), vs.view(torch.int32))):
+        assert torch.equal(a, b)
