@@ -81,7 +81,8 @@ struct PagedAttn {
 // lse, joined with the first pass's rows in part_o and part_lse (chunk kernel alone, or
 // decode with one CTA per (sequence, head)).  kPartRuns: decode whose runs are combined: rows
 // that one team has go to part_o and part_lse, and the combine joins all with first_o.
-// (The kernels of a translation unit without FA_PART_ROWS know kPartNone alone.)
+// (The kernels of a translation unit without FA_PART_ROWS know kPartNone alone, those with it the
+// others.)
 #ifndef FA_PART_ROWS
 #define FA_PART_ROWS 0
 #endif

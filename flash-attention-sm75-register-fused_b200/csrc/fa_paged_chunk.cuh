@@ -863,7 +863,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_chunk_kernel(const __grid_c
                                 : nullptr;
       // of two passes: where this one's row goes, or the first one's is
       float4* const first_o =
-          kPartRows && !partial && a.part != kPartNone ? reinterpret_cast<float4*>(a.part_at(row_id, 0)) : nullptr;
+          kPartRows && !partial ? reinterpret_cast<float4*>(a.part_at(row_id, 0)) : nullptr;
       const long long step_o = a.part_block / 4;
       if (n_tiles == 0) {
         if (first_o != nullptr) {
@@ -1085,27 +1085,24 @@ __global__ void __launch_bounds__(kJoinThreads) paged_part_join_kernel(const __g
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
   const int hq = c.h * a.group + r % a.group;
   const long long out = static_cast<long long>(c.c0 + tok) * a.Hq + hq;
-  float lse = sum == 0.f ? -INFINITY : mx + logf(sum);
+  const float lse = sum == 0.f ? -INFINITY : mx + logf(sum);
 #pragma unroll
   for (int e = 0; e < 4; ++e) acc[e] *= inv;
-  if (a.part != kPartNone) {
-    float4* const first_o = reinterpret_cast<float4*>(a.part_at(out, col));
-    if (a.part != kPartJoin) {
-      *first_o = make_float4(acc[0], acc[1], acc[2], acc[3]);
-      if (col == 0) a.part_lse[out] = lse;
-      return;
-    }
-    const Joined jn = join_passes(__ldcg(a.part_lse + out), lse);
-    const float4 f = __ldcg(first_o);
-    const float y4[4] = {f.x, f.y, f.z, f.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      acc[e] = (jn.own == 0.f ? 0.f : acc[e] * jn.own) + (jn.first == 0.f ? 0.f : y4[e] * jn.first);
-    lse = jn.lse;
+  float4* const first_o = reinterpret_cast<float4*>(a.part_at(out, col));
+  if (a.part != kPartJoin) {
+    *first_o = make_float4(acc[0], acc[1], acc[2], acc[3]);
+    if (col == 0) a.part_lse[out] = lse;
+    return;
   }
+  const Joined jn = join_passes(__ldcg(a.part_lse + out), lse);
+  const float4 f = __ldcg(first_o);
+  const float y4[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    acc[e] = (jn.own == 0.f ? 0.f : acc[e] * jn.own) + (jn.first == 0.f ? 0.f : y4[e] * jn.first);
   *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.o) + out * D + col) =
       make_uint2(pack2<BF16>(acc[0], acc[1]), pack2<BF16>(acc[2], acc[3]));
-  if (col == 0 && a.lse != nullptr) a.lse[static_cast<long long>(hq) * a.r.total + c.c0 + tok] = lse;
+  if (col == 0 && a.lse != nullptr) a.lse[static_cast<long long>(hq) * a.r.total + c.c0 + tok] = jn.lse;
 }
 
 // The visible keys and values of the chunk kernel's sequences as 16-bit rows:

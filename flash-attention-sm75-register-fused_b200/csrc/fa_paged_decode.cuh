@@ -117,22 +117,6 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   return y;
 }
 
-template <bool BF16>
-__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                         uint32_t a3, uint32_t b0, uint32_t b1) {
-  if constexpr (BF16) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  } else {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  }
-}
-
 // load_seq for this kernel, which takes sequences of at most max_rows query
 // rows per KV head (nq = vis = 0 for the others).
 __device__ __forceinline__ Seq load_short(const PagedAttn& a, int b, int max_rows) {
@@ -201,7 +185,7 @@ struct Partial {
   __device__ __forceinline__ void write(const PagedAttn& a, int tok, int hq, float up) const {
     const int lane = threadIdx.x & 31;
     const float inv = l == 0.f ? 0.f : up / l;
-    if (kPartRows && a.part != kPartNone) {
+    if (kPartRows) {
       const long long row = static_cast<long long>(tok) * a.Hq + hq;
       const float lse = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.69314718055994530942f;
       if (a.part == kPartFirst || a.part == kPartSecond) {
@@ -482,28 +466,7 @@ __device__ __forceinline__ void paged_decode_body(const DecodeParams& p) {
       }
       float unit = 1.f;
       if constexpr (C::k8 && QBF16) {
-        // q / 2^e with 2^e <= max |q| < 2^(e+1), as f16
-        float mx = 0.f;
-#pragma unroll
-        for (int k = 0; k < C::kKS; ++k)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&q[nt][k][i]));
-            mx = fmaxf(mx, fmaxf(fabsf(f.x), fabsf(f.y)));
-          }
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const uint32_t e = __float_as_uint(mx) & 0x7f800000u;
-        const bool plain = e == 0u || e >= 0x7e800000u;
-        unit = plain ? 1.f : __uint_as_float(e);
-        const float inv = plain ? 1.f : __uint_as_float(0x7f000000u - e);
-#pragma unroll
-        for (int k = 0; k < C::kKS; ++k)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&q[nt][k][i]));
-            q[nt][k][i] = pack2<false>(f.x * inv, f.y * inv);
-          }
+        unit = bf16_row_as_f16<2 * C::kKS>([&](int i) -> uint32_t& { return q[nt][i / 2][i % 2]; });
       }
 #pragma unroll
       for (int k = 0; k < C::kKS; ++k) {
@@ -779,7 +742,7 @@ __device__ __forceinline__ void paged_decode_body(const DecodeParams& p) {
         if (first && last && !p.solo) {
           const int tok = s.c0 + r / a.group, hq = cc.h * a.group + r % a.group;
           const float inv = l[nt][c] == 0.f ? 0.f : kUp / l[nt][c];
-          if (kPartRows && a.part != kPartNone) {
+          if (kPartRows) {
             const float lse_row =
                 l[nt][c] == 0.f ? -INFINITY : (m[nt][c] + (C::k8 ? 0.f : __log2f(l[nt][c]))) * 0.69314718055994530942f;
             const long long row = static_cast<long long>(tok) * a.Hq + hq;

@@ -1,6 +1,8 @@
 // Device helpers of the paged attention kernels: a sequence's part in a call,
-// the block-wide scan over sequences, and 8-bit values widened to f16.
+// the block-wide scan over sequences, 8-bit values widened to f16, the
+// register-operand product and the join of two passes.
 #pragma once
+#include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
@@ -34,6 +36,49 @@ __device__ __forceinline__ void widen(uint32_t w, uint32_t& p0, uint32_t& p1) {
         : "=r"(p0), "=r"(p1)
         : "r"(u));
   }
+}
+
+// m16n8k16 product of 16-bit registers, fp32 sums.
+template <bool BF16>
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (BF16) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  } else {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+}
+
+// bf16 queries over 8-bit pages are taken as f16, q / 2^e with 2^e the size of the
+// row's largest element (2^e <= max |q| < 2^(e+1)): bf16's 8 bits fit f16's 11, and elements
+// below 2^-14 of the largest lose at most 2^-25 of it, no more than the sum in fp32 does.
+// A quad's lanes have a row, N pairs each (at(i): pair i); returns 2^e.
+template <int N, typename At>
+__device__ __forceinline__ float bf16_row_as_f16(At at) {
+  float mx = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&at(i)));
+    mx = fmaxf(mx, fmaxf(fabsf(f.x), fabsf(f.y)));
+  }
+  mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+  mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+  const uint32_t e = __float_as_uint(mx) & 0x7f800000u;
+  const bool plain = e == 0u || e >= 0x7e800000u;
+  const float inv = plain ? 1.f : __uint_as_float(0x7f000000u - e);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&at(i)));
+    const __half2 x = __floats2half2_rn(f.x * inv, f.y * inv);
+    at(i) = *reinterpret_cast<const uint32_t*>(&x);
+  }
+  return plain ? 1.f : __uint_as_float(e);
 }
 
 // What a sequence brings to a call.

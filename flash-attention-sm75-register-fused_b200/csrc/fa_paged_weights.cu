@@ -39,22 +39,6 @@ namespace {
 
 constexpr int kWeightThreads = 128;
 
-template <bool BF16>
-__device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                          uint32_t b0, uint32_t b1) {
-  if constexpr (BF16) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  } else {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-        "{%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-  }
-}
-
 // Row r of (sequence, KV head): its packed token and query head.
 struct QueryRow {
   int tok, hq;
@@ -63,9 +47,6 @@ __device__ __forceinline__ QueryRow query_row(const PagedAttn& a, const Seq& s, 
   return {s.c0 + r / a.group, h * a.group + r % a.group};
 }
 
-// bf16 queries over 8-bit pages are taken as f16, q / 2^e with 2^e the size of
-// the row's largest element: bf16's 8 bits fit f16's 11, and elements below 2^-14 of
-// the largest lose at most 2^-25 of it, no more than the sum in fp32 does.
 // Positions of the work order that a (sequence, head) takes besides its steps: its
 // queries, and the wait for its first keys.
 constexpr int kSegmentCost = 2;
@@ -186,7 +167,7 @@ __global__ void __launch_bounds__(kWeightThreads, few_ctas_per_sm(NT))
         next_page = page_at(wbase + 32);
       };
       next_window();
-            const uint8_t* const k_lane = a.c.k + h * a.c.head_stride + g * a.c.row_stride + 16 * j;
+      const uint8_t* const k_lane = a.c.k + h * a.c.head_stride + g * a.c.row_stride + 16 * j;
       const long long row8 = 8 * a.c.row_stride;
       const float* const ks_lane = S::k8 ? a.c.ks + h * a.c.s_head + g * a.c.s_row : nullptr;
 
@@ -232,12 +213,12 @@ __global__ void __launch_bounds__(kWeightThreads, few_ctas_per_sm(NT))
       uint32_t q[NT][S::kPairs];
       float cs[NT][2], nlse[NT][2];
       int lim[NT][2];
-    #pragma unroll
+#pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const int r = nt * 8 + g;
         const QueryRow qr = query_row(a, s, h, r);
         const uint8_t* const src = a.q + static_cast<long long>(qr.tok) * a.q_token + qr.hq * a.q_head;
-    #pragma unroll
+#pragma unroll
         for (int i = 0; i < S::kPairs / 4; ++i) {
           // 16-bit keys: the piece of 8 columns at 32 i + 8 j; 8-bit keys: the half i % 2 of the
           // 16 columns at 64 (i / 2) + 16 j
@@ -250,26 +231,9 @@ __global__ void __launch_bounds__(kWeightThreads, few_ctas_per_sm(NT))
         }
         float unit = 1.f;
         if constexpr (S::k8 && QBF16) {
-          float mx = 0.f;
-    #pragma unroll
-          for (int i = 0; i < S::kPairs; ++i) {
-            const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&q[nt][i]));
-            mx = fmaxf(mx, fmaxf(fabsf(f.x), fabsf(f.y)));
-          }
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          const uint32_t e = __float_as_uint(mx) & 0x7f800000u;
-          const bool plain = e == 0u || e >= 0x7e800000u;
-          unit = plain ? 1.f : __uint_as_float(e);
-          const float inv = plain ? 1.f : __uint_as_float(0x7f000000u - e);
-    #pragma unroll
-          for (int i = 0; i < S::kPairs; ++i) {
-            const float2 f = __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&q[nt][i]));
-            const __half2 x = __floats2half2_rn(f.x * inv, f.y * inv);
-            q[nt][i] = *reinterpret_cast<const uint32_t*>(&x);
-          }
+          unit = bf16_row_as_f16<S::kPairs>([&](int i) -> uint32_t& { return q[nt][i]; });
         }
-    #pragma unroll
+#pragma unroll
         for (int c = 0; c < 2; ++c) {
           const int rc = nt * 8 + 2 * j + c;
           const QueryRow qc = query_row(a, s, h, rc);
@@ -282,7 +246,7 @@ __global__ void __launch_bounds__(kWeightThreads, few_ctas_per_sm(NT))
         }
       }
       int all = 0x7fffffff;  // every row sees the keys below
-    #pragma unroll
+#pragma unroll
       for (int nt = 0; nt < NT; ++nt) all = min(all, min(lim[nt][0], lim[nt][1]));
       all = __reduce_min_sync(0xffffffffu, all);
       auto compute = [&](const KeyStep<D, KV>& st, int t) {
@@ -302,7 +266,7 @@ __global__ void __launch_bounds__(kWeightThreads, few_ctas_per_sm(NT))
               for (int e = 0; e < 2; ++e)
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
-                  mma_16816<kBf16>(c[nt], k0[2 * e], k1[2 * e], k0[2 * e + 1], k1[2 * e + 1], q[nt][4 * i + 2 * e],
+                  mma16816<kBf16>(c[nt], k0[2 * e], k1[2 * e], k0[2 * e + 1], k1[2 * e + 1], q[nt][4 * i + 2 * e],
                                    q[nt][4 * i + 2 * e + 1]);
             } else {
 #pragma unroll
@@ -312,7 +276,7 @@ __global__ void __launch_bounds__(kWeightThreads, few_ctas_per_sm(NT))
                 widen<KV, false>(k1[e], a1, a3);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
-                  mma_16816<false>(c[nt], a0, a1, a2, a3, q[nt][8 * i + 2 * e], q[nt][8 * i + 2 * e + 1]);
+                  mma16816<false>(c[nt], a0, a1, a2, a3, q[nt][8 * i + 2 * e], q[nt][8 * i + 2 * e + 1]);
               }
             }
           }

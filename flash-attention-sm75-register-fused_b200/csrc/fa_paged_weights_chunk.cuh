@@ -40,6 +40,7 @@ constexpr int kExps = 512;   // threads of the exponentials: two per key, for ha
 constexpr int kWarpTma = 16, kWarpMma = 17, kWarpRows = 18;
 constexpr int kRowRing = 4;
 constexpr int kMaxSplit = 8;
+constexpr int kFmaPairs = 4;  // of 16 pairs of exponentials, on the FMA pipe
 
 // (y0, y1) = 2^t for two lanes on the FMA pipe, t in [-126, 127] (clamped): 2^t = 2^n
 // 2^f with n the nearest integer, and 2^f a polynomial of degree 5, fitted here by a Remez
@@ -91,7 +92,7 @@ struct Smem {
   static_assert(kBytes <= 227 * 1024, "shared memory budget");
 };
 
-template <int D, int KV, bool QBF16, int kFmaPairs>
+template <int D, int KV, bool QBF16>
 __global__ void __launch_bounds__(kThreads, 1) paged_weights_chunk_kernel(const __grid_constant__ WeightsChunkParams p) {
   using L = Smem<D>;
   constexpr bool k8 = KV >= FA_DTYPE_INT8;
@@ -430,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_weights_chunk_kernel(const 
 
 template <int D, int KV, bool QBF16>
 cudaError_t launch_impl(const WeightsChunkParams& p, cudaStream_t stream) {
-  auto kern = paged_weights_chunk_kernel<D, KV, QBF16, 4>;
+  auto kern = paged_weights_chunk_kernel<D, KV, QBF16>;
   static int attr_done[64] = {0};
   int dev = 0;
   cudaGetDevice(&dev);
