@@ -575,6 +575,7 @@ int fa_fwd_paged_prefix(const fa_paged_cache* cache, const int* prefix_table,
   const PagedPlan k1 = plan_of(first, of_prefixes), k2 = plan_of(a, *cache);
   const size_t part = part_bytes(total_q, Hq, cache->head_dim);
   const size_t parts = part_buffers(k2) * part;
+  // (the second pass may start while the first still uses its workspace: each has its own)
   const size_t need = parts + k1.ws_bytes + k2.ws_bytes;
   if (!workspace || workspace_bytes < need) return FA_ERR_INVALID_ARG;
   if (int rc = check_grid(k1, first)) return rc;

@@ -16,12 +16,19 @@
 //           is overwritten that a later group reads.  So the next group's loads are on
 //           their way while this one is stored.
 // Bound by memory: the weights are read once (the first kCacheSteps x 2048 of a CTA stay in
-// shared memory), rows that move are read and written once.  Measured, 8 KV heads, d = 128:
-// 32 ragged caches of up to 8192 bf16 positions cut to 2048, 187 MB moved, 74 us (29 at the
-// rate of a plain copy: three passes of selection and the places take 16, and the clusters run
-// in two rounds); 2 x 65536 int8 positions to 16384, 173 MB, 122 us (16 clusters of 8 on 128
-// SMs, 4 TB/s while rows move); 1 x 1024 to 512 16 us, all latency.  A CTA alone per head, with
-// 1024 positions' rows moved as they are found, took 80, 328 and 19 us.
+// shared memory), rows that move are read and written once.  Measured on caches not cut
+// before, 8 KV heads, d = 128:
+// 32 ragged caches of up to 8192 bf16 positions cut to 2048, 187 MB read and written, 74 us (29 at
+// the rate of a plain copy).  11 of them are longer, so 88 of the 256 clusters of two have work,
+// on 176 CTAs where 296 fit; three passes of selection and the places take 16 us, then rows move
+// in groups with a cluster barrier each.
+// 2 x 65536 int8 positions to 16384, 144 MB, 125 us (22): of the 16 clusters of 8 that it launches 15
+// are resident at a time (cudaOccupancyMaxActiveClusters), and the last one runs alone after
+// them.
+// 1 x 1024 to 512 17 us, all latency.
+// Rows that keep their place are not moved.  Of a cache that is cut to the same number again and
+// again that becomes most of them: the 32 ragged ones end at 43 us.  A CTA alone per head, with
+// 1024 positions' rows moved as they are found, took 80, 328 and 19 us for a first cut.
 #include <cuda_runtime.h>
 
 #include <cstdint>

@@ -5,11 +5,13 @@
 //
 // A prefix is computed once for all rows behind it: the first pass sees its tokens as one
 // sequence, of many rows, over the prefix's keys (few rows: the decode kernel, else the
-// tensor cores), the second every sequence over its own keys.  Measured, 8 KV heads, d = 128, GQA
-// 4, and in brackets the same batch as sequences that each have the prefix in their table:
-// 64 single tokens behind 8192 bf16 keys, up to 1024 of their own, 63 us (143); 48 behind
-// 16384 e4m3 keys 81 (186); 8 behind 1024 21 (16: two passes and a join have their fixed
-// costs); 8 x 512 tokens behind 8192 540 (498: chunks fill the tensor cores' tiles by
+// tensor cores), the second every sequence over its own keys.  Measured, calls among others, 8 KV
+// heads, d = 128, GQA 4, and in brackets the same batch as sequences that each have the prefix
+// in their table: 64 single tokens behind 8192 bf16 keys, up to 1024 of their own, 61 us (135);
+// 48 behind 16384 e4m3 keys 79 (181); 512 tokens and 31 single ones behind 8192 130 (192); 8
+// behind 1024 19 (15: two passes and a join have their fixed costs); 32 x 4 drafts of d = 64
+// behind three prefixes 41 (31: the first pass reads every unit in four warps); 8 x 512 tokens
+// behind 8192 522 to 593 from run to run (498 to 551: chunks fill the tensor cores' tiles by
 // themselves, and the first pass's 67 MB of fp32 rows are written and read).
 #define FA_PART_ROWS 1
 #include "fa_device.cuh"

@@ -22,8 +22,10 @@
 //
 // Measured, 8 KV heads, d = 128, GQA 4: 16 sequences x 8192 keys of bf16 pages, one token,
 // 48.1 us (5.8 TB/s; a plain copy runs at 6.5; one CTA per 64 keys and 32 rows, with the queries
-// in shared memory, 82).  32 ragged sequences over int8 pages, 3 tokens, 26.7 us (3.6 TB/s: 290
-// instructions per 16 keys, a third of them widening, at 0.4 of the issue rate).
+// in shared memory, 82).  32 ragged sequences over int8 pages, 3 tokens, 26.7 us (3.6 TB/s): 290
+// instructions per 16 keys, a third of them widening, and neither the issue slots (0.4 busy) nor DRAM
+// (42 %) are the limit, but the latency of three warps per scheduler, whose 168 registers hold two
+// steps of keys as they are read.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

@@ -23,10 +23,14 @@
 // Bound by the exponentials: 128 x 256 of them take the special-function unit 2048 cycles,
 // the two products about 1100.  kFmaPairs of 16 pairs go to the FMA pipe instead (0 / 2 / 4
 // / 6 of 16: 239 / 226 / 216 / 235 us for 2 x 1024 tokens over 8192 keys, bf16, d = 128, GQA
-// 4).  Now 207 us there: the unit is busy for 54 %, the issue slots for 55 %; what is left
-// is the latency between a tile's arrival and its last sum.  CTAs that walk several key
+// 4).  Now 201 to 207 us there (8-bit pages 201): the unit is busy for 54 %, the issue slots for 55 %;
+// what is left is the latency between a tile's arrival and its last sum, and that 512 equal CTAs
+// take four rounds on 148 SMs for 3.46 rounds of work.  CTAs that walk several key
 // blocks, with the next one's keys loaded by a warp of their own, took as long (the
 // registers that this takes spill), and so did two CTAs of one key tile per SM.
+// The grid has a CTA for every 256 keys that the bounds allow every sequence, whose shared memory
+// leaves room for one on an SM; those without work leave at once, but are placed: 1024
+// tokens beside 31 single ones, all over 8192 keys, take 242 us, 103 and 83 by themselves.
 #include "fa_paged.h"
 #include "fa_paged_dev.cuh"
 

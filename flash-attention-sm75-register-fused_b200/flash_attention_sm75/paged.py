@@ -134,11 +134,14 @@ def flash_attention_forward_paged_prefix(q, k_cache, v_cache, prefix_table, cu_p
         max_prefix_q, max_prefix_k: upper bounds of a prefix's tokens and keys
             (tokens beyond do not see it, keys beyond are not seen)
 
-    It pays where many sequences of few tokens share a long prefix (64 tokens
-    behind 8192 keys: 63 us instead of 143 with the prefix's pages at the head
-    of every table); a few sequences behind a short one (8 behind 1024: 21 / 16),
-    and chunks that fill tiles by themselves (8 x 512 behind 8192: 540 / 498),
-    are a little faster with tables that begin with the prefix's (whole) pages.
+    It pays where many sequences of few tokens share a long prefix, also beside a
+    chunk (64 tokens behind 8192 keys: 61 us instead of 135 with the prefix's
+    pages at the head of every table; 512 tokens and 31 single ones behind 8192:
+    130 / 192).  Tables that begin with the prefix's (whole) pages are faster for a
+    few sequences behind a short one (8 behind 1024: 19 / 15), for drafts of d = 64
+    behind several (32 x 4 behind three of up to 4096: 41 / 31) and for chunks that
+    fill tiles by themselves (8 x 512 behind 8192: 522 to 593 / 498 to 551, from run to
+    run; 4 x 512 over e4m3 pages 346 / 325).
 
     A token sees all keys of its prefix, and those of its own sequence that
     ``causal`` leaves.  Rows that see no key, rows of no sequence and tokens
@@ -181,6 +184,10 @@ def kvcache_weights_paged(q, lse, k_cache, block_table, cu_seqlens_q, seqlens_k,
             sequence's positions)
 
     Positions from a sequence's length (or max_seqlen_k) on are left as they are.
+    Chunks (more than 32 query rows per KV head) take a block for every 256 keys that
+    max_seqlen_k allows every sequence of the batch, so a bound near the lengths is
+    faster, and a chunk beside many long sequences pays for theirs (1024 tokens and 31
+    single ones, all over 8192 keys: 242 us; 103 and 83 by themselves).
     """
     if mode not in _WEIGHT_MODES:
         raise ValueError(f"mode must be one of {sorted(_WEIGHT_MODES)}, got {mode!r}")

@@ -359,9 +359,9 @@ int fa_fwd_paged_prefix(const fa_paged_cache* cache, const int* prefix_table,
                         int max_seqlen_k, float scale, int causal, int dtype, void* workspace,
                         size_t workspace_bytes, void* stream);
 
-/* Workspace bytes of fa_fwd_paged_prefix (a function of its sizes alone): the fp32
- * results of the prefixes, and the larger of the two passes' needs; 0 for what the
- * call refuses. */
+/* Workspace bytes of fa_fwd_paged_prefix (a function of its sizes alone): fp32 results
+ * of one pass or of both, and the sum of the two passes' workspaces (the second may start
+ * while the first still uses its own); 0 for what the call refuses. */
 size_t fa_fwd_paged_prefix_workspace_bytes(const fa_paged_cache* cache, int n_prefixes,
                                            int max_prefix_q, int max_prefix_k, int B, int Hq,
                                            int total_q, int max_seqlen_q, int max_seqlen_k);

@@ -221,3 +221,18 @@ def test_plain_evictions_agree(keep, recent, first):
     for a, b in ((got["k"].view(torch.uint8), k), (got["v"].view(torch.uint8), v),
                  (got["ks"].view(torch.int32), ks.view(torch.int32)), (got["vs"].view(torch.int32), vs.view(torch.int32))):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("cache", [dict(), EIGHT], ids=["f16", "int8"])
+@pytest.mark.parametrize("B,total,max_q", [(64, 64, 1), (4, 2048, 512), (9, 300, 200), (1, 1, 1)])
+def test_prefix_workspace_holds_both_passes_at_once(cache, B, total, max_q):
+    """The second pass may start while the first still runs: fp32 rows of one pass or of both (d + 1
+    numbers for every token and query head, in whole 128 bytes) and both passes' own workspaces."""
+    lib, c = abi.load(), _cache(**cache)
+    c.max_pages = 1 << 10
+    first = lib.fa_fwd_paged_workspace_bytes(ctypes.byref(c), 1, 8, total, total, 8192)
+    own = lib.fa_fwd_paged_workspace_bytes(ctypes.byref(c), B, 8, total, max_q, 900)
+    rows = -(-total * 8 * 65 * 4 // 128) * 128
+    both = lib.fa_fwd_paged_prefix_workspace_bytes(ctypes.byref(c), 1, total, 8192, B, 8, total, max_q, 900)
+    assert both - first - own in (rows, 2 * rows)
+    assert first > 0
